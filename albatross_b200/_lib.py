@@ -42,6 +42,26 @@ class ModelDesc(C.Structure):
                 ("head", Mat), ("layers", C.POINTER(Layer))]
 
 
+DT_F16, DT_BF16, DT_F32 = 0, 1, 2
+WKV_CHUNK = 16      # steps between two states that ab_wkv7_seq_fwd keeps (ab_wkv7_checkpoint_bytes)
+
+
+class Wkv7Seq(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("B", C.c_int32), ("T", C.c_int32), ("H", C.c_int32), ("x", C.c_void_p * 6),
+                ("batch_stride", C.c_int64 * 6), ("step_stride", C.c_int64 * 6), ("state", C.c_void_p), ("lengths", C.c_void_p),
+                ("checkpoints", C.c_void_p)]
+
+
+class LogitRows(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("vocab", C.c_int32), ("rows", C.c_int64), ("stride", C.c_int64),
+                ("logits", C.c_void_p), ("ids", C.c_void_p), ("mask", C.c_void_p)]
+
+
+class Policy(C.Structure):
+    _fields_ = [("old_logp", C.c_void_p), ("advantages", C.c_void_p), ("ref_logp", C.c_void_p),
+                ("clip_low", C.c_float), ("clip_high", C.c_float), ("kl", C.c_float), ("denom", C.c_float)]
+
+
 class LibraryError(RuntimeError):
     pass
 
@@ -85,6 +105,21 @@ def _load():
     lib.ab_decode_run.argtypes = [vp, vp, vp]
     lib.ab_decode_plan_selftest.argtypes = [vp, i32]
     lib.ab_glue_selftest.argtypes = [i32, C.c_uint64, C.c_uint64, vp, vp]
+    i64, f32 = C.c_int64, C.c_float
+    seq, rows, policy = C.POINTER(Wkv7Seq), C.POINTER(LogitRows), C.POINTER(Policy)
+    lib.ab_wkv7_checkpoint_bytes.argtypes = [seq]
+    lib.ab_wkv7_checkpoint_bytes.restype = sz
+    lib.ab_wkv7_seq_fwd.argtypes = [seq, vp, vp, vp]
+    lib.ab_wkv7_seq_bwd.argtypes = [seq, vp, i64, i64, vp, C.POINTER(vp), vp, vp]
+    lib.ab_layer_norm_fwd.argtypes = [i32, i32, i64, i32, i32, vp, i64, vp, vp, f32, vp, vp, vp, vp]
+    lib.ab_layer_norm_scratch_bytes.argtypes = [i64, i32]
+    lib.ab_layer_norm_scratch_bytes.restype = sz
+    lib.ab_layer_norm_bwd.argtypes = [i32, i32, i64, i32, i32, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp]
+    lib.ab_token_logp_fwd.argtypes = [rows, vp, vp, vp, vp]
+    lib.ab_token_logp_bwd.argtypes = [rows, vp, vp, i64, vp, vp, vp]
+    lib.ab_policy_loss_fwd.argtypes = [rows, policy, vp, vp, vp, vp, vp, vp]
+    lib.ab_policy_loss_grad.argtypes = [rows, policy, f32, vp, vp, vp, vp, vp]
+    lib.ab_preference_loss_fwd.argtypes = [rows, i64, i64, vp, f32, f32, vp, vp, vp, vp, vp, vp]
     return lib
 
 
@@ -92,7 +127,9 @@ lib = _load()
 
 EXPORTS = ["ab_last_error", "ab_version", "ab_device_status", "ab_wkv7_fwd", "ab_gemv", "ab_gemm_scratch_bytes",
            "ab_gemm", "ab_gemm_static", "ab_gemm_static_reset", "ab_gemm_static_debug_counter", "ab_sample_rows", "ab_sample_rows_i64", "ab_gemv_plan_selftest", "ab_gemm_plan_selftest", "ab_dequant", "ab_model_create", "ab_model_destroy", "ab_workspace_bytes", "ab_forward", "ab_forward_stage",
-           "ab_model_set_option", "ab_decode_program_bytes", "ab_decode_timeline_offset", "ab_decode_program_build", "ab_decode_run", "ab_decode_plan_selftest", "ab_glue_selftest"]
+           "ab_model_set_option", "ab_decode_program_bytes", "ab_decode_timeline_offset", "ab_decode_program_build", "ab_decode_run", "ab_decode_plan_selftest", "ab_glue_selftest",
+           "ab_wkv7_checkpoint_bytes", "ab_wkv7_seq_fwd", "ab_wkv7_seq_bwd", "ab_layer_norm_fwd", "ab_layer_norm_scratch_bytes", "ab_layer_norm_bwd",
+           "ab_token_logp_fwd", "ab_token_logp_bwd", "ab_policy_loss_fwd", "ab_policy_loss_grad", "ab_preference_loss_fwd"]
 
 
 def check(status: int, what: str = "") -> None:

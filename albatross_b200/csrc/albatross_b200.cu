@@ -5,5 +5,9 @@
 #include "gemm.cu"
 #include "gemv.cu"
 #include "head.cu"
+#include "loss.cu"
+#include "norm.cu"
 #include "rows.cu"
 #include "stream.cu"
+#include "train_api.cu"
+#include "wkv_train.cu"

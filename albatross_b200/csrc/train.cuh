@@ -1,0 +1,51 @@
+// Operators with gradients (see wkv_train.cu, norm.cu, loss.cu): what the C entries hand to the launchers.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "../../include/albatross_b200.h"
+#include "common.cuh"
+
+namespace ab {
+
+// values of the three element types as 32-bit floats, and back with one rounding
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class E> __device__ __forceinline__ E from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+constexpr int WKV_CHUNK = 16;   // steps between two states that the forward pass keeps for the backward pass
+
+struct WkvBackward {
+    const void* dy;                        // null: zeros
+    int64_t dy_batch_stride, dy_step_stride;
+    const float* dstate_out;               // null: zeros
+    void* dx[6];                           // dense [B, T, 64 H]; null: not wanted
+    float* dstate;                         // null: not wanted
+};
+int wkv_train_fwd(const ab_wkv7_seq& s, void* y, float* state_out, cudaStream_t st);
+int wkv_train_bwd(const ab_wkv7_seq& s, const WkvBackward& g, cudaStream_t st);
+
+struct NormArgs {
+    int dtype, wtype, C, groups;
+    int64_t rows, x_stride, dy_stride;     // elements between rows
+    float eps;
+    const void *x, *w, *b, *dy;
+    void *y, *dx, *dw, *db;
+    float *mean, *rstd, *scratch;
+};
+size_t layer_norm_scratch_bytes(int64_t rows, int C);
+int layer_norm_fwd(const NormArgs& a, cudaStream_t st);
+int layer_norm_bwd(const NormArgs& a, cudaStream_t st);
+
+int token_logp_fwd(const ab_logit_rows& t, double* logp, float* logp32, float* stats, cudaStream_t st);
+int token_logp_bwd(const ab_logit_rows& t, const float* stats, const float* g, int64_t rows_per_g, const float* scale, void* dlogits, cudaStream_t st);
+// loss and derivatives by the rows' log-probabilities (g), or (dlogits) scale times the gradient by the logits, in one pass
+int policy_loss(const ab_logit_rows& t, const ab_policy& p, float scale, float* loss, float* logp32, float* stats, float* g, void* dlogits,
+                double* rows_scratch, cudaStream_t st);
+int preference_loss(const ab_logit_rows& t, int64_t pairs, int64_t steps, const float* ref, float beta, float smoothing, float* loss, float* logp32,
+                    float* stats, float* g, double* rows_scratch, cudaStream_t st);
+
+}  // namespace ab

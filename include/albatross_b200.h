@@ -160,6 +160,81 @@ int ab_dequant(const ab_mat* m, float* out, void* stream);
  * *differ (device memory) how many results have other bits; two NaNs count as equal. */
 int ab_glue_selftest(int which, uint64_t first, uint64_t n, uint64_t* differ, void* stream);
 
+/* ---- operators with gradients (no counterpart in the reference, which only generates) -------------------------
+ * What turns sampled tokens into gradients: the WKV-7 recurrence over whole sequences, the norms of a block, and losses on
+ * logits. Each takes fp16 or bf16 (norms and logits fp32 too); sums, statistics and states are fp32 or wider. Results do not
+ * depend on the order in which blocks run. Nothing is kept from one call for the next. */
+#define AB_DT_F16 0
+#define AB_DT_BF16 1
+#define AB_DT_F32 2
+
+/* S_t = S_{t-1} diag(d_t) + (S_{t-1} a_t) b_t^T + v_t k_t^T, y_t = S_t r_t, d_t = exp(-exp(w_t)), for every head of 64: the
+ * operator of ab_wkv7_fwd, out of place, in two types, with strides and sequences of unequal length. */
+typedef struct ab_wkv7_seq {
+    int32_t dtype, B, T, H;      /* AB_DT_F16 or AB_DT_BF16; T may be 0 */
+    const void* x[6];            /* r, w, k, v, a, b: [B, T, 64 H] of dtype, the last dimension dense */
+    int64_t batch_stride[6], step_stride[6];   /* elements between sequences, and between steps */
+    const float* state;          /* [B, H, 64, 64] dense, before the first step; NULL: zeros */
+    const int32_t* lengths;      /* [B] or NULL: sequence b has lengths[b] steps (taken into 0 .. T); what x holds behind them is not used */
+    float* checkpoints;          /* ab_wkv7_checkpoint_bytes(s): states kept for the backward pass; NULL in ab_wkv7_seq_fwd: none are kept */
+} ab_wkv7_seq;
+/* bytes of `checkpoints` (16 KB per head and 16 steps); only B, T and H are looked at */
+size_t ab_wkv7_checkpoint_bytes(const ab_wkv7_seq* s);
+/* y: dense [B, T, 64 H] of dtype, zero behind a sequence's end. state_out: dense [B, H, 64, 64], after the last step; it may be s->state. */
+int ab_wkv7_seq_fwd(const ab_wkv7_seq* s, void* y, float* state_out, void* stream);
+/* Gradients, given those of y (strided as x; NULL: zeros) and of state_out (NULL: zeros). dx: HOST array of six device pointers to dense
+ * [B, T, 64 H] of dtype, for r, w, k, v, a, b (w before the transform), zero behind a sequence's end; dstate dense [B, H, 64, 64]. NULL
+ * for what is not wanted. `s` as it was in ab_wkv7_seq_fwd, with the checkpoints that it wrote. */
+int ab_wkv7_seq_bwd(const ab_wkv7_seq* s, const void* dy, int64_t dy_batch_stride, int64_t dy_step_stride, const float* dstate_out,
+                    void* const* dx, float* dstate, void* stream);
+
+/* y = (x - mean) / sqrt(var + eps) * w + b over each of `groups` equal parts of a row of C values (1: layer norm; one part per
+ * head: the norm behind the recurrence). x: rows of dtype, x_stride elements apart; y dense. w, b: [C] of wtype (dtype or AB_DT_F32), or
+ * NULL: 1, 0. mean, rstd: fp32 [rows, groups] for the backward pass, or both NULL. */
+int ab_layer_norm_fwd(int dtype, int wtype, int64_t rows, int C, int groups, const void* x, int64_t x_stride, const void* w, const void* b,
+                      float eps, void* y, float* mean, float* rstd, void* stream);
+/* dx dense of dtype, dw and db [C] of wtype; NULL for what is not wanted. scratch: ab_layer_norm_scratch_bytes(rows, C), needed for dw or db. */
+size_t ab_layer_norm_scratch_bytes(int64_t rows, int C);
+int ab_layer_norm_bwd(int dtype, int wtype, int64_t rows, int C, int groups, const void* x, int64_t x_stride, const void* w, const float* mean,
+                      const float* rstd, const void* dy, int64_t dy_stride, void* dx, void* dw, void* db, void* scratch, void* stream);
+
+/* Rows of logits and one id each. Rows whose mask is 0 are not looked at, whatever they or their ids hold. An id outside the vocabulary
+ * in a row that counts is clamped and reported (bit 8 of ab_device_status). */
+typedef struct ab_logit_rows {
+    int32_t dtype, vocab;
+    int64_t rows, stride;        /* elements between rows */
+    const void* logits;
+    const int64_t* ids;          /* [rows] */
+    const uint8_t* mask;         /* [rows] of 0 and 1, or NULL: every row counts */
+} ab_logit_rows;
+/* logp[r] = logits[r, ids[r]] - log sum exp logits[r, :] (0 where masked): fp64 in `logp`, and fp32 in `logp32` where it is not NULL.
+ * stats: fp32 [rows, 2], maximum and 1 / sum exp(logits - maximum), for ab_token_logp_bwd; or NULL. */
+int ab_token_logp_fwd(const ab_logit_rows* t, double* logp, float* logp32, float* stats, void* stream);
+/* dlogits[r, :] = g[r / rows_per_g] * (scale ? *scale : 1) * (onehot(ids[r]) - softmax(logits[r, :])), zero where masked; dense rows of
+ * dtype. g: fp32 [rows / rows_per_g], scale: fp32 [1], both on the device. */
+int ab_token_logp_bwd(const ab_logit_rows* t, const float* stats, const float* g, int64_t rows_per_g, const float* scale, void* dlogits,
+                      void* stream);
+/* The clipped policy loss: with ratio = exp(logp - old_logp), each row's is -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A), plus
+ * kl * (exp(ref_logp - logp) - (ref_logp - logp) - 1) where ref_logp is not NULL; the loss is their sum over the rows that count by `denom`, or
+ * where that is 0 by their number (at least 1). */
+typedef struct ab_policy {
+    const float *old_logp, *advantages, *ref_logp;   /* [rows]; old_logp NULL: the present policy's own (ratio 1) */
+    float clip_low, clip_high, kl, denom;
+} ab_policy;
+/* loss: fp32 [1]. logp32: fp32 [rows]. g: fp32 [rows], for ab_token_logp_bwd with rows_per_g 1: the derivative of the loss by each row's
+ * log-probability. rows_scratch: fp64 [2 * rows + 2]. stats as above. */
+int ab_policy_loss_fwd(const ab_logit_rows* t, const ab_policy* p, float* loss, float* logp32, float* stats, float* g, double* rows_scratch,
+                       void* stream);
+/* Loss and scale * its gradient by the logits in one pass. dlogits: dense rows of dtype; it may be the logits themselves where they are dense. */
+int ab_policy_loss_grad(const ab_logit_rows* t, const ab_policy* p, float scale, float* loss, float* logp32, void* dlogits,
+                        double* rows_scratch, void* stream);
+/* The preference loss of `pairs` pairs of answers of `steps` rows each, first the better ones, then the worse ones, t->rows = 2 * pairs * steps:
+ * with s the sum of an answer's log-probabilities and m = beta * ((s_better - ref_better) - (s_worse - ref_worse)), the mean over the pairs of
+ * -(1 - smoothing) log sigmoid(m) - smoothing log sigmoid(-m). ref_logp: fp32 [2 * pairs]. logp32: fp32 [2 * pairs], the sums.
+ * g: fp32 [2 * pairs], for ab_token_logp_bwd with rows_per_g = steps. rows_scratch: fp64 [rows]. */
+int ab_preference_loss_fwd(const ab_logit_rows* t, int64_t pairs, int64_t steps, const float* ref_logp, float beta, float smoothing, float* loss,
+                           float* logp32, float* stats, float* g, double* rows_scratch, void* stream);
+
 /* ---- whole-model forward -------------------------------------------------------------------
  * ab_forward replaces RWKV_x070.forward / forward_batch (reference/rwkv7.py:98-126, :128-221):
  * tokens int32 [B,T] on the device; state = HOST array of 3*n_layer device pointers laid out as

@@ -1,6 +1,9 @@
 // Log-probabilities of ids under rows of logits, the losses built on them, and their gradients by the logits.
 //
 // logp = x[id] - m - log(sum exp(x - m)) with m the row's maximum; d logp / dx = onehot(id) - exp(x - m) / sum.
+#include <algorithm>
+#include <type_traits>
+
 #include "train.cuh"
 
 namespace ab {
@@ -30,79 +33,626 @@ __device__ __forceinline__ int row_id(const ab_logit_rows& t, int64_t r) {
     return id < 0 ? 0 : t.vocab - 1;
 }
 
-// maximum and sum of exp(x - maximum) of two sets; a set without values above -inf has sum 0
-__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
-    const float top = fmaxf(m, m2);
-    s = (m == top ? s : s * expf(m - top)) + (m2 == top ? s2 : s2 * expf(m2 - top));
-    m = top;
+struct PolicyRow {
+    float A, old, ref;
+};
+__device__ __forceinline__ PolicyRow policy_load(const ab_policy& p, int64_t r) {
+    return {p.advantages[r], p.old_logp ? p.old_logp[r] : 0.f, p.ref_logp ? p.ref_logp[r] : 0.f};
 }
-// the row's loss and its derivative by the log-probability
-__device__ __forceinline__ double policy_row(const ab_policy& p, int64_t r, double logp, float* g) {
-    const double A = p.advantages[r], ratio = p.old_logp ? exp(logp - (double)p.old_logp[r]) : 1.0;
+// the row's loss, and its derivative by the log-probability
+template <class F>
+__device__ __forceinline__ F policy_slope_of(F plain, F clipped, bool ref, F kl, F e) {
+    return (clipped < plain ? (F)0 : -plain) + (ref ? kl * ((F)1 - e) : (F)0);
+}
+__device__ __forceinline__ double policy_row(const ab_policy& p, const PolicyRow& q, double logp, double* g) {
+    const double A = q.A, ratio = p.old_logp ? exp(logp - (double)q.old) : 1.0;
     const double plain = ratio * A, clipped = fmin(fmax(ratio, 1.0 - (double)p.clip_low), 1.0 + (double)p.clip_high) * A;
-    double loss = -(clipped < plain ? clipped : plain), d = clipped < plain ? 0.0 : -plain;
-    if (p.ref_logp) {
-        const double gap = (double)p.ref_logp[r] - logp;
-        loss += (double)p.kl * (exp(gap) - gap - 1.0);
-        d += (double)p.kl * (1.0 - exp(gap));
-    }
-    *g = (float)d;
-    return loss;
+    const double gap = (double)q.ref - logp, e = p.ref_logp ? exp(gap) : 1.0;
+    *g = policy_slope_of(plain, clipped, p.ref_logp != nullptr, (double)p.kl, e);
+    return -(clipped < plain ? clipped : plain) + (p.ref_logp ? (double)p.kl * (e - gap - 1.0) : 0.0);
+}
+__device__ __forceinline__ float policy_slope(const ab_policy& p, const PolicyRow& q, double logp) {
+    const float ratio = p.old_logp ? expf((float)(logp - (double)q.old)) : 1.f, plain = ratio * q.A;
+    const float clipped = fminf(fmaxf(ratio, 1.f - p.clip_low), 1.f + p.clip_high) * q.A;
+    return policy_slope_of(plain, clipped, p.ref_logp != nullptr, p.kl, p.ref_logp ? expf((float)((double)q.ref - logp)) : 1.f);
 }
 
+// ---- a row in registers --------------------------------------------------------------------------------------------
+// A row is taken in pieces of 16 bytes on 16-byte addresses, whatever address it starts on: the first and the last piece may hold
+// values of its neighbours, which count as -inf and are not written.
 template <class E>
-__global__ void __launch_bounds__(LT) logit_rows_kernel(const __grid_constant__ RowTask k) {
-    __shared__ float red_m[LT / 32], red_s[LT / 32], s_g;
-    const int64_t r = blockIdx.x;
-    const int V = k.t.vocab, tid = threadIdx.x;
+struct Pieces {
+    static constexpr int N = 16 / sizeof(E);
+    const E* x;        // the first piece's address
+    int lead, n, V;    // values of the first piece in front of the row; pieces; values of the row
+    __device__ __forceinline__ Pieces(const E* row, int V_) : V(V_) {
+        lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(E));
+        x = row - lead;
+        n = (V + lead + N - 1) / N;
+    }
+    // pieces i0 .. i1 - 1 hold values of the row alone
+    __device__ __forceinline__ bool all_whole(int i0, int i1) const { return i0 * N >= lead && i1 * N <= V + lead; }
+    template <bool FULL>
+    __device__ __forceinline__ uint4 get(int i) const {
+        if (FULL) return AB_BC(whole(i)) ? __ldcs(reinterpret_cast<const uint4*>(x) + i) : none();
+        return load(i);
+    }
+    __device__ __forceinline__ bool whole(int i) const { return i * N >= lead && (i + 1) * N <= V + lead; }
+    __device__ __forceinline__ uint4 load(int i) const {
+        if (i >= n) return none();
+        if (whole(i)) return AB_BC(i * N - lead + N <= V) ? __ldcs(reinterpret_cast<const uint4*>(x) + i) : none();
+        uint4 u = none();
+        E* e = reinterpret_cast<E*>(&u);
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+            if (i * N + c >= lead && i * N + c < V + lead) e[c] = x[i * N + c];
+        return u;
+    }
+    static __device__ __forceinline__ uint4 none() {   // -inf throughout
+        const uint32_t w = sizeof(E) == 4 ? 0xff800000u : std::is_same<E, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+        return make_uint4(w, w, w, w);
+    }
+};
+template <class E> __device__ __forceinline__ void unpack(const uint4& u, float* f);
+template <> __device__ __forceinline__ void unpack<float>(const uint4& u, float* f) {
+    f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+}
+template <> __device__ __forceinline__ void unpack<__half>(const uint4& u, float* f) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = __half22float2(h[i]);
+        f[2 * i] = v.x, f[2 * i + 1] = v.y;
+    }
+}
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& u, float* f) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+template <class E> __device__ __forceinline__ uint4 pack(const float* f);
+template <> __device__ __forceinline__ uint4 pack<float>(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+template <> __device__ __forceinline__ uint4 pack<__half>(const float* f) {
+    uint4 u;
+    __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    return u;
+}
+template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float* f) {
+    uint4 u;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    return u;
+}
+// the larger values of two pieces, place by place (a NaN gives way: it is left to the sums), and the largest of one
+template <class E>
+__device__ __forceinline__ uint4 piece_max(uint4 a, const uint4& b) {
+    uint32_t *x = &a.x;
+    const uint32_t* y = &b.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<E, float>::value) x[i] = __float_as_uint(fmaxf(__uint_as_float(x[i]), __uint_as_float(y[i])));
+        else if constexpr (std::is_same<E, __half>::value) asm("max.f16x2 %0, %0, %1;" : "+r"(x[i]) : "r"(y[i]));
+        else asm("max.bf16x2 %0, %0, %1;" : "+r"(x[i]) : "r"(y[i]));
+    }
+    return a;
+}
+template <class E>
+__device__ __forceinline__ float piece_top(const uint4& u) {
+    float f[Pieces<E>::N];
+    unpack<E>(u, f);
+    float m = f[0];
+#pragma unroll
+    for (int c = 1; c < Pieces<E>::N; ++c) m = fmaxf(m, f[c]);
+    return m;
+}
+// What exponentials are taken relative to: exp(x - m) = 2^(x log2(e) - c) with c = m log2(e) rounded, one multiply-add and one ex2.approx (good to 2^-22).
+// Joining parts takes the difference of two c, so that the rounding of c cancels. Beyond 2^20 it would be more than 2^-4 itself, and at the type's ends (rows of the
+// lowest value throughout, which some programs use for a mask) the product overflows: there the difference comes first.
+constexpr float LOG2E = 1.4426950408889634f;
+struct Ref {
+    float m, c;
+    bool huge;
+    __device__ __forceinline__ Ref(float top) : m(top == -INFINITY ? 0.f : top), c(m * LOG2E), huge(fabsf(m) > 1048576.f) {}   // (nothing above -inf: sums of 0 or NaN)
+};
+__device__ __forceinline__ float ex2(float x) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+    return e;
+}
+template <int N>
+__device__ __forceinline__ void exp_from(float* f, const Ref& r) {
+    if (r.huge) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = ex2((f[i] - r.m) * LOG2E);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = ex2(fmaf(f[i], LOG2E, -r.c));
+    }
+}
+__device__ __forceinline__ float exp_from(float x, const Ref& r) {
+    exp_from<1>(&x, r);
+    return x;
+}
+// 2^(difference of two references): what a sum relative to the first becomes relative to the second
+__device__ __forceinline__ float rebase(const Ref& from, const Ref& to) { return from.huge || to.huge ? ex2((from.m - to.m) * LOG2E) : ex2(from.c - to.c); }
+// Writes p times a piece's exponentials to the row `dx`, which starts `lead` values into a piece of 16 bytes as the row of logits does (aligned), or anywhere.
+// FULL: the piece holds values of the row alone, and dx is aligned.
+template <class E, bool FULL>
+__device__ __forceinline__ void write_piece(const Pieces<E>& row, const float* e, int i, E* dx, bool aligned, float p) {
+    constexpr int N = Pieces<E>::N;
+    if (!FULL && i >= row.n) return;
+    float f[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) f[c] = e[c] * p;
+    const int first = i * N - row.lead;
+    const uint4 out = pack<E>(f);
+    if (FULL || (aligned && row.whole(i))) {
+        if (AB_BC(first >= 0 && first + N <= row.V)) __stcs(reinterpret_cast<uint4*>(dx - row.lead) + i, out);
+    } else {
+        const E* o = reinterpret_cast<const E*>(&out);
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+            if (first + c >= 0 && first + c < row.V) dx[first + c] = o[c];
+    }
+}
+template <class E>
+__device__ __forceinline__ void write_zeros(E* dx, int V, int at, int step) {   // this thread's share: pieces at, at + step, ...
+    const Pieces<E> row(dx, V);
+    for (int i = at; i < row.n; i += step) {
+        const int first = i * Pieces<E>::N - row.lead;
+        if (row.whole(i)) __stcs(reinterpret_cast<uint4*>(dx + first), make_uint4(0, 0, 0, 0));
+        else
+            for (int c = max(first, 0); c < min(first + Pieces<E>::N, V); ++c) dx[c] = from_f<E>(0.f);
+    }
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_blocks() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+
+constexpr int LW = LT / 32, MAX_CLUSTER = 8;
+
+__device__ __forceinline__ float warp_top(float v) {   // warp_max in one instruction
+    asm("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
+    return v;
+}
+
+// rows that count, up to all of them, as this thread's share of a block of LT
+__device__ __forceinline__ int count_rows(const uint8_t* mask, int64_t rows) {
+    if (!mask) return threadIdx.x == 0 ? (int)rows : 0;
+    const int lead = (int)min((int64_t)((16 - (reinterpret_cast<uintptr_t>(mask) & 15)) & 15), rows), pieces = (int)((rows - lead) / 16);
+    int n = 0;
+    for (int i = threadIdx.x; i < pieces; i += LT) {
+        const uint4 u = *(reinterpret_cast<const uint4*>(mask + lead) + i);   // bytes of 0 and 1
+        n = __dp4a(u.x, 0x01010101u, __dp4a(u.y, 0x01010101u, __dp4a(u.z, 0x01010101u, __dp4a(u.w, 0x01010101u, (unsigned)n))));
+    }
+    if ((int)threadIdx.x < lead) n += mask[threadIdx.x];
+    const int64_t tail = lead + (int64_t)pieces * 16 + threadIdx.x;
+    if (threadIdx.x < 16 && tail < rows) n += mask[tail];
+    return n;
+}
+
+// One row per cluster of blocks, a run of pieces per block; a thread keeps the exponentials of EPT values in registers between the sums and the gradient, so
+// that the logits are read once and each exponential is taken once (rows longer than MAX_CLUSTER * LT * EPT values are read twice).
+template <class E, int EPT>
+__global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant__ RowTask k) {
+    constexpr int N = Pieces<E>::N, NV = EPT / N;
+    __shared__ float2 part[MAX_CLUSTER * LW];   // maximum and sum of every warp of the cluster
+    __shared__ int s_count[LW];
+    __shared__ float4 s_join;
+    const uint32_t rank = cluster_rank(), nb = cluster_blocks();
+    const int64_t r = blockIdx.x / nb;
+    const int V = k.t.vocab, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     E* dx = k.dlogits ? static_cast<E*>(k.dlogits) + r * V : nullptr;
+    pdl_launch_dependents();
     if (!counts(k.t, r)) {
-        if (tid == 0) {
+        if (tid == 0 && rank == 0) {
             if (k.logp) k.logp[r] = 0.0;
             if (k.logp32) k.logp32[r] = 0.f;
             if (k.row_loss) k.row_loss[r] = 0.0;
             if (k.g) k.g[r] = 0.f;
             if (k.stats) k.stats[2 * r] = k.stats[2 * r + 1] = 0.f;
         }
-        if (dx)
-            for (int i = tid; i < V; i += LT) dx[i] = from_f<E>(0.f);
+        if (dx) write_zeros(dx, V, (int)rank * LT + tid, (int)nb * LT);
         return;
     }
-    const E* x = static_cast<const E*>(k.t.logits) + r * k.t.stride;
-    const int id = row_id(k.t, r);
-    const float at = to_f(x[id]);
-    float m = -INFINITY, s = 0.f;
-    for (int i = tid; i < V; i += LT) m = fmaxf(m, to_f(x[i]));
-    m = warp_max(m);
-    if ((tid & 31) == 0) red_m[tid >> 5] = m;
-    __syncthreads();
-    for (int i = 0; i < LT / 32; ++i) m = fmaxf(m, red_m[i]);
-    for (int i = tid; i < V; i += LT) s += expf(to_f(x[i]) - m);
-    s = warp_sum(s);
-    if ((tid & 31) == 0) red_s[tid >> 5] = s;
-    __syncthreads();
-    s = 0.f;
-    for (int i = 0; i < LT / 32; ++i) s += red_s[i];
-    if (tid == 0) {
-        const double logp = (double)(at - m) - log((double)s);
-        if (k.logp) k.logp[r] = logp;
-        if (k.logp32) k.logp32[r] = (float)logp;
-        if (k.stats) {
-            k.stats[2 * r] = m;
-            k.stats[2 * r + 1] = 1.f / s;
+    const Pieces<E> row(static_cast<const E*>(k.t.logits) + r * k.t.stride, V);
+    const int step = (int)nb * LT * NV, at0 = (int)rank * LT * NV;
+    const bool aligned = dx && (reinterpret_cast<uintptr_t>(dx) & 15) == row.lead * sizeof(E);
+    const bool once = row.n <= step, full = once && row.all_whole(at0, at0 + LT * NV) && (aligned || !dx);
+    float e[EPT], m = -INFINITY, s = 0.f, at = 0.f;
+    int id = 0;
+    PolicyRow pr = {};
+    auto sums = [&](auto whole, int base) {
+        uint4 u[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) u[j] = row.template get<decltype(whole)::value>(base + at0 + j * LT + tid);
+        if (base == 0) {
+            id = row_id(k.t, r);
+            at = to_f(row.x[row.lead + id]);
+            if (k.policy) pr = policy_load(k.p, r);
         }
-        if (k.policy) {
-            float g;
-            const double loss = policy_row(k.p, r, logp, &g);
-            k.row_loss[r] = loss;
-            if (k.g) k.g[r] = g;
-            s_g = dx ? g * *k.inv_denom * k.scale : 0.f;
+        uint4 top4 = u[0];
+#pragma unroll
+        for (int j = 1; j < NV; ++j) top4 = piece_max<E>(top4, u[j]);
+        const float top = warp_top(fmaxf(m, piece_top<E>(top4)));
+        const Ref ref(top);
+        if (m != top) s *= m == -INFINITY ? 1.f : rebase(Ref(m), ref), m = top;   // (m -inf: s is 0 or NaN, and stays so)
+        float sum[4] = {s, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) unpack<E>(u[j], e + j * N);
+        exp_from<EPT>(e, ref);
+#pragma unroll
+        for (int c = 0; c < EPT; ++c) sum[c & 3] += e[c];
+        s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+    if (full) sums(std::true_type(), 0);
+    else
+        for (int base = 0; base < row.n; base += step) sums(std::false_type(), base);
+    s = warp_sum(s);
+    if (lane < (int)nb) {                                  // to every block of the cluster
+        uint32_t there;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(&part[rank * LW + warp])), "r"(lane));
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(m), "f"(s) : "memory");
+    }
+    const bool counting = k.policy && dx && !k.inv_denom;  // every block counts the rows that count, for the loss's denominator
+    if (counting) {
+        const int n = __reduce_add_sync(0xffffffffu, count_rows(k.t.mask, k.t.rows));
+        if (lane == 0) s_count[warp] = n;
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp == 0) {
+        // one warp joins the parts, in one order
+        float2 a = make_float2(-INFINITY, 0.f), b = a;
+        const int n_parts = (int)nb * LW;
+        if (lane < n_parts) a = part[lane];
+        if (lane + 32 < n_parts) b = part[lane + 32];
+        const float M = warp_top(fmaxf(a.x, b.x));
+        const Ref ref(M);
+        // (a part without values has sum 0 or NaN)
+        float S = warp_sum(a.y * (a.x == -INFINITY ? 1.f : rebase(Ref(a.x), ref)) + b.y * (b.x == -INFINITY ? 1.f : rebase(Ref(b.x), ref)));
+        if (M == -INFINITY) S = NAN;                       // no probabilities to speak of
+        // the id's value relative to the reference, with the constant that the exponentials were taken with
+        const double rel = ref.huge ? (double)at - (double)M : ((double)at * (double)LOG2E - (double)ref.c) * 0.6931471805599453094;
+        if (dx) {
+            // the gradient's coefficient in 32 bits: off by some 5e-7 of it, from the logarithm
+            int n = 0;
+            if (counting)
+                for (int i = 0; i < LW; ++i) n += s_count[i];
+            const float g = policy_slope(k.p, pr, rel - (double)logf(S)) * (counting ? 1.f / (float)max(n, 1) : *k.inv_denom) * k.scale;
+            if (lane == 0) s_join = make_float4(M, -g / S, g, 0.f);
+            __syncwarp();
+            asm volatile("bar.arrive 1, %0;" ::"n"(LT) : "memory");
+        }
+        if (lane == 0 && rank == 0) {                      // (while the other warps write)
+            const double logp = rel - log((double)S);
+            if (k.logp) k.logp[r] = logp;
+            if (k.logp32) k.logp32[r] = (float)logp;
+            if (k.stats) {
+                k.stats[2 * r] = M;
+                k.stats[2 * r + 1] = 1.f / S;
+            }
+            if (k.policy) {
+                double g;
+                k.row_loss[r] = policy_row(k.p, pr, logp, &g);
+                if (k.g) k.g[r] = (float)g;
+            }
         }
     }
     if (!dx) return;
+    if (warp != 0) asm volatile("bar.sync 1, %0;" ::"n"(LT) : "memory");
+    else __syncwarp();
+    const float4 join = s_join;
+    const float M = join.x, p = join.y, g = join.z;
+    const Ref ref(M);
+    const float mine = p * (m == -INFINITY ? 1.f : rebase(Ref(m), ref));   // the exponentials are relative to the warp's maximum
+    if (full) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) write_piece<E, true>(row, e + j * N, at0 + j * LT + tid, dx, aligned, mine);
+    } else if (once) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) write_piece<E, false>(row, e + j * N, at0 + j * LT + tid, dx, aligned, mine);
+    } else {
+        for (int i = at0; i < row.n; i += step)
+            for (int j = 0; j < NV; ++j) {
+                unpack<E>(row.load(i + j * LT + tid), e);
+                exp_from<N>(e, ref);
+                write_piece<E, false>(row, e, i + j * LT + tid, dx, aligned, p);
+            }
+    }
+    // the id's own value, by the thread that wrote its piece
+    const int own = (id + row.lead) / N - at0;
+    if (own >= 0 && own % step < LT * NV && own % LT == tid) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));
+}
+
+// ---- long rows, at least one per SM ----------------------------------------------------------------------------------
+// One block per SM takes row after row: a warp asks for a row's chunks with bulk copies into a ring, ahead of the warps that add them up and then go through the ring
+// once more for the gradient; as they hand chunks back the next row's come in, so that copies are under way through the sums, the join and the gradient alike. Which row
+// comes next is asked of the hardware (cluster launch control: the grid has a block per row, and a running block takes the place of one that has not started), because
+// masked rows cost little and would unbalance fixed shares. What a row needs besides its logits (id, policy) travels the same way ahead of it; a row's own
+// log-probability and loss, in 64 bits, are the business of another warp.
+// 4096 x 65536 fp16 rows with gradients, which a cluster of eight blocks per row (logit_rows_kernel) takes 302 us for: see row_shape.
+constexpr int RING_WARPS = 16, RING_THREADS = (RING_WARPS + 2) * 32, RING_CHUNK = 32768, RING_SLOTS = 7, RING_ROWS = 4;   // working warps; chunks, rows under way
+struct RingRow {
+    int64_t r;          // -1: no more
+    int on, id;
+    float at;
+    PolicyRow pr;
+    double rel;         // from the working warps for the finishing one
+    float M, S;
+};
+struct RingShared {
+    uint4 cancel;
+    uint64_t full[RING_SLOTS], vacant[RING_SLOTS], row_full[RING_ROWS], row_summed[RING_ROWS], row_vacant[RING_ROWS], joined, cancelled;
+    RingRow row[RING_ROWS];
+    float2 part[2][RING_WARPS];   // of a row, and of the one after it
+    int count[RING_WARPS + 2], failed;
+    uint32_t nobody;
+};
+
+template <class E>
+__global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __grid_constant__ RowTask k) {
+    constexpr int N = Pieces<E>::N, PER = RING_CHUNK / 16 / (RING_WARPS * 32);   // a thread's pieces of a chunk
+    extern __shared__ __align__(128) unsigned char ring[];            // RING_SLOTS chunks
+    __shared__ RingShared sh;
+    const int V = k.t.vocab, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < RING_SLOTS; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.vacant[i], RING_WARPS);
+        for (int i = 0; i < RING_ROWS; ++i) mbar_init(&sh.row_full[i], 1), mbar_init(&sh.row_summed[i], 1), mbar_init(&sh.row_vacant[i], RING_WARPS + 1);
+        mbar_init(&sh.joined, RING_WARPS);
+        mbar_init(&sh.cancelled, 1);
+        fence_mbar_init();
+        sh.failed = 0;
+    }
+    const bool counting = k.policy && k.dlogits && !k.inv_denom;
+    if (counting) {
+        int n = 0;
+        for (int64_t i = tid; i < k.t.rows; i += RING_THREADS) n += counts(k.t, i) ? 1 : 0;
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (lane == 0) sh.count[warp] = n;
+    }
     __syncthreads();
-    const float g = s_g, p = g / s;
-    for (int i = tid; i < V; i += LT) dx[i] = from_f<E>((i == id ? g : 0.f) - p * expf(to_f(x[i]) - m));
+    pdl_launch_dependents();
+    // after the first wait that runs out nobody waits any more
+    auto wait_for = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*reinterpret_cast<volatile int*>(&sh.failed)) return false;
+        if (mbar_wait_bounded(bar, parity, 1u << 18)) return true;
+        *reinterpret_cast<volatile int*>(&sh.failed) = 1;
+        atomicOr(&g_device_status, DEV_WAIT_HEAD);
+        return false;
+    };
+    const E* logits = static_cast<const E*>(k.t.logits);
+    // the pieces of a row that are copied: those that hold its values alone
+    auto span = [&](const Pieces<E>& row, int& first, int& end) {
+        first = row.lead ? 1 : 0;
+        end = (V + row.lead) / N;
+    };
+    constexpr int CP = RING_CHUNK / 16;   // pieces of a chunk
+
+    if (warp == RING_WARPS) {
+        if (lane == 0) {
+            int64_t r = blockIdx.x;
+            int c_issued = 0, asked = 0, answered = 0;
+            bool ok = true;
+            for (int n = 0; ok; ++n) {
+                RingRow& q = sh.row[n % RING_ROWS];
+                if (n >= RING_ROWS && !wait_for(&sh.row_vacant[n % RING_ROWS], (uint32_t)(n / RING_ROWS - 1) & 1u)) break;
+                if (r >= 0) {
+                    // ask for the row after this one
+                    fence_proxy_async();
+                    ++asked;
+                    mbar_expect_tx(&sh.cancelled, 16);
+                    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(&sh.cancel)),
+                                 "r"(smem_u32(&sh.cancelled)) : "memory");
+                }
+                q.r = r;
+                if (r >= 0) {
+                    q.on = counts(k.t, r);
+                    if (q.on) {
+                        const Pieces<E> row(logits + r * k.t.stride, V);
+                        int first, end;
+                        span(row, first, end);
+                        const int chunks = (end - first + CP - 1) / CP, rounds = chunks > RING_SLOTS && k.dlogits ? 2 : 1;
+                        bool published = false;
+                        for (int round = 0; round < rounds && ok; ++round)
+                            for (int c = 0; c < chunks && ok; ++c, ++c_issued) {
+                                const int slot = c_issued % RING_SLOTS, p0 = first + c * CP, np = min(CP, end - p0);
+                                if (c_issued >= RING_SLOTS) ok = wait_for(&sh.vacant[slot], (uint32_t)(c_issued / RING_SLOTS - 1) & 1u);
+                                if (!ok) break;
+                                mbar_expect_tx(&sh.full[slot], np * 16);
+                                bulk_g2s(ring + (size_t)slot * RING_CHUNK, reinterpret_cast<const uint4*>(row.x) + p0, np * 16, &sh.full[slot]);
+                                if (!published) {                        // the rest of what the row needs, while its first chunk travels
+                                    published = true;
+                                    const int64_t id = k.t.ids[r];
+                                    q.id = (uint64_t)id < (uint64_t)V ? (int)id : (atomicOr(&g_device_status, DEV_BAD_TOKEN), id < 0 ? 0 : V - 1);
+                                    q.at = to_f(row.x[row.lead + q.id]);
+                                    if (k.policy) q.pr = policy_load(k.p, r);
+                                    mbar_arrive(&sh.row_full[n % RING_ROWS]);
+                                }
+                            }
+                    } else {
+                        mbar_arrive(&sh.row_full[n % RING_ROWS]);
+                    }
+                    if (!ok || !wait_for(&sh.cancelled, (uint32_t)n & 1u)) break;
+                    ++answered;
+                    uint32_t got, next;
+                    asm volatile("{\n .reg .pred p;\n .reg .b128 h;\n ld.shared.b128 h, [%2];\n"
+                                 " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
+                                 " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n}"
+                                 : "=r"(got), "=r"(next) : "r"(smem_u32(&sh.cancel)) : "memory");
+                    r = got ? (int64_t)next : -1;
+                } else {
+                    mbar_arrive(&sh.row_full[n % RING_ROWS]);
+                    break;
+                }
+            }
+            // whatever became of the waits, all that was asked for lands before the block ends
+            for (int c = max(0, c_issued - RING_SLOTS); c < c_issued; ++c) mbar_wait_bounded(&sh.full[c % RING_SLOTS], (uint32_t)(c / RING_SLOTS) & 1u, 1u << 18);
+            if (answered < asked) mbar_wait_bounded(&sh.cancelled, (uint32_t)answered & 1u, 1u << 18);
+        }
+    } else if (warp == RING_WARPS + 1) {
+        if (lane == 0) {
+            for (int n = 0;; ++n) {
+                RingRow& q = sh.row[n % RING_ROWS];
+                if (!wait_for(&sh.row_full[n % RING_ROWS], (uint32_t)(n / RING_ROWS) & 1u) || q.r < 0) break;
+                if (!wait_for(&sh.row_summed[n % RING_ROWS], (uint32_t)(n / RING_ROWS) & 1u)) break;
+                double logp = 0.0, loss = 0.0, g = 0.0;
+                if (q.on) {
+                    logp = q.rel - log((double)q.S);
+                    if (k.policy) loss = policy_row(k.p, q.pr, logp, &g);
+                }
+                if (k.logp) k.logp[q.r] = logp;
+                if (k.logp32) k.logp32[q.r] = (float)logp;
+                if (k.stats) k.stats[2 * q.r] = q.on ? q.M : 0.f, k.stats[2 * q.r + 1] = q.on ? 1.f / q.S : 0.f;
+                if (k.policy) k.row_loss[q.r] = loss;
+                if (k.policy && k.g) k.g[q.r] = (float)g;
+                mbar_arrive(&sh.row_vacant[n % RING_ROWS]);
+            }
+        }
+    } else {
+        float inv_n = counting ? 0.f : k.inv_denom ? *k.inv_denom : 1.f;
+        if (counting) {
+            int n = 0;
+            for (int i = 0; i < RING_WARPS + 2; ++i) n += sh.count[i];
+            inv_n = 1.f / (float)max(n, 1);
+        }
+        int c_seen = 0, joins = 0;
+        for (int n = 0;; ++n) {
+            RingRow& q = sh.row[n % RING_ROWS];
+            if (!__all_sync(0xffffffffu, wait_for(&sh.row_full[n % RING_ROWS], (uint32_t)(n / RING_ROWS) & 1u))) break;
+            const int64_t r = q.r;
+            if (r < 0) break;
+            E* dx = k.dlogits ? static_cast<E*>(k.dlogits) + r * V : nullptr;
+            if (!q.on) {
+                if (dx) write_zeros(dx, V, tid, RING_WARPS * 32);
+                if (tid == 0) mbar_arrive(&sh.row_summed[n % RING_ROWS]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.row_vacant[n % RING_ROWS]);
+                continue;
+            }
+            const Pieces<E> row(logits + r * k.t.stride, V);
+            int first, end;
+            span(row, first, end);
+            const int chunks = (end - first + CP - 1) / CP;
+            const bool twice = chunks > RING_SLOTS && dx;
+            // the two ends of a row that are not copied, by the first two threads
+            const int edge = tid == 0 && first ? 0 : tid == 1 && end < row.n ? end : -1;
+            uint4 eu = Pieces<E>::none();
+            if (edge >= 0) eu = row.load(edge);
+            float m = -INFINITY, s = 0.f;
+            auto add = [&](const uint4* u, int np) {
+                uint4 t4 = u[0];
+                for (int j = 1; j < np; ++j) t4 = piece_max<E>(t4, u[j]);
+                const float top = warp_top(fmaxf(m, piece_top<E>(t4)));
+                const Ref ref(top);
+                if (m != top) s *= m == -INFINITY ? 1.f : rebase(Ref(m), ref), m = top;
+                float sum[4] = {s, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    if (j >= np) break;
+                    float e[N];
+                    unpack<E>(u[j], e);
+                    exp_from<N>(e, ref);
+#pragma unroll
+                    for (int c = 0; c < N; ++c) sum[c & 3] += e[c];
+                }
+                s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            };
+            if (warp == 0) add(&eu, 1);
+            auto hand_back = [&](int slot, const uint4* u) {
+                uint32_t used = 0;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) used ^= u[j].x ^ u[j].w;
+                loads_returned(used, &sh.nobody);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.vacant[slot]);
+            };
+            auto take = [&](int c, uint4* u) {   // chunk c of the row
+                const int slot = c_seen % RING_SLOTS, np = end - first - c * CP;
+                wait_for(&sh.full[slot], (uint32_t)(c_seen / RING_SLOTS) & 1u);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const int i = j * RING_WARPS * 32 + tid;
+                    u[j] = i < np ? *reinterpret_cast<const uint4*>(ring + (size_t)slot * RING_CHUNK + i * 16) : Pieces<E>::none();
+                }
+                ++c_seen;
+                return slot;
+            };
+            const int c0 = c_seen;
+            for (int c = 0; c < chunks; ++c) {
+                uint4 u[PER];
+                const int slot = take(c, u);
+                add(u, PER);
+                if (!dx || twice) hand_back(slot, u);
+            }
+            s = warp_sum(s);
+            float2* part = sh.part[joins & 1];   // (written again two rows on: behind the next row's join, which every warp reaches after it has read it)
+            if (lane == 0) {
+                part[warp] = make_float2(m, s);
+                mbar_arrive(&sh.joined);
+            }
+            wait_for(&sh.joined, (uint32_t)joins++ & 1u);
+            __syncwarp();
+            const float2 a = lane < RING_WARPS ? part[lane] : make_float2(-INFINITY, 0.f);
+            const float M = warp_top(a.x);
+            const Ref ref(M);
+            float S = warp_sum(a.y * (a.x == -INFINITY ? 1.f : rebase(Ref(a.x), ref)));   // (a part without values has sum 0 or NaN)
+            if (M == -INFINITY) S = NAN;
+            const float at = q.at;
+            const int id = q.id;
+            const double rel = ref.huge ? (double)at - (double)M : ((double)at * (double)LOG2E - (double)ref.c) * 0.6931471805599453094;
+            const float g = dx ? policy_slope(k.p, q.pr, rel - (double)logf(S)) * inv_n * k.scale : 0.f, p = -g / S;
+            if (tid == 0) {
+                q.rel = rel, q.M = M, q.S = S;
+                mbar_arrive(&sh.row_summed[n % RING_ROWS]);
+            }
+            if (dx) {
+                const bool aligned = (reinterpret_cast<uintptr_t>(dx) & 15) == row.lead * sizeof(E);
+                if (!twice) c_seen = c0;
+                for (int c = 0; c < chunks; ++c) {
+                    uint4 u[PER];
+                    const int slot = take(c, u);
+                    hand_back(slot, u);
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) {
+                        const int i = c * CP + j * RING_WARPS * 32 + tid;
+                        float e[N];
+                        unpack<E>(u[j], e);
+                        exp_from<N>(e, ref);
+                        if (i < end - first) {
+                            if (aligned) write_piece<E, true>(row, e, first + i, dx, true, p);
+                            else write_piece<E, false>(row, e, first + i, dx, false, p);
+                        }
+                    }
+                }
+                if (edge >= 0) {
+                    float e[N];
+                    unpack<E>(eu, e);
+                    exp_from<N>(e, ref);
+                    write_piece<E, false>(row, e, edge, dx, aligned, p);
+                }
+                // the id's own value, by the thread that wrote its piece
+                const int piece = (id + row.lead) / N;
+                if (piece >= first && piece < end ? (piece - first) % (RING_WARPS * 32) == tid : piece == edge) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.row_vacant[n % RING_ROWS]);
+        }
+    }
 }
 
 struct DlogitsTask {
@@ -110,20 +660,43 @@ struct DlogitsTask {
     const float *stats, *g, *scale;
     int64_t rows_per_g;
     void* dlogits;
+    int blocks;      // per row
 };
+constexpr int DV = 4;   // pieces per thread of the gradient's kernel
 template <class E>
-__global__ void __launch_bounds__(LT) dlogits_kernel(const __grid_constant__ DlogitsTask k) {
-    const int64_t r = blockIdx.x;
-    const int V = k.t.vocab;
+__global__ void __launch_bounds__(LT, 6) dlogits_kernel(const __grid_constant__ DlogitsTask k) {
+    constexpr int N = Pieces<E>::N;
+    const int64_t r = blockIdx.x / k.blocks;
+    const int V = k.t.vocab, blk = (int)(blockIdx.x - r * k.blocks), tid = threadIdx.x, at0 = blk * LT * DV;
     E* dx = static_cast<E*>(k.dlogits) + r * V;
     if (!counts(k.t, r)) {
-        for (int i = threadIdx.x; i < V; i += LT) dx[i] = from_f<E>(0.f);
+        write_zeros(dx, V, blk * LT + tid, k.blocks * LT);
         return;
     }
-    const E* x = static_cast<const E*>(k.t.logits) + r * k.t.stride;
-    const int id = row_id(k.t, r);
-    const float g = k.g[r / k.rows_per_g] * (k.scale ? *k.scale : 1.f), m = k.stats[2 * r], p = g * k.stats[2 * r + 1];
-    for (int i = threadIdx.x; i < V; i += LT) dx[i] = from_f<E>((i == id ? g : 0.f) - p * expf(to_f(x[i]) - m));
+    const Pieces<E> row(static_cast<const E*>(k.t.logits) + r * k.t.stride, V);
+    const bool aligned = (reinterpret_cast<uintptr_t>(dx) & 15) == row.lead * sizeof(E);
+    auto write = [&](auto whole) {
+        constexpr bool FULL = decltype(whole)::value;
+        uint4 u[DV];
+#pragma unroll
+        for (int j = 0; j < DV; ++j) u[j] = row.template get<FULL>(at0 + j * LT + tid);
+        const int id = row_id(k.t, r);
+        const float g = k.g[r / k.rows_per_g] * (k.scale ? *k.scale : 1.f), p = -g * k.stats[2 * r + 1];
+        const Ref ref(k.stats[2 * r]);
+        const int own = (id + row.lead) / N - at0;
+        const bool mine = own >= 0 && own < LT * DV && own % LT == tid;
+        const float x_id = mine ? to_f(row.x[row.lead + id]) : 0.f;
+#pragma unroll
+        for (int j = 0; j < DV; ++j) {
+            float e[N];
+            unpack<E>(u[j], e);
+            exp_from<N>(e, ref);
+            write_piece<E, FULL>(row, e, at0 + j * LT + tid, dx, aligned, p);
+        }
+        if (mine) dx[id] = from_f<E>(fmaf(p, exp_from(x_id, ref), g));
+    };
+    if (aligned && row.all_whole(at0, at0 + LT * DV)) write(std::true_type());
+    else write(std::false_type());
 }
 
 constexpr int JT = 1024;
@@ -139,30 +712,29 @@ __device__ __forceinline__ double block_sum_jt(double v, double* red) {
 }
 
 // 1 / what the rows' losses are divided by
-__global__ void __launch_bounds__(JT) policy_denom_kernel(const uint8_t* mask, int64_t rows, float denom, double* out, float* out32) {
+__device__ __forceinline__ double policy_inv_denom(const uint8_t* mask, int64_t rows, float denom, double* red) {
+    if (denom != 0.f) return 1.0 / (double)denom;
+    int n = 0;
+    for (int64_t r = threadIdx.x; r < rows; r += JT) n += !mask || mask[r] ? 1 : 0;
+    return 1.0 / fmax(block_sum_jt((double)n, red), 1.0);
+}
+__global__ void __launch_bounds__(JT) policy_denom_kernel(const uint8_t* mask, int64_t rows, float denom, float* inv) {
     __shared__ double red[JT / 32];
-    double n = 0.0;
-    if (denom == 0.f) {
-        for (int64_t r = threadIdx.x; r < rows; r += JT) n += !mask || mask[r] ? 1.0 : 0.0;
-        n = fmax(block_sum_jt(n, red), 1.0);
-    } else {
-        n = (double)denom;
-    }
-    if (threadIdx.x == 0) {
-        *out = 1.0 / n;
-        *out32 = (float)(1.0 / n);
-    }
+    const double d = policy_inv_denom(mask, rows, denom, red);
+    if (threadIdx.x == 0) *inv = (float)d;
 }
 // the loss, and the derivatives by the rows' log-probabilities divided as it is
-__global__ void __launch_bounds__(JT) policy_join_kernel(const double* row_loss, int64_t rows, const double* inv, float* loss, float* g) {
+__global__ void __launch_bounds__(JT) policy_join_kernel(const uint8_t* mask, float denom, const double* row_loss, int64_t rows, float* loss, float* g) {
     __shared__ double red[JT / 32];
+    const double inv = policy_inv_denom(mask, rows, denom, red);
+    pdl_wait();
     double s = 0.0;
     for (int64_t r = threadIdx.x; r < rows; r += JT) {
         s += row_loss[r];
-        if (g) g[r] = (float)((double)g[r] * *inv);
+        if (g) g[r] = (float)((double)g[r] * inv);
     }
     s = block_sum_jt(s, red);
-    if (threadIdx.x == 0) *loss = (float)(s * *inv);
+    if (threadIdx.x == 0) *loss = (float)(s * inv);
 }
 
 // sums of each answer's log-probabilities, the pairs' mean loss, its derivatives by the sums
@@ -170,6 +742,7 @@ __global__ void __launch_bounds__(JT) preference_join_kernel(const double* logp,
                                                              float smoothing, float* loss, float* logp32, float* g) {
     __shared__ double red[JT / 32];
     double total = 0.0;
+    pdl_wait();
     for (int64_t i = 0; i < pairs; ++i) {
         double side[2];
         for (int w = 0; w < 2; ++w) {
@@ -199,11 +772,71 @@ int with_type(int dtype, F f) {
     return dtype == AB_DT_F16 ? f(__half()) : dtype == AB_DT_BF16 ? f(__nv_bfloat16()) : f(0.f);
 }
 
+// pieces of the longest of the rows
+template <class E>
+int64_t row_pieces(const ab_logit_rows& t) {
+    constexpr int N = 16 / sizeof(E);
+    const bool on_boundaries = reinterpret_cast<uintptr_t>(t.logits) % 16 == 0 && (t.rows <= 1 || t.stride % N == 0);
+    return (t.vocab + (on_boundaries ? 0 : N - 1) + N - 1) / N;
+}
+
+// Blocks per row, and values per thread. Long rows take as few blocks as hold them with 32 values a thread; few rows are spread over more blocks.
+struct RowShape {
+    int cluster, ept;
+};
+RowShape row_shape(int64_t rows, int64_t values, int n_sm) {
+    RowShape s = {1, 8};
+    while (s.cluster < MAX_CLUSTER && (values > (int64_t)s.cluster * LT * 32 || (rows * s.cluster < n_sm && values > (int64_t)s.cluster * LT * 8))) s.cluster *= 2;
+    while (s.ept < 32 && values > (int64_t)s.cluster * LT * s.ept) s.ept *= 2;
+    return s;
+}
+
+// what waits for its predecessor only where it reads its results
+template <class... P, class... A>
+int launch_behind(void (*kernel)(P...), int threads, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...), "join of a loss");
+}
+
 int logit_rows(const RowTask& k, cudaStream_t st) {
     if (!k.t.rows) return OK;
-    return with_type(k.t.dtype, [&](auto e) {
-        logit_rows_kernel<decltype(e)><<<(unsigned)k.t.rows, LT, 0, st>>>(k);
-        return check_cuda(cudaGetLastError(), "rows of logits");
+    return with_type(k.t.dtype, [&](auto e) -> int {
+        using E = decltype(e);
+        constexpr int N = Pieces<E>::N;
+        const int n_sm = current_sm_count();
+        const int64_t values = row_pieces<E>(k.t) * N;
+        if (values > LT * 32 && k.t.rows >= n_sm) {
+            static PerDeviceOnce once;
+            const int st_ = once.run(nullptr, [&](const DeviceProps&) -> int {
+                AB_CUDA(cudaFuncSetAttribute(logit_ring_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_SLOTS * RING_CHUNK));
+                return OK;
+            });
+            if (st_ != OK) return st_;
+            logit_ring_kernel<E><<<(unsigned)k.t.rows, RING_THREADS, RING_SLOTS * RING_CHUNK, st>>>(k);
+            return check_cuda(cudaGetLastError(), "rows of logits");
+        }
+        const RowShape s = row_shape(k.t.rows, values, n_sm);
+        AB_CHECK_ARG(k.t.rows * s.cluster <= INT32_MAX, "too many rows of logits");
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(k.t.rows * s.cluster));
+        cfg.blockDim = dim3(LT);
+        cfg.stream = st;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = s.cluster;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        auto kernel = s.ept == 8 ? logit_rows_kernel<E, 8> : s.ept == 16 ? logit_rows_kernel<E, 16> : logit_rows_kernel<E, 32>;
+        return check_cuda(cudaLaunchKernelEx(&cfg, kernel, k), "rows of logits");
     });
 }
 
@@ -220,18 +853,25 @@ int token_logp_fwd(const ab_logit_rows& t, double* logp, float* logp32, float* s
 
 int token_logp_bwd(const ab_logit_rows& t, const float* stats, const float* g, int64_t rows_per_g, const float* scale, void* dlogits, cudaStream_t st) {
     if (!t.rows) return OK;
-    const DlogitsTask k = {t, stats, g, scale, rows_per_g, dlogits};
-    return with_type(t.dtype, [&](auto e) {
-        dlogits_kernel<decltype(e)><<<(unsigned)t.rows, LT, 0, st>>>(k);
+    return with_type(t.dtype, [&](auto e) -> int {
+        const int64_t pieces = row_pieces<decltype(e)>(t);
+        const int blocks = (int)((pieces + LT * DV - 1) / (LT * DV));
+        AB_CHECK_ARG(t.rows * blocks <= INT32_MAX, "ab_token_logp_bwd: too many rows");
+        const DlogitsTask k = {t, stats, g, scale, rows_per_g, dlogits, blocks};
+        dlogits_kernel<decltype(e)><<<(unsigned)(t.rows * blocks), LT, 0, st>>>(k);
         return check_cuda(cudaGetLastError(), "ab_token_logp_bwd");
     });
 }
 
 int policy_loss(const ab_logit_rows& t, const ab_policy& p, float scale, float* loss, float* logp32, float* stats, float* g, void* dlogits,
                 double* rows_scratch, cudaStream_t st) {
-    double* inv = rows_scratch + t.rows;
-    float* inv32 = reinterpret_cast<float*>(inv + 1);
-    policy_denom_kernel<<<1, JT, 0, st>>>(t.mask, t.rows, p.denom, inv, inv32);
+    // Where the gradient is made in this pass each block needs the denominator: it counts the rows itself up to 16384 of them (64 values a thread, from
+    // L2, beside its row), a launch ahead of it does beyond that.
+    float* inv = nullptr;
+    if (dlogits && (p.denom != 0.f || t.rows > 16384)) {
+        inv = reinterpret_cast<float*>(rows_scratch + t.rows);
+        policy_denom_kernel<<<1, JT, 0, st>>>(t.mask, t.rows, p.denom, inv);
+    }
     RowTask k = {};
     k.t = t;
     k.policy = 1;
@@ -241,20 +881,18 @@ int policy_loss(const ab_logit_rows& t, const ab_policy& p, float scale, float* 
     k.stats = stats;
     k.g = g;
     k.dlogits = dlogits;
-    k.inv_denom = inv32;
+    k.inv_denom = inv;
     k.scale = scale;
     const int s = logit_rows(k, st);
     if (s != OK) return s;
-    policy_join_kernel<<<1, JT, 0, st>>>(rows_scratch, t.rows, inv, loss, g);
-    return check_cuda(cudaGetLastError(), "policy loss");
+    return launch_behind(policy_join_kernel, JT, st, t.mask, p.denom, rows_scratch, t.rows, loss, g);
 }
 
 int preference_loss(const ab_logit_rows& t, int64_t pairs, int64_t steps, const float* ref, float beta, float smoothing, float* loss, float* logp32,
                     float* stats, float* g, double* rows_scratch, cudaStream_t st) {
     const int s = token_logp_fwd(t, rows_scratch, nullptr, stats, st);
     if (s != OK) return s;
-    preference_join_kernel<<<1, JT, 0, st>>>(rows_scratch, pairs, steps, ref, beta, smoothing, loss, logp32, g);
-    return check_cuda(cudaGetLastError(), "ab_preference_loss_fwd");
+    return launch_behind(preference_join_kernel, JT, st, rows_scratch, pairs, steps, ref, beta, smoothing, loss, logp32, g);
 }
 
 }  // namespace ab

@@ -115,14 +115,14 @@ int with_types(int dtype, int wtype, F f) {
 size_t layer_norm_scratch_bytes(int64_t rows, int C) { return (size_t)((rows + COL_ROWS - 1) / COL_ROWS) * 2 * C * sizeof(float); }
 
 int layer_norm_fwd(const NormArgs& a, cudaStream_t st) {
-    return with_types(a.dtype, a.wtype, [&](auto e, auto w) {
+    return with_types(a.dtype, a.wtype, [&](auto e, auto w) -> int {
         norm_fwd_kernel<decltype(e), decltype(w)><<<(unsigned)(a.rows * a.groups), NT, 0, st>>>(a);
         return check_cuda(cudaGetLastError(), "ab_layer_norm_fwd");
     });
 }
 
 int layer_norm_bwd(const NormArgs& a, cudaStream_t st) {
-    return with_types(a.dtype, a.wtype, [&](auto e, auto w) {
+    return with_types(a.dtype, a.wtype, [&](auto e, auto w) -> int {
         using E = decltype(e);
         using W = decltype(w);
         if (a.dx && a.rows) norm_dx_kernel<E, W><<<(unsigned)(a.rows * a.groups), NT, 0, st>>>(a);

@@ -93,41 +93,6 @@ struct Pieces {
         return make_uint4(w, w, w, w);
     }
 };
-template <class E> __device__ __forceinline__ void unpack(const uint4& u, float* f);
-template <> __device__ __forceinline__ void unpack<float>(const uint4& u, float* f) {
-    f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
-}
-template <> __device__ __forceinline__ void unpack<__half>(const uint4& u, float* f) {
-    const __half2* h = reinterpret_cast<const __half2*>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 v = __half22float2(h[i]);
-        f[2 * i] = v.x, f[2 * i + 1] = v.y;
-    }
-}
-template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& u, float* f) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-}
-template <class E> __device__ __forceinline__ uint4 pack(const float* f);
-template <> __device__ __forceinline__ uint4 pack<float>(const float* f) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-}
-template <> __device__ __forceinline__ uint4 pack<__half>(const float* f) {
-    uint4 u;
-    __half2* h = reinterpret_cast<__half2*>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    return u;
-}
-template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float* f) {
-    uint4 u;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    return u;
-}
 // the larger values of two pieces, place by place (a NaN gives way: it is left to the sums), and the largest of one
 template <class E>
 __device__ __forceinline__ uint4 piece_max(uint4 a, const uint4& b) {

@@ -165,9 +165,9 @@ __global__ void __launch_bounds__(NT) norm_rows_fwd_kernel(const __grid_constant
     __shared__ float red[2][NT / 32];
     const int tid = threadIdx.x, lane = BLOCK ? tid : tid & 31, pieces = a.C / N;
     const int parts = seg ? (pieces + 32 * NV - 1) / (32 * NV) : 1;   // of a row
-    const int64_t unit = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * (NT / 32) + (tid >> 5);
-    const int64_t row = unit / parts;
-    const int p0 = (int)(unit - row * parts) * 32 * NV + lane;
+    const unsigned unit = BLOCK ? blockIdx.x : blockIdx.x * (NT / 32) + (tid >> 5);   // (below 2^32: see fwd_rows)
+    const int64_t row = seg ? unit / (unsigned)parts : unit;
+    const int p0 = (int)(unit - (unsigned)row * (unsigned)parts) * 32 * NV * (seg ? 1 : 0) + lane;
     if (row >= a.rows) return;
     const E* x = static_cast<const E*>(a.x) + row * a.x_stride;
     const int m = a.C / a.groups;
@@ -246,7 +246,7 @@ struct NormBwd {
     NormArgs a;
     int tpr, seg, slots, row_bytes;   // threads per row, lanes per group (0: the row is one), rows in the ring
 };
-template <class E, class W, int NV>
+template <class E, class W, int NV, bool SEG>
 __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(const __grid_constant__ NormBwd k) {
     constexpr int N = per_piece<E>, MAX_SLOTS = 64;
     extern __shared__ __align__(128) unsigned char ring[];
@@ -273,7 +273,12 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
         atomicOr(&g_device_status, DEV_WAIT_HEAD);
         return false;
     };
-    const int64_t mine = a.rows > blockIdx.x ? (a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;   // rows blockIdx.x, + gridDim.x, ...
+    const int mine = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);   // rows blockIdx.x, + gridDim.x, ... (no more blocks than rows)
+    // a slot of the ring and the phase of its barriers, `by` rows further on
+    auto advance = [&](int& slot, uint32_t& phase, int by) {
+        slot += by;
+        if (slot >= k.slots) slot -= k.slots, phase ^= 1u;
+    };
     float dw[NV][N], db[NV][N];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -281,18 +286,18 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
         for (int c = 0; c < N; ++c) dw[j][c] = db[j][c] = 0.f;
     if (warp == BWD_THREADS / 32) {
         if (lane == 0) {
-            int64_t n = 0;
-            for (; n < mine; ++n) {
-                const int slot = (int)(n % k.slots);
-                if (n >= k.slots && !wait_for(&vacant[slot], (uint32_t)(n / k.slots - 1) & 1u)) break;
-                const int64_t r = blockIdx.x + n * gridDim.x;
+            int n = 0, slot = 0;
+            uint32_t phase = 0;
+            for (; n < mine; ++n, advance(slot, phase, 1)) {
+                if (n >= k.slots && !wait_for(&vacant[slot], phase ^ 1u)) break;
+                const int64_t r = blockIdx.x + (int64_t)n * gridDim.x;
                 unsigned char* to = ring + (size_t)slot * 2 * k.row_bytes;
                 mbar_expect_tx(&full[slot], 2 * k.row_bytes);
                 bulk_g2s(to, static_cast<const E*>(a.x) + r * a.x_stride, k.row_bytes, &full[slot]);
                 bulk_g2s(to + k.row_bytes, static_cast<const E*>(a.dy) + r * a.dy_stride, k.row_bytes, &full[slot]);
             }
             // whatever became of the waits, all that was asked for lands before the ring is used otherwise, or the block ends
-            for (int64_t c = max((int64_t)0, n - k.slots); c < n; ++c) mbar_wait_bounded(&full[c % k.slots], (uint32_t)(c / k.slots) & 1u, 1u << 18);
+            for (int c = max(0, n - k.slots); c < n; ++c) mbar_wait_bounded(&full[c % k.slots], (uint32_t)(c / k.slots) & 1u, 1u << 18);
         }
     } else {
         const int team = warp / wpt, t = tid - team * tpr;
@@ -301,22 +306,26 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (t + j * tpr < pieces) w[j].load(static_cast<const W*>(a.w), (t + j * tpr) * N);
-        float mean[NV], rstd[NV], mean1[NV], rstd1[NV];   // of a row, and of the team's next one
-        auto stats = [&](int64_t n) {
+        constexpr int NS = SEG ? NV : 1;                  // groups that a thread's pieces belong to
+        int group[NS];
+        float mean[NS], rstd[NS], mean1[NS], rstd1[NS];   // of a row, and of the team's next one
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t at = (blockIdx.x + n * gridDim.x) * a.groups + (k.seg ? min(t + j * tpr, pieces - 1) / k.seg : 0);
-                if (n < mine) mean1[j] = __ldg(a.mean + at), rstd1[j] = __ldg(a.rstd + at);
-            }
+        for (int j = 0; j < NS; ++j) group[j] = SEG ? min(t + j * tpr, pieces - 1) / k.seg : 0;
+        auto stats = [&](int n) {
+            if (n >= mine) return;
+            const int64_t at = (blockIdx.x + (int64_t)n * gridDim.x) * a.groups;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) mean1[j] = __ldg(a.mean + at + group[j]), rstd1[j] = __ldg(a.rstd + at + group[j]);
         };
         stats(team);
-        for (int64_t n = team; n < mine; n += teams) {
-            const int slot = (int)(n % k.slots);
-            const int64_t r = blockIdx.x + n * gridDim.x;
+        int slot = team, turn = 0;
+        uint32_t phase = 0;
+        for (int n = team; n < mine; n += teams, advance(slot, phase, teams), turn ^= 1) {
+            const int64_t r = blockIdx.x + (int64_t)n * gridDim.x;
 #pragma unroll
-            for (int j = 0; j < NV; ++j) mean[j] = mean1[j], rstd[j] = rstd1[j];
+            for (int j = 0; j < NS; ++j) mean[j] = mean1[j], rstd[j] = rstd1[j];
             stats(n + teams);
-            wait_for(&full[slot], (uint32_t)(n / k.slots) & 1u);
+            wait_for(&full[slot], phase);
             __syncwarp();
             const uint4* from = reinterpret_cast<const uint4*>(ring + (size_t)slot * 2 * k.row_bytes);
             uint4 ux[NV], ud[NV];
@@ -334,37 +343,37 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
             loads_returned(used, &nobody);
             __syncwarp();
             if (lane == 0) mbar_arrive(&vacant[slot]);
-            float s = 0.f, q = 0.f, sj[NV], qj[NV];
+            float s = 0.f, q = 0.f, sj[NS], qj[NS];
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                float fx[N], fd[N], fw[N];
+                const int g = SEG ? j : 0;
+                float fx[N], fd[N], fw[N], sp = 0.f, qp = 0.f;
                 unpack<E>(ux[j], fx);
                 unpack<E>(ud[j], fd);
                 w[j].get(fw);
-                sj[j] = qj[j] = 0.f;
                 if (t + j * tpr < pieces) {
 #pragma unroll
                     for (int c = 0; c < N; ++c) {
-                        const float xh = (fx[c] - mean[j]) * rstd[j], e = fd[c] * fw[c];
+                        const float xh = (fx[c] - mean[g]) * rstd[g], e = fd[c] * fw[c];
                         dw[j][c] = fmaf(fd[c], xh, dw[j][c]);
                         db[j][c] += fd[c];
-                        sj[j] += e;
-                        qj[j] = fmaf(e, xh, qj[j]);
+                        sp += e;
+                        qp = fmaf(e, xh, qp);
                     }
                 }
-                if (k.seg) {
-                    sj[j] = lanes_sum(sj[j], k.seg) * inv_m;
-                    qj[j] = lanes_sum(qj[j], k.seg) * inv_m;
+                if (SEG) {
+                    sj[g] = lanes_sum(sp, k.seg) * inv_m;
+                    qj[g] = lanes_sum(qp, k.seg) * inv_m;
                 } else {
-                    s += sj[j];
-                    q += qj[j];
+                    s += sp;
+                    q += qp;
                 }
             }
-            if (!k.seg) {
+            if (!SEG) {
                 s = warp_sum(s);
                 q = warp_sum(q);
                 if (wpt > 1) {
-                    float2* to = red[(n / teams) & 1];   // (written again two rows on, behind the next row's barrier)
+                    float2* to = red[turn];   // (written again two rows on, behind the next row's barrier)
                     if (lane == 0) to[warp] = make_float2(s, q);
                     asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(tpr) : "memory");
                     s = q = 0.f;
@@ -374,8 +383,7 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
                         q += v.y;
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < NV; ++j) sj[j] = s * inv_m, qj[j] = q * inv_m;
+                sj[0] = s * inv_m, qj[0] = q * inv_m;
             }
             if (a.dx) {
                 uint4* dx = reinterpret_cast<uint4*>(static_cast<E*>(a.dx) + r * a.C);
@@ -383,14 +391,15 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
                 for (int j = 0; j < NV; ++j) {
                     const int p = t + j * tpr;
                     if (p >= pieces) continue;
+                    const int g = SEG ? j : 0;
                     float fx[N], fd[N], fw[N];
                     unpack<E>(ux[j], fx);
                     unpack<E>(ud[j], fd);
                     w[j].get(fw);
 #pragma unroll
                     for (int c = 0; c < N; ++c) {
-                        const float xh = (fx[c] - mean[j]) * rstd[j];
-                        fx[c] = rstd[j] * fmaf(-xh, qj[j], fmaf(fd[c], fw[c], -sj[j]));
+                        const float xh = (fx[c] - mean[g]) * rstd[g];
+                        fx[c] = rstd[g] * fmaf(-xh, qj[g], fmaf(fd[c], fw[c], -sj[g]));
                     }
                     if (AB_BC((p + 1) * N <= a.C)) __stcs(dx + p, pack<E>(fx));
                 }
@@ -459,7 +468,10 @@ int fwd_rows(const NormArgs& a, const NormShape& s, cudaStream_t st, bool* done)
     if (s.seg || pieces <= 32 * 8) {   // a warp per row, or per 64 pieces of groups
         const int nv = s.seg ? (pieces <= 32 ? 1 : 2) : pieces <= 32 ? 1 : pieces <= 64 ? 2 : pieces <= 128 ? 4 : 8;
         const int64_t units = a.rows * (s.seg ? (pieces + 32 * nv - 1) / (32 * nv) : 1), blocks = (units + NT / 32 - 1) / (NT / 32);
-        AB_CHECK_ARG(blocks <= INT32_MAX, "ab_layer_norm_fwd: too many rows");
+        if (units > UINT32_MAX - NT) {
+            *done = false;
+            return OK;
+        }
         auto k = nv == 1 ? norm_rows_fwd_kernel<E, W, 1, false> : nv == 2 ? norm_rows_fwd_kernel<E, W, 2, false> : nv == 4 ? norm_rows_fwd_kernel<E, W, 4, false> : norm_rows_fwd_kernel<E, W, 8, false>;
         k<<<(unsigned)blocks, NT, 0, st>>>(a, s.seg);
     } else if (pieces <= NT * 4 && a.rows <= INT32_MAX) {
@@ -489,11 +501,12 @@ template <class E, class W>
 int bwd_rows(const NormArgs& a, const NormShape& s, cudaStream_t st) {
     NormBwd k = {a, s.tpr, s.seg, 0, a.C * (int)sizeof(E)};
     k.slots = std::min(64, BWD_RING / (2 * k.row_bytes));
-    auto kernel = s.nv == 1 ? norm_rows_bwd_kernel<E, W, 1> : norm_rows_bwd_kernel<E, W, 2>;
+    auto kernel = s.seg ? (s.nv == 1 ? norm_rows_bwd_kernel<E, W, 1, true> : norm_rows_bwd_kernel<E, W, 2, true>)
+                        : (s.nv == 1 ? norm_rows_bwd_kernel<E, W, 1, false> : norm_rows_bwd_kernel<E, W, 2, false>);
     static PerDeviceOnce once;
     const DeviceProps* props = nullptr;
     const int st_ = once.run(&props, [&](const DeviceProps&) -> int {
-        for (auto f : {norm_rows_bwd_kernel<E, W, 1>, norm_rows_bwd_kernel<E, W, 2>})
+        for (auto f : {norm_rows_bwd_kernel<E, W, 1, true>, norm_rows_bwd_kernel<E, W, 2, true>, norm_rows_bwd_kernel<E, W, 1, false>, norm_rows_bwd_kernel<E, W, 2, false>})
             AB_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_RING));
         return OK;
     });
@@ -534,7 +547,7 @@ int layer_norm_bwd(const NormArgs& a, cudaStream_t st) {
     return with_types(a.dtype, a.wtype, [&](auto e, auto w) -> int {
         using E = decltype(e);
         using W = decltype(w);
-        if (a.rows && norm_shape<E>(a).nv && current_sm_count() <= 256) return bwd_rows<E, W>(a, norm_shape<E>(a), st);
+        if (a.rows && a.rows <= INT32_MAX && norm_shape<E>(a).nv && current_sm_count() <= 256) return bwd_rows<E, W>(a, norm_shape<E>(a), st);
         if (a.dx && a.rows) norm_dx_kernel<E, W><<<(unsigned)std::min<int64_t>(a.rows * a.groups, 1 << 20), NT, 0, st>>>(a);
         if (a.dw || a.db) {
             const int parts = (int)col_parts(a.rows);

@@ -5,6 +5,8 @@
 //   G_t = (G_{t+1} diag(d_{t+1}) + h_{t+1} a_{t+1}^T) + dy_t r_t^T
 //   dr_t = S_t^T dy_t,  dv_t = G_t k_t,  dk_t = G_t^T v_t,  db_t = G_t^T u_t,  da_t = S_{t-1}^T h_t,
 //   dd_t[j] = sum_i G_t[i, j] S_{t-1}[i, j],  dw_t = dd_t d_t log d_t.
+#include <type_traits>
+
 #include "wkv_chunk.cuh"
 
 namespace ab {
@@ -30,35 +32,8 @@ struct WkvBwd {
     WkvBackward g;
 };
 
-constexpr int WT = 256;   // a thread has 16 columns (a quarter) of one row
-
 __device__ __forceinline__ int seq_length(const WkvSeq& s, int b) {
     return s.lengths ? min(max(s.lengths[b], 0), s.T) : s.T;
-}
-
-// One step's six vectors of a head in shared memory, as 32-bit floats; the decay in place of w.
-template <class E>
-__device__ __forceinline__ void load_step(const WkvSeq& s, int b, int h, int t, float (*vec)[64]) {
-    for (int i = threadIdx.x; i < 6 * 64; i += WT) {
-        const int n = i >> 6, j = i & 63;
-        const float v = to_f(static_cast<const E*>(s.x[n])[b * s.bs[n] + t * s.ss[n] + h * 64 + j]);
-        vec[n][j] = n == 1 ? expf(-expf(v)) : v;
-    }
-}
-__device__ __forceinline__ float quad_sum(float v) {
-    v += __shfl_xor_sync(0xffffffffu, v, 1);
-    return v + __shfl_xor_sync(0xffffffffu, v, 2);
-}
-// S_{t-1} -> S_t for this thread's 16 columns; returns u
-__device__ __forceinline__ float step_state(float* S, const float (*vec)[64], int row, int c0) {
-    float u = 0.f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) u = fmaf(S[j], vec[4][c0 + j], u);
-    u = quad_sum(u);
-    const float v = vec[3][row];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) S[j] = fmaf(v, vec[2][c0 + j], fmaf(u, vec[5][c0 + j], S[j] * vec[1][c0 + j]));
-    return u;
 }
 
 // ---- the forward pass ----------------------------------------------------------------------------------------------------
@@ -66,17 +41,20 @@ __device__ __forceinline__ float step_state(float* S, const float (*vec)[64], in
 // without leaving the warp), four others prepare chunks ahead, each a whole one by itself, in a ring of four buffers.
 using namespace wkvc;
 constexpr int CHUNK_BUFS = 4, CHUNK_THREADS = (CHUNK_BUFS + 4) * 32;
-constexpr int FWD_V = FWD_TILES * 2 * TILE, FWD_HEAD = FWD_V + TILE, FWD_BUF = FWD_HEAD + (int)((sizeof(ChunkHead) + 127) / 128 * 128);
+constexpr int HEAD_BYTES = (int)((sizeof(ChunkHead) + 127) / 128 * 128);
+constexpr int FWD_V = FWD_TILES * 2 * TILE, FWD_HEAD = FWD_V + TILE, FWD_BUF = FWD_HEAD + HEAD_BYTES;
 
 // one vector of a chunk's steps: a lane has columns 2 lane, 2 lane + 1
 template <class E>
 struct Vec {
     uint32_t raw[L];
-    __device__ __forceinline__ void load(const WkvSeq& s, int which, int64_t b, int h, int t0, int n_on, int lane) {
-        const E* p = static_cast<const E*>(s.x[which]) + b * s.bs[which] + (int64_t)t0 * s.ss[which] + h * N + 2 * lane;
-        const bool even = s.even >> which & 1;
+    __device__ __forceinline__ void load(const void* x, int64_t at, int64_t stride, bool even, int lo, int hi, int lane) {
+        const E* p = static_cast<const E*>(x) + at + 2 * lane;
 #pragma unroll
-        for (int t = 0; t < L; ++t) raw[t] = t < n_on ? load_raw(p + t * s.ss[which], even) : 0u;
+        for (int t = 0; t < L; ++t) raw[t] = t >= lo && t < hi ? load_raw(p + t * stride, even) : 0u;
+    }
+    __device__ __forceinline__ void load(const WkvSeq& s, int which, int64_t b, int h, int t0, int lo, int hi, int lane) {
+        load(s.x[which], b * s.bs[which] + (int64_t)t0 * s.ss[which] + h * N, s.ss[which], s.even >> which & 1, lo, hi, lane);
     }
     __device__ __forceinline__ float top() const {
         uint32_t m = 0;   // the order of non-negative floats is that of their bits
@@ -107,7 +85,7 @@ __device__ __forceinline__ float log2_decay(float w) {   // of exp(-exp(w)); fin
 template <class E>
 __device__ __forceinline__ bool load_decays(const WkvSeq& s, int64_t b, int h, int t0, int n_on, int lane, float2* lw) {
     Vec<E> w;
-    w.load(s, 1, b, h, t0, n_on, lane);
+    w.load(s, 1, b, h, t0, 0, n_on, lane);
     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int t = 0; t < L; ++t) {
@@ -176,7 +154,7 @@ __device__ __forceinline__ void load_frag(Frag& f, uint32_t tile, int c0, int la
     how(f.lo, tile + TILE, c0, lane);
 }
 // Q = (1 - A)^-1 for the strictly lower A in `work` (16 x 16), by columns: x_t = [t = c] + sum_{s < t} A[t, s] x_s. Left in `work`; as an A operand.
-__device__ __forceinline__ float invert(float* work, Frag& f, int lane) {
+__device__ __forceinline__ float invert(float* work, Frag& f, float (*v)[4], int lane) {
     float x[L];
     const int c = lane & 15;
 #pragma unroll
@@ -201,7 +179,6 @@ __device__ __forceinline__ float invert(float* work, Frag& f, int lane) {
         for (int t = 0; t < L; ++t) work[t * L + c] = x[t];
     __syncwarp();
     const int g = lane >> 2, q = lane & 3;
-    float v[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -214,36 +191,46 @@ __device__ __forceinline__ float invert(float* work, Frag& f, int lane) {
     return sc.down;
 }
 
-// Prepares steps lo .. hi - 1 of a chunk (of n_on that the sequence has in it); lw: log2 decays, zero at the other steps.
+// a vector's values as they are, in one fp16 each, scaled to the tile's largest (exact down to 2^-27 of it)
 template <class E>
-__device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h, int t0, int lo, int hi, const float2* lw, uint32_t buf, ChunkHead* head, int lane) {
-    const uint32_t tA = buf + T_A * 2 * TILE, tR = buf + T_R * 2 * TILE, tB = buf + T_B * 2 * TILE, tK = buf + T_K * 2 * TILE, tM = buf + T_M * 2 * TILE, tV = buf + FWD_V;
-    float2 end = make_float2(0.f, 0.f);
+__device__ __forceinline__ float put_exact(const Vec<E>& v, uint32_t tile, int lane) {
+    const Scale sc = scale_for(v.top());
 #pragma unroll
-    for (int t = 0; t < L; ++t) end.x += lw[t].x, end.y += lw[t].y;
-    auto load = [&](Vec<E>& v, int which) {
-        v.load(s, which, b, h, t0, hi, lane);
-        if (lo)
-#pragma unroll
-            for (int t = 0; t < L; ++t) v.raw[t] = t < lo ? 0u : v.raw[t];
-    };
-    Vec<E> x;
+    for (int t = 0; t < L; ++t) {
+        const float2 f = raw_pair<E>(v.raw[t]);
+        st32(tile + tile_pair(t, lane), pack_half(f.x * sc.up, f.y * sc.up));
+    }
+    return sc.down;
+}
+
+// Prepares steps lo .. hi - 1 of a chunk; lw: log2 decays, zero at the other steps. at: the buffer's tiles; v: where v goes; ap: the tile for a'. BWD: Q is kept too.
+template <class E, bool BWD>
+__device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h, int t0, int lo, int hi, bool piece, const float2* lw, uint32_t at, uint32_t v, ChunkHead* head,
+                                              int lane) {
+    constexpr int AP = BWD ? T_AP : T_A;
+    const uint32_t tA = at + T_A * 2 * TILE, tR = at + T_R * 2 * TILE, tB = at + T_B * 2 * TILE, tK = at + T_K * 2 * TILE, tM = at + T_M * 2 * TILE, tAP = at + AP * 2 * TILE;
     float down_b, down_k, down_a, down_r;
-    auto to_end = [&](float, float c, int i) { return (i ? end.y : end.x) - c; };                          // of steps 0 .. hi - 1: at most 0
-    load(x, 5);
-    down_b = put_tile(x, lw, tB, lane, 1.f, to_end);
-    load(x, 2);
-    down_k = put_tile(x, lw, tK, lane, 1.f, to_end);
-    load(x, 3);
+    {
+        float2 end = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int t = 0; t < L; ++t) st32(tV + tile_pair(t, lane), x.raw[t]);
-    // relative to the end a's and r's factors are at most `grow` (2^STEEP_LOG2); in a piece of one step r's is 1, and a's, which meet nothing, are left as they are
-    const bool piece = hi - lo == 1;
-    const float grow = piece ? 1.f : ex2_(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(-fminf(end.x, end.y), 0.f)))));
-    load(x, 4);
-    down_a = put_tile(x, lw, tA, lane, grow, [&](float c, float, int i) { return piece ? 0.f : c - (i ? end.y : end.x); });
-    load(x, 0);
-    down_r = put_tile(x, lw, tR, lane, grow, [&](float, float c, int i) { return piece ? 0.f : c - (i ? end.y : end.x); });
+        for (int t = 0; t < L; ++t) end.x += lw[t].x, end.y += lw[t].y;
+        Vec<E> x;
+        auto to_end = [&](float, float c, int i) { return (i ? end.y : end.x) - c; };   // at most 0
+        x.load(s, 5, b, h, t0, lo, hi, lane);
+        down_b = put_tile(x, lw, tB, lane, 1.f, to_end);
+        x.load(s, 2, b, h, t0, lo, hi, lane);
+        down_k = put_tile(x, lw, tK, lane, 1.f, to_end);
+        // a's and r's factors are at most `grow` (2^STEEP_LOG2); in a piece of one step they are 1
+        const float grow = piece ? 1.f : ex2_(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(-fminf(end.x, end.y), 0.f)))));
+        x.load(s, 4, b, h, t0, lo, hi, lane);
+        down_a = put_tile(x, lw, tA, lane, grow, [&](float c, float, int i) { return piece ? 0.f : c - (i ? end.y : end.x); });
+        x.load(s, 0, b, h, t0, lo, hi, lane);
+        down_r = put_tile(x, lw, tR, lane, grow, [&](float, float c, int i) { return piece ? 0.f : c - (i ? end.y : end.x); });
+        x.load(s, 3, b, h, t0, lo, hi, lane);
+        const float down_v = put_exact(x, v, lane);
+        *reinterpret_cast<float2*>(head->decay + 2 * lane) = make_float2(ex2_(end.x), ex2_(end.y));
+        if (lane == 0) head->down_v = down_v;
+    }
     __syncwarp();
     {
         float ab[2][4], ak[2][4], rb[2][4], rk[2][4];
@@ -273,24 +260,24 @@ __device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h,
         if (lane == 0) head->down_m[M_X] = dx, head->down_m[M_RB] = d1, head->down_m[M_RK] = d2;
     }
     __syncwarp();
-    // (the tiles relative to the end have been read)
-    load(x, 4);
-    down_a = put_tile(x, lw, tA, lane, 1.f, [](float c, float, int) { return c; });
-    load(x, 0);
-    down_r = put_tile(x, lw, tR, lane, 1.f, [](float, float c, int) { return c; });
     Frag q;
-    const float down_q = invert(head->work, q, lane);
+    float qv[2][4];
+    const float down_q = invert(head->work, q, qv, lane);
+    if (BWD) {
+        put_acc(qv, at + T_Q * 2 * TILE, 0, 1.f / down_q, lane);
+        if (lane == 0) head->down[T_Q] = down_q;
+    }
     float ap[4][2][4], akp[2][4], top = 0.f;
     zero2(akp);
     {
         Frag f;
         load_frag(f, tM, M_X * L, lane, load_bt);
         mma3(akp, q, f);
-        const float d = down_q, e = head->down_m[M_X];
+        const float e = head->down_m[M_X];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) akp[n][i] *= d * e;
+            for (int i = 0; i < 4; ++i) akp[n][i] *= down_q * e;
     }
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
@@ -303,11 +290,11 @@ __device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h,
     const Scale sa = scale_for(warp_top_abs(top));
     __syncwarp();
 #pragma unroll
-    for (int jj = 0; jj < 4; ++jj) put_acc(ap[jj], tA, jj * 16, sa.up, lane);
+    for (int jj = 0; jj < 4; ++jj) put_acc(ap[jj], tAP, jj * 16, sa.up, lane);
     const float dak = put_block(akp, tM, M_AK * L, lane);
-    *reinterpret_cast<float2*>(head->decay + 2 * lane) = make_float2(ex2_(end.x), ex2_(end.y));
     if (lane == 0) {
-        head->down[T_A] = sa.down * down_a * down_q;
+        if (BWD) head->down[T_A] = down_a;
+        head->down[AP] = sa.down * down_a * down_q;
         head->down[T_R] = down_r;
         head->down[T_B] = down_b;
         head->down[T_K] = down_k;
@@ -315,85 +302,110 @@ __device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h,
     }
 }
 
-// One chunk for 16 rows of the state: S (accumulators of eight n-tiles) becomes the state after it, y the outputs (rows as m, steps as n).
-template <class E>
-__device__ __forceinline__ void chunk_rows(float (*S)[4], float (*y)[4], uint32_t buf, const ChunkHead* head, int i0, int lane) {
-    const uint32_t tA = buf + T_A * 2 * TILE, tR = buf + T_R * 2 * TILE, tB = buf + T_B * 2 * TILE, tK = buf + T_K * 2 * TILE, tM = buf + T_M * 2 * TILE;
+__device__ __forceinline__ void decay_rows(float (*S)[4], const ChunkHead* head, int lane) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        const float2 d = *reinterpret_cast<const float2*>(head->decay + 8 * n + 2 * (lane & 3));
+        S[n][0] *= d.x, S[n][1] *= d.y, S[n][2] *= d.x, S[n][3] *= d.y;
+    }
+}
+__device__ __forceinline__ void row_scales(const float (*S)[4], Scale& s0, Scale& s1) {   // of rows g and g + 8
     float top0 = 0.f, top1 = 0.f;
 #pragma unroll
     for (int n = 0; n < 8; n += 2) top0 = fmaxf(top0, row_top(S + n, 0)), top1 = fmaxf(top1, row_top(S + n, 1));
-    const Scale s0 = scale_for(quad_top_abs(top0)), s1 = scale_for(quad_top_abs(top1));
-    float u[2][4], ys[2][4];
-    zero2(u), zero2(ys);
+    s0 = scale_for(quad_top_abs(top0)), s1 = scale_for(quad_top_abs(top1));
+}
+// c = c * (row's down) * d
+__device__ __forceinline__ void scale_acc(float (*c)[4], const Scale& s0, const Scale& s1, float d) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[n][i] = c[n][i] * (i < 2 ? s0.down : s1.down) * d;
+}
+__device__ __forceinline__ void add_acc(float (*c)[4], const float (*x)[4], float d) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[n][i] = fmaf(x[n][i], d, c[n][i]);
+}
+__device__ __forceinline__ void add_acc(float (*c)[4], const float (*x)[4], const Scale& s0, const Scale& s1, float d) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[n][i] = fmaf(x[n][i] * (i < 2 ? s0.down : s1.down), d, c[n][i]);
+}
+// c (16 rows x 16 steps) = S times a tile's rows
+__device__ __forceinline__ void state_times(float (*c)[4], const float (*S)[4], const Scale& s0, const Scale& s1, uint32_t tile, int lane) {
+    zero2(c);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
         Frag f, g;
         as_a(f, S + 2 * kk, s0.up, s1.up);
-        load_frag(g, tA, kk * 16, lane, load_b);
-        mma3(u, f, g);
-        load_frag(g, tR, kk * 16, lane, load_b);
-        mma3(ys, f, g);
+        load_frag(g, tile, kk * 16, lane, load_b);
+        mma3(c, f, g);
     }
-    float v[2][4], acc[2][4];
-    load_vt<E>(v, buf + FWD_V, i0, lane);
-    const float tv0 = quad_top_abs(row_top(v, 0)), tv1 = quad_top_abs(row_top(v, 1));
-    const Scale v0 = scale_for(tv0), v1 = scale_for(tv1);
+}
+
+// One chunk for 16 rows of the state: S (accumulators of eight n-tiles) becomes the state after it, y the outputs (rows as m, steps as n).
+__device__ __forceinline__ void chunk_rows(float (*S)[4], float (*y)[4], uint32_t at, uint32_t v, int ap, const ChunkHead* head, int i0, int lane) {
+    const uint32_t tA = at + ap * 2 * TILE, tR = at + T_R * 2 * TILE, tB = at + T_B * 2 * TILE, tK = at + T_K * 2 * TILE, tM = at + T_M * 2 * TILE;
+    const int piece = head->piece;
+    float u[2][4];
+    Scale s0, s1;
+    if (piece) {
+        row_scales(S, s0, s1);
+        state_times(u, S, s0, s1, tA, lane);
+        scale_acc(u, s0, s1, head->down[ap]);
+    }
+    decay_rows(S, head, lane);
+    row_scales(S, s0, s1);
+    if (!piece) {
+        zero2(u), zero2(y);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            Frag f, g;
+            as_a(f, S + 2 * kk, s0.up, s1.up);
+            load_frag(g, tA, kk * 16, lane, load_b);
+            mma3(u, f, g);
+            load_frag(g, tR, kk * 16, lane, load_b);
+            mma3(y, f, g);
+        }
+        scale_acc(u, s0, s1, head->down[ap]);
+    } else {
+        state_times(y, S, s0, s1, tR, lane);
+    }
+    scale_acc(y, s0, s1, head->down[T_R]);
     uint32_t fv[4];
-    as_a_exact(fv, v, v0.up, v1.up);
-    zero2(acc);
-    {
-        Frag g;
-        load_frag(g, tM, M_AK * L, lane, load_b);
-        mma2(acc, fv, g);
-    }
-    {
-        const float da = head->down[T_A], dr = head->down[T_R], dk = head->down_m[M_AK];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float ds = i < 2 ? s0.down : s1.down, dv = i < 2 ? v0.down : v1.down;
-                u[n][i] = fmaf(acc[n][i] * dv, dk, u[n][i] * ds * da);
-                ys[n][i] = ys[n][i] * ds * dr;
-            }
-    }
-    const float tu0 = quad_top_abs(row_top(u, 0)), tu1 = quad_top_abs(row_top(u, 1));
-    // u and v with one scale per row for a product with b's and k's side, whose own scales (powers of two) go to u's and v's
-    auto pair = [&](Frag& fu, uint32_t* fv_, float db, float dk, Scale& r0, Scale& r1) {
-        r0 = scale_for(fmaxf(tu0 * db, tv0 * dk)), r1 = scale_for(fmaxf(tu1 * db, tv1 * dk));
-        as_a(fu, u, db * r0.up, db * r1.up);
-        as_a_exact(fv_, v, dk * r0.up, dk * r1.up);
-    };
+    load_at(fv, v, i0, lane);
+    const float dv = head->down_v;
+    float x[2][4];
+    Frag g;
+    zero2(x);
+    load_frag(g, tM, M_AK * L, lane, load_b);
+    mma2(x, fv, g);
+    add_acc(u, x, dv * head->down_m[M_AK]);
+    s0 = scale_for(quad_top_abs(row_top(u, 0))), s1 = scale_for(quad_top_abs(row_top(u, 1)));
     Frag fu;
-    Scale r0, r1;
-    pair(fu, fv, head->down_m[M_RB], head->down_m[M_RK], r0, r1);
-    zero2(acc);
-    {
-        Frag g;
-        load_frag(g, tM, M_RB * L, lane, load_b);
-        mma3(acc, fu, g);
-        load_frag(g, tM, M_RK * L, lane, load_b);
-        mma2(acc, fv, g);
-    }
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[n][i] = fmaf(acc[n][i], i < 2 ? r0.down : r1.down, ys[n][i]);
-    pair(fu, fv, head->down[T_B], head->down[T_K], r0, r1);
+    as_a(fu, u, s0.up, s1.up);
+    zero2(x);
+    load_frag(g, tM, M_RB * L, lane, load_b);
+    mma3(x, fu, g);
+    add_acc(y, x, s0, s1, head->down_m[M_RB]);
+    zero2(x);
+    load_frag(g, tM, M_RK * L, lane, load_b);
+    mma2(x, fv, g);
+    add_acc(y, x, dv * head->down_m[M_RK]);
+    const float db = head->down[T_B], dk = dv * head->down[T_K];
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
-        Frag g;
-        zero2(acc);
+        float z[2][4];
+        zero2(x), zero2(z);
         load_frag(g, tB, jj * 16, lane, load_bt);
-        mma3(acc, fu, g);
+        mma3(x, fu, g);
         load_frag(g, tK, jj * 16, lane, load_bt);
-        mma2(acc, fv, g);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const float2 d = *reinterpret_cast<const float2*>(head->decay + jj * 16 + 8 * n + 2 * (lane & 3));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S[2 * jj + n][i] = fmaf(acc[n][i], i < 2 ? r0.down : r1.down, S[2 * jj + n][i] * (i & 1 ? d.y : d.x));
-        }
+        mma2(z, fv, g);
+        add_acc(S + 2 * jj, x, s0, s1, db);
+        add_acc(S + 2 * jj, z, dk);
     }
 }
 
@@ -482,7 +494,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const _
                 if (!ok) break;
                 phases ^= 1u << buf;
                 float o[2][4];
-                chunk_rows<E>(S, o, at, head, i0, lane);
+                chunk_rows(S, o, at, at + FWD_V, T_A, head, i0, lane);
                 const int lo = head->lo, t0 = head->t0;
                 more = head->more;
                 store_steps<E>(o, y + t0 * stride, stride, i0, lo, min(head->hi, s.T - t0), n_steps - t0, lane);
@@ -499,24 +511,21 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const _
         bool ok = true;
         for (int n = buf; n < chunks && ok; n += CHUNK_BUFS) {
             const int t0 = n * L, n_on = min(L, n_steps - t0);
-            float2 lw[L];
-            const bool steep = load_decays<E>(s, b, h, t0, n_on, lane, lw);
             if (n + CHUNK_BUFS < chunks) prefetch_chunk(s, b, h, t0 + CHUNK_BUFS * L, min(L, n_steps - t0 - CHUNK_BUFS * L), lane);
-            const int pieces = steep ? n_on : 1;
-            for (int i = 0; i < pieces; ++i) {
+            for (int i = 0, pieces = 1; i < pieces; ++i) {
+                float2 lw[L];
+                const bool steep = load_decays<E>(s, b, h, t0, n_on, lane, lw);
+                if (steep) {
+                    pieces = n_on;
+#pragma unroll
+                    for (int t = 0; t < L; ++t) lw[t] = t == i ? lw[t] : make_float2(0.f, 0.f);
+                }
                 if (uses > 0) ok = wait_for(&vacant[buf], (uint32_t)(uses - 1) & 1u);
                 if (!ok) break;
                 ++uses;
                 const int lo = steep ? i : 0, hi = steep ? i + 1 : n_on;
-                if (steep) {
-                    float2 one[L];
-#pragma unroll
-                    for (int t = 0; t < L; ++t) one[t] = t == i ? lw[t] : make_float2(0.f, 0.f);
-                    prepare_chunk<E>(s, b, h, t0, lo, hi, one, at, head, lane);
-                } else {
-                    prepare_chunk<E>(s, b, h, t0, lo, hi, lw, at, head, lane);
-                }
-                if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = i + 1 < pieces ? hi : L, head->more = i + 1 < pieces;
+                prepare_chunk<E, false>(s, b, h, t0, lo, hi, steep, lw, at, at + FWD_V, head, lane);
+                if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = i + 1 < pieces ? hi : L, head->more = i + 1 < pieces, head->piece = steep;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf]);
             }
@@ -527,67 +536,503 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const _
         *reinterpret_cast<uint32_t*>(y + (i >> 5) * stride + (i & 31) * 2) = 0u;
 }
 
+// ---- the backward pass -----------------------------------------------------------------------------------------------------
+// A block per head goes from the last chunk to the first. Four warps carry 16 rows of the state's gradient each and take the state before each chunk from what the
+// forward pass kept; what they make of a chunk (u, h, and both states, as bf16 pairs) crosses in shared memory to four others, which have 16 columns each and
+// work out the sums over rows: the gradients of r, a, b, k and the decays. Three warps prepare chunks ahead as in the forward pass.
+constexpr int BWD_BUFS = 3, BWD_WARPS = 8 + BWD_BUFS;
+constexpr int BWD_V = BWD_TILES * 2 * TILE, BWD_DY = BWD_V + TILE, BWD_V16 = BWD_DY + TILE, BWD_DY16 = BWD_V16 + 2 * TILE, BWD_CW = BWD_DY16 + 2 * TILE,
+              BWD_HEAD = BWD_CW + L * N * 4, BWD_BUF = BWD_HEAD + HEAD_BYTES;
+// what crosses: states 64 x 64 (bf16, hi and lo), slabs of u and h, the 16 x 16 matrices P (fp16), column sums of G o S_E by row warp
+constexpr int BIG = N * N * 2, X_S = 0, X_G = X_S + 2 * BIG, X_U = X_G + 2 * BIG, X_H = X_U + 2 * SLAB, X_P = X_H + 2 * SLAB, X_SUM = X_P + 2 * TILE, X_BYTES = X_SUM + 4 * N * 4;
+constexpr int BWD_SMEM = BWD_BUFS * BWD_BUF + X_BYTES;
+static_assert(BWD_SMEM <= 227 * 1024, "shared memory of a block");
+
+// values in bf16: one where the input's type is that, else two
 template <class E>
-__global__ void __launch_bounds__(WT) wkv_steps_bwd_kernel(const __grid_constant__ WkvBwd p) {
-    __shared__ float vec[6][64], part[WT / 32][5][64];
-    const WkvSeq& s = p.s;
-    const int bh = blockIdx.x, b = bh / s.H, h = bh - b * s.H;
-    const int tid = threadIdx.x, row = tid >> 2, c0 = (tid & 3) * 16, n = seq_length(s, b);
-    const size_t at = (size_t)bh * 4096 + row * 64 + c0;
-    E* dx[6];
-    for (int i = 0; i < 6; ++i) dx[i] = p.g.dx[i] ? static_cast<E*>(p.g.dx[i]) + ((size_t)b * s.T * s.H + h) * 64 : nullptr;
-    float G[16], S[16];
-    for (int j = 0; j < 16; ++j) G[j] = p.g.dstate_out ? p.g.dstate_out[at + j] : 0.f;
-    for (int t = s.T - 1; t >= n; --t)
-        for (int i = tid; i < 6 * 64; i += WT)
-            if (dx[i >> 6]) dx[i >> 6][(size_t)t * s.H * 64 + (i & 63)] = from_f<E>(0.f);
-    for (int t = n - 1; t >= 0; --t) {
-        const int first = t / WKV_CHUNK * WKV_CHUNK;
-        for (int j = 0; j < 16; ++j) S[j] = s.ckpt[((size_t)bh * s.n_chunks + t / WKV_CHUNK) * 4096 + row * 64 + c0 + j];
-        for (int q = first; q < t; ++q) {
-            __syncthreads();
-            load_step<E>(s, b, h, q, vec);
-            __syncthreads();
-            step_state(S, vec, row, c0);
-        }
-        __syncthreads();
-        load_step<E>(s, b, h, t, vec);
-        __syncthreads();
-        float before[16];
-        for (int j = 0; j < 16; ++j) before[j] = S[j];
-        const float u = step_state(S, vec, row, c0), v = vec[3][row];
-        const float dy = p.g.dy ? to_f(static_cast<const E*>(p.g.dy)[b * p.g.dy_batch_stride + t * p.g.dy_step_stride + h * 64 + row]) : 0.f;
-        float hh = 0.f, dv = 0.f;
-        for (int j = 0; j < 16; ++j) {
-            G[j] = fmaf(dy, vec[0][c0 + j], G[j]);
-            hh = fmaf(G[j], vec[5][c0 + j], hh);
-            dv = fmaf(G[j], vec[2][c0 + j], dv);
-        }
-        hh = quad_sum(hh);
-        dv = quad_sum(dv);
-        if (dx[3] && (tid & 3) == 0) dx[3][(size_t)t * s.H * 64 + row] = from_f<E>(dv);
-        for (int j = 0; j < 16; ++j) {
-            float sum[5] = {S[j] * dy, G[j] * before[j], G[j] * v, before[j] * hh, G[j] * u};   // r, w, k, a, b
-            for (int i = 0; i < 5; ++i)
-                for (int o = 4; o < 32; o <<= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
-            if ((tid & 31) < 4)
-                for (int i = 0; i < 5; ++i) part[tid >> 5][i][c0 + j] = sum[i];
-            G[j] = fmaf(hh, vec[4][c0 + j], G[j] * vec[1][c0 + j]);
-        }
-        __syncthreads();
-        for (int i = tid; i < 5 * 64; i += WT) {
-            const int which = i >> 6, j = i & 63, to = which < 3 ? which : which + 1;
-            float sum = 0.f;
-            for (int wp = 0; wp < WT / 32; ++wp) sum += part[wp][which][j];
-            if (which == 1) {
-                const float lw = -expf(to_f(static_cast<const E*>(s.x[1])[b * s.bs[1] + t * s.ss[1] + h * 64 + j]));
-                sum = vec[1][j] > 0.f ? sum * vec[1][j] * lw : 0.f;   // (d log d -> 0 where the decay underflows)
-            }
-            if (dx[to]) dx[to][(size_t)t * s.H * 64 + j] = from_f<E>(sum);
+__device__ __forceinline__ void put_bf16(const Vec<E>& v, uint32_t tile, int lane) {
+#pragma unroll
+    for (int t = 0; t < L; ++t) {
+        if (std::is_same<E, __nv_bfloat16>::value) {
+            st32(tile + tile_pair(t, lane), v.raw[t]);
+        } else {
+            const float2 f = raw_pair<E>(v.raw[t]);
+            uint32_t hi, lo;
+            split_bf16(f.x, f.y, hi, lo);
+            st32(tile + tile_pair(t, lane), hi);
+            st32(tile + TILE + tile_pair(t, lane), lo);
         }
     }
-    if (p.g.dstate)
-        for (int j = 0; j < 16; ++j) p.g.dstate[at + j] = G[j];
+}
+// the state alone, in pieces of a steep chunk
+__device__ __noinline__ void advance_rows(float* S, uint32_t at, const ChunkHead* head, int i0, int lane) {
+    float y[2][4];
+    chunk_rows(reinterpret_cast<float (*)[4]>(S), y, at, at + BWD_V, T_AP, head, i0, lane);
+}
+// 16 rows' share of the column sums of G o S (times d, per column): a lane's two columns, 2 lane and 2 lane + 1
+__device__ __forceinline__ float2 column_sums(const float (*G)[4], const float (*S)[4], const float* decay, bool with_decay, int lane) {
+    float2 p[8];
+#pragma unroll
+    for (int n = 0; n < 8; ++n) p[n] = make_float2(fmaf(G[n][0], S[n][0], G[n][2] * S[n][2]), fmaf(G[n][1], S[n][1], G[n][3] * S[n][3]));
+#pragma unroll
+    for (int o = 16, m = 4; m > 0; o >>= 1, m >>= 1) {   // half of what a lane holds goes to the lane that keeps it
+        const bool up = lane & o;
+#pragma unroll
+        for (int n = 0; n < m; ++n) {
+            const float2 keep = up ? p[n + m] : p[n], give = up ? p[n] : p[n + m];
+            p[n] = make_float2(keep.x + __shfl_xor_sync(0xffffffffu, give.x, o), keep.y + __shfl_xor_sync(0xffffffffu, give.y, o));
+        }
+    }
+    if (with_decay) {
+        const float2 d = *reinterpret_cast<const float2*>(decay + 2 * lane);
+        p[0].x *= d.x, p[0].y *= d.y;
+    }
+    return p[0];
+}
+// Sums over a chunk's steps within the columns of an accumulator fragment (step g in x0, g + 8 in x1): from a step on, and before it
+__device__ __forceinline__ void sums_from(float& x0, float& x1, int lane) {
+    const int g = lane >> 2;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        const float a = __shfl_down_sync(0xffffffffu, x0, 4 * o), b = __shfl_down_sync(0xffffffffu, x1, 4 * o);
+        if (g + o < 8) x0 += a, x1 += b;
+    }
+    x0 += __shfl_sync(0xffffffffu, x1, lane & 3);
+}
+__device__ __forceinline__ void sums_before(float& x0, float& x1, int lane) {
+    const int g = lane >> 2;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        const float a = __shfl_up_sync(0xffffffffu, x0, 4 * o), b = __shfl_up_sync(0xffffffffu, x1, 4 * o);
+        if (g >= o) x0 += a, x1 += b;
+    }
+    const float all0 = __shfl_sync(0xffffffffu, x0, 28 + (lane & 3));
+    x0 = __shfl_up_sync(0xffffffffu, x0, 4), x1 = __shfl_up_sync(0xffffffffu, x1, 4);
+    if (g == 0) x0 = 0.f, x1 = 0.f;
+    x1 += all0;
+}
+// the values of the step after, of the same column
+__device__ __forceinline__ void next_step(float& x0, float& x1, int lane) {
+    const int g = lane >> 2;
+    const float first1 = __shfl_sync(0xffffffffu, x1, lane & 3);
+    x0 = __shfl_down_sync(0xffffffffu, x0, 4), x1 = __shfl_down_sync(0xffffffffu, x1, 4);
+    if (g == 7) x0 = first1, x1 = 0.f;
+}
+
+template <class E>
+__global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const __grid_constant__ WkvBwd p) {
+    constexpr bool LO = std::is_same<E, __half>::value;   // inputs take two bf16 values
+    extern __shared__ __align__(128) unsigned char smem[];   // BWD_BUFS buffers, then what crosses
+    __shared__ uint64_t full[BWD_BUFS], vacant[BWD_BUFS], x_full, x_vacant, p_full;
+    __shared__ float p_down[4];
+    __shared__ int s_failed;
+    const WkvSeq& s = p.s;
+    const int bh = blockIdx.x, b = bh / s.H, h = bh - b * s.H;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const int n_steps = seq_length(s, b), chunks = (n_steps + L - 1) / L;
+    const int64_t stride = (int64_t)s.H * N, base = ((int64_t)b * s.T * s.H + h) * N;   // of the gradients
+    unsigned char* cross = smem + BWD_BUFS * BWD_BUF;
+    const uint32_t x = smem_u32(cross);
+    float* x_sum = reinterpret_cast<float*>(cross + X_SUM);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < BWD_BUFS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&vacant[i], 8);
+        }
+        mbar_init(&x_full, 4);
+        mbar_init(&x_vacant, 4);
+        mbar_init(&p_full, 4);
+        fence_mbar_init();
+        s_failed = 0;
+    }
+    __syncthreads();
+    // after the first wait that runs out nobody waits any more
+    auto wait_for = [&](uint64_t* bar, uint32_t parity) {
+        bool ok = mbar_try_wait(bar, parity);
+        if (!ok && !*reinterpret_cast<volatile int*>(&s_failed)) {
+            ok = mbar_wait_bounded(bar, parity, 1u << 18);
+            if (!ok) {
+                *reinterpret_cast<volatile int*>(&s_failed) = 1;
+                atomicOr(&g_device_status, DEV_WAIT_HEAD);
+            }
+        }
+        return __all_sync(0xffffffffu, ok) != 0;
+    };
+    bool ok = true;
+    if (warp < 4) {
+        const int i0 = warp * 16;
+        float G[8][4], S[8][4];
+        load_rows(G, p.g.dstate_out ? p.g.dstate_out + (size_t)bh * 4096 : nullptr, i0, lane);
+        E* dv_out = p.g.dx[3] ? static_cast<E*>(p.g.dx[3]) + base : nullptr;
+        uint32_t phases = 0;
+        int items = 0;
+        for (int n = chunks - 1, buf = 0; n >= 0 && ok; --n, buf = buf + 1 == BWD_BUFS ? 0 : buf + 1) {
+            const uint32_t at = smem_u32(smem) + buf * BWD_BUF;
+            const ChunkHead* head = reinterpret_cast<const ChunkHead*>(smem + buf * BWD_BUF + BWD_HEAD);
+            const float* before = s.ckpt + ((size_t)bh * s.n_chunks + n) * 4096;
+            load_rows(S, before, i0, lane);
+            for (int more = 1; more && ok;) {
+                ok = wait_for(&full[buf], phases >> buf & 1u);
+                if (!ok) break;
+                phases ^= 1u << buf;
+                more = head->more;
+                if (head->advance) {
+                    float T[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) T[i] = S[i >> 2][i & 3];
+                    advance_rows(T, at, head, i0, lane);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) S[i >> 2][i & 3] = T[i];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&vacant[buf]);
+                    continue;
+                }
+                const bool piece = head->piece;
+                const uint32_t tA = at + T_A * 2 * TILE, tR = at + T_R * 2 * TILE, tB = at + T_B * 2 * TILE, tK = at + T_K * 2 * TILE, tM = at + T_M * 2 * TILE;
+                Frag f, w;
+                Scale s0, s1;
+                float xb[2][4], xk[2][4], z[2][4];
+                // G b_E^T and G k_E^T, with dy's part
+                row_scales(G, s0, s1);
+                zero2(xb), zero2(xk);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    as_a(f, G + 2 * kk, s0.up, s1.up);
+                    load_frag(w, tB, kk * 16, lane, load_b);
+                    mma3(xb, f, w);
+                    load_frag(w, tK, kk * 16, lane, load_b);
+                    mma3(xk, f, w);
+                }
+                scale_acc(xb, s0, s1, head->down[T_B]);
+                scale_acc(xk, s0, s1, head->down[T_K]);
+                uint32_t fdy[4];
+                load_at(fdy, at + BWD_DY, i0, lane);
+                const float ddy = head->down_dy;
+                zero2(z);
+                load_frag(w, tM, M_RB * L, lane, load_bt);
+                mma2(z, fdy, w);
+                add_acc(xb, z, ddy * head->down_m[M_RB]);
+                zero2(z);
+                load_frag(w, tM, M_RK * L, lane, load_bt);
+                mma2(z, fdy, w);
+                add_acc(xk, z, ddy * head->down_m[M_RK]);
+                // h
+                s0 = scale_for(quad_top_abs(row_top(xb, 0))), s1 = scale_for(quad_top_abs(row_top(xb, 1)));
+                as_a(f, xb, s0.up, s1.up);
+                load_frag(w, at + T_Q * 2 * TILE, 0, lane, load_bt);
+                zero2(xb);
+                mma3(xb, f, w);
+                scale_acc(xb, s0, s1, head->down[T_Q]);
+                // dv
+                Scale h0 = scale_for(quad_top_abs(row_top(xb, 0))), h1 = scale_for(quad_top_abs(row_top(xb, 1)));
+                Frag fh;
+                as_a(fh, xb, h0.up, h1.up);
+                zero2(z);
+                load_frag(w, tM, M_X * L, lane, load_bt);
+                mma3(z, fh, w);
+                add_acc(xk, z, h0, h1, head->down_m[M_X]);
+                if (dv_out) store_steps<E>(xk, dv_out + head->t0 * stride, stride, i0, head->lo, min(head->hi, s.T - head->t0), n_steps - head->t0, lane);
+                // u
+                if (!piece) decay_rows(S, head, lane);
+                row_scales(S, s0, s1);
+                float u[2][4];
+                state_times(u, S, s0, s1, at + T_AP * 2 * TILE, lane);
+                scale_acc(u, s0, s1, head->down[T_AP]);
+                uint32_t fv[4];
+                load_at(fv, at + BWD_V, i0, lane);
+                zero2(z);
+                load_frag(w, tM, M_AK * L, lane, load_b);
+                mma2(z, fv, w);
+                add_acc(u, z, head->down_v * head->down_m[M_AK]);
+                const float2 gs = column_sums(G, S, head->decay, piece, lane);
+                // to the column warps
+                if (items > 0) ok = wait_for(&x_vacant, (uint32_t)(items - 1) & 1u);
+                if (!ok) break;
+                ++items;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t hi, lo;
+                        const uint32_t to = i0 * 128 + tile_at(g + 8 * half, 8 * i + 2 * q);
+                        split_bf16(S[i][2 * half], S[i][2 * half + 1], hi, lo);
+                        st32(x + X_S + to, hi);
+                        st32(x + X_S + BIG + to, lo);
+                        split_bf16(G[i][2 * half], G[i][2 * half + 1], hi, lo);
+                        st32(x + X_G + to, hi);
+                        st32(x + X_G + BIG + to, lo);
+                    }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t hi, lo;
+                        const uint32_t to = slab_at(i0 + g + 8 * half, 8 * i + 2 * q);
+                        split_bf16(u[i][2 * half], u[i][2 * half + 1], hi, lo);
+                        st32(x + X_U + to, hi);
+                        st32(x + X_U + SLAB + to, lo);
+                        split_bf16(xb[i][2 * half], xb[i][2 * half + 1], hi, lo);
+                        st32(x + X_H + to, hi);
+                        st32(x + X_H + SLAB + to, lo);
+                    }
+                *reinterpret_cast<float2*>(x_sum + warp * N + 2 * lane) = gs;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&x_full);
+                // the gradient of the state before the chunk
+                const float dr = ddy * head->down[T_R], da = head->down[T_A];
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    float y[2][4];
+                    zero2(y), zero2(z);
+                    load_frag(w, tR, jj * 16, lane, load_bt);
+                    mma2(y, fdy, w);
+                    load_frag(w, tA, jj * 16, lane, load_bt);
+                    mma3(z, fh, w);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 d = *reinterpret_cast<const float2*>(head->decay + jj * 16 + 8 * i + 2 * q);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const float e = c & 1 ? d.y : d.x, a = z[i][c] * (c < 2 ? h0.down : h1.down) * da, r = fmaf(y[i][c], dr, G[2 * jj + i][c]);
+                            G[2 * jj + i][c] = piece ? fmaf(r, e, a) : (r + a) * e;
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&vacant[buf]);
+                if (more) load_rows(S, before, i0, lane);
+            }
+        }
+        if (p.g.dstate) store_rows(G, p.g.dstate + (size_t)bh * 4096, i0, lane);
+    } else if (warp < 8) {
+        const int cw = warp - 4, c0 = cw * 16;
+        uint32_t phases = 0;
+        int items = 0;
+        for (int n = chunks - 1, buf = 0; n >= 0 && ok; --n, buf = buf + 1 == BWD_BUFS ? 0 : buf + 1) {
+            const uint32_t at = smem_u32(smem) + buf * BWD_BUF;
+            const ChunkHead* head = reinterpret_cast<const ChunkHead*>(smem + buf * BWD_BUF + BWD_HEAD);
+            const float* cws = reinterpret_cast<const float*>(smem + buf * BWD_BUF + BWD_CW);
+            for (int more = 1; more && ok;) {
+                ok = wait_for(&full[buf], phases >> buf & 1u);
+                if (!ok) break;
+                phases ^= 1u << buf;
+                more = head->more;
+                if (head->advance) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&vacant[buf]);
+                    continue;
+                }
+                const uint32_t tA = at + T_A * 2 * TILE, tR = at + T_R * 2 * TILE, tB = at + T_B * 2 * TILE, tK = at + T_K * 2 * TILE;
+                const uint32_t vt = at + BWD_V16, dyt = at + BWD_DY16, P = x + X_P;
+                ok = wait_for(&x_full, (uint32_t)items & 1u);
+                if (!ok) break;
+                auto input = [&](Frag& f, uint32_t tile, int i, void (*how)(uint32_t*, uint32_t, int, int)) {
+                    how(f.hi, tile, i, lane);
+                    if (LO) how(f.lo, tile + TILE, i, lane);
+                };
+                auto slab = [&](Frag& f, uint32_t from, int i, void (*how)(uint32_t*, uint32_t, int, int)) {
+                    how(f.hi, from, i, lane);
+                    how(f.lo, from + SLAB, i, lane);
+                };
+                {   // one of the four matrices P: (dy, h) by (u, v)
+                    float m[2][4];
+                    zero2(m);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        Frag f, w;
+                        if (cw < 2) input(f, dyt, kk * 16, load_a);
+                        else slab(f, x + X_H, kk * 16, slab_a);
+                        if (cw & 1) input(w, vt, kk * 16, load_b);
+                        else slab(w, x + X_U, kk * 16, slab_b);
+                        if (cw == 0) mmab<LO, true>(m, f, w);
+                        else if (cw == 1) mmab<LO, LO>(m, f, w);
+                        else if (cw == 2) mmab<true, true>(m, f, w);
+                        else mmab<true, LO>(m, f, w);
+                    }
+                    keep_lower(m, 1.f, 1.f, cw >> 1, lane);
+                    const float d = put_block(m, P, cw * L, lane);
+                    if (lane == 0) p_down[cw] = d;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full);
+                }
+                float dr[2][4], da[2][4], db[2][4], dk[2][4];
+                zero2(dr), zero2(da), zero2(db), zero2(dk);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    Frag f, w;
+                    load_bt(w.hi, x + X_S + kk * 2048, c0, lane);
+                    load_bt(w.lo, x + X_S + BIG + kk * 2048, c0, lane);
+                    input(f, dyt, kk * 16, load_a);
+                    mmab<LO, true>(dr, f, w);
+                    slab(f, x + X_H, kk * 16, slab_a);
+                    mmab<true, true>(da, f, w);
+                    load_bt(w.hi, x + X_G + kk * 2048, c0, lane);
+                    load_bt(w.lo, x + X_G + BIG + kk * 2048, c0, lane);
+                    slab(f, x + X_U, kk * 16, slab_a);
+                    mmab<true, true>(db, f, w);
+                    input(f, vt, kk * 16, load_a);
+                    mmab<LO, true>(dk, f, w);
+                }
+                ok = wait_for(&p_full, (uint32_t)items & 1u);
+                if (!ok) break;
+                ++items;
+                float pr[2][4], pa[2][4], pb[2][4], pk[2][4];
+                zero2(pr), zero2(pa), zero2(pb), zero2(pk);
+                auto times = [&](float (*c)[4], int block, const Frag& w, float d, void (*how)(uint32_t*, uint32_t, int, int)) {
+                    Frag f;
+                    float z[2][4];
+                    zero2(z);
+                    load_frag(f, P, block * L, lane, how);
+                    mma3(z, f, w);
+                    add_acc(c, z, d * p_down[block]);
+                };
+                {
+                    Frag w;
+                    load_frag(w, tB, c0, lane, load_bt);
+                    times(pr, 0, w, head->down[T_B], load_a);
+                    times(pa, 2, w, head->down[T_B], load_a);
+                    load_frag(w, tK, c0, lane, load_bt);
+                    times(pr, 1, w, head->down[T_K], load_a);
+                    times(pa, 3, w, head->down[T_K], load_a);
+                    load_frag(w, tR, c0, lane, load_bt);
+                    times(pb, 0, w, head->down[T_R], load_at);
+                    times(pk, 1, w, head->down[T_R], load_at);
+                    load_frag(w, tA, c0, lane, load_bt);
+                    times(pb, 2, w, head->down[T_A], load_at);
+                    times(pk, 3, w, head->down[T_A], load_at);
+                }
+                float2 gs[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    gs[i] = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float2 t = *reinterpret_cast<const float2*>(x_sum + r * N + c0 + 8 * i + 2 * q);
+                        gs[i].x += t.x, gs[i].y += t.y;
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&x_vacant);
+                const int t0 = head->t0, lo = head->lo, hi = min(head->hi, s.T - t0), n_on = n_steps - t0;
+                const bool piece = head->piece;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int j = c0 + 8 * i + 2 * q;
+                    const float2 end = *reinterpret_cast<const float2*>(cws + 15 * N + j);
+                    float pos[2][2], posa[2][2], flow[2][2], lw[2][2];   // [column][half]
+                    const int64_t at_j = (int64_t)h * N + j;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int t = g + 8 * half;
+                        const bool on = t >= lo && t < min(hi, n_on);
+                        const float2 c = *reinterpret_cast<const float2*>(cws + t * N + j);
+                        const float2 c1 = t ? *reinterpret_cast<const float2*>(cws + (t - 1) * N + j) : make_float2(0.f, 0.f);
+                        auto in = [&](int which) {
+                            return on ? raw_pair<E>(load_raw(static_cast<const E*>(s.x[which]) + b * s.bs[which] + (int64_t)(t0 + t) * s.ss[which] + at_j, s.even >> which & 1))
+                                      : make_float2(0.f, 0.f);
+                        };
+                        const float2 r = in(0), wv = in(1), k = in(2), a = in(4), bb = in(5);
+                        float out[5][2];   // r, w, k, a, b
+#pragma unroll
+                        for (int cc = 0; cc < 2; ++cc) {
+                            const int e = 2 * half + cc;
+                            const float ct = cc ? c.y : c.x, cp = cc ? c1.y : c1.x, en = cc ? end.y : end.x;
+                            const float er = piece ? 1.f : ex2_(ct - en), ea = piece ? 1.f : ex2_(cp - en), ei = ex2_(en - ct);
+                            const float grs = dr[i][e] * (piece ? ex2_(en) : er), gr = fmaf(pr[i][e], er, grs), ga = (da[i][e] + pa[i][e]) * ea;
+                            const float gbs = db[i][e] * ei, gks = dk[i][e] * ei, gbp = pb[i][e] * ei, gkp = pk[i][e] * ei;
+                            const float rv = cc ? r.y : r.x, kv = cc ? k.y : k.x, av = cc ? a.y : a.x, bv = cc ? bb.y : bb.x;
+                            out[0][cc] = gr, out[2][cc] = gks + gkp, out[3][cc] = ga, out[4][cc] = gbs + gbp;
+                            // (a step's pairs with itself cancel, and a piece has no others: left out, nothing of them is multiplied with a steep log decay)
+                            pos[cc][half] = piece ? rv * grs : fmaf(rv, gr, -fmaf(bv, gbp, kv * gkp));
+                            posa[cc][half] = av * ga;
+                            flow[cc][half] = fmaf(bv, gbs, kv * gks);
+                            lw[cc][half] = on ? log2_decay(cc ? wv.y : wv.x) * 0.6931471805599453f : 0.f;
+                        }
+                        if (t >= lo && t < hi) {
+                            const int64_t to = base + (t0 + t) * stride + j;
+                            if (p.g.dx[0]) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[0]) + to) = on ? pack_pair<E>(out[0][0], out[0][1]) : 0u;
+                            if (p.g.dx[2]) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[2]) + to) = on ? pack_pair<E>(out[2][0], out[2][1]) : 0u;
+                            if (p.g.dx[4]) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[4]) + to) = on ? pack_pair<E>(out[3][0], out[3][1]) : 0u;
+                            if (p.g.dx[5]) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[5]) + to) = on ? pack_pair<E>(out[4][0], out[4][1]) : 0u;
+                        }
+                    }
+                    if (p.g.dx[1]) {
+#pragma unroll
+                        for (int cc = 0; cc < 2; ++cc) {
+                            next_step(posa[cc][0], posa[cc][1], lane);
+                            pos[cc][0] += posa[cc][0], pos[cc][1] += posa[cc][1];
+                            sums_from(pos[cc][0], pos[cc][1], lane);
+                            sums_before(flow[cc][0], flow[cc][1], lane);
+                        }
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int t = g + 8 * half;
+                            const float x0 = (gs[i].x + flow[0][half] + pos[0][half]) * lw[0][half], x1 = (gs[i].y + flow[1][half] + pos[1][half]) * lw[1][half];
+                            if (t >= lo && t < hi) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[1]) + base + (t0 + t) * stride + j) = t < n_on ? pack_pair<E>(x0, x1) : 0u;
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&vacant[buf]);
+            }
+        }
+    } else {
+        const int buf = warp - 8;
+        const uint32_t at = smem_u32(smem) + buf * BWD_BUF;
+        ChunkHead* head = reinterpret_cast<ChunkHead*>(smem + buf * BWD_BUF + BWD_HEAD);
+        float* cws = reinterpret_cast<float*>(smem + buf * BWD_BUF + BWD_CW);
+        int uses = 0;
+        for (int n = chunks - 1 - buf; n >= 0 && ok; n -= BWD_BUFS) {
+            const int t0 = n * L, n_on = min(L, n_steps - t0);
+            if (n >= BWD_BUFS) prefetch_chunk(s, b, h, t0 - BWD_BUFS * L, L, lane);
+            // a steep chunk: for each step from the last one, the steps before it for the state's sake, and then the step itself
+            for (int i = 0, j = 0, last = 0, started = 0; !last && ok;) {
+                float2 lw[L];
+                const bool steep = load_decays<E>(s, b, h, t0, n_on, lane, lw);
+                if (!started) i = steep ? n_on - 1 : 0, started = 1;
+                const bool advance = steep && j < i;
+                const int step = advance ? j : i;
+                if (steep) {
+#pragma unroll
+                    for (int t = 0; t < L; ++t) lw[t] = t == step ? lw[t] : make_float2(0.f, 0.f);
+                }
+                last = !steep || (i == 0 && !advance);
+                if (uses > 0) ok = wait_for(&vacant[buf], (uint32_t)(uses - 1) & 1u);
+                if (!ok) break;
+                ++uses;
+                const int lo = steep ? step : 0, hi = steep ? step + 1 : n_on;
+                float2 c = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int t = 0; t < L; ++t) {
+                    c.x += lw[t].x, c.y += lw[t].y;
+                    *reinterpret_cast<float2*>(cws + t * N + 2 * lane) = c;
+                }
+                Vec<E> v;
+                if (p.g.dy) v.load(p.g.dy, b * p.g.dy_batch_stride + (int64_t)t0 * p.g.dy_step_stride + h * N, p.g.dy_step_stride, s.even >> 6 & 1, lo, hi, lane);
+                else
+#pragma unroll
+                    for (int t = 0; t < L; ++t) v.raw[t] = 0u;
+                const float down_dy = put_exact(v, at + BWD_DY, lane);
+                put_bf16(v, at + BWD_DY16, lane);
+                v.load(s, 3, b, h, t0, lo, hi, lane);
+                put_bf16(v, at + BWD_V16, lane);
+                prepare_chunk<E, true>(s, b, h, t0, lo, hi, steep, lw, at, at + BWD_V, head, lane);
+                if (lane == 0) {
+                    head->t0 = t0, head->lo = lo, head->hi = step + 1 == n_on || !steep ? L : hi, head->more = !last, head->piece = steep, head->advance = advance;
+                    head->down_dy = down_dy;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[buf]);
+                if (advance) ++j;
+                else --i, j = 0;
+            }
+        }
+    }
+    // steps behind the last chunk
+    for (int w = 0; w < 6; ++w)
+        if (p.g.dx[w])
+            for (int64_t i = (int64_t)chunks * L * 32 + threadIdx.x; i < (int64_t)s.T * 32; i += BWD_WARPS * 32)
+                *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[w]) + base + (i >> 5) * stride + (i & 31) * 2) = 0u;
 }
 
 WkvSeq seq_of(const ab_wkv7_seq& s) {
@@ -625,8 +1070,16 @@ int wkv_train_fwd(const ab_wkv7_seq& s, void* y, float* state_out, cudaStream_t 
 
 int wkv_train_bwd(const ab_wkv7_seq& s, const WkvBackward& g, cudaStream_t st) {
     WkvBwd p = {seq_of(s), g};
-    if (s.dtype == AB_DT_F16) wkv_steps_bwd_kernel<__half><<<s.B * s.H, WT, 0, st>>>(p);
-    else wkv_steps_bwd_kernel<__nv_bfloat16><<<s.B * s.H, WT, 0, st>>>(p);
+    if (reinterpret_cast<uintptr_t>(g.dy) % 4 == 0 && g.dy_batch_stride % 2 == 0 && g.dy_step_stride % 2 == 0) p.s.even |= 1u << 6;
+    static PerDeviceOnce once;
+    const int c = once.run(nullptr, [&](const DeviceProps&) -> int {
+        AB_CUDA(cudaFuncSetAttribute(wkv_chunk_bwd_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM));
+        AB_CUDA(cudaFuncSetAttribute(wkv_chunk_bwd_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM));
+        return OK;
+    });
+    if (c != OK) return c;
+    if (s.dtype == AB_DT_F16) wkv_chunk_bwd_kernel<__half><<<s.B * s.H, BWD_WARPS * 32, BWD_SMEM, st>>>(p);
+    else wkv_chunk_bwd_kernel<__nv_bfloat16><<<s.B * s.H, BWD_WARPS * 32, BWD_SMEM, st>>>(p);
     return check_cuda(cudaGetLastError(), "ab_wkv7_seq_bwd");
 }
 

@@ -125,24 +125,7 @@ __device__ __forceinline__ float row_top(const float (*c)[4], int half) {   // l
     return fmaxf(fmaxf(fabsf(c[0][2 * half]), fabsf(c[0][2 * half + 1])), fmaxf(fabsf(c[1][2 * half]), fabsf(c[1][2 * half + 1])));
 }
 
-// two neighbouring values of an input as floats; `even`: on a 4-byte boundary
-template <class E>
-__device__ __forceinline__ float2 load_pair(const E* p, bool even) {
-    E x, y;
-    if (even) {
-        const uint32_t u = __ldg(reinterpret_cast<const uint32_t*>(p));
-        const uint16_t ux = (uint16_t)u, uy = (uint16_t)(u >> 16);
-        x = *reinterpret_cast<const E*>(&ux), y = *reinterpret_cast<const E*>(&uy);
-    } else {
-        x = p[0], y = p[1];
-    }
-    return make_float2(to_f(x), to_f(y));
-}
-template <class E>
-__device__ __forceinline__ uint32_t load_raw(const E* p, bool even) {
-    if (even) return __ldg(reinterpret_cast<const uint32_t*>(p));
-    return (uint32_t)*reinterpret_cast<const uint16_t*>(p) | (uint32_t)*reinterpret_cast<const uint16_t*>(p + 1) << 16;
-}
+// two neighbouring values of an input as floats
 template <class E> __device__ __forceinline__ float2 raw_pair(uint32_t u);
 template <> __device__ __forceinline__ float2 raw_pair<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 template <> __device__ __forceinline__ float2 raw_pair<__nv_bfloat16>(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }

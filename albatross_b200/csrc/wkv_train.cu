@@ -20,7 +20,6 @@ struct WkvSeq {
     const int* lengths;
     float* ckpt;
     int T, H, n_chunks;
-    unsigned even;   // bit i: every pair of values of x[i] is on a 4-byte boundary; bit 6: of dy
 };
 struct WkvFwd {
     WkvSeq s;
@@ -48,13 +47,14 @@ constexpr int FWD_V = FWD_TILES * 2 * TILE, FWD_HEAD = FWD_V + TILE, FWD_BUF = F
 template <class E>
 struct Vec {
     uint32_t raw[L];
-    __device__ __forceinline__ void load(const void* x, int64_t at, int64_t stride, bool even, int lo, int hi, int lane) {
-        const E* p = static_cast<const E*>(x) + at + 2 * lane;
+    __device__ __forceinline__ void load(const void* x, int64_t at, int64_t stride, int lo, int hi, int lane) {
+        const char* p = reinterpret_cast<const char*>(static_cast<const E*>(x) + at + 2 * lane);
+        const int64_t step = stride * 2;
 #pragma unroll
-        for (int t = 0; t < L; ++t) raw[t] = t >= lo && t < hi ? load_raw(p + t * stride, even) : 0u;
+        for (int t = 0; t < L; ++t) raw[t] = t >= lo && t < hi ? __ldg(reinterpret_cast<const uint32_t*>(p + t * step)) : 0u;
     }
     __device__ __forceinline__ void load(const WkvSeq& s, int which, int64_t b, int h, int t0, int lo, int hi, int lane) {
-        load(s.x[which], b * s.bs[which] + (int64_t)t0 * s.ss[which] + h * N, s.ss[which], s.even >> which & 1, lo, hi, lane);
+        load(s.x[which], b * s.bs[which] + (int64_t)t0 * s.ss[which] + h * N, s.ss[which], lo, hi, lane);
     }
     __device__ __forceinline__ float top() const {
         uint32_t m = 0;   // the order of non-negative floats is that of their bits
@@ -203,10 +203,26 @@ __device__ __forceinline__ float put_exact(const Vec<E>& v, uint32_t tile, int l
     return sc.down;
 }
 
-// Prepares steps lo .. hi - 1 of a chunk; lw: log2 decays, zero at the other steps. at: the buffer's tiles; v: where v goes; ap: the tile for a'. BWD: Q is kept too.
+// values in bf16: one where the input's type is that, else two
+template <class E>
+__device__ __forceinline__ void put_bf16(const Vec<E>& v, uint32_t tile, int lane) {
+#pragma unroll
+    for (int t = 0; t < L; ++t) {
+        if (std::is_same<E, __nv_bfloat16>::value) {
+            st32(tile + tile_pair(t, lane), v.raw[t]);
+        } else {
+            const float2 f = raw_pair<E>(v.raw[t]);
+            uint32_t hi, lo;
+            split_bf16(f.x, f.y, hi, lo);
+            st32(tile + tile_pair(t, lane), hi);
+            st32(tile + TILE + tile_pair(t, lane), lo);
+        }
+    }
+}
+// Prepares steps lo .. hi - 1 of a chunk; lw: log2 decays, zero at the other steps. at: the buffer's tiles; v: where v goes. BWD: Q and v in bf16 (v16) are kept too.
 template <class E, bool BWD>
-__device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h, int t0, int lo, int hi, bool piece, const float2* lw, uint32_t at, uint32_t v, ChunkHead* head,
-                                              int lane) {
+__device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h, int t0, int lo, int hi, bool piece, const float2* lw, uint32_t at, uint32_t v, uint32_t v16,
+                                              ChunkHead* head, int lane) {
     constexpr int AP = BWD ? T_AP : T_A;
     const uint32_t tA = at + T_A * 2 * TILE, tR = at + T_R * 2 * TILE, tB = at + T_B * 2 * TILE, tK = at + T_K * 2 * TILE, tM = at + T_M * 2 * TILE, tAP = at + AP * 2 * TILE;
     float down_b, down_k, down_a, down_r;
@@ -214,20 +230,21 @@ __device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h,
         float2 end = make_float2(0.f, 0.f);
 #pragma unroll
         for (int t = 0; t < L; ++t) end.x += lw[t].x, end.y += lw[t].y;
-        Vec<E> x;
+        Vec<E> x, y;   // (a vector is on its way while the one before it is worked on)
         auto to_end = [&](float, float c, int i) { return (i ? end.y : end.x) - c; };   // at most 0
         x.load(s, 5, b, h, t0, lo, hi, lane);
+        y.load(s, 2, b, h, t0, lo, hi, lane);
         down_b = put_tile(x, lw, tB, lane, 1.f, to_end);
-        x.load(s, 2, b, h, t0, lo, hi, lane);
-        down_k = put_tile(x, lw, tK, lane, 1.f, to_end);
+        x.load(s, 4, b, h, t0, lo, hi, lane);
+        down_k = put_tile(y, lw, tK, lane, 1.f, to_end);
+        y.load(s, 0, b, h, t0, lo, hi, lane);
         // a's and r's factors are at most `grow` (2^STEEP_LOG2); in a piece of one step they are 1
         const float grow = piece ? 1.f : ex2_(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(-fminf(end.x, end.y), 0.f)))));
-        x.load(s, 4, b, h, t0, lo, hi, lane);
         down_a = put_tile(x, lw, tA, lane, grow, [&](float c, float, int i) { return piece ? 0.f : c - (i ? end.y : end.x); });
-        x.load(s, 0, b, h, t0, lo, hi, lane);
-        down_r = put_tile(x, lw, tR, lane, grow, [&](float, float c, int i) { return piece ? 0.f : c - (i ? end.y : end.x); });
         x.load(s, 3, b, h, t0, lo, hi, lane);
+        down_r = put_tile(y, lw, tR, lane, grow, [&](float, float c, int i) { return piece ? 0.f : c - (i ? end.y : end.x); });
         const float down_v = put_exact(x, v, lane);
+        if (BWD) put_bf16(x, v16, lane);
         *reinterpret_cast<float2*>(head->decay + 2 * lane) = make_float2(ex2_(end.x), ex2_(end.y));
         if (lane == 0) head->down_v = down_v;
     }
@@ -524,7 +541,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const _
                 if (!ok) break;
                 ++uses;
                 const int lo = steep ? i : 0, hi = steep ? i + 1 : n_on;
-                prepare_chunk<E, false>(s, b, h, t0, lo, hi, steep, lw, at, at + FWD_V, head, lane);
+                prepare_chunk<E, false>(s, b, h, t0, lo, hi, steep, lw, at, at + FWD_V, 0u, head, lane);
                 if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = i + 1 < pieces ? hi : L, head->more = i + 1 < pieces, head->piece = steep;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf]);
@@ -548,22 +565,6 @@ constexpr int BIG = N * N * 2, X_S = 0, X_G = X_S + 2 * BIG, X_U = X_G + 2 * BIG
 constexpr int BWD_SMEM = BWD_BUFS * BWD_BUF + X_BYTES;
 static_assert(BWD_SMEM <= 227 * 1024, "shared memory of a block");
 
-// values in bf16: one where the input's type is that, else two
-template <class E>
-__device__ __forceinline__ void put_bf16(const Vec<E>& v, uint32_t tile, int lane) {
-#pragma unroll
-    for (int t = 0; t < L; ++t) {
-        if (std::is_same<E, __nv_bfloat16>::value) {
-            st32(tile + tile_pair(t, lane), v.raw[t]);
-        } else {
-            const float2 f = raw_pair<E>(v.raw[t]);
-            uint32_t hi, lo;
-            split_bf16(f.x, f.y, hi, lo);
-            st32(tile + tile_pair(t, lane), hi);
-            st32(tile + TILE + tile_pair(t, lane), lo);
-        }
-    }
-}
 // the state alone, in pieces of a steep chunk
 __device__ __noinline__ void advance_rows(float* S, uint32_t at, const ChunkHead* head, int i0, int lane) {
     float y[2][4];
@@ -824,6 +825,21 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 }
                 const uint32_t tA = at + T_A * 2 * TILE, tR = at + T_R * 2 * TILE, tB = at + T_B * 2 * TILE, tK = at + T_K * 2 * TILE;
                 const uint32_t vt = at + BWD_V16, dyt = at + BWD_DY16, P = x + X_P;
+                const int t0 = head->t0, lo = head->lo, hi = min(head->hi, s.T - t0), n_on = n_steps - t0;
+                const bool piece = head->piece;
+                uint32_t raw[5][2][2];   // r, w, k, a, b of this warp's columns
+#pragma unroll
+                for (int v = 0; v < 5; ++v) {
+                    const int which = v < 3 ? v : v + 1;
+                    const E* from = static_cast<const E*>(s.x[which]) + b * s.bs[which] + (int64_t)t0 * s.ss[which] + h * N + c0 + 2 * q;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int t = g + 8 * half;
+                            raw[v][i][half] = t >= lo && t < min(hi, n_on) ? __ldg(reinterpret_cast<const uint32_t*>(from + t * s.ss[which] + 8 * i)) : 0u;
+                        }
+                }
                 ok = wait_for(&x_full, (uint32_t)items & 1u);
                 if (!ok) break;
                 auto input = [&](Frag& f, uint32_t tile, int i, void (*how)(uint32_t*, uint32_t, int, int)) {
@@ -913,25 +929,19 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&x_vacant);
-                const int t0 = head->t0, lo = head->lo, hi = min(head->hi, s.T - t0), n_on = n_steps - t0;
-                const bool piece = head->piece;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int j = c0 + 8 * i + 2 * q;
                     const float2 end = *reinterpret_cast<const float2*>(cws + 15 * N + j);
                     float pos[2][2], posa[2][2], flow[2][2], lw[2][2];   // [column][half]
-                    const int64_t at_j = (int64_t)h * N + j;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const int t = g + 8 * half;
                         const bool on = t >= lo && t < min(hi, n_on);
                         const float2 c = *reinterpret_cast<const float2*>(cws + t * N + j);
                         const float2 c1 = t ? *reinterpret_cast<const float2*>(cws + (t - 1) * N + j) : make_float2(0.f, 0.f);
-                        auto in = [&](int which) {
-                            return on ? raw_pair<E>(load_raw(static_cast<const E*>(s.x[which]) + b * s.bs[which] + (int64_t)(t0 + t) * s.ss[which] + at_j, s.even >> which & 1))
-                                      : make_float2(0.f, 0.f);
-                        };
-                        const float2 r = in(0), wv = in(1), k = in(2), a = in(4), bb = in(5);
+                        const float2 r = raw_pair<E>(raw[0][i][half]), wv = raw_pair<E>(raw[1][i][half]), k = raw_pair<E>(raw[2][i][half]);
+                        const float2 a = raw_pair<E>(raw[3][i][half]), bb = raw_pair<E>(raw[4][i][half]);
                         float out[5][2];   // r, w, k, a, b
 #pragma unroll
                         for (int cc = 0; cc < 2; ++cc) {
@@ -1008,15 +1018,10 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                     *reinterpret_cast<float2*>(cws + t * N + 2 * lane) = c;
                 }
                 Vec<E> v;
-                if (p.g.dy) v.load(p.g.dy, b * p.g.dy_batch_stride + (int64_t)t0 * p.g.dy_step_stride + h * N, p.g.dy_step_stride, s.even >> 6 & 1, lo, hi, lane);
-                else
-#pragma unroll
-                    for (int t = 0; t < L; ++t) v.raw[t] = 0u;
+                v.load(p.g.dy, b * p.g.dy_batch_stride + (int64_t)t0 * p.g.dy_step_stride + h * N, p.g.dy_step_stride, lo, p.g.dy ? hi : lo, lane);
                 const float down_dy = put_exact(v, at + BWD_DY, lane);
                 put_bf16(v, at + BWD_DY16, lane);
-                v.load(s, 3, b, h, t0, lo, hi, lane);
-                put_bf16(v, at + BWD_V16, lane);
-                prepare_chunk<E, true>(s, b, h, t0, lo, hi, steep, lw, at, at + BWD_V, head, lane);
+                prepare_chunk<E, true>(s, b, h, t0, lo, hi, steep, lw, at, at + BWD_V, at + BWD_V16, head, lane);
                 if (lane == 0) {
                     head->t0 = t0, head->lo = lo, head->hi = step + 1 == n_on || !steep ? L : hi, head->more = !last, head->piece = steep, head->advance = advance;
                     head->down_dy = down_dy;
@@ -1041,7 +1046,6 @@ WkvSeq seq_of(const ab_wkv7_seq& s) {
         q.x[i] = s.x[i];
         q.bs[i] = s.batch_stride[i];
         q.ss[i] = s.step_stride[i];
-        if (reinterpret_cast<uintptr_t>(s.x[i]) % 4 == 0 && s.batch_stride[i] % 2 == 0 && s.step_stride[i] % 2 == 0) q.even |= 1u << i;
     }
     q.state = s.state;
     q.lengths = s.lengths;
@@ -1070,7 +1074,6 @@ int wkv_train_fwd(const ab_wkv7_seq& s, void* y, float* state_out, cudaStream_t 
 
 int wkv_train_bwd(const ab_wkv7_seq& s, const WkvBackward& g, cudaStream_t st) {
     WkvBwd p = {seq_of(s), g};
-    if (reinterpret_cast<uintptr_t>(g.dy) % 4 == 0 && g.dy_batch_stride % 2 == 0 && g.dy_step_stride % 2 == 0) p.s.even |= 1u << 6;
     static PerDeviceOnce once;
     const int c = once.run(nullptr, [&](const DeviceProps&) -> int {
         AB_CUDA(cudaFuncSetAttribute(wkv_chunk_bwd_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD_SMEM));

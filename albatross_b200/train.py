@@ -46,6 +46,13 @@ def _dense_last(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
+def _steps(t: torch.Tensor) -> torch.Tensor:
+    """[B, T, C] with a dense last dimension and every step on a 4-byte boundary."""
+    if t.stride(2) == 1 and not (t.stride(0) | t.stride(1)) & 1 and not t.data_ptr() & 3:
+        return t
+    return t.contiguous() if not (t.is_contiguous() and t.data_ptr() & 3) else t.clone()
+
+
 def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -86,7 +93,7 @@ class _Wkv7(torch.autograd.Function):
         state, lengths, checkpoints, *xs = ctx.saved_tensors
         B, T, C_ = xs[0].shape
         device = xs[0].device
-        dy = None if dy is None else _dense_last(dy)
+        dy = None if dy is None else _steps(dy)
         dout = None if dout is None else dout.contiguous()
         need = ctx.needs_input_grad
         dxs = [torch.empty((B, T, C_), dtype=xs[0].dtype, device=device) if n else None for n in need[2:]]
@@ -115,7 +122,7 @@ def RWKV7_TRAIN_OP(state: Optional[torch.Tensor], r, w, k, v, a, b, lengths: Opt
     if lengths is not None:
         assert lengths.shape == (B,) and lengths.dtype == torch.int32 and lengths.device == r.device
         lengths = lengths.contiguous()
-    xs = tuple(_dense_last(x) for x in xs)
+    xs = tuple(_steps(x) for x in xs)
     if _needs_grad(state, *xs):
         return _Wkv7.apply(state, lengths, *xs)
     return _wkv_forward(state, xs, lengths, False)[:2]

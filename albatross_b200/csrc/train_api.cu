@@ -15,7 +15,7 @@ int check_seq(const ab_wkv7_seq* s, const char* who) {
     AB_CHECK_ARG((int64_t)s->B * s->H <= INT32_MAX && s->T <= INT32_MAX - 64, "%s: too many heads or steps", who);
     for (int i = 0; i < 6; ++i) {
         AB_CHECK_ARG(s->x[i] || s->T == 0, "%s: null pointer", who);
-        AB_CHECK_ARG(on_boundary(s->x[i], 4) && s->batch_stride[i] % 2 == 0 && s->step_stride[i] % 2 == 0, "%s: inputs and their steps must start on 4-byte boundaries", who);
+        AB_CHECK_ARG(on_boundary(s->x[i], 16) && s->batch_stride[i] % 8 == 0 && s->step_stride[i] % 8 == 0, "%s: inputs and their steps must start on 16-byte boundaries", who);
     }
     AB_CHECK_ARG(on_boundary(s->state, 16) && on_boundary(s->checkpoints, 16), "%s: states must start on a 16-byte boundary", who);
     AB_CHECK_ARG(on_boundary(s->lengths, 4), "%s: lengths must start on a 4-byte boundary", who);
@@ -78,7 +78,7 @@ int ab_wkv7_seq_bwd(const ab_wkv7_seq* s, const void* dy, int64_t dy_batch_strid
     AB_CHECK(check_seq(s, "ab_wkv7_seq_bwd"));
     AB_CHECK_ARG(dx, "ab_wkv7_seq_bwd: null pointer");
     AB_CHECK_ARG(s->checkpoints || s->T == 0, "ab_wkv7_seq_bwd: needs the checkpoints of the forward pass");
-    AB_CHECK_ARG(!dy || (on_boundary(dy, 4) && dy_batch_stride % 2 == 0 && dy_step_stride % 2 == 0), "ab_wkv7_seq_bwd: dy and its steps must start on 4-byte boundaries");
+    AB_CHECK_ARG(!dy || (on_boundary(dy, 16) && dy_batch_stride % 8 == 0 && dy_step_stride % 8 == 0), "ab_wkv7_seq_bwd: dy and its steps must start on 16-byte boundaries");
     AB_CHECK_ARG(on_boundary(dstate_out, 16) && on_boundary(dstate, 16), "ab_wkv7_seq_bwd: misaligned pointer");
     WkvBackward g = {dy, dy_batch_stride, dy_step_stride, dstate_out, {}, dstate};
     for (int i = 0; i < 6; ++i) {

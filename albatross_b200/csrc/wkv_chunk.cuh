@@ -112,6 +112,9 @@ __device__ __forceinline__ float ex2_(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
     return e;
 }
+__device__ __forceinline__ void st128(uint32_t addr, const uint32_t* v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
 __device__ __forceinline__ void st32(uint32_t addr, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 
 // An accumulator (two n-tiles of 16 rows) as the A operand of a product over its columns, with a scale per row (row g, row g + 8)
@@ -135,7 +138,7 @@ template <> __device__ __forceinline__ float2 raw_pair<__nv_bfloat16>(uint32_t u
 enum { T_A, T_R, T_B, T_K, T_M, FWD_TILES, T_AP = FWD_TILES, T_Q, BWD_TILES };
 enum { M_AK, M_RB, M_RK, M_X };                // 16 x 16 matrices side by side in T_M: A', A_rb, A_rk, A_ak
 struct ChunkHead {
-    float down[BWD_TILES], down_m[4], down_v, down_dy;
+    float down[BWD_TILES], down_m[4], down_in[6];   // of tiles, of the matrices in T_M, of b, k, a, r, v, dy as they come
     int t0, lo, hi, more;                      // steps t0 + lo .. t0 + hi - 1 of the sequence; more: the chunk goes on in this buffer
     int piece, advance;                        // piece: of one step of a steep chunk; advance: the state alone moves on (backward pass)
     alignas(16) float decay[N];                // exp(end)

@@ -40,31 +40,11 @@ __device__ __forceinline__ int seq_length(const WkvSeq& s, int b) {
 // without leaving the warp), four others prepare chunks ahead, each a whole one by itself, in a ring of four buffers.
 using namespace wkvc;
 constexpr int CHUNK_BUFS = 4, CHUNK_THREADS = (CHUNK_BUFS + 4) * 32;
+constexpr int CW_BYTES = (L + 1) * N * 4;   // log2 decays, summed up before the first step and after each one
 constexpr int HEAD_BYTES = (int)((sizeof(ChunkHead) + 127) / 128 * 128);
-constexpr int FWD_V = FWD_TILES * 2 * TILE, FWD_HEAD = FWD_V + TILE, FWD_BUF = FWD_HEAD + HEAD_BYTES;
+constexpr int FWD_V = FWD_TILES * 2 * TILE, FWD_CW = FWD_V + TILE, FWD_HEAD = FWD_CW + CW_BYTES, FWD_BUF = FWD_HEAD + HEAD_BYTES;
 
-// one vector of a chunk's steps: a lane has columns 2 lane, 2 lane + 1
-template <class E>
-struct Vec {
-    uint32_t raw[L];
-    __device__ __forceinline__ void load(const void* x, int64_t at, int64_t stride, int lo, int hi, int lane) {
-        const char* p = reinterpret_cast<const char*>(static_cast<const E*>(x) + at + 2 * lane);
-        const int64_t step = stride * 2;
-#pragma unroll
-        for (int t = 0; t < L; ++t) raw[t] = t >= lo && t < hi ? __ldg(reinterpret_cast<const uint32_t*>(p + t * step)) : 0u;
-    }
-    __device__ __forceinline__ void load(const WkvSeq& s, int which, int64_t b, int h, int t0, int lo, int hi, int lane) {
-        load(s.x[which], b * s.bs[which] + (int64_t)t0 * s.ss[which] + h * N, s.ss[which], lo, hi, lane);
-    }
-    __device__ __forceinline__ float top() const {
-        uint32_t m = 0;   // the order of non-negative floats is that of their bits
-#pragma unroll
-        for (int t = 0; t < L; ++t) m = __vmaxu2(m, raw[t] & 0x7fff7fffu);
-        const float2 f = raw_pair<E>(m);
-        return warp_top_abs(__uint_as_float(max(__float_as_uint(f.x), __float_as_uint(f.y))));   // (a NaN is the largest)
-    }
-};
-__device__ __forceinline__ uint32_t tile_pair(int t, int lane) { return (uint32_t)(t * 128 + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4); }
+__device__ __forceinline__ void prefetch_l2(const void* p, int bytes) { asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory"); }
 // asks for the rows of a later chunk
 __device__ __forceinline__ void prefetch_chunk(const WkvSeq& s, int64_t b, int h, int t0, int n_on, int lane) {
     const int t = lane & 15;
@@ -73,7 +53,7 @@ __device__ __forceinline__ void prefetch_chunk(const WkvSeq& s, int64_t b, int h
     for (int i = 0; i < 6; i += 2) {
         const int which = i + (lane >> 4);
         const char* p = static_cast<const char*>(s.x[which]) + 2 * (b * s.bs[which] + (int64_t)(t0 + t) * s.ss[which] + h * N);
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+        prefetch_l2(p, 2 * N);
     }
 }
 
@@ -81,38 +61,47 @@ __device__ __forceinline__ float log2_decay(float w) {   // of exp(-exp(w)); fin
     const float d = -expf(w) * 1.4426950408889634f;
     return d < -2000.f ? -2000.f : d;
 }
-// the log2 decays of a chunk, and whether it is steep
-template <class E>
-__device__ __forceinline__ bool load_decays(const WkvSeq& s, int64_t b, int h, int t0, int n_on, int lane, float2* lw) {
-    Vec<E> w;
-    w.load(s, 1, b, h, t0, 0, n_on, lane);
-    float2 sum = make_float2(0.f, 0.f);
+// One vector of a chunk's steps lo .. hi - 1, zeros at the others: a lane has eight columns (c8 = lane & 7) of steps lane >> 3, + 4, + 8, + 12. The loads are made for
+// all steps (the nearest one's in place of those that are not there), so that none waits for a branch.
+__device__ __forceinline__ void load_steps(uint4* u, const char* p, int64_t step, int lo, int hi, int lane) {
 #pragma unroll
-    for (int t = 0; t < L; ++t) {
-        const float2 f = raw_pair<E>(w.raw[t]);
-        lw[t] = t < n_on ? make_float2(log2_decay(f.x), log2_decay(f.y)) : make_float2(0.f, 0.f);
-        sum.x += lw[t].x, sum.y += lw[t].y;
+    for (int i = 0; i < 4; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(p + min(max((lane >> 3) + 4 * i, lo), hi - 1) * step));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int t = (lane >> 3) + 4 * i;
+        if (t < lo || t >= hi) u[i] = make_uint4(0, 0, 0, 0);
     }
-    return __any_sync(0xffffffffu, !(sum.x >= -STEEP_LOG2) || !(sum.y >= -STEEP_LOG2));
 }
-
-// Writes raw * 2^(exponent of the step) as hi and lo tiles; returns what its values are to be multiplied with. `head`: the exponents are of the sums before each step
-// (a), not after it; `sign` * (sum - from).
-template <class E, class X>
-__device__ __forceinline__ float put_tile(const Vec<E>& v, const float2* lw, uint32_t tile, int lane, float bound, X exponent) {
-    const Scale sc = scale_for(v.top() * bound);
-    float2 c = make_float2(0.f, 0.f);
+__device__ __forceinline__ const char* steps_of(const WkvSeq& s, int which, int64_t b, int h, int t0, int lane) {
+    return static_cast<const char*>(s.x[which]) + 2 * (b * s.bs[which] + (int64_t)t0 * s.ss[which] + h * N + 8 * (lane & 7));
+}
+// Sums of the log2 decays of a chunk's steps lo .. hi - 1 (of the others: 0) from the w in u, and whether they are steep.
+template <class E>
+__device__ __forceinline__ bool put_decays(const uint4* u, int lo, int hi, float* cws, int lane) {
+    const int c8 = lane & 7;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = (lane >> 3) + 4 * i;
+            const float2 x = raw_pair<E>(half ? u[i].z : u[i].x), y = raw_pair<E>(half ? u[i].w : u[i].y);
+            float4 d = make_float4(log2_decay(x.x), log2_decay(x.y), log2_decay(y.x), log2_decay(y.y));
+            if (t < lo || t >= hi) d = make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4*>(cws + (t + 1) * N + 8 * c8 + 4 * half) = d;
+        }
+    __syncwarp();
+    float2 c = make_float2(0.f, 0.f), d[L];
+    *reinterpret_cast<float2*>(cws + 2 * lane) = c;
+#pragma unroll
+    for (int t = 0; t < L; ++t) d[t] = *reinterpret_cast<const float2*>(cws + (t + 1) * N + 2 * lane);
 #pragma unroll
     for (int t = 0; t < L; ++t) {
-        const float2 before = c;
-        c.x += lw[t].x, c.y += lw[t].y;
-        const float2 f = raw_pair<E>(v.raw[t]);
-        uint32_t hi, lo;
-        split(f.x * sc.up * ex2_(exponent(before.x, c.x, 0)), f.y * sc.up * ex2_(exponent(before.y, c.y, 1)), hi, lo);
-        st32(tile + tile_pair(t, lane), hi);
-        st32(tile + TILE + tile_pair(t, lane), lo);
+        c.x += d[t].x, c.y += d[t].y;
+        *reinterpret_cast<float2*>(cws + (t + 1) * N + 2 * lane) = c;
     }
-    return sc.down;
+    const bool steep = __any_sync(0xffffffffu, !(c.x >= -STEEP_LOG2) || !(c.y >= -STEEP_LOG2));
+    __syncwarp();
+    return steep;
 }
 __device__ __forceinline__ float acc_top(const float (*c)[4]) {
     float m = 0.f;
@@ -191,97 +180,134 @@ __device__ __forceinline__ float invert(float* work, Frag& f, float (*v)[4], int
     return sc.down;
 }
 
-// a vector's values as they are, in one fp16 each, scaled to the tile's largest (exact down to 2^-27 of it)
-template <class E>
-__device__ __forceinline__ float put_exact(const Vec<E>& v, uint32_t tile, int lane) {
-    const Scale sc = scale_for(v.top());
-#pragma unroll
-    for (int t = 0; t < L; ++t) {
-        const float2 f = raw_pair<E>(v.raw[t]);
-        st32(tile + tile_pair(t, lane), pack_half(f.x * sc.up, f.y * sc.up));
-    }
-    return sc.down;
-}
-
-// values in bf16: one where the input's type is that, else two
-template <class E>
-__device__ __forceinline__ void put_bf16(const Vec<E>& v, uint32_t tile, int lane) {
-#pragma unroll
-    for (int t = 0; t < L; ++t) {
-        if (std::is_same<E, __nv_bfloat16>::value) {
-            st32(tile + tile_pair(t, lane), v.raw[t]);
-        } else {
-            const float2 f = raw_pair<E>(v.raw[t]);
-            uint32_t hi, lo;
-            split_bf16(f.x, f.y, hi, lo);
-            st32(tile + tile_pair(t, lane), hi);
-            st32(tile + TILE + tile_pair(t, lane), lo);
-        }
-    }
-}
-// Prepares steps lo .. hi - 1 of a chunk; lw: log2 decays, zero at the other steps. at: the buffer's tiles; v: where v goes. BWD: Q and v in bf16 (v16) are kept too.
+// Prepares steps lo .. hi - 1 of a chunk whose decays are in cws. at: the buffer's tiles; v, dy: where those go, in one fp16 each (exact down to 2^-27 of the largest);
+// v16, dy16: in bf16. BWD: dy, Q and the tile of a are kept too.
+// The code is kept short, in loops: a warp runs through it once per chunk, and unrolled (4000 instructions) it waited for them most of the time (a chunk took it 28000
+// cycles).
 template <class E, bool BWD>
-__device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h, int t0, int lo, int hi, bool piece, const float2* lw, uint32_t at, uint32_t v, uint32_t v16,
-                                              ChunkHead* head, int lane) {
-    constexpr int AP = BWD ? T_AP : T_A;
-    const uint32_t tA = at + T_A * 2 * TILE, tR = at + T_R * 2 * TILE, tB = at + T_B * 2 * TILE, tK = at + T_K * 2 * TILE, tM = at + T_M * 2 * TILE, tAP = at + AP * 2 * TILE;
-    float down_b, down_k, down_a, down_r;
-    {
-        float2 end = make_float2(0.f, 0.f);
+__device__ __forceinline__ void prepare_chunk(const WkvSeq& s, const WkvBackward* bwd, int64_t b, int h, int t0, int lo, int hi, bool piece, uint32_t at, uint32_t v, uint32_t v16,
+                                              const float* cws, ChunkHead* head, int lane) {
+    constexpr int AP = BWD ? T_AP : T_A, VECTORS = BWD ? 6 : 5;
+    const uint32_t tA = at + T_A * 2 * TILE, tM = at + T_M * 2 * TILE, tAP = at + AP * 2 * TILE;
+    const int c8 = lane & 7, tr = lane >> 3;
+    auto load = [&](uint4* u, int vec) {   // b, k, a, r, v, dy
+        if (BWD && vec == 5) {
+            if (bwd->dy) {
+                load_steps(u, static_cast<const char*>(bwd->dy) + 2 * (b * bwd->dy_batch_stride + (int64_t)t0 * bwd->dy_step_stride + h * N + 8 * c8), 2 * bwd->dy_step_stride, lo, hi, lane);
+            } else {
 #pragma unroll
-        for (int t = 0; t < L; ++t) end.x += lw[t].x, end.y += lw[t].y;
-        Vec<E> x, y;   // (a vector is on its way while the one before it is worked on)
-        auto to_end = [&](float, float c, int i) { return (i ? end.y : end.x) - c; };   // at most 0
-        x.load(s, 5, b, h, t0, lo, hi, lane);
-        y.load(s, 2, b, h, t0, lo, hi, lane);
-        down_b = put_tile(x, lw, tB, lane, 1.f, to_end);
-        x.load(s, 4, b, h, t0, lo, hi, lane);
-        down_k = put_tile(y, lw, tK, lane, 1.f, to_end);
-        y.load(s, 0, b, h, t0, lo, hi, lane);
-        // a's and r's factors are at most `grow` (2^STEEP_LOG2); in a piece of one step they are 1
-        const float grow = piece ? 1.f : ex2_(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(-fminf(end.x, end.y), 0.f)))));
-        down_a = put_tile(x, lw, tA, lane, grow, [&](float c, float, int i) { return piece ? 0.f : c - (i ? end.y : end.x); });
-        x.load(s, 3, b, h, t0, lo, hi, lane);
-        down_r = put_tile(y, lw, tR, lane, grow, [&](float, float c, int i) { return piece ? 0.f : c - (i ? end.y : end.x); });
-        const float down_v = put_exact(x, v, lane);
-        if (BWD) put_bf16(x, v16, lane);
-        *reinterpret_cast<float2*>(head->decay + 2 * lane) = make_float2(ex2_(end.x), ex2_(end.y));
-        if (lane == 0) head->down_v = down_v;
+                for (int i = 0; i < 4; ++i) u[i] = make_uint4(0, 0, 0, 0);
+            }
+            return;
+        }
+        const int which = vec == 0 ? 5 : vec == 1 ? 2 : vec == 2 ? 4 : vec == 3 ? 0 : 3;
+        load_steps(u, steps_of(s, which, b, h, t0, lane), 2 * s.ss[which], lo, hi, lane);
+    };
+    uint4 x[4], next[4];   // (a vector is on its way while the one before it is worked on)
+    load(x, 0);
+    const float2 end2 = *reinterpret_cast<const float2*>(cws + L * N + 2 * lane);
+    *reinterpret_cast<float2*>(head->decay + 2 * lane) = make_float2(ex2_(end2.x), ex2_(end2.y));
+    // a's and r's factors are at most `grow` (2^STEEP_LOG2), b's and k's at most 1; in a piece of one step all are 1
+    const int grow_by = piece ? 0 : (int)ceilf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(-fminf(end2.x, end2.y), 0.f)))));
+    const float grow = __int_as_float((127 + min(grow_by, (int)STEEP_LOG2)) << 23);
+    auto up_of = [](float down) { return __uint_as_float((254u << 23) - __float_as_uint(down)); };   // of a power of two
+    float end[8];
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(cws + L * N + 8 * c8 + i);
+        end[i] = f.x, end[i + 1] = f.y, end[i + 2] = f.z, end[i + 3] = f.w;
+    }
+#pragma unroll 1
+    for (int vec = 0; vec < VECTORS; ++vec) {
+        if (vec + 1 < VECTORS) load(next, vec + 1);
+        uint32_t m = 0;   // the order of non-negative floats is that of their bits
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            m = __vmaxu2(__vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu), __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)), m);
+        const float2 f = raw_pair<E>(m);
+        const Scale sc = scale_for(warp_top_abs(__uint_as_float(max(__float_as_uint(f.x), __float_as_uint(f.y)))) * (vec == 2 || vec == 3 ? grow : 1.f));   // (a NaN is the largest)
+        if (vec < 4) {
+            const int which = vec == 0 ? T_B : vec == 1 ? T_K : vec == 2 ? T_A : T_R;
+            const float sign = vec < 2 ? -1.f : piece ? 0.f : 1.f;
+            const uint32_t tile = at + which * 2 * TILE;
+            if (lane == 0) head->down[which] = sc.down;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = tr + 4 * i;
+                const float* cw = cws + (t + (vec != 2)) * N + 8 * c8;   // a: before the step
+                const float4 w0 = *reinterpret_cast<const float4*>(cw), w1 = *reinterpret_cast<const float4*>(cw + 4);
+                const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+                const uint32_t* raw = &x[i].x;
+                uint32_t hi4[4], lo4[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float2 e = raw_pair<E>(raw[c]);
+                    split(e.x * sc.up * ex2_((w[2 * c] - end[2 * c]) * sign), e.y * sc.up * ex2_((w[2 * c + 1] - end[2 * c + 1]) * sign), hi4[c], lo4[c]);
+                }
+                const uint32_t to = tile + t * 128 + ((c8 ^ (t & 7)) << 4);
+                st128(to, hi4);
+                st128(to + TILE, lo4);
+            }
+        } else {
+            if (lane == 0) head->down_in[vec] = sc.down;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = tr + 4 * i;
+                const uint32_t* raw = &x[i].x;
+                const uint32_t to = t * 128 + ((c8 ^ (t & 7)) << 4);
+                uint32_t h4[4], b4[4], l4[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float2 e = raw_pair<E>(raw[c]);
+                    h4[c] = pack_half(e.x * sc.up, e.y * sc.up);
+                    if (BWD && !std::is_same<E, __nv_bfloat16>::value) split_bf16(e.x, e.y, b4[c], l4[c]);
+                }
+                st128(v + (vec - 4) * TILE + to, h4);
+                if (BWD) {
+                    if (std::is_same<E, __nv_bfloat16>::value) {
+                        st128(v16 + (vec - 4) * 2 * TILE + to, raw);
+                    } else {
+                        st128(v16 + (vec - 4) * 2 * TILE + to, b4);
+                        st128(v16 + (vec - 4) * 2 * TILE + TILE + to, l4);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = next[i];
     }
     __syncwarp();
-    {
-        float ab[2][4], ak[2][4], rb[2][4], rk[2][4];
-        zero2(ab), zero2(ak), zero2(rb), zero2(rk);
+    const int g = lane >> 2, q = lane & 3;
+#pragma unroll 1
+    for (int m = 0; m < 4; ++m) {   // A_ab, A_ak, A_rb, A_rk
+        const int ta = m < 2 ? T_A : T_R, tb = m & 1 ? T_K : T_B;
+        float c[2][4];
+        zero2(c);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
-            Frag fb, fk, f;
-            load_frag(fb, tB, kk * 16, lane, load_b);
-            load_frag(fk, tK, kk * 16, lane, load_b);
-            load_frag(f, tA, kk * 16, lane, load_a);
-            mma3(ab, f, fb);
-            mma3(ak, f, fk);
-            load_frag(f, tR, kk * 16, lane, load_a);
-            mma3(rb, f, fb);
-            mma3(rk, f, fk);
+            Frag f, w;
+            load_frag(f, at + ta * 2 * TILE, kk * 16, lane, load_a);
+            load_frag(w, at + tb * 2 * TILE, kk * 16, lane, load_b);
+            mma3(c, f, w);
         }
-        keep_lower(ab, down_a, down_b, 1, lane);
-        keep_lower(ak, down_a, down_k, 1, lane);
-        keep_lower(rb, down_r, down_b, 0, lane);
-        keep_lower(rk, down_r, down_k, 0, lane);
-        const int g = lane >> 2, q = lane & 3;
+        keep_lower(c, head->down[ta], head->down[tb], m < 2 ? 1 : 0, lane);
+        if (m == 0) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) *reinterpret_cast<float2*>(head->work + (g + 8 * half) * L + 8 * n + 2 * q) = make_float2(ab[n][2 * half], ab[n][2 * half + 1]);
-        const float dx = put_block(ak, tM, M_X * L, lane), d1 = put_block(rb, tM, M_RB * L, lane), d2 = put_block(rk, tM, M_RK * L, lane);
-        if (lane == 0) head->down_m[M_X] = dx, head->down_m[M_RB] = d1, head->down_m[M_RK] = d2;
+                for (int half = 0; half < 2; ++half) *reinterpret_cast<float2*>(head->work + (g + 8 * half) * L + 8 * n + 2 * q) = make_float2(c[n][2 * half], c[n][2 * half + 1]);
+        } else {
+            const int block = m == 1 ? M_X : m == 2 ? M_RB : M_RK;
+            const float d = put_block(c, tM, block * L, lane);
+            if (lane == 0) head->down_m[block] = d;
+        }
     }
     __syncwarp();
-    Frag q;
+    Frag qf;
     float qv[2][4];
-    const float down_q = invert(head->work, q, qv, lane);
+    const float down_q = invert(head->work, qf, qv, lane);
     if (BWD) {
-        put_acc(qv, at + T_Q * 2 * TILE, 0, 1.f / down_q, lane);
+        put_acc(qv, at + T_Q * 2 * TILE, 0, up_of(down_q), lane);
         if (lane == 0) head->down[T_Q] = down_q;
     }
     float ap[4][2][4], akp[2][4], top = 0.f;
@@ -289,7 +315,7 @@ __device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h,
     {
         Frag f;
         load_frag(f, tM, M_X * L, lane, load_bt);
-        mma3(akp, q, f);
+        mma3(akp, qf, f);
         const float e = head->down_m[M_X];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -301,20 +327,17 @@ __device__ __forceinline__ void prepare_chunk(const WkvSeq& s, int64_t b, int h,
         Frag f;
         zero2(ap[jj]);
         load_frag(f, tA, jj * 16, lane, load_bt);
-        mma3(ap[jj], q, f);
+        mma3(ap[jj], qf, f);
         top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(acc_top(ap[jj]))));
     }
+    const float down_a = head->down[T_A];
     const Scale sa = scale_for(warp_top_abs(top));
     __syncwarp();
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) put_acc(ap[jj], tAP, jj * 16, sa.up, lane);
     const float dak = put_block(akp, tM, M_AK * L, lane);
     if (lane == 0) {
-        if (BWD) head->down[T_A] = down_a;
         head->down[AP] = sa.down * down_a * down_q;
-        head->down[T_R] = down_r;
-        head->down[T_B] = down_b;
-        head->down[T_K] = down_k;
         head->down_m[M_AK] = dak;
     }
 }
@@ -394,7 +417,7 @@ __device__ __forceinline__ void chunk_rows(float (*S)[4], float (*y)[4], uint32_
     scale_acc(y, s0, s1, head->down[T_R]);
     uint32_t fv[4];
     load_at(fv, v, i0, lane);
-    const float dv = head->down_v;
+    const float dv = head->down_in[4];
     float x[2][4];
     Frag g;
     zero2(x);
@@ -524,24 +547,25 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const _
         const int buf = warp - 4;
         const uint32_t at = smem_u32(smem) + buf * FWD_BUF;
         ChunkHead* head = reinterpret_cast<ChunkHead*>(smem + buf * FWD_BUF + FWD_HEAD);
+        float* cws = reinterpret_cast<float*>(smem + buf * FWD_BUF + FWD_CW);
         int uses = 0;
         bool ok = true;
         for (int n = buf; n < chunks && ok; n += CHUNK_BUFS) {
             const int t0 = n * L, n_on = min(L, n_steps - t0);
             if (n + CHUNK_BUFS < chunks) prefetch_chunk(s, b, h, t0 + CHUNK_BUFS * L, min(L, n_steps - t0 - CHUNK_BUFS * L), lane);
             for (int i = 0, pieces = 1; i < pieces; ++i) {
-                float2 lw[L];
-                const bool steep = load_decays<E>(s, b, h, t0, n_on, lane, lw);
-                if (steep) {
-                    pieces = n_on;
-#pragma unroll
-                    for (int t = 0; t < L; ++t) lw[t] = t == i ? lw[t] : make_float2(0.f, 0.f);
-                }
                 if (uses > 0) ok = wait_for(&vacant[buf], (uint32_t)(uses - 1) & 1u);
                 if (!ok) break;
                 ++uses;
+                uint4 w[4];
+                load_steps(w, steps_of(s, 1, b, h, t0, lane), 2 * s.ss[1], 0, n_on, lane);
+                const bool steep = put_decays<E>(w, 0, n_on, cws, lane);
+                if (steep) {
+                    pieces = n_on;
+                    put_decays<E>(w, i, i + 1, cws, lane);
+                }
                 const int lo = steep ? i : 0, hi = steep ? i + 1 : n_on;
-                prepare_chunk<E, false>(s, b, h, t0, lo, hi, steep, lw, at, at + FWD_V, 0u, head, lane);
+                prepare_chunk<E, false>(s, nullptr, b, h, t0, lo, hi, steep, at, at + FWD_V, 0u, cws, head, lane);
                 if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = i + 1 < pieces ? hi : L, head->more = i + 1 < pieces, head->piece = steep;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf]);
@@ -559,7 +583,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const _
 // work out the sums over rows: the gradients of r, a, b, k and the decays. Three warps prepare chunks ahead as in the forward pass.
 constexpr int BWD_BUFS = 3, BWD_WARPS = 8 + BWD_BUFS;
 constexpr int BWD_V = BWD_TILES * 2 * TILE, BWD_DY = BWD_V + TILE, BWD_V16 = BWD_DY + TILE, BWD_DY16 = BWD_V16 + 2 * TILE, BWD_CW = BWD_DY16 + 2 * TILE,
-              BWD_HEAD = BWD_CW + L * N * 4, BWD_BUF = BWD_HEAD + HEAD_BYTES;
+              BWD_HEAD = BWD_CW + CW_BYTES, BWD_BUF = BWD_HEAD + HEAD_BYTES;
 // what crosses: states 64 x 64 (bf16, hi and lo), slabs of u and h, the 16 x 16 matrices P (fp16), column sums of G o S_E by row warp
 constexpr int BIG = N * N * 2, X_S = 0, X_G = X_S + 2 * BIG, X_U = X_G + 2 * BIG, X_H = X_U + 2 * SLAB, X_P = X_H + 2 * SLAB, X_SUM = X_P + 2 * TILE, X_BYTES = X_SUM + 4 * N * 4;
 constexpr int BWD_SMEM = BWD_BUFS * BWD_BUF + X_BYTES;
@@ -708,7 +732,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 scale_acc(xk, s0, s1, head->down[T_K]);
                 uint32_t fdy[4];
                 load_at(fdy, at + BWD_DY, i0, lane);
-                const float ddy = head->down_dy;
+                const float ddy = head->down_in[5];
                 zero2(z);
                 load_frag(w, tM, M_RB * L, lane, load_bt);
                 mma2(z, fdy, w);
@@ -744,7 +768,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 zero2(z);
                 load_frag(w, tM, M_AK * L, lane, load_b);
                 mma2(z, fv, w);
-                add_acc(u, z, head->down_v * head->down_m[M_AK]);
+                add_acc(u, z, head->down_in[4] * head->down_m[M_AK]);
                 const float2 gs = column_sums(G, S, head->decay, piece, lane);
                 // to the column warps
                 if (items > 0) ok = wait_for(&x_vacant, (uint32_t)(items - 1) & 1u);
@@ -853,7 +877,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 {   // one of the four matrices P: (dy, h) by (u, v)
                     float m[2][4];
                     zero2(m);
-#pragma unroll
+#pragma unroll 1
                     for (int kk = 0; kk < 4; ++kk) {
                         Frag f, w;
                         if (cw < 2) input(f, dyt, kk * 16, load_a);
@@ -873,7 +897,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 }
                 float dr[2][4], da[2][4], db[2][4], dk[2][4];
                 zero2(dr), zero2(da), zero2(db), zero2(dk);
-#pragma unroll
+#pragma unroll 1
                 for (int kk = 0; kk < 4; ++kk) {
                     Frag f, w;
                     load_bt(w.hi, x + X_S + kk * 2048, c0, lane);
@@ -902,20 +926,21 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                     mma3(z, f, w);
                     add_acc(c, z, d * p_down[block]);
                 };
-                {
+#pragma unroll 1
+                for (int i = 0; i < 2; ++i) {
                     Frag w;
-                    load_frag(w, tB, c0, lane, load_bt);
-                    times(pr, 0, w, head->down[T_B], load_a);
-                    times(pa, 2, w, head->down[T_B], load_a);
-                    load_frag(w, tK, c0, lane, load_bt);
-                    times(pr, 1, w, head->down[T_K], load_a);
-                    times(pa, 3, w, head->down[T_K], load_a);
-                    load_frag(w, tR, c0, lane, load_bt);
-                    times(pb, 0, w, head->down[T_R], load_at);
-                    times(pk, 1, w, head->down[T_R], load_at);
-                    load_frag(w, tA, c0, lane, load_bt);
-                    times(pb, 2, w, head->down[T_A], load_at);
-                    times(pk, 3, w, head->down[T_A], load_at);
+                    const float d = head->down[i ? T_K : T_B];
+                    load_frag(w, i ? tK : tB, c0, lane, load_bt);
+                    times(pr, i, w, d, load_a);
+                    times(pa, 2 + i, w, d, load_a);
+                }
+#pragma unroll 1
+                for (int i = 0; i < 2; ++i) {
+                    Frag w;
+                    const float d = head->down[i ? T_A : T_R];
+                    load_frag(w, i ? tA : tR, c0, lane, load_bt);
+                    times(pb, 2 * i, w, d, load_at);
+                    times(pk, 2 * i + 1, w, d, load_at);
                 }
                 float2 gs[2];
 #pragma unroll
@@ -932,14 +957,13 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int j = c0 + 8 * i + 2 * q;
-                    const float2 end = *reinterpret_cast<const float2*>(cws + 15 * N + j);
+                    const float2 end = *reinterpret_cast<const float2*>(cws + L * N + j);
                     float pos[2][2], posa[2][2], flow[2][2], lw[2][2];   // [column][half]
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const int t = g + 8 * half;
                         const bool on = t >= lo && t < min(hi, n_on);
-                        const float2 c = *reinterpret_cast<const float2*>(cws + t * N + j);
-                        const float2 c1 = t ? *reinterpret_cast<const float2*>(cws + (t - 1) * N + j) : make_float2(0.f, 0.f);
+                        const float2 c = *reinterpret_cast<const float2*>(cws + (t + 1) * N + j), c1 = *reinterpret_cast<const float2*>(cws + t * N + j);   // after it, before it
                         const float2 r = raw_pair<E>(raw[0][i][half]), wv = raw_pair<E>(raw[1][i][half]), k = raw_pair<E>(raw[2][i][half]);
                         const float2 a = raw_pair<E>(raw[3][i][half]), bb = raw_pair<E>(raw[4][i][half]);
                         float out[5][2];   // r, w, k, a, b
@@ -994,37 +1018,29 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
         int uses = 0;
         for (int n = chunks - 1 - buf; n >= 0 && ok; n -= BWD_BUFS) {
             const int t0 = n * L, n_on = min(L, n_steps - t0);
-            if (n >= BWD_BUFS) prefetch_chunk(s, b, h, t0 - BWD_BUFS * L, L, lane);
+            if (n >= BWD_BUFS) {
+                const int t1 = t0 - BWD_BUFS * L;
+                prefetch_chunk(s, b, h, t1, L, lane);
+                if (p.g.dy && lane < L) prefetch_l2(static_cast<const char*>(p.g.dy) + 2 * (b * p.g.dy_batch_stride + (int64_t)(t1 + lane) * p.g.dy_step_stride + h * N), 2 * N);
+                if (lane == L) prefetch_l2(s.ckpt + ((size_t)bh * s.n_chunks + n - BWD_BUFS) * 4096, 16384);
+            }
             // a steep chunk: for each step from the last one, the steps before it for the state's sake, and then the step itself
             for (int i = 0, j = 0, last = 0, started = 0; !last && ok;) {
-                float2 lw[L];
-                const bool steep = load_decays<E>(s, b, h, t0, n_on, lane, lw);
-                if (!started) i = steep ? n_on - 1 : 0, started = 1;
-                const bool advance = steep && j < i;
-                const int step = advance ? j : i;
-                if (steep) {
-#pragma unroll
-                    for (int t = 0; t < L; ++t) lw[t] = t == step ? lw[t] : make_float2(0.f, 0.f);
-                }
-                last = !steep || (i == 0 && !advance);
                 if (uses > 0) ok = wait_for(&vacant[buf], (uint32_t)(uses - 1) & 1u);
                 if (!ok) break;
                 ++uses;
+                uint4 w[4];
+                load_steps(w, steps_of(s, 1, b, h, t0, lane), 2 * s.ss[1], 0, n_on, lane);
+                const bool steep = put_decays<E>(w, 0, n_on, cws, lane);
+                if (!started) i = steep ? n_on - 1 : 0, started = 1;
+                const bool advance = steep && j < i;
+                const int step = advance ? j : i;
+                if (steep) put_decays<E>(w, step, step + 1, cws, lane);
+                last = !steep || (i == 0 && !advance);
                 const int lo = steep ? step : 0, hi = steep ? step + 1 : n_on;
-                float2 c = make_float2(0.f, 0.f);
-#pragma unroll
-                for (int t = 0; t < L; ++t) {
-                    c.x += lw[t].x, c.y += lw[t].y;
-                    *reinterpret_cast<float2*>(cws + t * N + 2 * lane) = c;
-                }
-                Vec<E> v;
-                v.load(p.g.dy, b * p.g.dy_batch_stride + (int64_t)t0 * p.g.dy_step_stride + h * N, p.g.dy_step_stride, lo, p.g.dy ? hi : lo, lane);
-                const float down_dy = put_exact(v, at + BWD_DY, lane);
-                put_bf16(v, at + BWD_DY16, lane);
-                prepare_chunk<E, true>(s, b, h, t0, lo, hi, steep, lw, at, at + BWD_V, at + BWD_V16, head, lane);
+                prepare_chunk<E, true>(s, &p.g, b, h, t0, lo, hi, steep, at, at + BWD_V, at + BWD_V16, cws, head, lane);
                 if (lane == 0) {
                     head->t0 = t0, head->lo = lo, head->hi = step + 1 == n_on || !steep ? L : hi, head->more = !last, head->piece = steep, head->advance = advance;
-                    head->down_dy = down_dy;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf]);

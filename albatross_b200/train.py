@@ -47,10 +47,10 @@ def _dense_last(t: torch.Tensor) -> torch.Tensor:
 
 
 def _steps(t: torch.Tensor) -> torch.Tensor:
-    """[B, T, C] with a dense last dimension and every step on a 4-byte boundary."""
-    if t.stride(2) == 1 and not (t.stride(0) | t.stride(1)) & 1 and not t.data_ptr() & 3:
+    """[B, T, C] with a dense last dimension and every step on a 16-byte boundary."""
+    if t.stride(2) == 1 and not (t.stride(0) | t.stride(1)) & 7 and not t.data_ptr() & 15:
         return t
-    return t.contiguous() if not (t.is_contiguous() and t.data_ptr() & 3) else t.clone()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _needs_grad(*tensors) -> bool:

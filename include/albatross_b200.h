@@ -172,7 +172,7 @@ int ab_glue_selftest(int which, uint64_t first, uint64_t n, uint64_t* differ, vo
  * operator of ab_wkv7_fwd, out of place, in two types, with strides and sequences of unequal length. */
 typedef struct ab_wkv7_seq {
     int32_t dtype, B, T, H;      /* AB_DT_F16 or AB_DT_BF16; T may be 0 */
-    const void* x[6];            /* r, w, k, v, a, b: [B, T, 64 H] of dtype, the last dimension dense, every step on a 4-byte boundary */
+    const void* x[6];            /* r, w, k, v, a, b: [B, T, 64 H] of dtype, the last dimension dense, every step on a 16-byte boundary */
     int64_t batch_stride[6], step_stride[6];   /* elements between sequences, and between steps */
     const float* state;          /* [B, H, 64, 64] dense, before the first step; NULL: zeros */
     const int32_t* lengths;      /* [B] or NULL: sequence b has lengths[b] steps (taken into 0 .. T); what x holds behind them is not used */

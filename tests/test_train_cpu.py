@@ -47,11 +47,11 @@ def test_recurrence_refuses_missing_or_crooked_pointers():
     s.x[4] = None
     assert _fwd(s) == -1
     s = _seq()
-    s.x[2] = P + 2
+    s.x[2] = P + 8
     assert _fwd(s) == -1
     s = _seq()
-    s.step_stride[5] = 191
-    assert _fwd(s) == -1 and b"4-byte" in _lib.lib.ab_last_error()
+    s.step_stride[5] = 196
+    assert _fwd(s) == -1 and b"16-byte" in _lib.lib.ab_last_error()
     assert _fwd(_seq(), y=None) == -1 and _fwd(_seq(), out=None) == -1 and _fwd(_seq(), y=P + 8) == -1
     assert _bwd(_seq(checkpoints=None)) == -1 and _bwd(_seq(), dx=[P, P, P + 2, P, P, P]) == -1 and _bwd(_seq(), dy=P + 1) == -1
 

@@ -40,44 +40,54 @@ __device__ __forceinline__ int seq_length(const WkvSeq& s, int b) {
 // without leaving the warp), four others prepare chunks ahead, each a whole one by itself, in a ring of four buffers.
 using namespace wkvc;
 constexpr int CHUNK_BUFS = 4, CHUNK_THREADS = (CHUNK_BUFS + 4) * 32;
-constexpr int CW_BYTES = (L + 1) * N * 4;   // log2 decays, summed up before the first step and after each one
+constexpr int FE_BYTES = (L + 1) * N * 4;   // factors relative to the chunk's end (put_factors)
 constexpr int HEAD_BYTES = (int)((sizeof(ChunkHead) + 127) / 128 * 128);
-constexpr int FWD_V = FWD_TILES * 2 * TILE, FWD_CW = FWD_V + TILE, FWD_HEAD = FWD_CW + CW_BYTES, FWD_BUF = FWD_HEAD + HEAD_BYTES;
+constexpr int FWD_V = FWD_TILES * 2 * TILE, FWD_FE = FWD_V + TILE, FWD_HEAD = FWD_FE + FE_BYTES, FWD_BUF = FWD_HEAD + HEAD_BYTES;
 
-__device__ __forceinline__ void prefetch_l2(const void* p, int bytes) { asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory"); }
-// asks for the rows of a later chunk
-__device__ __forceinline__ void prefetch_chunk(const WkvSeq& s, int64_t b, int h, int t0, int n_on, int lane) {
-    const int t = lane & 15;
-    if (t >= n_on) return;
+// Asks for the rows of a later chunk, 32 bytes a lane. (One bulk request per row takes the warp some 50 cycles each.)
+__device__ __forceinline__ void prefetch_steps(const void* x, int64_t at, int64_t step, int n_on, int lane) {
 #pragma unroll
-    for (int i = 0; i < 6; i += 2) {
-        const int which = i + (lane >> 4);
-        const char* p = static_cast<const char*>(s.x[which]) + 2 * (b * s.bs[which] + (int64_t)(t0 + t) * s.ss[which] + h * N);
-        prefetch_l2(p, 2 * N);
+    for (int i = 0; i < 2; ++i) {
+        const int t = (lane >> 2) + 8 * i;
+        if (t < n_on) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(x) + 2 * (at + t * step) + (lane & 3) * 32));
     }
+}
+__device__ __forceinline__ void prefetch_chunk(const WkvSeq& s, int64_t b, int h, int t0, int n_on, int lane) {
+#pragma unroll 1
+    for (int i = 0; i < 6; ++i) prefetch_steps(s.x[i], b * s.bs[i] + (int64_t)t0 * s.ss[i] + h * N, s.ss[i], n_on, lane);
 }
 
 __device__ __forceinline__ float log2_decay(float w) {   // of exp(-exp(w)); finite (2^-2000 is 0 all the same), but for NaN
     const float d = -expf(w) * 1.4426950408889634f;
     return d < -2000.f ? -2000.f : d;
 }
-// One vector of a chunk's steps lo .. hi - 1, zeros at the others: a lane has eight columns (c8 = lane & 7) of steps lane >> 3, + 4, + 8, + 12. The loads are made for
-// all steps (the nearest one's in place of those that are not there), so that none waits for a branch.
-__device__ __forceinline__ void load_steps(uint4* u, const char* p, int64_t step, int lo, int hi, int lane) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(p + min(max((lane >> 3) + 4 * i, lo), hi - 1) * step));
+// Asks for one vector of a chunk's steps lo .. hi - 1 (zeros at the others) in a tile's place: a lane has eight columns (c8 = lane & 7) of steps lane >> 3, + 4, + 8,
+// + 12, here and when it takes them up again. All vectors of a chunk are on their way at once: one after the other they cost a warp 2000 cycles each.
+__device__ __forceinline__ void stage_steps(uint32_t tile, const char* p, int64_t step, int lo, int hi, bool there, int lane) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int t = (lane >> 3) + 4 * i;
-        if (t < lo || t >= hi) u[i] = make_uint4(0, 0, 0, 0);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + t * 128 + (((lane & 7) ^ (t & 7)) << 4)), "l"(p + (there ? min(max(t, lo), hi - 1) * step : 0)),
+                     "r"(there && t >= lo && t < hi ? 16 : 0) : "memory");
     }
 }
+__device__ __forceinline__ void staged(uint4* u, uint32_t tile, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int t = (lane >> 3) + 4 * i;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[i].x), "=r"(u[i].y), "=r"(u[i].z), "=r"(u[i].w) : "r"(tile + t * 128 + (((lane & 7) ^ (t & 7)) << 4)) : "memory");
+    }
+}
+template <int N_LEFT>
+__device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N_LEFT) : "memory"); }
+__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ const char* steps_of(const WkvSeq& s, int which, int64_t b, int h, int t0, int lane) {
     return static_cast<const char*>(s.x[which]) + 2 * (b * s.bs[which] + (int64_t)t0 * s.ss[which] + h * N + 8 * (lane & 7));
 }
-// Sums of the log2 decays of a chunk's steps lo .. hi - 1 (of the others: 0) from the w in u, and whether they are steep.
+// From the w of a chunk's steps lo .. hi - 1 (the others' decays are 1): whether they are steep; if they are not, or if they are a piece's (piece), the factors of the
+// steps. fe: [L + 1][N], exp(sum before and including the steps up to a row's - end), a row for no step first; fb: [L][N], exp(end - sum); decay: exp(end). In a piece fe is 1.
 template <class E>
-__device__ __forceinline__ bool put_decays(const uint4* u, int lo, int hi, float* cws, int lane) {
+__device__ __forceinline__ bool put_factors(const uint4* u, int lo, int hi, bool piece, float* fe, float* fb, float* decay, int lane) {
     const int c8 = lane & 7;
 #pragma unroll 1
     for (int half = 0; half < 2; ++half)
@@ -87,19 +97,25 @@ __device__ __forceinline__ bool put_decays(const uint4* u, int lo, int hi, float
             const float2 x = raw_pair<E>(half ? u[i].z : u[i].x), y = raw_pair<E>(half ? u[i].w : u[i].y);
             float4 d = make_float4(log2_decay(x.x), log2_decay(x.y), log2_decay(y.x), log2_decay(y.y));
             if (t < lo || t >= hi) d = make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(cws + (t + 1) * N + 8 * c8 + 4 * half) = d;
+            *reinterpret_cast<float4*>(fe + (t + 1) * N + 8 * c8 + 4 * half) = d;
         }
     __syncwarp();
     float2 c = make_float2(0.f, 0.f), d[L];
-    *reinterpret_cast<float2*>(cws + 2 * lane) = c;
-#pragma unroll
-    for (int t = 0; t < L; ++t) d[t] = *reinterpret_cast<const float2*>(cws + (t + 1) * N + 2 * lane);
 #pragma unroll
     for (int t = 0; t < L; ++t) {
-        c.x += d[t].x, c.y += d[t].y;
-        *reinterpret_cast<float2*>(cws + (t + 1) * N + 2 * lane) = c;
+        const float2 x = *reinterpret_cast<const float2*>(fe + (t + 1) * N + 2 * lane);
+        c.x += x.x, c.y += x.y;
+        d[t] = c;
     }
     const bool steep = __any_sync(0xffffffffu, !(c.x >= -STEEP_LOG2) || !(c.y >= -STEEP_LOG2));
+    if (steep && !piece) return true;
+    *reinterpret_cast<float2*>(decay + 2 * lane) = make_float2(ex2_(c.x), ex2_(c.y));
+    *reinterpret_cast<float2*>(fe + 2 * lane) = piece ? make_float2(1.f, 1.f) : make_float2(ex2_(-c.x), ex2_(-c.y));
+#pragma unroll
+    for (int t = 0; t < L; ++t) {
+        *reinterpret_cast<float2*>(fe + (t + 1) * N + 2 * lane) = piece ? make_float2(1.f, 1.f) : make_float2(ex2_(d[t].x - c.x), ex2_(d[t].y - c.y));
+        *reinterpret_cast<float2*>(fb + t * N + 2 * lane) = make_float2(ex2_(c.x - d[t].x), ex2_(c.y - d[t].y));
+    }
     __syncwarp();
     return steep;
 }
@@ -180,126 +196,146 @@ __device__ __forceinline__ float invert(float* work, Frag& f, float (*v)[4], int
     return sc.down;
 }
 
-// Prepares steps lo .. hi - 1 of a chunk whose decays are in cws. at: the buffer's tiles; v, dy: where those go, in one fp16 each (exact down to 2^-27 of the largest);
+// Asks for a chunk's vectors: w (in fb's place) ahead of the others, b, k, a and r in the low halves of their tiles, v and dy where one of their forms is themselves.
+template <class E, bool BWD>
+__device__ __forceinline__ void stage_chunk(const WkvSeq& s, const WkvBackward* bwd, int64_t b, int h, int t0, int lo, int hi, bool with_w, uint32_t at, uint32_t v, uint32_t v16, uint32_t fb,
+                                            int lane) {
+    if (with_w) stage_steps(fb, steps_of(s, 1, b, h, t0, lane), 2 * s.ss[1], lo, hi, true, lane);
+    stage_commit();
+#pragma unroll 1
+    for (int vec = 0; vec < 4; ++vec) {
+        const int which = vec == 0 ? 5 : vec == 1 ? 2 : vec == 2 ? 4 : 0, to = vec == 0 ? T_B : vec == 1 ? T_K : vec == 2 ? T_A : T_R;
+        stage_steps(at + to * 2 * TILE + TILE, steps_of(s, which, b, h, t0, lane), 2 * s.ss[which], lo, hi, true, lane);
+    }
+    constexpr bool OWN = std::is_same<E, __half>::value || !BWD;   // fp16 as it is; bf16 as it is for the sums over rows, else to be converted in place
+    stage_steps(OWN ? v : v16, steps_of(s, 3, b, h, t0, lane), 2 * s.ss[3], lo, hi, true, lane);
+    if (BWD)
+        stage_steps(OWN ? v + TILE : v16 + 2 * TILE, bwd->dy ? static_cast<const char*>(bwd->dy) + 2 * (b * bwd->dy_batch_stride + (int64_t)t0 * bwd->dy_step_stride + h * N + 8 * (lane & 7))
+                                                             : static_cast<const char*>(s.x[3]), bwd->dy ? 2 * bwd->dy_step_stride : 0, lo, hi, bwd->dy != nullptr, lane);
+    stage_commit();
+}
+
+// Prepares steps lo .. hi - 1 of a chunk whose factors are in fe and fb. at: the buffer's tiles; v, dy: where those go, in one fp16 each (exact down to 2^-27 of the largest);
 // v16, dy16: in bf16. BWD: dy, Q and the tile of a are kept too.
 // The code is kept short, in loops: a warp runs through it once per chunk, and unrolled (4000 instructions) it waited for them most of the time (a chunk took it 28000
 // cycles).
 template <class E, bool BWD>
-__device__ __forceinline__ void prepare_chunk(const WkvSeq& s, const WkvBackward* bwd, int64_t b, int h, int t0, int lo, int hi, bool piece, uint32_t at, uint32_t v, uint32_t v16,
-                                              const float* cws, ChunkHead* head, int lane) {
+__device__ __forceinline__ void prepare_chunk(const WkvSeq& s, const WkvBackward* bwd, int64_t b, int h, int t0, int lo, int hi, uint32_t at, uint32_t v, uint32_t v16,
+                                              const float* fe, const float* fb, ChunkHead* head, int lane) {
     constexpr int AP = BWD ? T_AP : T_A, VECTORS = BWD ? 6 : 5;
     const uint32_t tA = at + T_A * 2 * TILE, tM = at + T_M * 2 * TILE, tAP = at + AP * 2 * TILE;
     const int c8 = lane & 7, tr = lane >> 3;
-    auto load = [&](uint4* u, int vec) {   // b, k, a, r, v, dy
-        if (BWD && vec == 5) {
-            if (bwd->dy) {
-                load_steps(u, static_cast<const char*>(bwd->dy) + 2 * (b * bwd->dy_batch_stride + (int64_t)t0 * bwd->dy_step_stride + h * N + 8 * c8), 2 * bwd->dy_step_stride, lo, hi, lane);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) u[i] = make_uint4(0, 0, 0, 0);
-            }
-            return;
-        }
-        const int which = vec == 0 ? 5 : vec == 1 ? 2 : vec == 2 ? 4 : vec == 3 ? 0 : 3;
-        load_steps(u, steps_of(s, which, b, h, t0, lane), 2 * s.ss[which], lo, hi, lane);
-    };
-    uint4 x[4], next[4];   // (a vector is on its way while the one before it is worked on)
-    load(x, 0);
-    const float2 end2 = *reinterpret_cast<const float2*>(cws + L * N + 2 * lane);
-    *reinterpret_cast<float2*>(head->decay + 2 * lane) = make_float2(ex2_(end2.x), ex2_(end2.y));
-    // a's and r's factors are at most `grow` (2^STEEP_LOG2), b's and k's at most 1; in a piece of one step all are 1
-    const int grow_by = piece ? 0 : (int)ceilf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(-fminf(end2.x, end2.y), 0.f)))));
-    const float grow = __int_as_float((127 + min(grow_by, (int)STEEP_LOG2)) << 23);
+    stage_wait<0>();
+    // a's and r's factors are at most the first row of fe (2^STEEP_LOG2 or a little more), b's and k's at most 1
+    const float2 most = *reinterpret_cast<const float2*>(fe + 2 * lane);
+    const int grow_by = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(most.x, most.y), 1.f))) >> 23) + 1;
+    const float grow = __int_as_float(min(grow_by, 127 + (int)STEEP_LOG2 + 1) << 23);
     auto up_of = [](float down) { return __uint_as_float((254u << 23) - __float_as_uint(down)); };   // of a power of two
-    float end[8];
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(cws + L * N + 8 * c8 + i);
-        end[i] = f.x, end[i + 1] = f.y, end[i + 2] = f.z, end[i + 3] = f.w;
-    }
 #pragma unroll 1
-    for (int vec = 0; vec < VECTORS; ++vec) {
-        if (vec + 1 < VECTORS) load(next, vec + 1);
-        uint32_t m = 0;   // the order of non-negative floats is that of their bits
+    for (int vec = 0; vec < VECTORS; ++vec) {   // b, k, a, r, v, dy
+        if (!BWD && std::is_same<E, __half>::value && vec == 4) {
+            if (lane == 0) head->down_in[4] = 1.f;
+            break;
+        }
+        constexpr bool OWN = std::is_same<E, __half>::value || !BWD;
+        uint4 x[4];
+        staged(x, vec < 4 ? at + (vec == 0 ? T_B : vec == 1 ? T_K : vec == 2 ? T_A : T_R) * 2 * TILE + TILE : OWN ? v + (vec - 4) * TILE : v16 + (vec - 4) * 2 * TILE, lane);
+        Scale sc = {1.f, 1.f};
+        if (vec < 4 || std::is_same<E, __nv_bfloat16>::value) {   // (fp16 values are themselves in one fp16)
+            uint32_t m = 0;   // the order of non-negative floats is that of their bits
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            m = __vmaxu2(__vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu), __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)), m);
-        const float2 f = raw_pair<E>(m);
-        const Scale sc = scale_for(warp_top_abs(__uint_as_float(max(__float_as_uint(f.x), __float_as_uint(f.y)))) * (vec == 2 || vec == 3 ? grow : 1.f));   // (a NaN is the largest)
+            for (int i = 0; i < 4; ++i)
+                m = __vmaxu2(__vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu), __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)), m);
+            const float2 f = raw_pair<E>(m);
+            sc = scale_for(warp_top_abs(__uint_as_float(max(__float_as_uint(f.x), __float_as_uint(f.y)))) * (vec == 2 || vec == 3 ? grow : 1.f));   // (a NaN is the largest)
+        }
         if (vec < 4) {
             const int which = vec == 0 ? T_B : vec == 1 ? T_K : vec == 2 ? T_A : T_R;
-            const float sign = vec < 2 ? -1.f : piece ? 0.f : 1.f;
+            const float* from = (vec < 2 ? fb : vec == 2 ? fe : fe + N) + 8 * c8;   // (a's are of the sums before its step)
             const uint32_t tile = at + which * 2 * TILE;
             if (lane == 0) head->down[which] = sc.down;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = tr + 4 * i;
-                const float* cw = cws + (t + (vec != 2)) * N + 8 * c8;   // a: before the step
-                const float4 w0 = *reinterpret_cast<const float4*>(cw), w1 = *reinterpret_cast<const float4*>(cw + 4);
-                const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-                const uint32_t* raw = &x[i].x;
-                uint32_t hi4[4], lo4[4];
+            for (int i = 0; i < 4; i += 2) {   // two rows at a time: their loads, their stores
+                uint32_t hi4[2][4], lo4[2][4];
+                float4 w[2][2];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float2 e = raw_pair<E>(raw[c]);
-                    split(e.x * sc.up * ex2_((w[2 * c] - end[2 * c]) * sign), e.y * sc.up * ex2_((w[2 * c + 1] - end[2 * c + 1]) * sign), hi4[c], lo4[c]);
+                for (int k = 0; k < 2; ++k) w[k][0] = *reinterpret_cast<const float4*>(from + (tr + 4 * (i + k)) * N), w[k][1] = *reinterpret_cast<const float4*>(from + (tr + 4 * (i + k)) * N + 4);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t raw[4] = {x[i + k].x, x[i + k].y, x[i + k].z, x[i + k].w};
+                    const float f[8] = {w[k][0].x, w[k][0].y, w[k][0].z, w[k][0].w, w[k][1].x, w[k][1].y, w[k][1].z, w[k][1].w};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float2 e = raw_pair<E>(raw[c]);
+                        split(e.x * sc.up * f[2 * c], e.y * sc.up * f[2 * c + 1], hi4[k][c], lo4[k][c]);
+                    }
                 }
-                const uint32_t to = tile + t * 128 + ((c8 ^ (t & 7)) << 4);
-                st128(to, hi4);
-                st128(to + TILE, lo4);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int t = tr + 4 * (i + k);
+                    const uint32_t to = tile + t * 128 + ((c8 ^ (t & 7)) << 4);
+                    st128(to, hi4[k]);
+                    st128(to + TILE, lo4[k]);
+                }
             }
         } else {
             if (lane == 0) head->down_in[vec] = sc.down;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = tr + 4 * i;
-                const uint32_t* raw = &x[i].x;
+                const uint32_t raw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
                 const uint32_t to = t * 128 + ((c8 ^ (t & 7)) << 4);
-                uint32_t h4[4], b4[4], l4[4];
+                if (std::is_same<E, __half>::value) {
+                    if (BWD) {
+                        uint32_t hi4[4], lo4[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float2 e = raw_pair<E>(raw[c]);
-                    h4[c] = pack_half(e.x * sc.up, e.y * sc.up);
-                    if (BWD && !std::is_same<E, __nv_bfloat16>::value) split_bf16(e.x, e.y, b4[c], l4[c]);
-                }
-                st128(v + (vec - 4) * TILE + to, h4);
-                if (BWD) {
-                    if (std::is_same<E, __nv_bfloat16>::value) {
-                        st128(v16 + (vec - 4) * 2 * TILE + to, raw);
-                    } else {
-                        st128(v16 + (vec - 4) * 2 * TILE + to, b4);
-                        st128(v16 + (vec - 4) * 2 * TILE + TILE + to, l4);
+                        for (int c = 0; c < 4; ++c) {
+                            const float2 e = raw_pair<E>(raw[c]);
+                            split_bf16(e.x, e.y, hi4[c], lo4[c]);
+                        }
+                        st128(v16 + (vec - 4) * 2 * TILE + to, hi4);
+                        st128(v16 + (vec - 4) * 2 * TILE + TILE + to, lo4);
                     }
+                } else {
+                    uint32_t h4[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float2 e = raw_pair<E>(raw[c]);
+                        h4[c] = pack_half(e.x * sc.up, e.y * sc.up);
+                    }
+                    st128(v + (vec - 4) * TILE + to, h4);
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = next[i];
     }
     __syncwarp();
     const int g = lane >> 2, q = lane & 3;
 #pragma unroll 1
-    for (int m = 0; m < 4; ++m) {   // A_ab, A_ak, A_rb, A_rk
-        const int ta = m < 2 ? T_A : T_R, tb = m & 1 ? T_K : T_B;
-        float c[2][4];
-        zero2(c);
+    for (int m = 0; m < 2; ++m) {   // A_ab and A_ak, A_rb and A_rk
+        const int ta = m ? T_R : T_A;
+        float c[2][2][4];
+        zero2(c[0]), zero2(c[1]);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
             Frag f, w;
             load_frag(f, at + ta * 2 * TILE, kk * 16, lane, load_a);
-            load_frag(w, at + tb * 2 * TILE, kk * 16, lane, load_b);
-            mma3(c, f, w);
+            load_frag(w, at + T_B * 2 * TILE, kk * 16, lane, load_b);
+            mma3(c[0], f, w);
+            load_frag(w, at + T_K * 2 * TILE, kk * 16, lane, load_b);
+            mma3(c[1], f, w);
         }
-        keep_lower(c, head->down[ta], head->down[tb], m < 2 ? 1 : 0, lane);
+        keep_lower(c[0], head->down[ta], head->down[T_B], m ? 0 : 1, lane);
+        keep_lower(c[1], head->down[ta], head->down[T_K], m ? 0 : 1, lane);
+        const float d1 = put_block(c[1], tM, (m ? M_RK : M_X) * L, lane);
+        if (lane == 0) head->down_m[m ? M_RK : M_X] = d1;
         if (m == 0) {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int half = 0; half < 2; ++half) *reinterpret_cast<float2*>(head->work + (g + 8 * half) * L + 8 * n + 2 * q) = make_float2(c[n][2 * half], c[n][2 * half + 1]);
+                for (int half = 0; half < 2; ++half) *reinterpret_cast<float2*>(head->work + (g + 8 * half) * L + 8 * n + 2 * q) = make_float2(c[0][n][2 * half], c[0][n][2 * half + 1]);
         } else {
-            const int block = m == 1 ? M_X : m == 2 ? M_RB : M_RK;
-            const float d = put_block(c, tM, block * L, lane);
-            if (lane == 0) head->down_m[block] = d;
+            const float d = put_block(c[0], tM, M_RB * L, lane);
+            if (lane == 0) head->down_m[M_RB] = d;
         }
     }
     __syncwarp();
@@ -547,7 +583,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const _
         const int buf = warp - 4;
         const uint32_t at = smem_u32(smem) + buf * FWD_BUF;
         ChunkHead* head = reinterpret_cast<ChunkHead*>(smem + buf * FWD_BUF + FWD_HEAD);
-        float* cws = reinterpret_cast<float*>(smem + buf * FWD_BUF + FWD_CW);
+        float *fe = reinterpret_cast<float*>(smem + buf * FWD_BUF + FWD_FE), *fb = reinterpret_cast<float*>(smem + buf * FWD_BUF + T_M * 2 * TILE);   // (fb where T_M comes later)
         int uses = 0;
         bool ok = true;
         for (int n = buf; n < chunks && ok; n += CHUNK_BUFS) {
@@ -557,15 +593,20 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const _
                 if (uses > 0) ok = wait_for(&vacant[buf], (uint32_t)(uses - 1) & 1u);
                 if (!ok) break;
                 ++uses;
+                const uint32_t fbs = at + T_M * 2 * TILE;
+                stage_chunk<E, false>(s, nullptr, b, h, t0, 0, n_on, true, at, at + FWD_V, 0u, fbs, lane);
                 uint4 w[4];
-                load_steps(w, steps_of(s, 1, b, h, t0, lane), 2 * s.ss[1], 0, n_on, lane);
-                const bool steep = put_decays<E>(w, 0, n_on, cws, lane);
+                stage_wait<1>();
+                staged(w, fbs, lane);
+                const bool steep = put_factors<E>(w, 0, n_on, false, fe, fb, head->decay, lane);
                 if (steep) {
                     pieces = n_on;
-                    put_decays<E>(w, i, i + 1, cws, lane);
+                    stage_wait<0>();
+                    stage_chunk<E, false>(s, nullptr, b, h, t0, i, i + 1, false, at, at + FWD_V, 0u, fbs, lane);
+                    put_factors<E>(w, i, i + 1, true, fe, fb, head->decay, lane);
                 }
                 const int lo = steep ? i : 0, hi = steep ? i + 1 : n_on;
-                prepare_chunk<E, false>(s, nullptr, b, h, t0, lo, hi, steep, at, at + FWD_V, 0u, cws, head, lane);
+                prepare_chunk<E, false>(s, nullptr, b, h, t0, lo, hi, at, at + FWD_V, 0u, fe, fb, head, lane);
                 if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = i + 1 < pieces ? hi : L, head->more = i + 1 < pieces, head->piece = steep;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf]);
@@ -582,8 +623,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const _
 // forward pass kept; what they make of a chunk (u, h, and both states, as bf16 pairs) crosses in shared memory to four others, which have 16 columns each and
 // work out the sums over rows: the gradients of r, a, b, k and the decays. Three warps prepare chunks ahead as in the forward pass.
 constexpr int BWD_BUFS = 3, BWD_WARPS = 8 + BWD_BUFS;
-constexpr int BWD_V = BWD_TILES * 2 * TILE, BWD_DY = BWD_V + TILE, BWD_V16 = BWD_DY + TILE, BWD_DY16 = BWD_V16 + 2 * TILE, BWD_CW = BWD_DY16 + 2 * TILE,
-              BWD_HEAD = BWD_CW + CW_BYTES, BWD_BUF = BWD_HEAD + HEAD_BYTES;
+constexpr int BWD_V = BWD_TILES * 2 * TILE, BWD_DY = BWD_V + TILE, BWD_V16 = BWD_DY + TILE, BWD_DY16 = BWD_V16 + 2 * TILE, BWD_FE = BWD_DY16 + 2 * TILE,
+              BWD_FB = BWD_FE + FE_BYTES, BWD_HEAD = BWD_FB + L * N * 4, BWD_BUF = BWD_HEAD + HEAD_BYTES;
 // what crosses: states 64 x 64 (bf16, hi and lo), slabs of u and h, the 16 x 16 matrices P (fp16), column sums of G o S_E by row warp
 constexpr int BIG = N * N * 2, X_S = 0, X_G = X_S + 2 * BIG, X_U = X_G + 2 * BIG, X_H = X_U + 2 * SLAB, X_P = X_H + 2 * SLAB, X_SUM = X_P + 2 * TILE, X_BYTES = X_SUM + 4 * N * 4;
 constexpr int BWD_SMEM = BWD_BUFS * BWD_BUF + X_BYTES;
@@ -836,7 +877,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
         for (int n = chunks - 1, buf = 0; n >= 0 && ok; --n, buf = buf + 1 == BWD_BUFS ? 0 : buf + 1) {
             const uint32_t at = smem_u32(smem) + buf * BWD_BUF;
             const ChunkHead* head = reinterpret_cast<const ChunkHead*>(smem + buf * BWD_BUF + BWD_HEAD);
-            const float* cws = reinterpret_cast<const float*>(smem + buf * BWD_BUF + BWD_CW);
+            const float *fe = reinterpret_cast<const float*>(smem + buf * BWD_BUF + BWD_FE), *fb = reinterpret_cast<const float*>(smem + buf * BWD_BUF + BWD_FB);
             for (int more = 1; more && ok;) {
                 ok = wait_for(&full[buf], phases >> buf & 1u);
                 if (!ok) break;
@@ -957,22 +998,22 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int j = c0 + 8 * i + 2 * q;
-                    const float2 end = *reinterpret_cast<const float2*>(cws + L * N + j);
+                    const float2 dec = *reinterpret_cast<const float2*>(head->decay + j);
                     float pos[2][2], posa[2][2], flow[2][2], lw[2][2];   // [column][half]
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const int t = g + 8 * half;
                         const bool on = t >= lo && t < min(hi, n_on);
-                        const float2 c = *reinterpret_cast<const float2*>(cws + (t + 1) * N + j), c1 = *reinterpret_cast<const float2*>(cws + t * N + j);   // after it, before it
+                        const float2 fr = *reinterpret_cast<const float2*>(fe + (t + 1) * N + j), fa = *reinterpret_cast<const float2*>(fe + t * N + j);
+                        const float2 fi = *reinterpret_cast<const float2*>(fb + t * N + j);
                         const float2 r = raw_pair<E>(raw[0][i][half]), wv = raw_pair<E>(raw[1][i][half]), k = raw_pair<E>(raw[2][i][half]);
                         const float2 a = raw_pair<E>(raw[3][i][half]), bb = raw_pair<E>(raw[4][i][half]);
                         float out[5][2];   // r, w, k, a, b
 #pragma unroll
                         for (int cc = 0; cc < 2; ++cc) {
                             const int e = 2 * half + cc;
-                            const float ct = cc ? c.y : c.x, cp = cc ? c1.y : c1.x, en = cc ? end.y : end.x;
-                            const float er = piece ? 1.f : ex2_(ct - en), ea = piece ? 1.f : ex2_(cp - en), ei = ex2_(en - ct);
-                            const float grs = dr[i][e] * (piece ? ex2_(en) : er), gr = fmaf(pr[i][e], er, grs), ga = (da[i][e] + pa[i][e]) * ea;
+                            const float er = cc ? fr.y : fr.x, ea = cc ? fa.y : fa.x, ei = cc ? fi.y : fi.x;
+                            const float grs = dr[i][e] * (piece ? (cc ? dec.y : dec.x) : er), gr = fmaf(pr[i][e], er, grs), ga = (da[i][e] + pa[i][e]) * ea;
                             const float gbs = db[i][e] * ei, gks = dk[i][e] * ei, gbp = pb[i][e] * ei, gkp = pk[i][e] * ei;
                             const float rv = cc ? r.y : r.x, kv = cc ? k.y : k.x, av = cc ? a.y : a.x, bv = cc ? bb.y : bb.x;
                             out[0][cc] = gr, out[2][cc] = gks + gkp, out[3][cc] = ga, out[4][cc] = gbs + gbp;
@@ -1014,31 +1055,38 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
         const int buf = warp - 8;
         const uint32_t at = smem_u32(smem) + buf * BWD_BUF;
         ChunkHead* head = reinterpret_cast<ChunkHead*>(smem + buf * BWD_BUF + BWD_HEAD);
-        float* cws = reinterpret_cast<float*>(smem + buf * BWD_BUF + BWD_CW);
+        float *fe = reinterpret_cast<float*>(smem + buf * BWD_BUF + BWD_FE), *fb = reinterpret_cast<float*>(smem + buf * BWD_BUF + BWD_FB);
         int uses = 0;
         for (int n = chunks - 1 - buf; n >= 0 && ok; n -= BWD_BUFS) {
             const int t0 = n * L, n_on = min(L, n_steps - t0);
             if (n >= BWD_BUFS) {
                 const int t1 = t0 - BWD_BUFS * L;
                 prefetch_chunk(s, b, h, t1, L, lane);
-                if (p.g.dy && lane < L) prefetch_l2(static_cast<const char*>(p.g.dy) + 2 * (b * p.g.dy_batch_stride + (int64_t)(t1 + lane) * p.g.dy_step_stride + h * N), 2 * N);
-                if (lane == L) prefetch_l2(s.ckpt + ((size_t)bh * s.n_chunks + n - BWD_BUFS) * 4096, 16384);
+                if (p.g.dy) prefetch_steps(p.g.dy, b * p.g.dy_batch_stride + (int64_t)t1 * p.g.dy_step_stride + h * N, p.g.dy_step_stride, L, lane);
+                if (lane == 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], 16384;" ::"l"(s.ckpt + ((size_t)bh * s.n_chunks + n - BWD_BUFS) * 4096) : "memory");
             }
             // a steep chunk: for each step from the last one, the steps before it for the state's sake, and then the step itself
             for (int i = 0, j = 0, last = 0, started = 0; !last && ok;) {
                 if (uses > 0) ok = wait_for(&vacant[buf], (uint32_t)(uses - 1) & 1u);
                 if (!ok) break;
                 ++uses;
+                const uint32_t fbs = at + BWD_FB;
+                stage_chunk<E, true>(s, &p.g, b, h, t0, 0, n_on, true, at, at + BWD_V, at + BWD_V16, fbs, lane);
                 uint4 w[4];
-                load_steps(w, steps_of(s, 1, b, h, t0, lane), 2 * s.ss[1], 0, n_on, lane);
-                const bool steep = put_decays<E>(w, 0, n_on, cws, lane);
+                stage_wait<1>();
+                staged(w, fbs, lane);
+                const bool steep = put_factors<E>(w, 0, n_on, false, fe, fb, head->decay, lane);
                 if (!started) i = steep ? n_on - 1 : 0, started = 1;
                 const bool advance = steep && j < i;
                 const int step = advance ? j : i;
-                if (steep) put_decays<E>(w, step, step + 1, cws, lane);
+                if (steep) {
+                    stage_wait<0>();
+                    stage_chunk<E, true>(s, &p.g, b, h, t0, step, step + 1, false, at, at + BWD_V, at + BWD_V16, fbs, lane);
+                    put_factors<E>(w, step, step + 1, true, fe, fb, head->decay, lane);
+                }
                 last = !steep || (i == 0 && !advance);
                 const int lo = steep ? step : 0, hi = steep ? step + 1 : n_on;
-                prepare_chunk<E, true>(s, &p.g, b, h, t0, lo, hi, steep, at, at + BWD_V, at + BWD_V16, cws, head, lane);
+                prepare_chunk<E, true>(s, &p.g, b, h, t0, lo, hi, at, at + BWD_V, at + BWD_V16, fe, fb, head, lane);
                 if (lane == 0) {
                     head->t0 = t0, head->lo = lo, head->hi = step + 1 == n_on || !steep ? L : hi, head->more = !last, head->piece = steep, head->advance = advance;
                 }

@@ -3,7 +3,7 @@
     python -m albatross_b200.build [--force] [--verbose]
 
 Output: albatross_b200/_C/libalbatross_b200.so (git-ignored; it ships with the source tree) and, next to it,
-librwkv7_state_fwd_fp16.so: the torch operator shim (g++, csrc/torch_op.cpp).
+librwkv7_state_fwd_fp16.so and libalbatross_b200_train.so: the torch operator shims (g++, csrc/torch_op.cpp, csrc/train_op.cpp).
 """
 from __future__ import annotations
 
@@ -60,28 +60,40 @@ def build(force: bool = False, verbose: bool = False, bounds_check: bool = False
 
 
 TORCH_OP_LIB = os.path.join(OUT_DIR, "librwkv7_state_fwd_fp16.so")
+TRAIN_OP_LIB = os.path.join(OUT_DIR, "libalbatross_b200_train.so")
+
+
+def _build_shim(src: str, out: str, newest: float, force: bool, links: list) -> str:
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), newest):
+        return out
+    import torch
+    from torch.utils import cpp_extension as ce
+    os.makedirs(OUT_DIR, exist_ok=True)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", out,
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    cmd += ["-I" + p for p in ce.include_paths("cuda")] + ["-I/usr/local/cuda/include"]
+    cmd += ["-L" + p for p in ce.library_paths("cuda")] + ["-L" + OUT_DIR]
+    cmd += links + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-Wl,-rpath,$ORIGIN"]
+    cmd += ["-Wl,-rpath," + p for p in ce.library_paths("cuda")]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    log = os.path.join(OUT_DIR, "build_%s.log" % os.path.splitext(os.path.basename(src))[0])
+    with open(log, "w") as f:
+        f.write(" ".join(cmd) + "\n" + res.stdout + res.stderr)
+    if res.returncode != 0:
+        raise RuntimeError("building the torch operator shim failed; see " + log)
+    return out
 
 
 def build_torch_op(force: bool = False) -> str:
     """Builds the operator shim csrc/torch_op.cpp (plain C++, g++): `torch.ops.rwkv7_state_fwd_fp16.forward` backed by
     ab_wkv7_fwd. Links against the kernel library next to it (found at run time through $ORIGIN)."""
-    src = os.path.join(CSRC, "torch_op.cpp")
-    if not force and os.path.exists(TORCH_OP_LIB) and os.path.getmtime(TORCH_OP_LIB) >= max(os.path.getmtime(src), os.path.getmtime(LIB)):
-        return TORCH_OP_LIB
-    import torch
-    from torch.utils import cpp_extension as ce
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", TORCH_OP_LIB,
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
-    cmd += ["-I" + p for p in ce.include_paths("cuda")] + ["-I/usr/local/cuda/include"]
-    cmd += ["-L" + p for p in ce.library_paths("cuda")] + ["-L" + OUT_DIR]
-    cmd += ["-lalbatross_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-Wl,-rpath,$ORIGIN"]
-    cmd += ["-Wl,-rpath," + p for p in ce.library_paths("cuda")]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    with open(os.path.join(OUT_DIR, "build_torch_op.log"), "w") as f:
-        f.write(" ".join(cmd) + "\n" + res.stdout + res.stderr)
-    if res.returncode != 0:
-        raise RuntimeError("building the torch operator shim failed; see " + os.path.join(OUT_DIR, "build_torch_op.log"))
-    return TORCH_OP_LIB
+    return _build_shim(os.path.join(CSRC, "torch_op.cpp"), TORCH_OP_LIB, os.path.getmtime(LIB), force, ["-lalbatross_b200"])
+
+
+def build_train_op(force: bool = False) -> str:
+    """Builds csrc/train_op.cpp the same way: `torch.ops.albatross_b200.*`, the operators with gradients. It takes the kernel library's
+    entries at run time (train.py says from which build of it), so that it follows the header alone."""
+    return _build_shim(os.path.join(CSRC, "train_op.cpp"), TRAIN_OP_LIB, os.path.getmtime(os.path.join(HERE, "..", "include", "albatross_b200.h")), force, ["-ldl"])
 
 
 def resource_usage(log_path: str = os.path.join(OUT_DIR, "build.log")) -> dict:
@@ -117,3 +129,4 @@ if __name__ == "__main__":
     if "--bounds-check" in sys.argv:
         print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv, bounds_check=True))
     print(build_torch_op(force="--force" in sys.argv))
+    print(build_train_op(force="--force" in sys.argv))

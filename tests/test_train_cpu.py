@@ -114,14 +114,14 @@ def test_losses_refuse_the_rest():
 
 def test_python_entries_refuse_tensors_on_the_host():
     x = torch.zeros(2, 3, 64, dtype=torch.float16)
-    with pytest.raises(AssertionError):
+    with pytest.raises(RuntimeError):
         ab.RWKV7_TRAIN_OP(None, x, x, x, x, x, x)
-    with pytest.raises(AssertionError):
+    with pytest.raises(RuntimeError):
         ab.layer_norm(x)
     ids = torch.zeros(2, 3, dtype=torch.int64)
     for f in (lambda: ab.token_logp(x, ids), lambda: ab.policy_loss(x, ids, None, ids.float()), lambda: ab.policy_loss_grad(x, ids, None, ids.float()),
               lambda: ab.preference_loss(x, ids, torch.zeros(2))):
-        with pytest.raises(AssertionError):
+        with pytest.raises(RuntimeError):
             f()
 
 

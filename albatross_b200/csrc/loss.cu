@@ -116,13 +116,14 @@ __device__ __forceinline__ float piece_top(const uint4& u) {
     return m;
 }
 // What exponentials are taken relative to: exp(x - m) = 2^(x log2(e) - c) with c = m log2(e) rounded, one multiply-add and one ex2.approx (good to 2^-22).
-// Joining parts takes the difference of two c, so that the rounding of c cancels. Beyond 2^20 it would be more than 2^-4 itself, and at the type's ends (rows of the
-// lowest value throughout, which some programs use for a mask) the product overflows: there the difference comes first.
-constexpr float LOG2E = 1.4426950408889634f;
+// Joining parts takes the difference of two c, so that the rounding of c cancels. The constant's own rounding, 2^-25.7 of x, is left out of the gradient's exponentials only;
+// beyond |m| = 64 it would count, as would c's, and at the type's ends (rows of the lowest value throughout, which some programs use for a mask) the product
+// overflows: there the difference comes first.
+constexpr float LOG2E = 1.4426950408889634f, LOG2E_LOW = 1.925963033500e-8f;   // log2(e), and what its 24 bits leave of it
 struct Ref {
     float m, c;
     bool huge;
-    __device__ __forceinline__ Ref(float top) : m(top == -INFINITY ? 0.f : top), c(m * LOG2E), huge(fabsf(m) > 1048576.f) {}   // (nothing above -inf: sums of 0 or NaN)
+    __device__ __forceinline__ Ref(float top) : m(top == -INFINITY ? 0.f : top), c(m * LOG2E), huge(fabsf(m) > 64.f) {}   // (nothing above -inf: sums of 0 or NaN)
 };
 __device__ __forceinline__ float ex2(float x) {
     float e;
@@ -139,12 +140,30 @@ __device__ __forceinline__ void exp_from(float* f, const Ref& r) {
         for (int i = 0; i < N; ++i) f[i] = ex2(fmaf(f[i], LOG2E, -r.c));
     }
 }
+// The same for sums, with the constant in two parts: one part alone is off by 1.3e-8 of it, which all of a row's exponentials share, so that log-probabilities of -10 were off by
+// 1e-7 to one side and mean losses with them.
+template <int N>
+__device__ __forceinline__ void exp_to_add(float* f, const Ref& r) {
+    if (r.huge) {
+        exp_from<N>(f, r);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = ex2(fmaf(f[i], LOG2E_LOW, fmaf(f[i], LOG2E, -r.c)));
+    }
+}
 __device__ __forceinline__ float exp_from(float x, const Ref& r) {
     exp_from<1>(&x, r);
     return x;
 }
 // 2^(difference of two references): what a sum relative to the first becomes relative to the second
-__device__ __forceinline__ float rebase(const Ref& from, const Ref& to) { return from.huge || to.huge ? ex2((from.m - to.m) * LOG2E) : ex2(from.c - to.c); }
+__device__ __forceinline__ float rebase(const Ref& from, const Ref& to) {
+    if (from.huge && to.huge) return ex2((from.m - to.m) * LOG2E);
+    if (from.huge || to.huge) {
+        const float m = from.huge ? from.m : to.m, d = fmaf(m, LOG2E_LOW, fmaf(m, LOG2E, -(from.huge ? to.c : from.c)));
+        return ex2(from.huge ? d : -d);
+    }
+    return ex2(from.c - to.c);
+}
 // Writes p times a piece's exponentials to the row `dx`, which starts `lead` values into a piece of 16 bytes as the row of logits does (aligned), or anywhere.
 // FULL: the piece holds values of the row alone, and dx is aligned.
 template <class E, bool FULL>
@@ -258,7 +277,7 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
         float sum[4] = {s, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NV; ++j) unpack<E>(u[j], e + j * N);
-        exp_from<EPT>(e, ref);
+        exp_to_add<EPT>(e, ref);
 #pragma unroll
         for (int c = 0; c < EPT; ++c) sum[c & 3] += e[c];
         s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -289,8 +308,8 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
         // (a part without values has sum 0 or NaN)
         float S = warp_sum(a.y * (a.x == -INFINITY ? 1.f : rebase(Ref(a.x), ref)) + b.y * (b.x == -INFINITY ? 1.f : rebase(Ref(b.x), ref)));
         if (M == -INFINITY) S = NAN;                       // no probabilities to speak of
-        // the id's value relative to the reference, with the constant that the exponentials were taken with
-        const double rel = ref.huge ? (double)at - (double)M : ((double)at * (double)LOG2E - (double)ref.c) * 0.6931471805599453094;
+        // the id's value relative to the reference
+        const double rel = ref.huge ? (double)at - (double)M : ((double)at * 1.4426950408889634074 - (double)ref.c) * 0.6931471805599453094;
         if (dx) {
             // the gradient's coefficient in 32 bits: off by some 5e-7 of it, from the logarithm
             int n = 0;
@@ -530,7 +549,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
                     if (j >= np) break;
                     float e[N];
                     unpack<E>(u[j], e);
-                    exp_from<N>(e, ref);
+                    exp_to_add<N>(e, ref);
 #pragma unroll
                     for (int c = 0; c < N; ++c) sum[c & 3] += e[c];
                 }
@@ -579,7 +598,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
             if (M == -INFINITY) S = NAN;
             const float at = q.at;
             const int id = q.id;
-            const double rel = ref.huge ? (double)at - (double)M : ((double)at * (double)LOG2E - (double)ref.c) * 0.6931471805599453094;
+            const double rel = ref.huge ? (double)at - (double)M : ((double)at * 1.4426950408889634074 - (double)ref.c) * 0.6931471805599453094;
             const float g = dx ? policy_slope(k.p, q.pr, rel - (double)logf(S)) * inv_n * k.scale : 0.f, p = -g / S;
             if (tid == 0) {
                 q.rel = rel, q.M = M, q.S = S;

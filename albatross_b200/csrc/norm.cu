@@ -95,22 +95,27 @@ __global__ void __launch_bounds__(NT) norm_cols_kernel(const __grid_constant__ N
     a.scratch[((int64_t)blockIdx.y * 2 + 1) * a.C + c] = db;
 }
 
-// adds up the blocks' sums: 32 columns per block, eight threads a column, in one order
+// adds up the blocks' sums: 32 columns per block, 16 threads a column, in one order
+constexpr int FT = 512;
 template <class W>
-__global__ void __launch_bounds__(NT) norm_finish_kernel(const __grid_constant__ NormArgs a, int parts) {
-    __shared__ float2 red[8][32];
+__global__ void __launch_bounds__(FT) norm_finish_kernel(const __grid_constant__ NormArgs a, int parts) {
+    __shared__ float2 red[FT / 32][32];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
     pdl_wait();
     float dw = 0.f, db = 0.f;
-    if (c < a.C)
-        for (int i = g; i < parts; i += 8) {
-            dw += a.scratch[(int64_t)i * 2 * a.C + c];
-            db += a.scratch[((int64_t)i * 2 + 1) * a.C + c];
+    if (c < a.C) {
+        const float* p = a.scratch + c;
+#pragma unroll 4
+        for (int i = g; i < parts; i += FT / 32) {
+            dw += p[(int64_t)i * 2 * a.C];
+            db += p[((int64_t)i * 2 + 1) * a.C];
         }
+    }
     red[g][threadIdx.x & 31] = make_float2(dw, db);
     __syncthreads();
     if (g != 0 || c >= a.C) return;
-    for (int i = 1; i < 8; ++i) {
+#pragma unroll
+    for (int i = 1; i < FT / 32; ++i) {
         dw += red[i][threadIdx.x].x;
         db += red[i][threadIdx.x].y;
     }
@@ -159,10 +164,11 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {   // over align
 
 // One pass over x: a thread keeps NV pieces of its row in registers between the statistics and the output.
 // BLOCK: a block per row, else a warp per row; SEG (of a warp's lanes per group): a warp per NV * 32 pieces of a row.
+constexpr int BT = 128;   // threads of a row that has a block to itself: a thread's fixed work (addresses, reductions) is shared by 32 or 64 values
 template <class E, class W, int NV, bool BLOCK>
-__global__ void __launch_bounds__(NT) norm_rows_fwd_kernel(const __grid_constant__ NormArgs a, int seg) {
-    constexpr int N = per_piece<E>, TPR = BLOCK ? NT : 32;
-    __shared__ float red[2][NT / 32];
+__global__ void __launch_bounds__(BLOCK ? BT : NT) norm_rows_fwd_kernel(const __grid_constant__ NormArgs a, int seg) {
+    constexpr int N = per_piece<E>, TPR = BLOCK ? BT : 32;
+    __shared__ float red[2][BT / 32];
     const int tid = threadIdx.x, lane = BLOCK ? tid : tid & 31, pieces = a.C / N;
     const int parts = seg ? (pieces + 32 * NV - 1) / (32 * NV) : 1;   // of a row
     const unsigned unit = BLOCK ? blockIdx.x : blockIdx.x * (NT / 32) + (tid >> 5);   // (below 2^32: see fwd_rows)
@@ -185,7 +191,7 @@ __global__ void __launch_bounds__(NT) norm_rows_fwd_kernel(const __grid_constant
         __syncthreads();
         v = 0.f;
 #pragma unroll
-        for (int i = 0; i < NT / 32; ++i) v += r[i];
+        for (int i = 0; i < BT / 32; ++i) v += r[i];
         return v;
     };
     float s = 0.f;
@@ -212,11 +218,11 @@ __global__ void __launch_bounds__(NT) norm_rows_fwd_kernel(const __grid_constant
             t = fmaf(f[j][c], f[j][c], t);
         }
         if (p0 + j * TPR >= pieces) t = 0.f;
-        if (seg) rstd[j] = 1.f / sqrtf(lanes_sum(t, seg) * inv_m + a.eps);
+        if (seg) rstd[j] = rsqrtf(lanes_sum(t, seg) * inv_m + a.eps);
         else q += t;
     }
     if (!seg) {
-        q = 1.f / sqrtf(total(q, red[1]) * inv_m + a.eps);
+        q = rsqrtf(total(q, red[1]) * inv_m + a.eps);
 #pragma unroll
         for (int j = 0; j < NV; ++j) rstd[j] = q;
     }
@@ -241,7 +247,7 @@ __global__ void __launch_bounds__(NT) norm_rows_fwd_kernel(const __grid_constant
 
 // The backward pass, one read of x and dy: a block per SM, whose copying warp brings rows in ahead (a ring of bulk copies) and whose teams of TPR threads take them in
 // turn. A thread keeps the sums of its columns for dw and db from row to row; teams are added up in shared memory at the end, blocks by norm_finish_kernel, always in one order.
-constexpr int BWD_THREADS = 512, BWD_RING = 196608;
+constexpr int BWD_THREADS = 512, BWD_RING = 196608;   // (256 threads with twice the values each: 17 % fewer instructions, 71 us instead of 56 at 8192 x 4096 bf16)
 struct NormBwd {
     NormArgs a;
     int tpr, seg, slots, row_bytes;   // threads per row, lanes per group (0: the row is one), rows in the ring
@@ -343,22 +349,26 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
             loads_returned(used, &nobody);
             __syncwarp();
             if (lane == 0) mbar_arrive(&vacant[slot]);
-            float s = 0.f, q = 0.f, sj[NS], qj[NS];
+            // xh and dy w are worked out again for dx where a row is one group: kept over the block's exchange of sums they cost spills (65 us instead of 56 at 8192 x
+            // 4096 bf16; over a few lanes' exchange 30.5 instead of 35.5 at 4097 x 2560 fp16 in groups of 64)
+            float s = 0.f, q = 0.f, sj[NS], qj[NS], xh[SEG ? NV : 1][N], e[SEG ? NV : 1][N];
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int g = SEG ? j : 0;
-                float fx[N], fd[N], fw[N], sp = 0.f, qp = 0.f;
-                unpack<E>(ux[j], fx);
-                unpack<E>(ud[j], fd);
-                w[j].get(fw);
+                float sp = 0.f, qp = 0.f;
+                unpack<E>(ux[j], xh[g]);
+                unpack<E>(ud[j], e[g]);
                 if (t + j * tpr < pieces) {
+                    float fw[N];
+                    w[j].get(fw);
 #pragma unroll
                     for (int c = 0; c < N; ++c) {
-                        const float xh = (fx[c] - mean[g]) * rstd[g], e = fd[c] * fw[c];
-                        dw[j][c] = fmaf(fd[c], xh, dw[j][c]);
-                        db[j][c] += fd[c];
-                        sp += e;
-                        qp = fmaf(e, xh, qp);
+                        xh[g][c] = (xh[g][c] - mean[g]) * rstd[g];
+                        dw[j][c] = fmaf(e[g][c], xh[g][c], dw[j][c]);
+                        db[j][c] += e[g][c];
+                        e[g][c] *= fw[c];
+                        sp += e[g][c];
+                        qp = fmaf(e[g][c], xh[g][c], qp);
                     }
                 }
                 if (SEG) {
@@ -392,15 +402,17 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
                     const int p = t + j * tpr;
                     if (p >= pieces) continue;
                     const int g = SEG ? j : 0;
-                    float fx[N], fd[N], fw[N];
-                    unpack<E>(ux[j], fx);
-                    unpack<E>(ud[j], fd);
-                    w[j].get(fw);
+                    float fx[N];
+                    if (!SEG) {
+                        float fw[N];
+                        unpack<E>(ux[j], xh[0]);
+                        unpack<E>(ud[j], e[0]);
+                        w[j].get(fw);
 #pragma unroll
-                    for (int c = 0; c < N; ++c) {
-                        const float xh = (fx[c] - mean[g]) * rstd[g];
-                        fx[c] = rstd[g] * fmaf(-xh, qj[g], fmaf(fd[c], fw[c], -sj[g]));
+                        for (int c = 0; c < N; ++c) xh[0][c] = (xh[0][c] - mean[0]) * rstd[0], e[0][c] *= fw[c];
                     }
+#pragma unroll
+                    for (int c = 0; c < N; ++c) fx[c] = rstd[g] * fmaf(-xh[g][c], qj[g], e[g][c] - sj[g]);
                     if (AB_BC((p + 1) * N <= a.C)) __stcs(dx + p, pack<E>(fx));
                 }
             }
@@ -474,9 +486,9 @@ int fwd_rows(const NormArgs& a, const NormShape& s, cudaStream_t st, bool* done)
         }
         auto k = nv == 1 ? norm_rows_fwd_kernel<E, W, 1, false> : nv == 2 ? norm_rows_fwd_kernel<E, W, 2, false> : nv == 4 ? norm_rows_fwd_kernel<E, W, 4, false> : norm_rows_fwd_kernel<E, W, 8, false>;
         k<<<(unsigned)blocks, NT, 0, st>>>(a, s.seg);
-    } else if (pieces <= NT * 4 && a.rows <= INT32_MAX) {
-        auto k = pieces <= NT * 2 ? norm_rows_fwd_kernel<E, W, 2, true> : norm_rows_fwd_kernel<E, W, 4, true>;
-        k<<<(unsigned)a.rows, NT, 0, st>>>(a, 0);
+    } else if (pieces <= BT * 8 && a.rows <= INT32_MAX) {
+        auto k = pieces <= BT * 4 ? norm_rows_fwd_kernel<E, W, 4, true> : norm_rows_fwd_kernel<E, W, 8, true>;
+        k<<<(unsigned)a.rows, BT, 0, st>>>(a, 0);
     } else {
         *done = false;
     }
@@ -487,7 +499,7 @@ template <class W>
 int finish(const NormArgs& a, int parts, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((a.C + 31) / 32);
-    cfg.blockDim = dim3(NT);
+    cfg.blockDim = dim3(FT);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

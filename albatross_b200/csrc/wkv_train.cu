@@ -37,12 +37,12 @@ __device__ __forceinline__ int seq_length(const WkvSeq& s, int b) {
 
 // ---- the forward pass ----------------------------------------------------------------------------------------------------
 // A block per head: four warps carry 16 rows of the state each in registers (rows do not meet: the accumulators of one product are the operand of the next
-// without leaving the warp), four others prepare chunks ahead, each a whole one by itself, in a ring of four buffers.
+// without leaving the warp), others prepare chunks ahead, each a whole one by itself, in a ring of buffers.
 using namespace wkvc;
-constexpr int CHUNK_BUFS = 4, CHUNK_THREADS = (CHUNK_BUFS + 4) * 32;
 constexpr int FE_BYTES = (L + 1) * N * 4;   // factors relative to the chunk's end (put_factors)
 constexpr int HEAD_BYTES = (int)((sizeof(ChunkHead) + 127) / 128 * 128);
 constexpr int FWD_V = FWD_TILES * 2 * TILE, FWD_FE = FWD_V + TILE, FWD_HEAD = FWD_FE + FE_BYTES, FWD_BUF = FWD_HEAD + HEAD_BYTES;
+static_assert(8 * FWD_BUF <= 227 * 1024, "shared memory of a block");
 
 // Asks for the rows of a later chunk, 32 bytes a lane. (One bulk request per row takes the warp some 50 cycles each.)
 __device__ __forceinline__ void prefetch_steps(const void* x, int64_t at, int64_t step, int n_on, int lane) {
@@ -523,8 +523,10 @@ __device__ __forceinline__ void store_rows(const float (*S)[4], float* to, int i
             *reinterpret_cast<float2*>(to + (i0 + (lane >> 2) + 8 * half) * N + 8 * n + 2 * (lane & 3)) = make_float2(S[n][2 * half], S[n][2 * half + 1]);
 }
 
-template <class E>
-__global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const __grid_constant__ WkvFwd p) {
+// BUFS chunks under way. Four (two blocks per SM) where there are more heads than SMs; eight, which take an SM's shared memory, where there are not: a preparing warp takes
+// 18000 cycles a chunk beside one block's row warps, which take 3800, so that four of them hold these up (1024 steps x 64 heads 163 us, with eight 139).
+template <class E, int CHUNK_BUFS>
+__global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1) wkv_chunk_fwd_kernel(const __grid_constant__ WkvFwd p) {
     extern __shared__ __align__(128) unsigned char smem[];   // CHUNK_BUFS buffers
     __shared__ uint64_t full[CHUNK_BUFS], vacant[CHUNK_BUFS];
     __shared__ int s_failed;
@@ -614,7 +616,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 2) wkv_chunk_fwd_kernel(const _
         }
     }
     // steps behind the last chunk
-    for (int64_t i = (int64_t)chunks * L * 32 + threadIdx.x; i < (int64_t)s.T * 32; i += CHUNK_THREADS)
+    for (int64_t i = (int64_t)chunks * L * 32 + threadIdx.x; i < (int64_t)s.T * 32; i += (CHUNK_BUFS + 4) * 32)
         *reinterpret_cast<uint32_t*>(y + (i >> 5) * stride + (i & 31) * 2) = 0u;
 }
 
@@ -1125,14 +1127,16 @@ WkvSeq seq_of(const ab_wkv7_seq& s) {
 int wkv_train_fwd(const ab_wkv7_seq& s, void* y, float* state_out, cudaStream_t st) {
     WkvFwd p = {seq_of(s), y, state_out};
     static PerDeviceOnce once;
-    const int c = once.run(nullptr, [&](const DeviceProps&) -> int {
-        AB_CUDA(cudaFuncSetAttribute(wkv_chunk_fwd_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, CHUNK_BUFS * FWD_BUF));
-        AB_CUDA(cudaFuncSetAttribute(wkv_chunk_fwd_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, CHUNK_BUFS * FWD_BUF));
+    const DeviceProps* props = nullptr;
+    const int c = once.run(&props, [&](const DeviceProps&) -> int {
+        for (auto k : {wkv_chunk_fwd_kernel<__half, 4>, wkv_chunk_fwd_kernel<__nv_bfloat16, 4>}) AB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * FWD_BUF));
+        for (auto k : {wkv_chunk_fwd_kernel<__half, 8>, wkv_chunk_fwd_kernel<__nv_bfloat16, 8>}) AB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * FWD_BUF));
         return OK;
     });
     if (c != OK) return c;
-    if (s.dtype == AB_DT_F16) wkv_chunk_fwd_kernel<__half><<<s.B * s.H, CHUNK_THREADS, CHUNK_BUFS * FWD_BUF, st>>>(p);
-    else wkv_chunk_fwd_kernel<__nv_bfloat16><<<s.B * s.H, CHUNK_THREADS, CHUNK_BUFS * FWD_BUF, st>>>(p);
+    const bool f16 = s.dtype == AB_DT_F16;
+    if (s.B * s.H > props->n_sm) (f16 ? wkv_chunk_fwd_kernel<__half, 4> : wkv_chunk_fwd_kernel<__nv_bfloat16, 4>)<<<s.B * s.H, 8 * 32, 4 * FWD_BUF, st>>>(p);
+    else (f16 ? wkv_chunk_fwd_kernel<__half, 8> : wkv_chunk_fwd_kernel<__nv_bfloat16, 8>)<<<s.B * s.H, 12 * 32, 8 * FWD_BUF, st>>>(p);
     return check_cuda(cudaGetLastError(), "ab_wkv7_seq_fwd");
 }
 

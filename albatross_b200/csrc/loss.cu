@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
         if (dx) write_zeros(dx, V, (int)rank * LT + tid, (int)nb * LT);
         return;
     }
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // (the blocks of a row all come here: its mask is theirs)
     const Pieces<E> row(static_cast<const E*>(k.t.logits) + r * k.t.stride, V);
     const int step = (int)nb * LT * NV, at0 = (int)rank * LT * NV;
     const bool aligned = dx && (reinterpret_cast<uintptr_t>(dx) & 15) == row.lead * sizeof(E);
@@ -286,6 +287,7 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
     else
         for (int base = 0; base < row.n; base += step) sums(std::false_type(), base);
     s = warp_sum(s);
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every block of the cluster has started: its shared memory may be written
     if (lane < (int)nb) {                                  // to every block of the cluster
         uint32_t there;
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(&part[rank * LW + warp])), "r"(lane));

@@ -4,6 +4,7 @@
 //
 // The kernel library is not linked: albatross_b200_train_bind() is given the path of the one that the package has loaded (the normal or the range-checking build).
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <dlfcn.h>
@@ -38,7 +39,8 @@ struct Entries {
 #undef AB_ENTRY
 } lib;
 
-void check(int status, const char* what) { TORCH_CHECK(status == AB_OK, what, " failed with status ", status, ": ", lib.ab_last_error()); }
+// (numbers go into messages as strings: a number formatted by the stream of a shim built with another compiler's library than torch's has crashed)
+void check(int status, const char* what) { TORCH_CHECK(status == AB_OK, what, " failed with status ", std::to_string(status), ": ", lib.ab_last_error()); }
 
 int type_of(const Tensor& t) { return t.scalar_type() == at::kHalf ? AB_DT_F16 : t.scalar_type() == at::kBFloat16 ? AB_DT_BF16 : AB_DT_F32; }
 bool is_16bit(const Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
@@ -123,7 +125,7 @@ struct Wkv7 : torch::autograd::Function<Wkv7> {
 std::tuple<Tensor, Tensor> wkv7(const OptTensor& state_, const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, const Tensor& a, const Tensor& b, const OptTensor& lengths_) {
     TORCH_CHECK(r.dim() == 3 && r.is_cuda() && is_16bit(r), "RWKV7_TRAIN_OP: r must be [B, T, C], fp16 or bf16, on a CUDA device");
     const int64_t B = r.size(0), T = r.size(1), C = r.size(2);
-    TORCH_CHECK(B > 0 && C > 0 && C % 64 == 0, "RWKV7_TRAIN_OP: heads are of 64 channels, got C = ", C);
+    TORCH_CHECK(B > 0 && C > 0 && C % 64 == 0, "RWKV7_TRAIN_OP: heads are of 64 channels, got C = ", std::to_string(C));
     TORCH_CHECK(B * (C / 64) <= INT32_MAX && T <= INT32_MAX - 64, "RWKV7_TRAIN_OP: too many heads or steps");
     for (const Tensor* t : {&w, &k, &v, &a, &b})
         TORCH_CHECK(t->sizes() == r.sizes() && t->scalar_type() == r.scalar_type() && t->device() == r.device(), "RWKV7_TRAIN_OP: r, w, k, v, a, b differ in shape, type or device");
@@ -200,7 +202,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
     TORCH_CHECK(x.is_cuda() && is_known(x) && x.dim() >= 1, "layer_norm: x must be fp16, bf16 or fp32 on a CUDA device");
     const int64_t C = x.size(-1);
-    TORCH_CHECK(C > 0 && C <= INT32_MAX && groups > 0 && C % groups == 0, "layer_norm: ", C, " values do not make ", groups, " groups");
+    TORCH_CHECK(C > 0 && C <= INT32_MAX && groups > 0 && C % groups == 0, "layer_norm: ", std::to_string(C), " values do not make ", std::to_string(groups), " groups");
     Tensor w = given(weight), b = given(bias);
     for (Tensor* t : {&w, &b})
         if (t->defined()) {
@@ -342,6 +344,10 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_grad(const Tensor& logits, const 
     if (!out.defined()) out = like(logits.sizes(), logits, logits.scalar_type());
     TORCH_CHECK(out.sizes() == logits.sizes() && out.scalar_type() == logits.scalar_type() && out.device() == logits.device() && out.is_contiguous(),
                 "policy_loss_grad: out must be dense and like the logits");
+    if (out_.has_value()) {
+        at::assert_no_partial_overlap(out, logits);
+        if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();   // written in place: what autograd has kept of it is no longer good
+    }
     const Rows r(logits, ids, mask);
     Tensor loss = like({}, logits, at::kFloat), logp = like(ids.sizes(), logits, at::kFloat), scratch = like({2 * r.t.rows + 2}, logits, at::kDouble);
     check(lib.ab_policy_loss_grad(&r.t, &a.p, (float)scale, f32(loss), f32(logp), out.data_ptr(), scratch.data_ptr<double>(), stream()), "ab_policy_loss_grad");

@@ -87,7 +87,7 @@ struct Scale {
     float up, down;   // powers of two, up * down = 1
 };
 __device__ __forceinline__ Scale scale_for(float top) {   // brings `top` (>= 0) to 2^13 .. 2^14; of 0, infinities and NaN it makes nothing else
-    const int e = min(max((__float_as_int(top) >> 23) & 255, 20), 240);
+    const int e = min(max((__float_as_int(top) >> 23) & 255, 20), 253);
     return {__int_as_float((267 - e) << 23), __int_as_float((e - 13) << 23)};
 }
 __device__ __forceinline__ float warp_top_abs(float v) {   // largest of non-negative values of a warp; NaN wins

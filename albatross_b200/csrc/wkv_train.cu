@@ -64,6 +64,7 @@ __device__ __forceinline__ float log2_decay(float w) {   // of exp(-exp(w)); fin
 // Asks for one vector of a chunk's steps lo .. hi - 1 (zeros at the others) in a tile's place: a lane has eight columns (c8 = lane & 7) of steps lane >> 3, + 4, + 8,
 // + 12, here and when it takes them up again. All vectors of a chunk are on their way at once: one after the other they cost a warp 2000 cycles each.
 __device__ __forceinline__ void stage_steps(uint32_t tile, const char* p, int64_t step, int lo, int hi, bool there, int lane) {
+    if (!AB_BC(lo >= 0 && lo < hi && hi <= L)) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int t = (lane >> 3) + 4 * i;
@@ -502,7 +503,7 @@ __device__ __forceinline__ void store_steps(const float (*y)[4], E* out, int64_t
             uint32_t p = pack_pair<E>(y[n][2 * half], y[n][2 * half + 1]);
             asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(p));
             const int t = 8 * n + (lane >> 2);
-            if (t >= lo && t < hi) *reinterpret_cast<uint32_t*>(out + t * stride + i0 + 8 * half + 2 * (lane & 3)) = t < n_on ? p : 0u;
+            if (t >= lo && t < hi && AB_BC(t < L && i0 + 8 * half + 2 * (lane & 3) + 2 <= N)) *reinterpret_cast<uint32_t*>(out + t * stride + i0 + 8 * half + 2 * (lane & 3)) = t < n_on ? p : 0u;
         }
 }
 // a state's rows i0 .. i0 + 15 between accumulators and memory
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1
             const int buf = n % CHUNK_BUFS;
             const uint32_t at = smem_u32(smem) + buf * FWD_BUF;
             const ChunkHead* head = reinterpret_cast<const ChunkHead*>(smem + buf * FWD_BUF + FWD_HEAD);
-            if (s.ckpt) store_rows(S, s.ckpt + ((size_t)bh * s.n_chunks + n) * 4096, i0, lane);
+            if (s.ckpt && AB_BC(n < s.n_chunks)) store_rows(S, s.ckpt + ((size_t)bh * s.n_chunks + n) * 4096, i0, lane);
             for (int more = 1; more && ok;) {
                 ok = wait_for(&full[buf], phases >> buf & 1u);
                 if (!ok) break;
@@ -1025,7 +1026,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                             flow[cc][half] = fmaf(bv, gbs, kv * gks);
                             lw[cc][half] = on ? log2_decay(cc ? wv.y : wv.x) * 0.6931471805599453f : 0.f;
                         }
-                        if (t >= lo && t < hi) {
+                        if (t >= lo && t < hi && AB_BC(t0 + t < s.T && j + 2 <= N)) {
                             const int64_t to = base + (t0 + t) * stride + j;
                             if (p.g.dx[0]) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[0]) + to) = on ? pack_pair<E>(out[0][0], out[0][1]) : 0u;
                             if (p.g.dx[2]) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[2]) + to) = on ? pack_pair<E>(out[2][0], out[2][1]) : 0u;

@@ -70,7 +70,7 @@ typedef struct ab_model ab_model;
 const char* ab_last_error(void);
 int ab_version(void);
 /* Reads and clears the device-side status word. Bits: 1, 2, 4 = a bounded device wait gave up in the matrix-vector,
- * tensor-core or WKV / persistent kernels; 8 = a token id outside [0, vocab) reached a kernel (it was clamped to the
+ * tensor-core or WKV / persistent kernels (4 also in the operators with gradients); 8 = a token id outside [0, vocab) reached a kernel (it was clamped to the
  * table, never followed). Synchronises the device. Host pointer. After a non-zero wait bit, split-K arrival counters
  * may be stale: those of ab_gemm_static's built-in area are cleared here, a caller's own scratch / workspace is not. */
 int ab_device_status(uint32_t* status_host);
@@ -163,7 +163,8 @@ int ab_glue_selftest(int which, uint64_t first, uint64_t n, uint64_t* differ, vo
 /* ---- operators with gradients (no counterpart in the reference, which only generates) -------------------------
  * What turns sampled tokens into gradients: the WKV-7 recurrence over whole sequences, the norms of a block, and losses on
  * logits. Each takes fp16 or bf16 (norms and logits fp32 too); sums, statistics and states are fp32 or wider. Results do not
- * depend on the order in which blocks run. Nothing is kept from one call for the next. */
+ * depend on the order in which blocks run. Nothing is kept from one call for the next: calls on different streams may overlap as
+ * long as their buffers differ. */
 #define AB_DT_F16 0
 #define AB_DT_BF16 1
 #define AB_DT_F32 2

@@ -239,6 +239,72 @@ def test_recurrence_against_differences():
         assert abs(got - want) <= (2.0 ** -8 + 1e-4) * float((g.double() * step).norm()) * 2, name
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,T,H", [(150, 20, 1), (37, 35, 5), (1, 700, 1), (2, 129, 75)])
+def test_recurrence_of_more_heads_than_sms_and_of_long_sequences(B, T, H, dtype):
+    wkv_check(*wkv_inputs(B, T, H, dtype, seed=21))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_recurrence_of_unequal_lengths_with_steep_steps(dtype):
+    """Chunks that end inside, in pieces: their rows behind the end come back as zeros all the same."""
+    state, xs, dy, dout = wkv_inputs(4, 45, 2, dtype, seed=23, lo=-2.0, hi=3.0)
+    n = torch.tensor([45, 33, 17, 5], dtype=torch.int32, device="cuda")
+    behind = torch.arange(45, device="cuda")[None] >= n[:, None]
+    clean = [x.clone() for x in xs]
+    for x in xs + [dy]:
+        x[behind] = float("nan")
+    leaves = [t.detach().requires_grad_() for t in (state, *xs)]
+    y, out = ab.RWKV7_TRAIN_OP(*leaves, lengths=n)
+    got = torch.autograd.grad((y, out), leaves, (dy, dout))
+    exact = [t.double().requires_grad_() for t in (state, *clean)]
+    ye, oute = wkv_exact(exact[0], exact[1:], n)
+    want = torch.autograd.grad((ye, oute), exact, (dy.masked_fill(behind[..., None], 0).double(), dout.double()))
+    close(y, ye.detach(), "y")
+    close(out, oute.detach(), "state")
+    for name, p, q in zip(NAMES, got, want):
+        close(p, q, "d" + name)
+        assert name == "state" or bool((p[behind] == 0).all())
+
+
+def test_recurrence_of_small_and_large_values():
+    """Scales far from 1: gradients as small as those of a mean over many tokens, keys and states in the thousands. Everything is linear in v and the state together, and
+    in dy and the state's gradient together: exact powers of two change nothing but the exponent."""
+    state, xs, dy, dout = wkv_inputs(1, 40, 2, "bf16", seed=25)
+
+    def run(scale, gscale):
+        leaves = [t.detach().requires_grad_() for t in (state * scale, *xs[:3], xs[3] * scale, *xs[4:])]
+        y, out = ab.RWKV7_TRAIN_OP(*leaves)
+        return y, out, torch.autograd.grad((y, out), leaves, (dy * gscale, dout * gscale))
+    y, out, g = run(1.0, 1.0)
+    for scale, gscale in ((2.0 ** 12, 2.0 ** -30), (2.0 ** -20, 2.0 ** 10)):
+        y2, out2, g2 = run(scale, gscale)
+        assert torch.equal(y2, y * scale) and torch.equal(out2, out * scale)
+        for name, p, q in zip(NAMES, g2, g):
+            assert torch.equal(p, q * (gscale if name in ("state", "v") else scale * gscale)), name
+
+
+def test_recurrence_keeps_a_nan_in_its_head():
+    state, xs, dy, dout = wkv_inputs(2, 40, 2, "fp16", seed=27)
+    y, out = ab.RWKV7_TRAIN_OP(state, *xs)
+    xs[2][0, 20, 70] = float("nan")             # a key of sequence 0, head 1, step 20
+    y2, out2 = ab.RWKV7_TRAIN_OP(state, *xs)
+    assert torch.equal(y2[1], y[1]) and torch.equal(y2[0, :, :64], y[0, :, :64]) and torch.equal(y2[0, :16], y[0, :16])
+    assert bool(torch.isnan(y2[0, 20:, 64:]).all()) and torch.equal(out2[1], out[1]) and bool(torch.isnan(out2[0, 1, :, 6]).all())
+
+
+def test_recurrence_of_one_tensor_in_two_places():
+    """Its gradient is the sum of both places'."""
+    state, xs, dy, _ = wkv_inputs(1, 30, 1, "bf16", seed=29)
+    x = xs[0].detach().requires_grad_()
+    y, _ = ab.RWKV7_TRAIN_OP(state, x, xs[1], x, xs[3], xs[4], xs[5])
+    got, = torch.autograd.grad(y, x, dy)
+    r, k = (xs[0].detach().clone().requires_grad_() for _ in range(2))
+    y2, _ = ab.RWKV7_TRAIN_OP(state, r, xs[1], k, xs[3], xs[4], xs[5])
+    dr, dk = torch.autograd.grad(y2, (r, k), dy)
+    assert torch.equal(y, y2) and torch.equal(got, dr + dk)
+
+
 # ------------------------------------------------------------------------------------------------------------------
 # the norms
 # ------------------------------------------------------------------------------------------------------------------
@@ -325,6 +391,24 @@ def test_layer_norm_of_nothing_and_of_constants():
     x[1, 5] = float("nan")
     y = ab.layer_norm(x)
     assert bool(torch.isnan(y[1]).all()) and float(y[0].abs().max()) == 0 and float(y[2].abs().max()) == 0
+
+
+@pytest.mark.parametrize("n,Cn,groups,dtype", [(70001, 33, 1, "bf16"), (30000, 64, 1, "fp16"), (20000, 128, 2, "bf16"), (5000, 1024, 16, "fp32")])
+def test_layer_norm_of_many_short_rows(n, Cn, groups, dtype):
+    norm_check(*norm_inputs(n, Cn, dtype), groups=groups)
+
+
+def test_layer_norm_gradients_of_some_inputs():
+    x, w, b = norm_inputs(50, 512, "bf16")
+    dy = torch.randn_like(x)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(ab.layer_norm(*leaves), leaves, dy)
+    for i in range(3):
+        mine = [t.detach() for t in (x, w, b)]
+        mine[i].requires_grad_()
+        assert torch.equal(torch.autograd.grad(ab.layer_norm(*mine), mine[i], dy)[0], want[i])
+    lb = b.detach().requires_grad_()
+    assert torch.equal(torch.autograd.grad(ab.layer_norm(x, None, lb), lb, dy)[0], want[2])
 
 
 # ------------------------------------------------------------------------------------------------------------------
@@ -564,6 +648,40 @@ def test_preference_loss_and_its_gradient(P, T, V, smoothing, dtype):
     assert bool((dx[~mask] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("n,V", [(160, 9001), (149, 16384), (150, 70001), (333, 57352)])
+def test_policy_loss_of_many_long_rows(n, V, dtype):
+    """At least a row per SM: the ring of copies, rows that fit it and rows that do not, masked ones among them."""
+    x, ids, old, A, mask, ref = policy_inputs(n, V, dtype)
+    scale = 65536.0 if dtype == "fp16" else 1.0
+    more = {"mask": mask, "ref_logp": ref, "clip": (0.1, 0.3), "kl": 0.05, "denom": None}
+    x[~mask] = float("nan")
+    xe = torch.where(mask[:, None], x, torch.zeros_like(x)).double().requires_grad_()
+    le, logpe = policy_exact(xe, ids, old, A.double(), **more)
+    want, = torch.autograd.grad(le * scale, xe)
+    loss, logp, dx = ab.policy_loss_grad(x, ids, old, A, scale=scale, **more)
+    assert abs(float(loss) - float(le)) <= F32 * (float(A.abs().max()) * 3 + 1)
+    close(logp, logpe.detach(), "logp")
+    close(dx, want, "dlogits")
+    here = x.clone()
+    again = ab.policy_loss_grad(here, ids, old, A, scale=scale, out=here, **more)
+    assert torch.equal(again[0], loss) and torch.equal(again[1], logp) and torch.equal(here, dx)
+    lx = x.requires_grad_()
+    loss2, logp2 = ab.policy_loss(lx, ids, old, A, **more)
+    dx2, = torch.autograd.grad(loss2 * scale, lx)
+    assert torch.equal(logp2, logp)
+    close(dx2, want, "dlogits, two passes")
+    assert _lib.device_status() == 0
+
+
+def test_preference_loss_of_no_steps():
+    x, ids = torch.zeros(2, 0, 50, device="cuda"), torch.zeros(2, 0, dtype=torch.int64, device="cuda")
+    lx = x.requires_grad_()
+    loss, sums = ab.preference_loss(lx, ids, torch.tensor([1.0, -2.0], device="cuda"), beta=0.5)
+    assert abs(float(loss) - float(torch.nn.functional.softplus(torch.tensor(1.5)))) < 1e-6 and float(sums.abs().sum()) == 0
+    assert torch.autograd.grad(loss, lx)[0].shape == (2, 0, 50)
+
+
 # ------------------------------------------------------------------------------------------------------------------
 # streams, graphs, and all of them together
 # ------------------------------------------------------------------------------------------------------------------
@@ -674,3 +792,71 @@ def test_entries_take_a_state_in_place_and_refuse_bad_pointers():
     assert _lib.lib.ab_wkv7_seq_fwd(C.byref(s), y2.data_ptr(), here.data_ptr(), st) == 0
     assert torch.equal(y2, y) and torch.equal(here, out)
     assert _lib.lib.ab_wkv7_seq_fwd(C.byref(s), y2.data_ptr() + 2, here.data_ptr(), st) == -1 and b"boundary" in _lib.lib.ab_last_error()
+
+
+def test_what_cannot_be_right_is_refused():
+    x, ids, old, A, mask, ref = policy_inputs(6, 500, "fp16")
+    buf = torch.empty(6 * 500 + 8, dtype=torch.float16, device="cuda")
+    with pytest.raises(RuntimeError):           # out lies across the logits
+        ab.policy_loss_grad(buf[:3000].view(6, 500), ids, old, A, out=buf[8:].view(6, 500))
+    for bad in (x[:, ::2], x.float(), x[:5]):
+        with pytest.raises(RuntimeError):
+            ab.policy_loss_grad(x, ids, old, A, out=bad)
+    with pytest.raises(RuntimeError):
+        ab.policy_loss(x, ids, old, A, denom=-1.0)
+    with pytest.raises(RuntimeError):
+        ab.policy_loss(x, ids, old, A, clip=(1.5, 0.2))
+    with pytest.raises(RuntimeError):
+        ab.policy_loss(x, ids, old, A, mask=mask.float())
+    with pytest.raises(RuntimeError):
+        ab.policy_loss(x, ids, old.cpu(), A)
+    with pytest.raises(RuntimeError):
+        ab.token_logp(x, ids[:5])
+    with pytest.raises(RuntimeError):
+        ab.preference_loss(x.view(3, 2, 500), ids.view(3, 2), old[:3])
+    y = torch.zeros(2, 5, 64, device="cuda", dtype=torch.float16)
+    for args in ((None, y.float(), y, y, y, y, y), (None, y, y, y, y, y, y[:1]), (torch.zeros(2, 1, 64, 64, device="cuda", dtype=torch.float16), y, y, y, y, y, y),
+                 (None, y, y, y, y, y, y, torch.tensor([1, 2], device="cuda")), (None, *(t[..., :63] for t in (y,) * 6))):
+        with pytest.raises(RuntimeError):
+            ab.RWKV7_TRAIN_OP(*args)
+    for args in ((y, y[0, 0, :63]), (y, y[0, 0].float(), y[0, 0]), (y, None, None, 1e-5, 5), (y, y[0, 0].bfloat16())):
+        with pytest.raises(RuntimeError):
+            ab.layer_norm(*args)
+
+
+def test_gradients_are_first_order_and_of_what_was_given():
+    x, w, b = norm_inputs(4, 256, "fp32")
+    lx = x.requires_grad_()
+    y = ab.layer_norm(lx, w, b)
+    with pytest.raises(RuntimeError, match="again"):
+        torch.autograd.grad(y.sum(), lx, create_graph=True)
+    lg, ids, g = logit_inputs(4, 300, "fp16")
+    lg.requires_grad_()
+    z = lg * 1.0
+    loss, _ = ab.policy_loss(z, ids, None, torch.ones(4, device="cuda"))
+    ab.policy_loss_grad(z, ids, None, torch.ones(4, device="cuda"), out=z.detach())      # the logits are written over: autograd says so
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, lg)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap share nothing."""
+    p, ids, mask, A = small_problem()
+    p2 = {k: t.detach() * 1.25 for k, t in p.items()}
+
+    def step(values):
+        q = {k: t.detach().requires_grad_() for k, t in values.items()}
+        loss = small_step(q, ids, mask, None, A)
+        return (loss.detach(),) + torch.autograd.grad(loss, [t for n, t in q.items() if n != "emb"])
+    want = step(p), step(p2)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, values in enumerate((p, p2)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step(values))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i]))

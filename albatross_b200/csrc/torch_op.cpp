@@ -9,6 +9,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <string>
+
 #include "../../include/albatross_b200.h"
 
 namespace {
@@ -17,7 +19,7 @@ void check(const at::Tensor& t, const char* name, at::ScalarType dt, int64_t num
     TORCH_CHECK(t.is_cuda(), "rwkv7_state_fwd_fp16.forward: ", name, " must be a CUDA tensor");
     TORCH_CHECK(t.scalar_type() == dt, "rwkv7_state_fwd_fp16.forward: ", name, " has the wrong dtype");
     TORCH_CHECK(t.is_contiguous(), "rwkv7_state_fwd_fp16.forward: ", name, " must be contiguous");
-    TORCH_CHECK(t.numel() == numel, "rwkv7_state_fwd_fp16.forward: ", name, " has ", t.numel(), " elements, expected ", numel);
+    TORCH_CHECK(t.numel() == numel, "rwkv7_state_fwd_fp16.forward: ", name, " has ", std::to_string(t.numel()), " elements, expected ", std::to_string(numel));
 }
 
 void forward(int64_t B, int64_t T, int64_t C, int64_t H, at::Tensor& state, at::Tensor& r, at::Tensor& w,

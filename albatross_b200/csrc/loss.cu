@@ -369,7 +369,8 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
 // comes next is asked of the hardware (cluster launch control: the grid has a block per row, and a running block takes the place of one that has not started), because
 // masked rows cost little and would unbalance fixed shares. What a row needs besides its logits (id, policy) travels the same way ahead of it; a row's own
 // log-probability and loss, in 64 bits, are the business of another warp.
-// 4096 x 65536 fp16 rows with gradients, which a cluster of eight blocks per row (logit_rows_kernel) takes 302 us for: see row_shape.
+// 4096 x 65536 fp16 rows, the policy loss with its gradient (85 % of the rows count): 225 us = 4.8 TB/s, 73 % of the copy rate; 12 instructions per value and 2.2 per cycle bound it
+// before memory does (20 to 28 working warps, smaller or larger chunks and a chunk kept ahead in registers: 242 to 367 us).
 constexpr int RING_WARPS = 16, RING_THREADS = (RING_WARPS + 2) * 32, RING_CHUNK = 32768, RING_SLOTS = 7, RING_ROWS = 4;   // working warps; chunks, rows under way
 struct RingRow {
     int64_t r;          // -1: no more
@@ -641,6 +642,86 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
     }
 }
 
+// ---- short rows --------------------------------------------------------------------------------------------------------
+// Up to 1024 values: a warp per row, which then needs no other warp. (4096 rows of 1000 fp16 values with gradients: a block per row takes 30 us.)
+constexpr int SHORT_EPT = 32;
+template <class E>
+__global__ void __launch_bounds__(LT, 3) logit_short_kernel(const __grid_constant__ RowTask k) {
+    constexpr int N = Pieces<E>::N, NV = SHORT_EPT / N;
+    __shared__ int s_count[LW];
+    const int V = k.t.vocab, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_launch_dependents();
+    float inv_n = 0.f;
+    if (k.policy && k.dlogits) {
+        if (k.inv_denom) {
+            inv_n = *k.inv_denom;
+        } else {                                   // every block counts the rows that count
+            const int n = __reduce_add_sync(0xffffffffu, count_rows(k.t.mask, k.t.rows));
+            if (lane == 0) s_count[warp] = n;
+            __syncthreads();
+            int all = 0;
+            for (int i = 0; i < LW; ++i) all += s_count[i];
+            inv_n = 1.f / (float)max(all, 1);
+        }
+    }
+    const int64_t r = (int64_t)blockIdx.x * LW + warp;
+    if (r >= k.t.rows) return;
+    E* dx = k.dlogits ? static_cast<E*>(k.dlogits) + r * V : nullptr;
+    if (!counts(k.t, r)) {
+        if (lane == 0) {
+            if (k.logp) k.logp[r] = 0.0;
+            if (k.logp32) k.logp32[r] = 0.f;
+            if (k.row_loss) k.row_loss[r] = 0.0;
+            if (k.g) k.g[r] = 0.f;
+            if (k.stats) k.stats[2 * r] = k.stats[2 * r + 1] = 0.f;
+        }
+        if (dx) write_zeros(dx, V, lane, 32);
+        return;
+    }
+    const Pieces<E> row(static_cast<const E*>(k.t.logits) + r * k.t.stride, V);
+    uint4 u[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) u[j] = row.load(j * 32 + lane);
+    const int64_t said = k.t.ids[r];
+    const int id = (uint64_t)said < (uint64_t)V ? (int)said : said < 0 ? 0 : V - 1;
+    if (lane == 0 && id != said) atomicOr(&g_device_status, DEV_BAD_TOKEN);
+    const float at = to_f(row.x[row.lead + id]);
+    PolicyRow pr = {};
+    if (k.policy) pr = policy_load(k.p, r);
+    uint4 top4 = u[0];
+#pragma unroll
+    for (int j = 1; j < NV; ++j) top4 = piece_max<E>(top4, u[j]);
+    const float M = warp_top(piece_top<E>(top4));
+    const Ref ref(M);
+    float e[SHORT_EPT], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) unpack<E>(u[j], e + j * N);
+    exp_to_add<SHORT_EPT>(e, ref);
+#pragma unroll
+    for (int c = 0; c < SHORT_EPT; ++c) sum[c & 3] += e[c];
+    float S = warp_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    if (M == -INFINITY) S = NAN;                   // no probabilities to speak of
+    const double rel = ref.huge ? (double)at - (double)M : ((double)at * 1.4426950408889634074 - (double)ref.c) * 0.6931471805599453094;
+    if (lane == 0) {
+        const double logp = rel - log((double)S);
+        if (k.logp) k.logp[r] = logp;
+        if (k.logp32) k.logp32[r] = (float)logp;
+        if (k.stats) k.stats[2 * r] = M, k.stats[2 * r + 1] = 1.f / S;
+        if (k.policy) {
+            double g;
+            k.row_loss[r] = policy_row(k.p, pr, logp, &g);
+            if (k.g) k.g[r] = (float)g;
+        }
+    }
+    if (!dx) return;
+    __syncwarp();
+    const float g = policy_slope(k.p, pr, rel - (double)logf(S)) * inv_n * k.scale, p = -g / S;
+    const bool aligned = (reinterpret_cast<uintptr_t>(dx) & 15) == row.lead * sizeof(E);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) write_piece<E, false>(row, e + j * N, j * 32 + lane, dx, aligned, p);
+    if (((id + row.lead) / N) % 32 == lane) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));   // (by the thread that wrote its piece)
+}
+
 struct DlogitsTask {
     ab_logit_rows t;
     const float *stats, *g, *scale;
@@ -799,7 +880,14 @@ int logit_rows(const RowTask& k, cudaStream_t st) {
         constexpr int N = Pieces<E>::N;
         const int n_sm = current_sm_count();
         const int64_t values = row_pieces<E>(k.t) * N;
-        if (values > LT * 32 && k.t.rows >= n_sm) {
+        if (values <= 32 * SHORT_EPT) {
+            logit_short_kernel<E><<<(unsigned)((k.t.rows + LW - 1) / LW), LT, 0, st>>>(k);
+            return check_cuda(cudaGetLastError(), "rows of logits");
+        }
+        // The ring where a row would take more than two blocks of a cluster, and every SM has one. Ring and cluster, us, policy loss with gradient, fp16: 4096 x 65536 256
+        // and 319, 1000 x 65536 72 and 85, 4096 x 32003 162 and 180, 148 x 65536 16 and 19; on the other side 4096 x 16384 106 and 80, 4096 x 9001 111 and 88, 100 x 65536
+        // 16 and 14. fp32: 4096 x 32003 195 and 255, 1000 x 16384 36 and 37.
+        if (values > 2 * LT * 32 && k.t.rows >= n_sm) {
             static PerDeviceOnce once;
             const int st_ = once.run(nullptr, [&](const DeviceProps&) -> int {
                 AB_CUDA(cudaFuncSetAttribute(logit_ring_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_SLOTS * RING_CHUNK));

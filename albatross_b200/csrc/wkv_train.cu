@@ -525,7 +525,8 @@ __device__ __forceinline__ void store_rows(const float (*S)[4], float* to, int i
 }
 
 // BUFS chunks under way. Four (two blocks per SM) where there are more heads than SMs; eight, which take an SM's shared memory, where there are not: a preparing warp takes
-// 18000 cycles a chunk beside one block's row warps, which take 3800, so that four of them hold these up (1024 steps x 64 heads 163 us, with eight 139).
+// 18000 cycles a chunk beside one block's row warps, which take 3800, so that four of them hold these up (1024 steps x 64 heads 163 us, with eight 153; 2 x 4096 x 32
+// with states kept 774 and 669).
 template <class E, int CHUNK_BUFS>
 __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1) wkv_chunk_fwd_kernel(const __grid_constant__ WkvFwd p) {
     extern __shared__ __align__(128) unsigned char smem[];   // CHUNK_BUFS buffers

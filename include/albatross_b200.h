@@ -1,5 +1,5 @@
 /*
- * albatross_b200 — C ABI of the sm_100a kernels for the RWKV-7 decode hot path.
+ * albatross_b200 — C ABI of the sm_100a kernels for the RWKV-7 decode hot path, and of operators with gradients beside it.
  *
  * Plain pointers and sizes only; every pointer is a DEVICE pointer unless said otherwise; `stream`
  * is a cudaStream_t passed as void*. Every function returns 0 on success and a negative code

@@ -21,8 +21,9 @@
 // What only ends in 16-bit gradients and sums over the rows of a state is split into two bf16 values instead (16 bits, no scale to agree on among warps).
 //
 // Factors relative to the end grow as the decays shrink: up to exp(-end). Up to 2^16 (decays of 0.5 per step; the model's are above 0.545) the split's 22 bits
-// stand, since a tile's values down to 2^-16 of its largest keep them. A chunk beyond that ("steep") is taken in pieces of one step: the same code, with the other
-// steps' inputs as zeros and their decays as ones. In a piece r_E = r, b_E = b, k_E = k, there is no A_ab and A_ak, and u = S a with the state before its decay.
+// stand, since a tile's values down to 2^-16 of its largest keep them. A chunk beyond that ("steep") is taken in pieces of 8, 4, 2 or 1 steps: the same code, with the other
+// steps' inputs as zeros and their decays as ones. In a piece of one step (whose decay may be anything) r_E = r, b_E = b, k_E = k, there is no A_ab and A_ak, and u = S a with the state
+// before its decay. Backwards the state before each piece is made again from the one before the chunk.
 #pragma once
 #include "train.cuh"
 
@@ -140,7 +141,7 @@ enum { M_AK, M_RB, M_RK, M_X };                // 16 x 16 matrices side by side 
 struct ChunkHead {
     float down[BWD_TILES], down_m[4], down_in[6];   // of tiles, of the matrices in T_M, of b, k, a, r, v, dy as they come
     int t0, lo, hi, more;                      // steps t0 + lo .. t0 + hi - 1 of the sequence; more: the chunk goes on in this buffer
-    int piece, advance;                        // piece: of one step of a steep chunk; advance: the state alone moves on (backward pass)
+    int piece, advance;                        // piece: one step of a steep chunk; advance: the state alone moves on (backward pass)
     alignas(16) float decay[N];                // exp(end)
     alignas(16) float work[L * L];             // the preparing warp's own
 };

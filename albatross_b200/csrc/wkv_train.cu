@@ -85,10 +85,33 @@ __device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_g
 __device__ __forceinline__ const char* steps_of(const WkvSeq& s, int which, int64_t b, int h, int t0, int lane) {
     return static_cast<const char*>(s.x[which]) + 2 * (b * s.bs[which] + (int64_t)t0 * s.ss[which] + h * N + 8 * (lane & 7));
 }
-// From the w of a chunk's steps lo .. hi - 1 (the others' decays are 1): whether they are steep; if they are not, or if they are a piece's (piece), the factors of the
-// steps. fe: [L + 1][N], exp(sum before and including the steps up to a row's - end), a row for no step first; fb: [L][N], exp(end - sum); decay: exp(end). In a piece fe is 1.
+// The factors of steps lo .. hi - 1 (the others' decays are 1), from the log decays behind fe's first row. fe: [L + 1][N], exp(sum before and including the steps up to a row's - end), a row
+// for no step first; fb: [L][N], exp(end - sum); decay: exp(end). In a piece of one step (single) fe is 1. Returns whether the chunk is steep, and then, but for a piece, writes nothing.
+template <bool PIECE>
+__device__ __forceinline__ bool factors_of(int lo, int hi, bool single, float* fe, float* fb, float* decay, int lane) {
+    float2 c = make_float2(0.f, 0.f), d[L];
+#pragma unroll
+    for (int t = 0; t < L; ++t) {
+        float2 x = *reinterpret_cast<const float2*>(fe + (t + 1) * N + 2 * lane);
+        if (PIECE && (t < lo || t >= hi)) x = make_float2(0.f, 0.f);
+        c.x += x.x, c.y += x.y;
+        d[t] = c;
+    }
+    if (!PIECE && __any_sync(0xffffffffu, !(c.x >= -STEEP_LOG2) || !(c.y >= -STEEP_LOG2))) return true;
+    const bool one = PIECE && single;
+    *reinterpret_cast<float2*>(decay + 2 * lane) = make_float2(ex2_(c.x), ex2_(c.y));
+    *reinterpret_cast<float2*>(fe + 2 * lane) = one ? make_float2(1.f, 1.f) : make_float2(ex2_(-c.x), ex2_(-c.y));
+#pragma unroll
+    for (int t = 0; t < L; ++t) {
+        *reinterpret_cast<float2*>(fe + (t + 1) * N + 2 * lane) = one ? make_float2(1.f, 1.f) : make_float2(ex2_(d[t].x - c.x), ex2_(d[t].y - c.y));
+        *reinterpret_cast<float2*>(fb + t * N + 2 * lane) = make_float2(ex2_(c.x - d[t].x), ex2_(c.y - d[t].y));
+    }
+    __syncwarp();
+    return false;
+}
+// From the w of a chunk's n_on steps; true: the chunk is steep, and fe has its log decays.
 template <class E>
-__device__ __forceinline__ bool put_factors(const uint4* u, int lo, int hi, bool piece, float* fe, float* fb, float* decay, int lane) {
+__device__ __forceinline__ bool put_factors(const uint4* u, int n_on, float* fe, float* fb, float* decay, int lane) {
     const int c8 = lane & 7;
 #pragma unroll 1
     for (int half = 0; half < 2; ++half)
@@ -97,29 +120,29 @@ __device__ __forceinline__ bool put_factors(const uint4* u, int lo, int hi, bool
             const int t = (lane >> 3) + 4 * i;
             const float2 x = raw_pair<E>(half ? u[i].z : u[i].x), y = raw_pair<E>(half ? u[i].w : u[i].y);
             float4 d = make_float4(log2_decay(x.x), log2_decay(x.y), log2_decay(y.x), log2_decay(y.y));
-            if (t < lo || t >= hi) d = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (t >= n_on) d = make_float4(0.f, 0.f, 0.f, 0.f);
             *reinterpret_cast<float4*>(fe + (t + 1) * N + 8 * c8 + 4 * half) = d;
         }
     __syncwarp();
-    float2 c = make_float2(0.f, 0.f), d[L];
-#pragma unroll
-    for (int t = 0; t < L; ++t) {
-        const float2 x = *reinterpret_cast<const float2*>(fe + (t + 1) * N + 2 * lane);
-        c.x += x.x, c.y += x.y;
-        d[t] = c;
-    }
-    const bool steep = __any_sync(0xffffffffu, !(c.x >= -STEEP_LOG2) || !(c.y >= -STEEP_LOG2));
-    if (steep && !piece) return true;
-    *reinterpret_cast<float2*>(decay + 2 * lane) = make_float2(ex2_(c.x), ex2_(c.y));
-    *reinterpret_cast<float2*>(fe + 2 * lane) = piece ? make_float2(1.f, 1.f) : make_float2(ex2_(-c.x), ex2_(-c.y));
-#pragma unroll
-    for (int t = 0; t < L; ++t) {
-        *reinterpret_cast<float2*>(fe + (t + 1) * N + 2 * lane) = piece ? make_float2(1.f, 1.f) : make_float2(ex2_(d[t].x - c.x), ex2_(d[t].y - c.y));
-        *reinterpret_cast<float2*>(fb + t * N + 2 * lane) = make_float2(ex2_(c.x - d[t].x), ex2_(c.y - d[t].y));
-    }
-    __syncwarp();
-    return steep;
+    return factors_of<false>(0, L, false, fe, fb, decay, lane);
 }
+// How many steps of a steep chunk are taken at once: 8, 4, 2 or 1, in pieces from its start on. 1024 steps x 64 heads, decays of 2^-2, 2^-3, 2^-6, 2^-17 a step: 0.66, 1.9, 4.3, 9.3 ms forward
+// and 2.2, 7.7, 27, 100 ms backward; 0.14 and 0.41 without a steep chunk. This and the next one are not inlined: there they cost every chunk registers (4% forward).
+__device__ __noinline__ int steep_steps(const float* fe, int lane) {
+    int size = 8;
+    for (; size > 1; size >>= 1) {
+        bool bad = false;
+        float2 sum = make_float2(0.f, 0.f);
+        for (int t = 0; t < L; ++t) {
+            const float2 x = *reinterpret_cast<const float2*>(fe + (t + 1) * N + 2 * lane);
+            sum = t & (size - 1) ? make_float2(sum.x + x.x, sum.y + x.y) : x;
+            bad |= !(sum.x >= -STEEP_LOG2) || !(sum.y >= -STEEP_LOG2);
+        }
+        if (!__any_sync(0xffffffffu, bad)) break;
+    }
+    return size;
+}
+__device__ __noinline__ void put_piece(int lo, int hi, bool single, float* fe, float* fb, float* decay, int lane) { factors_of<true>(lo, hi, single, fe, fb, decay, lane); }
 __device__ __forceinline__ float acc_top(const float (*c)[4]) {
     float m = 0.f;
 #pragma unroll
@@ -602,16 +625,16 @@ __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1
                 uint4 w[4];
                 stage_wait<1>();
                 staged(w, fbs, lane);
-                const bool steep = put_factors<E>(w, 0, n_on, false, fe, fb, head->decay, lane);
-                if (steep) {
-                    pieces = n_on;
+                int lo = 0, hi = n_on, single = 0;
+                if (put_factors<E>(w, n_on, fe, fb, head->decay, lane)) {
+                    const int size = steep_steps(fe, lane);
+                    pieces = (n_on + size - 1) / size, lo = i * size, hi = min(lo + size, n_on), single = size == 1;
                     stage_wait<0>();
-                    stage_chunk<E, false>(s, nullptr, b, h, t0, i, i + 1, false, at, at + FWD_V, 0u, fbs, lane);
-                    put_factors<E>(w, i, i + 1, true, fe, fb, head->decay, lane);
+                    stage_chunk<E, false>(s, nullptr, b, h, t0, lo, hi, false, at, at + FWD_V, 0u, fbs, lane);
+                    put_piece(lo, hi, single, fe, fb, head->decay, lane);
                 }
-                const int lo = steep ? i : 0, hi = steep ? i + 1 : n_on;
+                if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = i + 1 < pieces ? hi : L, head->more = i + 1 < pieces, head->piece = single;
                 prepare_chunk<E, false>(s, nullptr, b, h, t0, lo, hi, at, at + FWD_V, 0u, fe, fb, head, lane);
-                if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = i + 1 < pieces ? hi : L, head->more = i + 1 < pieces, head->piece = steep;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf]);
             }
@@ -1069,8 +1092,8 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 if (p.g.dy) prefetch_steps(p.g.dy, b * p.g.dy_batch_stride + (int64_t)t1 * p.g.dy_step_stride + h * N, p.g.dy_step_stride, L, lane);
                 if (lane == 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], 16384;" ::"l"(s.ckpt + ((size_t)bh * s.n_chunks + n - BWD_BUFS) * 4096) : "memory");
             }
-            // a steep chunk: for each step from the last one, the steps before it for the state's sake, and then the step itself
-            for (int i = 0, j = 0, last = 0, started = 0; !last && ok;) {
+            // a steep chunk: for each piece from the last one, the pieces before it for the state's sake, and then the piece itself
+            for (int i = -1, j = 0, last = 0; !last && ok;) {
                 if (uses > 0) ok = wait_for(&vacant[buf], (uint32_t)(uses - 1) & 1u);
                 if (!ok) break;
                 ++uses;
@@ -1079,25 +1102,23 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 uint4 w[4];
                 stage_wait<1>();
                 staged(w, fbs, lane);
-                const bool steep = put_factors<E>(w, 0, n_on, false, fe, fb, head->decay, lane);
-                if (!started) i = steep ? n_on - 1 : 0, started = 1;
-                const bool advance = steep && j < i;
-                const int step = advance ? j : i;
-                if (steep) {
+                int lo = 0, hi = n_on, single = 0, advance = 0;
+                last = 1;
+                if (put_factors<E>(w, n_on, fe, fb, head->decay, lane)) {
+                    const int size = steep_steps(fe, lane);
+                    if (i < 0) i = (n_on - 1) / size;
+                    advance = j < i, last = i == 0, single = size == 1;
+                    lo = (advance ? j : i) * size, hi = min(lo + size, n_on);
+                    if (advance) ++j;
+                    else --i, j = 0;
                     stage_wait<0>();
-                    stage_chunk<E, true>(s, &p.g, b, h, t0, step, step + 1, false, at, at + BWD_V, at + BWD_V16, fbs, lane);
-                    put_factors<E>(w, step, step + 1, true, fe, fb, head->decay, lane);
+                    stage_chunk<E, true>(s, &p.g, b, h, t0, lo, hi, false, at, at + BWD_V, at + BWD_V16, fbs, lane);
+                    put_piece(lo, hi, single, fe, fb, head->decay, lane);
                 }
-                last = !steep || (i == 0 && !advance);
-                const int lo = steep ? step : 0, hi = steep ? step + 1 : n_on;
+                if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = hi == n_on ? L : hi, head->more = !last, head->piece = single, head->advance = advance;
                 prepare_chunk<E, true>(s, &p.g, b, h, t0, lo, hi, at, at + BWD_V, at + BWD_V16, fe, fb, head, lane);
-                if (lane == 0) {
-                    head->t0 = t0, head->lo = lo, head->hi = step + 1 == n_on || !steep ? L : hi, head->more = !last, head->piece = steep, head->advance = advance;
-                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf]);
-                if (advance) ++j;
-                else --i, j = 0;
             }
         }
     }

@@ -99,6 +99,16 @@ def test_recurrence_with_any_decay(lo, hi, dtype):
     wkv_check(*wkv_inputs(2, 53, 2, dtype, seed=3, lo=lo, hi=hi))
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("bits", [0.99, 1.01, 1.9, 2.1, 3.9, 4.1, 7.9, 8.1, 15.0, 17.0])
+def test_recurrence_around_the_sizes_of_a_steep_chunks_pieces(bits, dtype):
+    """Decays of 2^-bits per step, some channels of less: chunks of 16, 8, 4, 2 and 1 steps at once; 37 steps end inside a piece."""
+    state, xs, dy, dout = wkv_inputs(2, 37, 2, dtype, seed=31)
+    xs[1][:] = torch.log(torch.tensor(bits * 0.6931, dtype=torch.float64)).item()
+    xs[1][:, :, ::7] = -1.0
+    wkv_check(state, xs, dy, dout)
+
+
 def test_recurrence_with_a_few_steep_steps():
     """Chunks of ordinary decays beside chunks of steep ones, and single steep channels."""
     state, xs, dy, dout = wkv_inputs(1, 90, 2, "bf16", seed=5)

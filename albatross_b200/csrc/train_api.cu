@@ -40,6 +40,15 @@ int check_rows(const ab_logit_rows* t, const char* who) {
     return OK;
 }
 
+// the gradient may take the logits' own place, value for value; any other overlap overwrites what another row still reads
+int check_in_place(const ab_logit_rows* t, const void* dlogits, const char* who) {
+    if (t->rows == 0 || (dlogits == t->logits && (t->rows == 1 || t->stride == t->vocab))) return OK;
+    const uintptr_t in = reinterpret_cast<uintptr_t>(t->logits), out = reinterpret_cast<uintptr_t>(dlogits);
+    const uint64_t bytes = elem_bytes(t->dtype), in_bytes = ((uint64_t)(t->rows - 1) * t->stride + t->vocab) * bytes, out_bytes = (uint64_t)t->rows * t->vocab * bytes;
+    AB_CHECK_ARG(out >= in + in_bytes || in >= out + out_bytes, "%s: the gradient overlaps the logits; in place only where the rows are dense", who);
+    return OK;
+}
+
 int check_policy(const ab_policy* p, const ab_logit_rows& t, const void* scratch, const char* who) {
     AB_CHECK_ARG(p && scratch, "%s: null pointer", who);
     AB_CHECK_ARG(p->advantages || t.rows == 0, "%s: no advantages", who);
@@ -130,6 +139,7 @@ int ab_token_logp_bwd(const ab_logit_rows* t, const float* stats, const float* g
     AB_CHECK(check_rows(t, "ab_token_logp_bwd"));
     AB_CHECK_ARG(t->rows == 0 || (stats && g && dlogits), "ab_token_logp_bwd: null pointer");
     AB_CHECK_ARG(rows_per_g > 0, "ab_token_logp_bwd: bad number of rows per gradient");
+    AB_CHECK(check_in_place(t, dlogits, "ab_token_logp_bwd"));
     return token_logp_bwd(*t, stats, g, rows_per_g, scale, dlogits, (cudaStream_t)stream);
 }
 
@@ -146,7 +156,7 @@ int ab_policy_loss_grad(const ab_logit_rows* t, const ab_policy* p, float scale,
     AB_CHECK(check_rows(t, "ab_policy_loss_grad"));
     AB_CHECK(check_policy(p, *t, rows_scratch, "ab_policy_loss_grad"));
     AB_CHECK_ARG(loss && ((logp32 && dlogits) || t->rows == 0), "ab_policy_loss_grad: null pointer");
-    AB_CHECK_ARG(dlogits != t->logits || t->rows <= 1 || t->stride == t->vocab, "ab_policy_loss_grad: in place only where the rows are dense");
+    AB_CHECK(check_in_place(t, dlogits, "ab_policy_loss_grad"));
     return policy_loss(*t, *p, scale, loss, logp32, nullptr, nullptr, dlogits, rows_scratch, (cudaStream_t)stream);
 }
 

@@ -66,6 +66,11 @@ Tensor steps(const Tensor& t) {
     if (t.stride(2) == 1 && ((t.stride(0) | t.stride(1)) & 7) == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0) return t;
     return t.clone(at::MemoryFormat::Contiguous);
 }
+// a state, dense and on a 16-byte boundary (a view into a larger tensor need not be)
+Tensor dense_state(const Tensor& t) {
+    const Tensor d = t.contiguous();
+    return (reinterpret_cast<uintptr_t>(d.data_ptr()) & 15) == 0 ? d : d.clone();
+}
 ab_wkv7_seq seq_of(const Tensor* x, const Tensor& state, const Tensor& lengths, const Tensor& checkpoints) {
     ab_wkv7_seq s = {};
     s.dtype = type_of(x[0]);
@@ -116,7 +121,7 @@ struct Wkv7 : torch::autograd::Function<Wkv7> {
             if (ctx->needs_input_grad(i)) out[i] = like({B, T, C}, x[0], x[0].scalar_type());
             dx[i] = ptr(out[i]);
         }
-        const Tensor dy = grads[0].defined() ? steps(grads[0]) : Tensor(), dout = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        const Tensor dy = grads[0].defined() ? steps(grads[0]) : Tensor(), dout = grads[1].defined() ? dense_state(grads[1]) : Tensor();
         const ab_wkv7_seq s = seq_of(x, saved[0], saved[7], saved[8]);
         check(lib.ab_wkv7_seq_bwd(&s, ptr(dy), dy.defined() ? dy.stride(0) : 0, dy.defined() ? dy.stride(1) : 0, f32(dout), dx, f32(out[6]), stream()), "ab_wkv7_seq_bwd");
         return out;
@@ -133,7 +138,7 @@ std::tuple<Tensor, Tensor> wkv7(const OptTensor& state_, const Tensor& r, const 
     if (state.defined()) {
         TORCH_CHECK(state.sizes() == at::IntArrayRef({B, C / 64, 64, 64}) && state.scalar_type() == at::kFloat && state.device() == r.device(),
                     "RWKV7_TRAIN_OP: the state must be fp32 [B, H, 64, 64] on the device of r");
-        state = state.contiguous();
+        state = dense_state(state);
     }
     if (lengths.defined()) {
         TORCH_CHECK(lengths.sizes() == at::IntArrayRef({B}) && lengths.scalar_type() == at::kInt && lengths.device() == r.device(),
@@ -292,7 +297,7 @@ PolicyArgs policy_args(const Tensor& logits, const Tensor& ids, const OptTensor&
     };
     PolicyArgs a = {rows(given(old_logp)), rows(advantages), rows(given(ref_logp))};
     TORCH_CHECK(low >= 0 && low <= 1 && high >= 0, "policy_loss: bad clip range");
-    TORCH_CHECK(denom >= 0, "policy_loss: the denominator must be positive");
+    TORCH_CHECK(denom == 0 || (float)denom > 0, "policy_loss: the denominator must be positive, in 32 bits too");   // 0 stands for the number of tokens
     a.p = {f32(a.old_logp), f32(a.advantages), f32(a.ref_logp), (float)low, (float)high, (float)kl, (float)denom};
     return a;
 }

@@ -208,11 +208,11 @@ typedef struct ab_logit_rows {
     const int64_t* ids;          /* [rows] */
     const uint8_t* mask;         /* [rows] of 0 and 1, or NULL: every row counts */
 } ab_logit_rows;
-/* logp[r] = logits[r, ids[r]] - log sum exp logits[r, :] (0 where masked): fp64 in `logp`, and fp32 in `logp32` where it is not NULL.
+/* logp[r] = logits[r, ids[r]] - log sum exp logits[r, :] (0 where masked): fp64 in `logp` and fp32 in `logp32`, one of them or both.
  * stats: fp32 [rows, 2], maximum and 1 / sum exp(logits - maximum), for ab_token_logp_bwd; or NULL. */
 int ab_token_logp_fwd(const ab_logit_rows* t, double* logp, float* logp32, float* stats, void* stream);
 /* dlogits[r, :] = g[r / rows_per_g] * (scale ? *scale : 1) * (onehot(ids[r]) - softmax(logits[r, :])), zero where masked; dense rows of
- * dtype. g: fp32 [rows / rows_per_g], scale: fp32 [1], both on the device. */
+ * dtype, over the logits themselves where those are dense, or apart from them. g: fp32 [rows / rows_per_g], scale: fp32 [1], both on the device. */
 int ab_token_logp_bwd(const ab_logit_rows* t, const float* stats, const float* g, int64_t rows_per_g, const float* scale, void* dlogits,
                       void* stream);
 /* The clipped policy loss: with ratio = exp(logp - old_logp), each row's is -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A), plus
@@ -226,7 +226,7 @@ typedef struct ab_policy {
  * log-probability. rows_scratch: fp64 [2 * rows + 2]. stats as above. */
 int ab_policy_loss_fwd(const ab_logit_rows* t, const ab_policy* p, float* loss, float* logp32, float* stats, float* g, double* rows_scratch,
                        void* stream);
-/* Loss and scale * its gradient by the logits in one pass. dlogits: dense rows of dtype; it may be the logits themselves where they are dense. */
+/* Loss and scale * its gradient by the logits in one pass. dlogits: dense rows of dtype, over the logits themselves where those are dense, or apart from them. */
 int ab_policy_loss_grad(const ab_logit_rows* t, const ab_policy* p, float scale, float* loss, float* logp32, void* dlogits,
                         double* rows_scratch, void* stream);
 /* The preference loss of `pairs` pairs of answers of `steps` rows each, first the better ones, then the worse ones, t->rows = 2 * pairs * steps:

@@ -173,6 +173,20 @@ def test_recurrence_of_strided_inputs(dtype):
     wkv_check(state, odd, torch.cat([dy.new_zeros(3), dy.reshape(-1)])[3:].view(dy.shape), dout)
 
 
+def test_recurrence_of_states_inside_larger_tensors():
+    """A state and its gradient that start 4 bytes behind a 16-byte boundary, as narrowing a larger tensor leaves them."""
+    state, xs, dy, dout = wkv_inputs(1, 20, 2, "fp16")
+    inside = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)  # noqa: E731
+    leaves = [state.clone().requires_grad_()] + [x.clone().requires_grad_() for x in xs]
+    want = ab.RWKV7_TRAIN_OP(*leaves)
+    want_g = torch.autograd.grad(want, leaves, (dy, dout))
+    y, out = ab.RWKV7_TRAIN_OP(inside(leaves[0]), *leaves[1:])
+    joined = torch.cat([out.new_zeros(1), out.flatten()])
+    got_g = torch.autograd.grad((y, joined), leaves, (dy, torch.cat([dout.new_zeros(1), dout.flatten()])))
+    assert torch.equal(y, want[0]) and torch.equal(out, want[1])
+    assert all(torch.equal(a, b) for a, b in zip(got_g, want_g))
+
+
 def test_recurrence_without_a_state_and_with_some_gradients():
     state, xs, dy, dout = wkv_inputs(2, 21, 2, "bf16", seed=11)
     leaves = [t.detach().requires_grad_() for t in xs]
@@ -812,6 +826,12 @@ def test_what_cannot_be_right_is_refused():
     for bad in (x[:, ::2], x.float(), x[:5]):
         with pytest.raises(RuntimeError):
             ab.policy_loss_grad(x, ids, old, A, out=bad)
+    wide = buf[:3000].view(6, 500)[:, :400]
+    with pytest.raises(RuntimeError, match="overlaps"):                # out over a part of the rows that lie between padding
+        ab.policy_loss_grad(wide, ids % 400, old, A, out=buf[8:2408].view(6, 400))
+    for denom in (-1.0, 0.0, float("nan"), 1e-60):                     # (1e-60 is 0 in 32 bits)
+        with pytest.raises(RuntimeError):
+            ab.policy_loss(x, ids, old, A, denom=denom)
     with pytest.raises(RuntimeError):
         ab.policy_loss(x, ids, old, A, denom=-1.0)
     with pytest.raises(RuntimeError):

@@ -112,6 +112,12 @@ def test_losses_refuse_the_rest():
         assert _lib.lib.ab_preference_loss_fwd(C.byref(t), pairs, steps, P, 0.1, smoothing, P, P, P, P, P, None) == -1
 
 
+def test_gradients_over_other_rows_logits_are_refused():
+    for t, at in ((_rows(stride=128), P + 16), (_rows(), P + 2), (_rows(), P + 1198), (_rows(stride=128), P - 1198)):     # (6 rows of 100 values of 2 bytes)
+        assert _lib.lib.ab_policy_loss_grad(C.byref(t), C.byref(_policy()), 1.0, P, P, at, P, None) == -1 and b"overlaps" in _lib.lib.ab_last_error()
+        assert _lib.lib.ab_token_logp_bwd(C.byref(t), P, P, 1, None, at, None) == -1 and b"overlaps" in _lib.lib.ab_last_error()
+
+
 def test_python_entries_refuse_tensors_on_the_host():
     x = torch.zeros(2, 3, 64, dtype=torch.float16)
     with pytest.raises(RuntimeError):

@@ -6,9 +6,11 @@
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/library.h>
 
 #include <string>
@@ -57,8 +59,20 @@ struct Plain {
     Tensor t;
 };
 OptTensor or_none(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-// gradients are not differentiable: asking for a graph of them is an error, not a silent zero
-void first_order() { TORCH_CHECK(!at::GradMode::is_enabled(), "albatross_b200: the gradients of these operators cannot be differentiated again (create_graph)"); }
+// What a backward pass refuses. Gradients are not differentiable: asking for a graph of them is an error, not a silent zero. And in a stream capture a leaf that an earlier graph still ties
+// to the default stream: adding its gradient would make that stream wait for the capturing one, which the default stream cannot, and the capture would be lost with a less telling error.
+void check_backward() {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "albatross_b200: the gradients of these operators cannot be differentiated again (create_graph)");
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    for (const torch::autograd::Edge& e : node->next_edges()) {
+        if (!e.function || !dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) continue;
+        const auto s = e.function->stream();
+        TORCH_CHECK(!s || at::cuda::CUDAStream(*s).stream() != nullptr,
+                    "albatross_b200: a gradient is captured into a CUDA graph while an earlier autograd graph of the same leaf, made on the default stream, still lives; release that one first");
+    }
+}
 
 // ---- the recurrence ----------------------------------------------------------------------------------------------------------------
 // [B, T, C] with a dense last dimension and every step on a 16-byte boundary; others are copied
@@ -108,7 +122,7 @@ struct Wkv7 : torch::autograd::Function<Wkv7> {
         return {y, out};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        first_order();
+        check_backward();
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list saved = ctx->get_saved_variables();
         const Tensor* x = saved.data() + 1;
@@ -184,7 +198,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        first_order();
+        check_backward();
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &stats = saved[3];
@@ -268,7 +282,7 @@ struct TokenLogp : torch::autograd::Function<TokenLogp> {
         return logp;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        first_order();
+        check_backward();
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list s = ctx->get_saved_variables();
         return {dlogits_of(s[0], s[1], s[2], s[3], grads[0].contiguous(), 1, Tensor()), Tensor(), Tensor()};
@@ -320,7 +334,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         return {loss, logp};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        first_order();
+        check_backward();
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list s = ctx->get_saved_variables();
         return {dlogits_of(s[0], s[1], s[2], s[3], s[4], 1, grads[0].contiguous()), Tensor(), Tensor(), Tensor()};
@@ -380,7 +394,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
         return {loss, logp};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        first_order();
+        check_backward();
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list s = ctx->get_saved_variables();
         variable_list out(6);

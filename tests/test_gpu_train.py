@@ -869,6 +869,33 @@ def test_gradients_are_first_order_and_of_what_was_given():
         torch.autograd.grad(loss, lg)
 
 
+def test_capture_beside_a_living_graph_of_the_same_leaf_is_refused():
+    """On the default stream such a graph ties the leaf to that stream, which cannot join a capture; nothing of the process is lost, and without that graph the capture is taken."""
+    x = torch.randn(4, 256, device="cuda", requires_grad=True)
+    lg, ids, _ = logit_inputs(4, 300, "fp16")
+    lg.requires_grad_()
+    A = torch.ones(4, device="cuda")
+    for leaf, run in ((x, lambda: ab.layer_norm(x).square().sum()), (lg, lambda: ab.token_logp(lg, ids).sum()), (lg, lambda: ab.policy_loss(lg, ids, None, A)[0])):
+        leaf.grad = None
+        living = run()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with pytest.raises(RuntimeError, match="still lives"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=s):
+                run().backward()
+        living.backward()
+        want, leaf.grad, living = leaf.grad, None, None
+        with torch.cuda.stream(s):
+            run().backward()
+        leaf.grad = None
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            run().backward()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(leaf.grad, want)
+
+
 def test_two_streams_at_once():
     """Calls that overlap share nothing."""
     p, ids, mask, A = small_problem()

@@ -239,13 +239,12 @@ __device__ __forceinline__ void stage_chunk(const WkvSeq& s, const WkvBackward* 
     stage_commit();
 }
 
-// Prepares steps lo .. hi - 1 of a chunk whose factors are in fe and fb. at: the buffer's tiles; v, dy: where those go, in one fp16 each (exact down to 2^-27 of the largest);
+// Prepares a chunk (or a piece of one) that is staged and whose factors are in fe and fb. at: the buffer's tiles; v, dy: where those go, in one fp16 each (exact down to 2^-27 of the largest);
 // v16, dy16: in bf16. BWD: dy, Q and the tile of a are kept too.
 // The code is kept short, in loops: a warp runs through it once per chunk, and unrolled (4000 instructions) it waited for them most of the time (a chunk took it 28000
 // cycles).
 template <class E, bool BWD>
-__device__ __forceinline__ void prepare_chunk(const WkvSeq& s, const WkvBackward* bwd, int64_t b, int h, int t0, int lo, int hi, uint32_t at, uint32_t v, uint32_t v16,
-                                              const float* fe, const float* fb, ChunkHead* head, int lane) {
+__device__ __forceinline__ void prepare_chunk(uint32_t at, uint32_t v, uint32_t v16, const float* fe, const float* fb, ChunkHead* head, int lane) {
     constexpr int AP = BWD ? T_AP : T_A, VECTORS = BWD ? 6 : 5;
     const uint32_t tA = at + T_A * 2 * TILE, tM = at + T_M * 2 * TILE, tAP = at + AP * 2 * TILE;
     const int c8 = lane & 7, tr = lane >> 3;
@@ -634,7 +633,7 @@ __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1
                     put_piece(lo, hi, single, fe, fb, head->decay, lane);
                 }
                 if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = i + 1 < pieces ? hi : L, head->more = i + 1 < pieces, head->piece = single;
-                prepare_chunk<E, false>(s, nullptr, b, h, t0, lo, hi, at, at + FWD_V, 0u, fe, fb, head, lane);
+                prepare_chunk<E, false>(at, at + FWD_V, 0u, fe, fb, head, lane);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf]);
             }
@@ -1116,7 +1115,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                     put_piece(lo, hi, single, fe, fb, head->decay, lane);
                 }
                 if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = hi == n_on ? L : hi, head->more = !last, head->piece = single, head->advance = advance;
-                prepare_chunk<E, true>(s, &p.g, b, h, t0, lo, hi, at, at + BWD_V, at + BWD_V16, fe, fb, head, lane);
+                prepare_chunk<E, true>(at, at + BWD_V, at + BWD_V16, fe, fb, head, lane);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf]);
             }

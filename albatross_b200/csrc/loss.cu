@@ -17,10 +17,10 @@ struct RowTask {
     int policy;                  // 1: the row's loss and its derivative by logp too
     ab_policy p;
     double* logp;                // or null
-    double* row_loss;
-    float *logp32, *stats, *g;   // or null
+    double *row_loss, *slope;    // the rows' losses and, or null, their derivatives by logp
+    float *logp32, *stats;       // or null
     void* dlogits;               // null: no gradient in this pass
-    const float* inv_denom;      // of the gradient in this pass
+    const double* inv_denom;     // of the gradient in this pass
     float scale;
 };
 
@@ -39,22 +39,42 @@ struct PolicyRow {
 __device__ __forceinline__ PolicyRow policy_load(const ab_policy& p, int64_t r) {
     return {p.advantages[r], p.old_logp ? p.old_logp[r] : 0.f, p.ref_logp ? p.ref_logp[r] : 0.f};
 }
-// the row's loss, and its derivative by the log-probability
-template <class F>
-__device__ __forceinline__ F policy_slope_of(F plain, F clipped, bool ref, F kl, F e) {
-    return (clipped < plain ? (F)0 : -plain) + (ref ? kl * ((F)1 - e) : (F)0);
+// What a row's loss and its derivative by the log-probability are made of, in 64 bits and the same whichever way the gradient is made: a ratio or the penalty's exponential may be
+// infinite in 32 bits beside a factor that makes them small or nothing, and 1 - exp(gap) is small where the reference is near. With logp = rel - log(S) the logarithm is not needed:
+// ratio = exp(rel - old) / S, exp(gap) = exp(ref - rel) S. A factor of 0 counts for more than an infinite ratio: the ratio's exponential is held finite (exp(709) is; a NaN stays one), and without
+// a weight the reference is not looked at.
+struct PolicyTerms {
+    double least, slope, e;      // min(ratio A, clipped A); the derivative by logp; exp(gap), or 1
+    __device__ __forceinline__ double loss(const ab_policy& p, const PolicyRow& q, double logp) const {
+        return -least + (p.ref_logp && p.kl != 0.f ? (double)p.kl * (e - ((double)q.ref - logp) - 1.0) : 0.0);
+    }
+};
+// By a whole warp: its even lanes take the ratio's exponential, its odd ones the penalty's. All of a row's other warps wait for the slope. (old: the ratio is not 1; kl 0: no reference)
+__device__ __forceinline__ PolicyTerms policy_terms(bool old, float old_logp, float A, float low, float high, float kl, float ref_logp, double rel, float S) {
+    const bool odd = threadIdx.x & 1;
+    const double x = odd ? (kl != 0.f ? (double)ref_logp - rel : 0.0) : old ? rel - (double)old_logp : 0.0;
+    const double f = exp(x > 709.0 && !odd ? 709.0 : x);
+    const float near = 1.f / S;
+    const double inv = fma((double)near, fma(-(double)S, (double)near, 1.0), (double)near);   // 1 / S to 2^-46
+    const double ratio = old ? __shfl_sync(0xffffffffu, f, 0) * inv : 1.0, most = 1.0 + (double)high, fewest = 1.0 - (double)low;
+    const bool cut = (A > 0.f && ratio > most) || (A < 0.f && ratio < fewest);
+    const double plain = ratio * (double)A;
+    PolicyTerms t;
+    t.e = kl != 0.f ? __shfl_sync(0xffffffffu, f, 1) * (double)S : 1.0;
+    t.least = cut ? (A > 0.f ? most : fewest) * (double)A : plain;
+    t.slope = (cut ? 0.0 : -plain) + (kl != 0.f ? (double)kl * (1.0 - t.e) : 0.0);
+    return t;
 }
-__device__ __forceinline__ double policy_row(const ab_policy& p, const PolicyRow& q, double logp, double* g) {
-    const double A = q.A, ratio = p.old_logp ? exp(logp - (double)q.old) : 1.0;
-    const double plain = ratio * A, clipped = fmin(fmax(ratio, 1.0 - (double)p.clip_low), 1.0 + (double)p.clip_high) * A;
-    const double gap = (double)q.ref - logp, e = p.ref_logp ? exp(gap) : 1.0;
-    *g = policy_slope_of(plain, clipped, p.ref_logp != nullptr, (double)p.kl, e);
-    return -(clipped < plain ? clipped : plain) + (p.ref_logp ? (double)p.kl * (e - gap - 1.0) : 0.0);
+__device__ __forceinline__ float policy_kl(const ab_policy& p) { return p.ref_logp ? p.kl : 0.f; }
+__device__ __forceinline__ PolicyTerms policy_terms(const ab_policy& p, const PolicyRow& q, double rel, float S) {
+    return policy_terms(p.old_logp != nullptr, q.old, q.A, p.clip_low, p.clip_high, policy_kl(p), q.ref, rel, S);
 }
-__device__ __forceinline__ float policy_slope(const ab_policy& p, const PolicyRow& q, double logp) {
-    const float ratio = p.old_logp ? expf((float)(logp - (double)q.old)) : 1.f, plain = ratio * q.A;
-    const float clipped = fminf(fmaxf(ratio, 1.f - p.clip_low), 1.f + p.clip_high) * q.A;
-    return policy_slope_of(plain, clipped, p.ref_logp != nullptr, p.kl, p.ref_logp ? expf((float)((double)q.ref - logp)) : 1.f);
+// The same where every register counts: inlined, it made the rows' exponentials spill (4096 x 9001 fp16 rows with gradient 90 us, called 85; 4096 x 32003 in the ring the other way round, 158 and 165).
+__device__ __noinline__ PolicyTerms policy_terms_call(bool old, float old_logp, float A, float low, float high, float kl, float ref_logp, double rel, float S) {
+    return policy_terms(old, old_logp, A, low, high, kl, ref_logp, rel, S);
+}
+__device__ __forceinline__ PolicyTerms policy_terms_apart(const ab_policy& p, const PolicyRow& q, double rel, float S) {
+    return policy_terms_call(p.old_logp != nullptr, q.old, q.A, p.clip_low, p.clip_high, policy_kl(p), q.ref, rel, S);
 }
 
 // ---- a row in registers --------------------------------------------------------------------------------------------
@@ -233,6 +253,21 @@ __device__ __forceinline__ float warp_top(float v) {   // warp_max in one instru
     return v;
 }
 
+// A row's maximum and sum, in every lane, from the warps' parts that the lanes hold (one of no values has sum 0 or NaN), in one order.
+struct RowSum {
+    float M;
+    Ref ref;
+    float S;
+    __device__ __forceinline__ RowSum(const float2& a, const float2& b) : M(warp_top(fmaxf(a.x, b.x))), ref(M) {
+        S = warp_sum(a.y * (a.x == -INFINITY ? 1.f : rebase(Ref(a.x), ref)) + b.y * (b.x == -INFINITY ? 1.f : rebase(Ref(b.x), ref)));
+        if (M == -INFINITY) S = NAN;                       // no probabilities to speak of
+    }
+};
+// a value relative to the reference
+__device__ __forceinline__ double relative(float at, const Ref& ref) {
+    return ref.huge ? (double)at - (double)ref.m : ((double)at * 1.4426950408889634074 - (double)ref.c) * 0.6931471805599453094;
+}
+
 // rows that count, up to all of them, as this thread's share of a block of LT
 __device__ __forceinline__ int count_rows(const uint8_t* mask, int64_t rows) {
     if (!mask) return threadIdx.x == 0 ? (int)rows : 0;
@@ -266,7 +301,7 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
             if (k.logp) k.logp[r] = 0.0;
             if (k.logp32) k.logp32[r] = 0.f;
             if (k.row_loss) k.row_loss[r] = 0.0;
-            if (k.g) k.g[r] = 0.f;
+            if (k.slope) k.slope[r] = 0.0;
             if (k.stats) k.stats[2 * r] = k.stats[2 * r + 1] = 0.f;
         }
         if (dx) write_zeros(dx, V, (int)rank * LT + tid, (int)nb * LT);
@@ -325,35 +360,31 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
         const int n_parts = (int)nb * LW;
         if (lane < n_parts) a = part[lane];
         if (lane + 32 < n_parts) b = part[lane + 32];
-        const float M = warp_top(fmaxf(a.x, b.x));
-        const Ref ref(M);
-        // (a part without values has sum 0 or NaN)
-        float S = warp_sum(a.y * (a.x == -INFINITY ? 1.f : rebase(Ref(a.x), ref)) + b.y * (b.x == -INFINITY ? 1.f : rebase(Ref(b.x), ref)));
-        if (M == -INFINITY) S = NAN;                       // no probabilities to speak of
-        // the id's value relative to the reference
-        const double rel = ref.huge ? (double)at - (double)M : ((double)at * 1.4426950408889634074 - (double)ref.c) * 0.6931471805599453094;
+        const RowSum t(a, b);
+        const double rel = relative(at, t.ref);
+        PolicyTerms terms = {};
         if (dx) {
-            // the gradient's coefficient in 32 bits: off by some 5e-7 of it, from the logarithm
             int n = 0;
             if (counting)
                 for (int i = 0; i < LW; ++i) n += s_count[i];
-            const float g = policy_slope(k.p, pr, rel - (double)logf(S)) * (counting ? 1.f / (float)max(n, 1) : *k.inv_denom) * k.scale;
-            if (lane == 0) s_join = make_float4(M, -g / S, g, 0.f);
+            terms = policy_terms_apart(k.p, pr, rel, t.S);
+            const float g = (float)(terms.slope * ((counting ? 1.0 / (double)max(n, 1) : *k.inv_denom) * (double)k.scale));
+            if (lane == 0) s_join = make_float4(t.M, -g / t.S, g, 0.f);
             __syncwarp();
             asm volatile("bar.arrive 1, %0;" ::"n"(LT) : "memory");
         }
+        if (k.policy && !dx && rank == 0) terms = policy_terms_apart(k.p, pr, rel, t.S);
         if (lane == 0 && rank == 0) {                      // (while the other warps write)
-            const double logp = rel - log((double)S);
+            const double logp = rel - log((double)t.S);
             if (k.logp) k.logp[r] = logp;
             if (k.logp32) k.logp32[r] = (float)logp;
             if (k.stats) {
-                k.stats[2 * r] = M;
-                k.stats[2 * r + 1] = 1.f / S;
+                k.stats[2 * r] = t.M;
+                k.stats[2 * r + 1] = 1.f / t.S;
             }
             if (k.policy) {
-                double g;
-                k.row_loss[r] = policy_row(k.p, pr, logp, &g);
-                if (k.g) k.g[r] = (float)g;
+                k.row_loss[r] = terms.loss(k.p, pr, logp);
+                if (k.slope) k.slope[r] = terms.slope;
             }
         }
     }
@@ -397,14 +428,13 @@ struct RingRow {
     int on, id;
     float at;
     PolicyRow pr;
-    double rel;         // from the working warps for the finishing one
-    float M, S;
+    float g;            // from the finishing warp, where a gradient is made: its coefficient
+    float2 part[RING_WARPS];   // the working warps' maxima and sums
 };
 struct RingShared {
     uint4 cancel;
-    uint64_t full[RING_SLOTS], vacant[RING_SLOTS], row_full[RING_ROWS], row_summed[RING_ROWS], row_vacant[RING_ROWS], joined, cancelled;
+    uint64_t full[RING_SLOTS], vacant[RING_SLOTS], row_full[RING_ROWS], row_summed[RING_ROWS], row_sloped[RING_ROWS], row_vacant[RING_ROWS], cancelled;
     RingRow row[RING_ROWS];
-    float2 part[2][RING_WARPS];   // of a row, and of the one after it
     int count[RING_WARPS + 2], failed;
     uint32_t nobody;
 };
@@ -417,8 +447,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
     const int V = k.t.vocab, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < RING_SLOTS; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.vacant[i], RING_WARPS);
-        for (int i = 0; i < RING_ROWS; ++i) mbar_init(&sh.row_full[i], 1), mbar_init(&sh.row_summed[i], 1), mbar_init(&sh.row_vacant[i], RING_WARPS + 1);
-        mbar_init(&sh.joined, RING_WARPS);
+        for (int i = 0; i < RING_ROWS; ++i) mbar_init(&sh.row_full[i], 1), mbar_init(&sh.row_summed[i], RING_WARPS), mbar_init(&sh.row_sloped[i], 1), mbar_init(&sh.row_vacant[i], RING_WARPS + 1);
         mbar_init(&sh.cancelled, 1);
         fence_mbar_init();
         sh.failed = 0;
@@ -511,32 +540,51 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
             if (answered < asked) mbar_wait_bounded(&sh.cancelled, (uint32_t)answered & 1u, 1u << 18);
         }
     } else if (warp == RING_WARPS + 1) {
-        if (lane == 0) {
-            for (int n = 0;; ++n) {
-                RingRow& q = sh.row[n % RING_ROWS];
-                if (!wait_for(&sh.row_full[n % RING_ROWS], (uint32_t)(n / RING_ROWS) & 1u) || q.r < 0) break;
-                if (!wait_for(&sh.row_summed[n % RING_ROWS], (uint32_t)(n / RING_ROWS) & 1u)) break;
-                double logp = 0.0, loss = 0.0, g = 0.0;
-                if (q.on) {
-                    logp = q.rel - log((double)q.S);
-                    if (k.policy) loss = policy_row(k.p, q.pr, logp, &g);
-                }
-                if (k.logp) k.logp[q.r] = logp;
-                if (k.logp32) k.logp32[q.r] = (float)logp;
-                if (k.stats) k.stats[2 * q.r] = q.on ? q.M : 0.f, k.stats[2 * q.r + 1] = q.on ? 1.f / q.S : 0.f;
-                if (k.policy) k.row_loss[q.r] = loss;
-                if (k.policy && k.g) k.g[q.r] = (float)g;
-                mbar_arrive(&sh.row_vacant[n % RING_ROWS]);
-            }
-        }
-    } else {
-        float inv_n = counting ? 0.f : k.inv_denom ? *k.inv_denom : 1.f;
+        double inv_n = k.inv_denom ? *k.inv_denom : 1.0;
         if (counting) {
             int n = 0;
             for (int i = 0; i < RING_WARPS + 2; ++i) n += sh.count[i];
-            inv_n = 1.f / (float)max(n, 1);
+            inv_n = 1.0 / (double)max(n, 1);
         }
-        int c_seen = 0, joins = 0;
+        inv_n *= (double)k.scale;
+        for (int n = 0;; ++n) {
+            RingRow& q = sh.row[n % RING_ROWS];
+            if (!__all_sync(0xffffffffu, wait_for(&sh.row_full[n % RING_ROWS], (uint32_t)(n / RING_ROWS) & 1u)) || q.r < 0) break;
+            if (!__all_sync(0xffffffffu, wait_for(&sh.row_summed[n % RING_ROWS], (uint32_t)(n / RING_ROWS) & 1u))) break;
+            double logp = 0.0, loss = 0.0, slope = 0.0;
+            float M = 0.f, inv_s = 0.f;
+            if (q.on) {
+                const float2 none = make_float2(-INFINITY, 0.f);
+                const RowSum t(lane < RING_WARPS ? q.part[lane] : none, none);
+                const double rel = relative(q.at, t.ref);
+                if (k.policy) {
+                    const PolicyTerms terms = policy_terms(k.p, q.pr, rel, t.S);
+                    slope = terms.slope;
+                    if (k.dlogits && lane == 0) {
+                        q.g = (float)(slope * inv_n);
+                        mbar_arrive(&sh.row_sloped[n % RING_ROWS]);
+                    }
+                    logp = rel - log((double)t.S);
+                    loss = terms.loss(k.p, q.pr, logp);
+                } else {
+                    logp = rel - log((double)t.S);
+                }
+                M = t.M, inv_s = 1.f / t.S;
+            } else if (k.dlogits && lane == 0) {
+                mbar_arrive(&sh.row_sloped[n % RING_ROWS]);
+            }
+            if (lane == 0) {
+                if (k.logp) k.logp[q.r] = logp;
+                if (k.logp32) k.logp32[q.r] = (float)logp;
+                if (k.stats) k.stats[2 * q.r] = M, k.stats[2 * q.r + 1] = inv_s;
+                if (k.policy) k.row_loss[q.r] = loss;
+                if (k.slope) k.slope[q.r] = slope;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.row_vacant[n % RING_ROWS]);
+        }
+    } else {
+        int c_seen = 0;
         for (int n = 0;; ++n) {
             RingRow& q = sh.row[n % RING_ROWS];
             if (!__all_sync(0xffffffffu, wait_for(&sh.row_full[n % RING_ROWS], (uint32_t)(n / RING_ROWS) & 1u))) break;
@@ -545,9 +593,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
             E* dx = k.dlogits ? static_cast<E*>(k.dlogits) + r * V : nullptr;
             if (!q.on) {
                 if (dx) write_zeros(dx, V, tid, RING_WARPS * 32);
-                if (tid == 0) mbar_arrive(&sh.row_summed[n % RING_ROWS]);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.row_vacant[n % RING_ROWS]);
+                if (lane == 0) mbar_arrive(&sh.row_summed[n % RING_ROWS]), mbar_arrive(&sh.row_vacant[n % RING_ROWS]);
                 continue;
             }
             const Pieces<E> row(logits + r * k.t.stride, V);
@@ -607,42 +654,44 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
                 if (!dx || twice) hand_back(slot, u);
             }
             s = warp_sum(s);
-            float2* part = sh.part[joins & 1];   // (written again two rows on: behind the next row's join, which every warp reaches after it has read it)
             if (lane == 0) {
-                part[warp] = make_float2(m, s);
-                mbar_arrive(&sh.joined);
-            }
-            wait_for(&sh.joined, (uint32_t)joins++ & 1u);
-            __syncwarp();
-            const float2 a = lane < RING_WARPS ? part[lane] : make_float2(-INFINITY, 0.f);
-            const float M = warp_top(a.x);
-            const Ref ref(M);
-            float S = warp_sum(a.y * (a.x == -INFINITY ? 1.f : rebase(Ref(a.x), ref)));   // (a part without values has sum 0 or NaN)
-            if (M == -INFINITY) S = NAN;
-            const float at = q.at;
-            const int id = q.id;
-            const double rel = ref.huge ? (double)at - (double)M : ((double)at * 1.4426950408889634074 - (double)ref.c) * 0.6931471805599453094;
-            const float g = dx ? policy_slope(k.p, q.pr, rel - (double)logf(S)) * inv_n * k.scale : 0.f, p = -g / S;
-            if (tid == 0) {
-                q.rel = rel, q.M = M, q.S = S;
+                q.part[warp] = make_float2(m, s);
                 mbar_arrive(&sh.row_summed[n % RING_ROWS]);
             }
             if (dx) {
+                wait_for(&sh.row_summed[n % RING_ROWS], (uint32_t)(n / RING_ROWS) & 1u);
+                __syncwarp();
+                const float2 none = make_float2(-INFINITY, 0.f);
+                const RowSum t(lane < RING_WARPS ? q.part[lane] : none, none);
+                const Ref ref = t.ref;
+                const float S = t.S, at = q.at;
+                const int id = q.id;
                 const bool aligned = (reinterpret_cast<uintptr_t>(dx) & 15) == row.lead * sizeof(E);
+                float g = 0.f, p = 0.f;
+                auto slope = [&]() {   // taken by the finishing warp, beside the first exponentials
+                    wait_for(&sh.row_sloped[n % RING_ROWS], (uint32_t)(n / RING_ROWS) & 1u);
+                    __syncwarp();
+                    g = q.g, p = -g / S;
+                };
+                if (chunks == 0) slope();
                 if (!twice) c_seen = c0;
                 for (int c = 0; c < chunks; ++c) {
                     uint4 u[PER];
                     const int slot = take(c, u);
                     hand_back(slot, u);
+                    float e[PER][N];
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) {
+                        unpack<E>(u[j], e[j]);
+                        exp_from<N>(e[j], ref);
+                    }
+                    if (c == 0) slope();
 #pragma unroll
                     for (int j = 0; j < PER; ++j) {
                         const int i = c * CP + j * RING_WARPS * 32 + tid;
-                        float e[N];
-                        unpack<E>(u[j], e);
-                        exp_from<N>(e, ref);
                         if (i < end - first) {
-                            if (aligned) write_piece<E, true>(row, e, first + i, dx, true, p);
-                            else write_piece<E, false>(row, e, first + i, dx, false, p);
+                            if (aligned) write_piece<E, true>(row, e[j], first + i, dx, true, p);
+                            else write_piece<E, false>(row, e[j], first + i, dx, false, p);
                         }
                     }
                 }
@@ -671,7 +720,7 @@ __global__ void __launch_bounds__(LT, 3) logit_short_kernel(const __grid_constan
     __shared__ int s_count[LW];
     const int V = k.t.vocab, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_launch_dependents();
-    float inv_n = 0.f;
+    double inv_n = 0.0;
     if (k.policy && k.dlogits) {
         if (k.inv_denom) {
             inv_n = *k.inv_denom;
@@ -681,7 +730,7 @@ __global__ void __launch_bounds__(LT, 3) logit_short_kernel(const __grid_constan
             __syncthreads();
             int all = 0;
             for (int i = 0; i < LW; ++i) all += s_count[i];
-            inv_n = 1.f / (float)max(all, 1);
+            inv_n = 1.0 / (double)max(all, 1);
         }
     }
     const int64_t r = (int64_t)blockIdx.x * LW + warp;
@@ -692,7 +741,7 @@ __global__ void __launch_bounds__(LT, 3) logit_short_kernel(const __grid_constan
             if (k.logp) k.logp[r] = 0.0;
             if (k.logp32) k.logp32[r] = 0.f;
             if (k.row_loss) k.row_loss[r] = 0.0;
-            if (k.g) k.g[r] = 0.f;
+            if (k.slope) k.slope[r] = 0.0;
             if (k.stats) k.stats[2 * r] = k.stats[2 * r + 1] = 0.f;
         }
         if (dx) write_zeros(dx, V, lane, 32);
@@ -721,21 +770,24 @@ __global__ void __launch_bounds__(LT, 3) logit_short_kernel(const __grid_constan
     for (int c = 0; c < SHORT_EPT; ++c) sum[c & 3] += e[c];
     float S = warp_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
     if (M == -INFINITY) S = NAN;                   // no probabilities to speak of
-    const double rel = ref.huge ? (double)at - (double)M : ((double)at * 1.4426950408889634074 - (double)ref.c) * 0.6931471805599453094;
+    const double rel = relative(at, ref);
+    PolicyTerms terms = {};
+    float g = 0.f;
+    if (k.policy) {
+        terms = policy_terms(k.p, pr, rel, S);
+        g = (float)(terms.slope * (inv_n * (double)k.scale));
+    }
     if (lane == 0) {
         const double logp = rel - log((double)S);
+        if (k.policy) k.row_loss[r] = terms.loss(k.p, pr, logp);
+        if (k.slope) k.slope[r] = terms.slope;
         if (k.logp) k.logp[r] = logp;
         if (k.logp32) k.logp32[r] = (float)logp;
         if (k.stats) k.stats[2 * r] = M, k.stats[2 * r + 1] = 1.f / S;
-        if (k.policy) {
-            double g;
-            k.row_loss[r] = policy_row(k.p, pr, logp, &g);
-            if (k.g) k.g[r] = (float)g;
-        }
     }
     if (!dx) return;
     __syncwarp();
-    const float g = policy_slope(k.p, pr, rel - (double)logf(S)) * inv_n * k.scale, p = -g / S;
+    const float p = -g / S;
     const bool aligned = (reinterpret_cast<uintptr_t>(dx) & 15) == row.lead * sizeof(E);
 #pragma unroll
     for (int j = 0; j < NV; ++j) write_piece<E, false>(row, e + j * N, j * 32 + lane, dx, aligned, p);
@@ -805,20 +857,20 @@ __device__ __forceinline__ double policy_inv_denom(const uint8_t* mask, int64_t 
     for (int64_t r = threadIdx.x; r < rows; r += JT) n += !mask || mask[r] ? 1 : 0;
     return 1.0 / fmax(block_sum_jt((double)n, red), 1.0);
 }
-__global__ void __launch_bounds__(JT) policy_denom_kernel(const uint8_t* mask, int64_t rows, float denom, float* inv) {
+__global__ void __launch_bounds__(JT) policy_denom_kernel(const uint8_t* mask, int64_t rows, float denom, double* inv) {
     __shared__ double red[JT / 32];
     const double d = policy_inv_denom(mask, rows, denom, red);
-    if (threadIdx.x == 0) *inv = (float)d;
+    if (threadIdx.x == 0) *inv = d;
 }
 // the loss, and the derivatives by the rows' log-probabilities divided as it is
-__global__ void __launch_bounds__(JT) policy_join_kernel(const uint8_t* mask, float denom, const double* row_loss, int64_t rows, float* loss, float* g) {
+__global__ void __launch_bounds__(JT) policy_join_kernel(const uint8_t* mask, float denom, const double* row_loss, const double* slope, int64_t rows, float* loss, float* g) {
     __shared__ double red[JT / 32];
     const double inv = policy_inv_denom(mask, rows, denom, red);
     pdl_wait();
     double s = 0.0;
     for (int64_t r = threadIdx.x; r < rows; r += JT) {
         s += row_loss[r];
-        if (g) g[r] = (float)((double)g[r] * inv);
+        if (g) g[r] = (float)(slope[r] * inv);
     }
     s = block_sum_jt(s, red);
     if (threadIdx.x == 0) *loss = (float)(s * inv);
@@ -961,9 +1013,10 @@ int policy_loss(const ab_logit_rows& t, const ab_policy& p, float scale, float* 
                 double* rows_scratch, cudaStream_t st) {
     // Where the gradient is made in this pass each block needs the denominator: it counts the rows itself up to 16384 of them (64 values a thread, from
     // L2, beside its row), a launch ahead of it does beyond that.
-    float* inv = nullptr;
+    // rows_scratch: the rows' losses, that, and the rows' slopes.
+    double* inv = nullptr;
     if (dlogits && (p.denom != 0.f || t.rows > 16384)) {
-        inv = reinterpret_cast<float*>(rows_scratch + t.rows);
+        inv = rows_scratch + t.rows;
         policy_denom_kernel<<<1, JT, 0, st>>>(t.mask, t.rows, p.denom, inv);
     }
     RowTask k = {};
@@ -973,13 +1026,13 @@ int policy_loss(const ab_logit_rows& t, const ab_policy& p, float scale, float* 
     k.row_loss = rows_scratch;
     k.logp32 = logp32;
     k.stats = stats;
-    k.g = g;
+    k.slope = g ? rows_scratch + t.rows + 1 : nullptr;
     k.dlogits = dlogits;
     k.inv_denom = inv;
     k.scale = scale;
     const int s = logit_rows(k, st);
     if (s != OK) return s;
-    return launch_behind(policy_join_kernel, JT, st, t.mask, p.denom, rows_scratch, t.rows, loss, g);
+    return launch_behind(policy_join_kernel, JT, st, t.mask, p.denom, rows_scratch, k.slope, t.rows, loss, g);
 }
 
 int preference_loss(const ab_logit_rows& t, int64_t pairs, int64_t steps, const float* ref, float beta, float smoothing, float* loss, float* logp32,

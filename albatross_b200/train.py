@@ -79,7 +79,8 @@ def policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logp: Optional[torc
 
     Per token, with ratio = exp(logp - old_logp): -min(ratio A, clamp(ratio, 1 - clip[0], 1 + clip[1]) A) + kl (exp(ref_logp - logp) - (ref_logp - logp) - 1);
     their sum where `mask` (bool [...]) is True, divided by `denom` or else by the number of such tokens (at least 1). logits [..., V], ids [...];
-    old_logp, advantages and ref_logp broadcast to the ids' shape and get no gradient; old_logp None: the ratio is 1, as on the first step after
+    with kl 0 ref_logp is not looked at, and an advantage of 0
+    makes nothing of any ratio. old_logp, advantages and ref_logp broadcast to the ids' shape and get no gradient; old_logp None: the ratio is 1, as on the first step after
     sampling. At a border of the clip range the unclipped side's gradient counts."""
     return _policy_loss(logits, ids, old_logp, advantages, mask, ref_logp, clip[0], clip[1], kl, _denom(denom))
 

@@ -623,6 +623,75 @@ def test_policy_loss_and_its_gradient(n, V, dtype, form):
     assert dx3.data_ptr() == here.data_ptr() and torch.equal(dx3, dx2) and torch.equal(loss3, loss) and torch.equal(logp3, logp)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("n,V", [(160, 500), (9, 4099), (160, 20011)])
+def test_policy_gradients_where_a_factor_is_nothing_or_exponentials_are_large(n, V, dtype):
+    """Advantages of 0 (a group whose rewards are all equal), a reference without weight, ratios and penalties beyond what an exponential holds in 32 bits: one pass and
+    autograd both, in each of the kernels. The coefficient of a row whose exponential e is finite in 64 bits is taken there: what is left is its rounding, beside e's own
+    relative error, which is the log-probability's absolute one of 2^-21 at most."""
+    x, ids, old, A, mask, ref = policy_inputs(n, V, dtype, seed=3)
+    mask[:] = True
+    A = A.abs() + 0.5
+    logp = logp_exact(x.double(), ids).float()
+    none = {"mask": mask, "clip": (0.2, 0.2), "denom": None}
+
+    def both(old_, A_, **more):
+        lx = x.detach().requires_grad_()
+        loss, _ = ab.policy_loss(lx, ids, old_, A_, **more)
+        one, _, dx = ab.policy_loss_grad(x, ids, old_, A_, **more)
+        assert torch.equal(one, loss)
+        return loss, torch.autograd.grad(loss, lx)[0], dx
+
+    def check(old_, A_, **more):
+        xe = x.double().requires_grad_()
+        le, _ = policy_exact(xe, ids, old_, A_.double(), **none, **more)
+        want, = torch.autograd.grad(le, xe)
+        assert bool(torch.isfinite(want).all())
+        loss, *got = both(old_, A_, **none, **more)
+        assert abs(float(loss) - float(le)) <= (F32 + 2.0 ** -21) * max(1.0, abs(float(le)))
+        for g in got:
+            close(g, want, "dlogits", more=2.0 ** -21)
+    zero = torch.where(torch.arange(n, device="cuda") % 3 == 0, torch.zeros_like(A), A)
+    far = torch.where(torch.arange(n, device="cuda") % 3 == 0, logp - 100.0, old)
+    check(far, zero, ref_logp=None, kl=0.0)                              # a ratio of e^100 with an advantage of 0
+    check(far, zero, ref_logp=ref, kl=0.05)
+    check(old, A, ref_logp=torch.where(torch.arange(n, device="cuda") % 4 == 1, logp + 100.0, ref), kl=0.0)
+    # e^89.5 is beyond 32 bits, a tenth of a millionth of it is not (and, times a probability, what the type holds)
+    if dtype != "fp16":
+        check(old, A, ref_logp=torch.where(torch.arange(n, device="cuda") == 1, logp + 89.5, ref), kl=1e-7)
+    # beyond 64 bits a factor of 0 is still 0
+    want = both(old, zero, ref_logp=None, kl=0.0, **none)
+    for got in (both(torch.where(zero == 0, logp - 800.0, old), zero, ref_logp=None, kl=0.0, **none), both(old, zero, ref_logp=logp + 800.0, kl=0.0, **none)):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    # with another sign the loss has no bound; a clipped ratio has one, and no gradient
+    gone = torch.where(torch.arange(n, device="cuda") == 2, logp - 800.0, old)
+    loss, *got = both(gone, A, ref_logp=None, kl=0.0, **none)
+    assert bool(torch.isfinite(loss)) and all(bool((g[2] == 0).all()) and bool(torch.isfinite(g).all()) for g in got)
+    assert float(both(gone, -A, ref_logp=None, kl=0.0, **none)[0]) == float("inf")
+
+
+@pytest.mark.parametrize("n,V", [(7, 1000), (7, 3001), (160, 20011)])
+def test_policy_gradient_of_small_gaps(n, V):
+    """Where the advantage is 0 the penalty's kl (1 - exp(ref - logp)) is the whole gradient. Rows of equal logits: exponentials and their sum are exact, so that the coefficient
+    is a matter of its own arithmetic. It comes from 64 bits (2^-52 of a log-probability of about 10, which over a gap of 1e-5 is 2e-10); up to six roundings to 32 bits follow
+    (the coefficient, the scale, the sum's reciprocal, products), 4e-7. A logarithm in 32 bits, 5e-7 off, would put it off by 5 %."""
+    x = torch.zeros(n, V, device="cuda")
+    ids = torch.arange(n, device="cuda") * 3 % V
+    logp = -torch.log(torch.tensor(float(V), dtype=torch.float64, device="cuda"))
+    gap = 10.0 ** -(1 + torch.arange(n, device="cuda", dtype=torch.float64) % 5)
+    ref = (logp + gap).float()
+    A = torch.zeros(n, device="cuda")
+    xe = x.double().requires_grad_()
+    le, _ = policy_exact(xe, ids, None, A.double(), None, ref, (0.2, 0.2), 0.05, None)
+    want, = torch.autograd.grad(le, xe)
+    lx = x.requires_grad_()
+    loss, _ = ab.policy_loss(lx, ids, None, A, ref_logp=ref, kl=0.05)
+    two, = torch.autograd.grad(loss, lx)
+    one = ab.policy_loss_grad(x.detach(), ids, None, A, ref_logp=ref, kl=0.05)[2]
+    for got in (one, two):
+        assert bool(((got.double() - want).abs() <= 1e-6 * want.abs()).all()), float(((got.double() - want).abs() / want.abs()).max())
+
+
 def test_policy_loss_of_no_tokens():
     x, ids, old, A, mask, ref = policy_inputs(9, 1000, "fp16")
     x[2], ids[3], old[4], A[5], ref[6] = float("nan"), -100, float("nan"), float("inf"), float("nan")

@@ -9,8 +9,9 @@
     preference_loss  pairs of a better and a worse answer; differentiable
 
 They run on the current stream of their tensors' device and take strided inputs (the last dimension dense; others are
-copied). Gradients are those of the formulas in include/albatross_b200.h; they cannot be differentiated again. The reference
-only generates: none of these has a counterpart there.
+copied). Gradients are those of the formulas in include/albatross_b200.h; they cannot be differentiated again,
+and there are no forward-mode derivatives: a tensor with a tangent is refused. The reference only generates: none of these has a
+counterpart there.
 
 Arguments are checked, memory is taken and gradients are tied to autograd in csrc/train_op.cpp (`torch.ops.albatross_b200`), which
 calls the C entries of the kernel library; what does not fit raises RuntimeError.
@@ -79,8 +80,8 @@ def policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logp: Optional[torc
 
     Per token, with ratio = exp(logp - old_logp): -min(ratio A, clamp(ratio, 1 - clip[0], 1 + clip[1]) A) + kl (exp(ref_logp - logp) - (ref_logp - logp) - 1);
     their sum where `mask` (bool [...]) is True, divided by `denom` or else by the number of such tokens (at least 1). logits [..., V], ids [...];
-    with kl 0 ref_logp is not looked at, and an advantage of 0
-    makes nothing of any ratio. old_logp, advantages and ref_logp broadcast to the ids' shape and get no gradient; old_logp None: the ratio is 1, as on the first step after
+    old_logp, advantages and ref_logp broadcast to the ids' shape and get no gradient; with kl 0 ref_logp does not count, and an advantage of 0
+    makes nothing of any ratio. old_logp None: the ratio is 1, as on the first step after
     sampling. At a border of the clip range the unclipped side's gradient counts."""
     return _policy_loss(logits, ids, old_logp, advantages, mask, ref_logp, clip[0], clip[1], kl, _denom(denom))
 

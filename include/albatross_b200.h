@@ -216,9 +216,9 @@ int ab_token_logp_fwd(const ab_logit_rows* t, double* logp, float* logp32, float
 int ab_token_logp_bwd(const ab_logit_rows* t, const float* stats, const float* g, int64_t rows_per_g, const float* scale, void* dlogits,
                       void* stream);
 /* The clipped policy loss: with ratio = exp(logp - old_logp), each row's is -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A), plus
- * kl * (exp(ref_logp - logp) - (ref_logp - logp) - 1) where ref_logp is not NULL and kl not 0 (ref_logp is not read otherwise); an
- * advantage of 0 makes nothing of any ratio. The loss is their sum over the rows that count by `denom`, or
- * where that is 0 by their number (at least 1). */
+ * kl * (exp(ref_logp - logp) - (ref_logp - logp) - 1) where ref_logp is not NULL and kl not 0 (what ref_logp holds does not count otherwise); an
+ * advantage of 0 makes nothing of any ratio. The loss is their sum over the rows that count by `denom`, or where that is 0 by their number (at
+ * least 1). */
 typedef struct ab_policy {
     const float *old_logp, *advantages, *ref_logp;   /* [rows]; old_logp NULL: the present policy's own (ratio 1) */
     float clip_low, clip_high, kl, denom;

@@ -938,6 +938,24 @@ def test_gradients_are_first_order_and_of_what_was_given():
         torch.autograd.grad(loss, lg)
 
 
+def test_forward_mode_derivatives_are_refused():
+    """A tangent is an error, not a derivative of zero; with and without a gradient asked for."""
+    import torch.autograd.forward_ad as forward_ad
+    x, w, b = norm_inputs(4, 256, "fp32")
+    lg, ids, _ = logit_inputs(4, 300, "fp16")
+    one, pairs = torch.ones(4, device="cuda"), (lg.view(4, 1, 300), ids.view(4, 1))
+    state, xs, _, _ = wkv_inputs(1, 5, 1, "fp16")
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for f in (lambda: ab.layer_norm(dual(x), w, b), lambda: ab.layer_norm(x, dual(w), b), lambda: ab.layer_norm(x, w, dual(b)), lambda: ab.layer_norm(dual(x.requires_grad_())),
+                  lambda: ab.token_logp(dual(lg), ids), lambda: ab.policy_loss(dual(lg), ids, None, one), lambda: ab.policy_loss(lg, ids, None, dual(one)),
+                  lambda: ab.policy_loss_grad(dual(lg), ids, None, one), lambda: ab.preference_loss(dual(pairs[0]), pairs[1], one),
+                  lambda: ab.RWKV7_TRAIN_OP(dual(state), *xs), lambda: ab.RWKV7_TRAIN_OP(state, *xs[:5], dual(xs[5]))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f()
+    ab.layer_norm(x, w, b)
+
+
 def test_capture_beside_a_living_graph_of_the_same_leaf_is_refused():
     """On the default stream such a graph ties the leaf to that stream, which cannot join a capture; nothing of the process is lost, and without that graph the capture is taken."""
     x = torch.randn(4, 256, device="cuda", requires_grad=True)

@@ -131,5 +131,17 @@ def test_python_entries_refuse_tensors_on_the_host():
             f()
 
 
+def test_python_entries_refuse_forward_mode_derivatives():
+    """Before anything else of the arguments is looked at, so that it shows on the host."""
+    import torch.autograd.forward_ad as forward_ad
+    x, ids, one = torch.zeros(2, 3, 64), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for f in (lambda: ab.RWKV7_TRAIN_OP(None, x, x, x, x, x, d), lambda: ab.layer_norm(x, None, d), lambda: ab.token_logp(d, ids), lambda: ab.policy_loss(x, ids, d, ids),
+                  lambda: ab.policy_loss_grad(x, ids, None, x, ref_logp=d), lambda: ab.preference_loss(d, ids, one)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f()
+
+
 def test_struct_layouts_match_the_header():
     assert C.sizeof(_lib.Wkv7Seq) == 16 + 48 + 96 + 24 and C.sizeof(_lib.LogitRows) == 48 and C.sizeof(_lib.Policy) == 40

@@ -7,6 +7,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -59,14 +60,24 @@ struct Plain {
     Tensor t;
 };
 OptTensor or_none(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-// A tangent would be lost without a word: its tensor need not require a gradient, and is then taken below autograd.
+// What would be lost without a word. A trace in the making would hold the outputs' allocation and not the call, and torch.func's wrappers have no memory. A tangent's tensor need not
+// require a gradient, and would be taken below autograd.
+bool traced() {
+    using Key = c10::impl::TorchDispatchModeKey;
+    for (const Key k : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL})
+        if (c10::impl::TorchDispatchModeTLS::get_mode(k).has_value()) return true;
+    return false;
+}
 template <class... T>
-void check_tangents(const char* who, const T&... t) {
+void check_plain(const char* who, const T&... t) {
+    TORCH_CHECK(!traced() && ((!t.defined() || t.has_storage()) && ...), who,
+                ": cannot be traced or transformed (torch.compile, torch.export, make_fx, torch.func.grad); in a compiled program call it from a function under torch.compiler.disable");
     TORCH_CHECK(!((t.defined() && t._fw_grad(/*level=*/0).defined()) || ...), who, ": forward-mode derivatives are not available");
 }
 // What a backward pass refuses. Gradients are not differentiable: asking for a graph of them is an error, not a silent zero. And in a stream capture a leaf that an earlier graph still ties
 // to the default stream: adding its gradient would make that stream wait for the capturing one, which the default stream cannot, and the capture would be lost with a less telling error.
 void check_backward() {
+    check_plain("albatross_b200: gradients");
     TORCH_CHECK(!at::GradMode::is_enabled(), "albatross_b200: the gradients of these operators cannot be differentiated again (create_graph)");
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
     const auto node = torch::autograd::get_current_node();
@@ -147,7 +158,7 @@ struct Wkv7 : torch::autograd::Function<Wkv7> {
     }
 };
 std::tuple<Tensor, Tensor> wkv7(const OptTensor& state_, const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, const Tensor& a, const Tensor& b, const OptTensor& lengths_) {
-    check_tangents("RWKV7_TRAIN_OP", given(state_), r, w, k, v, a, b);
+    check_plain("RWKV7_TRAIN_OP", given(state_), r, w, k, v, a, b, given(lengths_));
     TORCH_CHECK(r.dim() == 3 && r.is_cuda() && is_16bit(r), "RWKV7_TRAIN_OP: r must be [B, T, C], fp16 or bf16, on a CUDA device");
     const int64_t B = r.size(0), T = r.size(1), C = r.size(2);
     TORCH_CHECK(B > 0 && C > 0 && C % 64 == 0, "RWKV7_TRAIN_OP: heads are of 64 channels, got C = ", std::to_string(C));
@@ -225,7 +236,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
 };
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
-    check_tangents("layer_norm", x, given(weight), given(bias));
+    check_plain("layer_norm", x, given(weight), given(bias));
     TORCH_CHECK(x.is_cuda() && is_known(x) && x.dim() >= 1, "layer_norm: x must be fp16, bf16 or fp32 on a CUDA device");
     const int64_t C = x.size(-1);
     TORCH_CHECK(C > 0 && C <= INT32_MAX && groups > 0 && C % groups == 0, "layer_norm: ", std::to_string(C), " values do not make ", std::to_string(groups), " groups");
@@ -297,7 +308,7 @@ struct TokenLogp : torch::autograd::Function<TokenLogp> {
 };
 Tensor token_logp(const Tensor& logits, const Tensor& ids_, const OptTensor& mask_) {
     Tensor ids = ids_, mask = given(mask_);
-    check_tangents("token_logp", logits);
+    check_plain("token_logp", logits, ids_, given(mask_));
     check_rows("token_logp", logits, ids, mask);
     if (needs_grad(logits)) return TokenLogp::apply(logits, Plain{ids}, Plain{mask});
     at::AutoDispatchBelowADInplaceOrView below;
@@ -351,7 +362,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
 std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& ids_, const OptTensor& old_logp, const Tensor& advantages, const OptTensor& mask_, const OptTensor& ref_logp,
                                        double low, double high, double kl, double denom) {
     Tensor ids = ids_, mask = given(mask_);
-    check_tangents("policy_loss", logits, given(old_logp), advantages, given(ref_logp));
+    check_plain("policy_loss", logits, ids_, given(mask_), given(old_logp), advantages, given(ref_logp));
     check_rows("policy_loss", logits, ids, mask);
     const PolicyArgs a = policy_args(logits, ids, old_logp, advantages, ref_logp, low, high, kl, denom);
     if (needs_grad(logits)) {
@@ -365,7 +376,7 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& ids_,
 std::tuple<Tensor, Tensor, Tensor> policy_loss_grad(const Tensor& logits, const Tensor& ids_, const OptTensor& old_logp, const Tensor& advantages, const OptTensor& mask_,
                                                     const OptTensor& ref_logp, double low, double high, double kl, double denom, double scale, const OptTensor& out_) {
     Tensor ids = ids_, mask = given(mask_), out = given(out_);
-    check_tangents("policy_loss_grad", logits, given(old_logp), advantages, given(ref_logp));
+    check_plain("policy_loss_grad", logits, ids_, given(mask_), given(old_logp), advantages, given(ref_logp), given(out_));
     check_rows("policy_loss_grad", logits, ids, mask);
     const PolicyArgs a = policy_args(logits, ids, old_logp, advantages, ref_logp, low, high, kl, denom);
     at::AutoDispatchBelowADInplaceOrView below;
@@ -414,7 +425,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
 };
 std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& ids_, const Tensor& ref_logp, const OptTensor& mask_, double beta, double smoothing) {
     Tensor ids = ids_, mask = given(mask_);
-    check_tangents("preference_loss", logits, ref_logp);
+    check_plain("preference_loss", logits, ids_, given(mask_), ref_logp);
     check_rows("preference_loss", logits, ids, mask);
     TORCH_CHECK(logits.dim() == 3 && logits.size(0) % 2 == 0 && logits.size(0) > 0, "preference_loss: logits must be [2 P, T, V]");
     TORCH_CHECK(ref_logp.sizes() == at::IntArrayRef({logits.size(0)}) && ref_logp.device() == logits.device(), "preference_loss: ref_logp must be [2 P] on the device of logits");

@@ -10,8 +10,9 @@
 
 They run on the current stream of their tensors' device and take strided inputs (the last dimension dense; others are
 copied). Gradients are those of the formulas in include/albatross_b200.h; they cannot be differentiated again,
-and there are no forward-mode derivatives: a tensor with a tangent is refused. The reference only generates: none of these has a
-counterpart there.
+and there are no forward-mode derivatives: a tensor with a tangent is refused. Neither can they be traced (torch.compile, torch.export,
+make_fx: call them from a function under torch.compiler.disable) or transformed by torch.func.grad; torch.vmap calls them slice by slice. The
+reference only generates: none of these has a counterpart there.
 
 Arguments are checked, memory is taken and gradients are tied to autograd in csrc/train_op.cpp (`torch.ops.albatross_b200`), which
 calls the C entries of the kernel library; what does not fit raises RuntimeError.

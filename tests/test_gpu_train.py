@@ -956,6 +956,27 @@ def test_forward_mode_derivatives_are_refused():
     ab.layer_norm(x, w, b)
 
 
+def test_tracing_is_refused_and_slices_are_taken():
+    """A trace would hold the outputs' allocation and not the call. (torch.vmap calls the operator slice by slice.)"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, b = norm_inputs(4, 256, "fp32")
+    lg, ids, _ = logit_inputs(4, 300, "fp16")
+    state, xs, _, _ = wkv_inputs(1, 5, 1, "fp16")
+    one = torch.ones(4, device="cuda")
+    for f, args in ((lambda t: ab.layer_norm(t, w, b), x), (lambda t: ab.token_logp(t, ids), lg), (lambda t: ab.policy_loss(t, ids, None, one)[0], lg),
+                    (lambda t: ab.policy_loss_grad(t, ids, None, one)[2], lg), (lambda t: ab.preference_loss(t.view(4, 1, 300), ids.view(4, 1), one)[0], lg),
+                    (lambda t: ab.RWKV7_TRAIN_OP(t, *xs)[0], state)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(f)(args)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.func.grad(lambda t: f(t).float().sum())(args)
+        f(args)
+    assert torch.equal(torch.vmap(lambda t: ab.layer_norm(t, w, b))(x), ab.layer_norm(x, w, b))
+    # as a compiled program has them
+    part = torch.compiler.disable(lambda t: ab.layer_norm(t, w, b))
+    assert torch.equal(torch.compile(lambda t: part(t * 2.0) + 1.0, backend="eager")(x), ab.layer_norm(x * 2.0, w, b) + 1.0)
+
+
 def test_capture_beside_a_living_graph_of_the_same_leaf_is_refused():
     """On the default stream such a graph ties the leaf to that stream, which cannot join a capture; nothing of the process is lost, and without that graph the capture is taken."""
     x = torch.randn(4, 256, device="cuda", requires_grad=True)

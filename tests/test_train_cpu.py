@@ -143,5 +143,16 @@ def test_python_entries_refuse_forward_mode_derivatives():
                 f()
 
 
+def test_python_entries_refuse_to_be_traced():
+    """Tensors without memory, ahead of every other check."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, ids, one = torch.empty(2, 3, 64, device="cuda", dtype=torch.float16), torch.empty(2, 3, device="cuda", dtype=torch.int64), torch.empty(2, device="cuda")
+        for f in (lambda: ab.RWKV7_TRAIN_OP(None, x, x, x, x, x, x), lambda: ab.layer_norm(x), lambda: ab.token_logp(x, ids), lambda: ab.policy_loss(x, ids, None, one),
+                  lambda: ab.policy_loss_grad(x, ids, None, one), lambda: ab.preference_loss(x, ids, one)):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                f()
+
+
 def test_struct_layouts_match_the_header():
     assert C.sizeof(_lib.Wkv7Seq) == 16 + 48 + 96 + 24 and C.sizeof(_lib.LogitRows) == 48 and C.sizeof(_lib.Policy) == 40

@@ -258,6 +258,7 @@ struct Rows {   // what a loss works on; the tensors that are kept for its gradi
     Tensor logits, ids, mask, rows;
     ab_logit_rows t = {};
     Rows(const Tensor& logits_, const Tensor& ids_, const Tensor& mask_) : logits(logits_), ids(ids_), mask(mask_), rows(as_rows(logits_)) {
+        if (rows.size(0) > 1 && rows.stride(0) < rows.size(1)) rows = rows.contiguous();   // rows that share their values, as expand() makes them
         t.dtype = type_of(rows);
         t.vocab = (int32_t)rows.size(1);
         t.rows = rows.size(0), t.stride = rows.stride(0);

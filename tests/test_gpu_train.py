@@ -554,6 +554,32 @@ def test_token_logp_of_strided_logits_and_short_ids():
     assert ab.token_logp(x[:0], ids[:0]).shape == (0,)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_losses_of_rows_that_share_their_logits(dtype):
+    """One row of logits for many ids, by expand() or as a window over a longer one: gradients come back summed, as torch adds up what it expanded."""
+    x, ids, g = logit_inputs(6, 700, dtype)
+    dl = torch.randn(6, device="cuda", generator=g)
+    A = torch.randn(6, device="cuda", generator=g)
+    row = x[0].clone()
+    for shared in (lambda t: t.expand(6, 700), lambda t: t.as_strided((6, 400), (60, 1))):
+        one = row.detach().requires_grad_()
+        wide = shared(one)
+        at = ids % wide.shape[1]
+        dense = wide.detach().contiguous().requires_grad_()
+        logp, want = ab.token_logp(wide, at), ab.token_logp(dense, at)
+        assert torch.equal(logp, want)
+        got, = torch.autograd.grad(logp, wide, dl, retain_graph=True)
+        d, = torch.autograd.grad(want, dense, dl)
+        assert torch.equal(got, d)
+        if wide.stride(0) == 0:
+            assert torch.equal(torch.autograd.grad(logp, one, dl)[0], d.sum(0))
+        with torch.no_grad():
+            assert all(torch.equal(p, q) for p, q in zip(ab.policy_loss_grad(wide, at, None, A), ab.policy_loss_grad(dense, at, None, A)))
+            assert all(torch.equal(p, q) for p, q in zip(ab.policy_loss(wide, at, None, A), ab.policy_loss(dense, at, None, A)))
+    cube = row.expand(2, 3, 700)
+    assert all(torch.equal(p, q) for p, q in zip(ab.preference_loss(cube, ids.view(2, 3), A[:2]), ab.preference_loss(cube.contiguous(), ids.view(2, 3), A[:2])))
+
+
 def test_token_logp_of_more_than_2_to_the_31_logits():
     V, n = 65536, 33000
     x = torch.zeros(n, V, dtype=torch.float16, device="cuda")

@@ -82,7 +82,9 @@ void check_backward() {
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
-    for (const torch::autograd::Edge& e : node->next_edges()) {
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+        const torch::autograd::Edge& e = node->next_edge(i);
+        if (!node->task_should_compute_output(i)) continue;   // its gradient is not asked for: nothing waits
         if (!e.function || !dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) continue;
         const auto s = e.function->stream();
         TORCH_CHECK(!s || at::cuda::CUDAStream(*s).stream() != nullptr,

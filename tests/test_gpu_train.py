@@ -1030,6 +1030,26 @@ def test_capture_beside_a_living_graph_of_the_same_leaf_is_refused():
         assert torch.equal(leaf.grad, want)
 
 
+def test_capture_of_some_gradients_beside_a_living_graph_of_another_leaf():
+    """Only leaves whose gradient is asked for have to join the capture."""
+    x, w, b = (t.requires_grad_() for t in norm_inputs(4, 256, "fp32"))
+    living = ab.layer_norm(x.detach(), w, b).square().sum()         # ties weight and bias to the default stream
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        warm, = torch.autograd.grad(ab.layer_norm(x, w, b).square().sum(), x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        dx, = torch.autograd.grad(ab.layer_norm(x, w, b).square().sum(), x)
+    dx.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(dx, warm)
+    living.backward()
+    assert w.grad is not None and b.grad is not None
+
+
 def test_two_streams_at_once():
     """Calls that overlap share nothing."""
     p, ids, mask, A = small_problem()

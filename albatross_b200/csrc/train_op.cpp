@@ -382,12 +382,15 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_grad(const Tensor& logits, const 
     check_plain("policy_loss_grad", logits, ids_, given(mask_), given(old_logp), advantages, given(ref_logp), given(out_));
     check_rows("policy_loss_grad", logits, ids, mask);
     const PolicyArgs a = policy_args(logits, ids, old_logp, advantages, ref_logp, low, high, kl, denom);
+    // (torch refuses its own operators in place over these; a tensor that is no leaf has its version counted up)
+    const bool over_leaf = needs_grad(out) && (out.is_leaf() || (out.is_view() && out._base().is_leaf()));
     at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard guard(logits.device());
     if (!out.defined()) out = like(logits.sizes(), logits, logits.scalar_type());
     TORCH_CHECK(out.sizes() == logits.sizes() && out.scalar_type() == logits.scalar_type() && out.device() == logits.device() && out.is_contiguous(),
                 "policy_loss_grad: out must be dense and like the logits");
     if (out_.has_value()) {
+        TORCH_CHECK(!over_leaf, "policy_loss_grad: out is a leaf that requires a gradient, or a view of one");
         at::assert_no_partial_overlap(out, logits);
         if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();   // written in place: what autograd has kept of it is no longer good
     }

@@ -91,7 +91,7 @@ def policy_loss_grad(logits: torch.Tensor, ids: torch.Tensor, old_logp: Optional
                      mask: Optional[torch.Tensor] = None, ref_logp: Optional[torch.Tensor] = None, clip: Sequence[float] = (0.2, 0.2), kl: float = 0.0,
                      denom: Optional[float] = None, scale: float = 1.0, out: Optional[torch.Tensor] = None):
     """`policy_loss` and `scale` times its gradient by the logits, which are read once: (loss, logp, dlogits). `out`: where the gradient goes, dense
-    and like the logits; it may be the logits themselves. (For `logits.backward(dlogits)`; no autograd graph is made here.)"""
+    and like the logits; it may be the logits themselves, but, where gradients are recorded, no leaf that requires one. (For `logits.backward(dlogits)`; no autograd graph is made here.)"""
     return _policy_loss_grad(logits, ids, old_logp, advantages, mask, ref_logp, clip[0], clip[1], kl, _denom(denom), scale, out)
 
 

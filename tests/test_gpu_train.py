@@ -1003,6 +1003,25 @@ def test_tracing_is_refused_and_slices_are_taken():
     assert torch.equal(torch.compile(lambda t: part(t * 2.0) + 1.0, backend="eager")(x), ab.layer_norm(x * 2.0, w, b) + 1.0)
 
 
+def test_gradients_are_not_written_over_a_leaf_that_wants_one():
+    """As torch refuses its own operators in place; outside of a graph, and over logits that are no leaf, it is done."""
+    lg, ids, _ = logit_inputs(4, 300, "fp16")
+    A = torch.ones(4, device="cuda")
+    want = ab.policy_loss_grad(lg, ids, None, A)
+    leaf = lg.clone().requires_grad_()
+    before = leaf.detach().clone()
+    for out in (leaf, leaf.view(4, 300), leaf[:]):
+        with pytest.raises(RuntimeError, match="leaf"):
+            ab.policy_loss_grad(leaf, ids, None, A, out=out)
+        with pytest.raises(RuntimeError, match="leaf"):
+            ab.policy_loss_grad(lg, ids, None, A, out=out)
+    assert torch.equal(leaf.detach(), before)
+    with torch.no_grad():
+        assert torch.equal(ab.policy_loss_grad(leaf, ids, None, A, out=leaf)[2], want[2])
+    z = lg.clone().requires_grad_() * 1.0
+    assert torch.equal(ab.policy_loss_grad(z, ids, None, A, out=z)[2], want[2])
+
+
 def test_capture_beside_a_living_graph_of_the_same_leaf_is_refused():
     """On the default stream such a graph ties the leaf to that stream, which cannot join a capture; nothing of the process is lost, and without that graph the capture is taken."""
     x = torch.randn(4, 256, device="cuda", requires_grad=True)

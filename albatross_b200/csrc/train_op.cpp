@@ -189,6 +189,18 @@ std::tuple<Tensor, Tensor> wkv7(const OptTensor& state_, const Tensor& r, const 
 }
 
 // ---- the norms ---------------------------------------------------------------------------------------------------------------------
+// [..., C] with a dense last dimension and one stride between rows, of `least` values or more; others are copied. Here, ahead of autograd, so that the backward pass reads the same
+// copy (logits[:, :-1] of several sequences are copied once, not once in each pass).
+Tensor one_stride(const Tensor& t, int64_t least) {
+    bool fits = t.dim() < 1 || t.size(-1) <= 1 || t.stride(-1) == 1;
+    int64_t outer = -1;   // the stride that goes with the dimensions so far
+    for (int64_t d = t.dim() - 2; d >= 0 && fits; --d) {
+        if (t.size(d) == 1) continue;
+        fits = outer < 0 ? t.stride(d) >= least : t.stride(d) == outer;
+        outer = t.stride(d) * t.size(d);
+    }
+    return fits || t.numel() == 0 ? t : t.contiguous();
+}
 // [..., C] as rows [n, C] with a dense last dimension; a view where the strides allow one
 Tensor as_rows(const Tensor& t) {
     const Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
@@ -237,9 +249,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         return out;
     }
 };
-Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
-    check_plain("layer_norm", x, given(weight), given(bias));
-    TORCH_CHECK(x.is_cuda() && is_known(x) && x.dim() >= 1, "layer_norm: x must be fp16, bf16 or fp32 on a CUDA device");
+Tensor layer_norm(const Tensor& x_, const OptTensor& weight, const OptTensor& bias, double eps, int64_t groups) {
+    check_plain("layer_norm", x_, given(weight), given(bias));
+    TORCH_CHECK(x_.is_cuda() && is_known(x_) && x_.dim() >= 1, "layer_norm: x must be fp16, bf16 or fp32 on a CUDA device");
+    const Tensor x = one_stride(x_, 0);
     const int64_t C = x.size(-1);
     TORCH_CHECK(C > 0 && C <= INT32_MAX && groups > 0 && C % groups == 0, "layer_norm: ", std::to_string(C), " values do not make ", std::to_string(groups), " groups");
     Tensor w = given(weight), b = given(bias);
@@ -260,7 +273,6 @@ struct Rows {   // what a loss works on; the tensors that are kept for its gradi
     Tensor logits, ids, mask, rows;
     ab_logit_rows t = {};
     Rows(const Tensor& logits_, const Tensor& ids_, const Tensor& mask_) : logits(logits_), ids(ids_), mask(mask_), rows(as_rows(logits_)) {
-        if (rows.size(0) > 1 && rows.stride(0) < rows.size(1)) rows = rows.contiguous();   // rows that share their values, as expand() makes them
         t.dtype = type_of(rows);
         t.vocab = (int32_t)rows.size(1);
         t.rows = rows.size(0), t.stride = rows.stride(0);
@@ -269,12 +281,13 @@ struct Rows {   // what a loss works on; the tensors that are kept for its gradi
         t.mask = static_cast<const uint8_t*>(ptr(mask));
     }
 };
-void check_rows(const char* who, const Tensor& logits, Tensor& ids, Tensor& mask) {
+void check_rows(const char* who, Tensor& logits, Tensor& ids, Tensor& mask) {
     TORCH_CHECK(logits.is_cuda() && is_known(logits) && logits.dim() >= 1 && logits.size(-1) > 0 && logits.size(-1) <= INT32_MAX, who,
                 ": logits must be [..., V], fp16, bf16 or fp32, on a CUDA device");
     TORCH_CHECK(ids.sizes() == logits.sizes().slice(0, logits.dim() - 1) && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.device() == logits.device(), who,
                 ": ids must be int64 or int32 of the shape of logits without its last dimension, on its device");
     TORCH_CHECK(!mask.defined() || (mask.sizes() == ids.sizes() && mask.scalar_type() == at::kBool && mask.device() == logits.device()), who, ": mask must be bool of the ids' shape");
+    logits = one_stride(logits, logits.size(-1));   // (rows that share their values, as expand() makes them, are copied too)
     ids = ids.to(at::kLong).contiguous();
     if (mask.defined()) mask = mask.contiguous();
 }
@@ -309,9 +322,9 @@ struct TokenLogp : torch::autograd::Function<TokenLogp> {
         return {dlogits_of(s[0], s[1], s[2], s[3], grads[0].contiguous(), 1, Tensor()), Tensor(), Tensor()};
     }
 };
-Tensor token_logp(const Tensor& logits, const Tensor& ids_, const OptTensor& mask_) {
-    Tensor ids = ids_, mask = given(mask_);
-    check_plain("token_logp", logits, ids_, given(mask_));
+Tensor token_logp(const Tensor& logits_, const Tensor& ids_, const OptTensor& mask_) {
+    Tensor logits = logits_, ids = ids_, mask = given(mask_);
+    check_plain("token_logp", logits_, ids_, given(mask_));
     check_rows("token_logp", logits, ids, mask);
     if (needs_grad(logits)) return TokenLogp::apply(logits, Plain{ids}, Plain{mask});
     at::AutoDispatchBelowADInplaceOrView below;
@@ -362,10 +375,10 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         return {dlogits_of(s[0], s[1], s[2], s[3], s[4], 1, grads[0].contiguous()), Tensor(), Tensor(), Tensor()};
     }
 };
-std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& ids_, const OptTensor& old_logp, const Tensor& advantages, const OptTensor& mask_, const OptTensor& ref_logp,
+std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits_, const Tensor& ids_, const OptTensor& old_logp, const Tensor& advantages, const OptTensor& mask_, const OptTensor& ref_logp,
                                        double low, double high, double kl, double denom) {
-    Tensor ids = ids_, mask = given(mask_);
-    check_plain("policy_loss", logits, ids_, given(mask_), given(old_logp), advantages, given(ref_logp));
+    Tensor logits = logits_, ids = ids_, mask = given(mask_);
+    check_plain("policy_loss", logits_, ids_, given(mask_), given(old_logp), advantages, given(ref_logp));
     check_rows("policy_loss", logits, ids, mask);
     const PolicyArgs a = policy_args(logits, ids, old_logp, advantages, ref_logp, low, high, kl, denom);
     if (needs_grad(logits)) {
@@ -376,10 +389,10 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& ids_,
     auto [loss, logp] = policy_forward(logits, ids, mask, a, nullptr, nullptr);
     return {loss, logp};
 }
-std::tuple<Tensor, Tensor, Tensor> policy_loss_grad(const Tensor& logits, const Tensor& ids_, const OptTensor& old_logp, const Tensor& advantages, const OptTensor& mask_,
+std::tuple<Tensor, Tensor, Tensor> policy_loss_grad(const Tensor& logits_, const Tensor& ids_, const OptTensor& old_logp, const Tensor& advantages, const OptTensor& mask_,
                                                     const OptTensor& ref_logp, double low, double high, double kl, double denom, double scale, const OptTensor& out_) {
-    Tensor ids = ids_, mask = given(mask_), out = given(out_);
-    check_plain("policy_loss_grad", logits, ids_, given(mask_), given(old_logp), advantages, given(ref_logp), given(out_));
+    Tensor logits = logits_, ids = ids_, mask = given(mask_), out = given(out_);
+    check_plain("policy_loss_grad", logits_, ids_, given(mask_), given(old_logp), advantages, given(ref_logp), given(out_));
     check_rows("policy_loss_grad", logits, ids, mask);
     const PolicyArgs a = policy_args(logits, ids, old_logp, advantages, ref_logp, low, high, kl, denom);
     // (torch refuses its own operators in place over these; a tensor that is no leaf has its version counted up)
@@ -391,7 +404,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_grad(const Tensor& logits, const 
                 "policy_loss_grad: out must be dense and like the logits");
     if (out_.has_value()) {
         TORCH_CHECK(!over_leaf, "policy_loss_grad: out is a leaf that requires a gradient, or a view of one");
-        at::assert_no_partial_overlap(out, logits);
+        at::assert_no_partial_overlap(out, logits_);
         if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();   // written in place: what autograd has kept of it is no longer good
     }
     const Rows r(logits, ids, mask);
@@ -429,9 +442,9 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
         return out;
     }
 };
-std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& ids_, const Tensor& ref_logp, const OptTensor& mask_, double beta, double smoothing) {
-    Tensor ids = ids_, mask = given(mask_);
-    check_plain("preference_loss", logits, ids_, given(mask_), ref_logp);
+std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits_, const Tensor& ids_, const Tensor& ref_logp, const OptTensor& mask_, double beta, double smoothing) {
+    Tensor logits = logits_, ids = ids_, mask = given(mask_);
+    check_plain("preference_loss", logits_, ids_, given(mask_), ref_logp);
     check_rows("preference_loss", logits, ids, mask);
     TORCH_CHECK(logits.dim() == 3 && logits.size(0) % 2 == 0 && logits.size(0) > 0, "preference_loss: logits must be [2 P, T, V]");
     TORCH_CHECK(ref_logp.sizes() == at::IntArrayRef({logits.size(0)}) && ref_logp.device() == logits.device(), "preference_loss: ref_logp must be [2 P] on the device of logits");

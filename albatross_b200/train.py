@@ -8,8 +8,8 @@
     policy_loss_grad the same, loss and gradient by the logits in one pass over them
     preference_loss  pairs of a better and a worse answer; differentiable
 
-They run on the current stream of their tensors' device and take strided inputs (the last dimension dense; others are
-copied). Gradients are those of the formulas in include/albatross_b200.h; they cannot be differentiated again,
+They run on the current stream of their tensors' device and take strided inputs (the last dimension dense and, but for
+the recurrence, one stride between rows: logits[:, :-1] of several sequences has two. Others are copied, once for both passes). Gradients are those of the formulas in include/albatross_b200.h; they cannot be differentiated again,
 and there are no forward-mode derivatives: a tensor with a tangent is refused. Neither can they be traced (torch.compile, torch.export,
 make_fx: call them from a function under torch.compiler.disable) or transformed by torch.func.grad; torch.vmap calls them slice by slice. The
 reference only generates: none of these has a counterpart there.

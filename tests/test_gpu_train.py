@@ -793,6 +793,42 @@ def test_policy_loss_of_many_long_rows(n, V, dtype):
     assert _lib.device_status() == 0
 
 
+def test_losses_of_next_tokens_copy_their_logits_once():
+    """logits[:, :-1] of several sequences has no one stride between rows: it is copied, and the copy is what the backward pass reads."""
+    x, ids, g = logit_inputs(2 * 33, 60000, "fp32")
+    cube, ids = x.view(2, 33, 60000), ids.view(2, 33)
+    A = torch.randn(2, 32, device="cuda", generator=g)
+    size = 2 * 32 * 60000 * 4
+    for f in (lambda t: ab.token_logp(t, ids[:, 1:]).sum(), lambda t: ab.policy_loss(t, ids[:, 1:], None, A)[0], lambda t: ab.preference_loss(t, ids[:, 1:], A[:, 0])[0]):
+        leaf = cube.detach().requires_grad_()
+        part = leaf[:, :-1]
+        loss = f(part)
+        dense = part.detach().contiguous().requires_grad_()
+        want, = torch.autograd.grad(f(dense), dense)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got, = torch.autograd.grad(loss, part)
+        assert torch.cuda.max_memory_allocated() - before < 1.5 * size      # the gradient, and no second copy
+        assert torch.equal(got, want)
+
+
+def test_layer_norm_of_rows_with_two_strides_copies_them_once():
+    x, w, b = norm_inputs(2 * 1025, 4096, "fp32")
+    leaf = x.view(2, 1025, 4096).requires_grad_()
+    part = leaf[:, 1:]
+    y = ab.layer_norm(part, w, b)
+    dy = torch.randn_like(y)
+    dense = part.detach().contiguous().requires_grad_()
+    want, = torch.autograd.grad(ab.layer_norm(dense, w, b), dense, dy)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got, = torch.autograd.grad(y, part, dy)
+    assert torch.cuda.max_memory_allocated() - before < 1.5 * 2 * 1024 * 4096 * 4
+    assert torch.equal(got, want) and torch.equal(y, ab.layer_norm(dense, w, b))
+
+
 def test_preference_loss_of_no_steps():
     x, ids = torch.zeros(2, 0, 50, device="cuda"), torch.zeros(2, 0, dtype=torch.int64, device="cuda")
     lx = x.requires_grad_()

@@ -829,6 +829,44 @@ def test_layer_norm_of_rows_with_two_strides_copies_them_once():
     assert torch.equal(got, want) and torch.equal(y, ab.layer_norm(dense, w, b))
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("V", [16385, 16391, 32771, 7 * 16384 - 3, 7 * 16384 + 5, 8 * 16384 - 7, 57341, 57347])
+def test_policy_loss_over_the_ends_of_long_rows(V, dtype):
+    """Rows just beyond what clusters take, and around the ring's seven chunks (16384 values of two bytes each, 8192 of four), on every address that their type allows; the id and a
+    value that outweighs the rest stand at the ends in turn, where a row's first and last pieces are not copied. A sum of exponentials good to 2^-22 each: its logarithm is
+    off by 2^-21, and a log-probability of up to 30 is rounded by 2^-20 more at most."""
+    n = 152
+    x, ids, old, A, mask, ref = policy_inputs(n, V, dtype, seed=V)
+    ends = torch.tensor([0, 1, V - 2, V - 1], device="cuda")
+    rows = torch.arange(n, device="cuda")
+    top, ids = ends[rows % 4], ends[rows // 4 % 4]
+    x[rows, top] = 14.0
+    mask[rows[::11]] = False
+    logp = logp_exact(x.double(), ids)
+    old, ref = (logp + 0.05 * old.sin()).float(), (logp + 0.3 * ref.cos()).float()
+    scale = 65536.0 if dtype == "fp16" else 1.0
+    more = {"mask": mask, "ref_logp": ref, "clip": (0.1, 0.3), "kl": 0.05, "denom": None}
+    xe = x.double().requires_grad_()
+    le, logpe = policy_exact(xe, ids, old, A.double(), **more)
+    want, = torch.autograd.grad(le * scale, xe)
+    x[~mask] = float("nan")
+    here = x.clone()
+    lx = x.requires_grad_()
+    loss, logp = ab.policy_loss(lx, ids, old, A, **more)
+    two, = torch.autograd.grad(loss * scale, lx)
+    one = ab.policy_loss_grad(x.detach(), ids, old, A, scale=scale, **more)
+    place = ab.policy_loss_grad(here, ids, old, A, scale=scale, out=here, **more)
+    for a, b, g in ((loss, logp, two), one, place):
+        assert abs(float(a) - float(le)) <= F32 * (float(A.abs().max()) * 3 + 1)
+        assert float((b.detach().double() - logpe.detach()).abs().max()) <= 2.0 ** -21 + 2.0 ** -20
+        close(g, want, "dlogits")
+        # the ids' own values, each for itself: coefficient (1 - p), where p is off by its exponential's 2^-22, the sum's as much and, for logits of 14, 2.7e-7 of log2(e)'s own rounding
+        most = (1.1 * float(A.abs().max()) + 0.1) * scale / float(mask.sum())
+        own = want[rows, ids]
+        assert bool(((g.double()[rows, ids] - own).abs() <= torch.finfo(g.dtype).eps / 2 * own.abs() + 2.0 ** -20 * most + 2.0 ** -25).all())
+    assert _lib.device_status() == 0
+
+
 def test_preference_loss_of_no_steps():
     x, ids = torch.zeros(2, 0, 50, device="cuda"), torch.zeros(2, 0, dtype=torch.int64, device="cuda")
     lx = x.requires_grad_()

@@ -85,7 +85,8 @@ struct Pieces {
     static constexpr int N = 16 / sizeof(E);
     const E* x;        // the first piece's address
     int lead, n, V;    // values of the first piece in front of the row; pieces; values of the row
-    __device__ __forceinline__ Pieces(const E* row, int V_) : V(V_) {
+    Extent in;         // the rows' whole array
+    __device__ __forceinline__ Pieces(const E* row, int V_, const Extent& in_) : V(V_), in(in_) {
         lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(E));
         x = row - lead;
         n = (V + lead + N - 1) / N;
@@ -94,20 +95,25 @@ struct Pieces {
     __device__ __forceinline__ bool all_whole(int i0, int i1) const { return i0 * N >= lead && i1 * N <= V + lead; }
     template <bool FULL>
     __device__ __forceinline__ uint4 get(int i) const {
-        if (FULL) return AB_BC(whole(i)) ? __ldcs(reinterpret_cast<const uint4*>(x) + i) : none();
+        if (FULL) return piece(i);
         return load(i);
     }
     __device__ __forceinline__ bool whole(int i) const { return i * N >= lead && (i + 1) * N <= V + lead; }
     __device__ __forceinline__ uint4 load(int i) const {
         if (i >= n) return none();
-        if (whole(i)) return AB_BC(i * N - lead + N <= V) ? __ldcs(reinterpret_cast<const uint4*>(x) + i) : none();
+        if (whole(i)) return piece(i);
         uint4 u = none();
         E* e = reinterpret_cast<E*>(&u);
 #pragma unroll
         for (int c = 0; c < N; ++c)
-            if (i * N + c >= lead && i * N + c < V + lead) e[c] = x[i * N + c];
+            if (i * N + c >= lead && i * N + c < V + lead && in.holds(x + i * N + c)) e[c] = x[i * N + c];
         return u;
     }
+    __device__ __forceinline__ uint4 piece(int i) const {
+        const uint4* p = reinterpret_cast<const uint4*>(x) + i;
+        return in.holds(p) ? __ldcs(p) : none();
+    }
+    __device__ __forceinline__ float value(int id) const { return in.holds(x + lead + id) ? to_f(x[lead + id]) : 0.f; }
     static __device__ __forceinline__ uint4 none() {   // -inf throughout
         const uint32_t w = sizeof(E) == 4 ? 0xff800000u : std::is_same<E, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
         return make_uint4(w, w, w, w);
@@ -207,7 +213,7 @@ __device__ __forceinline__ float rebase(const Ref& from, const Ref& to) {
 // Writes p times a piece's exponentials to the row `dx`, which starts `lead` values into a piece of 16 bytes as the row of logits does (aligned), or anywhere.
 // FULL: the piece holds values of the row alone, and dx is aligned.
 template <class E, bool FULL>
-__device__ __forceinline__ void write_piece(const Pieces<E>& row, const float* e, int i, E* dx, bool aligned, float p) {
+__device__ __forceinline__ void write_piece(const Pieces<E>& row, const float* e, int i, E* dx, bool aligned, float p, const Extent& grads) {
     constexpr int N = Pieces<E>::N;
     if (!FULL && i >= row.n) return;
     float f[N];
@@ -216,24 +222,33 @@ __device__ __forceinline__ void write_piece(const Pieces<E>& row, const float* e
     const int first = i * N - row.lead;
     const uint4 out = pack<E>(f);
     if (FULL || (aligned && row.whole(i))) {
-        if (AB_BC(first >= 0 && first + N <= row.V)) __stcs(reinterpret_cast<uint4*>(dx - row.lead) + i, out);
+        uint4* to = reinterpret_cast<uint4*>(dx - row.lead) + i;
+        if (grads.holds(to)) __stcs(to, out);
     } else {
         const E* o = reinterpret_cast<const E*>(&out);
 #pragma unroll
         for (int c = 0; c < N; ++c)
-            if (first + c >= 0 && first + c < row.V) dx[first + c] = o[c];
+            if (first + c >= 0 && first + c < row.V && grads.holds(dx + first + c)) dx[first + c] = o[c];
     }
 }
 template <class E>
-__device__ __forceinline__ void write_zeros(E* dx, int V, int at, int step) {   // this thread's share: pieces at, at + step, ...
-    const Pieces<E> row(dx, V);
+__device__ __forceinline__ void write_zeros(E* dx, int V, int at, int step, const Extent& grads) {   // this thread's share: pieces at, at + step, ...
+    const Pieces<E> row(dx, V, grads);
     for (int i = at; i < row.n; i += step) {
         const int first = i * Pieces<E>::N - row.lead;
-        if (row.whole(i)) __stcs(reinterpret_cast<uint4*>(dx + first), make_uint4(0, 0, 0, 0));
-        else
-            for (int c = max(first, 0); c < min(first + Pieces<E>::N, V); ++c) dx[c] = from_f<E>(0.f);
+        if (row.whole(i)) {
+            if (grads.holds(reinterpret_cast<uint4*>(dx + first))) __stcs(reinterpret_cast<uint4*>(dx + first), make_uint4(0, 0, 0, 0));
+        } else {
+            for (int c = max(first, 0); c < min(first + Pieces<E>::N, V); ++c)
+                if (grads.holds(dx + c)) dx[c] = from_f<E>(0.f);
+        }
     }
 }
+
+template <class E>
+__device__ __forceinline__ Extent logits_extent(const ab_logit_rows& t) { return rows_extent(t.logits, t.rows, t.stride, t.vocab, sizeof(E)); }
+template <class E>
+__device__ __forceinline__ Extent grads_extent(const ab_logit_rows& t, const void* dlogits) { return rows_extent(dlogits, t.rows, t.vocab, t.vocab, sizeof(E)); }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -274,7 +289,8 @@ __device__ __forceinline__ int count_rows(const uint8_t* mask, int64_t rows) {
     const int lead = (int)min((int64_t)((16 - (reinterpret_cast<uintptr_t>(mask) & 15)) & 15), rows), pieces = (int)((rows - lead) / 16);
     int n = 0;
     for (int i = threadIdx.x; i < pieces; i += LT) {
-        const uint4 u = *(reinterpret_cast<const uint4*>(mask + lead) + i);   // bytes of 0 and 1
+        const uint4* p = reinterpret_cast<const uint4*>(mask + lead) + i;
+        const uint4 u = Extent(mask, rows).holds(p) ? *p : make_uint4(0, 0, 0, 0);   // bytes of 0 and 1
         n = __dp4a(u.x, 0x01010101u, __dp4a(u.y, 0x01010101u, __dp4a(u.z, 0x01010101u, __dp4a(u.w, 0x01010101u, (unsigned)n))));
     }
     if ((int)threadIdx.x < lead) n += mask[threadIdx.x];
@@ -295,7 +311,9 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
     const int64_t r = blockIdx.x / nb;
     const int V = k.t.vocab, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     E* dx = k.dlogits ? static_cast<E*>(k.dlogits) + r * V : nullptr;
+    const Extent grads = grads_extent<E>(k.t, k.dlogits);
     pdl_launch_dependents();
+    if (!AB_BC(r < k.t.rows)) return;
     if (!counts(k.t, r)) {
         if (tid == 0 && rank == 0) {
             if (k.logp) k.logp[r] = 0.0;
@@ -304,11 +322,11 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
             if (k.slope) k.slope[r] = 0.0;
             if (k.stats) k.stats[2 * r] = k.stats[2 * r + 1] = 0.f;
         }
-        if (dx) write_zeros(dx, V, (int)rank * LT + tid, (int)nb * LT);
+        if (dx) write_zeros(dx, V, (int)rank * LT + tid, (int)nb * LT, grads);
         return;
     }
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // (the blocks of a row all come here: its mask is theirs)
-    const Pieces<E> row(static_cast<const E*>(k.t.logits) + r * k.t.stride, V);
+    const Pieces<E> row(static_cast<const E*>(k.t.logits) + r * k.t.stride, V, logits_extent<E>(k.t));
     const int step = (int)nb * LT * NV, at0 = (int)rank * LT * NV;
     const bool aligned = dx && (reinterpret_cast<uintptr_t>(dx) & 15) == row.lead * sizeof(E);
     const bool once = row.n <= step, full = once && row.all_whole(at0, at0 + LT * NV) && (aligned || !dx);
@@ -321,7 +339,7 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
         for (int j = 0; j < NV; ++j) u[j] = row.template get<decltype(whole)::value>(base + at0 + j * LT + tid);
         if (base == 0) {
             id = row_id(k.t, r);
-            at = to_f(row.x[row.lead + id]);
+            at = row.value(id);
             if (k.policy) pr = policy_load(k.p, r);
         }
         uint4 top4 = u[0];
@@ -397,21 +415,21 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
     const float mine = p * (m == -INFINITY ? 1.f : rebase(Ref(m), ref));   // the exponentials are relative to the warp's maximum
     if (full) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) write_piece<E, true>(row, e + j * N, at0 + j * LT + tid, dx, aligned, mine);
+        for (int j = 0; j < NV; ++j) write_piece<E, true>(row, e + j * N, at0 + j * LT + tid, dx, aligned, mine, grads);
     } else if (once) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) write_piece<E, false>(row, e + j * N, at0 + j * LT + tid, dx, aligned, mine);
+        for (int j = 0; j < NV; ++j) write_piece<E, false>(row, e + j * N, at0 + j * LT + tid, dx, aligned, mine, grads);
     } else {
         for (int i = at0; i < row.n; i += step)
             for (int j = 0; j < NV; ++j) {
                 unpack<E>(row.load(i + j * LT + tid), e);
                 exp_from<N>(e, ref);
-                write_piece<E, false>(row, e, i + j * LT + tid, dx, aligned, p);
+                write_piece<E, false>(row, e, i + j * LT + tid, dx, aligned, p, grads);
             }
     }
     // the id's own value, by the thread that wrote its piece
     const int own = (id + row.lead) / N - at0;
-    if (own >= 0 && own % step < LT * NV && own % LT == tid) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));
+    if (own >= 0 && own % step < LT * NV && own % LT == tid && grads.holds(dx + id)) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));
 }
 
 // ---- long rows, at least one per SM ----------------------------------------------------------------------------------
@@ -471,6 +489,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
         return false;
     };
     const E* logits = static_cast<const E*>(k.t.logits);
+    const Extent in = logits_extent<E>(k.t), grads = grads_extent<E>(k.t, k.dlogits);
     // the pieces of a row that are copied: those that hold its values alone
     auto span = [&](const Pieces<E>& row, int& first, int& end) {
         first = row.lead ? 1 : 0;
@@ -498,7 +517,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
                 if (r >= 0) {
                     q.on = counts(k.t, r);
                     if (q.on) {
-                        const Pieces<E> row(logits + r * k.t.stride, V);
+                        const Pieces<E> row(logits + r * k.t.stride, V, in);
                         int first, end;
                         span(row, first, end);
                         const int chunks = (end - first + CP - 1) / CP, rounds = chunks > RING_SLOTS && k.dlogits ? 2 : 1;
@@ -508,13 +527,18 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
                                 const int slot = c_issued % RING_SLOTS, p0 = first + c * CP, np = min(CP, end - p0);
                                 if (c_issued >= RING_SLOTS) ok = wait_for(&sh.vacant[slot], (uint32_t)(c_issued / RING_SLOTS - 1) & 1u);
                                 if (!ok) break;
-                                mbar_expect_tx(&sh.full[slot], np * 16);
-                                bulk_g2s(ring + (size_t)slot * RING_CHUNK, reinterpret_cast<const uint4*>(row.x) + p0, np * 16, &sh.full[slot]);
+                                const uint4* from = reinterpret_cast<const uint4*>(row.x) + p0;
+                                if (in.holds(from, np) && AB_BC(slot >= 0 && np > 0 && slot * RING_CHUNK + np * 16 <= RING_SLOTS * RING_CHUNK && np * 16 <= RING_CHUNK)) {
+                                    mbar_expect_tx(&sh.full[slot], np * 16);
+                                    bulk_g2s(ring + (size_t)slot * RING_CHUNK, from, np * 16, &sh.full[slot]);
+                                } else {
+                                    mbar_arrive(&sh.full[slot]);
+                                }
                                 if (!published) {                        // the rest of what the row needs, while its first chunk travels
                                     published = true;
                                     const int64_t id = k.t.ids[r];
                                     q.id = (uint64_t)id < (uint64_t)V ? (int)id : (atomicOr(&g_device_status, DEV_BAD_TOKEN), id < 0 ? 0 : V - 1);
-                                    q.at = to_f(row.x[row.lead + q.id]);
+                                    q.at = row.value(q.id);
                                     if (k.policy) q.pr = policy_load(k.p, r);
                                     mbar_arrive(&sh.row_full[n % RING_ROWS]);
                                 }
@@ -529,7 +553,7 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
                                  " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
                                  " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n}"
                                  : "=r"(got), "=r"(next) : "r"(smem_u32(&sh.cancel)) : "memory");
-                    r = got ? (int64_t)next : -1;
+                    r = got && AB_BC(next < k.t.rows) ? (int64_t)next : -1;
                 } else {
                     mbar_arrive(&sh.row_full[n % RING_ROWS]);
                     break;
@@ -592,12 +616,12 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
             if (r < 0) break;
             E* dx = k.dlogits ? static_cast<E*>(k.dlogits) + r * V : nullptr;
             if (!q.on) {
-                if (dx) write_zeros(dx, V, tid, RING_WARPS * 32);
+                if (dx) write_zeros(dx, V, tid, RING_WARPS * 32, grads);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.row_summed[n % RING_ROWS]), mbar_arrive(&sh.row_vacant[n % RING_ROWS]);
                 continue;
             }
-            const Pieces<E> row(logits + r * k.t.stride, V);
+            const Pieces<E> row(logits + r * k.t.stride, V, in);
             int first, end;
             span(row, first, end);
             const int chunks = (end - first + CP - 1) / CP;
@@ -690,8 +714,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
                     for (int j = 0; j < PER; ++j) {
                         const int i = c * CP + j * RING_WARPS * 32 + tid;
                         if (i < end - first) {
-                            if (aligned) write_piece<E, true>(row, e[j], first + i, dx, true, p);
-                            else write_piece<E, false>(row, e[j], first + i, dx, false, p);
+                            if (aligned) write_piece<E, true>(row, e[j], first + i, dx, true, p, grads);
+                            else write_piece<E, false>(row, e[j], first + i, dx, false, p, grads);
                         }
                     }
                 }
@@ -699,11 +723,11 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
                     float e[N];
                     unpack<E>(eu, e);
                     exp_from<N>(e, ref);
-                    write_piece<E, false>(row, e, edge, dx, aligned, p);
+                    write_piece<E, false>(row, e, edge, dx, aligned, p, grads);
                 }
                 // the id's own value, by the thread that wrote its piece
                 const int piece = (id + row.lead) / N;
-                if (piece >= first && piece < end ? (piece - first) % (RING_WARPS * 32) == tid : piece == edge) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));
+                if ((piece >= first && piece < end ? (piece - first) % (RING_WARPS * 32) == tid : piece == edge) && grads.holds(dx + id)) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.row_vacant[n % RING_ROWS]);
@@ -736,6 +760,7 @@ __global__ void __launch_bounds__(LT, 3) logit_short_kernel(const __grid_constan
     const int64_t r = (int64_t)blockIdx.x * LW + warp;
     if (r >= k.t.rows) return;
     E* dx = k.dlogits ? static_cast<E*>(k.dlogits) + r * V : nullptr;
+    const Extent grads = grads_extent<E>(k.t, k.dlogits);
     if (!counts(k.t, r)) {
         if (lane == 0) {
             if (k.logp) k.logp[r] = 0.0;
@@ -744,17 +769,17 @@ __global__ void __launch_bounds__(LT, 3) logit_short_kernel(const __grid_constan
             if (k.slope) k.slope[r] = 0.0;
             if (k.stats) k.stats[2 * r] = k.stats[2 * r + 1] = 0.f;
         }
-        if (dx) write_zeros(dx, V, lane, 32);
+        if (dx) write_zeros(dx, V, lane, 32, grads);
         return;
     }
-    const Pieces<E> row(static_cast<const E*>(k.t.logits) + r * k.t.stride, V);
+    const Pieces<E> row(static_cast<const E*>(k.t.logits) + r * k.t.stride, V, logits_extent<E>(k.t));
     uint4 u[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) u[j] = row.load(j * 32 + lane);
     const int64_t said = k.t.ids[r];
     const int id = (uint64_t)said < (uint64_t)V ? (int)said : said < 0 ? 0 : V - 1;
     if (lane == 0 && id != said) atomicOr(&g_device_status, DEV_BAD_TOKEN);
-    const float at = to_f(row.x[row.lead + id]);
+    const float at = row.value(id);
     PolicyRow pr = {};
     if (k.policy) pr = policy_load(k.p, r);
     uint4 top4 = u[0];
@@ -790,8 +815,8 @@ __global__ void __launch_bounds__(LT, 3) logit_short_kernel(const __grid_constan
     const float p = -g / S;
     const bool aligned = (reinterpret_cast<uintptr_t>(dx) & 15) == row.lead * sizeof(E);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) write_piece<E, false>(row, e + j * N, j * 32 + lane, dx, aligned, p);
-    if (((id + row.lead) / N) % 32 == lane) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));   // (by the thread that wrote its piece)
+    for (int j = 0; j < NV; ++j) write_piece<E, false>(row, e + j * N, j * 32 + lane, dx, aligned, p, grads);
+    if (((id + row.lead) / N) % 32 == lane && grads.holds(dx + id)) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));   // (by the thread that wrote its piece)
 }
 
 struct DlogitsTask {
@@ -808,11 +833,13 @@ __global__ void __launch_bounds__(LT, 6) dlogits_kernel(const __grid_constant__ 
     const int64_t r = blockIdx.x / k.blocks;
     const int V = k.t.vocab, blk = (int)(blockIdx.x - r * k.blocks), tid = threadIdx.x, at0 = blk * LT * DV;
     E* dx = static_cast<E*>(k.dlogits) + r * V;
+    const Extent grads = grads_extent<E>(k.t, k.dlogits);
+    if (!AB_BC(r < k.t.rows)) return;
     if (!counts(k.t, r)) {
-        write_zeros(dx, V, blk * LT + tid, k.blocks * LT);
+        write_zeros(dx, V, blk * LT + tid, k.blocks * LT, grads);
         return;
     }
-    const Pieces<E> row(static_cast<const E*>(k.t.logits) + r * k.t.stride, V);
+    const Pieces<E> row(static_cast<const E*>(k.t.logits) + r * k.t.stride, V, logits_extent<E>(k.t));
     const bool aligned = (reinterpret_cast<uintptr_t>(dx) & 15) == row.lead * sizeof(E);
     auto write = [&](auto whole) {
         constexpr bool FULL = decltype(whole)::value;
@@ -820,19 +847,20 @@ __global__ void __launch_bounds__(LT, 6) dlogits_kernel(const __grid_constant__ 
 #pragma unroll
         for (int j = 0; j < DV; ++j) u[j] = row.template get<FULL>(at0 + j * LT + tid);
         const int id = row_id(k.t, r);
-        const float g = k.g[r / k.rows_per_g] * (k.scale ? *k.scale : 1.f), p = -g * k.stats[2 * r + 1];
+        const float* gr = k.g + r / k.rows_per_g;
+        const float g = (Extent(k.g, (uint64_t)((k.t.rows + k.rows_per_g - 1) / k.rows_per_g) * sizeof(float)).holds(gr) ? *gr : 0.f) * (k.scale ? *k.scale : 1.f), p = -g * k.stats[2 * r + 1];
         const Ref ref(k.stats[2 * r]);
         const int own = (id + row.lead) / N - at0;
         const bool mine = own >= 0 && own < LT * DV && own % LT == tid;
-        const float x_id = mine ? to_f(row.x[row.lead + id]) : 0.f;
+        const float x_id = mine ? row.value(id) : 0.f;
 #pragma unroll
         for (int j = 0; j < DV; ++j) {
             float e[N];
             unpack<E>(u[j], e);
             exp_from<N>(e, ref);
-            write_piece<E, FULL>(row, e, at0 + j * LT + tid, dx, aligned, p);
+            write_piece<E, FULL>(row, e, at0 + j * LT + tid, dx, aligned, p, grads);
         }
-        if (mine) dx[id] = from_f<E>(fmaf(p, exp_from(x_id, ref), g));
+        if (mine && grads.holds(dx + id)) dx[id] = from_f<E>(fmaf(p, exp_from(x_id, ref), g));
     };
     if (aligned && row.all_whole(at0, at0 + LT * DV)) write(std::true_type());
     else write(std::false_type());
@@ -886,7 +914,10 @@ __global__ void __launch_bounds__(JT) preference_join_kernel(const double* logp,
         double side[2];
         for (int w = 0; w < 2; ++w) {
             double s = 0.0;
-            for (int64_t t = threadIdx.x; t < steps; t += JT) s += logp[(i + w * pairs) * steps + t];
+            for (int64_t t = threadIdx.x; t < steps; t += JT) {
+                const double* p = logp + (i + w * pairs) * steps + t;
+                s += Extent(logp, (uint64_t)(2 * pairs * steps) * sizeof(double)).holds(p) ? *p : 0.0;
+            }
             side[w] = block_sum_jt(s, red);
         }
         const double m = (double)beta * ((side[0] - (double)ref[i]) - (side[1] - (double)ref[pairs + i]));

@@ -24,6 +24,23 @@ __device__ __forceinline__ float block_sum_nt(float v, float* red) {
     return t;
 }
 
+// the arrays of a call
+template <class E>
+__device__ __forceinline__ Extent x_extent(const NormArgs& a) { return rows_extent(a.x, a.rows, a.x_stride, a.C, sizeof(E)); }
+template <class E>
+__device__ __forceinline__ Extent dy_extent(const NormArgs& a) { return rows_extent(a.dy, a.rows, a.dy_stride, a.C, sizeof(E)); }
+template <class E>
+__device__ __forceinline__ Extent dense_extent(const NormArgs& a, const void* p) { return rows_extent(p, a.rows, a.C, a.C, sizeof(E)); }
+template <class W>
+__device__ __forceinline__ Extent weight_extent(const NormArgs& a, const void* w) { return Extent(w, (uint64_t)a.C * sizeof(W)); }
+__device__ __forceinline__ Extent stats_extent(const NormArgs& a, const float* p) { return Extent(p, (uint64_t)a.rows * a.groups * sizeof(float)); }
+template <class E>
+__device__ __forceinline__ float get(const E* p, const Extent& in) { return in.holds(p) ? to_f(*p) : 0.f; }
+template <class E>
+__device__ __forceinline__ void put(E* p, E v, const Extent& out) {
+    if (out.holds(p)) *p = v;
+}
+
 template <class E, class W>
 __global__ void __launch_bounds__(NT) norm_fwd_kernel(const __grid_constant__ NormArgs a) {
     __shared__ float red[NT / 32];
@@ -33,21 +50,23 @@ __global__ void __launch_bounds__(NT) norm_fwd_kernel(const __grid_constant__ No
     const int g = (int)(unit - row * a.groups);
     const E* x = static_cast<const E*>(a.x) + row * a.x_stride + g * m;
     const W *w = static_cast<const W*>(a.w), *b = static_cast<const W*>(a.b);
+    const Extent in = x_extent<E>(a);
     float s = 0.f;
-    for (int i = threadIdx.x; i < m; i += NT) s += to_f(x[i]);
+    for (int i = threadIdx.x; i < m; i += NT) s += get(x + i, in);
     const float mean = block_sum_nt(s, red) / (float)m;
     float q = 0.f;
     for (int i = threadIdx.x; i < m; i += NT) {
-        const float d = to_f(x[i]) - mean;
+        const float d = get(x + i, in) - mean;
         q = fmaf(d, d, q);
     }
     const float rstd = 1.f / sqrtf(block_sum_nt(q, red) / (float)m + a.eps);
     E* y = static_cast<E*>(a.y) + row * a.C + g * m;
     for (int i = threadIdx.x; i < m; i += NT)
-        y[i] = from_f<E>(fmaf((to_f(x[i]) - mean) * rstd, w ? to_f(w[g * m + i]) : 1.f, b ? to_f(b[g * m + i]) : 0.f));
+        put(y + i, from_f<E>(fmaf((get(x + i, in) - mean) * rstd, w ? get(w + g * m + i, weight_extent<W>(a, w)) : 1.f, b ? get(b + g * m + i, weight_extent<W>(a, b)) : 0.f)),
+            dense_extent<E>(a, a.y));
     if (a.mean && threadIdx.x == 0) {
-        a.mean[unit] = mean;
-        a.rstd[unit] = rstd;
+        put(a.mean + unit, mean, stats_extent(a, a.mean));
+        put(a.rstd + unit, rstd, stats_extent(a, a.rstd));
     }
     }
 }
@@ -61,19 +80,20 @@ __global__ void __launch_bounds__(NT) norm_dx_kernel(const __grid_constant__ Nor
     const int g = (int)(unit - row * a.groups);
     const E *x = static_cast<const E*>(a.x) + row * a.x_stride + g * m, *dy = static_cast<const E*>(a.dy) + row * a.dy_stride + g * m;
     const W* w = static_cast<const W*>(a.w);
-    const float mean = a.mean[unit], rstd = a.rstd[unit];
+    const Extent in = x_extent<E>(a), up = dy_extent<E>(a), weights = weight_extent<W>(a, a.w);
+    const float mean = get(a.mean + unit, stats_extent(a, a.mean)), rstd = get(a.rstd + unit, stats_extent(a, a.rstd));
     float s = 0.f, q = 0.f;
     for (int i = threadIdx.x; i < m; i += NT) {
-        const float e = to_f(dy[i]) * (w ? to_f(w[g * m + i]) : 1.f);
+        const float e = get(dy + i, up) * (w ? get(w + g * m + i, weights) : 1.f);
         s += e;
-        q = fmaf(e, (to_f(x[i]) - mean) * rstd, q);
+        q = fmaf(e, (get(x + i, in) - mean) * rstd, q);
     }
     s = block_sum_nt(s, red) / (float)m;
     q = block_sum_nt(q, red) / (float)m;
     E* dx = static_cast<E*>(a.dx) + row * a.C + g * m;
     for (int i = threadIdx.x; i < m; i += NT) {
-        const float e = to_f(dy[i]) * (w ? to_f(w[g * m + i]) : 1.f);
-        dx[i] = from_f<E>(rstd * (e - s - (to_f(x[i]) - mean) * rstd * q));
+        const float e = get(dy + i, up) * (w ? get(w + g * m + i, weights) : 1.f);
+        put(dx + i, from_f<E>(rstd * (e - s - (get(x + i, in) - mean) * rstd * q)), dense_extent<E>(a, a.dx));
     }
     }
 }
@@ -86,13 +106,13 @@ __global__ void __launch_bounds__(NT) norm_cols_kernel(const __grid_constant__ N
     if (c >= a.C) return;
     float dw = 0.f, db = 0.f;
     for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const float dy = to_f(static_cast<const E*>(a.dy)[r * a.dy_stride + c]);
+        const float dy = get(static_cast<const E*>(a.dy) + r * a.dy_stride + c, dy_extent<E>(a));
         const int64_t at = r * a.groups + c / m;
         db += dy;
-        dw = fmaf(dy, (to_f(static_cast<const E*>(a.x)[r * a.x_stride + c]) - a.mean[at]) * a.rstd[at], dw);
+        dw = fmaf(dy, (get(static_cast<const E*>(a.x) + r * a.x_stride + c, x_extent<E>(a)) - get(a.mean + at, stats_extent(a, a.mean))) * get(a.rstd + at, stats_extent(a, a.rstd)), dw);
     }
-    a.scratch[((int64_t)blockIdx.y * 2) * a.C + c] = dw;
-    a.scratch[((int64_t)blockIdx.y * 2 + 1) * a.C + c] = db;
+    put(a.scratch + ((int64_t)blockIdx.y * 2) * a.C + c, dw, Extent(a.scratch, a.scratch_bytes));
+    put(a.scratch + ((int64_t)blockIdx.y * 2 + 1) * a.C + c, db, Extent(a.scratch, a.scratch_bytes));
 }
 
 // adds up the blocks' sums: 32 columns per block, 16 threads a column, in one order
@@ -107,8 +127,8 @@ __global__ void __launch_bounds__(FT) norm_finish_kernel(const __grid_constant__
         const float* p = a.scratch + c;
 #pragma unroll 4
         for (int i = g; i < parts; i += FT / 32) {
-            dw += p[(int64_t)i * 2 * a.C];
-            db += p[((int64_t)i * 2 + 1) * a.C];
+            dw += get(p + (int64_t)i * 2 * a.C, Extent(a.scratch, a.scratch_bytes));
+            db += get(p + ((int64_t)i * 2 + 1) * a.C, Extent(a.scratch, a.scratch_bytes));
         }
     }
     red[g][threadIdx.x & 31] = make_float2(dw, db);
@@ -119,8 +139,8 @@ __global__ void __launch_bounds__(FT) norm_finish_kernel(const __grid_constant__
         dw += red[i][threadIdx.x].x;
         db += red[i][threadIdx.x].y;
     }
-    if (a.dw) static_cast<W*>(a.dw)[c] = from_f<W>(dw);
-    if (a.db) static_cast<W*>(a.db)[c] = from_f<W>(db);
+    if (a.dw) put(static_cast<W*>(a.dw) + c, from_f<W>(dw), weight_extent<W>(a, a.dw));
+    if (a.db) put(static_cast<W*>(a.db) + c, from_f<W>(db), weight_extent<W>(a, a.db));
 }
 
 // ---- rows in pieces of 16 bytes ----------------------------------------------------------------------------------------
@@ -130,7 +150,7 @@ template <class E>
 constexpr int per_piece = 16 / sizeof(E);
 
 template <class E, class W>
-__device__ __forceinline__ void load_weights(const W* w, int c, float other, float* f) {   // the weights of a piece's columns
+__device__ __forceinline__ void load_weights(const W* w, int c, float other, float* f, const Extent& weights) {   // the weights of a piece's columns
     constexpr int N = per_piece<E>;
     if (!w) {
 #pragma unroll
@@ -138,15 +158,18 @@ __device__ __forceinline__ void load_weights(const W* w, int c, float other, flo
         return;
     }
 #pragma unroll
-    for (int i = 0; i < N; i += per_piece<W>) unpack<W>(__ldg(reinterpret_cast<const uint4*>(w + c + i)), f + i);
+    for (int i = 0; i < N; i += per_piece<W>) {
+        const uint4* p = reinterpret_cast<const uint4*>(w + c + i);
+        unpack<W>(weights.holds(p) ? __ldg(p) : make_uint4(0, 0, 0, 0), f + i);
+    }
 }
 template <class E, class W>
 struct PieceWeights {   // kept as they are stored
     static constexpr int N = per_piece<E>, U = N / per_piece<W>;
     uint4 u[U];
-    __device__ __forceinline__ void load(const W* w, int c) {
+    __device__ __forceinline__ void load(const W* w, int c, const Extent& weights) {
 #pragma unroll
-        for (int i = 0; i < U; ++i) u[i] = w ? __ldg(reinterpret_cast<const uint4*>(w + c) + i) : ones();
+        for (int i = 0; i < U; ++i) u[i] = w && weights.holds(reinterpret_cast<const uint4*>(w + c) + i) ? __ldg(reinterpret_cast<const uint4*>(w + c) + i) : ones();
     }
     __device__ __forceinline__ void get(float* f) const {
 #pragma unroll
@@ -182,7 +205,7 @@ __global__ void __launch_bounds__(BLOCK ? BT : NT) norm_rows_fwd_kernel(const __
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int p = p0 + j * TPR;
-        unpack<E>(p < pieces ? __ldcs(reinterpret_cast<const uint4*>(x) + p) : make_uint4(0, 0, 0, 0), f[j]);
+        unpack<E>(p < pieces && x_extent<E>(a).holds(reinterpret_cast<const uint4*>(x) + p) ? __ldcs(reinterpret_cast<const uint4*>(x) + p) : make_uint4(0, 0, 0, 0), f[j]);
     }
     auto total = [&](float v, float* r) {     // over the row
         v = warp_sum(v);
@@ -232,15 +255,15 @@ __global__ void __launch_bounds__(BLOCK ? BT : NT) norm_rows_fwd_kernel(const __
         const int p = p0 + j * TPR;
         if (p >= pieces) continue;
         float w[N], b[N];
-        load_weights<E>(static_cast<const W*>(a.w), p * N, 1.f, w);
-        load_weights<E>(static_cast<const W*>(a.b), p * N, 0.f, b);
+        load_weights<E>(static_cast<const W*>(a.w), p * N, 1.f, w, weight_extent<W>(a, a.w));
+        load_weights<E>(static_cast<const W*>(a.b), p * N, 0.f, b, weight_extent<W>(a, a.b));
 #pragma unroll
         for (int c = 0; c < N; ++c) w[c] = fmaf(f[j][c] * rstd[j], w[c], b[c]);
-        if (AB_BC((p + 1) * N <= a.C)) __stcs(reinterpret_cast<uint4*>(y) + p, pack<E>(w));
+        if (dense_extent<E>(a, a.y).holds(reinterpret_cast<uint4*>(y) + p)) __stcs(reinterpret_cast<uint4*>(y) + p, pack<E>(w));
         if (a.mean && (seg ? p % seg == 0 : p == 0)) {
             const int64_t at = row * a.groups + (seg ? p / seg : 0);
-            a.mean[at] = mean[j];
-            a.rstd[at] = rstd[j];
+            put(a.mean + at, mean[j], stats_extent(a, a.mean));
+            put(a.rstd + at, rstd[j], stats_extent(a, a.rstd));
         }
     }
 }
@@ -298,9 +321,15 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
                 if (n >= k.slots && !wait_for(&vacant[slot], phase ^ 1u)) break;
                 const int64_t r = blockIdx.x + (int64_t)n * gridDim.x;
                 unsigned char* to = ring + (size_t)slot * 2 * k.row_bytes;
-                mbar_expect_tx(&full[slot], 2 * k.row_bytes);
-                bulk_g2s(to, static_cast<const E*>(a.x) + r * a.x_stride, k.row_bytes, &full[slot]);
-                bulk_g2s(to + k.row_bytes, static_cast<const E*>(a.dy) + r * a.dy_stride, k.row_bytes, &full[slot]);
+                const E *x = static_cast<const E*>(a.x) + r * a.x_stride, *dy = static_cast<const E*>(a.dy) + r * a.dy_stride;
+                if (x_extent<E>(a).holds(x, k.row_bytes / sizeof(E)) && dy_extent<E>(a).holds(dy, k.row_bytes / sizeof(E)) &&
+                    AB_BC(slot >= 0 && slot < MAX_SLOTS && (slot + 1) * 2 * k.row_bytes <= BWD_RING)) {
+                    mbar_expect_tx(&full[slot], 2 * k.row_bytes);
+                    bulk_g2s(to, x, k.row_bytes, &full[slot]);
+                    bulk_g2s(to + k.row_bytes, dy, k.row_bytes, &full[slot]);
+                } else {
+                    mbar_arrive(&full[slot]);
+                }
             }
             // whatever became of the waits, all that was asked for lands before the ring is used otherwise, or the block ends
             for (int c = max(0, n - k.slots); c < n; ++c) mbar_wait_bounded(&full[c % k.slots], (uint32_t)(c / k.slots) & 1u, 1u << 18);
@@ -311,7 +340,7 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
         PieceWeights<E, W> w[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            if (t + j * tpr < pieces) w[j].load(static_cast<const W*>(a.w), (t + j * tpr) * N);
+            if (t + j * tpr < pieces) w[j].load(static_cast<const W*>(a.w), (t + j * tpr) * N, weight_extent<W>(a, a.w));
         constexpr int NS = SEG ? NV : 1;                  // groups that a thread's pieces belong to
         int group[NS];
         float mean[NS], rstd[NS], mean1[NS], rstd1[NS];   // of a row, and of the team's next one
@@ -321,7 +350,8 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
             if (n >= mine) return;
             const int64_t at = (blockIdx.x + (int64_t)n * gridDim.x) * a.groups;
 #pragma unroll
-            for (int j = 0; j < NS; ++j) mean1[j] = __ldg(a.mean + at + group[j]), rstd1[j] = __ldg(a.rstd + at + group[j]);
+            for (int j = 0; j < NS; ++j)
+                if (stats_extent(a, a.mean).holds(a.mean + at + group[j])) mean1[j] = __ldg(a.mean + at + group[j]), rstd1[j] = __ldg(a.rstd + at + group[j]);
         };
         stats(team);
         int slot = team, turn = 0;
@@ -413,7 +443,7 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
                     }
 #pragma unroll
                     for (int c = 0; c < N; ++c) fx[c] = rstd[g] * fmaf(-xh[g][c], qj[g], e[g][c] - sj[g]);
-                    if (AB_BC((p + 1) * N <= a.C)) __stcs(dx + p, pack<E>(fx));
+                    if (dense_extent<E>(a, a.dx).holds(dx + p)) __stcs(dx + p, pack<E>(fx));
                 }
             }
         }
@@ -429,13 +459,14 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
             for (int j = 0; j < NV; ++j)
                 if (t + j * tpr < pieces)
 #pragma unroll
-                    for (int c = 0; c < N; ++c) sums[team * a.C + (t + j * tpr) * N + c] = which ? db[j][c] : dw[j][c];
+                    for (int c = 0; c < N; ++c)
+                        if (Extent(ring, BWD_RING).holds(sums + team * a.C + (t + j * tpr) * N + c)) sums[team * a.C + (t + j * tpr) * N + c] = which ? db[j][c] : dw[j][c];
         }
         __syncthreads();
         for (int c = tid; c < a.C; c += BWD_THREADS + 32) {
             float s = 0.f;
             for (int i = 0; i < teams; ++i) s += sums[i * a.C + c];
-            a.scratch[((int64_t)blockIdx.x * 2 + which) * a.C + c] = s;
+            put(a.scratch + ((int64_t)blockIdx.x * 2 + which) * a.C + c, s, Extent(a.scratch, a.scratch_bytes));
         }
     }
 }

@@ -7,6 +7,29 @@
 
 namespace ab {
 
+// An array as the caller gave it. In the range-checking build an access's final address is held against it, whatever led to that address (loop bounds, strides, a ring's slots); what is
+// outside is recorded and not made. Nothing at all in the normal build.
+struct Extent {
+#ifdef AB_BOUNDS_CHECK
+    const char* base;
+    uint64_t bytes;
+    __device__ __forceinline__ Extent(const void* b, uint64_t n) : base(static_cast<const char*>(b)), bytes(b ? n : 0) {}
+    template <class T>
+    __device__ __forceinline__ bool holds(const T* p, uint64_t n = 1) const {   // n values from p on
+        const int64_t at = reinterpret_cast<const char*>(p) - base;
+        return AB_BC(at >= 0 && (uint64_t)at + n * sizeof(T) <= bytes);
+    }
+#else
+    __device__ __forceinline__ Extent(const void*, uint64_t) {}
+    template <class T>
+    __device__ __forceinline__ bool holds(const T*, uint64_t = 1) const { return true; }
+#endif
+};
+// rows of n values of `size` bytes, `stride` values apart
+__device__ __forceinline__ Extent rows_extent(const void* p, int64_t rows, int64_t stride, int64_t n, int size) {
+    return Extent(p, rows > 0 ? (uint64_t)((rows - 1) * stride + n) * size : 0);
+}
+
 // values of the three element types as 32-bit floats, and back with one rounding
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
@@ -72,6 +95,7 @@ struct NormArgs {
     const void *x, *w, *b, *dy;
     void *y, *dx, *dw, *db;
     float *mean, *rstd, *scratch;
+    int64_t scratch_bytes;                 // what the caller was told to bring
 };
 size_t layer_norm_scratch_bytes(int64_t rows, int C);   // on the current device
 int layer_norm_fwd(const NormArgs& a, cudaStream_t st);

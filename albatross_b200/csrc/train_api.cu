@@ -125,6 +125,7 @@ int ab_layer_norm_bwd(int dtype, int wtype, int64_t rows, int C, int groups, con
     a.dtype = dtype; a.wtype = wtype; a.C = C; a.groups = groups; a.rows = rows; a.x_stride = x_stride; a.dy_stride = dy_stride;
     a.x = x; a.w = w; a.dy = dy; a.dx = dx; a.dw = dw; a.db = db;
     a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd); a.scratch = static_cast<float*>(scratch);
+    a.scratch_bytes = (int64_t)layer_norm_scratch_bytes(rows, C);
     return layer_norm_bwd(a, (cudaStream_t)stream);
 }
 

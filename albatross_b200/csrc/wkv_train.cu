@@ -35,6 +35,16 @@ __device__ __forceinline__ int seq_length(const WkvSeq& s, int b) {
     return s.lengths ? min(max(s.lengths[b], 0), s.T) : s.T;
 }
 
+// A head's steps 0 .. n - 1 of an array, 64 values each, `step` values apart from the first one at `p` on; all heads' states, `each` of them per head.
+__device__ __forceinline__ Extent steps_extent(const void* p, int64_t n, int64_t step) {
+    const int64_t last = n > 0 ? (n - 1) * step : 0, low = last < 0 ? last : 0;
+    return Extent(p ? static_cast<const char*>(p) + 2 * low : nullptr, n > 0 ? (uint64_t)((last < 0 ? -last : last) + 64) * 2 : 0);
+}
+__device__ __forceinline__ Extent input_extent(const WkvSeq& s, int which, int64_t b, int h, int64_t n) {   // of a sequence of n steps
+    return steps_extent(static_cast<const char*>(s.x[which]) + 2 * (b * s.bs[which] + h * 64), n, s.ss[which]);
+}
+__device__ __forceinline__ Extent states_extent(const float* p, int64_t each) { return Extent(p, (uint64_t)gridDim.x * each * 4096 * sizeof(float)); }
+
 // ---- the forward pass ----------------------------------------------------------------------------------------------------
 // A block per head: four warps carry 16 rows of the state each in registers (rows do not meet: the accumulators of one product are the operand of the next
 // without leaving the warp), others prepare chunks ahead, each a whole one by itself, in a ring of buffers.
@@ -45,16 +55,17 @@ constexpr int FWD_V = FWD_TILES * 2 * TILE, FWD_FE = FWD_V + TILE, FWD_HEAD = FW
 static_assert(8 * FWD_BUF <= 227 * 1024, "shared memory of a block");
 
 // Asks for the rows of a later chunk, 32 bytes a lane. (One bulk request per row takes the warp some 50 cycles each.)
-__device__ __forceinline__ void prefetch_steps(const void* x, int64_t at, int64_t step, int n_on, int lane) {
+__device__ __forceinline__ void prefetch_steps(const void* x, int64_t at, int64_t step, int n_on, int lane, const Extent& in) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int t = (lane >> 2) + 8 * i;
-        if (t < n_on) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(x) + 2 * (at + t * step) + (lane & 3) * 32));
+        const char* p = static_cast<const char*>(x) + 2 * (at + t * step) + (lane & 3) * 32;
+        if (t < n_on && in.holds(p, 32)) asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
     }
 }
-__device__ __forceinline__ void prefetch_chunk(const WkvSeq& s, int64_t b, int h, int t0, int n_on, int lane) {
+__device__ __forceinline__ void prefetch_chunk(const WkvSeq& s, int64_t b, int h, int t0, int n_on, int lane, int n_steps) {
 #pragma unroll 1
-    for (int i = 0; i < 6; ++i) prefetch_steps(s.x[i], b * s.bs[i] + (int64_t)t0 * s.ss[i] + h * N, s.ss[i], n_on, lane);
+    for (int i = 0; i < 6; ++i) prefetch_steps(s.x[i], b * s.bs[i] + (int64_t)t0 * s.ss[i] + h * N, s.ss[i], n_on, lane, input_extent(s, i, b, h, n_steps));
 }
 
 __device__ __forceinline__ float log2_decay(float w) {   // of exp(-exp(w)); finite (2^-2000 is 0 all the same), but for NaN
@@ -63,13 +74,14 @@ __device__ __forceinline__ float log2_decay(float w) {   // of exp(-exp(w)); fin
 }
 // Asks for one vector of a chunk's steps lo .. hi - 1 (zeros at the others) in a tile's place: a lane has eight columns (c8 = lane & 7) of steps lane >> 3, + 4, + 8,
 // + 12, here and when it takes them up again. All vectors of a chunk are on their way at once: one after the other they cost a warp 2000 cycles each.
-__device__ __forceinline__ void stage_steps(uint32_t tile, const char* p, int64_t step, int lo, int hi, bool there, int lane) {
+__device__ __forceinline__ void stage_steps(uint32_t tile, const char* p, int64_t step, int lo, int hi, bool there, int lane, const Extent& in) {
     if (!AB_BC(lo >= 0 && lo < hi && hi <= L)) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int t = (lane >> 3) + 4 * i;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + t * 128 + (((lane & 7) ^ (t & 7)) << 4)), "l"(p + (there ? min(max(t, lo), hi - 1) * step : 0)),
-                     "r"(there && t >= lo && t < hi ? 16 : 0) : "memory");
+        const char* from = p + (there ? min(max(t, lo), hi - 1) * step : 0);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + t * 128 + (((lane & 7) ^ (t & 7)) << 4)), "l"(from),
+                     "r"(there && t >= lo && t < hi && in.holds(from, 16) ? 16 : 0) : "memory");
     }
 }
 __device__ __forceinline__ void staged(uint4* u, uint32_t tile, int lane) {
@@ -220,22 +232,27 @@ __device__ __forceinline__ float invert(float* work, Frag& f, float (*v)[4], int
     return sc.down;
 }
 
+__device__ __forceinline__ Extent upstream_extent(const WkvBackward* g, int64_t b, int h, int64_t n) {
+    return g && g->dy ? steps_extent(static_cast<const char*>(g->dy) + 2 * (b * g->dy_batch_stride + h * N), n, g->dy_step_stride) : Extent(nullptr, 0);
+}
 // Asks for a chunk's vectors: w (in fb's place) ahead of the others, b, k, a and r in the low halves of their tiles, v and dy where one of their forms is themselves.
 template <class E, bool BWD>
 __device__ __forceinline__ void stage_chunk(const WkvSeq& s, const WkvBackward* bwd, int64_t b, int h, int t0, int lo, int hi, bool with_w, uint32_t at, uint32_t v, uint32_t v16, uint32_t fb,
-                                            int lane) {
-    if (with_w) stage_steps(fb, steps_of(s, 1, b, h, t0, lane), 2 * s.ss[1], lo, hi, true, lane);
+                                            int lane, int n_steps) {
+    if (with_w) stage_steps(fb, steps_of(s, 1, b, h, t0, lane), 2 * s.ss[1], lo, hi, true, lane, input_extent(s, 1, b, h, n_steps));
     stage_commit();
 #pragma unroll 1
     for (int vec = 0; vec < 4; ++vec) {
         const int which = vec == 0 ? 5 : vec == 1 ? 2 : vec == 2 ? 4 : 0, to = vec == 0 ? T_B : vec == 1 ? T_K : vec == 2 ? T_A : T_R;
-        stage_steps(at + to * 2 * TILE + TILE, steps_of(s, which, b, h, t0, lane), 2 * s.ss[which], lo, hi, true, lane);
+        stage_steps(at + to * 2 * TILE + TILE, steps_of(s, which, b, h, t0, lane), 2 * s.ss[which], lo, hi, true, lane, input_extent(s, which, b, h, n_steps));
     }
     constexpr bool OWN = std::is_same<E, __half>::value || !BWD;   // fp16 as it is; bf16 as it is for the sums over rows, else to be converted in place
-    stage_steps(OWN ? v : v16, steps_of(s, 3, b, h, t0, lane), 2 * s.ss[3], lo, hi, true, lane);
-    if (BWD)
-        stage_steps(OWN ? v + TILE : v16 + 2 * TILE, bwd->dy ? static_cast<const char*>(bwd->dy) + 2 * (b * bwd->dy_batch_stride + (int64_t)t0 * bwd->dy_step_stride + h * N + 8 * (lane & 7))
-                                                             : static_cast<const char*>(s.x[3]), bwd->dy ? 2 * bwd->dy_step_stride : 0, lo, hi, bwd->dy != nullptr, lane);
+    stage_steps(OWN ? v : v16, steps_of(s, 3, b, h, t0, lane), 2 * s.ss[3], lo, hi, true, lane, input_extent(s, 3, b, h, n_steps));
+    if (BWD) {
+        const bool there = bwd->dy != nullptr;
+        const char* dy = static_cast<const char*>(there ? bwd->dy : s.x[3]) + (there ? 2 * (b * bwd->dy_batch_stride + (int64_t)t0 * bwd->dy_step_stride + h * N + 8 * (lane & 7)) : 0);
+        stage_steps(OWN ? v + TILE : v16 + 2 * TILE, dy, there ? 2 * bwd->dy_step_stride : 0, lo, hi, there, lane, upstream_extent(bwd, b, h, n_steps));
+    }
     stage_commit();
 }
 
@@ -517,7 +534,7 @@ template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float x
 // Accumulators (rows i0 .. as m, steps as n) to out[step][row], 64 channels per step and `stride` values between steps, steps lo .. hi - 1 of the chunk; zeros
 // from step n_on on.
 template <class E>
-__device__ __forceinline__ void store_steps(const float (*y)[4], E* out, int64_t stride, int i0, int lo, int hi, int n_on, int lane) {
+__device__ __forceinline__ void store_steps(const float (*y)[4], E* out, int64_t stride, int i0, int lo, int hi, int n_on, int lane, const Extent& all) {
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -525,25 +542,29 @@ __device__ __forceinline__ void store_steps(const float (*y)[4], E* out, int64_t
             uint32_t p = pack_pair<E>(y[n][2 * half], y[n][2 * half + 1]);
             asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(p));
             const int t = 8 * n + (lane >> 2);
-            if (t >= lo && t < hi && AB_BC(t < L && i0 + 8 * half + 2 * (lane & 3) + 2 <= N)) *reinterpret_cast<uint32_t*>(out + t * stride + i0 + 8 * half + 2 * (lane & 3)) = t < n_on ? p : 0u;
+            uint32_t* to = reinterpret_cast<uint32_t*>(out + t * stride + i0 + 8 * half + 2 * (lane & 3));
+            if (t >= lo && t < hi && all.holds(to)) *to = t < n_on ? p : 0u;
         }
 }
 // a state's rows i0 .. i0 + 15 between accumulators and memory
-__device__ __forceinline__ void load_rows(float (*S)[4], const float* from, int i0, int lane) {
+__device__ __forceinline__ void load_rows(float (*S)[4], const float* from, int i0, int lane, const Extent& states) {
 #pragma unroll
     for (int n = 0; n < 8; ++n)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const float2 u = from ? *reinterpret_cast<const float2*>(from + (i0 + (lane >> 2) + 8 * half) * N + 8 * n + 2 * (lane & 3)) : make_float2(0.f, 0.f);
+            const float2* p = reinterpret_cast<const float2*>(from + (i0 + (lane >> 2) + 8 * half) * N + 8 * n + 2 * (lane & 3));
+            const float2 u = from && states.holds(p) ? *p : make_float2(0.f, 0.f);
             S[n][2 * half] = u.x, S[n][2 * half + 1] = u.y;
         }
 }
-__device__ __forceinline__ void store_rows(const float (*S)[4], float* to, int i0, int lane) {
+__device__ __forceinline__ void store_rows(const float (*S)[4], float* to, int i0, int lane, const Extent& states) {
 #pragma unroll
     for (int n = 0; n < 8; ++n)
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-            *reinterpret_cast<float2*>(to + (i0 + (lane >> 2) + 8 * half) * N + 8 * n + 2 * (lane & 3)) = make_float2(S[n][2 * half], S[n][2 * half + 1]);
+        for (int half = 0; half < 2; ++half) {
+            float2* p = reinterpret_cast<float2*>(to + (i0 + (lane >> 2) + 8 * half) * N + 8 * n + 2 * (lane & 3));
+            if (states.holds(p)) *p = make_float2(S[n][2 * half], S[n][2 * half + 1]);
+        }
 }
 
 // BUFS chunks under way. Four (two blocks per SM) where there are more heads than SMs; eight, which take an SM's shared memory, where there are not: a preparing warp takes
@@ -583,14 +604,14 @@ __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1
     if (warp < 4) {
         const int i0 = warp * 16;
         float S[8][4];
-        load_rows(S, s.state ? s.state + (size_t)bh * 4096 : nullptr, i0, lane);
+        load_rows(S, s.state ? s.state + (size_t)bh * 4096 : nullptr, i0, lane, states_extent(s.state, 1));
         uint32_t phases = 0;
         bool ok = true;
         for (int n = 0; n < chunks && ok; ++n) {
             const int buf = n % CHUNK_BUFS;
             const uint32_t at = smem_u32(smem) + buf * FWD_BUF;
             const ChunkHead* head = reinterpret_cast<const ChunkHead*>(smem + buf * FWD_BUF + FWD_HEAD);
-            if (s.ckpt && AB_BC(n < s.n_chunks)) store_rows(S, s.ckpt + ((size_t)bh * s.n_chunks + n) * 4096, i0, lane);
+            if (s.ckpt) store_rows(S, s.ckpt + ((size_t)bh * s.n_chunks + n) * 4096, i0, lane, states_extent(s.ckpt, s.n_chunks));
             for (int more = 1; more && ok;) {
                 ok = wait_for(&full[buf], phases >> buf & 1u);
                 if (!ok) break;
@@ -599,12 +620,12 @@ __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1
                 chunk_rows(S, o, at, at + FWD_V, T_A, head, i0, lane);
                 const int lo = head->lo, t0 = head->t0;
                 more = head->more;
-                store_steps<E>(o, y + t0 * stride, stride, i0, lo, min(head->hi, s.T - t0), n_steps - t0, lane);
+                store_steps<E>(o, y + t0 * stride, stride, i0, lo, min(head->hi, s.T - t0), n_steps - t0, lane, steps_extent(y, s.T, stride));
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&vacant[buf]);
             }
         }
-        store_rows(S, p.state_out + (size_t)bh * 4096, i0, lane);
+        store_rows(S, p.state_out + (size_t)bh * 4096, i0, lane, states_extent(p.state_out, 1));
     } else {
         const int buf = warp - 4;
         const uint32_t at = smem_u32(smem) + buf * FWD_BUF;
@@ -614,13 +635,13 @@ __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1
         bool ok = true;
         for (int n = buf; n < chunks && ok; n += CHUNK_BUFS) {
             const int t0 = n * L, n_on = min(L, n_steps - t0);
-            if (n + CHUNK_BUFS < chunks) prefetch_chunk(s, b, h, t0 + CHUNK_BUFS * L, min(L, n_steps - t0 - CHUNK_BUFS * L), lane);
+            if (n + CHUNK_BUFS < chunks) prefetch_chunk(s, b, h, t0 + CHUNK_BUFS * L, min(L, n_steps - t0 - CHUNK_BUFS * L), lane, n_steps);
             for (int i = 0, pieces = 1; i < pieces; ++i) {
                 if (uses > 0) ok = wait_for(&vacant[buf], (uint32_t)(uses - 1) & 1u);
                 if (!ok) break;
                 ++uses;
                 const uint32_t fbs = at + T_M * 2 * TILE;
-                stage_chunk<E, false>(s, nullptr, b, h, t0, 0, n_on, true, at, at + FWD_V, 0u, fbs, lane);
+                stage_chunk<E, false>(s, nullptr, b, h, t0, 0, n_on, true, at, at + FWD_V, 0u, fbs, lane, n_steps);
                 uint4 w[4];
                 stage_wait<1>();
                 staged(w, fbs, lane);
@@ -629,7 +650,7 @@ __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1
                     const int size = steep_steps(fe, lane);
                     pieces = (n_on + size - 1) / size, lo = i * size, hi = min(lo + size, n_on), single = size == 1;
                     stage_wait<0>();
-                    stage_chunk<E, false>(s, nullptr, b, h, t0, lo, hi, false, at, at + FWD_V, 0u, fbs, lane);
+                    stage_chunk<E, false>(s, nullptr, b, h, t0, lo, hi, false, at, at + FWD_V, 0u, fbs, lane, n_steps);
                     put_piece(lo, hi, single, fe, fb, head->decay, lane);
                 }
                 if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = i + 1 < pieces ? hi : L, head->more = i + 1 < pieces, head->piece = single;
@@ -641,7 +662,7 @@ __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1
     }
     // steps behind the last chunk
     for (int64_t i = (int64_t)chunks * L * 32 + threadIdx.x; i < (int64_t)s.T * 32; i += (CHUNK_BUFS + 4) * 32)
-        *reinterpret_cast<uint32_t*>(y + (i >> 5) * stride + (i & 31) * 2) = 0u;
+        if (uint32_t* to = reinterpret_cast<uint32_t*>(y + (i >> 5) * stride + (i & 31) * 2); steps_extent(y, s.T, stride).holds(to)) *to = 0u;
 }
 
 // ---- the backward pass -----------------------------------------------------------------------------------------------------
@@ -750,11 +771,16 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
         }
         return __all_sync(0xffffffffu, ok) != 0;
     };
+    auto put_grads = [&](int which, int64_t at, uint32_t two) {   // two values of a gradient
+        if (!p.g.dx[which]) return;
+        uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[which]) + at);
+        if (steps_extent(static_cast<E*>(p.g.dx[which]) + base, s.T, stride).holds(to)) *to = two;
+    };
     bool ok = true;
     if (warp < 4) {
         const int i0 = warp * 16;
         float G[8][4], S[8][4];
-        load_rows(G, p.g.dstate_out ? p.g.dstate_out + (size_t)bh * 4096 : nullptr, i0, lane);
+        load_rows(G, p.g.dstate_out ? p.g.dstate_out + (size_t)bh * 4096 : nullptr, i0, lane, states_extent(p.g.dstate_out, 1));
         E* dv_out = p.g.dx[3] ? static_cast<E*>(p.g.dx[3]) + base : nullptr;
         uint32_t phases = 0;
         int items = 0;
@@ -762,7 +788,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
             const uint32_t at = smem_u32(smem) + buf * BWD_BUF;
             const ChunkHead* head = reinterpret_cast<const ChunkHead*>(smem + buf * BWD_BUF + BWD_HEAD);
             const float* before = s.ckpt + ((size_t)bh * s.n_chunks + n) * 4096;
-            load_rows(S, before, i0, lane);
+            load_rows(S, before, i0, lane, states_extent(s.ckpt, s.n_chunks));
             for (int more = 1; more && ok;) {
                 ok = wait_for(&full[buf], phases >> buf & 1u);
                 if (!ok) break;
@@ -823,7 +849,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 load_frag(w, tM, M_X * L, lane, load_bt);
                 mma3(z, fh, w);
                 add_acc(xk, z, h0, h1, head->down_m[M_X]);
-                if (dv_out) store_steps<E>(xk, dv_out + head->t0 * stride, stride, i0, head->lo, min(head->hi, s.T - head->t0), n_steps - head->t0, lane);
+                if (dv_out) store_steps<E>(xk, dv_out + head->t0 * stride, stride, i0, head->lo, min(head->hi, s.T - head->t0), n_steps - head->t0, lane, steps_extent(dv_out, s.T, stride));
                 // u
                 if (!piece) decay_rows(S, head, lane);
                 row_scales(S, s0, s1);
@@ -892,10 +918,10 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&vacant[buf]);
-                if (more) load_rows(S, before, i0, lane);
+                if (more) load_rows(S, before, i0, lane, states_extent(s.ckpt, s.n_chunks));
             }
         }
-        if (p.g.dstate) store_rows(G, p.g.dstate + (size_t)bh * 4096, i0, lane);
+        if (p.g.dstate) store_rows(G, p.g.dstate + (size_t)bh * 4096, i0, lane, states_extent(p.g.dstate, 1));
     } else if (warp < 8) {
         const int cw = warp - 4, c0 = cw * 16;
         uint32_t phases = 0;
@@ -928,7 +954,8 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             const int t = g + 8 * half;
-                            raw[v][i][half] = t >= lo && t < min(hi, n_on) ? __ldg(reinterpret_cast<const uint32_t*>(from + t * s.ss[which] + 8 * i)) : 0u;
+                            const uint32_t* p = reinterpret_cast<const uint32_t*>(from + t * s.ss[which] + 8 * i);
+                            raw[v][i][half] = t >= lo && t < min(hi, n_on) && input_extent(s, which, b, h, n_steps).holds(p) ? __ldg(p) : 0u;
                         }
                 }
                 ok = wait_for(&x_full, (uint32_t)items & 1u);
@@ -1049,12 +1076,12 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                             flow[cc][half] = fmaf(bv, gbs, kv * gks);
                             lw[cc][half] = on ? log2_decay(cc ? wv.y : wv.x) * 0.6931471805599453f : 0.f;
                         }
-                        if (t >= lo && t < hi && AB_BC(t0 + t < s.T && j + 2 <= N)) {
+                        if (t >= lo && t < hi) {
                             const int64_t to = base + (t0 + t) * stride + j;
-                            if (p.g.dx[0]) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[0]) + to) = on ? pack_pair<E>(out[0][0], out[0][1]) : 0u;
-                            if (p.g.dx[2]) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[2]) + to) = on ? pack_pair<E>(out[2][0], out[2][1]) : 0u;
-                            if (p.g.dx[4]) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[4]) + to) = on ? pack_pair<E>(out[3][0], out[3][1]) : 0u;
-                            if (p.g.dx[5]) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[5]) + to) = on ? pack_pair<E>(out[4][0], out[4][1]) : 0u;
+                            put_grads(0, to, on ? pack_pair<E>(out[0][0], out[0][1]) : 0u);
+                            put_grads(2, to, on ? pack_pair<E>(out[2][0], out[2][1]) : 0u);
+                            put_grads(4, to, on ? pack_pair<E>(out[3][0], out[3][1]) : 0u);
+                            put_grads(5, to, on ? pack_pair<E>(out[4][0], out[4][1]) : 0u);
                         }
                     }
                     if (p.g.dx[1]) {
@@ -1069,7 +1096,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                         for (int half = 0; half < 2; ++half) {
                             const int t = g + 8 * half;
                             const float x0 = (gs[i].x + flow[0][half] + pos[0][half]) * lw[0][half], x1 = (gs[i].y + flow[1][half] + pos[1][half]) * lw[1][half];
-                            if (t >= lo && t < hi) *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[1]) + base + (t0 + t) * stride + j) = t < n_on ? pack_pair<E>(x0, x1) : 0u;
+                            if (t >= lo && t < hi) put_grads(1, base + (t0 + t) * stride + j, t < n_on ? pack_pair<E>(x0, x1) : 0u);
                         }
                     }
                 }
@@ -1083,13 +1110,15 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
         ChunkHead* head = reinterpret_cast<ChunkHead*>(smem + buf * BWD_BUF + BWD_HEAD);
         float *fe = reinterpret_cast<float*>(smem + buf * BWD_BUF + BWD_FE), *fb = reinterpret_cast<float*>(smem + buf * BWD_BUF + BWD_FB);
         int uses = 0;
+        const Extent upstream = upstream_extent(&p.g, b, h, n_steps);
         for (int n = chunks - 1 - buf; n >= 0 && ok; n -= BWD_BUFS) {
             const int t0 = n * L, n_on = min(L, n_steps - t0);
             if (n >= BWD_BUFS) {
                 const int t1 = t0 - BWD_BUFS * L;
-                prefetch_chunk(s, b, h, t1, L, lane);
-                if (p.g.dy) prefetch_steps(p.g.dy, b * p.g.dy_batch_stride + (int64_t)t1 * p.g.dy_step_stride + h * N, p.g.dy_step_stride, L, lane);
-                if (lane == 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], 16384;" ::"l"(s.ckpt + ((size_t)bh * s.n_chunks + n - BWD_BUFS) * 4096) : "memory");
+                prefetch_chunk(s, b, h, t1, L, lane, n_steps);
+                if (p.g.dy) prefetch_steps(p.g.dy, b * p.g.dy_batch_stride + (int64_t)t1 * p.g.dy_step_stride + h * N, p.g.dy_step_stride, L, lane, upstream);
+                const float* kept = s.ckpt + ((size_t)bh * s.n_chunks + n - BWD_BUFS) * 4096;
+                if (lane == 0 && states_extent(s.ckpt, s.n_chunks).holds(kept, 4096)) asm volatile("cp.async.bulk.prefetch.L2.global [%0], 16384;" ::"l"(kept) : "memory");
             }
             // a steep chunk: for each piece from the last one, the pieces before it for the state's sake, and then the piece itself
             for (int i = -1, j = 0, last = 0; !last && ok;) {
@@ -1097,7 +1126,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                 if (!ok) break;
                 ++uses;
                 const uint32_t fbs = at + BWD_FB;
-                stage_chunk<E, true>(s, &p.g, b, h, t0, 0, n_on, true, at, at + BWD_V, at + BWD_V16, fbs, lane);
+                stage_chunk<E, true>(s, &p.g, b, h, t0, 0, n_on, true, at, at + BWD_V, at + BWD_V16, fbs, lane, n_steps);
                 uint4 w[4];
                 stage_wait<1>();
                 staged(w, fbs, lane);
@@ -1111,7 +1140,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                     if (advance) ++j;
                     else --i, j = 0;
                     stage_wait<0>();
-                    stage_chunk<E, true>(s, &p.g, b, h, t0, lo, hi, false, at, at + BWD_V, at + BWD_V16, fbs, lane);
+                    stage_chunk<E, true>(s, &p.g, b, h, t0, lo, hi, false, at, at + BWD_V, at + BWD_V16, fbs, lane, n_steps);
                     put_piece(lo, hi, single, fe, fb, head->decay, lane);
                 }
                 if (lane == 0) head->t0 = t0, head->lo = lo, head->hi = hi == n_on ? L : hi, head->more = !last, head->piece = single, head->advance = advance;
@@ -1125,7 +1154,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
     for (int w = 0; w < 6; ++w)
         if (p.g.dx[w])
             for (int64_t i = (int64_t)chunks * L * 32 + threadIdx.x; i < (int64_t)s.T * 32; i += BWD_WARPS * 32)
-                *reinterpret_cast<uint32_t*>(static_cast<E*>(p.g.dx[w]) + base + (i >> 5) * stride + (i & 31) * 2) = 0u;
+                put_grads(w, base + (i >> 5) * stride + (i & 31) * 2, 0u);
 }
 
 WkvSeq seq_of(const ab_wkv7_seq& s) {

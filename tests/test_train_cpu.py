@@ -156,3 +156,17 @@ def test_python_entries_refuse_to_be_traced():
 
 def test_struct_layouts_match_the_header():
     assert C.sizeof(_lib.Wkv7Seq) == 16 + 48 + 96 + 24 and C.sizeof(_lib.LogitRows) == 48 and C.sizeof(_lib.Policy) == 40
+
+
+def test_the_range_checking_build_holds_asynchronous_copies_against_their_arrays():
+    """What no loop bound stands next to: bulk copies, staged vectors and prefetches ask the extent of the caller's array for their final address."""
+    import os
+    from albatross_b200 import build
+    seen = 0
+    for name in ("loss.cu", "norm.cu", "wkv_train.cu"):
+        lines = open(os.path.join(build.CSRC, name)).read().split("\n")
+        for i, line in enumerate(lines):
+            if any(op in line for op in ("bulk_g2s(", "prefetch.global", "bulk.prefetch", "cp.async.cg")):
+                assert ".holds(" in " ".join(lines[max(0, i - 5):i + 2]), (name, i + 1)
+                seen += 1
+    assert seen >= 6

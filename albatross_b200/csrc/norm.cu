@@ -185,6 +185,13 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {   // over align
     return v;
 }
 
+// s / m from 1 / m rounded, by one step on the remainder (which is exact): exact where the quotient is, so that rows of one value have no deviation. (The product alone is off by up to 1.5
+// units, which rows of 1000 whose length is not a power of two showed as 0.019, times 1 / sqrt(eps).)
+__device__ __forceinline__ float quotient(float s, float m, float inv_m) {
+    const float q = s * inv_m;
+    return fmaf(fmaf(-q, m, s), inv_m, q);
+}
+
 // One pass over x: a thread keeps NV pieces of its row in registers between the statistics and the output.
 // BLOCK: a block per row, else a warp per row; SEG (of a warp's lanes per group): a warp per NV * 32 pieces of a row.
 constexpr int BT = 128;   // threads of a row that has a block to itself: a thread's fixed work (addresses, reductions) is shared by 32 or 64 values
@@ -223,11 +230,11 @@ __global__ void __launch_bounds__(BLOCK ? BT : NT) norm_rows_fwd_kernel(const __
         float t = 0.f;
 #pragma unroll
         for (int c = 0; c < N; ++c) t += f[j][c];
-        if (seg) mean[j] = lanes_sum(t, seg) * inv_m;
+        if (seg) mean[j] = quotient(lanes_sum(t, seg), (float)m, inv_m);
         else s += t;
     }
     if (!seg) {
-        s = total(s, red[0]) * inv_m;
+        s = quotient(total(s, red[0]), (float)m, inv_m);
 #pragma unroll
         for (int j = 0; j < NV; ++j) mean[j] = s;
     }

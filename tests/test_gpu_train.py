@@ -417,6 +417,19 @@ def test_layer_norm_of_nothing_and_of_constants():
     assert bool(torch.isnan(y[1]).all()) and float(y[0].abs().max()) == 0 and float(y[2].abs().max()) == 0
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("Cn,groups", [(768, 1), (1000, 1), (2560, 1), (33, 1), (5000, 1), (12288, 1), (2560, 40), (96, 12), (96, 1), (4104, 1)])
+def test_layer_norm_of_rows_of_one_value_is_the_bias(Cn, groups, dtype):
+    """The sum of Cn equal values of few bits is exact, and so has their mean to be, whether or not 1 / Cn is: with rstd = 316 (eps 1e-5, no variance) a mean of
+    1000 that is off by half a step, 3e-5, would come out as 0.01."""
+    x = torch.tensor([7.0, 1000.0, -1000.0, 96.0], device="cuda").to(DT[dtype])[:, None].expand(4, Cn).contiguous()
+    b = torch.randn(Cn, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(DT[dtype])
+    assert float(ab.layer_norm(x, groups=groups).abs().max()) == 0
+    leaf = x.clone().requires_grad_()
+    y = ab.layer_norm(leaf, torch.ones_like(b).requires_grad_(), b, groups=groups)
+    assert torch.equal(y, b.expand(4, Cn))
+
+
 @pytest.mark.parametrize("n,Cn,groups,dtype", [(70001, 33, 1, "bf16"), (30000, 64, 1, "fp16"), (20000, 128, 2, "bf16"), (5000, 1024, 16, "fp32")])
 def test_layer_norm_of_many_short_rows(n, Cn, groups, dtype):
     norm_check(*norm_inputs(n, Cn, dtype), groups=groups)

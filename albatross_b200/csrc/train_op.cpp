@@ -353,7 +353,7 @@ PolicyArgs policy_args(const Tensor& logits, const Tensor& ids, const OptTensor&
 std::pair<Tensor, Tensor> policy_forward(const Tensor& logits, const Tensor& ids, const Tensor& mask, const PolicyArgs& a, Tensor* stats, Tensor* g) {
     const c10::cuda::CUDAGuard guard(logits.device());
     const Rows r(logits, ids, mask);
-    Tensor loss = like({}, logits, at::kFloat), logp = like(ids.sizes(), logits, at::kFloat), scratch = like({2 * r.t.rows + 2}, logits, at::kDouble);
+    Tensor loss = like({}, logits, at::kFloat), logp = like(ids.sizes(), logits, at::kFloat), scratch = like({2 * r.t.rows + 1}, logits, at::kDouble);
     if (stats) *stats = like({r.t.rows, 2}, logits, at::kFloat), *g = like({r.t.rows}, logits, at::kFloat);
     check(lib.ab_policy_loss_fwd(&r.t, &a.p, f32(loss), f32(logp), stats ? f32(*stats) : nullptr, stats ? f32(*g) : nullptr, scratch.data_ptr<double>(), stream()), "ab_policy_loss_fwd");
     return {loss, logp};
@@ -408,7 +408,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_grad(const Tensor& logits_, const
         if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();   // written in place: what autograd has kept of it is no longer good
     }
     const Rows r(logits, ids, mask);
-    Tensor loss = like({}, logits, at::kFloat), logp = like(ids.sizes(), logits, at::kFloat), scratch = like({2 * r.t.rows + 2}, logits, at::kDouble);
+    Tensor loss = like({}, logits, at::kFloat), logp = like(ids.sizes(), logits, at::kFloat), scratch = like({r.t.rows + 1}, logits, at::kDouble);
     check(lib.ab_policy_loss_grad(&r.t, &a.p, (float)scale, f32(loss), f32(logp), out.data_ptr(), scratch.data_ptr<double>(), stream()), "ab_policy_loss_grad");
     return {loss, logp, out};
 }

@@ -224,10 +224,10 @@ typedef struct ab_policy {
     float clip_low, clip_high, kl, denom;
 } ab_policy;
 /* loss: fp32 [1]. logp32: fp32 [rows]. g: fp32 [rows], for ab_token_logp_bwd with rows_per_g 1: the derivative of the loss by each row's
- * log-probability. rows_scratch: fp64 [2 * rows + 2]. stats as above. */
+ * log-probability. rows_scratch: fp64 [2 * rows + 1]. stats as above. */
 int ab_policy_loss_fwd(const ab_logit_rows* t, const ab_policy* p, float* loss, float* logp32, float* stats, float* g, double* rows_scratch,
                        void* stream);
-/* Loss and scale * its gradient by the logits in one pass. dlogits: dense rows of dtype, over the logits themselves where those are dense, or apart from them. */
+/* Loss and scale * its gradient by the logits in one pass. rows_scratch: fp64 [rows + 1]. dlogits: dense rows of dtype, over the logits themselves where those are dense, or apart from them. */
 int ab_policy_loss_grad(const ab_logit_rows* t, const ab_policy* p, float scale, float* loss, float* logp32, void* dlogits,
                         double* rows_scratch, void* stream);
 /* The preference loss of `pairs` pairs of answers of `steps` rows each, first the better ones, then the worse ones, t->rows = 2 * pairs * steps:

@@ -1000,6 +1000,23 @@ def test_entries_take_a_state_in_place_and_refuse_bad_pointers():
     assert _lib.lib.ab_wkv7_seq_fwd(C.byref(s), y2.data_ptr() + 2, here.data_ptr(), st) == -1 and b"boundary" in _lib.lib.ab_last_error()
 
 
+@pytest.mark.parametrize("n,V,denom", [(37, 500, 0.0), (37, 5000, 3.0), (160, 20011, 3.0), (16400, 64, 0.0)])
+def test_policy_entries_keep_to_the_scratch_that_the_header_names(n, V, denom):
+    x, ids, old, A, mask, ref = policy_inputs(n, V, "fp16")
+    t = _lib.LogitRows(_lib.DT_F16, V, n, V, x.data_ptr(), ids.data_ptr(), mask.data_ptr())
+    p = _lib.Policy(old.data_ptr(), A.data_ptr(), ref.data_ptr(), 0.2, 0.2, 0.05, denom)
+    loss, logp, stats, g, dx = (torch.empty(s, device="cuda") for s in (2, n, 2 * n, n, 0))
+    dx = torch.empty_like(x)
+    st = torch.cuda.current_stream().cuda_stream
+    for size, call in ((2 * n + 1, lambda s: _lib.lib.ab_policy_loss_fwd(C.byref(t), C.byref(p), loss.data_ptr(), logp.data_ptr(), stats.data_ptr(), g.data_ptr(), s, st)),
+                       (n + 1, lambda s: _lib.lib.ab_policy_loss_grad(C.byref(t), C.byref(p), 1.0, loss.data_ptr() + 4, logp.data_ptr(), dx.data_ptr(), s, st))):
+        scratch = torch.full((size + 64,), 7.25, dtype=torch.float64, device="cuda")
+        assert call(scratch.data_ptr()) == 0
+        assert bool((scratch[size:] == 7.25).all())
+    want, wlogp, wdx = ab.policy_loss_grad(x, ids, old, A, mask=mask, ref_logp=ref, kl=0.05, denom=denom or None)
+    assert float(loss[0]) == float(want) and float(loss[1]) == float(want) and torch.equal(logp, wlogp) and torch.equal(dx, wdx)
+
+
 def test_what_cannot_be_right_is_refused():
     x, ids, old, A, mask, ref = policy_inputs(6, 500, "fp16")
     buf = torch.empty(6 * 500 + 8, dtype=torch.float16, device="cuda")

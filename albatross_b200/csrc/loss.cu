@@ -438,8 +438,8 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
 // comes next is asked of the hardware (cluster launch control: the grid has a block per row, and a running block takes the place of one that has not started), because
 // masked rows cost little and would unbalance fixed shares. What a row needs besides its logits (id, policy) travels the same way ahead of it; a row's own
 // log-probability and loss, in 64 bits, are the business of another warp.
-// 4096 x 65536 fp16 rows, the policy loss with its gradient (85 % of the rows count): 225 us = 4.8 TB/s, 73 % of the copy rate; 12 instructions per value and 2.2 per cycle bound it
-// before memory does (20 to 28 working warps, smaller or larger chunks and a chunk kept ahead in registers: 242 to 367 us).
+// 4096 x 65536 fp16 rows, the policy loss with its gradient (85 % of the rows count, the others' logits are not read): 243 us for 0.99 GB, 4.1 TB/s, 63 % of the copy rate. 21 instructions a
+// value at 2.2 a cycle; without a gradient 11 at 2.4, 111 us (20 to 28 working warps, smaller or larger chunks and a chunk kept ahead in registers: slower by 8 to 60 %).
 constexpr int RING_WARPS = 16, RING_THREADS = (RING_WARPS + 2) * 32, RING_CHUNK = 32768, RING_SLOTS = 7, RING_ROWS = 4;   // working warps; chunks, rows under way
 struct RingRow {
     int64_t r;          // -1: no more
@@ -987,9 +987,9 @@ int logit_rows(const RowTask& k, cudaStream_t st) {
             logit_short_kernel<E><<<(unsigned)((k.t.rows + LW - 1) / LW), LT, 0, st>>>(k);
             return check_cuda(cudaGetLastError(), "rows of logits");
         }
-        // The ring where a row would take more than two blocks of a cluster, and every SM has one. Ring and cluster, us, policy loss with gradient, fp16: 4096 x 65536 256
-        // and 319, 1000 x 65536 72 and 85, 4096 x 32003 162 and 180, 148 x 65536 16 and 19; on the other side 4096 x 16384 106 and 80, 4096 x 9001 111 and 88, 100 x 65536
-        // 16 and 14. fp32: 4096 x 32003 195 and 255, 1000 x 16384 36 and 37.
+        // The ring where a row would take more than two blocks of a cluster, and every SM has one. Ring and cluster, us, policy loss with gradient, every row counting, fp16:
+        // 4096 x 65536 269 and 372, 1000 x 65536 76 and 100, 4096 x 32003 172 and 204, 4096 x 20011 166 and 189, 148 x 65536 19 and 21; on the other side 4096 x 16384 109 and 95,
+        // 4096 x 9001 114 and 97, 100 x 65536 19 and 19. fp32: 4096 x 32003 206 and 241, 1000 x 16384 39 and 35.
         if (values > 2 * LT * 32 && k.t.rows >= n_sm) {
             static PerDeviceOnce once;
             const int st_ = once.run(nullptr, [&](const DeviceProps&) -> int {

@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(BLOCK ? BT : NT) norm_rows_fwd_kernel(const __
 
 // The backward pass, one read of x and dy: a block per SM, whose copying warp brings rows in ahead (a ring of bulk copies) and whose teams of TPR threads take them in
 // turn. A thread keeps the sums of its columns for dw and db from row to row; teams are added up in shared memory at the end, blocks by norm_finish_kernel, always in one order.
-constexpr int BWD_THREADS = 512, BWD_RING = 196608;   // (256 threads with twice the values each: 17 % fewer instructions, 71 us instead of 56 at 8192 x 4096 bf16)
+constexpr int BWD_THREADS = 512, BWD_RING = 196608;   // (256 threads with twice the values each: 17 % fewer instructions, 71 us instead of 56 at 8192 x 4096 bf16. 96 registers a thread: bf16 rows keep within them, fp16 rows of two pieces spill 116 bytes, 72 us, 160 with fp32 weights, and groups 104 to 132)
 struct NormBwd {
     NormArgs a;
     int tpr, seg, slots, row_bytes;   // threads per row, lanes per group (0: the row is one), rows in the ring

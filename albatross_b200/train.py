@@ -2,17 +2,17 @@
 
     RWKV7_TRAIN_OP   the WKV-7 recurrence of `RWKV7_BATCH_OP` over whole sequences, out of place and differentiable
     layer_norm       a block's norms, also in groups of a head (the norm behind the recurrence), differentiable
-    token_logp       log-probabilities of given ids under logits, differentiable: what the policy, the sampler or a reference
-                     model gave the tokens
+    token_logp       log-probabilities of given ids under logits, differentiable: what the policy or a reference model gave the tokens
     policy_loss      clipped ratios against the policy that sampled, with a penalty for leaving a reference; differentiable
     policy_loss_grad the same, loss and gradient by the logits in one pass over them
     preference_loss  pairs of a better and a worse answer; differentiable
 
-They run on the current stream of their tensors' device and take strided inputs (the last dimension dense and, but for
-the recurrence, one stride between rows: logits[:, :-1] of several sequences has two. Others are copied, once for both passes). Gradients are those of the formulas in include/albatross_b200.h; they cannot be differentiated again,
-and there are no forward-mode derivatives: a tensor with a tangent is refused. Neither can they be traced (torch.compile, torch.export,
-make_fx: call them from a function under torch.compiler.disable) or transformed by torch.func.grad; torch.vmap calls them slice by slice. The
-reference only generates: none of these has a counterpart there.
+They run on the current stream of their tensors' device and take strided inputs: the last dimension dense and, but for the recurrence,
+one stride between rows (logits[:, :-1] of several sequences has two). Others are copied, once for both passes. Gradients are those of
+the formulas in include/albatross_b200.h; they cannot be differentiated again, and there are no forward-mode derivatives: a tensor with a
+tangent is refused. Neither can they be traced (torch.compile, torch.export, make_fx: call them from a function under
+torch.compiler.disable) or transformed by torch.func.grad; torch.vmap calls them slice by slice. The reference only generates: none of
+these has a counterpart there.
 
 Arguments are checked, memory is taken and gradients are tied to autograd in csrc/train_op.cpp (`torch.ops.albatross_b200`), which
 calls the C entries of the kernel library; what does not fit raises RuntimeError.
@@ -51,7 +51,13 @@ def RWKV7_TRAIN_OP(state: Optional[torch.Tensor], r, w, k, v, a, b, lengths: Opt
     (None: zeros), which is left as it is. Returns y [B, T, C] and the state after the last step. `lengths`, int32 [B] on the device:
     sequence b ends after lengths[b] steps; what the inputs hold behind its end is not used, y and all gradients are zero there.
     Training keeps 16 KB per head and 16 steps between the passes. A NaN or an infinity in a step's inputs may show in the outputs of up to
-    15 steps before it."""
+    15 steps before it.
+
+    Decays: as long as none of a chunk of 16 steps' channels shrinks below 2^-16 over it (0.5 a step; a model's own, exp(-exp(w)) with w below
+    -0.5, stays above 0.545) a chunk is taken at once. Beyond that it is taken in pieces, down to single steps: up to 60 times as long forward and
+    250 times backward for decays below 2^-16 in a step.
+    Precision: states and sums are 32-bit; gradients that end in 16 bits are summed over a state's rows with 16-bit factors, and in bf16 what v and
+    the gradient of y hold below 2^-27 of a chunk's largest value loses bits."""
     return _wkv7(state, r, w, k, v, a, b, lengths)
 
 
@@ -82,8 +88,12 @@ def policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logp: Optional[torc
     Per token, with ratio = exp(logp - old_logp): -min(ratio A, clamp(ratio, 1 - clip[0], 1 + clip[1]) A) + kl (exp(ref_logp - logp) - (ref_logp - logp) - 1);
     their sum where `mask` (bool [...]) is True, divided by `denom` or else by the number of such tokens (at least 1). logits [..., V], ids [...];
     old_logp, advantages and ref_logp broadcast to the ids' shape and get no gradient; with kl 0 ref_logp does not count, and an advantage of 0
-    makes nothing of any ratio. old_logp None: the ratio is 1, as on the first step after
-    sampling. At a border of the clip range the unclipped side's gradient counts."""
+    makes nothing of any ratio. old_logp None: the ratio is 1, as on the first step after sampling. At a border of the clip range the unclipped
+    side's gradient counts.
+
+    old_logp are log-probabilities under the distribution that the tokens were drawn from. token_logp gives those of softmax(logits);
+    `sampler_simple_batch` of this package draws from another one (the argmax of logits plus uniform noise), and ratios against token_logp of its
+    logits carry the difference."""
     return _policy_loss(logits, ids, old_logp, advantages, mask, ref_logp, clip[0], clip[1], kl, _denom(denom))
 
 

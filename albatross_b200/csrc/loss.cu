@@ -39,17 +39,18 @@ struct PolicyRow {
 __device__ __forceinline__ PolicyRow policy_load(const ab_policy& p, int64_t r) {
     return {p.advantages[r], p.old_logp ? p.old_logp[r] : 0.f, p.ref_logp ? p.ref_logp[r] : 0.f};
 }
-// What a row's loss and its derivative by the log-probability are made of, in 64 bits and the same whichever way the gradient is made: a ratio or the penalty's exponential may be
-// infinite in 32 bits beside a factor that makes them small or nothing, and 1 - exp(gap) is small where the reference is near. With logp = rel - log(S) the logarithm is not needed:
-// ratio = exp(rel - old) / S, exp(gap) = exp(ref - rel) S. A factor of 0 counts for more than an infinite ratio: the ratio's exponential is held finite (exp(709) is; a NaN stays one), and without
-// a weight the reference is not looked at.
+// What a row's loss and its derivative by the log-probability are made of, in 64 bits and the same whichever way the gradient is made: a ratio or the
+// penalty's exponential may be infinite in 32 bits beside a factor that makes them small or nothing, and 1 - exp(gap) is small where the reference is
+// near. With logp = rel - log(S) the logarithm is not needed: ratio = exp(rel - old) / S, exp(gap) = exp(ref - rel) S. A factor of 0 counts for more
+// than an infinite ratio: the ratio's exponential is held finite (exp(709) is; a NaN stays one), and without a weight the reference is not looked at.
 struct PolicyTerms {
     double least, slope, e;      // min(ratio A, clipped A); the derivative by logp; exp(gap), or 1
     __device__ __forceinline__ double loss(const ab_policy& p, const PolicyRow& q, double logp) const {
         return -least + (p.ref_logp && p.kl != 0.f ? (double)p.kl * (e - ((double)q.ref - logp) - 1.0) : 0.0);
     }
 };
-// By a whole warp: its even lanes take the ratio's exponential, its odd ones the penalty's. All of a row's other warps wait for the slope. (old: the ratio is not 1; kl 0: no reference)
+// By a whole warp: its even lanes take the ratio's exponential, its odd ones the penalty's. All of a row's other warps wait for the slope. (old: the
+// ratio is not 1; kl 0: no reference)
 __device__ __forceinline__ PolicyTerms policy_terms(bool old, float old_logp, float A, float low, float high, float kl, float ref_logp, double rel, float S) {
     const bool odd = threadIdx.x & 1;
     const double x = odd ? (kl != 0.f ? (double)ref_logp - rel : 0.0) : old ? rel - (double)old_logp : 0.0;
@@ -69,7 +70,8 @@ __device__ __forceinline__ float policy_kl(const ab_policy& p) { return p.ref_lo
 __device__ __forceinline__ PolicyTerms policy_terms(const ab_policy& p, const PolicyRow& q, double rel, float S) {
     return policy_terms(p.old_logp != nullptr, q.old, q.A, p.clip_low, p.clip_high, policy_kl(p), q.ref, rel, S);
 }
-// The same where every register counts: inlined, it made the rows' exponentials spill (4096 x 9001 fp16 rows with gradient 90 us, called 85; 4096 x 32003 in the ring the other way round, 158 and 165).
+// The same where every register counts: inlined, it made the rows' exponentials spill (4096 x 9001 fp16 rows with gradient 90 us, called 85; 4096 x
+// 32003 in the ring the other way round, 158 and 165).
 __device__ __noinline__ PolicyTerms policy_terms_call(bool old, float old_logp, float A, float low, float high, float kl, float ref_logp, double rel, float S) {
     return policy_terms(old, old_logp, A, low, high, kl, ref_logp, rel, S);
 }
@@ -141,10 +143,10 @@ __device__ __forceinline__ float piece_top(const uint4& u) {
     for (int c = 1; c < Pieces<E>::N; ++c) m = fmaxf(m, f[c]);
     return m;
 }
-// What exponentials are taken relative to: exp(x - m) = 2^(x log2(e) - c) with c = m log2(e) rounded, one multiply-add and one ex2.approx (good to 2^-22).
-// Joining parts takes the difference of two c, so that the rounding of c cancels. The constant's own rounding, 2^-25.7 of x, is left out of the gradient's exponentials only;
-// beyond |m| = 64 it would count, as would c's, and at the type's ends (rows of the lowest value throughout, which some programs use for a mask) the product
-// overflows: there the difference comes first.
+// What exponentials are taken relative to: exp(x - m) = 2^(x log2(e) - c) with c = m log2(e) rounded, one multiply-add and one ex2.approx (good to
+// 2^-22). Joining parts takes the difference of two c, so that the rounding of c cancels. The constant's own rounding, 2^-25.7 of x, is left out of
+// the gradient's exponentials only; beyond |m| = 64 it would count, as would c's, and at the type's ends (rows of the lowest value throughout, which
+// some programs use for a mask) the product overflows: there the difference comes first.
 constexpr float LOG2E = 1.4426950408889634f, LOG2E_LOW = 1.925963033500e-8f;   // log2(e), and what its 24 bits leave of it
 struct Ref {
     float m, c;
@@ -166,8 +168,8 @@ __device__ __forceinline__ void exp_from(float* f, const Ref& r) {
         for (int i = 0; i < N; ++i) f[i] = ex2(fmaf(f[i], LOG2E, -r.c));
     }
 }
-// The same for sums, with the constant in two parts: one part alone is off by 1.3e-8 of it, which all of a row's exponentials share, so that log-probabilities of -10 were off by
-// 1e-7 to one side and mean losses with them.
+// The same for sums, with the constant in two parts: one part alone is off by 1.3e-8 of it, which all of a row's exponentials share, so that
+// log-probabilities of -10 were off by 1e-7 to one side and mean losses with them.
 template <int N>
 __device__ __forceinline__ void exp_to_add(float* f, const Ref& r) {
     if (r.huge) {
@@ -182,9 +184,9 @@ __device__ __forceinline__ float exp_from(float x, const Ref& r) {
     exp_from<1>(&x, r);
     return x;
 }
-// 2^x for factors of whole sums, by the series of exp((x - n) log(2)) up to the seventh power, n the nearest integer: within 2^-23 and to neither side. (ex2.approx is 4e-8 too small on
-// average; a sum goes through two or three factors on its way, so that log-probabilities over 65536 values were 1.1e-7 too large, and are 5e-8 now, for 1.5% of the
-// time of 4096 rows.)
+// 2^x for factors of whole sums, by the series of exp((x - n) log(2)) up to the seventh power, n the nearest integer: within 2^-23 and to neither
+// side. (ex2.approx is 4e-8 too small on average; a sum goes through two or three factors on its way, so that log-probabilities over 65536 values
+// were 1.1e-7 too large, and are 5e-8 now, for 1.5% of the time of 4096 rows.)
 __device__ __forceinline__ float ex2_factor(float x) {
     if (!(fabsf(x) < 126.f)) return ex2(x);
     const float n = rintf(x), y = (x - n) * 0.69314718f;
@@ -210,8 +212,8 @@ __device__ __forceinline__ float rebase(const Ref& from, const Ref& to) {
     }
     return ex2_factor(d);
 }
-// Writes p times a piece's exponentials to the row `dx`, which starts `lead` values into a piece of 16 bytes as the row of logits does (aligned), or anywhere.
-// FULL: the piece holds values of the row alone, and dx is aligned.
+// Writes p times a piece's exponentials to the row `dx`, which starts `lead` values into a piece of 16 bytes as the row of logits does (aligned), or
+// anywhere. FULL: the piece holds values of the row alone, and dx is aligned.
 template <class E, bool FULL>
 __device__ __forceinline__ void write_piece(const Pieces<E>& row, const float* e, int i, E* dx, bool aligned, float p, const Extent& grads) {
     constexpr int N = Pieces<E>::N;
@@ -299,8 +301,8 @@ __device__ __forceinline__ int count_rows(const uint8_t* mask, int64_t rows) {
     return n;
 }
 
-// One row per cluster of blocks, a run of pieces per block; a thread keeps the exponentials of EPT values in registers between the sums and the gradient, so
-// that the logits are read once and each exponential is taken once (rows longer than MAX_CLUSTER * LT * EPT values are read twice).
+// One row per cluster of blocks, a run of pieces per block; a thread keeps the exponentials of EPT values in registers between the sums and the
+// gradient, so that the logits are read once and each exponential is taken once (rows longer than MAX_CLUSTER * LT * EPT values are read twice).
 template <class E, int EPT>
 __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant__ RowTask k) {
     constexpr int N = Pieces<E>::N, NV = EPT / N;
@@ -433,13 +435,14 @@ __global__ void __launch_bounds__(LT, 4) logit_rows_kernel(const __grid_constant
 }
 
 // ---- long rows, at least one per SM ----------------------------------------------------------------------------------
-// One block per SM takes row after row: a warp asks for a row's chunks with bulk copies into a ring, ahead of the warps that add them up and then go through the ring
-// once more for the gradient; as they hand chunks back the next row's come in, so that copies are under way through the sums, the join and the gradient alike. Which row
-// comes next is asked of the hardware (cluster launch control: the grid has a block per row, and a running block takes the place of one that has not started), because
-// masked rows cost little and would unbalance fixed shares. What a row needs besides its logits (id, policy) travels the same way ahead of it; a row's own
-// log-probability and loss, in 64 bits, are the business of another warp.
-// 4096 x 65536 fp16 rows, the policy loss with its gradient (85 % of the rows count, the others' logits are not read): 243 us for 0.99 GB, 4.1 TB/s, 63 % of the copy rate. 21 instructions a
-// value at 2.2 a cycle; without a gradient 11 at 2.4, 111 us (20 to 28 working warps, smaller or larger chunks and a chunk kept ahead in registers: slower by 8 to 60 %).
+// One block per SM takes row after row: a warp asks for a row's chunks with bulk copies into a ring, ahead of the warps that add them up and then go
+// through the ring once more for the gradient; as they hand chunks back the next row's come in, so that copies are under way through the sums, the
+// join and the gradient alike. Which row comes next is asked of the hardware (cluster launch control: the grid has a block per row, and a running
+// block takes the place of one that has not started), because masked rows cost little and would unbalance fixed shares. What a row needs besides its
+// logits (id, policy) travels the same way ahead of it; a row's own log-probability and loss, in 64 bits, are the business of another warp. 4096 x
+// 65536 fp16 rows, the policy loss with its gradient (85 % of the rows count, the others' logits are not read): 243 us for 0.99 GB, 4.1 TB/s, 63 % of
+// the copy rate. 21 instructions a value at 2.2 a cycle; without a gradient 11 at 2.4, 111 us (20 to 28 working warps, smaller or larger chunks and a
+// chunk kept ahead in registers: slower by 8 to 60 %).
 constexpr int RING_WARPS = 16, RING_THREADS = (RING_WARPS + 2) * 32, RING_CHUNK = 32768, RING_SLOTS = 7, RING_ROWS = 4;   // working warps; chunks, rows under way
 struct RingRow {
     int64_t r;          // -1: no more
@@ -465,7 +468,10 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
     const int V = k.t.vocab, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < RING_SLOTS; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.vacant[i], RING_WARPS);
-        for (int i = 0; i < RING_ROWS; ++i) mbar_init(&sh.row_full[i], 1), mbar_init(&sh.row_summed[i], RING_WARPS), mbar_init(&sh.row_sloped[i], 1), mbar_init(&sh.row_vacant[i], RING_WARPS + 1);
+        for (int i = 0; i < RING_ROWS; ++i) {
+            mbar_init(&sh.row_full[i], 1), mbar_init(&sh.row_summed[i], RING_WARPS);
+            mbar_init(&sh.row_sloped[i], 1), mbar_init(&sh.row_vacant[i], RING_WARPS + 1);
+        }
         mbar_init(&sh.cancelled, 1);
         fence_mbar_init();
         sh.failed = 0;
@@ -727,7 +733,8 @@ __global__ void __launch_bounds__(RING_THREADS, 1) logit_ring_kernel(const __gri
                 }
                 // the id's own value, by the thread that wrote its piece
                 const int piece = (id + row.lead) / N;
-                if ((piece >= first && piece < end ? (piece - first) % (RING_WARPS * 32) == tid : piece == edge) && grads.holds(dx + id)) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));
+                const bool mine = piece >= first && piece < end ? (piece - first) % (RING_WARPS * 32) == tid : piece == edge;
+                if (mine && grads.holds(dx + id)) dx[id] = from_f<E>(fmaf(p, exp_from(at, ref), g));
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.row_vacant[n % RING_ROWS]);
@@ -848,7 +855,8 @@ __global__ void __launch_bounds__(LT, 6) dlogits_kernel(const __grid_constant__ 
         for (int j = 0; j < DV; ++j) u[j] = row.template get<FULL>(at0 + j * LT + tid);
         const int id = row_id(k.t, r);
         const float* gr = k.g + r / k.rows_per_g;
-        const float g = (Extent(k.g, (uint64_t)((k.t.rows + k.rows_per_g - 1) / k.rows_per_g) * sizeof(float)).holds(gr) ? *gr : 0.f) * (k.scale ? *k.scale : 1.f), p = -g * k.stats[2 * r + 1];
+        const Extent all(k.g, (uint64_t)((k.t.rows + k.rows_per_g - 1) / k.rows_per_g) * sizeof(float));
+        const float g = (all.holds(gr) ? *gr : 0.f) * (k.scale ? *k.scale : 1.f), p = -g * k.stats[2 * r + 1];
         const Ref ref(k.stats[2 * r]);
         const int own = (id + row.lead) / N - at0;
         const bool mine = own >= 0 && own < LT * DV && own % LT == tid;
@@ -987,9 +995,10 @@ int logit_rows(const RowTask& k, cudaStream_t st) {
             logit_short_kernel<E><<<(unsigned)((k.t.rows + LW - 1) / LW), LT, 0, st>>>(k);
             return check_cuda(cudaGetLastError(), "rows of logits");
         }
-        // The ring where a row would take more than two blocks of a cluster, and every SM has one. Ring and cluster, us, policy loss with gradient, every row counting, fp16:
-        // 4096 x 65536 269 and 372, 1000 x 65536 76 and 100, 4096 x 32003 172 and 204, 4096 x 20011 166 and 189, 148 x 65536 19 and 21; on the other side 4096 x 16384 109 and 95,
-        // 4096 x 9001 114 and 97, 100 x 65536 19 and 19. fp32: 4096 x 32003 206 and 241, 1000 x 16384 39 and 35.
+        // The ring where a row would take more than two blocks of a cluster, and every SM has one. Ring and cluster, us, policy loss with gradient,
+        // every row counting, fp16: 4096 x 65536 269 and 372, 1000 x 65536 76 and 100, 4096 x 32003 172 and 204, 4096 x 20011 166 and 189, 148 x
+        // 65536 19 and 21; on the other side 4096 x 16384 109 and 95, 4096 x 9001 114 and 97, 100 x 65536 19 and 19. fp32: 4096 x 32003 206 and 241,
+        // 1000 x 16384 39 and 35.
         if (values > 2 * LT * 32 && k.t.rows >= n_sm) {
             static PerDeviceOnce once;
             const int st_ = once.run(nullptr, [&](const DeviceProps&) -> int {
@@ -1042,9 +1051,8 @@ int token_logp_bwd(const ab_logit_rows& t, const float* stats, const float* g, i
 
 int policy_loss(const ab_logit_rows& t, const ab_policy& p, float scale, float* loss, float* logp32, float* stats, float* g, void* dlogits,
                 double* rows_scratch, cudaStream_t st) {
-    // Where the gradient is made in this pass each block needs the denominator: it counts the rows itself up to 16384 of them (64 values a thread, from
-    // L2, beside its row), a launch ahead of it does beyond that.
-    // rows_scratch: the rows' losses, that, and the rows' slopes.
+    // Where the gradient is made in this pass each block needs the denominator: it counts the rows itself up to 16384 of them (64 values a thread,
+    // from L2, beside its row), a launch ahead of it does beyond that. rows_scratch: the rows' losses, that, and the rows' slopes.
     double* inv = nullptr;
     if (dlogits && (p.denom != 0.f || t.rows > 16384)) {
         inv = rows_scratch + t.rows;

@@ -62,7 +62,9 @@ __global__ void __launch_bounds__(NT) norm_fwd_kernel(const __grid_constant__ No
     const float rstd = 1.f / sqrtf(block_sum_nt(q, red) / (float)m + a.eps);
     E* y = static_cast<E*>(a.y) + row * a.C + g * m;
     for (int i = threadIdx.x; i < m; i += NT)
-        put(y + i, from_f<E>(fmaf((get(x + i, in) - mean) * rstd, w ? get(w + g * m + i, weight_extent<W>(a, w)) : 1.f, b ? get(b + g * m + i, weight_extent<W>(a, b)) : 0.f)),
+        put(y + i,
+            from_f<E>(fmaf((get(x + i, in) - mean) * rstd, w ? get(w + g * m + i, weight_extent<W>(a, w)) : 1.f,
+                           b ? get(b + g * m + i, weight_extent<W>(a, b)) : 0.f)),
             dense_extent<E>(a, a.y));
     if (a.mean && threadIdx.x == 0) {
         put(a.mean + unit, mean, stats_extent(a, a.mean));
@@ -108,8 +110,9 @@ __global__ void __launch_bounds__(NT) norm_cols_kernel(const __grid_constant__ N
     for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
         const float dy = get(static_cast<const E*>(a.dy) + r * a.dy_stride + c, dy_extent<E>(a));
         const int64_t at = r * a.groups + c / m;
+        const float x = get(static_cast<const E*>(a.x) + r * a.x_stride + c, x_extent<E>(a));
         db += dy;
-        dw = fmaf(dy, (get(static_cast<const E*>(a.x) + r * a.x_stride + c, x_extent<E>(a)) - get(a.mean + at, stats_extent(a, a.mean))) * get(a.rstd + at, stats_extent(a, a.rstd)), dw);
+        dw = fmaf(dy, (x - get(a.mean + at, stats_extent(a, a.mean))) * get(a.rstd + at, stats_extent(a, a.rstd)), dw);
     }
     put(a.scratch + ((int64_t)blockIdx.y * 2) * a.C + c, dw, Extent(a.scratch, a.scratch_bytes));
     put(a.scratch + ((int64_t)blockIdx.y * 2 + 1) * a.C + c, db, Extent(a.scratch, a.scratch_bytes));
@@ -144,8 +147,8 @@ __global__ void __launch_bounds__(FT) norm_finish_kernel(const __grid_constant__
 }
 
 // ---- rows in pieces of 16 bytes ----------------------------------------------------------------------------------------
-// For rows, weights and outputs on 16-byte boundaries; others take the kernels above. A group is a row (its values are spread over a team of TPR threads), or
-// SEG lanes of a warp, one piece each.
+// For rows, weights and outputs on 16-byte boundaries; others take the kernels above. A group is a row (its values are spread over a team of TPR
+// threads), or SEG lanes of a warp, one piece each.
 template <class E>
 constexpr int per_piece = 16 / sizeof(E);
 
@@ -185,8 +188,8 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {   // over align
     return v;
 }
 
-// s / m from 1 / m rounded, by one step on the remainder (which is exact): exact where the quotient is, so that rows of one value have no deviation. (The product alone is off by up to 1.5
-// units, which rows of 1000 whose length is not a power of two showed as 0.019, times 1 / sqrt(eps).)
+// s / m from 1 / m rounded, by one step on the remainder (which is exact): exact where the quotient is, so that rows of one value have no deviation.
+// (The product alone is off by up to 1.5 units, which rows of 1000 whose length is not a power of two showed as 0.019, times 1 / sqrt(eps).)
 __device__ __forceinline__ float quotient(float s, float m, float inv_m) {
     const float q = s * inv_m;
     return fmaf(fmaf(-q, m, s), inv_m, q);
@@ -212,7 +215,8 @@ __global__ void __launch_bounds__(BLOCK ? BT : NT) norm_rows_fwd_kernel(const __
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int p = p0 + j * TPR;
-        unpack<E>(p < pieces && x_extent<E>(a).holds(reinterpret_cast<const uint4*>(x) + p) ? __ldcs(reinterpret_cast<const uint4*>(x) + p) : make_uint4(0, 0, 0, 0), f[j]);
+        const uint4* from = reinterpret_cast<const uint4*>(x) + p;
+        unpack<E>(p < pieces && x_extent<E>(a).holds(from) ? __ldcs(from) : make_uint4(0, 0, 0, 0), f[j]);
     }
     auto total = [&](float v, float* r) {     // over the row
         v = warp_sum(v);
@@ -275,9 +279,12 @@ __global__ void __launch_bounds__(BLOCK ? BT : NT) norm_rows_fwd_kernel(const __
     }
 }
 
-// The backward pass, one read of x and dy: a block per SM, whose copying warp brings rows in ahead (a ring of bulk copies) and whose teams of TPR threads take them in
-// turn. A thread keeps the sums of its columns for dw and db from row to row; teams are added up in shared memory at the end, blocks by norm_finish_kernel, always in one order.
-constexpr int BWD_THREADS = 512, BWD_RING = 196608;   // (256 threads with twice the values each: 17 % fewer instructions, 71 us instead of 56 at 8192 x 4096 bf16. 96 registers a thread: bf16 rows keep within them, fp16 rows of two pieces spill 116 bytes, 72 us, 160 with fp32 weights, and groups 104 to 132)
+// The backward pass, one read of x and dy: a block per SM, whose copying warp brings rows in ahead (a ring of bulk copies) and whose teams of TPR
+// threads take them in turn. A thread keeps the sums of its columns for dw and db from row to row; teams are added up in shared memory at the end,
+// blocks by norm_finish_kernel, always in one order.
+// (256 threads with twice the values each: 17 % fewer instructions, 71 us instead of 56 at 8192 x 4096 bf16. 96 registers a thread: bf16 rows keep
+// within them, fp16 rows of two pieces spill 116 bytes, 72 us, 160 with fp32 weights, and groups 104 to 132.)
+constexpr int BWD_THREADS = 512, BWD_RING = 196608;
 struct NormBwd {
     NormArgs a;
     int tpr, seg, slots, row_bytes;   // threads per row, lanes per group (0: the row is one), rows in the ring
@@ -386,8 +393,8 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
             loads_returned(used, &nobody);
             __syncwarp();
             if (lane == 0) mbar_arrive(&vacant[slot]);
-            // xh and dy w are worked out again for dx where a row is one group: kept over the block's exchange of sums they cost spills (65 us instead of 56 at 8192 x
-            // 4096 bf16; over a few lanes' exchange 30.5 instead of 35.5 at 4097 x 2560 fp16 in groups of 64)
+            // xh and dy w are worked out again for dx where a row is one group: kept over the block's exchange of sums they cost spills (65 us
+            // instead of 56 at 8192 x 4096 bf16; over a few lanes' exchange 30.5 instead of 35.5 at 4097 x 2560 fp16 in groups of 64)
             float s = 0.f, q = 0.f, sj[NS], qj[NS], xh[SEG ? NV : 1][N], e[SEG ? NV : 1][N];
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
@@ -467,7 +474,7 @@ __global__ void __launch_bounds__(BWD_THREADS + 32, 1) norm_rows_bwd_kernel(cons
                 if (t + j * tpr < pieces)
 #pragma unroll
                     for (int c = 0; c < N; ++c)
-                        if (Extent(ring, BWD_RING).holds(sums + team * a.C + (t + j * tpr) * N + c)) sums[team * a.C + (t + j * tpr) * N + c] = which ? db[j][c] : dw[j][c];
+                        put(sums + team * a.C + (t + j * tpr) * N + c, which ? db[j][c] : dw[j][c], Extent(ring, BWD_RING));
         }
         __syncthreads();
         for (int c = tid; c < a.C; c += BWD_THREADS + 32) {

@@ -7,8 +7,8 @@
 
 namespace ab {
 
-// An array as the caller gave it. In the range-checking build an access's final address is held against it, whatever led to that address (loop bounds, strides, a ring's slots); what is
-// outside is recorded and not made. Nothing at all in the normal build.
+// An array as the caller gave it. In the range-checking build an access's final address is held against it, whatever led to that address (loop
+// bounds, strides, a ring's slots); what is outside is recorded and not made. Nothing at all in the normal build.
 struct Extent {
 #ifdef AB_BOUNDS_CHECK
     const char* base;

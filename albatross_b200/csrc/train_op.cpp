@@ -1,8 +1,9 @@
-// The operators with gradients as torch operators (torch.ops.albatross_b200.*): arguments checked, memory from torch's allocator, the C entries of the kernel library
-// called on torch's current stream of the tensors' device, gradients through torch's C++ autograd. In Python the same costs 100 us a training pass more than the engine's
-// own 50, which is what small calls take.
+// The operators with gradients as torch operators (torch.ops.albatross_b200.*): arguments checked, memory from torch's allocator, the C entries of
+// the kernel library called on torch's current stream of the tensors' device, gradients through torch's C++ autograd. In Python the same costs 100 us
+// a training pass more than the engine's own 50, which is what small calls take.
 //
-// The kernel library is not linked: albatross_b200_train_bind() is given the path of the one that the package has loaded (the normal or the range-checking build).
+// The kernel library is not linked: albatross_b200_train_bind() is given the path of the one that the package has loaded (the normal or the
+// range-checking build).
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -60,8 +61,8 @@ struct Plain {
     Tensor t;
 };
 OptTensor or_none(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-// What would be lost without a word. A trace in the making would hold the outputs' allocation and not the call, and torch.func's wrappers have no memory. A tangent's tensor need not
-// require a gradient, and would be taken below autograd.
+// What would be lost without a word. A trace in the making would hold the outputs' allocation and not the call, and torch.func's wrappers have no
+// memory. A tangent's tensor need not require a gradient, and would be taken below autograd.
 bool traced() {
     using Key = c10::impl::TorchDispatchModeKey;
     for (const Key k : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL})
@@ -74,8 +75,9 @@ void check_plain(const char* who, const T&... t) {
                 ": cannot be traced or transformed (torch.compile, torch.export, make_fx, torch.func.grad); in a compiled program call it from a function under torch.compiler.disable");
     TORCH_CHECK(!((t.defined() && t._fw_grad(/*level=*/0).defined()) || ...), who, ": forward-mode derivatives are not available");
 }
-// What a backward pass refuses. Gradients are not differentiable: asking for a graph of them is an error, not a silent zero. And in a stream capture a leaf that an earlier graph still ties
-// to the default stream: adding its gradient would make that stream wait for the capturing one, which the default stream cannot, and the capture would be lost with a less telling error.
+// What a backward pass refuses. Gradients are not differentiable: asking for a graph of them is an error, not a silent zero. And in a stream capture
+// a leaf that an earlier graph still ties to the default stream: adding its gradient would make that stream wait for the capturing one, which the
+// default stream cannot, and the capture would be lost with a less telling error.
 void check_backward() {
     check_plain("albatross_b200: gradients");
     TORCH_CHECK(!at::GradMode::is_enabled(), "albatross_b200: the gradients of these operators cannot be differentiated again (create_graph)");
@@ -189,8 +191,8 @@ std::tuple<Tensor, Tensor> wkv7(const OptTensor& state_, const Tensor& r, const 
 }
 
 // ---- the norms ---------------------------------------------------------------------------------------------------------------------
-// [..., C] with a dense last dimension and one stride between rows, of `least` values or more; others are copied. Here, ahead of autograd, so that the backward pass reads the same
-// copy (logits[:, :-1] of several sequences are copied once, not once in each pass).
+// [..., C] with a dense last dimension and one stride between rows, of `least` values or more; others are copied. Here, ahead of autograd, so that
+// the backward pass reads the same copy (logits[:, :-1] of several sequences are copied once, not once in each pass).
 Tensor one_stride(const Tensor& t, int64_t least) {
     bool fits = t.dim() < 1 || t.size(-1) <= 1 || t.stride(-1) == 1;
     int64_t outer = -1;   // the stride that goes with the dimensions so far

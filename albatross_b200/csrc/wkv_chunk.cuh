@@ -5,25 +5,27 @@
 //   A_ab = tril(a_E b_E^T, -1),  A_ak = tril(a_E k_E^T, -1),  A_rb = tril(r_E b_E^T),  A_rk = tril(r_E k_E^T)        16 x 16
 //   Q = (1 - A_ab)^-1,  a' = Q a_E,  A' = Q A_ak
 //   u^T = S_E a'^T + v^T A'^T,   y^T = S_E r_E^T + u^T A_rb^T + v^T A_rk^T,   S <- S_E + u^T b_E + v^T k_E
-// (the triangular form of the delta rule's chunks, Yang et al., "Parallelizing linear transformers with the delta rule over sequence length", 2024, here for a decay
-// per channel and separate a and b). Backwards, with G the gradient of the state after the chunk, h of u:
+// (the triangular form of the delta rule's chunks, Yang et al., "Parallelizing linear transformers with the delta rule over sequence length", 2024,
+// here for a decay per channel and separate a and b). Backwards, with G the gradient of the state after the chunk, h of u:
 //   h^T = (dy^T A_rb + G b_E^T) Q,   dv^T = dy^T A_rk + G k_E^T + h^T A_ak,   G <- (G + dy^T r_E + h^T a_E) diag(exp(end))
 //   P_yu = tril(dy u^T),  P_yv = tril(dy v^T),  P_hu = tril(h u^T, -1),  P_hv = tril(h v^T, -1)                       16 x 16
 //   dr = (dy S_E + P_yu b_E + P_yv k_E) exp(cw_t - end),   da = (h S_E + P_hu b_E + P_hv k_E) exp(cw_{t-1} - end)
 //   db = (u G + P_yu^T r_E + P_hu^T a_E) exp(end - cw_t),   dk = (v G + P_yv^T r_E + P_hv^T a_E) exp(end - cw_t)
-// and the gradient of a step's log decay collects what flows through it: from the state before to the state after the chunk (the column sums of G o S_E), from steps
-// before it to the state after (b, k times their G parts), from the state before to steps from it on (r, a times their S parts), and between steps on both sides
-// (r, a times their P parts less b, k times theirs, summed from it on).
+// and the gradient of a step's log decay collects what flows through it: from the state before to the state after the chunk (the column sums of G o
+// S_E), from steps before it to the state after (b, k times their G parts), from the state before to steps from it on (r, a times their S parts), and
+// between steps on both sides (r, a times their P parts less b, k times theirs, summed from it on).
 //
-// Precision. States and sums are 32-bit. A factor of a product that meets a state is the sum of two fp16 values, hi + lo (22 bits), after scaling by a power of two that
-// brings the largest value of its tile (of its row, for states) to 2^13 .. 2^14; three of the four partial products are made, the fourth is 2^-22 of the
-// result. v and dy are exact in one fp16 value. One product therefore costs three (two) mma.sync.m16n8k16; tf32 with its own three would cost six of the same rate.
-// What only ends in 16-bit gradients and sums over the rows of a state is split into two bf16 values instead (16 bits, no scale to agree on among warps).
+// Precision. States and sums are 32-bit. A factor of a product that meets a state is the sum of two fp16 values, hi + lo (22 bits), after scaling by
+// a power of two that brings the largest value of its tile (of its row, for states) to 2^13 .. 2^14; three of the four partial products are made, the
+// fourth is 2^-22 of the result. v and dy are held in one fp16 value (fp16: as they are; bf16: exact down to 2^-27 of the largest). One product
+// therefore costs three (two) mma.sync.m16n8k16; tf32 with its own three would cost six of the same rate. What only ends in 16-bit gradients and sums
+// over the rows of a state is split into two bf16 values instead (16 bits, no scale to agree on among warps).
 //
-// Factors relative to the end grow as the decays shrink: up to exp(-end). Up to 2^16 (decays of 0.5 per step; the model's are above 0.545) the split's 22 bits
-// stand, since a tile's values down to 2^-16 of its largest keep them. A chunk beyond that ("steep") is taken in pieces of 8, 4, 2 or 1 steps: the same code, with the other
-// steps' inputs as zeros and their decays as ones. In a piece of one step (whose decay may be anything) r_E = r, b_E = b, k_E = k, there is no A_ab and A_ak, and u = S a with the state
-// before its decay. Backwards the state before each piece is made again from the one before the chunk.
+// Factors relative to the end grow as the decays shrink: up to exp(-end). Up to 2^16 (decays of 0.5 per step; the model's are above 0.545) the
+// split's 22 bits stand, since a tile's values down to 2^-16 of its largest keep them. A chunk beyond that ("steep") is taken in pieces of 8, 4, 2 or
+// 1 steps: the same code, with the other steps' inputs as zeros and their decays as ones. In a piece of one step (whose decay may be anything) r_E =
+// r, b_E = b, k_E = k, there is no A_ab and A_ak, and u = S a with the state before its decay. Backwards the state before each piece is made again
+// from the one before the chunk.
 #pragma once
 #include "train.cuh"
 

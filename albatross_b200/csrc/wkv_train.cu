@@ -35,7 +35,8 @@ __device__ __forceinline__ int seq_length(const WkvSeq& s, int b) {
     return s.lengths ? min(max(s.lengths[b], 0), s.T) : s.T;
 }
 
-// A head's steps 0 .. n - 1 of an array, 64 values each, `step` values apart from the first one at `p` on; all heads' states, `each` of them per head.
+// A head's steps 0 .. n - 1 of an array, 64 values each, `step` values apart from the first one at `p` on; all heads' states, `each` of them per
+// head.
 __device__ __forceinline__ Extent steps_extent(const void* p, int64_t n, int64_t step) {
     const int64_t last = n > 0 ? (n - 1) * step : 0, low = last < 0 ? last : 0;
     return Extent(p ? static_cast<const char*>(p) + 2 * low : nullptr, n > 0 ? (uint64_t)((last < 0 ? -last : last) + 64) * 2 : 0);
@@ -46,8 +47,8 @@ __device__ __forceinline__ Extent input_extent(const WkvSeq& s, int which, int64
 __device__ __forceinline__ Extent states_extent(const float* p, int64_t each) { return Extent(p, (uint64_t)gridDim.x * each * 4096 * sizeof(float)); }
 
 // ---- the forward pass ----------------------------------------------------------------------------------------------------
-// A block per head: four warps carry 16 rows of the state each in registers (rows do not meet: the accumulators of one product are the operand of the next
-// without leaving the warp), others prepare chunks ahead, each a whole one by itself, in a ring of buffers.
+// A block per head: four warps carry 16 rows of the state each in registers (rows do not meet: the accumulators of one product are the operand of the
+// next without leaving the warp), others prepare chunks ahead, each a whole one by itself, in a ring of buffers.
 using namespace wkvc;
 constexpr int FE_BYTES = (L + 1) * N * 4;   // factors relative to the chunk's end (put_factors)
 constexpr int HEAD_BYTES = (int)((sizeof(ChunkHead) + 127) / 128 * 128);
@@ -72,8 +73,9 @@ __device__ __forceinline__ float log2_decay(float w) {   // of exp(-exp(w)); fin
     const float d = -expf(w) * 1.4426950408889634f;
     return d < -2000.f ? -2000.f : d;
 }
-// Asks for one vector of a chunk's steps lo .. hi - 1 (zeros at the others) in a tile's place: a lane has eight columns (c8 = lane & 7) of steps lane >> 3, + 4, + 8,
-// + 12, here and when it takes them up again. All vectors of a chunk are on their way at once: one after the other they cost a warp 2000 cycles each.
+// Asks for one vector of a chunk's steps lo .. hi - 1 (zeros at the others) in a tile's place: a lane has eight columns (c8 = lane & 7) of steps lane
+// >> 3, + 4, + 8, + 12, here and when it takes them up again. All vectors of a chunk are on their way at once: one after the other they cost a warp
+// 2000 cycles each.
 __device__ __forceinline__ void stage_steps(uint32_t tile, const char* p, int64_t step, int lo, int hi, bool there, int lane, const Extent& in) {
     if (!AB_BC(lo >= 0 && lo < hi && hi <= L)) return;
 #pragma unroll
@@ -97,8 +99,9 @@ __device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_g
 __device__ __forceinline__ const char* steps_of(const WkvSeq& s, int which, int64_t b, int h, int t0, int lane) {
     return static_cast<const char*>(s.x[which]) + 2 * (b * s.bs[which] + (int64_t)t0 * s.ss[which] + h * N + 8 * (lane & 7));
 }
-// The factors of steps lo .. hi - 1 (the others' decays are 1), from the log decays behind fe's first row. fe: [L + 1][N], exp(sum before and including the steps up to a row's - end), a row
-// for no step first; fb: [L][N], exp(end - sum); decay: exp(end). In a piece of one step (single) fe is 1. Returns whether the chunk is steep, and then, but for a piece, writes nothing.
+// The factors of steps lo .. hi - 1 (the others' decays are 1), from the log decays behind fe's first row. fe: [L + 1][N], exp(sum before and
+// including the steps up to a row's - end), a row for no step first; fb: [L][N], exp(end - sum); decay: exp(end). In a piece of one step (single) fe
+// is 1. Returns whether the chunk is steep, and then, but for a piece, writes nothing.
 template <bool PIECE>
 __device__ __forceinline__ bool factors_of(int lo, int hi, bool single, float* fe, float* fb, float* decay, int lane) {
     float2 c = make_float2(0.f, 0.f), d[L];
@@ -138,8 +141,9 @@ __device__ __forceinline__ bool put_factors(const uint4* u, int n_on, float* fe,
     __syncwarp();
     return factors_of<false>(0, L, false, fe, fb, decay, lane);
 }
-// How many steps of a steep chunk are taken at once: 8, 4, 2 or 1, in pieces from its start on. 1024 steps x 64 heads, decays of 2^-2, 2^-3, 2^-6, 2^-17 a step: 0.66, 1.9, 4.3, 9.3 ms forward
-// and 2.2, 7.7, 27, 100 ms backward; 0.14 and 0.41 without a steep chunk. This and the next one are not inlined: there they cost every chunk registers (4% forward).
+// How many steps of a steep chunk are taken at once: 8, 4, 2 or 1, in pieces from its start on. 1024 steps x 64 heads, decays of 2^-2, 2^-3, 2^-6,
+// 2^-17 a step: 0.66, 1.9, 4.3, 9.3 ms forward and 2.2, 7.7, 27, 100 ms backward; 0.14 and 0.41 without a steep chunk. This and the next one are not
+// inlined: there they cost every chunk registers (4% forward).
 __device__ __noinline__ int steep_steps(const float* fe, int lane) {
     int size = 8;
     for (; size > 1; size >>= 1) {
@@ -235,7 +239,8 @@ __device__ __forceinline__ float invert(float* work, Frag& f, float (*v)[4], int
 __device__ __forceinline__ Extent upstream_extent(const WkvBackward* g, int64_t b, int h, int64_t n) {
     return g && g->dy ? steps_extent(static_cast<const char*>(g->dy) + 2 * (b * g->dy_batch_stride + h * N), n, g->dy_step_stride) : Extent(nullptr, 0);
 }
-// Asks for a chunk's vectors: w (in fb's place) ahead of the others, b, k, a and r in the low halves of their tiles, v and dy where one of their forms is themselves.
+// Asks for a chunk's vectors: w (in fb's place) ahead of the others, b, k, a and r in the low halves of their tiles, v and dy where one of their
+// forms is themselves.
 template <class E, bool BWD>
 __device__ __forceinline__ void stage_chunk(const WkvSeq& s, const WkvBackward* bwd, int64_t b, int h, int t0, int lo, int hi, bool with_w, uint32_t at, uint32_t v, uint32_t v16, uint32_t fb,
                                             int lane, int n_steps) {
@@ -250,16 +255,16 @@ __device__ __forceinline__ void stage_chunk(const WkvSeq& s, const WkvBackward* 
     stage_steps(OWN ? v : v16, steps_of(s, 3, b, h, t0, lane), 2 * s.ss[3], lo, hi, true, lane, input_extent(s, 3, b, h, n_steps));
     if (BWD) {
         const bool there = bwd->dy != nullptr;
-        const char* dy = static_cast<const char*>(there ? bwd->dy : s.x[3]) + (there ? 2 * (b * bwd->dy_batch_stride + (int64_t)t0 * bwd->dy_step_stride + h * N + 8 * (lane & 7)) : 0);
+        const int64_t at_dy = there ? b * bwd->dy_batch_stride + (int64_t)t0 * bwd->dy_step_stride + h * N + 8 * (lane & 7) : 0;
+        const char* dy = static_cast<const char*>(there ? bwd->dy : s.x[3]) + 2 * at_dy;
         stage_steps(OWN ? v + TILE : v16 + 2 * TILE, dy, there ? 2 * bwd->dy_step_stride : 0, lo, hi, there, lane, upstream_extent(bwd, b, h, n_steps));
     }
     stage_commit();
 }
 
-// Prepares a chunk (or a piece of one) that is staged and whose factors are in fe and fb. at: the buffer's tiles; v, dy: where those go, in one fp16 each (exact down to 2^-27 of the largest);
-// v16, dy16: in bf16. BWD: dy, Q and the tile of a are kept too.
-// The code is kept short, in loops: a warp runs through it once per chunk, and unrolled (4000 instructions) it waited for them most of the time (a chunk took it 28000
-// cycles).
+// Prepares a chunk (or a piece of one) that is staged and whose factors are in fe and fb. at: the buffer's tiles; v, dy: where those go, in one fp16
+// each (exact down to 2^-27 of the largest); v16, dy16: in bf16. BWD: dy, Q and the tile of a are kept too. The code is kept short, in loops: a warp
+// runs through it once per chunk, and unrolled (4000 instructions) it waited for them most of the time (a chunk took it 28000 cycles).
 template <class E, bool BWD>
 __device__ __forceinline__ void prepare_chunk(uint32_t at, uint32_t v, uint32_t v16, const float* fe, const float* fb, ChunkHead* head, int lane) {
     constexpr int AP = BWD ? T_AP : T_A, VECTORS = BWD ? 6 : 5;
@@ -531,8 +536,8 @@ template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float x
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Accumulators (rows i0 .. as m, steps as n) to out[step][row], 64 channels per step and `stride` values between steps, steps lo .. hi - 1 of the chunk; zeros
-// from step n_on on.
+// Accumulators (rows i0 .. as m, steps as n) to out[step][row], 64 channels per step and `stride` values between steps, steps lo .. hi - 1 of the
+// chunk; zeros from step n_on on.
 template <class E>
 __device__ __forceinline__ void store_steps(const float (*y)[4], E* out, int64_t stride, int i0, int lo, int hi, int n_on, int lane, const Extent& all) {
 #pragma unroll
@@ -567,9 +572,9 @@ __device__ __forceinline__ void store_rows(const float (*S)[4], float* to, int i
         }
 }
 
-// BUFS chunks under way. Four (two blocks per SM) where there are more heads than SMs; eight, which take an SM's shared memory, where there are not: a preparing warp takes
-// 18000 cycles a chunk beside one block's row warps, which take 3800, so that four of them hold these up (1024 steps x 64 heads 163 us, with eight 153; 2 x 4096 x 32
-// with states kept 774 and 669).
+// BUFS chunks under way. Four (two blocks per SM) where there are more heads than SMs; eight, which take an SM's shared memory, where there are not:
+// a preparing warp takes 18000 cycles a chunk beside one block's row warps, which take 3800, so that four of them hold these up (1024 steps x 64
+// heads 163 us, with eight 153; 2 x 4096 x 32 with states kept 774 and 669).
 template <class E, int CHUNK_BUFS>
 __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1) wkv_chunk_fwd_kernel(const __grid_constant__ WkvFwd p) {
     extern __shared__ __align__(128) unsigned char smem[];   // CHUNK_BUFS buffers
@@ -666,9 +671,10 @@ __global__ void __launch_bounds__((CHUNK_BUFS + 4) * 32, CHUNK_BUFS == 4 ? 2 : 1
 }
 
 // ---- the backward pass -----------------------------------------------------------------------------------------------------
-// A block per head goes from the last chunk to the first. Four warps carry 16 rows of the state's gradient each and take the state before each chunk from what the
-// forward pass kept; what they make of a chunk (u, h, and both states, as bf16 pairs) crosses in shared memory to four others, which have 16 columns each and
-// work out the sums over rows: the gradients of r, a, b, k and the decays. Three warps prepare chunks ahead as in the forward pass.
+// A block per head goes from the last chunk to the first. Four warps carry 16 rows of the state's gradient each and take the state before each chunk
+// from what the forward pass kept; what they make of a chunk (u, h, and both states, as bf16 pairs) crosses in shared memory to four others, which
+// have 16 columns each and work out the sums over rows: the gradients of r, a, b, k and the decays. Three warps prepare chunks ahead as in the
+// forward pass.
 constexpr int BWD_BUFS = 3, BWD_WARPS = 8 + BWD_BUFS;
 constexpr int BWD_V = BWD_TILES * 2 * TILE, BWD_DY = BWD_V + TILE, BWD_V16 = BWD_DY + TILE, BWD_DY16 = BWD_V16 + 2 * TILE, BWD_FE = BWD_DY16 + 2 * TILE,
               BWD_FB = BWD_FE + FE_BYTES, BWD_HEAD = BWD_FB + L * N * 4, BWD_BUF = BWD_HEAD + HEAD_BYTES;
@@ -1070,7 +1076,8 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, 1) wkv_chunk_bwd_kernel(const 
                             const float gbs = db[i][e] * ei, gks = dk[i][e] * ei, gbp = pb[i][e] * ei, gkp = pk[i][e] * ei;
                             const float rv = cc ? r.y : r.x, kv = cc ? k.y : k.x, av = cc ? a.y : a.x, bv = cc ? bb.y : bb.x;
                             out[0][cc] = gr, out[2][cc] = gks + gkp, out[3][cc] = ga, out[4][cc] = gbs + gbp;
-                            // (a step's pairs with itself cancel, and a piece has no others: left out, nothing of them is multiplied with a steep log decay)
+                            // (a step's pairs with itself cancel, and a piece has no others: left out, nothing of them is multiplied with a steep log
+                            // decay)
                             pos[cc][half] = piece ? rv * grs : fmaf(rv, gr, -fmaf(bv, gbp, kv * gkp));
                             posa[cc][half] = av * ga;
                             flow[cc][half] = fmaf(bv, gbs, kv * gks);

@@ -203,7 +203,7 @@ int ab_layer_norm_bwd(int dtype, int wtype, int64_t rows, int C, int groups, con
  * in a row that counts is clamped and reported (bit 8 of ab_device_status). */
 typedef struct ab_logit_rows {
     int32_t dtype, vocab;
-    int64_t rows, stride;        /* elements between rows */
+    int64_t rows, stride;        /* elements between rows: vocab or more */
     const void* logits;
     const int64_t* ids;          /* [rows] */
     const uint8_t* mask;         /* [rows] of 0 and 1, or NULL: every row counts */

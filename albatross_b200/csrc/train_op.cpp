@@ -75,6 +75,7 @@ void check_plain(const char* who, const T&... t) {
                 ": cannot be traced or transformed (torch.compile, torch.export, make_fx, torch.func.grad); in a compiled program call it from a function under torch.compiler.disable");
     TORCH_CHECK(!((t.defined() && t._fw_grad(/*level=*/0).defined()) || ...), who, ": forward-mode derivatives are not available");
 }
+// (Backward passes take their saved tensors before they go below autograd: unpacking one may recompute the forward pass, which has to be recorded.)
 // What a backward pass refuses. Gradients are not differentiable: asking for a graph of them is an error, not a silent zero. And in a stream capture
 // a leaf that an earlier graph still ties to the default stream: adding its gradient would make that stream wait for the capturing one, which the
 // default stream cannot, and the capture would be lost with a less telling error.
@@ -143,8 +144,8 @@ struct Wkv7 : torch::autograd::Function<Wkv7> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         check_backward();
-        at::AutoDispatchBelowADInplaceOrView below;
         const variable_list saved = ctx->get_saved_variables();
+        at::AutoDispatchBelowADInplaceOrView below;
         const Tensor* x = saved.data() + 1;
         const c10::cuda::CUDAGuard guard(x[0].device());
         const int64_t B = x[0].size(0), T = x[0].size(1), C = x[0].size(2);
@@ -232,8 +233,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         check_backward();
-        at::AutoDispatchBelowADInplaceOrView below;
         const variable_list saved = ctx->get_saved_variables();
+        at::AutoDispatchBelowADInplaceOrView below;
         const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &stats = saved[3];
         const int64_t groups = ctx->saved_data["groups"].toInt();
         const c10::cuda::CUDAGuard guard(x.device());
@@ -319,8 +320,8 @@ struct TokenLogp : torch::autograd::Function<TokenLogp> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         check_backward();
-        at::AutoDispatchBelowADInplaceOrView below;
         const variable_list s = ctx->get_saved_variables();
+        at::AutoDispatchBelowADInplaceOrView below;
         return {dlogits_of(s[0], s[1], s[2], s[3], grads[0].contiguous(), 1, Tensor()), Tensor(), Tensor()};
     }
 };
@@ -372,8 +373,8 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         check_backward();
-        at::AutoDispatchBelowADInplaceOrView below;
         const variable_list s = ctx->get_saved_variables();
+        at::AutoDispatchBelowADInplaceOrView below;
         return {dlogits_of(s[0], s[1], s[2], s[3], s[4], 1, grads[0].contiguous()), Tensor(), Tensor(), Tensor()};
     }
 };
@@ -437,8 +438,8 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         check_backward();
-        at::AutoDispatchBelowADInplaceOrView below;
         const variable_list s = ctx->get_saved_variables();
+        at::AutoDispatchBelowADInplaceOrView below;
         variable_list out(6);
         out[0] = dlogits_of(s[0], s[1], s[2], s[3], s[4], std::max<int64_t>(1, s[1].size(1)), grads[0].contiguous());
         return out;

@@ -1173,6 +1173,36 @@ def test_capture_of_some_gradients_beside_a_living_graph_of_another_leaf():
     assert w.grad is not None and b.grad is not None
 
 
+def test_under_checkpointing_saved_tensors_on_the_host_and_inference_mode():
+    """What programs put around operators: recomputation, saved tensors that come back as other tensors, no autograd at all."""
+    from torch.utils.checkpoint import checkpoint
+    state, xs, dy, dout = wkv_inputs(2, 35, 2, "bf16", seed=33)
+    packed = torch.cat(xs, -1)
+    x, w, b = norm_inputs(40, 2304, "bf16")
+    lg, ids, _ = logit_inputs(24, 3003, "bf16")
+    A = torch.randn(24, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    calls = ((lambda s, p: sum((t.float() * g.float()).sum() for t, g in zip(ab.RWKV7_TRAIN_OP(s, *p.split(128, -1)), (dy, dout))), (state, packed)),
+             (lambda x, w, b: ab.layer_norm(x[:, 256:1280], w, b).float().square().sum(), (x, w[:1024].clone(), b[:1024].clone())),
+             (lambda t: ab.token_logp(t[:, 3:2003], ids % 2000).square().sum(), (lg,)),
+             (lambda t: ab.policy_loss(t.view(2, 12, 3003)[:, :-1], ids.view(2, 12)[:, 1:], None, A.view(2, 12)[:, 1:])[0], (lg,)),
+             (lambda t: ab.preference_loss(t.view(2, 12, 3003), ids.view(2, 12), A[:2])[0], (lg,)))
+    for f, args in calls:
+        def grads(run):
+            leaves = [t.detach().clone().requires_grad_() for t in args]
+            out = run(leaves)
+            return (out.detach(),) + torch.autograd.grad(out, leaves)
+        want = grads(lambda leaves: f(*leaves))
+        again = grads(lambda leaves: checkpoint(f, *leaves, use_reentrant=False))
+        with torch.autograd.graph.save_on_cpu():
+            host = grads(lambda leaves: f(*leaves))
+        assert all(torch.equal(p, q) for p, q in zip(again, want)) and all(torch.equal(p, q) for p, q in zip(host, want))
+        with torch.inference_mode():
+            assert torch.equal(f(*[t.clone() for t in args]), want[0])
+    with torch.inference_mode():
+        here = lg.clone()
+        assert torch.equal(ab.policy_loss_grad(here, ids, None, A, out=here)[2], ab.policy_loss_grad(lg, ids, None, A)[2])
+
+
 def test_two_streams_at_once():
     """Calls that overlap share nothing."""
     p, ids, mask, A = small_problem()

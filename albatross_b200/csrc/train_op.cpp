@@ -79,8 +79,8 @@ void check_plain(const char* who, const T&... t) {
 // What a backward pass refuses. Gradients are not differentiable: asking for a graph of them is an error, not a silent zero. And in a stream capture
 // a leaf that an earlier graph still ties to the default stream: adding its gradient would make that stream wait for the capturing one, which the
 // default stream cannot, and the capture would be lost with a less telling error.
-void check_backward() {
-    check_plain("albatross_b200: gradients");
+void check_backward(const variable_list& grads) {
+    for (const Tensor& g : grads) check_plain("albatross_b200: gradients", g);
     TORCH_CHECK(!at::GradMode::is_enabled(), "albatross_b200: the gradients of these operators cannot be differentiated again (create_graph)");
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
     const auto node = torch::autograd::get_current_node();
@@ -143,7 +143,7 @@ struct Wkv7 : torch::autograd::Function<Wkv7> {
         return {y, out};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        check_backward();
+        check_backward(grads);
         const variable_list saved = ctx->get_saved_variables();
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor* x = saved.data() + 1;
@@ -232,7 +232,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        check_backward();
+        check_backward(grads);
         const variable_list saved = ctx->get_saved_variables();
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &stats = saved[3];
@@ -319,7 +319,7 @@ struct TokenLogp : torch::autograd::Function<TokenLogp> {
         return logp;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        check_backward();
+        check_backward(grads);
         const variable_list s = ctx->get_saved_variables();
         at::AutoDispatchBelowADInplaceOrView below;
         return {dlogits_of(s[0], s[1], s[2], s[3], grads[0].contiguous(), 1, Tensor()), Tensor(), Tensor()};
@@ -372,7 +372,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         return {loss, logp};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        check_backward();
+        check_backward(grads);
         const variable_list s = ctx->get_saved_variables();
         at::AutoDispatchBelowADInplaceOrView below;
         return {dlogits_of(s[0], s[1], s[2], s[3], s[4], 1, grads[0].contiguous()), Tensor(), Tensor(), Tensor()};
@@ -437,7 +437,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
         return {loss, logp};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        check_backward();
+        check_backward(grads);
         const variable_list s = ctx->get_saved_variables();
         at::AutoDispatchBelowADInplaceOrView below;
         variable_list out(6);

@@ -1126,6 +1126,19 @@ def test_gradients_are_not_written_over_a_leaf_that_wants_one():
     assert torch.equal(ab.policy_loss_grad(z, ids, None, A, out=z)[2], want[2])
 
 
+def test_batched_upstream_gradients_are_refused():
+    """torch.autograd.grad(is_grads_batched=True) hands wrappers without memory to the backward passes."""
+    x, w, b = (t.requires_grad_() for t in norm_inputs(4, 256, "fp32"))
+    lg, ids, _ = logit_inputs(4, 300, "fp32")
+    lg.requires_grad_()
+    state, xs, _, _ = wkv_inputs(1, 5, 1, "fp16")
+    state.requires_grad_()
+    for y, leaf in ((ab.layer_norm(x, w, b), x), (ab.token_logp(lg, ids), lg), (ab.policy_loss(lg, ids, None, lg.detach()[:, 0])[0], lg), (ab.RWKV7_TRAIN_OP(state, *xs)[1], state)):
+        with pytest.raises(RuntimeError, match="cannot be traced or transformed"):
+            torch.autograd.grad(y, leaf, torch.ones(2, *y.shape, device="cuda"), is_grads_batched=True, retain_graph=True)
+        assert torch.autograd.grad(y, leaf, torch.ones_like(y))[0].shape == leaf.shape
+
+
 def test_capture_beside_a_living_graph_of_the_same_leaf_is_refused():
     """On the default stream such a graph ties the leaf to that stream, which cannot join a capture; nothing of the process is lost, and without that graph the capture is taken."""
     x = torch.randn(4, 256, device="cuda", requires_grad=True)

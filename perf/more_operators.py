@@ -166,7 +166,7 @@ def prepare(case, seed):
 # plain forms
 # ------------------------------------------------------------------------------------------------------------------
 def _plain_sample(s):
-    """In 64 bits: which token is kept, and which is drawn, is decided next to borders."""
+    """In 64 bits: which token is kept, and which is drawn, is decided next to borders. The likelier token comes first, of equals that of the lower id."""
     x, u = s["logits"], s["u"].double()[:, None]
     T, k, p, m = (s[n].double()[:, None] if torch.is_tensor(s[n]) else torch.full_like(u, s[n]) for n in "Tkpm")
     values, index = torch.sort(x, dim=-1, descending=True, stable=True)      # equals keep their order
@@ -179,10 +179,10 @@ def _plain_sample(s):
     keep &= (before < p * e.sum(-1, keepdim=True)) | (p >= 1)
     keep &= e >= m
     keep[:, 0] = True
-    weights = torch.zeros_like(e).scatter_(1, index, e * keep)
-    cum = torch.cumsum(weights, -1)
-    ids = (cum <= u * cum[:, -1:]).sum(-1, keepdim=True)
-    return {"ids": ids, "logp": torch.log(weights.gather(1, ids) / cum[:, -1:]).float()}
+    e = e * keep
+    cum = torch.cumsum(e, -1)
+    at = (cum <= u * cum[:, -1:]).sum(-1, keepdim=True)
+    return {"ids": index.gather(1, at), "logp": torch.log(e.gather(1, at) / cum[:, -1:]).float()}
 
 
 def _plain_int4(s):
@@ -258,7 +258,7 @@ def _exact_sample(s):
         if p < 1:
             cum = np.cumsum(w[order])
             order = order[:1 + int(np.count_nonzero(cum[:-1] < p * cum[-1]))]
-        kept = np.sort(np.concatenate([order[:1], order[1:][w[order[1:]] >= m]]))
+        kept = np.concatenate([order[:1], order[1:][w[order[1:]] >= m]])
         cum = np.cumsum(w[kept])
         i = kept[np.searchsorted(cum, u * cum[-1], side="right")]
         ids.append(int(i))

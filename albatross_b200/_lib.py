@@ -62,6 +62,20 @@ class Policy(C.Structure):
                 ("clip_low", C.c_float), ("clip_high", C.c_float), ("kl", C.c_float), ("denom", C.c_float)]
 
 
+class Grad(C.Structure):
+    _fields_ = [("g", C.c_void_p), ("out", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32), ("out_dtype", C.c_int32)]
+
+
+class Int4(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("n_out", C.c_int32), ("k", C.c_int32), ("group", C.c_int32), ("w", C.c_void_p), ("scale", C.c_void_p),
+                ("zero", C.c_void_p)]
+
+
+class Sampling(C.Structure):
+    _fields_ = [("temperature", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("top_k", C.c_void_p), ("temperature_all", C.c_double),
+                ("top_p_all", C.c_double), ("min_p_all", C.c_double), ("top_k_all", C.c_int32), ("_pad", C.c_int32)]
+
+
 class LibraryError(RuntimeError):
     pass
 
@@ -120,6 +134,11 @@ def _load():
     lib.ab_policy_loss_fwd.argtypes = [rows, policy, vp, vp, vp, vp, vp, vp]
     lib.ab_policy_loss_grad.argtypes = [rows, policy, f32, vp, vp, vp, vp, vp]
     lib.ab_preference_loss_fwd.argtypes = [rows, i64, i64, vp, f32, f32, vp, vp, vp, vp, vp, vp]
+    lib.ab_clip_grad_norm_scratch_bytes.argtypes = [i64]
+    lib.ab_clip_grad_norm_scratch_bytes.restype = sz
+    lib.ab_clip_grad_norm.argtypes = [C.POINTER(Grad), i64, C.c_double, C.c_double, vp, vp, vp]
+    lib.ab_linear_int4.argtypes = [C.POINTER(Int4), i32, vp, i64, vp, vp]
+    lib.ab_sample_filtered.argtypes = [i32, i64, i32, vp, i64, vp, C.POINTER(Sampling), vp, vp, vp]
     return lib
 
 
@@ -129,7 +148,8 @@ EXPORTS = ["ab_last_error", "ab_version", "ab_device_status", "ab_wkv7_fwd", "ab
            "ab_gemm", "ab_gemm_static", "ab_gemm_static_reset", "ab_gemm_static_debug_counter", "ab_sample_rows", "ab_sample_rows_i64", "ab_gemv_plan_selftest", "ab_gemm_plan_selftest", "ab_dequant", "ab_model_create", "ab_model_destroy", "ab_workspace_bytes", "ab_forward", "ab_forward_stage",
            "ab_model_set_option", "ab_decode_program_bytes", "ab_decode_timeline_offset", "ab_decode_program_build", "ab_decode_run", "ab_decode_plan_selftest", "ab_glue_selftest",
            "ab_wkv7_checkpoint_bytes", "ab_wkv7_seq_fwd", "ab_wkv7_seq_bwd", "ab_layer_norm_fwd", "ab_layer_norm_scratch_bytes", "ab_layer_norm_bwd",
-           "ab_token_logp_fwd", "ab_token_logp_bwd", "ab_policy_loss_fwd", "ab_policy_loss_grad", "ab_preference_loss_fwd"]
+           "ab_token_logp_fwd", "ab_token_logp_bwd", "ab_policy_loss_fwd", "ab_policy_loss_grad", "ab_preference_loss_fwd",
+           "ab_clip_grad_norm_scratch_bytes", "ab_clip_grad_norm", "ab_linear_int4", "ab_sample_filtered"]
 
 
 def check(status: int, what: str = "") -> None:

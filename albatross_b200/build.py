@@ -3,7 +3,8 @@
     python -m albatross_b200.build [--force] [--verbose]
 
 Output: albatross_b200/_C/libalbatross_b200.so (git-ignored; it ships with the source tree) and, next to it,
-librwkv7_state_fwd_fp16.so and libalbatross_b200_train.so: the torch operator shims (g++, csrc/torch_op.cpp, csrc/train_op.cpp).
+librwkv7_state_fwd_fp16.so, libalbatross_b200_train.so and libalbatross_b200_serve.so: the torch operator shims (g++, csrc/torch_op.cpp,
+csrc/train_op.cpp, csrc/serve_op.cpp).
 """
 from __future__ import annotations
 
@@ -61,6 +62,7 @@ def build(force: bool = False, verbose: bool = False, bounds_check: bool = False
 
 TORCH_OP_LIB = os.path.join(OUT_DIR, "librwkv7_state_fwd_fp16.so")
 TRAIN_OP_LIB = os.path.join(OUT_DIR, "libalbatross_b200_train.so")
+SERVE_OP_LIB = os.path.join(OUT_DIR, "libalbatross_b200_serve.so")
 
 
 def _build_shim(src: str, out: str, newest: float, force: bool, links: list) -> str:
@@ -90,10 +92,20 @@ def build_torch_op(force: bool = False) -> str:
     return _build_shim(os.path.join(CSRC, "torch_op.cpp"), TORCH_OP_LIB, os.path.getmtime(LIB), force, ["-lalbatross_b200"])
 
 
+def _interface() -> float:
+    """When what the shims share with the kernel library last changed: they take its entries at run time, and follow its header alone."""
+    return max(os.path.getmtime(p) for p in (os.path.join(HERE, "..", "include", "albatross_b200.h"), os.path.join(CSRC, "op.h")))
+
+
 def build_train_op(force: bool = False) -> str:
     """Builds csrc/train_op.cpp the same way: `torch.ops.albatross_b200.*`, the operators with gradients. It takes the kernel library's
-    entries at run time (train.py says from which build of it), so that it follows the header alone."""
-    return _build_shim(os.path.join(CSRC, "train_op.cpp"), TRAIN_OP_LIB, os.path.getmtime(os.path.join(HERE, "..", "include", "albatross_b200.h")), force, ["-ldl"])
+    entries at run time (_shim.py says from which build of it)."""
+    return _build_shim(os.path.join(CSRC, "train_op.cpp"), TRAIN_OP_LIB, _interface(), force, ["-ldl"])
+
+
+def build_serve_op(force: bool = False) -> str:
+    """Builds csrc/serve_op.cpp the same way: the operators of serve.py."""
+    return _build_shim(os.path.join(CSRC, "serve_op.cpp"), SERVE_OP_LIB, _interface(), force, ["-ldl"])
 
 
 def resource_usage(log_path: str = os.path.join(OUT_DIR, "build.log")) -> dict:
@@ -130,3 +142,4 @@ if __name__ == "__main__":
         print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv, bounds_check=True))
     print(build_torch_op(force="--force" in sys.argv))
     print(build_train_op(force="--force" in sys.argv))
+    print(build_serve_op(force="--force" in sys.argv))

@@ -1,0 +1,473 @@
+// One id per row of logits, drawn under a temperature, top-k, top-p and min-p from a given uniform number.
+//
+//   w_i = exp((l_i - max l) / T);  the values in order: larger ones first, equals by index.  Kept is the longest front part of that order in which
+//   each value but the first has   rank < k,   sum of the w in front of it < p * (sum of w over the first k),   w >= m.
+//   The id is the first one whose sum of w up to and with it exceeds u * (sum of w that is kept).
+//
+// All three filters keep a front part of one and the same order, and so does the draw: each is a question "where in that order do the weights (or the
+// ranks) reach X?". Nothing is sorted for that. Weights are taken as multiples of 2^-44 (the largest is 2^44 of them), so that sums are whole numbers, which
+// do not depend on the order of additions: a histogram over 4096 bins of max - l, made by atomics on shared memory, has exact sums, and its running sums answer every
+// question down to a bin. The few values of that bin are gathered and compared with each other. Where a bin holds more than SP_LIST
+// values (ties of 16-bit logits), its keys' range is divided again.
+//
+// Precision: weights come from a table and a polynomial in 64 bits (off by 1e-15) and are rounded to 2^-45 of the largest one. What comes out is the id that
+// the definition in 64 bits gives, unless u or p meets a border within some 1e-9 of the sum.
+#include <cooperative_groups.h>
+
+#include "train.cuh"
+
+namespace ab {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int SP_BINS = 4096, SP_SUB = 1024;   // bins of the first histogram, and of a division of one of its bins
+constexpr int SP_LIST = 256;                   // values that are compared with each other
+constexpr int SP_MAX_BLOCKS = 8;               // of a cluster: a row's at most
+constexpr int SP_ROW_BYTES = 129 * 1024;       // of a row in a block's shared memory, at most
+constexpr uint64_t SP_ONE = 1ull << 44;        // a weight of 1
+
+struct SampleArgs {
+    const void* logits;
+    const float *u, *T, *p, *m;   // T, p, m: null, or one per row
+    const int32_t* k;
+    double T_all, p_all, m_all;
+    int32_t k_all, V;
+    int64_t rows, stride;
+    int64_t* ids;
+    float* logp;
+    int32_t share;                // 16-byte pieces of a row that a block takes
+};
+
+__device__ __forceinline__ uint32_t key_of(float v) {   // larger values, larger keys; -0 is 0
+    const uint32_t b = __float_as_uint(v + 0.f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+
+struct RowScale {
+    float top;          // the row's largest value
+    float bins;         // bins per unit of top - l
+    double c;           // log2(e) / T
+    const double* tab;  // 2^(j / 16), j = 0 .. 15
+};
+__device__ __forceinline__ int bin_of(const RowScale& r, float v) {   // never falls as v does; rounding and all
+    const float d = v == r.top ? 0.f : r.top - v;
+    return min(SP_BINS - 1, __float2int_rz(d * r.bins));   // (a NaN, 0 bins per unit times infinity, gives bin 0)
+}
+// exp((v - top) / T): 2^z with z = n / 16 + f, |f| <= 1 / 32, and the series of exp(f ln 2) to the sixth power (what is left is below 5e-16)
+__device__ __forceinline__ double weight(const RowScale& r, float v) {
+    if (v == r.top) return 1.0;
+    const double z = ((double)v - (double)r.top) * r.c;
+    if (!(z > -46.0)) return 0.0;
+    constexpr double ROUND = 6755399441055744.0;   // 1.5 * 2^52
+    const double b = fma(z, 16.0, ROUND);
+    const int n = (int)(uint32_t)__double_as_longlong(b);
+    const double x = fma(b - ROUND, -0.0625, z) * 0.693147180559945309417;
+    double q = fma(x, 1.0 / 720.0, 1.0 / 120.0);
+    q = fma(q, x, 1.0 / 24.0);
+    q = fma(q, x, 1.0 / 6.0);
+    q = fma(q, x, 0.5);
+    q = fma(q, x, 1.0);
+    q = fma(q, x, 1.0) * r.tab[n & 15];
+    return __longlong_as_double(__double_as_longlong(q) + ((long long)(n >> 4) << 52));
+}
+__device__ __forceinline__ uint64_t whole_weight(double w) {   // in units of 2^-44: those are the last places of numbers from 256 to 512
+    return (uint64_t)(__double_as_longlong(w + 384.0) - __double_as_longlong(384.0));
+}
+
+struct Found {
+    uint32_t key;
+    uint32_t equals;      // values of that key
+    uint64_t before;      // sum in front of the first of them
+};
+
+template <int NT>
+struct alignas(16) SampleShared {
+    uint64_t cum[SP_BINS], sub[SP_SUB];
+    uint32_t part[3][SP_BINS];   // sums of a weight's lowest 15 bits, the next 15, and the rest
+    uint32_t list[SP_LIST], own[SP_LIST];
+    double tab[16];
+    uint64_t red[NT / 32], mine;
+    uint32_t least, most, n, matches[NT / 32], matched;
+    Found found;
+};
+
+template <class E, int NT>
+struct Sampler {
+    static constexpr int PER = 16 / sizeof(E), WARPS = NT / 32;
+    SampleShared<NT>& s;
+    const uint4* row;      // this block's pieces, in shared memory
+    int pieces, per_warp;  // of this block; of a warp: whole rounds of 32
+    cg::cluster_group cluster;
+    int blocks, rank;
+    RowScale r;
+    int lane, warp;
+
+    __device__ __forceinline__ void join() {   // all blocks of the row
+        if (blocks > 1) cluster.sync();
+        else __syncthreads();
+    }
+    template <class T>
+    __device__ __forceinline__ T* of(T* p, int other) { return blocks > 1 ? cluster.map_shared_rank(p, other) : p; }
+
+    // f(value, piece of the warp's round) for every value of the block
+    template <class F>
+    __device__ __forceinline__ void each(F f) {
+        const int end = min(pieces, (warp + 1) * per_warp);
+        for (int c = warp * per_warp + lane; c < end; c += 32) {
+            float v[PER];
+            unpack<E>(row[c], v);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) f(v[i]);
+        }
+    }
+    template <class Op>
+    __device__ __forceinline__ uint64_t reduce(uint64_t v, Op op) {   // over all threads of all blocks
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v = op(v, (uint64_t)__shfl_xor_sync(0xffffffffu, v, o));
+        if (lane == 0) s.red[warp] = v;
+        __syncthreads();
+        v = s.red[lane % WARPS];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const uint64_t w = __shfl_xor_sync(0xffffffffu, v, o);
+            if (o < WARPS) v = op(v, w);
+        }
+        if (blocks > 1) {
+            if (threadIdx.x == 0) s.mine = v;
+            cluster.sync();
+            for (int b = 1; b < blocks; ++b) v = op(v, *of(&s.mine, (rank + b) % blocks));
+            cluster.sync();
+        } else {
+            __syncthreads();
+        }
+        return v;
+    }
+    __device__ __forceinline__ void clear(int bins) {
+        for (int i = threadIdx.x; i < bins; i += NT) s.part[0][i] = s.part[1][i] = s.part[2][i] = 0;
+        __syncthreads();
+    }
+    template <bool COUNT>
+    __device__ __forceinline__ void add(int bin, float v) {
+        if (COUNT) {
+            atomicAdd(&s.part[0][bin], 1u);
+            return;
+        }
+        const uint64_t w = whole_weight(weight(r, v));
+        if (w == 0) return;
+        atomicAdd(&s.part[0][bin], (uint32_t)w & 0x7fffu);
+        atomicAdd(&s.part[1][bin], (uint32_t)(w >> 15) & 0x7fffu);
+        atomicAdd(&s.part[2][bin], (uint32_t)(w >> 30));
+    }
+    // running sums of the histogram, over all blocks; every block has them
+    template <int BINS>
+    __device__ __forceinline__ void run_up(uint64_t* cum) {
+        constexpr int EACH = (BINS + NT - 1) / NT;
+        join();
+        uint64_t v[EACH], sum = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int bin = threadIdx.x * EACH + i;
+            for (int b = 0; b < blocks; ++b)
+                if (bin < BINS) sum += (uint64_t)*of(&s.part[0][bin], b) + ((uint64_t)*of(&s.part[1][bin], b) << 15) + ((uint64_t)*of(&s.part[2][bin], b) << 30);
+            v[i] = sum;
+        }
+        uint64_t up = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t w = __shfl_up_sync(0xffffffffu, up, o);
+            if (lane >= o) up += w;
+        }
+        if (lane == 31) s.red[warp] = up;
+        __syncthreads();
+        uint64_t base = up - sum;
+        for (int i = 0; i < warp; ++i) base += s.red[i];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (threadIdx.x * EACH + i < BINS) cum[threadIdx.x * EACH + i] = base + v[i];
+        join();
+    }
+    template <int BINS>
+    static __device__ __forceinline__ int search(const uint64_t* cum, uint64_t X) {   // the first bin that reaches X
+        int lo = 0, hi = BINS - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (cum[mid] >= X) hi = mid;
+            else lo = mid + 1;
+        }
+        return lo;
+    }
+
+    // Where the running sum over the keys above `floor_` reaches X (1 <= X <= their sum, which s.cum has): weights, or ranks (COUNT).
+    template <bool COUNT>
+    __device__ Found locate(uint64_t X, uint32_t floor_) {
+        const int bin = search<SP_BINS>(s.cum, X);
+        Found out = {0, 0, bin ? s.cum[bin - 1] : 0};
+        uint32_t lo = 0, hi = 0xffffffffu;
+        for (int level = 0;; ++level) {
+            auto inside = [&](float v, uint32_t key) { return key > floor_ && (level ? key >= lo && key <= hi : bin_of(r, v) == bin); };
+            if (threadIdx.x == 0) s.n = 0, s.least = 0xffffffffu, s.most = 0;
+            __syncthreads();
+            each([&](float v) {
+                const uint32_t key = key_of(v);
+                if (!inside(v, key)) return;
+                const uint32_t at = atomicAdd(&s.n, 1u);
+                if (at < SP_LIST) s.own[at] = key;
+                atomicMin(&s.least, key);
+                atomicMax(&s.most, key);
+            });
+            join();
+            uint32_t n = 0;
+            lo = 0xffffffffu, hi = 0;
+            for (int b = 0; b < blocks; ++b) {
+                const uint32_t have = *of(&s.n, b);
+                if (n + have <= SP_LIST)
+                    for (uint32_t i = threadIdx.x; i < have; i += NT) s.list[n + i] = *of(&s.own[0] + i, b);
+                n += have;
+                lo = min(lo, *of(&s.least, b)), hi = max(hi, *of(&s.most, b));
+            }
+            join();
+            out.key = lo, out.equals = n;
+            if (lo >= hi || level > 5) return out;   // (four divisions take 32 bits apart)
+            if (n <= SP_LIST) break;
+            // the keys between in 1024 parts
+            const int shift = max(0, 32 - __clz(hi - lo) - 10);
+            clear(SP_SUB);
+            each([&](float v) {
+                const uint32_t key = key_of(v);
+                if (key > floor_ && key >= lo && key <= hi) add<COUNT>((int)((hi - key) >> shift), v);
+            });
+            run_up<SP_SUB>(s.sub);
+            const int part = search<SP_SUB>(s.sub, X - out.before);
+            if (part) out.before += s.sub[part - 1];
+            const uint32_t top = hi - ((uint32_t)part << shift);
+            if (top - lo >= 1u << shift) lo = top - ((1u << shift) - 1);
+            hi = top;
+        }
+        const uint32_t i = threadIdx.x, n = out.equals;
+        if (i < n) s.sub[i] = COUNT ? 1 : whole_weight(weight(r, value_of(s.list[i])));
+        __syncthreads();
+        if (i < n) {
+            const uint32_t key = s.list[i];
+            uint64_t before = out.before;
+            uint32_t equals = 0;
+            for (uint32_t j = 0; j < n; ++j) {
+                const uint32_t other = s.list[j];
+                if (other > key) before += s.sub[j];
+                equals += other == key;
+            }
+            if (before < X && X <= before + equals * s.sub[i]) s.found = Found{key, equals, before};
+        }
+        __syncthreads();
+        out = s.found;
+        __syncthreads();
+        return out;
+    }
+};
+
+template <class E, int NT>
+__global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a) {
+    extern __shared__ __align__(16) unsigned char sample_smem[];
+    SampleShared<NT>& s = *reinterpret_cast<SampleShared<NT>*>(sample_smem);
+    unsigned char* row_bytes = sample_smem + sizeof(SampleShared<NT>);
+    constexpr int PER = 16 / sizeof(E);
+    Sampler<E, NT> x = {s, reinterpret_cast<const uint4*>(row_bytes), 0, 0, cg::this_cluster()};
+    x.blocks = (int)x.cluster.num_blocks(), x.rank = (int)x.cluster.block_rank();
+    x.lane = threadIdx.x & 31, x.warp = threadIdx.x >> 5;
+    const int64_t row = blockIdx.x / x.blocks;
+    const E* logits = static_cast<const E*>(a.logits) + row * a.stride;
+    const Extent all = rows_extent(a.logits, a.rows, a.stride, a.V, sizeof(E));
+    // the row from its last 16-byte boundary on: the first `skip` values of the first piece are not its own
+    const int skip = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(E)), all_pieces = (skip + a.V + PER - 1) / PER;
+    const int first = x.rank * a.share;
+    x.pieces = max(0, min(a.share, all_pieces - first));
+    x.per_warp = (x.pieces + NT - 1) / NT * 32;
+    if (threadIdx.x < 16) s.tab[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
+    float top = -INFINITY, low = INFINITY;
+    bool nan = false;
+    {
+        uint4* to = reinterpret_cast<uint4*>(row_bytes);
+        const int end = min(x.pieces, (x.warp + 1) * x.per_warp);
+        for (int c = x.warp * x.per_warp + x.lane; c < end; c += 32) {
+            const int at = (first + c) * PER - skip;   // of the row
+            uint4 q;
+            float v[PER];
+            if (at >= 0 && at + PER <= a.V) {
+                q = make_uint4(0, 0, 0, 0);
+                if (all.holds(logits + at, PER)) q = __ldcs(reinterpret_cast<const uint4*>(logits + at));
+                unpack<E>(q, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) v[i] = at + i >= 0 && at + i < a.V && all.holds(logits + at + i) ? to_f(logits[at + i]) : -INFINITY;
+                q = pack<E>(v);
+            }
+            to[c] = q;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                nan |= v[i] != v[i];
+                top = fmaxf(top, v[i]);
+                if (v[i] > -INFINITY) low = fminf(low, v[i]);
+            }
+        }
+    }
+    auto larger = [](uint64_t p, uint64_t q) { return p > q ? p : q; };
+    auto sum = [](uint64_t p, uint64_t q) { return p + q; };
+    // (both in one: the key of the largest value above, the inverted key of the smallest below it; a NaN on top of all)
+    const uint64_t high = x.reduce(nan ? ~0ull : (uint64_t)key_of(top), larger);
+    low = value_of(~(uint32_t)x.reduce((uint64_t)~key_of(low), larger));
+    const double T = a.T ? (double)a.T[row] : a.T_all, p = a.p ? (double)a.p[row] : a.p_all, m = a.m ? (double)a.m[row] : a.m_all;
+    const int k = a.k ? a.k[row] : a.k_all;
+    top = value_of((uint32_t)high);
+    if (high == ~0ull || top == -INFINITY) {   // a NaN, or nothing to draw
+        if (x.rank == 0 && threadIdx.x == 0) a.ids[row] = -1, a.logp[row] = NAN;
+        if (x.blocks > 1) x.cluster.sync();
+        return;
+    }
+    uint32_t key = (uint32_t)high;
+    uint64_t ordinal = 0;
+    double logp = 0.0;
+    if (T > 0.0 && k != 1 && a.V > 1) {
+        const float range = (float)fmin(32.0 * T, (double)top - (double)low);
+        x.r = {top, range > 0.f ? SP_BINS / range : 0.f, 1.4426950408889634074 / T, s.tab};
+        uint32_t floor_ = 0;       // keys above this one count (0 is no value's)
+        uint64_t ties = 0, tied = 0;
+        if (k > 0 && k < a.V) {
+            x.clear(SP_BINS);
+            x.each([&](float v) { x.template add<true>(bin_of(x.r, v), v); });
+            x.template run_up<SP_BINS>(s.cum);
+            const Found f = x.template locate<true>((uint64_t)k, 0);
+            floor_ = f.key;
+            ties = (uint64_t)k - f.before;
+            tied = whole_weight(weight(x.r, value_of(floor_)));
+        }
+        x.clear(SP_BINS);
+        x.each([&](float v) {
+            if (key_of(v) > floor_) x.template add<false>(bin_of(x.r, v), v);
+        });
+        x.template run_up<SP_BINS>(s.cum);
+        const uint64_t above = s.cum[SP_BINS - 1];
+        uint64_t kept = above + ties * tied;
+        uint32_t last = floor_;    // key of the last value that is kept, where a filter has set one
+        // the front part that reaches X ends at ...
+        auto reach = [&](uint64_t X, uint64_t& before, uint64_t& w) {
+            if (X > above) {
+                before = above, w = tied;
+                return floor_;
+            }
+            const Found f = x.template locate<false>(X, floor_);
+            before = f.before, w = whole_weight(weight(x.r, value_of(f.key)));
+            return f.key;
+        };
+        if (p < 1.0) {
+            const uint64_t X = min(kept, (uint64_t)fmax(1.0, ceil(p * (double)kept)));
+            uint64_t before, w;
+            last = reach(X, before, w);
+            kept = before + (X - before + w - 1) / w * w;
+        }
+        if (m > 0.0 && !(last != 0 && weight(x.r, value_of(last)) >= m)) {
+            const double far = 1e-6 - log2(m);   // (a little too far)
+            uint64_t mine = 0;
+            x.each([&](float v) {
+                if (key_of(v) <= floor_ || !(v == top || ((double)top - (double)v) * x.r.c <= far)) return;
+                const double w = weight(x.r, v);
+                if (w >= m) mine += whole_weight(w);
+            });
+            kept = max(SP_ONE, min(kept, x.reduce(mine, sum)));
+        }
+        const double u = fmin(fmax((double)a.u[row], 0.0), 1.0);
+        const uint64_t X = min(kept, (uint64_t)floor(u * (double)kept) + 1);
+        uint64_t before, w;
+        key = reach(X, before, w);
+        ordinal = (X - before + w - 1) / w - 1;
+        logp = -log((double)kept * (1.0 / SP_ONE));
+        if (value_of(key) != top) logp += ((double)value_of(key) - (double)top) / T;
+    }
+    // the value of that key with `ordinal` of them in front of it
+    uint32_t matches = 0;
+    x.each([&](float v) { matches += key_of(v) == key; });
+    matches = __reduce_add_sync(0xffffffffu, matches);
+    if (x.lane == 0) s.matches[x.warp] = matches;
+    __syncthreads();
+    uint32_t before = 0, in_block = 0;
+    for (int i = 0; i < NT / 32; ++i) {
+        if (i < x.warp) before += s.matches[i];
+        in_block += s.matches[i];
+    }
+    if (x.blocks > 1) {
+        if (threadIdx.x == 0) s.matched = in_block;
+        x.cluster.sync();
+        for (int b = 0; b < x.rank; ++b) before += *x.of(&s.matched, b);
+        x.cluster.sync();
+    }
+    if (ordinal < before || ordinal >= (uint64_t)before + matches) return;
+    const int end = min(x.pieces, (x.warp + 1) * x.per_warp);
+    for (int c0 = x.warp * x.per_warp; c0 < end; c0 += 32) {
+        const int c = c0 + x.lane;
+        uint32_t mask = 0;
+        if (c < end) {
+            float v[PER];
+            unpack<E>(x.row[c], v);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) mask |= (uint32_t)(key_of(v[i]) == key) << i;
+        }
+        const uint32_t n = __popc(mask);
+        uint32_t up = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t w = __shfl_up_sync(0xffffffffu, up, o);
+            if (x.lane >= o) up += w;
+        }
+        const uint32_t from = before + up - n;
+        if (ordinal >= from && ordinal < from + n) {
+            for (uint32_t i = from; i < ordinal; ++i) mask &= mask - 1;
+            a.ids[row] = (int64_t)(first + c) * PER - skip + __ffs(mask) - 1;
+            a.logp[row] = (float)logp;
+        }
+        before += __shfl_sync(0xffffffffu, up, 31);
+    }
+}
+
+template <class E>
+int sample_launch(SampleArgs a, cudaStream_t st) {
+    constexpr int PER = 16 / sizeof(E), NT = 1024;
+    static PerDeviceOnce once;
+    const DeviceProps* dev;
+    const auto kernel = sample_filtered_kernel<E, NT>;
+    const int head = (int)sizeof(SampleShared<NT>);
+    const int err = once.run(&dev, [&](const DeviceProps& d) -> int {
+        AB_CHECK_ARG(d.smem_optin >= (size_t)head + SP_ROW_BYTES, "sampling: %zu bytes of shared memory per block are too few", d.smem_optin);
+        return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, head + SP_ROW_BYTES), "cudaFuncSetAttribute(sampling)");
+    });
+    if (err != OK) return err;
+    const int pieces = (a.V + 2 * PER - 2) / PER;   // wherever the row starts
+    int blocks = 1;
+    while ((pieces + blocks - 1) / blocks * 16 > SP_ROW_BYTES) blocks *= 2;
+    AB_CHECK_ARG(blocks <= SP_MAX_BLOCKS, "sampling: a vocabulary of %d is too large", a.V);
+    while (blocks < SP_MAX_BLOCKS && a.rows * blocks * 2 <= dev->n_sm && pieces > 1024 * blocks) blocks *= 2;
+    AB_CHECK_ARG(a.rows <= INT32_MAX / blocks, "sampling: too many rows");
+    a.share = (pieces + blocks - 1) / blocks;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.rows * blocks));
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = (size_t)head + (size_t)a.share * 16;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = blocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    AB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+    return OK;
+}
+
+}  // namespace
+
+int sample_filtered(int dtype, int64_t rows, int V, const void* logits, int64_t stride, const float* u, const ab_sampling& p, int64_t* ids, float* logp, cudaStream_t st) {
+    const SampleArgs a = {logits, u, p.temperature, p.top_p, p.min_p, p.top_k, p.temperature_all, p.top_p_all, p.min_p_all, p.top_k_all, V, rows, stride, ids, logp, 0};
+    return dtype == AB_DT_F16 ? sample_launch<__half>(a, st) : dtype == AB_DT_BF16 ? sample_launch<__nv_bfloat16>(a, st) : sample_launch<float>(a, st);
+}
+
+}  // namespace ab

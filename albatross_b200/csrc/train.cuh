@@ -109,4 +109,11 @@ int policy_loss(const ab_logit_rows& t, const ab_policy& p, float scale, float* 
 int preference_loss(const ab_logit_rows& t, int64_t pairs, int64_t steps, const float* ref, float beta, float smoothing, float* loss, float* logp32,
                     float* stats, float* g, double* rows_scratch, cudaStream_t st);
 
+// writes: there are outputs, else the norm alone is wanted
+int clip_grad_norm(const ab_grad* t, int64_t n, bool writes, double scale, double max_norm, float* norm, double* sums, cudaStream_t st);
+size_t clip_scratch_bytes(int64_t n);   // on the current device
+
+int linear_int4(const ab_int4& m, int rows, const void* x, int64_t x_stride, void* y, cudaStream_t st);
+int sample_filtered(int dtype, int64_t rows, int V, const void* logits, int64_t stride, const float* u, const ab_sampling& p, int64_t* ids, float* logp, cudaStream_t st);
+
 }  // namespace ab

@@ -1,4 +1,9 @@
-// C entries of the operators with gradients: arguments checked, then the launchers of wkv_train.cu, norm.cu and loss.cu.
+// C entries of the operators with gradients, of the gradient norm and of what serves a token: arguments checked, then the launchers of wkv_train.cu,
+// norm.cu, loss.cu, clip.cu, sample.cu and int4.cu.
+#include <algorithm>
+#include <exception>
+#include <vector>
+
 #include "train.cuh"
 
 namespace ab {
@@ -54,6 +59,36 @@ int check_policy(const ab_policy* p, const ab_logit_rows& t, const void* scratch
     AB_CHECK_ARG(p->advantages || t.rows == 0, "%s: no advantages", who);
     AB_CHECK_ARG(p->clip_low >= 0.f && p->clip_low <= 1.f && p->clip_high >= 0.f, "%s: bad clip range", who);
     AB_CHECK_ARG(p->denom >= 0.f, "%s: the denominator is negative or not a number", who);
+    return OK;
+}
+
+// Outputs that lie on one another, or on gradients other than their own, would be read and written in any order.
+struct GradSpan {
+    uintptr_t from, to;
+    int64_t i;
+    bool operator<(const GradSpan& o) const { return from < o.from; }
+};
+void in_order(std::vector<GradSpan>& v) {
+    if (!std::is_sorted(v.begin(), v.end())) std::sort(v.begin(), v.end());
+}
+int check_apart(const ab_grad* t, int64_t n) {
+    std::vector<GradSpan> out, in;
+    out.reserve(n);
+    for (int64_t i = 0; i < n; ++i) {
+        if (t[i].n == 0) continue;
+        const uintptr_t o = reinterpret_cast<uintptr_t>(t[i].out), g = reinterpret_cast<uintptr_t>(t[i].g);
+        out.push_back({o, o + (uintptr_t)t[i].n * elem_bytes(t[i].out_dtype), i});
+        if (o != g || elem_bytes(t[i].dtype) != elem_bytes(t[i].out_dtype)) in.push_back({g, g + (uintptr_t)t[i].n * elem_bytes(t[i].dtype), i});
+    }
+    in_order(out);
+    for (size_t i = 1; i < out.size(); ++i)
+        AB_CHECK_ARG(out[i].from >= out[i - 1].to, "ab_clip_grad_norm: outputs %lld and %lld overlap", (long long)out[i - 1].i, (long long)out[i].i);
+    in_order(in);
+    size_t at = 0;
+    for (const GradSpan& s : in) {   // (outputs do not overlap: their ends are in order too. A later s begins no earlier, so what ends before this one is done with)
+        while (at < out.size() && out[at].to <= s.from) ++at;
+        AB_CHECK_ARG(at == out.size() || out[at].from >= s.to, "ab_clip_grad_norm: output %lld overlaps gradient %lld", (long long)out[at].i, (long long)s.i);
+    }
     return OK;
 }
 
@@ -168,6 +203,60 @@ int ab_preference_loss_fwd(const ab_logit_rows* t, int64_t pairs, int64_t steps,
     AB_CHECK_ARG(ref_logp && loss && logp32 && (rows_scratch || t->rows == 0), "ab_preference_loss_fwd: null pointer");
     AB_CHECK_ARG(smoothing >= 0.f && smoothing <= 1.f, "ab_preference_loss_fwd: smoothing outside 0 .. 1");
     return preference_loss(*t, pairs, steps, ref_logp, beta, smoothing, loss, logp32, stats, g, rows_scratch, (cudaStream_t)stream);
+}
+
+size_t ab_clip_grad_norm_scratch_bytes(int64_t tensors) { return tensors < 0 ? 0 : clip_scratch_bytes(tensors); }
+
+int ab_clip_grad_norm(const ab_grad* t, int64_t tensors, double scale, double max_norm, float* norm, void* scratch, void* stream) {
+    AB_CHECK_ARG(tensors >= 0 && (t || tensors == 0) && norm && scratch, "ab_clip_grad_norm: null pointer, or a negative number of tensors");
+    AB_CHECK_ARG(on_boundary(scratch, 8) && on_boundary(norm, 4), "ab_clip_grad_norm: misaligned pointer");
+    AB_CHECK_ARG(scale > 0 && scale < INFINITY, "ab_clip_grad_norm: the scale must be positive and finite");
+    AB_CHECK_ARG(max_norm >= 0, "ab_clip_grad_norm: the largest norm is negative or not a number");
+    bool with = false, without = false;
+    for (int64_t i = 0; i < tensors; ++i) {
+        const ab_grad& e = t[i];
+        AB_CHECK_ARG((is_16bit(e.dtype) || e.dtype == AB_DT_F32) && (is_16bit(e.out_dtype) || e.out_dtype == AB_DT_F32), "ab_clip_grad_norm: tensor %lld has a bad dtype", (long long)i);
+        AB_CHECK_ARG(e.n >= 0 && e.n <= (int64_t)1 << 40 && (e.g || e.n == 0), "ab_clip_grad_norm: tensor %lld has a bad size or no values", (long long)i);
+        AB_CHECK_ARG(on_boundary(e.g, elem_bytes(e.dtype)) && on_boundary(e.out, elem_bytes(e.out_dtype)), "ab_clip_grad_norm: tensor %lld is misaligned", (long long)i);
+        if (e.n > 0) (e.out ? with : without) = true;
+    }
+    AB_CHECK_ARG(!(with && without), "ab_clip_grad_norm: outputs for some tensors only");
+    if (with) {
+        try {
+            AB_CHECK(check_apart(t, tensors));
+        } catch (const std::exception&) {
+            set_error("ab_clip_grad_norm: out of host memory");
+            return ERR_TOO_LARGE;
+        }
+    }
+    return clip_grad_norm(t, tensors, with, scale, max_norm, norm, static_cast<double*>(scratch), (cudaStream_t)stream);
+}
+
+int ab_linear_int4(const ab_int4* m, int rows, const void* x, int64_t x_stride, void* y, void* stream) {
+    AB_CHECK_ARG(m, "ab_linear_int4: null pointer");
+    AB_CHECK_ARG(is_16bit(m->dtype), "ab_linear_int4: dtype %d is neither fp16 nor bf16", m->dtype);
+    AB_CHECK_ARG(rows >= 0 && m->n_out > 0 && m->k > 0 && x_stride >= 0, "ab_linear_int4: bad shape (rows=%d n_out=%d k=%d)", rows, m->n_out, m->k);
+    AB_CHECK_ARG((m->group == 32 || m->group == 64 || (m->group > 0 && m->group % 128 == 0)) && m->k % m->group == 0,
+                 "ab_linear_int4: groups of %d inputs (32, 64 or a multiple of 128, which divides %d)", m->group, m->k);
+    if (rows == 0) return OK;
+    AB_CHECK_ARG(m->w && m->scale && x && y, "ab_linear_int4: null pointer");
+    AB_CHECK_ARG(on_boundary(m->w, 16), "ab_linear_int4: the codes must start on a 16-byte boundary");
+    AB_CHECK_ARG(on_boundary(m->scale, 2) && on_boundary(x, 2) && on_boundary(y, 2), "ab_linear_int4: misaligned pointer");
+    return linear_int4(*m, rows, x, x_stride, y, (cudaStream_t)stream);
+}
+
+int ab_sample_filtered(int dtype, int64_t rows, int vocab, const void* logits, int64_t stride, const float* uniform, const ab_sampling* p,
+                       int64_t* ids, float* logp, void* stream) {
+    AB_CHECK_ARG(p, "ab_sample_filtered: null pointer");
+    AB_CHECK_ARG(is_16bit(dtype) || dtype == AB_DT_F32, "ab_sample_filtered: bad dtype %d", dtype);
+    AB_CHECK_ARG(rows >= 0 && vocab > 0 && vocab <= 1 << 18 && stride >= 0, "ab_sample_filtered: bad shape (a vocabulary of up to 2^18)");
+    AB_CHECK_ARG(p->temperature || p->temperature_all >= 0, "ab_sample_filtered: the temperature is negative or not a number");
+    AB_CHECK_ARG((p->top_p || p->top_p_all >= 0) && (p->min_p || p->min_p_all >= 0), "ab_sample_filtered: top_p or min_p is negative or not a number");
+    if (rows == 0) return OK;
+    AB_CHECK_ARG(logits && uniform && ids && logp, "ab_sample_filtered: null pointer");
+    AB_CHECK_ARG(on_boundary(logits, elem_bytes(dtype)) && on_boundary(uniform, 4) && on_boundary(ids, 8) && on_boundary(logp, 4) && on_boundary(p->temperature, 4) &&
+                 on_boundary(p->top_p, 4) && on_boundary(p->min_p, 4) && on_boundary(p->top_k, 4), "ab_sample_filtered: misaligned pointer");
+    return sample_filtered(dtype, rows, vocab, logits, stride, uniform, *p, ids, logp, (cudaStream_t)stream);
 }
 
 }  // extern "C"

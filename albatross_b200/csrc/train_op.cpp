@@ -4,27 +4,16 @@
 //
 // The kernel library is not linked: albatross_b200_train_bind() is given the path of the one that the package has loaded (the normal or the
 // range-checking build).
-#include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
-#include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <dlfcn.h>
-#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
-#include <torch/library.h>
 
-#include <string>
-
-#include "../../include/albatross_b200.h"
+#include "op.h"
 
 namespace {
 
-using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-using OptTensor = std::optional<Tensor>;
 
 struct Entries {
 #define AB_ENTRY(name) decltype(&::name) name = nullptr
@@ -40,41 +29,11 @@ struct Entries {
     AB_ENTRY(ab_policy_loss_fwd);
     AB_ENTRY(ab_policy_loss_grad);
     AB_ENTRY(ab_preference_loss_fwd);
+    AB_ENTRY(ab_clip_grad_norm_scratch_bytes);
+    AB_ENTRY(ab_clip_grad_norm);
 #undef AB_ENTRY
 } lib;
 
-// (numbers go into messages as strings: a number formatted by the stream of a shim built with another compiler's library than torch's has crashed)
-void check(int status, const char* what) { TORCH_CHECK(status == AB_OK, what, " failed with status ", std::to_string(status), ": ", lib.ab_last_error()); }
-
-int type_of(const Tensor& t) { return t.scalar_type() == at::kHalf ? AB_DT_F16 : t.scalar_type() == at::kBFloat16 ? AB_DT_BF16 : AB_DT_F32; }
-bool is_16bit(const Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
-bool is_known(const Tensor& t) { return is_16bit(t) || t.scalar_type() == at::kFloat; }
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-float* f32(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
-void* stream() { return (void*)at::cuda::getCurrentCUDAStream().stream(); }
-Tensor like(at::IntArrayRef sizes, const Tensor& t, at::ScalarType type) { return at::empty(sizes, t.options().dtype(type)); }
-Tensor given(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
-template <class... T>
-bool needs_grad(const T&... t) { return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...); }
-// a tensor that autograd does not look at, or none
-struct Plain {
-    Tensor t;
-};
-OptTensor or_none(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-// What would be lost without a word. A trace in the making would hold the outputs' allocation and not the call, and torch.func's wrappers have no
-// memory. A tangent's tensor need not require a gradient, and would be taken below autograd.
-bool traced() {
-    using Key = c10::impl::TorchDispatchModeKey;
-    for (const Key k : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL})
-        if (c10::impl::TorchDispatchModeTLS::get_mode(k).has_value()) return true;
-    return false;
-}
-template <class... T>
-void check_plain(const char* who, const T&... t) {
-    TORCH_CHECK(!traced() && ((!t.defined() || t.has_storage()) && ...), who,
-                ": cannot be traced or transformed (torch.compile, torch.export, make_fx, torch.func.grad); in a compiled program call it from a function under torch.compiler.disable");
-    TORCH_CHECK(!((t.defined() && t._fw_grad(/*level=*/0).defined()) || ...), who, ": forward-mode derivatives are not available");
-}
 // (Backward passes take their saved tensors before they go below autograd: unpacking one may recompute the forward pass, which has to be recorded.)
 // What a backward pass refuses. Gradients are not differentiable: asking for a graph of them is an error, not a silent zero. And in a stream capture
 // a leaf that an earlier graph still ties to the default stream: adding its gradient would make that stream wait for the capturing one, which the
@@ -192,23 +151,6 @@ std::tuple<Tensor, Tensor> wkv7(const OptTensor& state_, const Tensor& r, const 
 }
 
 // ---- the norms ---------------------------------------------------------------------------------------------------------------------
-// [..., C] with a dense last dimension and one stride between rows, of `least` values or more; others are copied. Here, ahead of autograd, so that
-// the backward pass reads the same copy (logits[:, :-1] of several sequences are copied once, not once in each pass).
-Tensor one_stride(const Tensor& t, int64_t least) {
-    bool fits = t.dim() < 1 || t.size(-1) <= 1 || t.stride(-1) == 1;
-    int64_t outer = -1;   // the stride that goes with the dimensions so far
-    for (int64_t d = t.dim() - 2; d >= 0 && fits; --d) {
-        if (t.size(d) == 1) continue;
-        fits = outer < 0 ? t.stride(d) >= least : t.stride(d) == outer;
-        outer = t.stride(d) * t.size(d);
-    }
-    return fits || t.numel() == 0 ? t : t.contiguous();
-}
-// [..., C] as rows [n, C] with a dense last dimension; a view where the strides allow one
-Tensor as_rows(const Tensor& t) {
-    const Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
-    return r.stride(1) == 1 || r.size(1) <= 1 ? r : r.contiguous();
-}
 int weight_type(const Tensor& x, const Tensor& w, const Tensor& b) { return type_of(w.defined() ? w : b.defined() ? b : x); }
 Tensor norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps, int64_t groups, Tensor* stats) {
     const c10::cuda::CUDAGuard guard(x.device());
@@ -462,6 +404,57 @@ std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits_, const Tensor& 
     return {loss, logp};
 }
 
+// ---- the norm over all gradients -------------------------------------------------------------------------------------------------------
+bool same_order(const Tensor& a, const Tensor& b) { return a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous()); }
+// out: empty (the norm alone), the gradients themselves, or one tensor for each. What is not dense, or lies in another order than its gradient, goes by way of a copy.
+Tensor clip_grad_norm(at::TensorList grads, double max_norm, double scale, at::TensorList out) {
+    constexpr const char* who = "clip_grad_norm";
+    TORCH_CHECK(!grads.empty(), who, ": no gradients");
+    TORCH_CHECK(out.empty() || out.size() == grads.size(), who, ": ", std::to_string(grads.size()), " gradients and ", std::to_string(out.size()), " outputs");
+    TORCH_CHECK(scale > 0 && scale <= std::numeric_limits<double>::max(), who, ": the scale must be positive and finite");
+    TORCH_CHECK(max_norm >= 0, who, ": the largest norm is negative or not a number");
+    const at::Device device = grads[0].device();
+    const bool grad_mode = at::GradMode::is_enabled();
+    check_plain(who);
+    std::vector<ab_grad> list(grads.size());
+    std::vector<Tensor> dense;                          // copies, kept until the kernels are launched
+    std::vector<std::pair<size_t, Tensor>> back;        // outputs that are copied to where they belong
+    at::AutoDispatchBelowADInplaceOrView below;
+    for (size_t i = 0; i < grads.size(); ++i) {
+        const Tensor& g = grads[i];
+        TORCH_CHECK(g.defined() && g.is_cuda() && g.layout() == at::kStrided && g.device() == device && is_known(g), who, ": gradient ", std::to_string(i),
+                    " is not a dense fp16, bf16 or fp32 tensor on the device of the first");
+        check_plain(who, g);
+        Tensor from = g, to;
+        const bool in_order = g.is_non_overlapping_and_dense();
+        if (!out.empty()) {
+            const Tensor& o = out[i];
+            TORCH_CHECK(o.defined() && o.is_cuda() && o.layout() == at::kStrided && o.device() == device && is_known(o) && o.sizes() == g.sizes(), who, ": output ", std::to_string(i),
+                        " is not a dense fp16, bf16 or fp32 tensor of its gradient's shape and device");
+            check_plain(who, o);
+            TORCH_CHECK(!(grad_mode && o.requires_grad()), who, ": output ", std::to_string(i), " requires a gradient; write over it under torch.no_grad()");
+            at::assert_no_internal_overlap(o);
+            if (!in_order || !o.is_non_overlapping_and_dense() || !same_order(g, o)) {
+                from = g.contiguous();
+                to = o.is_contiguous() ? o : at::empty(g.sizes(), o.options());
+                if (!to.is_same(o)) back.emplace_back(i, to);
+            } else {
+                to = o;
+            }
+            if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
+        } else if (!in_order) {
+            from = g.contiguous();
+        }
+        if (!from.is_same(g)) dense.push_back(from);
+        list[i] = {from.data_ptr(), ptr(to), from.numel(), type_of(from), to.defined() ? type_of(to) : 0};
+    }
+    const c10::cuda::CUDAGuard guard(device);
+    Tensor norm = like({}, grads[0], at::kFloat), scratch = like({(int64_t)lib.ab_clip_grad_norm_scratch_bytes((int64_t)list.size())}, grads[0], at::kByte);
+    check(lib.ab_clip_grad_norm(list.data(), (int64_t)list.size(), scale, max_norm, f32(norm), scratch.data_ptr(), stream()), "ab_clip_grad_norm");
+    for (const auto& b : back) out[b.first].copy_(b.second);
+    return norm;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(albatross_b200, m) {
@@ -472,6 +465,7 @@ TORCH_LIBRARY(albatross_b200, m) {
           "-> (Tensor, Tensor)", policy_loss);
     m.def("policy_loss_grad(Tensor logits, Tensor ids, Tensor? old_logp, Tensor advantages, Tensor? mask, Tensor? ref_logp, float clip_low, float clip_high, float kl, float denom, "
           "float scale, Tensor? out) -> (Tensor, Tensor, Tensor)", policy_loss_grad);
+    m.def("clip_grad_norm(Tensor[] grads, float max_norm, float scale, Tensor[] out) -> Tensor", clip_grad_norm);
     m.def("preference_loss(Tensor logits, Tensor ids, Tensor ref_logp, Tensor? mask, float beta, float smoothing) -> (Tensor, Tensor)", preference_loss);
 }
 
@@ -480,24 +474,20 @@ extern "C" int albatross_b200_train_bind(const char* path, const char** missing)
     void* h = dlopen(path, RTLD_NOW | RTLD_LOCAL);
     *missing = path;
     if (!h) return -1;
-#define AB_ENTRY(name)                                                                        \
-    lib.name = reinterpret_cast<decltype(lib.name)>(dlsym(h, #name));                         \
-    if (!lib.name) {                                                                          \
-        *missing = #name;                                                                     \
-        return -1;                                                                            \
-    }
-    AB_ENTRY(ab_last_error)
-    AB_ENTRY(ab_wkv7_checkpoint_bytes)
-    AB_ENTRY(ab_wkv7_seq_fwd)
-    AB_ENTRY(ab_wkv7_seq_bwd)
-    AB_ENTRY(ab_layer_norm_fwd)
-    AB_ENTRY(ab_layer_norm_scratch_bytes)
-    AB_ENTRY(ab_layer_norm_bwd)
-    AB_ENTRY(ab_token_logp_fwd)
-    AB_ENTRY(ab_token_logp_bwd)
-    AB_ENTRY(ab_policy_loss_fwd)
-    AB_ENTRY(ab_policy_loss_grad)
-    AB_ENTRY(ab_preference_loss_fwd)
-#undef AB_ENTRY
+    AB_TAKE(ab_last_error)
+    AB_TAKE(ab_wkv7_checkpoint_bytes)
+    AB_TAKE(ab_wkv7_seq_fwd)
+    AB_TAKE(ab_wkv7_seq_bwd)
+    AB_TAKE(ab_layer_norm_fwd)
+    AB_TAKE(ab_layer_norm_scratch_bytes)
+    AB_TAKE(ab_layer_norm_bwd)
+    AB_TAKE(ab_token_logp_fwd)
+    AB_TAKE(ab_token_logp_bwd)
+    AB_TAKE(ab_policy_loss_fwd)
+    AB_TAKE(ab_policy_loss_grad)
+    AB_TAKE(ab_preference_loss_fwd)
+    AB_TAKE(ab_clip_grad_norm_scratch_bytes)
+    AB_TAKE(ab_clip_grad_norm)
+    last_error = lib.ab_last_error;
     return 0;
 }

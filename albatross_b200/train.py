@@ -6,8 +6,10 @@
     policy_loss      clipped ratios against the policy that sampled, with a penalty for leaving a reference; differentiable
     policy_loss_grad the same, loss and gradient by the logits in one pass over them
     preference_loss  pairs of a better and a worse answer; differentiable
+    grad_norm        the norm over all gradients of a model
+    clip_grad_norm   the same, and the gradients scaled down to a largest norm, a loss scale taken out on the way
 
-They run on the current stream of their tensors' device and take strided inputs: the last dimension dense and, but for the recurrence,
+They run on the current stream of their tensors' device and take strided inputs. For those with gradients: the last dimension dense and, but for the recurrence,
 one stride between rows (logits[:, :-1] of several sequences has two). Others are copied, once for both passes. Gradients are those of
 the formulas in include/albatross_b200.h; they cannot be differentiated again, and there are no forward-mode derivatives: a tensor with a
 tangent is refused. Neither can they be traced (torch.compile, torch.export, make_fx: call them from a function under
@@ -19,31 +21,17 @@ calls the C entries of the kernel library; what does not fit raises RuntimeError
 """
 from __future__ import annotations
 
-import ctypes as C
-import os
 from typing import Optional, Sequence, Tuple
 
 import torch
 
-from . import _lib
+from . import _shim
 from . import build as _build
 
 
-def _load():
-    if not os.path.exists(_build.TRAIN_OP_LIB):
-        raise ImportError(f"{_build.TRAIN_OP_LIB} is missing: build it with `python -m albatross_b200.build`")
-    torch.ops.load_library(_build.TRAIN_OP_LIB)
-    missing = C.c_char_p()
-    bind = C.CDLL(_build.TRAIN_OP_LIB).albatross_b200_train_bind
-    bind.argtypes = [C.c_char_p, C.POINTER(C.c_char_p)]
-    if bind(_lib.LIB_PATH.encode(), C.byref(missing)):
-        raise ImportError(f"{_lib.LIB_PATH} does not have {missing.value.decode()}: build both again with `python -m albatross_b200.build`")
-    ops = torch.ops.albatross_b200
-    return {n: getattr(ops, n).default for n in ("wkv7", "layer_norm", "token_logp", "policy_loss", "policy_loss_grad", "preference_loss")}
-
-
-_ops = _load()
-_wkv7, _layer_norm, _token_logp, _policy_loss, _policy_loss_grad, _preference_loss = _ops.values()
+_wkv7, _layer_norm, _token_logp, _policy_loss, _policy_loss_grad, _preference_loss, _clip_grad_norm = _shim.load(
+    _build.TRAIN_OP_LIB, "albatross_b200_train_bind",
+    ("wkv7", "layer_norm", "token_logp", "policy_loss", "policy_loss_grad", "preference_loss", "clip_grad_norm"))
 
 
 def RWKV7_TRAIN_OP(state: Optional[torch.Tensor], r, w, k, v, a, b, lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -112,3 +100,20 @@ def preference_loss(logits: torch.Tensor, ids: torch.Tensor, ref_logp: torch.Ten
     the mean of -(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m). `ref_logp` [2P]: the sums under the reference model (no
     gradient). Returns the loss and the sums s (without gradient)."""
     return _preference_loss(logits, ids, ref_logp, mask, beta, label_smoothing)
+
+
+def grad_norm(grads: Sequence[torch.Tensor], scale: float = 1.0) -> torch.Tensor:
+    """`scale` times the 2-norm over all values of all tensors (fp16, bf16 and fp32, mixed as they come), as an fp32 number on their device. The
+    squares are added up in 64 bits. A tensor that stands in the list twice counts twice."""
+    return _clip_grad_norm(grads, float("inf"), scale, [])
+
+
+def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, scale: float = 1.0, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    """Writes grad * f with f = scale * min(1, max_norm / norm) over the gradients, or into `out` (a tensor for each, of its shape; fp16, bf16 or fp32), and
+    returns norm = scale * (the 2-norm over all values) from before the clipping. `scale` takes a loss scale out: 1 / 65536 where the loss was multiplied by
+    65536; gradients in fp16 then want `out` in fp32, in which small ones do not vanish. Where the norm is not finite nothing is clipped (f = scale), and what
+    is wrong stays visible: a training loop skips that step by norm.isfinite(). Nothing is read back to the host.
+
+    Outputs may not overlap each other, nor gradients other than their own. Up to 1000 tensors take two launches; tensors that are not dense, or lie in another
+    order than their output, are copied."""
+    return _clip_grad_norm(grads, max_norm, scale, grads if out is None else out)

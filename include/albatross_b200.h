@@ -140,6 +140,19 @@ int ab_gemm_static_reset(void* stream);
  * of the built-in area of the current device through the HOST pointer `value_host`; synchronises the device. */
 int ab_gemm_static_debug_counter(int index, int write, uint32_t* value_host);
 
+/* ---- products with 4-bit weights in groups ---------------------------------------------------
+ * No counterpart in the reference: the format that 4-bit checkpoints commonly come in, beside AB_FMT_FP4, which is made here from fp16 ones.
+ * y[r, n] = sum_k x[r, k] * (q[n, k] - z[n, k / group]) * s[n, k / group], for few rows: the codes are read once for up to 16 of them (8 where group
+ * is 32 and rows exceed 4), again for each further 16. Products of codes and activations are exact, their sums and scales 32-bit. */
+typedef struct ab_int4 {
+    int32_t dtype, n_out, k, group;   /* of scale, x and y: AB_DT_F16 or AB_DT_BF16; group: 32, 64 or a multiple of 128, divides k */
+    const void* w;                    /* uint8 [n_out, k/2], even k in the low nibble, codes 0 .. 15; on a 16-byte boundary */
+    const void* scale;                /* dtype [n_out, k/group] */
+    const void* zero;                 /* uint8 [n_out, k/group] of 0 .. 15, or NULL: 8 everywhere */
+} ab_int4;
+/* x: rows of dtype, x_stride elements apart; y: dense [rows, n_out]. */
+int ab_linear_int4(const ab_int4* m, int rows, const void* x, int64_t x_stride, void* y, void* stream);
+
 /* ---- token sampling on the device -----------------------------------------------------------
  * Replaces sampler_simple_batch (reference/utils.py:43-45: uniform noise in [0, noise) added to the logits, then
  * the first column of a descending argsort) without sorting and without leaving the device: out[r] = argmax over
@@ -149,6 +162,23 @@ int ab_sample_rows(const void* logits, int rows, int vocab, float noise, uint32_
 /* The same with 64-bit ids (the dtype the reference's sampler returns). `out` may be device memory or pinned host
  * memory that the device can address: the ids then need no copy of their own on the way to the host. */
 int ab_sample_rows_i64(const void* logits, int rows, int vocab, float noise, uint32_t seed, int64_t* out, void* stream);
+
+/* Draws out[r] from a row's distribution under filters, by a given uniform number (no counterpart in the reference, whose sampler is the one above).
+ * With w_i = exp((l_i - max l) / temperature) and the values in order, larger ones first, equals by index, the front part is kept in which each
+ * value but the first has a rank below top_k, a sum of w in front of it below top_p * (the sum of w over the first top_k), and w >= min_p; the id is the
+ * first whose sum of w up to and with it exceeds uniform[r] * (the sum that is kept). logp[r]: log(w / the sum that is kept), the log-probability under
+ * the distribution drawn from. temperature 0, or top_k 1: the first largest value, logp 0. top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 filter
+ * nothing, and neither does a NaN among the rows' numbers (as a temperature it is 0). -inf is never drawn; +inf leaves nothing but itself; a row with a NaN, or of -inf alone, gives -1 and NaN. */
+typedef struct ab_sampling {
+    const float *temperature, *top_p, *min_p;   /* [rows] on the device, or NULL: the value below for every row */
+    const int32_t* top_k;
+    double temperature_all, top_p_all, min_p_all;
+    int32_t top_k_all, _pad;
+} ab_sampling;
+/* logits: rows of dtype (AB_DT_*), `stride` elements apart, vocab up to 2^18; uniform: fp32 [rows] in [0, 1) (others are taken into it); ids, logp: [rows], device or
+ * pinned host memory. */
+int ab_sample_filtered(int dtype, int64_t rows, int vocab, const void* logits, int64_t stride, const float* uniform, const ab_sampling* p,
+                       int64_t* ids, float* logp, void* stream);
 
 /* ---- de-quantisation dump (parity checks) ---------------------------------------------------
  * Writes the kernels' in-register de-quantised weights as fp32 [n_out,k] (tensor/row/column scales applied). */
@@ -236,6 +266,19 @@ int ab_policy_loss_grad(const ab_logit_rows* t, const ab_policy* p, float scale,
  * g: fp32 [2 * pairs], for ab_token_logp_bwd with rows_per_g = steps. rows_scratch: fp64 [rows]. */
 int ab_preference_loss_fwd(const ab_logit_rows* t, int64_t pairs, int64_t steps, const float* ref_logp, float beta, float smoothing, float* loss,
                            float* logp32, float* stats, float* g, double* rows_scratch, void* stream);
+
+/* ---- the norm over all gradients, and clipping (no counterpart in the reference) -----------------------------------
+ * norm = scale * sqrt(sum of g^2 over all tensors); out = g * f with f = scale * min(1, max_norm / norm), or f = scale where the norm is not
+ * finite. Two launches for up to 1000 tensors, two more for each further 1000. */
+typedef struct ab_grad {
+    const void* g;               /* n values of dtype, dense */
+    void* out;                   /* n values of out_dtype: g itself, or apart from every tensor of the list; NULL in all of them: the norm alone */
+    int64_t n;
+    int32_t dtype, out_dtype;    /* AB_DT_* */
+} ab_grad;
+size_t ab_clip_grad_norm_scratch_bytes(int64_t tensors);
+/* t: HOST array, read before the call returns. norm: fp32 [1]. scratch: on the device, ab_clip_grad_norm_scratch_bytes(tensors). */
+int ab_clip_grad_norm(const ab_grad* t, int64_t tensors, double scale, double max_norm, float* norm, void* scratch, void* stream);
 
 /* ---- whole-model forward -------------------------------------------------------------------
  * ab_forward replaces RWKV_x070.forward / forward_batch (reference/rwkv7.py:98-126, :128-221):

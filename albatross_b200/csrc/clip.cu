@@ -27,7 +27,7 @@ constexpr int CL_LOADS = 8;                     // units in flight per lane
 constexpr uint32_t CL_SHARE = 32 * CL_LOADS;    // units that a warp takes at a time
 constexpr int CL_BLOCKS_PER_SM = 2;
 // The list of a launch: few tensors in a small parameter (a launch copies all of it), many in the largest there is.
-constexpr int CL_FEW = 60, CL_MANY = 1000;
+constexpr int CL_FEW = 120, CL_MANY = 1000;
 
 struct ClipTensor {
     const void* g;
@@ -36,7 +36,7 @@ struct ClipTensor {
     uint32_t first;        // first unit
     uint16_t head;         // values in front of the first 16-byte boundary
     uint8_t types;         // type of g, and of out in bits 2 and 3
-    uint8_t out_apart;     // out does not lie on the boundaries that g's units need: stored value by value
+    uint8_t out_apart;     // how a unit's outputs lie: 0 on a boundary of their size, 1 on one of 16 bytes (they have 32), 2 elsewhere: stored value by value
 };
 template <int CAP>
 struct ClipList {
@@ -142,6 +142,11 @@ __global__ void __launch_bounds__(CL_THREADS, CL_BLOCKS_PER_SM) grad_squares_ker
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
 
+// 32 bytes at once: as two stores of 16, each lane's halves lie 32 bytes apart, and the two cost as much as whole lines each
+__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+}
+
 template <class E, class O>
 __device__ __forceinline__ void scale_units(const ClipTensor& t, uint32_t lo, uint32_t hi, float f, int lane) {
     constexpr int N = 16 / sizeof(E), W = N * sizeof(O) / 16;   // stores of 16 bytes per unit (0: of 8)
@@ -166,9 +171,11 @@ __device__ __forceinline__ void scale_units(const ClipTensor& t, uint32_t lo, ui
         for (int k = 0; k < N; ++k) v[k] *= f;
         O* to = out + t.head + (uint64_t)u * N;
         if (!all_out.holds(to, N)) continue;
-        if (t.out_apart) {
+        if (t.out_apart == 2) {
 #pragma unroll
             for (int k = 0; k < N; ++k) to[k] = from_f<O>(v[k]);
+        } else if (W == 2 && t.out_apart == 0) {
+            store32(to, pack<O>(v), pack<O>(v + 16 / sizeof(O) % N));
         } else if (W == 0) {
             O half_[8];
 #pragma unroll
@@ -230,55 +237,65 @@ __global__ void __launch_bounds__(CL_THREADS, CL_BLOCKS_PER_SM) grad_scale_kerne
     }
 }
 
+// up to CAP tensors from t[from] on
+template <int CAP>
+int clip_list(const ab_grad* t, int64_t from, int64_t n, ClipList<CAP>& list) {
+    list.n = 0;
+    uint64_t units = 0;
+    for (int64_t i = from; i < n && i < from + CAP; ++i) {
+        const int size = t[i].dtype == AB_DT_F32 ? 4 : 2, out_size = t[i].out_dtype == AB_DT_F32 ? 4 : 2, per = clip_per_unit(t[i].dtype);
+        if (t[i].n == 0) continue;
+        ClipTensor& e = list.t[list.n];
+        e.g = t[i].g, e.out = t[i].out, e.n = (uint64_t)t[i].n, e.first = (uint32_t)units;
+        const uint64_t head = (16 - (reinterpret_cast<uintptr_t>(e.g) & 15)) % 16 / size;
+        e.head = (uint16_t)(head < e.n ? head : e.n);
+        e.types = (uint8_t)(t[i].dtype | t[i].out_dtype << 2);
+        // a unit's outputs: 8 bytes (32 bits into 16), 16 or 32
+        const uint64_t bytes = per * out_size, to = reinterpret_cast<uintptr_t>(e.out) + (uint64_t)e.head * out_size;
+        e.out_apart = to % bytes == 0 ? 0 : bytes == 32 && to % 16 == 0 ? 1 : 2;
+        units += (e.n - e.head) / per + (e.head != 0 || (e.n - e.head) % per != 0 ? 1 : 0);
+        AB_CHECK_ARG(units < UINT32_MAX, "clip_grad_norm: the tensors of a launch have too many values");
+        ++list.n;
+    }
+    list.units = (uint32_t)units;
+    return OK;
+}
+
 template <int CAP>
 int clip_launch(const ab_grad* t, int64_t n, bool writes, double scale, double max_norm, float* norm, double* sums, cudaStream_t st) {
-    const int n_sm = current_sm_count();
-    bool in_place = true;
-    ClipHow how = {sums, 0, 0, writes ? 1 : 0, scale, max_norm, nullptr};
-    for (int pass = 0; pass < 2; ++pass) {   // the squares of all lists, then the scaling of all
-        how.in_place = in_place ? 1 : 0;
-        for (int64_t from = 0; from == 0 || from < n; from += CAP) {
-            ClipList<CAP> list;
-            list.n = 0;
-            uint64_t units = 0;
-            for (int64_t i = from; i < n && i < from + CAP; ++i) {
-                const int size = t[i].dtype == AB_DT_F32 ? 4 : 2, out_size = t[i].out_dtype == AB_DT_F32 ? 4 : 2, per = clip_per_unit(t[i].dtype);
-                if (t[i].n == 0) continue;
-                ClipTensor& e = list.t[list.n];
-                e.g = t[i].g, e.out = t[i].out, e.n = (uint64_t)t[i].n, e.first = (uint32_t)units;
-                const uint64_t head = (16 - (reinterpret_cast<uintptr_t>(e.g) & 15)) % 16 / size;
-                e.head = (uint16_t)(head < e.n ? head : e.n);
-                e.types = (uint8_t)(t[i].dtype | t[i].out_dtype << 2);
-                // a unit's outputs: 8 bytes (32 bits into 16), 16 or 32
-                const int bytes = per * out_size;
-                e.out_apart = (reinterpret_cast<uintptr_t>(e.out) + (uint64_t)e.head * out_size) % (bytes < 16 ? bytes : 16) != 0;
-                in_place = in_place && e.g == e.out;
-                units += (e.n - e.head) / per + (e.head != 0 || (e.n - e.head) % per != 0 ? 1 : 0);
-                AB_CHECK_ARG(units < UINT32_MAX, "clip_grad_norm: the tensors of a launch have too many values");
-                ++list.n;
-            }
-            list.units = (uint32_t)units;
-            const uint64_t shares = (units + CL_SHARE - 1) / CL_SHARE, wanted = (shares + CL_WARPS - 1) / CL_WARPS;
-            const int blocks = (int)(wanted < 1 ? 1 : wanted > (uint64_t)n_sm * CL_BLOCKS_PER_SM ? n_sm * CL_BLOCKS_PER_SM : wanted);
-            if (pass == 0) {
-                grad_squares_kernel<CAP><<<blocks, CL_THREADS, 0, st>>>(list, sums + how.n_sums);
-                AB_CUDA(cudaGetLastError());
-                how.n_sums += blocks;
-                continue;
-            }
-            how.norm = from == 0 ? norm : nullptr;
-            if (from > 0 && !writes) break;
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(writes ? blocks : 1);
-            cfg.blockDim = dim3(CL_THREADS);
-            cfg.stream = st;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-            attr[0].val.programmaticStreamSerializationAllowed = 1;
-            cfg.attrs = attr;
-            cfg.numAttrs = from == 0 ? 1 : 0;   // (it begins while the last sums are made; further launches follow one another)
-            AB_CUDA(cudaLaunchKernelEx(&cfg, grad_scale_kernel<CAP>, list, how));
+    const int most = current_sm_count() * CL_BLOCKS_PER_SM;
+    ClipList<CAP> list;
+    auto blocks = [&]() {
+        const uint64_t wanted = ((uint64_t)list.units + CL_SHARE * CL_WARPS - 1) / (CL_SHARE * CL_WARPS);
+        return (int)(wanted < 1 ? 1 : wanted > (uint64_t)most ? most : wanted);
+    };
+    ClipHow how = {sums, 0, 1, writes ? 1 : 0, scale, max_norm, norm};
+    for (int64_t from = 0; from == 0 || from < n; from += CAP) {   // the squares of all lists
+        const int err = clip_list(t, from, n, list);
+        if (err != OK) return err;
+        for (int i = 0; i < list.n; ++i)
+            if (list.t[i].g != list.t[i].out) how.in_place = 0;
+        const int grid = blocks();
+        grad_squares_kernel<CAP><<<grid, CL_THREADS, 0, st>>>(list, sums + how.n_sums);
+        AB_CUDA(cudaGetLastError());
+        how.n_sums += grid;
+    }
+    for (int64_t from = 0; from == 0 || (writes && from < n); from += CAP) {   // then the scaling
+        if (n > CAP) {
+            const int err = clip_list(t, from, n, list);
+            if (err != OK) return err;
         }
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(writes ? blocks() : 1);
+        cfg.blockDim = dim3(CL_THREADS);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = from == 0 ? 1 : 0;   // (it begins while the last sums are made; further launches follow one another)
+        AB_CUDA(cudaLaunchKernelEx(&cfg, grad_scale_kernel<CAP>, list, how));
+        how.norm = nullptr;
     }
     return OK;
 }

@@ -20,7 +20,7 @@ namespace ab {
 namespace {
 
 constexpr int I4_WARPS = 16, I4_THREADS = 32 * I4_WARPS;
-constexpr int I4_AHEAD = 4;                  // chunks in flight per warp
+__host__ __device__ constexpr int i4_ahead(int groups, int nt) { return nt * groups < 8 ? 4 : 3; }   // chunks in flight per warp (as registers allow)
 constexpr int I4_X_BYTES = 128 * 1024;       // activations of a block at most
 constexpr int I4_BLOCK_TILES = 32;           // tiles of a cluster at most
 
@@ -56,6 +56,10 @@ template <> struct I4Type<__half> {
             a[i] = *reinterpret_cast<const uint32_t*>(&v);
         }
     }
+    static __device__ __forceinline__ void first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    }
     static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -74,6 +78,10 @@ template <> struct I4Type<__nv_bfloat16> {
             a[i] = *reinterpret_cast<const uint32_t*>(&v);
         }
     }
+    static __device__ __forceinline__ void first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    }
     static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -84,6 +92,11 @@ __device__ __forceinline__ uint4 i4_load(const uint4* p) {
     uint4 v;
     asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
+}
+// where `on` is false the registers keep what they have, with no instruction for it
+__device__ __forceinline__ void i4_x(uint4& v, const uint4* p, bool on) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n @p ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
+                 : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w) : "r"(smem_u32(p)), "r"((uint32_t)on) : "memory");
 }
 __device__ __forceinline__ float i4_peer(const float* own, uint32_t rank) {
     float v;
@@ -96,6 +109,7 @@ template <class E, int GROUPS, int NT>
 __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_constant__ I4Args a) {
     extern __shared__ __align__(16) unsigned char i4_smem[];
     using T = I4Type<E>;
+    constexpr int AHEAD = i4_ahead(GROUPS, NT);
     constexpr int MR = NT * 8 / GROUPS, SCALES = GROUPS == 1 ? 1 : 2;   // batch rows; scales of a lane's two columns
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int cl = (int)blockIdx.x / a.ks, rank = (int)blockIdx.x - cl * a.ks;
@@ -112,36 +126,52 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     const Extent w_all(a.w, (uint64_t)a.N * (a.K / 2)), s_all(a.scale, (uint64_t)a.N * a.groups * sizeof(E)), z_all(a.zero, (uint64_t)a.N * a.groups);
     pdl_wait();
 
-    // What a chunk needs, in a ring of registers.
-    uint4 w[I4_AHEAD][2];
-    E s[I4_AHEAD][2][SCALES];
-    uint32_t z[I4_AHEAD][2];
+    // What a chunk needs, in a ring of registers. Addresses are made once for a tile; a chunk is 64 bytes further than the one before.
+    uint4 w[AHEAD][2];
+    E s[AHEAD][2][SCALES];
+    uint32_t z[AHEAD][2];
     int in_tile = slot, in_c = 0;
-    auto request = [&](uint4 (&w)[2], E (&s)[2][SCALES], uint32_t (&z)[2]) {
-        const int c = c0 + lo + in_c, k = c * 128 + t * 32;
+    bool on[2];
+    uint32_t w_at[2], s_at[2];   // in 16 bytes; in groups (32 bits hold them: checked by the launch)
+    const int first = c0 + lo, of_code = GROUPS == 1 ? 0 : t * GROUPS / 4;   // the group, of a chunk, of this lane's codes
+    // where a row ends inside of a chunk: chunks of this warp in which this lane has codes, and (from its columns) scales
+    const int codes_to = GROUPS == 1 ? INT32_MAX : (a.K - t * 32 + 127) / 128 - first;
+    auto open = [&]() {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int n = n0 + in_tile * 16 + h * 8 + g;
-            const bool on = n < n1 && in_tile < tiles;
-            const uint4* p = reinterpret_cast<const uint4*>(a.w + (int64_t)n * (a.K / 2) + k / 2);
-            w[h] = on && k < a.K && w_all.holds(p) ? i4_load(p) : make_uint4(0, 0, 0, 0);
+            on[h] = n < n1;
+            const uint32_t row = on[h] ? n : n0;
+            w_at[h] = row * (uint32_t)(a.K / 32) + first * 4 + t;
+            s_at[h] = row * (uint32_t)a.groups + (GROUPS > 1 || a.per_group == 1 ? first * GROUPS : 0);
+        }
+    };
+    auto request = [&](uint4 (&w)[2], E (&s)[2][SCALES], uint32_t (&z)[2]) {
+        const int group = GROUPS > 1 || a.per_group == 1 ? in_c * GROUPS : (first + in_c) / a.per_group;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4* p_w = reinterpret_cast<const uint4*>(a.w) + (w_at[h] + in_c * 4);
+            w[h] = make_uint4(0, 0, 0, 0);
+            if (on[h] && in_c < codes_to && w_all.holds(p_w)) w[h] = i4_load(p_w);
 #pragma unroll
             for (int i = 0; i < SCALES; ++i) {
-                const int group = GROUPS == 1 ? (a.per_group == 1 ? c : c / a.per_group) : c * GROUPS + (2 * t + i) % GROUPS;
-                const E* p_s = static_cast<const E*>(a.scale) + (int64_t)n * a.groups + group;
-                s[h][i] = on && group < a.groups && s_all.holds(p_s) ? __ldg(p_s) : from_f<E>(0.f);
+                const int at = group + (SCALES == 1 ? 0 : (2 * t + i) % GROUPS);
+                const E* p = static_cast<const E*>(a.scale) + (s_at[h] + at);
+                s[h][i] = from_f<E>(0.f);
+                if (on[h] && (GROUPS == 1 || first * GROUPS + at < a.groups) && s_all.holds(p)) s[h][i] = __ldg(p);
             }
             z[h] = 8;
-            if (a.zero) {
-                const int group = GROUPS == 1 ? (a.per_group == 1 ? c : c / a.per_group) : c * GROUPS + t / (4 / GROUPS);
-                const uint8_t* p_z = a.zero + (int64_t)n * a.groups + group;
-                if (on && group < a.groups && z_all.holds(p_z)) z[h] = __ldg(p_z);
-            }
+            const uint8_t* p_z = a.zero + (s_at[h] + group + of_code);
+            if (a.zero && on[h] && in_c < codes_to && z_all.holds(p_z)) z[h] = __ldg(p_z);
         }
-        if (++in_c == len) in_c = 0, in_tile += slots;
+        if (++in_c == len) {
+            in_c = 0, in_tile += slots;
+            open();
+        }
     };
+    open();
 #pragma unroll
-    for (int i = 0; i < I4_AHEAD; ++i)
+    for (int i = 0; i < AHEAD; ++i)
         if (i < total) request(w[i], s[i], z[i]);
 
     // Activations: 16 bytes for each word of codes, [chunk][word of a lane][batch row][lane's quarter].
@@ -173,12 +203,15 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     float sum[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
-    // batch row of this lane's column in eight n, and whether its inputs are of that column's group
-    const bool mine = GROUPS == 1 || t / (4 / GROUPS) == g % GROUPS;
+    // Where this lane's inputs lie: of its column's batch row, if they are of its column's group; else its registers stay zero. (Columns behind the last batch
+    // row read that one's, and nobody reads them.)
+    const bool has = GROUPS == 1 || of_code == g % GROUPS;
+    const uint4* x_at[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x_at[n] = sx + min(n * (8 / GROUPS) + g / GROUPS, rows - 1) * 4 + t;
+    uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};   // (in turn)
     auto chunk = [&](const uint4 (&w)[2], const E (&s)[2][SCALES], const uint32_t (&z)[2], int c) {
         float d[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
         const uint32_t zl = z[0] * 0x00010001u, zh = z[1] * 0x00010001u;
 #pragma unroll
         for (int word = 0; word < 4; ++word) {
@@ -189,11 +222,11 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
             T::less(h, zh);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int m = n * (8 / GROUPS) + g / GROUPS;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (mine && m < rows && AB_BC((c * 4 + word + 1) * rows * 64 <= a.x_bytes)) x = sx[(c * 4 + word) * (rows * 4) + m * 4 + t];
-                T::mma(d[n], l[0], h[0], l[1], h[1], x.x, x.y);
-                T::mma(d[n], l[2], h[2], l[3], h[3], x.z, x.w);
+                uint4& v = x[(word * NT + n) & 1];
+                i4_x(v, x_at[n] + (c * 4 + word) * (rows * 4), has && AB_BC((c * 4 + word + 1) * rows * 64 <= a.x_bytes));
+                if (word == 0) T::first(d[n], l[0], h[0], l[1], h[1], v.x, v.y);
+                else T::mma(d[n], l[0], h[0], l[1], h[1], v.x, v.y);
+                T::mma(d[n], l[2], h[2], l[3], h[3], v.z, v.w);
             }
         }
 #pragma unroll
@@ -241,12 +274,12 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     int tile = slot, c = 0;
     if (len == 0)   // (fewer chunks than warps of a tile: this one adds zeros)
         for (int i = 0; i < rounds; ++i) finish(slot + i * slots);
-    for (int i = 0; i < total; i += I4_AHEAD) {
+    for (int i = 0; i < total; i += AHEAD) {
 #pragma unroll
-        for (int j = 0; j < I4_AHEAD; ++j) {
+        for (int j = 0; j < AHEAD; ++j) {
             if (i + j < total) {
                 chunk(w[j], s[j], z[j], lo + c);
-                if (i + j + I4_AHEAD < total) request(w[j], s[j], z[j]);
+                if (i + j + AHEAD < total) request(w[j], s[j], z[j]);
                 if (++c == len) {
                     finish(tile);
                     c = 0, tile += slots;
@@ -279,6 +312,7 @@ int i4_launch(I4Args a, cudaStream_t st) {
         return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST), "cudaFuncSetAttribute(linear_int4)");
     });
     if (err != OK) return err;
+    AB_CHECK_ARG((int64_t)a.N * (a.K / 32) < UINT32_MAX, "linear_int4: a matrix of %d x %d is too large", a.N, a.K);
     const int chunks = (a.K + 127) / 128;
     a.pass = MR < a.rows ? MR : a.rows;
     a.ks = 1;
@@ -318,7 +352,12 @@ int i4_launch(I4Args a, cudaStream_t st) {
 template <class E, int GROUPS>
 int i4_columns(const I4Args& a, cudaStream_t st) {
     const int tiles = (a.rows * GROUPS + 7) / 8;
-    return tiles <= 1 ? i4_launch<E, GROUPS, 1>(a, st) : tiles <= 2 ? i4_launch<E, GROUPS, 2>(a, st) : i4_launch<E, GROUPS, 4>(a, st);
+    // (16 batch rows are two eights in groups of 128, and four in groups of 64; four in groups of 32 are 8 rows)
+    if (tiles <= 1) return i4_launch<E, GROUPS, 1>(a, st);
+    if constexpr (GROUPS > 1) {
+        if (tiles > 2) return i4_launch<E, GROUPS, 4>(a, st);
+    }
+    return i4_launch<E, GROUPS, 2>(a, st);
 }
 template <class E>
 int i4_groups(const I4Args& a, int group, cudaStream_t st) {

@@ -413,40 +413,40 @@ Tensor clip_grad_norm(at::TensorList grads, double max_norm, double scale, at::T
     TORCH_CHECK(out.empty() || out.size() == grads.size(), who, ": ", std::to_string(grads.size()), " gradients and ", std::to_string(out.size()), " outputs");
     TORCH_CHECK(scale > 0 && scale <= std::numeric_limits<double>::max(), who, ": the scale must be positive and finite");
     TORCH_CHECK(max_norm >= 0, who, ": the largest norm is negative or not a number");
+    check_plain(who);
     const at::Device device = grads[0].device();
     const bool grad_mode = at::GradMode::is_enabled();
-    check_plain(who);
     std::vector<ab_grad> list(grads.size());
-    std::vector<Tensor> dense;                          // copies, kept until the kernels are launched
+    std::vector<Tensor> copies;                         // kept until the kernels are launched
     std::vector<std::pair<size_t, Tensor>> back;        // outputs that are copied to where they belong
+    auto fits = [&](const Tensor& t) {
+        return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.device() == device && is_known(t) && t.has_storage() && !t._fw_grad(/*level=*/0).defined();
+    };
     at::AutoDispatchBelowADInplaceOrView below;
-    for (size_t i = 0; i < grads.size(); ++i) {
+    for (size_t i = 0; i < grads.size(); ++i) {   // (a model has hundreds of them: what each needs is kept short)
         const Tensor& g = grads[i];
-        TORCH_CHECK(g.defined() && g.is_cuda() && g.layout() == at::kStrided && g.device() == device && is_known(g), who, ": gradient ", std::to_string(i),
-                    " is not a dense fp16, bf16 or fp32 tensor on the device of the first");
-        check_plain(who, g);
-        Tensor from = g, to;
-        const bool in_order = g.is_non_overlapping_and_dense();
-        if (!out.empty()) {
-            const Tensor& o = out[i];
-            TORCH_CHECK(o.defined() && o.is_cuda() && o.layout() == at::kStrided && o.device() == device && is_known(o) && o.sizes() == g.sizes(), who, ": output ", std::to_string(i),
-                        " is not a dense fp16, bf16 or fp32 tensor of its gradient's shape and device");
-            check_plain(who, o);
-            TORCH_CHECK(!(grad_mode && o.requires_grad()), who, ": output ", std::to_string(i), " requires a gradient; write over it under torch.no_grad()");
-            at::assert_no_internal_overlap(o);
-            if (!in_order || !o.is_non_overlapping_and_dense() || !same_order(g, o)) {
-                from = g.contiguous();
-                to = o.is_contiguous() ? o : at::empty(g.sizes(), o.options());
-                if (!to.is_same(o)) back.emplace_back(i, to);
-            } else {
-                to = o;
-            }
-            if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
-        } else if (!in_order) {
-            from = g.contiguous();
+        TORCH_CHECK(fits(g), who, ": gradient ", std::to_string(i), " is not a dense fp16, bf16 or fp32 tensor on the device of the first");
+        ab_grad& e = list[i];
+        e = {g.data_ptr(), nullptr, g.numel(), type_of(g), AB_DT_F16};
+        const bool dense = g.is_non_overlapping_and_dense();
+        if (out.empty()) {
+            if (!dense) e.g = copies.emplace_back(g.contiguous()).data_ptr();
+            continue;
         }
-        if (!from.is_same(g)) dense.push_back(from);
-        list[i] = {from.data_ptr(), ptr(to), from.numel(), type_of(from), to.defined() ? type_of(to) : 0};
+        const Tensor& o = out[i];
+        const bool in_place = o.is_same(g);
+        TORCH_CHECK(in_place || (fits(o) && o.sizes() == g.sizes()), who, ": output ", std::to_string(i), " is not a dense fp16, bf16 or fp32 tensor of its gradient's shape and device");
+        TORCH_CHECK(!(grad_mode && o.requires_grad()), who, ": output ", std::to_string(i), " requires a gradient; write over it under torch.no_grad()");
+        if (dense && (in_place || (o.is_non_overlapping_and_dense() && same_order(g, o)))) {
+            e.out = o.data_ptr();
+        } else {
+            at::assert_no_internal_overlap(o);
+            e.g = copies.emplace_back(g.contiguous()).data_ptr();
+            if (!in_place && o.is_contiguous()) e.out = o.data_ptr();
+            else e.out = back.emplace_back(i, at::empty(g.sizes(), o.options())).second.data_ptr();
+        }
+        e.out_dtype = type_of(o);
+        if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
     }
     const c10::cuda::CUDAGuard guard(device);
     Tensor norm = like({}, grads[0], at::kFloat), scratch = like({(int64_t)lib.ab_clip_grad_norm_scratch_bytes((int64_t)list.size())}, grads[0], at::kByte);

@@ -1,18 +1,20 @@
 // Products of a few rows with 4-bit weights in groups:   y[m, n] = sum_k x[m, k] (q[n, k] - z[n, k / G]) s[n, k / G]
 //
-// What bounds it: reading the codes, half a byte each, and their scales. A warp takes 16 outputs (rows of the matrix) and 128 inputs at a time, a chunk:
-// a lane loads 16 bytes of two rows, 32 consecutive codes of each, straight into registers, four chunks ahead (64 KB per SM in flight), and turns
-// them into exact fp16 or bf16 by setting them into the last places of a constant and taking that and the zero point away, one operation for two codes
-// each. What a lane holds is its own share of the inner indices of eight MMAs (m16n8k16); x lies in shared memory in the order in which the
-// codes fall out of their words, 16 bytes for each word.
+// What bounds it: reading the codes, half a byte each, and their scales. Every warp streams pieces of its own, 32 outputs (rows of the matrix) by 256 inputs, into
+// a ring in shared memory (TMA, 4 KB, 128 to 192 KB per SM in flight); nobody else is waited for until a tile of 32 outputs is done. It turns codes into exact
+// fp16 or bf16 by setting them into the last places of a constant and taking that and the zero point away, one operation each for two codes. A lane's 16
+// bytes of a row, 32 codes, are its own share of the inner indices of eight MMAs (m16n8k16); x lies in shared memory in the order in which codes fall
+// out of their words, 16 bytes for each word.
 // An MMA adds up over four lanes, which hold 128 inputs, and those may be of one, two or four groups. Scales are applied to its 32-bit sums, so the groups
-// must not meet in it: of its eight columns, a batch row takes as many as there are groups in a chunk, and in each of them only the lanes
+// must not meet in it: of its eight columns, a batch row takes as many as there are groups in 128 inputs, and in each of them only the lanes
 // of that group have inputs, the others zeros. For one batch row (where seven columns would be idle) this costs nothing.
 //
-// Blocks divide the outputs evenly, to single ones (a tile's rows beyond a block's are not loaded); `kw` warps of a block share a tile's inputs and add their sums in one order. Where
-// the activations do not fit into shared memory, a cluster of `ks` blocks divides the inputs.
+// Blocks divide the outputs evenly, to single ones (the tiles of a block are as high as its share asks for); `kw` warps of a block share a tile's inputs and
+// add their sums in one order. Where the activations do not fit into shared memory, a cluster of `ks` blocks divides the inputs.
+#include <cuda.h>
 #include <cuda_bf16.h>
 
+#include "gemm.cuh"
 #include "train.cuh"
 
 namespace ab {
@@ -20,32 +22,40 @@ namespace ab {
 namespace {
 
 constexpr int I4_WARPS = 16, I4_THREADS = 32 * I4_WARPS;
-__host__ __device__ constexpr int i4_ahead(int groups, int nt) { return nt * groups < 8 ? 4 : 3; }   // chunks in flight per warp (as registers allow)
-constexpr int I4_X_BYTES = 128 * 1024;       // activations of a block at most
-constexpr int I4_BLOCK_TILES = 32;           // tiles of a cluster at most
+constexpr int I4_ROWS = 32, I4_PIECE = I4_ROWS * 128;   // a piece: 128 bytes of up to 32 rows
+constexpr int I4_STAGES = 3;                 // pieces in flight per warp (two where shared memory is needed elsewhere)
+constexpr int I4_SMEM = 225 * 1024;
+constexpr int I4_X_BYTES = 64 * 1024;        // activations of a block at most
+constexpr int I4_BLOCK_SUMS = 16 * 1024;     // sums of the tiles of a cluster's block at most
 
 struct I4Args {
-    const uint8_t *w, *zero;   // zero: null, or a byte per group
+    const uint8_t* zero;       // null, or a byte per group
     const void *scale, *x;
     void* y;
     int64_t x_stride;
     int32_t N, K, rows;
     int32_t groups;            // of a row
-    int32_t per_group;         // chunks of a group (groups of 128 and more; else 1)
+    int32_t per_group;         // chunks (of 128 inputs) of a group (groups of 128 and more; else 1)
+    int32_t pairs;             // two scales next to each other are 4 bytes on their boundary
     int32_t pass;              // batch rows of a block
-    int32_t clusters, ks, kw;
-    int32_t x_bytes;           // shared memory: activations, then the warps' sums, then (ks > 1) the block's
+    int32_t clusters, ks, kw, height, stages;
+    int32_t x_bytes;           // shared memory: activations, then the rings, the warps' sums, and (ks > 1) the block's
 };
 
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {   // one operation (as operators, two immediates made two of it)
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(a), "r"(mask), "r"(bits));
+    return v;
+}
 template <class E> struct I4Type;
 template <> struct I4Type<__half> {
     // two codes each: 0 and 4, 1 and 5, 2 and 6, 3 and 7 of a word
     static __device__ __forceinline__ void codes(uint32_t w, uint32_t (&a)[4]) {
-        a[0] = (w & 0x000f000fu) | 0x64006400u;   // 1024 + q
-        a[1] = (w & 0x00f000f0u) | 0x54005400u;   // 64 + q
+        a[0] = and_or(w, 0x000f000fu, 0x64006400u);   // 1024 + q
+        a[1] = and_or(w, 0x00f000f0u, 0x54005400u);   // 64 + q
         w >>= 8;
-        a[2] = (w & 0x000f000fu) | 0x64006400u;
-        a[3] = (w & 0x00f000f0u) | 0x54005400u;
+        a[2] = and_or(w, 0x000f000fu, 0x64006400u);
+        a[3] = and_or(w, 0x00f000f0u, 0x54005400u);
     }
     static __device__ __forceinline__ void less(uint32_t (&a)[4], uint32_t z) {   // z: the zero point in both halves
         const uint32_t even = z | 0x64006400u, odd = (z << 4) | 0x54005400u;
@@ -68,7 +78,7 @@ template <> struct I4Type<__half> {
 template <> struct I4Type<__nv_bfloat16> {
     static __device__ __forceinline__ void codes(uint32_t w, uint32_t (&a)[4]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;   // 128 + q
+        for (int i = 0; i < 4; ++i) a[i] = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);   // 128 + q
     }
     static __device__ __forceinline__ void less(uint32_t (&a)[4], uint32_t z) {
         const uint32_t t = z | 0x43004300u;
@@ -88,10 +98,9 @@ template <> struct I4Type<__nv_bfloat16> {
     }
 };
 
-__device__ __forceinline__ uint4 i4_load(const uint4* p) {
-    uint4 v;
-    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+__device__ __forceinline__ void i4_tma(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y),
+                 "r"(smem_u32(bar)) : "memory");
 }
 // where `on` is false the registers keep what they have, with no instruction for it
 __device__ __forceinline__ void i4_x(uint4& v, const uint4* p, bool on) {
@@ -106,82 +115,96 @@ __device__ __forceinline__ float i4_peer(const float* own, uint32_t rank) {
 
 // GROUPS: of a chunk (1: groups of 128 or more, 2: of 64, 4: of 32). NT: eights of MMA columns, each 8 / GROUPS batch rows.
 template <class E, int GROUPS, int NT>
-__global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_constant__ I4Args a) {
-    extern __shared__ __align__(16) unsigned char i4_smem[];
+__global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ I4Args a) {
+    extern __shared__ __align__(1024) unsigned char i4_smem[];
+    __shared__ uint64_t full[I4_WARPS][I4_STAGES];
+    __shared__ uint32_t s_nobody;
     using T = I4Type<E>;
-    constexpr int AHEAD = i4_ahead(GROUPS, NT);
-    constexpr int MR = NT * 8 / GROUPS, SCALES = GROUPS == 1 ? 1 : 2;   // batch rows; scales of a lane's two columns
+    constexpr int MR = NT * 8 / GROUPS;            // batch rows
+    constexpr int PAIRS = GROUPS == 1 ? 1 : 2;     // pairs of scales of a lane and row: of the piece's two chunks, or in each of them of its two columns
+    constexpr int MS = NT <= 2 ? 2 : 1;            // halves of a tile that share what is read of the activations (as registers allow)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int cl = (int)blockIdx.x / a.ks, rank = (int)blockIdx.x - cl * a.ks;
-    const int n0 = (int)((int64_t)a.N * cl / a.clusters), n1 = (int)((int64_t)a.N * (cl + 1) / a.clusters), tiles = (n1 - n0 + 15) / 16;
+    const int n0 = (int)((int64_t)a.N * cl / a.clusters), n1 = (int)((int64_t)a.N * (cl + 1) / a.clusters), tiles = (n1 - n0 + a.height - 1) / a.height;
     const int m0 = blockIdx.y * a.pass, rows = min(a.pass, a.rows - m0);
-    const int all_chunks = (a.K + 127) / 128;
-    const int c0 = (int)((int64_t)all_chunks * rank / a.ks), nc = (int)((int64_t)all_chunks * (rank + 1) / a.ks) - c0;   // of this block
+    const int all_pieces = (a.K + 255) / 256;
+    const int c0 = (int)((int64_t)all_pieces * rank / a.ks), nc = (int)((int64_t)all_pieces * (rank + 1) / a.ks) - c0;   // of this block
     const int kw = a.kw, slot = warp / kw, kwi = warp - slot * kw, slots = I4_WARPS / kw;
-    const int lo = nc * kwi / kw, len = nc * (kwi + 1) / kw - lo;                                                     // of this warp
+    const int lo = nc * kwi / kw, len = nc * (kwi + 1) / kw - lo;                                                      // of this warp
     const int rounds = slot < tiles ? (tiles - slot + slots - 1) / slots : 0, total = rounds * len;
-    uint4* sx = reinterpret_cast<uint4*>(i4_smem);
-    float* sums = reinterpret_cast<float*>(i4_smem + a.x_bytes);
+    unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)i4_smem + 1023) & ~(uintptr_t)1023);
+    unsigned char* ring = base + warp * a.stages * I4_PIECE;
+    uint4* sx = reinterpret_cast<uint4*>(base + I4_WARPS * a.stages * I4_PIECE);
+    float* sums = reinterpret_cast<float*>(base + I4_WARPS * a.stages * I4_PIECE + a.x_bytes);
     float* block_sums = sums + I4_WARPS * 16 * MR;
-    const Extent w_all(a.w, (uint64_t)a.N * (a.K / 2)), s_all(a.scale, (uint64_t)a.N * a.groups * sizeof(E)), z_all(a.zero, (uint64_t)a.N * a.groups);
+    const Extent s_all(a.scale, (uint64_t)a.N * a.groups * sizeof(E)), z_all(a.zero, (uint64_t)a.N * a.groups);
+    if (lane == 0) {
+        for (int i = 0; i < a.stages; ++i) mbar_init(&full[warp][i], 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
     pdl_wait();
 
-    // What a chunk needs, in a ring of registers. Addresses are made once for a tile; a chunk is 64 bytes further than the one before.
-    uint4 w[AHEAD][2];
-    E s[AHEAD][2][SCALES];
-    uint32_t z[AHEAD][2];
-    int in_tile = slot, in_c = 0;
-    bool on[2];
-    uint32_t w_at[2], s_at[2];   // in 16 bytes; in groups (32 bits hold them: checked by the launch)
-    const int first = c0 + lo, of_code = GROUPS == 1 ? 0 : t * GROUPS / 4;   // the group, of a chunk, of this lane's codes
-    // where a row ends inside of a chunk: chunks of this warp in which this lane has codes, and (from its columns) scales
-    const int codes_to = GROUPS == 1 ? INT32_MAX : (a.K - t * 32 + 127) / 128 - first;
-    auto open = [&]() {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int n = n0 + in_tile * 16 + h * 8 + g;
-            on[h] = n < n1;
-            const uint32_t row = on[h] ? n : n0;
-            w_at[h] = row * (uint32_t)(a.K / 32) + first * 4 + t;
-            s_at[h] = row * (uint32_t)a.groups + (GROUPS > 1 || a.per_group == 1 ? first * GROUPS : 0);
-        }
+    // The warp's pieces one behind the other, tile after tile; its first lane asks for them, a.stages ahead of the one worked on.
+    int in_i = 0, in_c = 0, in_row = n0 + slot * a.height, in_stage = 0;
+    auto request = [&]() {   // (one lane)
+        if (in_i >= total) return;
+        uint64_t* bar = &full[warp][in_stage];
+        mbar_expect_tx(bar, (uint32_t)a.height * 128u);
+        i4_tma(ring + in_stage * I4_PIECE, &map, (c0 + lo + in_c) * 128, in_row, bar);
+        ++in_i;
+        if (++in_stage == a.stages) in_stage = 0;
+        if (++in_c == len) in_c = 0, in_row += slots * a.height;
     };
-    auto request = [&](uint4 (&w)[2], E (&s)[2][SCALES], uint32_t (&z)[2]) {
-        const int group = GROUPS > 1 || a.per_group == 1 ? in_c * GROUPS : (first + in_c) / a.per_group;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint4* p_w = reinterpret_cast<const uint4*>(a.w) + (w_at[h] + in_c * 4);
-            w[h] = make_uint4(0, 0, 0, 0);
-            if (on[h] && in_c < codes_to && w_all.holds(p_w)) w[h] = i4_load(p_w);
-#pragma unroll
-            for (int i = 0; i < SCALES; ++i) {
-                const int at = group + (SCALES == 1 ? 0 : (2 * t + i) % GROUPS);
-                const E* p = static_cast<const E*>(a.scale) + (s_at[h] + at);
-                s[h][i] = from_f<E>(0.f);
-                if (on[h] && (GROUPS == 1 || first * GROUPS + at < a.groups) && s_all.holds(p)) s[h][i] = __ldg(p);
-            }
-            z[h] = 8;
-            const uint8_t* p_z = a.zero + (s_at[h] + group + of_code);
-            if (a.zero && on[h] && in_c < codes_to && z_all.holds(p_z)) z[h] = __ldg(p_z);
-        }
-        if (++in_c == len) {
-            in_c = 0, in_tile += slots;
-            open();
-        }
-    };
-    open();
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-        if (i < total) request(w[i], s[i], z[i]);
+    if (lane == 0)
+        for (int i = 0; i < a.stages; ++i) request();
 
-    // Activations: 16 bytes for each word of codes, [chunk][word of a lane][batch row][lane's quarter].
+    // Scales and zero points of a piece, in registers, one piece ahead: of rows g, g + 8, g + 16 and g + 24 of the tile.
+    struct Scales {
+        uint32_t s[4][PAIRS], z[4];   // z: of the first chunk, and of the second one in the high half
+    };
+    const int of_code = GROUPS == 1 ? 0 : t * GROUPS / 4;   // the group, of a chunk, of this lane's codes
+    const unsigned short* scale = static_cast<const unsigned short*>(a.scale);
+    auto one_scale = [&](uint32_t at, int group) -> uint32_t { return group < a.groups && s_all.holds(scale + at + group) ? __ldg(scale + at + group) : 0u; };
+    auto one_zero = [&](uint32_t at, int group) -> uint32_t { return group < a.groups && z_all.holds(a.zero + at + group) ? __ldg(a.zero + at + group) : 8u; };
+    auto load_scales = [&](int tile, int c, Scales& v) {
+        const int chunk = 2 * (c0 + lo + c);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int in_tile = r * 8 + g, n = n0 + tile * a.height + in_tile;
+            const bool on = in_tile < a.height && n < n1;
+            const uint32_t at = (uint32_t)n * (uint32_t)a.groups;
+#pragma unroll
+            for (int p = 0; p < PAIRS; ++p) {
+                const int group = GROUPS == 1 ? chunk : (chunk + p) * GROUPS + 2 * t % GROUPS;
+                v.s[r][p] = 0;
+                if (!on) continue;
+                if (a.pairs) {
+                    if (group < a.groups && s_all.holds(scale + at + group, 2)) v.s[r][p] = __ldg(reinterpret_cast<const uint32_t*>(scale + at + group));
+                } else if (a.per_group == 1) {
+                    v.s[r][p] = one_scale(at, group) | one_scale(at, group + 1) << 16;
+                } else {
+                    v.s[r][p] = one_scale(at, chunk / a.per_group) | one_scale(at, (chunk + 1) / a.per_group) << 16;
+                }
+            }
+            v.z[r] = 0x00080008u;
+            if (a.zero && on) {
+                if (a.per_group == 1) v.z[r] = one_zero(at, chunk * GROUPS + of_code) | one_zero(at, (chunk + 1) * GROUPS + of_code) << 16;
+                else v.z[r] = one_zero(at, chunk / a.per_group) | one_zero(at, (chunk + 1) / a.per_group) << 16;
+            }
+        }
+    };
+    Scales cur, next;
+    if (total > 0) load_scales(slot, 0, next);
+
+    // Activations: 16 bytes for each word of codes, [chunk][word of a lane][batch row][lane's quarter]; zeros behind the last input.
     {
         const E* x = static_cast<const E*>(a.x) + (int64_t)m0 * a.x_stride;
         const Extent x_all = rows_extent(a.x, a.rows, a.x_stride, a.K, sizeof(E));
         const bool wide = ((reinterpret_cast<uintptr_t>(x) | (uint64_t)a.x_stride * sizeof(E)) & 15) == 0;
-        for (int i = threadIdx.x; i < nc * 16 * rows; i += I4_THREADS) {
-            const int m = i / (nc * 16), piece = i - m * (nc * 16), c = piece >> 4, quarter = (piece >> 2) & 3, word = piece & 3;
-            const int k = (c0 * 16 + piece) * 8;
+        for (int i = threadIdx.x; i < nc * 32 * rows; i += I4_THREADS) {
+            const int m = i / (nc * 32), eight = i - m * (nc * 32), c = eight >> 4, quarter = (eight >> 2) & 3, word = eight & 3;
+            const int k = (c0 * 32 + eight) * 8;
             const E* p = x + (int64_t)m * a.x_stride + k;
             uint32_t v[4] = {0, 0, 0, 0};
             if (k < a.K && x_all.holds(p, 8)) {
@@ -200,9 +223,11 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     }
     __syncthreads();
 
-    float sum[NT][4];
+    float sum[2][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sum[m][n][0] = sum[m][n][1] = sum[m][n][2] = sum[m][n][3] = 0.f;
     // Where this lane's inputs lie: of its column's batch row, if they are of its column's group; else its registers stay zero. (Columns behind the last batch
     // row read that one's, and nobody reads them.)
     const bool has = GROUPS == 1 || of_code == g % GROUPS;
@@ -210,133 +235,194 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
 #pragma unroll
     for (int n = 0; n < NT; ++n) x_at[n] = sx + min(n * (8 / GROUPS) + g / GROUPS, rows - 1) * 4 + t;
     uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};   // (in turn)
-    auto chunk = [&](const uint4 (&w)[2], const E (&s)[2][SCALES], const uint32_t (&z)[2], int c) {
-        float d[NT][4];
-        const uint32_t zl = z[0] * 0x00010001u, zh = z[1] * 0x00010001u;
+    auto low = [](uint32_t v) { return from_bits<E>((unsigned short)v); };
+    auto high = [](uint32_t v) { return from_bits<E>((unsigned short)(v >> 16)); };
+    // (returns a combination of a word of each load from the stage)
+    auto piece = [&](const unsigned char* w, const Scales& v, int c) -> uint32_t {
+        uint32_t used = 0;
 #pragma unroll
-        for (int word = 0; word < 4; ++word) {
-            uint32_t l[4], h[4];
-            T::codes(word == 0 ? w[0].x : word == 1 ? w[0].y : word == 2 ? w[0].z : w[0].w, l);
-            T::codes(word == 0 ? w[1].x : word == 1 ? w[1].y : word == 2 ? w[1].z : w[1].w, h);
-            T::less(l, zl);
-            T::less(h, zh);
+        for (int ch = 0; ch < 2; ++ch) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                uint4& v = x[(word * NT + n) & 1];
-                i4_x(v, x_at[n] + (c * 4 + word) * (rows * 4), has && AB_BC((c * 4 + word + 1) * rows * 64 <= a.x_bytes));
-                if (word == 0) T::first(d[n], l[0], h[0], l[1], h[1], v.x, v.y);
-                else T::mma(d[n], l[0], h[0], l[1], h[1], v.x, v.y);
-                T::mma(d[n], l[2], h[2], l[3], h[3], v.z, v.w);
+            for (int mb = 0; mb < 2; mb += MS) {
+                float d[MS][NT][4];
+                uint4 q[MS][2];
+#pragma unroll
+                for (int m = 0; m < MS; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        q[m][h] = *reinterpret_cast<const uint4*>(w + (16 * (mb + m) + 8 * h + g) * 128 + (((4 * ch + t) ^ g) << 4));
+                        used ^= q[m][h].x;
+                    }
+#pragma unroll
+                for (int word = 0; word < 4; ++word) {
+                    uint32_t l[MS][4], h[MS][4];
+#pragma unroll
+                    for (int m = 0; m < MS; ++m) {
+                        T::codes(word == 0 ? q[m][0].x : word == 1 ? q[m][0].y : word == 2 ? q[m][0].z : q[m][0].w, l[m]);
+                        T::codes(word == 0 ? q[m][1].x : word == 1 ? q[m][1].y : word == 2 ? q[m][1].z : q[m][1].w, h[m]);
+                        const uint32_t zl = v.z[2 * (mb + m)], zh = v.z[2 * (mb + m) + 1];
+                        T::less(l[m], __byte_perm(zl, 0, ch ? 0x3232 : 0x1010));
+                        T::less(h[m], __byte_perm(zh, 0, ch ? 0x3232 : 0x1010));
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        uint4& b = x[(word * NT + n) & 1];
+                        i4_x(b, x_at[n] + ((2 * c + ch) * 4 + word) * (rows * 4), has && AB_BC(((2 * c + ch) * 4 + word + 1) * rows * 64 <= a.x_bytes));
+#pragma unroll
+                        for (int m = 0; m < MS; ++m) {
+                            if (word == 0) T::first(d[m][n], l[m][0], h[m][0], l[m][1], h[m][1], b.x, b.y);
+                            else T::mma(d[m][n], l[m][0], h[m][0], l[m][1], h[m][1], b.x, b.y);
+                            T::mma(d[m][n], l[m][2], h[m][2], l[m][3], h[m][3], b.z, b.w);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < MS; ++m)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t two = v.s[2 * (mb + m) + (e >> 1)][PAIRS == 1 ? 0 : ch];
+                            const bool second = PAIRS == 1 ? ch == 1 : (e & 1) == 1;
+                            sum[mb + m][n][e] = fmaf(to_f(second ? high(two) : low(two)), d[m][n][e], sum[mb + m][n][e]);
+                        }
             }
         }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[n][e] = fmaf(to_f(s[e >> 1][SCALES == 1 ? 0 : e & 1]), d[n][e], sum[n][e]);
+        return used;
     };
     auto store = [&](int n, int m, float v) {
         E* y = static_cast<E*>(a.y) + (int64_t)(m0 + m) * a.N + n;
         if (AB_BC(n >= 0 && n < a.N && m >= 0 && m0 + m < a.rows)) *y = from_f<E>(v);
     };
-    // the tile's sums: [warp][batch row][output]
+    // the tile's sums, half after half: [warp][batch row][output]
     auto finish = [&](int tile) {
         auto meet = [&]() {
             if (kw == 1) __syncwarp();
             else asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(kw * 32) : "memory");
         };
-        meet();   // the tile before has been read
         float* own = sums + warp * (16 * MR);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (GROUPS == 1) {
-                    own[(n * 8 + 2 * t) * 16 + g + 8 * h] = sum[n][2 * h];
-                    own[(n * 8 + 2 * t + 1) * 16 + g + 8 * h] = sum[n][2 * h + 1];
-                } else {
-                    float v = sum[n][2 * h] + sum[n][2 * h + 1];
-                    if (GROUPS == 4) v += __shfl_xor_sync(0xffffffffu, v, 1);
-                    if (GROUPS == 2 || (t & 1) == 0) own[(n * (8 / GROUPS) + 2 * t / GROUPS) * 16 + g + 8 * h] = v;
-                }
-                sum[n][2 * h] = sum[n][2 * h + 1] = 0.f;
-            }
-        }
-        meet();
         const float* first = sums + slot * kw * (16 * MR);
-        for (int e = kwi * 32 + lane; e < 16 * rows; e += kw * 32) {
-            float v = 0.f;
-            for (int i = 0; i < kw; ++i) v += first[i * (16 * MR) + e];
-            const int n = n0 + tile * 16 + (e & 15), m = e >> 4;
-            if (a.ks > 1) block_sums[tile * (16 * MR) + e] = v;
-            else if (n < n1) store(n, m, v);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (half * 16 < a.height) {
+                meet();   // what was there before has been read
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float l = sum[half][n][2 * h], r = sum[half][n][2 * h + 1];
+                        if (GROUPS == 1) {
+                            own[(n * 8 + 2 * t) * 16 + g + 8 * h] = l;
+                            own[(n * 8 + 2 * t + 1) * 16 + g + 8 * h] = r;
+                        } else {
+                            float v = l + r;
+                            if (GROUPS == 4) v += __shfl_xor_sync(0xffffffffu, v, 1);
+                            if (GROUPS == 2 || (t & 1) == 0) own[(n * (8 / GROUPS) + 2 * t / GROUPS) * 16 + g + 8 * h] = v;
+                        }
+                    }
+                }
+                meet();
+                for (int e = kwi * 32 + lane; e < 16 * rows; e += kw * 32) {
+                    float v = 0.f;
+                    for (int i = 0; i < kw; ++i) v += first[i * (16 * MR) + e];
+                    const int in_tile = half * 16 + (e & 15), n = n0 + tile * a.height + in_tile;
+                    if (in_tile >= a.height || n >= n1) continue;
+                    if (a.ks > 1) block_sums[(tile * MR + (e >> 4)) * I4_ROWS + in_tile] = v;
+                    else store(n, e >> 4, v);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sum[half][n][0] = sum[half][n][1] = sum[half][n][2] = sum[half][n][3] = 0.f;
         }
     };
-    int tile = slot, c = 0;
-    if (len == 0)   // (fewer chunks than warps of a tile: this one adds zeros)
+    bool failed = false;
+    int tile = slot, c = 0, stage = 0;
+    uint32_t parity = 0;
+    if (len == 0)   // (fewer pieces than warps of a tile: this one adds zeros)
         for (int i = 0; i < rounds; ++i) finish(slot + i * slots);
-    for (int i = 0; i < total; i += AHEAD) {
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            if (i + j < total) {
-                chunk(w[j], s[j], z[j], lo + c);
-                if (i + j + AHEAD < total) request(w[j], s[j], z[j]);
-                if (++c == len) {
-                    finish(tile);
-                    c = 0, tile += slots;
-                }
-            }
-        }
+    for (int i = 0; i < total; ++i) {
+        cur = next;
+        const bool last = c + 1 == len;
+        if (i + 1 < total) load_scales(last ? tile + slots : tile, last ? 0 : c + 1, next);
+        if (!failed && !mbar_wait_bounded(&full[warp][stage], parity, 1u << 16)) failed = true;
+        const uint32_t used = piece(ring + stage * I4_PIECE, cur, lo + c);
+        loads_returned(used, &s_nobody);
+        __syncwarp();   // every lane has read the stage
+        if (lane == 0 && !failed) request();
+        if (++stage == a.stages) stage = 0, parity ^= 1u;
+        if (last) finish(tile), tile += slots;
+        c = last ? 0 : c + 1;
     }
     if (a.ks > 1) {   // the blocks of a cluster finish its tiles in turn
         asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
         for (int i = rank; i < tiles; i += a.ks)
-            for (int e = threadIdx.x; e < 16 * rows; e += I4_THREADS) {
+            for (int e = threadIdx.x; e < I4_ROWS * rows; e += I4_THREADS) {
+                const int in_tile = e % I4_ROWS, n = n0 + i * a.height + in_tile;
+                if (in_tile >= a.height || n >= n1) continue;
                 float v = 0.f;
-                for (int r = 0; r < a.ks; ++r) v += i4_peer(block_sums + i * (16 * MR) + e, (uint32_t)r);
-                const int n = n0 + i * 16 + (e & 15);
-                if (n < n1) store(n, e >> 4, v);
+                for (int r = 0; r < a.ks; ++r) v += i4_peer(block_sums + i * MR * I4_ROWS + e, (uint32_t)r);
+                store(n, e / I4_ROWS, v);
             }
         asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    if (failed) {   // (copies on their way still find their shared memory)
+        if (lane == 0) atomicOr(&g_device_status, DEV_WAIT_GEMM);
+        for (int i = 0; i < 100; ++i) __nanosleep(1000);
     }
 }
 
 template <class E, int GROUPS, int NT>
-int i4_launch(I4Args a, cudaStream_t st) {
-    constexpr int MR = NT * 8 / GROUPS, MOST = I4_X_BYTES + (I4_WARPS + I4_BLOCK_TILES) * 16 * MR * 4;
-    static_assert(MOST <= 227 * 1024, "shared memory of the 4-bit products");
+int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
+    constexpr int MR = NT * 8 / GROUPS, SUMS = I4_WARPS * 16 * MR * 4;
+    static_assert(1024 + 2 * I4_WARPS * I4_PIECE + I4_X_BYTES + SUMS + I4_BLOCK_SUMS <= I4_SMEM, "shared memory of the 4-bit products");
     static PerDeviceOnce once;
     const DeviceProps* dev;
     const auto kernel = int4_rows_kernel<E, GROUPS, NT>;
-    const int err = once.run(&dev, [&](const DeviceProps& d) -> int {
-        AB_CHECK_ARG(d.smem_optin >= (size_t)MOST, "linear_int4: %zu bytes of shared memory per block are too few", d.smem_optin);
-        return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST), "cudaFuncSetAttribute(linear_int4)");
+    const int err = once.run(&dev, [&](const DeviceProps&) -> int {
+        return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, I4_SMEM), "cudaFuncSetAttribute(linear_int4)");
     });
     if (err != OK) return err;
     AB_CHECK_ARG((int64_t)a.N * (a.K / 32) < UINT32_MAX, "linear_int4: a matrix of %d x %d is too large", a.N, a.K);
-    const int chunks = (a.K + 127) / 128;
+    const int pieces = (a.K + 255) / 256;
     a.pass = MR < a.rows ? MR : a.rows;
     a.ks = 1;
-    while ((int64_t)((chunks + a.ks - 1) / a.ks) * 256 * a.pass > I4_X_BYTES) {
+    while ((int64_t)((pieces + a.ks - 1) / a.ks) * 512 * a.pass > I4_X_BYTES) {
         if (a.ks < 8) a.ks *= 2;
         else if (a.pass > 1) a.pass = (a.pass + 1) / 2;
         else AB_CHECK_ARG(false, "linear_int4: %d inputs are too many", a.K);
     }
-    const int nc = (chunks + a.ks - 1) / a.ks;
-    a.x_bytes = nc * 256 * a.pass;
-    const int fit = dev->n_sm / a.ks;
+    const int nc = (pieces + a.ks - 1) / a.ks;
+    a.x_bytes = nc * 512 * a.pass;
+    const int fit = dev->n_sm / a.ks, most = I4_BLOCK_SUMS / (I4_ROWS * MR * 4) * I4_ROWS;   // outputs of a cluster's block at most
     a.clusters = a.N < fit ? a.N : fit;
-    if (a.ks > 1 && (a.N + a.clusters - 1) / a.clusters > 16 * I4_BLOCK_TILES) a.clusters = (a.N + 16 * I4_BLOCK_TILES - 1) / (16 * I4_BLOCK_TILES);
-    // warps that share a tile: the fewest rounds of chunks, a tile's end counted as two of them
-    const int tiles = ((a.N + a.clusters - 1) / a.clusters + 15) / 16;
+    if (a.ks > 1 && (a.N + a.clusters - 1) / a.clusters > most) a.clusters = (a.N + most - 1) / most;
+    const int share = (a.N + a.clusters - 1) / a.clusters, tiles = (share + I4_ROWS - 1) / I4_ROWS;
+    a.height = (share + tiles - 1) / tiles;
+    // warps that share a tile: the fewest rounds of pieces, a tile's end counted as one
     int best = 0;
     for (int kw = I4_WARPS; kw >= 1; kw /= 2) {
-        const int slots = I4_WARPS / kw, cost = (tiles + slots - 1) / slots * ((nc + kw - 1) / kw + 2);
+        const int slots = I4_WARPS / kw, cost = (tiles + slots - 1) / slots * ((nc + kw - 1) / kw + 1);
         if (best == 0 || cost < best) best = cost, a.kw = kw;
+    }
+    const int rest = I4_SMEM - 1024 - a.x_bytes - SUMS - (a.ks > 1 ? tiles * I4_ROWS * MR * 4 : 0);
+    a.stages = rest / (I4_WARPS * I4_PIECE) < I4_STAGES ? rest / (I4_WARPS * I4_PIECE) : I4_STAGES;
+    a.pairs = a.per_group == 1 && a.groups % 2 == 0 && (reinterpret_cast<uintptr_t>(a.scale) & 3) == 0;
+    EncodeTiledFn encode;
+    const int found = get_encode_fn(&encode);
+    if (found != OK) return found;
+    CUtensorMap map;
+    const cuuint64_t dim[2] = {(cuuint64_t)a.K / 2, (cuuint64_t)a.N}, pitch[1] = {(cuuint64_t)a.K / 2};
+    const cuuint32_t box[2] = {128, (cuuint32_t)a.height}, step[2] = {1, 1};
+    const CUresult cr = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dim, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS) {
+        set_error("linear_int4: cuTensorMapEncodeTiled failed with %d (%d x %d)", (int)cr, a.N, a.K);
+        return ERR_CUDA;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.clusters * a.ks, (a.rows + a.pass - 1) / a.pass);
     cfg.blockDim = dim3(I4_THREADS);
-    cfg.dynamicSmemBytes = a.x_bytes + (I4_WARPS + (a.ks > 1 ? tiles : 0)) * 16 * MR * 4;
+    cfg.dynamicSmemBytes = 1024 + a.stages * I4_WARPS * I4_PIECE + a.x_bytes + SUMS + (a.ks > 1 ? tiles * I4_ROWS * MR * 4 : 0);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -346,31 +432,31 @@ int i4_launch(I4Args a, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = a.ks > 1 ? 2 : 1;
-    AB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+    AB_CUDA(cudaLaunchKernelEx(&cfg, kernel, map, a));
     return OK;
 }
 template <class E, int GROUPS>
-int i4_columns(const I4Args& a, cudaStream_t st) {
+int i4_columns(const void* codes, const I4Args& a, cudaStream_t st) {
     const int tiles = (a.rows * GROUPS + 7) / 8;
     // (16 batch rows are two eights in groups of 128, and four in groups of 64; four in groups of 32 are 8 rows)
-    if (tiles <= 1) return i4_launch<E, GROUPS, 1>(a, st);
+    if (tiles <= 1) return i4_launch<E, GROUPS, 1>(codes, a, st);
     if constexpr (GROUPS > 1) {
-        if (tiles > 2) return i4_launch<E, GROUPS, 4>(a, st);
+        if (tiles > 2) return i4_launch<E, GROUPS, 4>(codes, a, st);
     }
-    return i4_launch<E, GROUPS, 2>(a, st);
+    return i4_launch<E, GROUPS, 2>(codes, a, st);
 }
 template <class E>
-int i4_groups(const I4Args& a, int group, cudaStream_t st) {
-    return group == 32 ? i4_columns<E, 4>(a, st) : group == 64 ? i4_columns<E, 2>(a, st) : i4_columns<E, 1>(a, st);
+int i4_groups(const void* codes, const I4Args& a, int group, cudaStream_t st) {
+    return group == 32 ? i4_columns<E, 4>(codes, a, st) : group == 64 ? i4_columns<E, 2>(codes, a, st) : i4_columns<E, 1>(codes, a, st);
 }
 
 }  // namespace
 
 int linear_int4(const ab_int4& m, int rows, const void* x, int64_t x_stride, void* y, cudaStream_t st) {
     I4Args a = {};
-    a.w = static_cast<const uint8_t*>(m.w), a.zero = static_cast<const uint8_t*>(m.zero), a.scale = m.scale, a.x = x, a.y = y, a.x_stride = x_stride;
+    a.zero = static_cast<const uint8_t*>(m.zero), a.scale = m.scale, a.x = x, a.y = y, a.x_stride = x_stride;
     a.N = m.n_out, a.K = m.k, a.rows = rows, a.groups = m.k / m.group, a.per_group = m.group > 128 ? m.group / 128 : 1;
-    return m.dtype == AB_DT_F16 ? i4_groups<__half>(a, m.group, st) : i4_groups<__nv_bfloat16>(a, m.group, st);
+    return m.dtype == AB_DT_F16 ? i4_groups<__half>(m.w, a, m.group, st) : i4_groups<__nv_bfloat16>(m.w, a, m.group, st);
 }
 
 }  // namespace ab

@@ -39,6 +39,10 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+template <class E> __device__ __forceinline__ E from_bits(unsigned short v);
+template <> __device__ __forceinline__ __half from_bits<__half>(unsigned short v) { return __ushort_as_half(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_bits<__nv_bfloat16>(unsigned short v) { return __ushort_as_bfloat16(v); }
+
 // 16 bytes of values
 template <class E> __device__ __forceinline__ void unpack(const uint4& u, float* f);
 template <> __device__ __forceinline__ void unpack<float>(const uint4& u, float* f) {

@@ -103,9 +103,8 @@ __device__ __forceinline__ void i4_tma(void* dst, const CUtensorMap* map, int x,
                  "r"(smem_u32(bar)) : "memory");
 }
 // where `on` is false the registers keep what they have, with no instruction for it
-__device__ __forceinline__ void i4_x(uint4& v, const uint4* p, bool on) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n @p ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
-                 : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w) : "r"(smem_u32(p)), "r"((uint32_t)on) : "memory");
+__device__ __forceinline__ void i4_x(uint4& v, uint32_t p, uint32_t on) {
+    asm("{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n @p ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n}" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w) : "r"(p), "r"(on));
 }
 __device__ __forceinline__ float i4_peer(const float* own, uint32_t rank) {
     float v;
@@ -114,7 +113,7 @@ __device__ __forceinline__ float i4_peer(const float* own, uint32_t rank) {
 }
 
 // GROUPS: of a chunk (1: groups of 128 or more, 2: of 64, 4: of 32). NT: eights of MMA columns, each 8 / GROUPS batch rows.
-template <class E, int GROUPS, int NT>
+template <class E, int GROUPS, int NT, bool ZERO>
 __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ I4Args a) {
     extern __shared__ __align__(1024) unsigned char i4_smem[];
     __shared__ uint64_t full[I4_WARPS][I4_STAGES];
@@ -159,43 +158,53 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     if (lane == 0)
         for (int i = 0; i < a.stages; ++i) request();
 
-    // Scales and zero points of a piece, in registers, one piece ahead: of rows g, g + 8, g + 16 and g + 24 of the tile.
+    // Scales and zero points of a piece, in registers, one piece ahead: of rows g, g + 8, g + 16 and g + 24 of the tile. Rows behind the tile's, whose sums nobody
+    // reads, take the last one's, and so do groups behind a row's, whose inputs are zeros.
     struct Scales {
-        uint32_t s[4][PAIRS], z[4];   // z: of the first chunk, and of the second one in the high half
+        uint32_t s[4][PAIRS], z[ZERO ? 4 : 1];   // z: of the first chunk, and of the second one in the high half
     };
     const int of_code = GROUPS == 1 ? 0 : t * GROUPS / 4;   // the group, of a chunk, of this lane's codes
     const unsigned short* scale = static_cast<const unsigned short*>(a.scale);
-    auto one_scale = [&](uint32_t at, int group) -> uint32_t { return group < a.groups && s_all.holds(scale + at + group) ? __ldg(scale + at + group) : 0u; };
-    auto one_zero = [&](uint32_t at, int group) -> uint32_t { return group < a.groups && z_all.holds(a.zero + at + group) ? __ldg(a.zero + at + group) : 8u; };
-    auto load_scales = [&](int tile, int c, Scales& v) {
-        const int chunk = 2 * (c0 + lo + c);
+    uint32_t s_row[4];
+    auto scale_rows = [&](int tile) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int in_tile = r * 8 + g, n = n0 + tile * a.height + in_tile;
-            const bool on = in_tile < a.height && n < n1;
-            const uint32_t at = (uint32_t)n * (uint32_t)a.groups;
+        for (int r = 0; r < 4; ++r) s_row[r] = (uint32_t)min(n0 + tile * a.height + r * 8 + g, n1 - 1) * (uint32_t)a.groups;
+    };
+    auto load_scales = [&](int c, Scales& v) {
+        const int chunk = 2 * (c0 + lo + c), last = a.groups - 1;
+        if (a.pairs) {
 #pragma unroll
             for (int p = 0; p < PAIRS; ++p) {
-                const int group = GROUPS == 1 ? chunk : (chunk + p) * GROUPS + 2 * t % GROUPS;
-                v.s[r][p] = 0;
-                if (!on) continue;
-                if (a.pairs) {
-                    if (group < a.groups && s_all.holds(scale + at + group, 2)) v.s[r][p] = __ldg(reinterpret_cast<const uint32_t*>(scale + at + group));
-                } else if (a.per_group == 1) {
-                    v.s[r][p] = one_scale(at, group) | one_scale(at, group + 1) << 16;
-                } else {
-                    v.s[r][p] = one_scale(at, chunk / a.per_group) | one_scale(at, (chunk + 1) / a.per_group) << 16;
+                const int group = min(GROUPS == 1 ? chunk : (chunk + p) * GROUPS + 2 * t % GROUPS, last - 1);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v.s[r][p] = s_all.holds(scale + s_row[r] + group, 2) ? __ldg(reinterpret_cast<const uint32_t*>(scale + (s_row[r] + group))) : 0u;
+            }
+        } else {
+#pragma unroll 1
+            for (int p = 0; p < PAIRS; ++p) {
+                const int first = GROUPS == 1 ? chunk / a.per_group : (chunk + p) * GROUPS + 2 * t % GROUPS, second = GROUPS == 1 ? (chunk + 1) / a.per_group : first + 1;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const unsigned short *l = scale + s_row[r] + min(first, last), *h = scale + s_row[r] + min(second, last);
+                    const uint32_t two = s_all.holds(l) && s_all.holds(h) ? __ldg(l) | (uint32_t)__ldg(h) << 16 : 0u;
+                    if (p == 0) v.s[r][0] = two;
+                    else v.s[r][PAIRS - 1] = two;
                 }
             }
-            v.z[r] = 0x00080008u;
-            if (a.zero && on) {
-                if (a.per_group == 1) v.z[r] = one_zero(at, chunk * GROUPS + of_code) | one_zero(at, (chunk + 1) * GROUPS + of_code) << 16;
-                else v.z[r] = one_zero(at, chunk / a.per_group) | one_zero(at, (chunk + 1) / a.per_group) << 16;
+        }
+        if (ZERO) {
+            const int l = min(GROUPS == 1 ? (a.per_group == 1 ? chunk : chunk / a.per_group) : chunk * GROUPS + of_code, last);
+            const int h = min(GROUPS == 1 ? (a.per_group == 1 ? chunk + 1 : (chunk + 1) / a.per_group) : (chunk + 1) * GROUPS + of_code, last);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint8_t *zl = a.zero + (s_row[r] + l), *zh = a.zero + (s_row[r] + h);
+                v.z[r] = z_all.holds(zl) && z_all.holds(zh) ? __ldg(zl) | (uint32_t)__ldg(zh) << 16 : 0u;
             }
         }
     };
     Scales cur, next;
-    if (total > 0) load_scales(slot, 0, next);
+    scale_rows(slot);
+    if (total > 0) load_scales(0, next);
 
     // Activations: 16 bytes for each word of codes, [chunk][word of a lane][batch row][lane's quarter]; zeros behind the last input.
     {
@@ -231,17 +240,23 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     // Where this lane's inputs lie: of its column's batch row, if they are of its column's group; else its registers stay zero. (Columns behind the last batch
     // row read that one's, and nobody reads them.)
     const bool has = GROUPS == 1 || of_code == g % GROUPS;
-    const uint4* x_at[NT];
+    uint32_t x_at[NT];   // (defined behind the barrier: what reads through them cannot be moved in front of it)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) x_at[n] = sx + min(n * (8 / GROUPS) + g / GROUPS, rows - 1) * 4 + t;
+    for (int n = 0; n < NT; ++n) {
+        x_at[n] = smem_u32(sx + min(n * (8 / GROUPS) + g / GROUPS, rows - 1) * 4 + t);
+        asm volatile("" : "+r"(x_at[n])::"memory");
+    }
     uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};   // (in turn)
+    const uint32_t has_it = has, x_word = rows * 64;
     auto low = [](uint32_t v) { return from_bits<E>((unsigned short)v); };
     auto high = [](uint32_t v) { return from_bits<E>((unsigned short)(v >> 16)); };
-    // (returns a combination of a word of each load from the stage)
-    auto piece = [&](const unsigned char* w, const Scales& v, int c) -> uint32_t {
-        uint32_t used = 0;
-#pragma unroll
-        for (int ch = 0; ch < 2; ++ch) {
+    // The piece's two chunks. (Not unrolled: the code of both did not fit the instruction cache's first level.) Returns a combination of a word of each load from the stage.
+    auto piece = [&](const unsigned char* w, Scales& v, int c) -> uint32_t {
+        uint32_t used = 0, x_c = (uint32_t)c * 8 * x_word;
+        const unsigned char* w_at = w + g * 128 + ((t ^ g) << 4);   // (the second chunk's 16 bytes: bit 6 of the address)
+#pragma unroll 1
+        for (int ch = 0; ch < 2; ++ch, x_c += 4 * x_word) {
+            const unsigned char* w_ch = reinterpret_cast<const unsigned char*>(reinterpret_cast<uintptr_t>(w_at) ^ (uintptr_t)(ch * 64));
 #pragma unroll
             for (int mb = 0; mb < 2; mb += MS) {
                 float d[MS][NT][4];
@@ -250,7 +265,7 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
                 for (int m = 0; m < MS; ++m)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        q[m][h] = *reinterpret_cast<const uint4*>(w + (16 * (mb + m) + 8 * h + g) * 128 + (((4 * ch + t) ^ g) << 4));
+                        q[m][h] = *reinterpret_cast<const uint4*>(w_ch + (16 * (mb + m) + 8 * h) * 128);
                         used ^= q[m][h].x;
                     }
 #pragma unroll
@@ -260,14 +275,13 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
                     for (int m = 0; m < MS; ++m) {
                         T::codes(word == 0 ? q[m][0].x : word == 1 ? q[m][0].y : word == 2 ? q[m][0].z : q[m][0].w, l[m]);
                         T::codes(word == 0 ? q[m][1].x : word == 1 ? q[m][1].y : word == 2 ? q[m][1].z : q[m][1].w, h[m]);
-                        const uint32_t zl = v.z[2 * (mb + m)], zh = v.z[2 * (mb + m) + 1];
-                        T::less(l[m], __byte_perm(zl, 0, ch ? 0x3232 : 0x1010));
-                        T::less(h[m], __byte_perm(zh, 0, ch ? 0x3232 : 0x1010));
+                        T::less(l[m], ZERO ? __byte_perm(v.z[ZERO ? 2 * (mb + m) : 0], 0, 0x1010) : 0x00080008u);
+                        T::less(h[m], ZERO ? __byte_perm(v.z[ZERO ? 2 * (mb + m) + 1 : 0], 0, 0x1010) : 0x00080008u);
                     }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         uint4& b = x[(word * NT + n) & 1];
-                        i4_x(b, x_at[n] + ((2 * c + ch) * 4 + word) * (rows * 4), has && AB_BC(((2 * c + ch) * 4 + word + 1) * rows * 64 <= a.x_bytes));
+                        i4_x(b, x_at[n] + x_c + word * x_word, has_it && AB_BC(x_c + (word + 1) * x_word <= (uint32_t)a.x_bytes));
 #pragma unroll
                         for (int m = 0; m < MS; ++m) {
                             if (word == 0) T::first(d[m][n], l[m][0], h[m][0], l[m][1], h[m][1], b.x, b.y);
@@ -282,10 +296,15 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const uint32_t two = v.s[2 * (mb + m) + (e >> 1)][PAIRS == 1 ? 0 : ch];
-                            const bool second = PAIRS == 1 ? ch == 1 : (e & 1) == 1;
-                            sum[mb + m][n][e] = fmaf(to_f(second ? high(two) : low(two)), d[m][n][e], sum[mb + m][n][e]);
+                            const uint32_t two = v.s[2 * (mb + m) + (e >> 1)][0];
+                            sum[mb + m][n][e] = fmaf(to_f(PAIRS == 1 || (e & 1) == 0 ? low(two) : high(two)), d[m][n][e], sum[mb + m][n][e]);
                         }
+            }
+            // the second chunk's
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                v.s[r][0] = PAIRS == 1 ? v.s[r][0] >> 16 : v.s[r][PAIRS - 1];
+                if (ZERO) v.z[ZERO ? r : 0] >>= 16;
             }
         }
         return used;
@@ -343,7 +362,10 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     for (int i = 0; i < total; ++i) {
         cur = next;
         const bool last = c + 1 == len;
-        if (i + 1 < total) load_scales(last ? tile + slots : tile, last ? 0 : c + 1, next);
+        if (i + 1 < total) {
+            if (last) scale_rows(tile + slots);
+            load_scales(last ? 0 : c + 1, next);
+        }
         if (!failed && !mbar_wait_bounded(&full[warp][stage], parity, 1u << 16)) failed = true;
         const uint32_t used = piece(ring + stage * I4_PIECE, cur, lo + c);
         loads_returned(used, &s_nobody);
@@ -371,13 +393,13 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     }
 }
 
-template <class E, int GROUPS, int NT>
+template <class E, int GROUPS, int NT, bool ZERO>
 int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
     constexpr int MR = NT * 8 / GROUPS, SUMS = I4_WARPS * 16 * MR * 4;
     static_assert(1024 + 2 * I4_WARPS * I4_PIECE + I4_X_BYTES + SUMS + I4_BLOCK_SUMS <= I4_SMEM, "shared memory of the 4-bit products");
     static PerDeviceOnce once;
     const DeviceProps* dev;
-    const auto kernel = int4_rows_kernel<E, GROUPS, NT>;
+    const auto kernel = int4_rows_kernel<E, GROUPS, NT, ZERO>;
     const int err = once.run(&dev, [&](const DeviceProps&) -> int {
         return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, I4_SMEM), "cudaFuncSetAttribute(linear_int4)");
     });
@@ -435,15 +457,19 @@ int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
     AB_CUDA(cudaLaunchKernelEx(&cfg, kernel, map, a));
     return OK;
 }
+template <class E, int GROUPS, int NT>
+int i4_zeros(const void* codes, const I4Args& a, cudaStream_t st) {
+    return a.zero ? i4_launch<E, GROUPS, NT, true>(codes, a, st) : i4_launch<E, GROUPS, NT, false>(codes, a, st);
+}
 template <class E, int GROUPS>
 int i4_columns(const void* codes, const I4Args& a, cudaStream_t st) {
     const int tiles = (a.rows * GROUPS + 7) / 8;
     // (16 batch rows are two eights in groups of 128, and four in groups of 64; four in groups of 32 are 8 rows)
-    if (tiles <= 1) return i4_launch<E, GROUPS, 1>(codes, a, st);
+    if (tiles <= 1) return i4_zeros<E, GROUPS, 1>(codes, a, st);
     if constexpr (GROUPS > 1) {
-        if (tiles > 2) return i4_launch<E, GROUPS, 4>(codes, a, st);
+        if (tiles > 2) return i4_zeros<E, GROUPS, 4>(codes, a, st);
     }
-    return i4_launch<E, GROUPS, 2>(codes, a, st);
+    return i4_zeros<E, GROUPS, 2>(codes, a, st);
 }
 template <class E>
 int i4_groups(const void* codes, const I4Args& a, int group, cudaStream_t st) {

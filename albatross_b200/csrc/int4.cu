@@ -9,10 +9,13 @@
 // must not meet in it: of its eight columns, a batch row takes as many as there are groups in 128 inputs, and in each of them only the lanes
 // of that group have inputs, the others zeros. For one batch row (where seven columns would be idle) this costs nothing.
 //
-// Blocks divide the outputs evenly, to single ones (the tiles of a block are as high as its share asks for); `kw` warps of a block share a tile's inputs and
-// add their sums in one order. Where the activations do not fit into shared memory, a cluster of `ks` blocks divides the inputs.
+// Blocks divide the outputs evenly, to single ones (the tiles of a block are as high as its share asks for), and a block's warps its pieces, tile after tile: a warp
+// stores the tiles that it has to itself, leaves its sums of those that it shares in shared memory, and at the end they are added up in one order. Nobody waits before
+// that. Where the activations do not fit into shared memory, a cluster of `ks` blocks divides the inputs.
 #include <cuda.h>
 #include <cuda_bf16.h>
+
+#include <algorithm>
 
 #include "gemm.cuh"
 #include "train.cuh"
@@ -25,8 +28,7 @@ constexpr int I4_WARPS = 16, I4_THREADS = 32 * I4_WARPS;
 constexpr int I4_ROWS = 32, I4_PIECE = I4_ROWS * 128;   // a piece: 128 bytes of up to 32 rows
 constexpr int I4_STAGES = 3;                 // pieces in flight per warp (two where shared memory is needed elsewhere)
 constexpr int I4_SMEM = 225 * 1024;
-constexpr int I4_X_BYTES = 64 * 1024;        // activations of a block at most
-constexpr int I4_BLOCK_SUMS = 16 * 1024;     // sums of the tiles of a cluster's block at most
+constexpr int I4_SHARED = 2 * I4_WARPS;      // sums of shared tiles: a warp's first and its last
 
 struct I4Args {
     const uint8_t* zero;       // null, or a byte per group
@@ -38,8 +40,8 @@ struct I4Args {
     int32_t per_group;         // chunks (of 128 inputs) of a group (groups of 128 and more; else 1)
     int32_t pairs;             // two scales next to each other are 4 bytes on their boundary
     int32_t pass;              // batch rows of a block
-    int32_t clusters, ks, kw, height, stages;
-    int32_t x_bytes;           // shared memory: activations, then the rings, the warps' sums, and (ks > 1) the block's
+    int32_t clusters, ks, height, stages;
+    int32_t x_bytes;           // shared memory: the rings, then activations, the warps' sums, and (ks > 1) those of the block's tiles
 };
 
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {   // one operation (as operators, two immediates made two of it)
@@ -117,9 +119,9 @@ template <class E, int GROUPS, int NT, bool ZERO>
 __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ I4Args a) {
     extern __shared__ __align__(1024) unsigned char i4_smem[];
     __shared__ uint64_t full[I4_WARPS][I4_STAGES];
+    __shared__ int first_tile[I4_WARPS];
     __shared__ uint32_t s_nobody;
     using T = I4Type<E>;
-    constexpr int MR = NT * 8 / GROUPS;            // batch rows
     constexpr int PAIRS = GROUPS == 1 ? 1 : 2;     // pairs of scales of a lane and row: of the piece's two chunks, or in each of them of its two columns
     constexpr int MS = NT <= 2 ? 2 : 1;            // halves of a tile that share what is read of the activations (as registers allow)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -128,32 +130,33 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     const int m0 = blockIdx.y * a.pass, rows = min(a.pass, a.rows - m0);
     const int all_pieces = (a.K + 255) / 256;
     const int c0 = (int)((int64_t)all_pieces * rank / a.ks), nc = (int)((int64_t)all_pieces * (rank + 1) / a.ks) - c0;   // of this block
-    const int kw = a.kw, slot = warp / kw, kwi = warp - slot * kw, slots = I4_WARPS / kw;
-    const int lo = nc * kwi / kw, len = nc * (kwi + 1) / kw - lo;                                                      // of this warp
-    const int rounds = slot < tiles ? (tiles - slot + slots - 1) / slots : 0, total = rounds * len;
+    auto run_of = [&](int w) { return tiles * nc * w / I4_WARPS; };   // pieces through all tiles: a warp's first
+    const int run0 = run_of(warp), total = run_of(warp + 1) - run0;
+    const int tile0 = run0 / nc, in0 = run0 - tile0 * nc;
     unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)i4_smem + 1023) & ~(uintptr_t)1023);
     unsigned char* ring = base + warp * a.stages * I4_PIECE;
     uint4* sx = reinterpret_cast<uint4*>(base + I4_WARPS * a.stages * I4_PIECE);
     float* sums = reinterpret_cast<float*>(base + I4_WARPS * a.stages * I4_PIECE + a.x_bytes);
-    float* block_sums = sums + I4_WARPS * 16 * MR;
+    float* block_sums = sums + I4_SHARED * I4_ROWS * rows;
     const Extent s_all(a.scale, (uint64_t)a.N * a.groups * sizeof(E)), z_all(a.zero, (uint64_t)a.N * a.groups);
     if (lane == 0) {
         for (int i = 0; i < a.stages; ++i) mbar_init(&full[warp][i], 1);
         fence_mbar_init();
+        first_tile[warp] = tile0;
     }
     __syncwarp();
     pdl_wait();
 
     // The warp's pieces one behind the other, tile after tile; its first lane asks for them, a.stages ahead of the one worked on.
-    int in_i = 0, in_c = 0, in_row = n0 + slot * a.height, in_stage = 0;
+    int in_i = 0, in_c = in0, in_row = n0 + tile0 * a.height, in_stage = 0;
     auto request = [&]() {   // (one lane)
         if (in_i >= total) return;
         uint64_t* bar = &full[warp][in_stage];
         mbar_expect_tx(bar, (uint32_t)a.height * 128u);
-        i4_tma(ring + in_stage * I4_PIECE, &map, (c0 + lo + in_c) * 128, in_row, bar);
+        i4_tma(ring + in_stage * I4_PIECE, &map, (c0 + in_c) * 128, in_row, bar);
         ++in_i;
         if (++in_stage == a.stages) in_stage = 0;
-        if (++in_c == len) in_c = 0, in_row += slots * a.height;
+        if (++in_c == nc) in_c = 0, in_row += a.height;
     };
     if (lane == 0)
         for (int i = 0; i < a.stages; ++i) request();
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
         for (int r = 0; r < 4; ++r) s_row[r] = (uint32_t)min(n0 + tile * a.height + r * 8 + g, n1 - 1) * (uint32_t)a.groups;
     };
     auto load_scales = [&](int c, Scales& v) {
-        const int chunk = 2 * (c0 + lo + c), last = a.groups - 1;
+        const int chunk = 2 * (c0 + c), last = a.groups - 1;
         if (a.pairs) {
 #pragma unroll
             for (int p = 0; p < PAIRS; ++p) {
@@ -203,31 +206,41 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
         }
     };
     Scales cur, next;
-    scale_rows(slot);
-    if (total > 0) load_scales(0, next);
+    scale_rows(tile0);
+    if (total > 0) load_scales(in0, next);
 
     // Activations: 16 bytes for each word of codes, [chunk][word of a lane][batch row][lane's quarter]; zeros behind the last input.
     {
         const E* x = static_cast<const E*>(a.x) + (int64_t)m0 * a.x_stride;
         const Extent x_all = rows_extent(a.x, a.rows, a.x_stride, a.K, sizeof(E));
         const bool wide = ((reinterpret_cast<uintptr_t>(x) | (uint64_t)a.x_stride * sizeof(E)) & 15) == 0;
-        for (int i = threadIdx.x; i < nc * 32 * rows; i += I4_THREADS) {
-            const int m = i / (nc * 32), eight = i - m * (nc * 32), c = eight >> 4, quarter = (eight >> 2) & 3, word = eight & 3;
-            const int k = (c0 * 32 + eight) * 8;
-            const E* p = x + (int64_t)m * a.x_stride + k;
-            uint32_t v[4] = {0, 0, 0, 0};
-            if (k < a.K && x_all.holds(p, 8)) {
-                if (wide) {
-                    const uint4 q = *reinterpret_cast<const uint4*>(p);
-                    v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-                } else {
-                    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+        constexpr int AT_ONCE = 4;   // loads of a thread in flight (one after the other 8 rows of 4096 took 3 us)
+        const int eights = nc * 32 * rows;
+        for (int i0 = threadIdx.x; i0 < eights; i0 += AT_ONCE * I4_THREADS) {
+            uint32_t v[AT_ONCE][4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
+            for (int j = 0; j < AT_ONCE; ++j) {
+                const int i = i0 + j * I4_THREADS, m = i / (nc * 32), k = (c0 * 32 + i - m * (nc * 32)) * 8;
+                const E* p = x + (int64_t)m * a.x_stride + k;
+                v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0;
+                if (i < eights && k < a.K && x_all.holds(p, 8)) {
+                    if (wide) {
+                        const uint4 q = *reinterpret_cast<const uint4*>(p);
+                        v[j][0] = q.x, v[j][1] = q.y, v[j][2] = q.z, v[j][3] = q.w;
+                    } else {
+                        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[j][e] = h[2 * e] | (uint32_t)h[2 * e + 1] << 16;
+                    }
                 }
             }
-            sx[(c * 4 + word) * (rows * 4) + m * 4 + quarter] =
-                make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632), __byte_perm(v[1], v[3], 0x5410), __byte_perm(v[1], v[3], 0x7632));
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                const int i = i0 + j * I4_THREADS, m = i / (nc * 32), eight = i - m * (nc * 32), c = eight >> 4, quarter = (eight >> 2) & 3, word = eight & 3;
+                if (i < eights)
+                    sx[(c * 4 + word) * (rows * 4) + m * 4 + quarter] = make_uint4(__byte_perm(v[j][0], v[j][2], 0x5410), __byte_perm(v[j][0], v[j][2], 0x7632),
+                                                                                   __byte_perm(v[j][1], v[j][3], 0x5410), __byte_perm(v[j][1], v[j][3], 0x7632));
+            }
         }
     }
     __syncthreads();
@@ -313,67 +326,70 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
         E* y = static_cast<E*>(a.y) + (int64_t)(m0 + m) * a.N + n;
         if (AB_BC(n >= 0 && n < a.N && m >= 0 && m0 + m < a.rows)) *y = from_f<E>(v);
     };
-    // the tile's sums, half after half: [warp][batch row][output]
-    auto finish = [&](int tile) {
-        auto meet = [&]() {
-            if (kw == 1) __syncwarp();
-            else asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(kw * 32) : "memory");
-        };
-        float* own = sums + warp * (16 * MR);
-        const float* first = sums + slot * kw * (16 * MR);
+    // the sum of an output and batch row goes to its place, or (ks > 1) to the block's sums
+    auto put = [&](int tile, int in_tile, int m, float v) {
+        const int n = n0 + tile * a.height + in_tile;
+        if (in_tile >= a.height || n >= n1) return;
+        if (a.ks > 1) block_sums[(tile * rows + m) * I4_ROWS + in_tile] = v;
+        else store(n, m, v);
+    };
+    auto finish = [&](int tile, bool alone, int at) {
+        float* own = sums + at * I4_ROWS * rows;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            if (half * 16 < a.height) {
-                meet();   // what was there before has been read
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float l = sum[half][n][2 * h], r = sum[half][n][2 * h + 1];
-                        if (GROUPS == 1) {
-                            own[(n * 8 + 2 * t) * 16 + g + 8 * h] = l;
-                            own[(n * 8 + 2 * t + 1) * 16 + g + 8 * h] = r;
-                        } else {
-                            float v = l + r;
-                            if (GROUPS == 4) v += __shfl_xor_sync(0xffffffffu, v, 1);
-                            if (GROUPS == 2 || (t & 1) == 0) own[(n * (8 / GROUPS) + 2 * t / GROUPS) * 16 + g + 8 * h] = v;
-                        }
+                for (int e = 0; e < 4; ++e) {
+                    float v = sum[half][n][e];
+                    sum[half][n][e] = 0.f;
+                    if (GROUPS > 1) {   // the columns of a batch row: this lane's two, and with four groups the next lane's
+                        if (e & 1) continue;
+                        v += sum[half][n][e + 1];
+                        if (GROUPS == 4) v += __shfl_xor_sync(0xffffffffu, v, 1);
+                        if (GROUPS == 4 && (t & 1)) continue;
                     }
-                }
-                meet();
-                for (int e = kwi * 32 + lane; e < 16 * rows; e += kw * 32) {
-                    float v = 0.f;
-                    for (int i = 0; i < kw; ++i) v += first[i * (16 * MR) + e];
-                    const int in_tile = half * 16 + (e & 15), n = n0 + tile * a.height + in_tile;
-                    if (in_tile >= a.height || n >= n1) continue;
-                    if (a.ks > 1) block_sums[(tile * MR + (e >> 4)) * I4_ROWS + in_tile] = v;
-                    else store(n, e >> 4, v);
+                    const int m = GROUPS == 1 ? n * 8 + 2 * t + (e & 1) : n * (8 / GROUPS) + 2 * t / GROUPS, in_tile = half * 16 + g + 8 * (e >> 1);
+                    if (m >= rows) continue;
+                    if (alone) put(tile, in_tile, m, v);
+                    else own[m * I4_ROWS + in_tile] = v;
                 }
             }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) sum[half][n][0] = sum[half][n][1] = sum[half][n][2] = sum[half][n][3] = 0.f;
-        }
     };
     bool failed = false;
-    int tile = slot, c = 0, stage = 0;
+    int tile = tile0, c = in0, stage = 0;
     uint32_t parity = 0;
-    if (len == 0)   // (fewer pieces than warps of a tile: this one adds zeros)
-        for (int i = 0; i < rounds; ++i) finish(slot + i * slots);
     for (int i = 0; i < total; ++i) {
         cur = next;
-        const bool last = c + 1 == len;
+        const bool last = c + 1 == nc;
         if (i + 1 < total) {
-            if (last) scale_rows(tile + slots);
+            if (last) scale_rows(tile + 1);
             load_scales(last ? 0 : c + 1, next);
         }
         if (!failed && !mbar_wait_bounded(&full[warp][stage], parity, 1u << 16)) failed = true;
-        const uint32_t used = piece(ring + stage * I4_PIECE, cur, lo + c);
+        const uint32_t used = piece(ring + stage * I4_PIECE, cur, c);
         loads_returned(used, &s_nobody);
         __syncwarp();   // every lane has read the stage
         if (lane == 0 && !failed) request();
         if (++stage == a.stages) stage = 0, parity ^= 1u;
-        if (last) finish(tile), tile += slots;
+        if (last || i + 1 == total) {   // alone: all of the tile's pieces were this warp's
+            finish(tile, last && i + 1 >= nc, 2 * warp + (tile != tile0));
+            ++tile;
+        }
         c = last ? 0 : c + 1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < tiles * rows * I4_ROWS; i += I4_THREADS) {   // the tiles that warps share
+        const int tile = i / (rows * I4_ROWS), e = i - tile * (rows * I4_ROWS);
+        // warps w with a part of it: those from the last that begins at its first piece or before, on
+        int w = tile * I4_WARPS / tiles;
+        while (w > 0 && run_of(w) > tile * nc) --w;
+        while (run_of(w + 1) <= tile * nc) ++w;
+        if (run_of(w) <= tile * nc && run_of(w + 1) >= (tile + 1) * nc) continue;   // (it has all of it, and has stored it)
+        float v = 0.f;
+        for (; w < I4_WARPS && run_of(w) < (tile + 1) * nc; ++w)
+            if (run_of(w) < run_of(w + 1)) v += sums[(2 * w + (tile != first_tile[w])) * I4_ROWS * rows + e];   // (with fewer pieces than warps some have none)
+        put(tile, e % I4_ROWS, e / I4_ROWS, v);
     }
     if (a.ks > 1) {   // the blocks of a cluster finish its tiles in turn
         asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -382,7 +398,7 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
                 const int in_tile = e % I4_ROWS, n = n0 + i * a.height + in_tile;
                 if (in_tile >= a.height || n >= n1) continue;
                 float v = 0.f;
-                for (int r = 0; r < a.ks; ++r) v += i4_peer(block_sums + i * MR * I4_ROWS + e, (uint32_t)r);
+                for (int r = 0; r < a.ks; ++r) v += i4_peer(block_sums + i * rows * I4_ROWS + e, (uint32_t)r);
                 store(n, e / I4_ROWS, v);
             }
         asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -395,8 +411,7 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
 
 template <class E, int GROUPS, int NT, bool ZERO>
 int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
-    constexpr int MR = NT * 8 / GROUPS, SUMS = I4_WARPS * 16 * MR * 4;
-    static_assert(1024 + 2 * I4_WARPS * I4_PIECE + I4_X_BYTES + SUMS + I4_BLOCK_SUMS <= I4_SMEM, "shared memory of the 4-bit products");
+    constexpr int MR = NT * 8 / GROUPS, ROOM = I4_SMEM - 1024 - 2 * I4_WARPS * I4_PIECE;   // beside two stages
     static PerDeviceOnce once;
     const DeviceProps* dev;
     const auto kernel = int4_rows_kernel<E, GROUPS, NT, ZERO>;
@@ -407,27 +422,27 @@ int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
     AB_CHECK_ARG((int64_t)a.N * (a.K / 32) < UINT32_MAX, "linear_int4: a matrix of %d x %d is too large", a.N, a.K);
     const int pieces = (a.K + 255) / 256;
     a.pass = MR < a.rows ? MR : a.rows;
-    a.ks = 1;
-    while ((int64_t)((pieces + a.ks - 1) / a.ks) * 512 * a.pass > I4_X_BYTES) {
+    int tiles = 0, shared = 0;   // of a block; shared memory behind the activations
+    for (a.ks = 1;;) {
+        const int64_t x_bytes = (int64_t)((pieces + a.ks - 1) / a.ks) * 512 * a.pass;
+        const int tile_bytes = I4_ROWS * a.pass * 4;
+        if (x_bytes + (I4_SHARED + (a.ks > 1 ? 8 : 0)) * tile_bytes <= ROOM) {
+            const int fit = dev->n_sm / a.ks, most = (int)((ROOM - x_bytes) / tile_bytes - I4_SHARED) * I4_ROWS;   // outputs whose sums fit (ks > 1)
+            a.x_bytes = (int)x_bytes;
+            a.clusters = a.N < fit ? a.N : fit;
+            if (a.ks > 1 && (a.N + a.clusters - 1) / a.clusters > most) a.clusters = (a.N + most - 1) / most;
+            const int share = (a.N + a.clusters - 1) / a.clusters;
+            tiles = (share + I4_ROWS - 1) / I4_ROWS;
+            a.height = (share + tiles - 1) / tiles;
+            shared = (I4_SHARED + (a.ks > 1 ? tiles : 0)) * tile_bytes;
+            break;
+        }
         if (a.ks < 8) a.ks *= 2;
         else if (a.pass > 1) a.pass = (a.pass + 1) / 2;
         else AB_CHECK_ARG(false, "linear_int4: %d inputs are too many", a.K);
     }
-    const int nc = (pieces + a.ks - 1) / a.ks;
-    a.x_bytes = nc * 512 * a.pass;
-    const int fit = dev->n_sm / a.ks, most = I4_BLOCK_SUMS / (I4_ROWS * MR * 4) * I4_ROWS;   // outputs of a cluster's block at most
-    a.clusters = a.N < fit ? a.N : fit;
-    if (a.ks > 1 && (a.N + a.clusters - 1) / a.clusters > most) a.clusters = (a.N + most - 1) / most;
-    const int share = (a.N + a.clusters - 1) / a.clusters, tiles = (share + I4_ROWS - 1) / I4_ROWS;
-    a.height = (share + tiles - 1) / tiles;
-    // warps that share a tile: the fewest rounds of pieces, a tile's end counted as one
-    int best = 0;
-    for (int kw = I4_WARPS; kw >= 1; kw /= 2) {
-        const int slots = I4_WARPS / kw, cost = (tiles + slots - 1) / slots * ((nc + kw - 1) / kw + 1);
-        if (best == 0 || cost < best) best = cost, a.kw = kw;
-    }
-    const int rest = I4_SMEM - 1024 - a.x_bytes - SUMS - (a.ks > 1 ? tiles * I4_ROWS * MR * 4 : 0);
-    a.stages = rest / (I4_WARPS * I4_PIECE) < I4_STAGES ? rest / (I4_WARPS * I4_PIECE) : I4_STAGES;
+    AB_CHECK_ARG((int64_t)tiles * ((pieces + a.ks - 1) / a.ks) * I4_WARPS <= INT32_MAX, "linear_int4: a matrix of %d x %d is too large", a.N, a.K);
+    a.stages = std::min(I4_STAGES, (I4_SMEM - 1024 - a.x_bytes - shared) / (I4_WARPS * I4_PIECE));
     a.pairs = a.per_group == 1 && a.groups % 2 == 0 && (reinterpret_cast<uintptr_t>(a.scale) & 3) == 0;
     EncodeTiledFn encode;
     const int found = get_encode_fn(&encode);
@@ -444,7 +459,7 @@ int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.clusters * a.ks, (a.rows + a.pass - 1) / a.pass);
     cfg.blockDim = dim3(I4_THREADS);
-    cfg.dynamicSmemBytes = 1024 + a.stages * I4_WARPS * I4_PIECE + a.x_bytes + SUMS + (a.ks > 1 ? tiles * I4_ROWS * MR * 4 : 0);
+    cfg.dynamicSmemBytes = 1024 + a.stages * I4_WARPS * I4_PIECE + a.x_bytes + shared;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -5,13 +5,21 @@
 //   The id is the first one whose sum of w up to and with it exceeds u * (sum of w that is kept).
 //
 // All three filters keep a front part of one and the same order, and so does the draw: each is a question "where in that order do the weights (or the
-// ranks) reach X?". Nothing is sorted for that. Weights are taken as multiples of 2^-44 (the largest is 2^44 of them), so that sums are whole numbers, which
-// do not depend on the order of additions: a histogram over 4096 bins of max - l, made by atomics on shared memory, has exact sums, and its running sums answer every
-// question down to a bin. The few values of that bin are gathered and compared with each other. Where a bin holds more than SP_LIST
-// values (ties of 16-bit logits), its keys' range is divided again.
+// ranks) reach X?". What bounds it is less the reading of a row (it stays in shared memory, of one block or of a cluster's) than what is done for each of its values, so
+// the way goes by what the filters leave:
+//   few values    top-k up to 1024, or min-p: the k-th largest of the threads' own maxima is a bound that some k values and a few more reach. Those are
+//                 gathered, sorted, and their weights added up: every question is answered among them, without an exponential for any other value.
+//   a bracket     else the sum over the row is needed: 32-bit exponentials and a histogram of counts over 4096 bins of max - l in one pass. A bin's counts
+//                 bound its weights within a percent, so they say in which few bins X is reached; their values are gathered and sorted, and what lies
+//                 in front of them is added up in 32 bits (nothing, where the values down to there are few). Those sums are off by EPS at most: where a
+//                 border lies nearer than that, or the bracket holds more than 1024 values, it is done again in whole numbers.
+//   whole numbers a histogram over the same bins with exact sums, by atomics on shared memory; its running sums answer every question down to a bin. The
+//                 few values of that bin are gathered and compared with each other; where they are more than SP_LIST (ties of 16-bit logits), the
+//                 bin's keys' range is divided again.
 //
-// Precision: weights come from a table and a polynomial in 64 bits (off by 1e-15) and are rounded to 2^-45 of the largest one. What comes out is the id that
-// the definition in 64 bits gives, unless u or p meets a border within some 1e-9 of the sum.
+// Precision: weights are taken as multiples of 2^-44 (the largest is 2^44 of them), so that sums are whole numbers and do not depend on the order of additions; they
+// come from a table and a polynomial in 64 bits (off by 1e-15). What comes out is the id that the definition in 64 bits gives, unless u or p meets a border
+// within some 1e-9 of the sum. The log-probability has the 32-bit sum where a bracket sufficed: off by EPS.
 #include <cooperative_groups.h>
 
 #include "train.cuh"
@@ -27,6 +35,7 @@ constexpr int SP_LIST = 256;                   // values that are compared with 
 constexpr int SP_MAX_BLOCKS = 8;               // of a cluster: a row's at most
 constexpr int SP_ROW_BYTES = 129 * 1024;       // of a row in a block's shared memory, at most
 constexpr uint64_t SP_ONE = 1ull << 44;        // a weight of 1
+constexpr int SP_FEW = 1024;                   // values that are sorted: one per thread
 
 struct SampleArgs {
     const void* logits;
@@ -54,7 +63,15 @@ struct RowScale {
 };
 __device__ __forceinline__ int bin_of(const RowScale& r, float v) {   // never falls as v does; rounding and all
     const float d = v == r.top ? 0.f : r.top - v;
-    return min(SP_BINS - 1, __float2int_rz(d * r.bins));   // (a NaN, 0 bins per unit times infinity, gives bin 0)
+    return (int)(__float_as_uint(fminf(d * r.bins, SP_BINS - 1) + 8388608.f) & (2 * SP_BINS - 1));   // (2^23: the last places are whole numbers. A conversion has a quarter of the rate)
+}
+// w in 32 bits: z = n + f, 2^f by the hardware (relative error 2^-22). The product's rounding is made good, so that for 16-bit logits, whose differences
+// are exact where they matter, 2^-22 + 2^-23 remains; 32-bit ones add 2^-24 z ln 2 for the difference's rounding, below 2^-20 on average over the weights.
+__device__ __forceinline__ float weight32(float d, float c, float c_low) {
+    const float t = fmaf(-d, c, 12582912.f), n = t - 12582912.f;   // 1.5 * 2^23: n stands in the last places of t
+    float w;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaf(-d, c_low, fmaf(-d, c, -n))));
+    return d * c < 46.f ? __uint_as_float(__float_as_uint(w) + (__float_as_uint(t) << 23)) : 0.f;
 }
 // exp((v - top) / T): 2^z with z = n / 16 + f, |f| <= 1 / 32, and the series of exp(f ln 2) to the sixth power (what is left is below 5e-16)
 __device__ __forceinline__ double weight(const RowScale& r, float v) {
@@ -90,9 +107,14 @@ struct alignas(16) SampleShared {
     uint32_t list[SP_LIST], own[SP_LIST];
     double tab[16];
     uint64_t red[NT / 32], mine;
+    double part_sum;
     uint32_t least, most, n, matches[NT / 32], matched;
+    uint32_t digit, left, bound;   // of the search among the threads' maxima
+    int from, to;                  // bins of the next bracket; what is next instead
+    uint64_t told;
     Found found;
 };
+constexpr int SP_DONE = -1, SP_AGAIN = -2;   // SampleShared::from: the row has its id; it has to be done in whole numbers
 
 template <class E, int NT>
 struct Sampler {
@@ -121,6 +143,17 @@ struct Sampler {
             unpack<E>(row[c], v);
 #pragma unroll
             for (int i = 0; i < PER; ++i) f(v[i]);
+        }
+    }
+    // f(value, its id)
+    template <class F>
+    __device__ __forceinline__ void each_at(int first_id, F f) {
+        const int end = min(pieces, (warp + 1) * per_warp);
+        for (int c = warp * per_warp + lane; c < end; c += 32) {
+            float v[PER];
+            unpack<E>(row[c], v);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) f(v[i], first_id + c * PER + i);
         }
     }
     template <class Op>
@@ -161,6 +194,85 @@ struct Sampler {
         atomicAdd(&s.part[1][bin], (uint32_t)(w >> 15) & 0x7fffu);
         atomicAdd(&s.part[2][bin], (uint32_t)(w >> 30));
     }
+    __device__ __forceinline__ uint64_t running(uint64_t v) {   // over the threads of this block, this one included
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t w = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += w;
+        }
+        __syncthreads();   // (s.red)
+        if (lane == 31) s.red[warp] = v;
+        __syncthreads();
+        for (int i = 0; i < warp; ++i) v += s.red[i];
+        return v;
+    }
+
+    // ---- few values: key and id of each, in the first block
+    __device__ __forceinline__ uint64_t* few() { return reinterpret_cast<uint64_t*>(s.part[1]); }   // twice NT
+    __device__ __forceinline__ void keep(float v, int id) {
+        const uint32_t at = atomicAdd(of(&s.n, 0), 1u);
+        if (at < (uint32_t)NT) of(few(), 0)[at] = (uint64_t)key_of(v) << 32 | (0xffffffffu - (uint32_t)id);
+    }
+    // A bound that at least k of this block's threads reach with their maxima (to its upper 16 bits), or 0. Each digit by a histogram of the threads.
+    __device__ uint32_t reached(uint32_t k, uint32_t key) {
+        uint32_t bound = 0;
+        for (int shift = 24; shift >= 16; shift -= 8) {
+            if (threadIdx.x < 256) s.part[0][threadIdx.x] = 0;
+            if (threadIdx.x == 0) s.digit = 256;
+            __syncthreads();
+            if (key != 0 && (shift == 24 || key >> 24 == bound >> 24)) atomicAdd(&s.part[0][key >> shift & 255], 1u);
+            __syncthreads();
+            if (warp == 0) {
+                uint32_t n[8], sum = 0, up;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += n[i] = s.part[0][255 - 8 * lane - i];
+                up = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t w = __shfl_up_sync(0xffffffffu, up, o);
+                    if (lane >= o) up += w;
+                }
+                uint32_t before = up - sum;
+                if (before < k && k <= up) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (before < k && k <= before + n[i]) s.digit = 255 - 8 * lane - i, s.left = k - before;
+                        before += n[i];
+                    }
+                }
+            }
+            __syncthreads();
+            if (s.digit == 256) return 0;
+            bound |= s.digit << shift;
+            k = s.left;
+        }
+        return bound;
+    }
+    // thread r's: the r-th of n <= NT values that were kept, larger ones first (0 behind them)
+    __device__ uint64_t sorted(uint32_t n) {
+        const uint32_t i = threadIdx.x;
+        uint32_t size = 32;
+        while (size < n) size *= 2;
+        uint64_t v = i < n ? few()[i] : 0;
+        int buffer = 1;
+        for (uint32_t run = 2; run <= size; run *= 2)
+            for (uint32_t far = run / 2; far > 0; far /= 2) {
+                uint64_t other = 0;
+                if (far >= 32) {   // (two buffers in turn: one barrier each)
+                    uint64_t* x = few() + NT * buffer;
+                    if (i < size) x[i] = v;
+                    __syncthreads();
+                    if (i < size) other = x[i ^ far];
+                    buffer ^= 1;
+                } else if (i < size) {
+                    other = __shfl_xor_sync(0xffffffffu, v, far);
+                }
+                const bool larger = ((i & far) == 0) == ((i & run) == 0);
+                if (i < size) v = larger == (v > other) ? v : other;
+            }
+        return v;
+    }
+
     // running sums of the histogram, over all blocks; every block has them
     template <int BINS>
     __device__ __forceinline__ void run_up(uint64_t* cum) {
@@ -314,10 +426,10 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
     }
     auto larger = [](uint64_t p, uint64_t q) { return p > q ? p : q; };
     auto sum = [](uint64_t p, uint64_t q) { return p + q; };
-    // (both in one: the key of the largest value above, the inverted key of the smallest below it; a NaN on top of all)
-    const uint64_t high = x.reduce(nan ? ~0ull : (uint64_t)key_of(top), larger);
-    low = value_of(~(uint32_t)x.reduce((uint64_t)~key_of(low), larger));
-    const double T = a.T ? (double)a.T[row] : a.T_all, p = a.p ? (double)a.p[row] : a.p_all, m = a.m ? (double)a.m[row] : a.m_all;
+    if (threadIdx.x == 0) s.n = 0;
+    const uint32_t own_top = x.pieces > x.warp * x.per_warp + x.lane ? key_of(top) : 0;   // (0: a thread without values)
+    const uint64_t high = x.reduce(nan ? ~0ull : (uint64_t)key_of(top), larger);   // a NaN on top of all
+    const double T = a.T ? (double)a.T[row] : a.T_all, p = a.p ? (double)a.p[row] : a.p_all, m = a.m ? (double)a.m[row] : a.m_all, u = fmin(fmax((double)a.u[row], 0.0), 1.0);
     const int k = a.k ? a.k[row] : a.k_all;
     top = value_of((uint32_t)high);
     if (high == ~0ull || top == -INFINITY) {   // a NaN, or nothing to draw
@@ -325,15 +437,232 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
         if (x.blocks > 1) x.cluster.sync();
         return;
     }
+    const bool greedy = !(T > 0.0 && k != 1 && a.V > 1);
+    x.r = {top, 0.f, 1.4426950408889634074 / T, s.tab};
+    const bool by_rank = k > 0 && k < a.V, by_sum = p < 1.0, by_size = m > 0.0;
+    const int first_id = first * PER - skip;
+
+    // The n values that were kept, behind a sum `front` (in whole numbers; off by `off` of itself and of X, as X is) of all values in front of them, answer for the row, or say
+    // where to look next. total: the row's sum, likewise off, or 0: that of the first k is theirs. This in the first block; the others wait.
+    uint64_t kept = 0;       // the sum that is kept, once it is known
+    auto answer = [&](uint32_t n, uint64_t front, uint64_t total, double off, bool from_top) {
+        const uint64_t e = x.sorted(n);
+        const float v = value_of((uint32_t)(e >> 32));
+        const bool on = threadIdx.x < n;
+        const double wd = on ? weight(x.r, v) : 0.0;
+        const uint64_t w = whole_weight(wd), cum = front + x.running(w), before = cum - w;
+        auto tell = [&](uint64_t c) {   // the running sum of the c-th value
+            if (threadIdx.x + 1 == c) s.told = cum;
+            __syncthreads();
+            const uint64_t v = s.told;
+            __syncthreads();
+            return v;
+        };
+        // whether X is met too closely, or not at all
+        auto unsure = [&](uint64_t X) {
+            const double slack = off * ((double)front + (double)X);
+            const bool close = on && fabs((double)cum - (double)X) <= slack, met = on && (double)cum >= (double)X + slack;
+            return (bool)(__syncthreads_or(close) | !__syncthreads_or(met) | ((double)front > 0 && (double)front + slack >= (double)X));
+        };
+        if (kept == 0) {
+            uint32_t count = by_rank ? min((uint32_t)k, n) : n;
+            if (by_rank) total = tell(count);
+            bool cut = by_rank;
+            if (by_sum) {
+                const uint64_t X = (uint64_t)fmax(1.0, ceil(p * (double)total));
+                if (off > 0 && unsure(X)) return SP_AGAIN;
+                count = min(count, (uint32_t)__syncthreads_count(on && before < X));
+                cut = true;
+            }
+            if (by_size) {
+                const uint32_t large = __syncthreads_count(on && wd >= m);
+                if (!from_top && large < count) return SP_AGAIN;   // (the end lies in front of these)
+                count = max(1u, min(count, large));
+                cut = true;
+            }
+            kept = cut ? tell(count) : total;
+        }
+        const uint64_t X = min(kept, (uint64_t)floor(u * (double)kept) + 1);
+        if (front >= X) return 0;                       // look further up
+        if ((off > 0 && (!from_top || !(by_sum || by_size))) && unsure(X)) return SP_AGAIN;
+        if (on && before < X && X <= cum) {
+            a.ids[row] = 0xffffffffu - (uint32_t)e;
+            double logp = -log((double)kept * (1.0 / SP_ONE));
+            if (v != top) logp += ((double)v - (double)top) / T;
+            a.logp[row] = (float)logp;
+        }
+        return SP_DONE;
+    };
+    bool done = false;
+    if (!greedy && ((by_rank && k <= 600 / x.blocks) || (!by_rank && !by_sum && by_size && top < INFINITY))) {
+        // ---- few values
+        float least;
+        if (by_rank) {
+            uint32_t bound = x.reached((uint32_t)k, own_top);
+            if (x.blocks > 1) {   // the largest of the blocks' bounds will do
+                if (threadIdx.x == 0) s.bound = bound;
+                x.cluster.sync();
+                for (int b = 0; b < x.blocks; ++b) bound = max(bound, *x.of(&s.bound, b));
+            }
+            least = bound > key_of(-INFINITY) ? value_of(bound) : -INFINITY;
+        } else {
+            least = m >= 1.0 ? top : (float)fmax(-3.4e38, (double)top + T * log(m) * (1 + 1e-6));   // (a little too low: the weights decide)
+            least = fminf(least, top) - 1e-6f * fabsf(fminf(least, top));
+        }
+        __syncthreads();
+        x.each_at(first_id, [&](float v, int id) {
+            if (v >= least && v > -INFINITY) x.keep(v, id);
+        });
+        x.join();
+        const uint32_t n = *x.of(&s.n, 0);
+        if (n <= (uint32_t)NT) {   // (the same in all blocks)
+            if (x.rank == 0) answer(n, 0, 0, 0.0, true);
+            done = true;
+        }
+        if (x.blocks > 1) x.cluster.sync();   // (the first block's count has been read)
+    } else if (!greedy && !by_rank && top < INFINITY && T > 1e-6 && T < 1e6) {
+        // ---- a bracket
+        constexpr double EPS = sizeof(E) == 2 ? 0x1p-21 : 0x1p-19;   // of sums of weight32, with room for the additions' own rounding
+        const float c = (float)x.r.c, c_low = (float)(x.r.c - (double)c), bins = (float)(SP_BINS / (32.0 * T));
+        for (int i = threadIdx.x; i < SP_BINS; i += NT) s.part[0][i] = 0;
+        __syncthreads();
+        auto at_bin = [&](float d) { return fminf(d * bins, SP_BINS - 1) + 8388608.f; };
+        auto block_sum = [&](double v) {   // in the first block: over all blocks
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (x.lane == 0) reinterpret_cast<double*>(s.red)[x.warp] = v;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                v = 0.0;
+                for (int i = 0; i < NT / 32; ++i) v += reinterpret_cast<double*>(s.red)[i];
+                s.part_sum = v;
+            }
+            x.join();
+            v = 0.0;
+            if (x.rank == 0)
+                for (int b = 0; b < x.blocks; ++b) v += *x.of(&s.part_sum, b);
+            return v;
+        };
+        double mine = 0.0;
+        const int end = min(x.pieces, (x.warp + 1) * x.per_warp);
+        for (int i = x.warp * x.per_warp + x.lane; i < end; i += 32) {
+            float v[PER], w = 0.f;
+            unpack<E>(x.row[i], v);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const float d = top - v[j];
+                atomicAdd(&s.part[0][__float_as_uint(at_bin(d)) & (2 * SP_BINS - 1)], 1u);
+                w += weight32(d, c, c_low);
+            }
+            mine += (double)w;
+        }
+        const double total = block_sum(mine);
+        // In the first block: running bounds of the weights, and counts. A bin's values lie within half a bin of its middle; 4e-5 covers the rounding of all this.
+        float2* bounds = reinterpret_cast<float2*>(s.cum);
+        int from = 0, to = 0;
+        auto bracket = [&](double X) {   // the bins in which X (of the sum of weights) is reached
+            int lo = 0, hi = SP_BINS - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (bounds[mid].y >= (float)(X * (1 - 2 * EPS))) hi = mid;
+                else lo = mid + 1;
+            }
+            from = lo, hi = SP_BINS - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (bounds[mid].x >= (float)(X * (1 + 2 * EPS))) hi = mid;
+                else lo = mid + 1;
+            }
+            to = lo;
+            if (s.part[0][to] <= (uint32_t)NT) from = 0;   // (running counts: all from the top are few enough)
+            else if (s.part[0][to] - (from ? s.part[0][from - 1] : 0) > (uint32_t)NT) from = SP_AGAIN;
+        };
+        const uint64_t whole = (uint64_t)(total * SP_ONE);
+        if (x.rank == 0) {
+            constexpr int EACH = SP_BINS / NT;
+            const float q = c / bins;
+            uint32_t n[EACH];
+            float2 b[EACH];
+            uint64_t count = 0;
+            float low_sum = 0.f, high_sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int bin = threadIdx.x * EACH + i;
+                n[i] = 0;
+                for (int o = 0; o < x.blocks; ++o) n[i] += *x.of(&s.part[0][bin], o);
+                low_sum += bin + 1 < SP_BINS ? (float)n[i] * exp2f(-((float)bin + 0.5f) * q) * (1.f - 4e-5f) : 0.f;
+                high_sum += (float)n[i] * exp2f(-fmaxf((float)bin - 0.5f, 0.f) * q) * (1.f + 4e-5f);
+                count += n[i];
+                b[i] = make_float2(low_sum, high_sum);
+                n[i] = (uint32_t)count;
+            }
+            float low_up = low_sum, high_up = high_sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const float l = __shfl_up_sync(0xffffffffu, low_up, o), h = __shfl_up_sync(0xffffffffu, high_up, o);
+                if (x.lane >= o) low_up += l, high_up += h;
+            }
+            const uint32_t ahead = (uint32_t)(x.running(count) - count);   // (its barriers also: all counts have been read)
+            float2* warps = reinterpret_cast<float2*>(s.sub);
+            if (x.lane == 31) warps[x.warp] = make_float2(low_up, high_up);
+            __syncthreads();
+            float low_base = low_up - low_sum, high_base = high_up - high_sum;
+            for (int i = 0; i < x.warp; ++i) low_base += warps[i].x, high_base += warps[i].y;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                bounds[threadIdx.x * EACH + i] = make_float2((low_base + b[i].x) * (1.f - 4e-5f), (high_base + b[i].y) * (1.f + 4e-5f));
+                s.part[0][threadIdx.x * EACH + i] = ahead + n[i];
+            }
+            __syncthreads();
+            bracket(by_sum ? p * total : u * total);
+            if (threadIdx.x == 0) s.from = from, s.to = to;
+        }
+        for (int round = 0; round < 3; ++round) {
+            x.join();
+            from = *x.of(&s.from, 0), to = *x.of(&s.to, 0);
+            if (from < 0) break;
+            const float f0 = 8388608.f + (float)from, f1 = 8388608.f + (float)to;
+            mine = 0.0;
+            for (int i = x.warp * x.per_warp + x.lane; i < end; i += 32) {
+                float v[PER], w = 0.f;
+                unpack<E>(x.row[i], v);
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const float d = top - v[j], f = at_bin(d);
+                    if (f < f0) w += weight32(d, c, c_low);
+                    else if (f <= f1 && v[j] > -INFINITY) x.keep(v[j], first_id + i * PER + j);
+                }
+                mine += (double)w;
+            }
+            const double front = block_sum(mine);
+            if (x.rank == 0) {
+                const uint32_t n = s.n;
+                int next = n <= (uint32_t)NT ? answer(n, from ? (uint64_t)(front * SP_ONE) : 0, whole, EPS, from == 0) : SP_AGAIN;
+                if (next == 0) {   // the draw lies further up than the end of what is kept
+                    bracket(u * ((double)kept * (1.0 / SP_ONE)));
+                    next = from;
+                }
+                __syncthreads();   // (s.n)
+                if (threadIdx.x == 0) s.from = next, s.to = to, s.n = 0;
+            }
+        }
+        x.join();
+        done = *x.of(&s.from, 0) == SP_DONE;
+        x.join();   // (the first block's word has been read)
+    }
+    if (done) return;
+
+    // ---- whole numbers
     uint32_t key = (uint32_t)high;
     uint64_t ordinal = 0;
     double logp = 0.0;
-    if (T > 0.0 && k != 1 && a.V > 1) {
+    if (!greedy) {
+        low = value_of(~(uint32_t)x.reduce((uint64_t)~key_of(low), larger));
         const float range = (float)fmin(32.0 * T, (double)top - (double)low);
-        x.r = {top, range > 0.f ? SP_BINS / range : 0.f, 1.4426950408889634074 / T, s.tab};
+        x.r.bins = range > 0.f ? SP_BINS / range : 0.f;
         uint32_t floor_ = 0;       // keys above this one count (0 is no value's)
         uint64_t ties = 0, tied = 0;
-        if (k > 0 && k < a.V) {
+        if (by_rank) {
             x.clear(SP_BINS);
             x.each([&](float v) { x.template add<true>(bin_of(x.r, v), v); });
             x.template run_up<SP_BINS>(s.cum);
@@ -348,7 +677,7 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
         });
         x.template run_up<SP_BINS>(s.cum);
         const uint64_t above = s.cum[SP_BINS - 1];
-        uint64_t kept = above + ties * tied;
+        kept = above + ties * tied;
         uint32_t last = floor_;    // key of the last value that is kept, where a filter has set one
         // the front part that reaches X ends at ...
         auto reach = [&](uint64_t X, uint64_t& before, uint64_t& w) {
@@ -360,13 +689,13 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
             before = f.before, w = whole_weight(weight(x.r, value_of(f.key)));
             return f.key;
         };
-        if (p < 1.0) {
+        if (by_sum) {
             const uint64_t X = min(kept, (uint64_t)fmax(1.0, ceil(p * (double)kept)));
             uint64_t before, w;
             last = reach(X, before, w);
             kept = before + (X - before + w - 1) / w * w;
         }
-        if (m > 0.0 && !(last != 0 && weight(x.r, value_of(last)) >= m)) {
+        if (by_size && !(last != 0 && weight(x.r, value_of(last)) >= m)) {
             const double far = 1e-6 - log2(m);   // (a little too far)
             uint64_t mine = 0;
             x.each([&](float v) {
@@ -376,7 +705,6 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
             });
             kept = max(SP_ONE, min(kept, x.reduce(mine, sum)));
         }
-        const double u = fmin(fmax((double)a.u[row], 0.0), 1.0);
         const uint64_t X = min(kept, (uint64_t)floor(u * (double)kept) + 1);
         uint64_t before, w;
         key = reach(X, before, w);

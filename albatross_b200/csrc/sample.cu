@@ -65,13 +65,13 @@ __device__ __forceinline__ int bin_of(const RowScale& r, float v) {   // never f
     const float d = v == r.top ? 0.f : r.top - v;
     return (int)(__float_as_uint(fminf(d * r.bins, SP_BINS - 1) + 8388608.f) & (2 * SP_BINS - 1));   // (2^23: the last places are whole numbers. A conversion has a quarter of the rate)
 }
-// w in 32 bits: z = n + f, 2^f by the hardware (relative error 2^-22). The product's rounding is made good, so that for 16-bit logits, whose differences
-// are exact where they matter, 2^-22 + 2^-23 remains; 32-bit ones add 2^-24 z ln 2 for the difference's rounding, below 2^-20 on average over the weights.
+// w in 32 bits, by the hardware's 2^x (relative error 2^-22). The product's rounding and what 32 bits leave of c are made good, so that for 16-bit logits, whose differences
+// are exact where they matter, 2^-22 + 2^-23 remains; 32-bit ones add 2^-24 z ln 2 for the difference's rounding, below 2^-20 for z up to 22. d is finite.
 __device__ __forceinline__ float weight32(float d, float c, float c_low) {
-    const float t = fmaf(-d, c, 12582912.f), n = t - 12582912.f;   // 1.5 * 2^23: n stands in the last places of t
+    const float z = d * c, rest = fmaf(d, c_low, fmaf(d, c, -z));
     float w;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaf(-d, c_low, fmaf(-d, c, -n))));
-    return d * c < 46.f ? __uint_as_float(__float_as_uint(w) + (__float_as_uint(t) << 23)) : 0.f;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(-z));
+    return fmaf(w * -0.693147181f, rest, w);
 }
 // exp((v - top) / T): 2^z with z = n / 16 + f, |f| <= 1 / 32, and the series of exp(f ln 2) to the sixth power (what is left is below 5e-16)
 __device__ __forceinline__ double weight(const RowScale& r, float v) {
@@ -94,6 +94,27 @@ __device__ __forceinline__ uint64_t whole_weight(double w) {   // in units of 2^
     return (uint64_t)(__double_as_longlong(w + 384.0) - __double_as_longlong(384.0));
 }
 
+// the largest of a piece's values, NaN if one is
+template <class E> __device__ __forceinline__ float largest(const uint4& q);
+template <> __device__ __forceinline__ float largest<__half>(const uint4& q) {
+    const __half2* h = reinterpret_cast<const __half2*>(&q);
+    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+}
+template <> __device__ __forceinline__ float largest<__nv_bfloat16>(const uint4& q) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
+}
+__device__ __forceinline__ float larger_or_nan(float p, float q) {
+    float v;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(p), "f"(q));
+    return v;
+}
+template <> __device__ __forceinline__ float largest<float>(const uint4& q) {
+    return larger_or_nan(larger_or_nan(__uint_as_float(q.x), __uint_as_float(q.y)), larger_or_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
+}
+
 struct Found {
     uint32_t key;
     uint32_t equals;      // values of that key
@@ -107,14 +128,17 @@ struct alignas(16) SampleShared {
     uint32_t list[SP_LIST], own[SP_LIST];
     double tab[16];
     uint64_t red[NT / 32], mine;
-    double part_sum;
-    uint32_t least, most, n, matches[NT / 32], matched;
-    uint32_t digit, left, bound;   // of the search among the threads' maxima
-    int from, to;                  // bins of the next bracket; what is next instead
-    uint64_t told;
+    double part_sum[2];
+    uint32_t least, most, n[2], matches[NT / 32], matched;
+    uint32_t top, tops[NT / 32];
+    uint32_t digit, left, bound;          // of the search among the threads' maxima
+    uint32_t votes[2][NT / 32];
+    uint64_t told[2];
+    int state;                            // what comes next: the bins of up to two brackets, or a SampleState
+    int bins[4];
     Found found;
 };
-constexpr int SP_DONE = -1, SP_AGAIN = -2;   // SampleShared::from: the row has its id; it has to be done in whole numbers
+enum SampleState : int { SP_LOOK, SP_DONE, SP_AGAIN };   // the row has its id; it has to be done in whole numbers
 
 template <class E, int NT>
 struct Sampler {
@@ -143,17 +167,6 @@ struct Sampler {
             unpack<E>(row[c], v);
 #pragma unroll
             for (int i = 0; i < PER; ++i) f(v[i]);
-        }
-    }
-    // f(value, its id)
-    template <class F>
-    __device__ __forceinline__ void each_at(int first_id, F f) {
-        const int end = min(pieces, (warp + 1) * per_warp);
-        for (int c = warp * per_warp + lane; c < end; c += 32) {
-            float v[PER];
-            unpack<E>(row[c], v);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) f(v[i], first_id + c * PER + i);
         }
     }
     template <class Op>
@@ -194,24 +207,44 @@ struct Sampler {
         atomicAdd(&s.part[1][bin], (uint32_t)(w >> 15) & 0x7fffu);
         atomicAdd(&s.part[2][bin], (uint32_t)(w >> 30));
     }
-    __device__ __forceinline__ uint64_t running(uint64_t v) {   // over the threads of this block, this one included
+    // ---- few values: key and id of each, in the first block, which works on them with its first `size` threads
+    __device__ __forceinline__ uint64_t* few() { return reinterpret_cast<uint64_t*>(s.part[1]); }   // 4 NT of them
+    __device__ __forceinline__ void keep(float v, int id, int list = 0) {
+        const uint32_t at = atomicAdd(of(&s.n[list], 0), 1u);
+        if (at < (uint32_t)NT) of(few() + NT * list, 0)[at] = (uint64_t)key_of(v) << 32 | (0xffffffffu - (uint32_t)id);
+    }
+    int size, turn;        // (two buffers in turn for what the threads tell each other: one barrier each)
+    __device__ __forceinline__ void meet() {
+        if (size == 32) __syncwarp();
+        else asm volatile("bar.sync 1, %0;" ::"r"(size) : "memory");
+    }
+    __device__ __forceinline__ uint32_t vote(bool yes) {   // how many
+        uint32_t n = __popc(__ballot_sync(0xffffffffu, yes));
+        if (size == 32) return n;
+        turn ^= 1;
+        if (lane == 0) s.votes[turn][warp] = n;
+        meet();
+        return __reduce_add_sync(0xffffffffu, 32 * lane < size ? s.votes[turn][lane] : 0u);
+    }
+    __device__ __forceinline__ uint64_t tell(bool mine, uint64_t v) {   // that of the thread for which it is `mine`
+        turn ^= 1;
+        if (mine) s.told[turn] = v;
+        meet();
+        return s.told[turn];
+    }
+    __device__ __forceinline__ uint64_t running(uint64_t v) {   // over the threads up to this one
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t w = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += w;
         }
-        __syncthreads();   // (s.red)
+        if (size == 32) return v;
         if (lane == 31) s.red[warp] = v;
-        __syncthreads();
-        for (int i = 0; i < warp; ++i) v += s.red[i];
-        return v;
-    }
-
-    // ---- few values: key and id of each, in the first block
-    __device__ __forceinline__ uint64_t* few() { return reinterpret_cast<uint64_t*>(s.part[1]); }   // twice NT
-    __device__ __forceinline__ void keep(float v, int id) {
-        const uint32_t at = atomicAdd(of(&s.n, 0), 1u);
-        if (at < (uint32_t)NT) of(few(), 0)[at] = (uint64_t)key_of(v) << 32 | (0xffffffffu - (uint32_t)id);
+        meet();
+        uint64_t ahead = lane < warp ? s.red[lane] : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+        return v + ahead;
     }
     // A bound that at least k of this block's threads reach with their maxima (to its upper 16 bits), or 0. Each digit by a histogram of the threads.
     __device__ uint32_t reached(uint32_t k, uint32_t key) {
@@ -248,27 +281,24 @@ struct Sampler {
         }
         return bound;
     }
-    // thread r's: the r-th of n <= NT values that were kept, larger ones first (0 behind them)
-    __device__ uint64_t sorted(uint32_t n) {
+    // thread r's: the r-th of n <= size values, larger ones first (0 behind them)
+    __device__ uint64_t sorted(const uint64_t* list, uint32_t n) {
         const uint32_t i = threadIdx.x;
-        uint32_t size = 32;
-        while (size < n) size *= 2;
-        uint64_t v = i < n ? few()[i] : 0;
-        int buffer = 1;
-        for (uint32_t run = 2; run <= size; run *= 2)
+        uint64_t v = i < n ? list[i] : 0;
+        for (uint32_t run = 2; run <= (uint32_t)size; run *= 2)
             for (uint32_t far = run / 2; far > 0; far /= 2) {
-                uint64_t other = 0;
-                if (far >= 32) {   // (two buffers in turn: one barrier each)
-                    uint64_t* x = few() + NT * buffer;
-                    if (i < size) x[i] = v;
-                    __syncthreads();
-                    if (i < size) other = x[i ^ far];
-                    buffer ^= 1;
-                } else if (i < size) {
+                uint64_t other;
+                if (far >= 32) {
+                    turn ^= 1;
+                    uint64_t* x = few() + NT * (2 + turn);
+                    x[i] = v;
+                    meet();
+                    other = x[i ^ far];
+                } else {
                     other = __shfl_xor_sync(0xffffffffu, v, far);
                 }
                 const bool larger = ((i & far) == 0) == ((i & run) == 0);
-                if (i < size) v = larger == (v > other) ? v : other;
+                v = larger == (v > other) ? v : other;
             }
         return v;
     }
@@ -320,12 +350,12 @@ struct Sampler {
         uint32_t lo = 0, hi = 0xffffffffu;
         for (int level = 0;; ++level) {
             auto inside = [&](float v, uint32_t key) { return key > floor_ && (level ? key >= lo && key <= hi : bin_of(r, v) == bin); };
-            if (threadIdx.x == 0) s.n = 0, s.least = 0xffffffffu, s.most = 0;
+            if (threadIdx.x == 0) s.n[0] = 0, s.least = 0xffffffffu, s.most = 0;
             __syncthreads();
             each([&](float v) {
                 const uint32_t key = key_of(v);
                 if (!inside(v, key)) return;
-                const uint32_t at = atomicAdd(&s.n, 1u);
+                const uint32_t at = atomicAdd(&s.n[0], 1u);
                 if (at < SP_LIST) s.own[at] = key;
                 atomicMin(&s.least, key);
                 atomicMax(&s.most, key);
@@ -334,7 +364,7 @@ struct Sampler {
             uint32_t n = 0;
             lo = 0xffffffffu, hi = 0;
             for (int b = 0; b < blocks; ++b) {
-                const uint32_t have = *of(&s.n, b);
+                const uint32_t have = *of(&s.n[0], b);
                 if (n + have <= SP_LIST)
                     for (uint32_t i = threadIdx.x; i < have; i += NT) s.list[n + i] = *of(&s.own[0] + i, b);
                 n += have;
@@ -397,102 +427,95 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
     x.pieces = max(0, min(a.share, all_pieces - first));
     x.per_warp = (x.pieces + NT - 1) / NT * 32;
     if (threadIdx.x < 16) s.tab[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
-    float top = -INFINITY, low = INFINITY;
-    bool nan = false;
+    if (threadIdx.x < 2) s.n[threadIdx.x] = 0;
+    const double T = a.T ? (double)a.T[row] : a.T_all, p = a.p ? (double)a.p[row] : a.p_all, m = a.m ? (double)a.m[row] : a.m_all, u = fmin(fmax((double)a.u[row], 0.0), 1.0);
+    const int k = a.k ? a.k[row] : a.k_all;
+    const int own = x.warp * x.per_warp + x.lane, end = min(x.pieces, (x.warp + 1) * x.per_warp);   // a thread's pieces: own, own + 32 ..
+    float top = -INFINITY;
     {
         uint4* to = reinterpret_cast<uint4*>(row_bytes);
-        const int end = min(x.pieces, (x.warp + 1) * x.per_warp);
-        for (int c = x.warp * x.per_warp + x.lane; c < end; c += 32) {
+        for (int c = own; c < end; c += 32) {
             const int at = (first + c) * PER - skip;   // of the row
             uint4 q;
-            float v[PER];
             if (at >= 0 && at + PER <= a.V) {
                 q = make_uint4(0, 0, 0, 0);
                 if (all.holds(logits + at, PER)) q = __ldcs(reinterpret_cast<const uint4*>(logits + at));
-                unpack<E>(q, v);
             } else {
+                float v[PER];
 #pragma unroll
                 for (int i = 0; i < PER; ++i) v[i] = at + i >= 0 && at + i < a.V && all.holds(logits + at + i) ? to_f(logits[at + i]) : -INFINITY;
                 q = pack<E>(v);
             }
             to[c] = q;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                nan |= v[i] != v[i];
-                top = fmaxf(top, v[i]);
-                if (v[i] > -INFINITY) low = fminf(low, v[i]);
-            }
+            top = larger_or_nan(top, largest<E>(q));
         }
+    }
+    const uint32_t own_top = own < end ? (top == top ? key_of(top) : 0xffffffffu) : 0;   // 0: a thread without values; a NaN on top of all
+    uint32_t key = __reduce_max_sync(0xffffffffu, own_top);
+    if (x.lane == 0) s.tops[x.warp] = key;
+    __syncthreads();
+    key = __reduce_max_sync(0xffffffffu, s.tops[x.lane % (NT / 32)]);
+    if (x.blocks > 1) {
+        if (threadIdx.x == 0) s.top = key;
+        x.cluster.sync();
+        for (int b = 0; b < x.blocks; ++b) key = max(key, *x.of(&s.top, b));
     }
     auto larger = [](uint64_t p, uint64_t q) { return p > q ? p : q; };
     auto sum = [](uint64_t p, uint64_t q) { return p + q; };
-    if (threadIdx.x == 0) s.n = 0;
-    const uint32_t own_top = x.pieces > x.warp * x.per_warp + x.lane ? key_of(top) : 0;   // (0: a thread without values)
-    const uint64_t high = x.reduce(nan ? ~0ull : (uint64_t)key_of(top), larger);   // a NaN on top of all
-    const double T = a.T ? (double)a.T[row] : a.T_all, p = a.p ? (double)a.p[row] : a.p_all, m = a.m ? (double)a.m[row] : a.m_all, u = fmin(fmax((double)a.u[row], 0.0), 1.0);
-    const int k = a.k ? a.k[row] : a.k_all;
-    top = value_of((uint32_t)high);
-    if (high == ~0ull || top == -INFINITY) {   // a NaN, or nothing to draw
+    if (key == 0xffffffffu || key <= key_of(-INFINITY)) {   // a NaN, or nothing to draw
         if (x.rank == 0 && threadIdx.x == 0) a.ids[row] = -1, a.logp[row] = NAN;
         if (x.blocks > 1) x.cluster.sync();
         return;
     }
+    top = value_of(key);
     const bool greedy = !(T > 0.0 && k != 1 && a.V > 1);
     x.r = {top, 0.f, 1.4426950408889634074 / T, s.tab};
     const bool by_rank = k > 0 && k < a.V, by_sum = p < 1.0, by_size = m > 0.0;
     const int first_id = first * PER - skip;
 
-    // The n values that were kept, behind a sum `front` (in whole numbers; off by `off` of itself and of X, as X is) of all values in front of them, answer for the row, or say
-    // where to look next. total: the row's sum, likewise off, or 0: that of the first k is theirs. This in the first block; the others wait.
-    uint64_t kept = 0;       // the sum that is kept, once it is known
-    auto answer = [&](uint32_t n, uint64_t front, uint64_t total, double off, bool from_top) {
-        const uint64_t e = x.sorted(n);
+    // Of the n values of a list, behind a sum `front` of all in front of them: what is kept (`ends`: with total the row's sum, or 0: that of the first k is theirs), and the
+    // draw (`draws`). front, and total, may be `off` relative. In the first block, by its first x.size threads; the others wait.
+    uint64_t kept = 0;
+    auto answer = [&](const uint64_t* list, uint32_t n, uint64_t front, uint64_t total, double off, bool from_top, bool ends, bool draws) {
+        const uint64_t e = x.sorted(list, n);
         const float v = value_of((uint32_t)(e >> 32));
         const bool on = threadIdx.x < n;
         const double wd = on ? weight(x.r, v) : 0.0;
         const uint64_t w = whole_weight(wd), cum = front + x.running(w), before = cum - w;
-        auto tell = [&](uint64_t c) {   // the running sum of the c-th value
-            if (threadIdx.x + 1 == c) s.told = cum;
-            __syncthreads();
-            const uint64_t v = s.told;
-            __syncthreads();
-            return v;
-        };
         // whether X is met too closely, or not at all
         auto unsure = [&](uint64_t X) {
             const double slack = off * ((double)front + (double)X);
             const bool close = on && fabs((double)cum - (double)X) <= slack, met = on && (double)cum >= (double)X + slack;
-            return (bool)(__syncthreads_or(close) | !__syncthreads_or(met) | ((double)front > 0 && (double)front + slack >= (double)X));
+            return x.vote(close) != 0 || x.vote(met) == 0 || (!from_top && (double)front + slack >= (double)X);
         };
-        if (kept == 0) {
+        if (ends) {
             uint32_t count = by_rank ? min((uint32_t)k, n) : n;
-            if (by_rank) total = tell(count);
-            bool cut = by_rank;
+            if (by_rank) total = x.tell(threadIdx.x + 1 == count, cum);
             if (by_sum) {
                 const uint64_t X = (uint64_t)fmax(1.0, ceil(p * (double)total));
                 if (off > 0 && unsure(X)) return SP_AGAIN;
-                count = min(count, (uint32_t)__syncthreads_count(on && before < X));
-                cut = true;
+                count = min(count, x.vote(on && before < X));
             }
             if (by_size) {
-                const uint32_t large = __syncthreads_count(on && wd >= m);
-                if (!from_top && large < count) return SP_AGAIN;   // (the end lies in front of these)
+                const uint32_t large = x.vote(on && wd >= m);
+                if (!from_top && large < count) return SP_AGAIN;   // (the end may lie in front of these)
                 count = max(1u, min(count, large));
-                cut = true;
             }
-            kept = cut ? tell(count) : total;
+            kept = by_rank || by_sum || by_size ? x.tell(threadIdx.x + 1 == count, cum) : total;
         }
-        const uint64_t X = min(kept, (uint64_t)floor(u * (double)kept) + 1);
-        if (front >= X) return 0;                       // look further up
-        if ((off > 0 && (!from_top || !(by_sum || by_size))) && unsure(X)) return SP_AGAIN;
-        if (on && before < X && X <= cum) {
-            a.ids[row] = 0xffffffffu - (uint32_t)e;
-            double logp = -log((double)kept * (1.0 / SP_ONE));
-            if (v != top) logp += ((double)v - (double)top) / T;
-            a.logp[row] = (float)logp;
+        if (draws) {
+            const uint64_t X = min(kept, (uint64_t)floor(u * (double)kept) + 1);
+            if (off > 0 && (!from_top || !(by_sum || by_size)) && unsure(X)) return SP_AGAIN;
+            if (on && before < X && X <= cum) {
+                a.ids[row] = 0xffffffffu - (uint32_t)e;
+                double logp = -log((double)kept * (1.0 / SP_ONE));
+                if (v != top) logp += ((double)v - (double)top) / T;
+                a.logp[row] = (float)logp;
+            }
         }
         return SP_DONE;
     };
+    auto width = [](uint32_t n) { return n <= 32 ? 32 : 1 << (32 - __clz(n - 1)); };   // threads for n values
     bool done = false;
     if (!greedy && ((by_rank && k <= 600 / x.blocks) || (!by_rank && !by_sum && by_size && top < INFINITY))) {
         // ---- few values
@@ -505,158 +528,192 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
                 for (int b = 0; b < x.blocks; ++b) bound = max(bound, *x.of(&s.bound, b));
             }
             least = bound > key_of(-INFINITY) ? value_of(bound) : -INFINITY;
-        } else {
-            least = m >= 1.0 ? top : (float)fmax(-3.4e38, (double)top + T * log(m) * (1 + 1e-6));   // (a little too low: the weights decide)
-            least = fminf(least, top) - 1e-6f * fabsf(fminf(least, top));
+        } else {   // (a little too low: the weights decide)
+            least = m >= 1.0 ? top : fminf(top, (float)fmax(-3.4e38, (double)top + T * log(m) * (1 + 1e-6)));
+            least -= 1e-6f * fabsf(least);
         }
         __syncthreads();
-        x.each_at(first_id, [&](float v, int id) {
-            if (v >= least && v > -INFINITY) x.keep(v, id);
-        });
+        for (int c = own; c < end; c += 32) {
+            const uint4 q = x.row[c];
+            if (!(largest<E>(q) >= least)) continue;
+            float v[PER];
+            unpack<E>(q, v);
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (v[i] >= least && v[i] > -INFINITY) x.keep(v[i], first_id + c * PER + i);
+        }
         x.join();
-        const uint32_t n = *x.of(&s.n, 0);
+        const uint32_t n = *x.of(&s.n[0], 0);
         if (n <= (uint32_t)NT) {   // (the same in all blocks)
-            if (x.rank == 0) answer(n, 0, 0, 0.0, true);
+            x.size = width(n), x.turn = 0;
+            if (x.rank == 0 && (int)threadIdx.x < x.size) answer(x.few(), n, 0, 0, 0.0, true, true, true);
             done = true;
         }
         if (x.blocks > 1) x.cluster.sync();   // (the first block's count has been read)
     } else if (!greedy && !by_rank && top < INFINITY && T > 1e-6 && T < 1e6) {
         // ---- a bracket
         constexpr double EPS = sizeof(E) == 2 ? 0x1p-21 : 0x1p-19;   // of sums of weight32, with room for the additions' own rounding
-        const float c = (float)x.r.c, c_low = (float)(x.r.c - (double)c), bins = (float)(SP_BINS / (32.0 * T));
+        constexpr float MAGIC = 8388608.f;                           // 2^23: the last places are whole numbers
+        const float c = (float)x.r.c, c_low = (float)(x.r.c - (double)c), bins = (float)(SP_BINS / (32.0 * T)), far = (SP_BINS - 1) / bins;
         for (int i = threadIdx.x; i < SP_BINS; i += NT) s.part[0][i] = 0;
+        if (threadIdx.x == 0) s.state = SP_LOOK;
         __syncthreads();
-        auto at_bin = [&](float d) { return fminf(d * bins, SP_BINS - 1) + 8388608.f; };
-        auto block_sum = [&](double v) {   // in the first block: over all blocks
+        auto block_sums = [&](double v, double w, double (&out)[2]) {   // in the first block: over all blocks
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (x.lane == 0) reinterpret_cast<double*>(s.red)[x.warp] = v;
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o), w += __shfl_xor_sync(0xffffffffu, w, o);
+            double* r = reinterpret_cast<double*>(s.sub);
+            if (x.lane == 0) r[x.warp] = v, r[32 + x.warp] = w;
             __syncthreads();
-            if (threadIdx.x == 0) {
-                v = 0.0;
-                for (int i = 0; i < NT / 32; ++i) v += reinterpret_cast<double*>(s.red)[i];
-                s.part_sum = v;
+            if (x.warp < 2) {
+                v = x.lane < NT / 32 ? r[32 * x.warp + x.lane] : 0.0;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                if (x.lane == 0) s.part_sum[x.warp] = v;
             }
             x.join();
-            v = 0.0;
+            out[0] = out[1] = 0.0;
             if (x.rank == 0)
-                for (int b = 0; b < x.blocks; ++b) v += *x.of(&s.part_sum, b);
-            return v;
+                for (int b = 0; b < x.blocks; ++b) out[0] += *x.of(&s.part_sum[0], b), out[1] += *x.of(&s.part_sum[1], b);
         };
-        double mine = 0.0;
-        const int end = min(x.pieces, (x.warp + 1) * x.per_warp);
-        for (int i = x.warp * x.per_warp + x.lane; i < end; i += 32) {
+        // (values beyond `far`, -inf among them, count as those there: 2^-46 each)
+        double mine = 0.0, sums[2];
+        for (int i = own; i < end; i += 32) {
             float v[PER], w = 0.f;
             unpack<E>(x.row[i], v);
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                const float d = top - v[j];
-                atomicAdd(&s.part[0][__float_as_uint(at_bin(d)) & (2 * SP_BINS - 1)], 1u);
+                const float d = fminf(top - v[j], far);
+                atomicAdd(&s.part[0][__float_as_uint(fmaf(d, bins, MAGIC)) - __float_as_uint(MAGIC)], 1u);
                 w += weight32(d, c, c_low);
             }
             mine += (double)w;
         }
-        const double total = block_sum(mine);
-        // In the first block: running bounds of the weights, and counts. A bin's values lie within half a bin of its middle; 4e-5 covers the rounding of all this.
-        float2* bounds = reinterpret_cast<float2*>(s.cum);
-        int from = 0, to = 0;
-        auto bracket = [&](double X) {   // the bins in which X (of the sum of weights) is reached
-            int lo = 0, hi = SP_BINS - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (bounds[mid].y >= (float)(X * (1 - 2 * EPS))) hi = mid;
-                else lo = mid + 1;
-            }
-            from = lo, hi = SP_BINS - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (bounds[mid].x >= (float)(X * (1 + 2 * EPS))) hi = mid;
-                else lo = mid + 1;
-            }
-            to = lo;
-            if (s.part[0][to] <= (uint32_t)NT) from = 0;   // (running counts: all from the top are few enough)
-            else if (s.part[0][to] - (from ? s.part[0][from - 1] : 0) > (uint32_t)NT) from = SP_AGAIN;
-        };
+        block_sums(mine, 0.0, sums);
+        const double total = sums[0];
         const uint64_t whole = (uint64_t)(total * SP_ONE);
         if (x.rank == 0) {
+            // Running counts, and sums of the weights as if a bin's values lay in its middle: they are off by half a bin's width each, 0.4 %, to either side. That they say
+            // where to look is all that is asked of them: `answer` sees whether the place was right.
             constexpr int EACH = SP_BINS / NT;
+            float* run = reinterpret_cast<float*>(s.cum);
+            uint32_t n[EACH], count = 0;
+            float b[EACH], weights = 0.f;
             const float q = c / bins;
-            uint32_t n[EACH];
-            float2 b[EACH];
-            uint64_t count = 0;
-            float low_sum = 0.f, high_sum = 0.f;
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
                 const int bin = threadIdx.x * EACH + i;
                 n[i] = 0;
                 for (int o = 0; o < x.blocks; ++o) n[i] += *x.of(&s.part[0][bin], o);
-                low_sum += bin + 1 < SP_BINS ? (float)n[i] * exp2f(-((float)bin + 0.5f) * q) * (1.f - 4e-5f) : 0.f;
-                high_sum += (float)n[i] * exp2f(-fmaxf((float)bin - 0.5f, 0.f) * q) * (1.f + 4e-5f);
+                float w;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(-(float)bin * q));
+                weights += (float)n[i] * w;
                 count += n[i];
-                b[i] = make_float2(low_sum, high_sum);
-                n[i] = (uint32_t)count;
+                b[i] = weights;
+                n[i] = count;
             }
-            float low_up = low_sum, high_up = high_sum;
+            float w_up = weights;
+            uint32_t n_up = count;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const float l = __shfl_up_sync(0xffffffffu, low_up, o), h = __shfl_up_sync(0xffffffffu, high_up, o);
-                if (x.lane >= o) low_up += l, high_up += h;
+                const float l = __shfl_up_sync(0xffffffffu, w_up, o);
+                const uint32_t h = __shfl_up_sync(0xffffffffu, n_up, o);
+                if (x.lane >= o) w_up += l, n_up += h;
             }
-            const uint32_t ahead = (uint32_t)(x.running(count) - count);   // (its barriers also: all counts have been read)
-            float2* warps = reinterpret_cast<float2*>(s.sub);
-            if (x.lane == 31) warps[x.warp] = make_float2(low_up, high_up);
-            __syncthreads();
-            float low_base = low_up - low_sum, high_base = high_up - high_sum;
-            for (int i = 0; i < x.warp; ++i) low_base += warps[i].x, high_base += warps[i].y;
+            float2* warps = reinterpret_cast<float2*>(s.red);
+            if (x.lane == 31) warps[x.warp] = make_float2(w_up, __uint_as_float(n_up));
+            __syncthreads();   // (and all counts have been read)
+            float w_base = x.lane < x.warp ? warps[x.lane].x : 0.f;
+            const uint32_t n_base = __reduce_add_sync(0xffffffffu, x.lane < x.warp ? __float_as_uint(warps[x.lane].y) : 0u) + n_up - count;
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-                bounds[threadIdx.x * EACH + i] = make_float2((low_base + b[i].x) * (1.f - 4e-5f), (high_base + b[i].y) * (1.f + 4e-5f));
-                s.part[0][threadIdx.x * EACH + i] = ahead + n[i];
-            }
-            __syncthreads();
-            bracket(by_sum ? p * total : u * total);
-            if (threadIdx.x == 0) s.from = from, s.to = to;
-        }
-        for (int round = 0; round < 3; ++round) {
-            x.join();
-            from = *x.of(&s.from, 0), to = *x.of(&s.to, 0);
-            if (from < 0) break;
-            const float f0 = 8388608.f + (float)from, f1 = 8388608.f + (float)to;
-            mine = 0.0;
-            for (int i = x.warp * x.per_warp + x.lane; i < end; i += 32) {
-                float v[PER], w = 0.f;
-                unpack<E>(x.row[i], v);
+            for (int o = 16; o > 0; o >>= 1) w_base += __shfl_xor_sync(0xffffffffu, w_base, o);
+            w_base += w_up - weights;
 #pragma unroll
-                for (int j = 0; j < PER; ++j) {
-                    const float d = top - v[j], f = at_bin(d);
-                    if (f < f0) w += weight32(d, c, c_low);
-                    else if (f <= f1 && v[j] > -INFINITY) x.keep(v[j], first_id + i * PER + j);
+            for (int i = 0; i < EACH; ++i) run[threadIdx.x * EACH + i] = w_base + b[i], s.part[0][threadIdx.x * EACH + i] = n_base + n[i];
+            __syncthreads();
+            if (x.warp == 0) {   // lane 0 .. 3: the bins in which the lower and upper end of the draw's bracket lie, and of the end of what is kept
+                const double X = (x.lane < 2 ? u : 1.0) * (by_sum ? p : 1.0) * total;
+                const float at = (float)(x.lane & 1 ? X * 1.004 : X * 0.997);
+                int lo = 0, hi = SP_BINS - 1;
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (run[mid] >= at) hi = mid;
+                    else lo = mid + 1;
                 }
-                mine += (double)w;
-            }
-            const double front = block_sum(mine);
-            if (x.rank == 0) {
-                const uint32_t n = s.n;
-                int next = n <= (uint32_t)NT ? answer(n, from ? (uint64_t)(front * SP_ONE) : 0, whole, EPS, from == 0) : SP_AGAIN;
-                if (next == 0) {   // the draw lies further up than the end of what is kept
-                    bracket(u * ((double)kept * (1.0 / SP_ONE)));
-                    next = from;
+                int u0 = __shfl_sync(0xffffffffu, lo, 0), u1 = __shfl_sync(0xffffffffu, lo, 1), p0 = SP_BINS, p1 = SP_BINS - 1;
+                if (by_sum) p0 = __shfl_sync(0xffffffffu, lo, 2), p1 = __shfl_sync(0xffffffffu, lo, 3);
+                auto values = [&](int from, int to) { return s.part[0][to] - (from > 0 ? s.part[0][from - 1] : 0); };
+                const int last = by_sum ? p1 : u1;
+                int state = SP_LOOK;
+                if (values(0, last) <= (uint32_t)NT) {           // all from the top are few enough
+                    u0 = 0, u1 = last, p0 = SP_BINS;
+                } else if (by_sum && values(u0, p1) <= (uint32_t)NT) {   // one bracket for both
+                    u1 = p1, p0 = SP_BINS;
+                } else if (values(u0, u1) > (uint32_t)NT || (by_sum && (u1 >= p0 || values(p0, p1) > (uint32_t)NT))) {
+                    state = SP_AGAIN;
                 }
-                __syncthreads();   // (s.n)
-                if (threadIdx.x == 0) s.from = next, s.to = to, s.n = 0;
+                if (x.lane == 0) s.bins[0] = u0, s.bins[1] = u1, s.bins[2] = p0, s.bins[3] = p1, s.state = state;
             }
         }
         x.join();
-        done = *x.of(&s.from, 0) == SP_DONE;
+        int state = *x.of(&s.state, 0);
+        if (state == SP_LOOK) {
+            const float u0 = MAGIC + (float)*x.of(&s.bins[0], 0), u1 = MAGIC + (float)*x.of(&s.bins[1], 0), p0 = MAGIC + (float)*x.of(&s.bins[2], 0), p1 = MAGIC + (float)*x.of(&s.bins[3], 0);
+            const bool two = p0 < MAGIC + SP_BINS, from_top = u0 == MAGIC;
+            double ahead = 0.0;
+            mine = 0.0;
+            for (int i = own; i < end; i += 32) {
+                const uint4 q = x.row[i];
+                if (from_top && !two && fmaf(fminf(top - largest<E>(q), far), bins, MAGIC) > u1) continue;
+                float v[PER], w0 = 0.f, w1 = 0.f;
+                unpack<E>(q, v);
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const float d = fminf(top - v[j], far), f = fmaf(d, bins, MAGIC);
+                    if (f < u0 || (two && f < p0)) {
+                        const float w = weight32(d, c, c_low);
+                        w1 += w;
+                        if (f < u0) w0 += w;
+                    }
+                    if (f >= u0 && f <= u1 && v[j] > -INFINITY) x.keep(v[j], first_id + i * PER + j);
+                    else if (two && f >= p0 && f <= p1 && v[j] > -INFINITY) x.keep(v[j], first_id + i * PER + j, 1);
+                }
+                mine += (double)w0, ahead += (double)w1;
+            }
+            block_sums(mine, ahead, sums);
+            if (x.rank == 0) {
+                const uint32_t n0 = s.n[0], n1 = s.n[1];
+                const uint64_t front = from_top ? 0 : (uint64_t)(sums[0] * SP_ONE);
+                state = n0 <= (uint32_t)NT && n1 <= (uint32_t)NT ? SP_DONE : SP_AGAIN;
+                if (two && state == SP_DONE) {
+                    x.size = width(n1), x.turn = 0;
+                    if ((int)threadIdx.x < x.size) state = answer(x.few() + NT, n1, (uint64_t)(sums[1] * SP_ONE), whole, EPS, false, true, false);
+                    if (threadIdx.x == 0) s.state = state, s.told[0] = kept;
+                    __syncthreads();
+                    state = s.state, kept = s.told[0];
+                    __syncthreads();
+                }
+                if (state == SP_DONE) {
+                    x.size = width(n0), x.turn = 0;
+                    if ((int)threadIdx.x < x.size) state = answer(x.few(), n0, front, whole, EPS, from_top, !two, true);
+                }
+                if (threadIdx.x == 0) s.state = state;
+            }
+            x.join();
+            state = *x.of(&s.state, 0);
+        }
+        done = state == SP_DONE;
         x.join();   // (the first block's word has been read)
     }
     if (done) return;
 
     // ---- whole numbers
-    uint32_t key = (uint32_t)high;
     uint64_t ordinal = 0;
     double logp = 0.0;
     if (!greedy) {
+        float low = INFINITY;
+        x.each([&](float v) {
+            if (v > -INFINITY) low = fminf(low, v);
+        });
         low = value_of(~(uint32_t)x.reduce((uint64_t)~key_of(low), larger));
         const float range = (float)fmin(32.0 * T, (double)top - (double)low);
         x.r.bins = range > 0.f ? SP_BINS / range : 0.f;
@@ -730,7 +787,6 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
         x.cluster.sync();
     }
     if (ordinal < before || ordinal >= (uint64_t)before + matches) return;
-    const int end = min(x.pieces, (x.warp + 1) * x.per_warp);
     for (int c0 = x.warp * x.per_warp; c0 < end; c0 += 32) {
         const int c = c0 + x.lane;
         uint32_t mask = 0;

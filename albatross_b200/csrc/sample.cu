@@ -47,6 +47,7 @@ struct SampleArgs {
     int64_t* ids;
     float* logp;
     int32_t share;                // 16-byte pieces of a row that a block takes
+    int32_t ahead;                // rows from one that is worked on to the one that follows it there
 };
 
 __device__ __forceinline__ uint32_t key_of(float v) {   // larger values, larger keys; -0 is 0
@@ -813,6 +814,326 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
     }
 }
 
+// ---- 16-bit logits: one counter for each of their 65536 values ------------------------------------------------------------------------------
+// A row's histogram over the values themselves, in shared memory, says everything but which id has a value: what is kept and drawn is found among the
+// counters, whose running sums are exact, and the row is read once more (from L2) for the id. No value of the row needs an exponential: the counters in use, some
+// 15 000 of a row of 65536 fp16 logits, do. What bounds it: the atomics (3.3 cycles for a warp's, two values meet a bank), then the counters' weights in 64 bits.
+//
+// Counters lie in the order of the values, larger ones first, eight in 16 bytes: a unit. Eight units are a group; a warp's eight lanes take one at a time, and groups
+// go round the warps, since values lie densely in a few binades. Sums of groups are run up over the block; a question is answered by a search among them and by the 64
+// counters of one group, by every warp for itself.
+//
+// A counter holds up to 65535: the row's last value is added when the others are counted, so that only a row of 65536 equal ones exceeds it (`extra`).
+constexpr int SK_NT = 1024, SK_BINS = 65536, SK_GROUPS = SK_BINS / 64, SK_ROUNDS = SK_BINS / 8 / SK_NT;
+
+template <class E> struct KeyType;   // how a type's 16 bits are ordered
+template <> struct KeyType<__half> {
+    static constexpr int NEG_INF = 0xfc00;   // its bin; NaNs lie behind it, and in front of the other infinity
+    static __device__ __forceinline__ uint32_t same(uint32_t two, uint32_t as) {   // 16 bits of ones where equal (0 and -0 are)
+        return __heq2_mask(*reinterpret_cast<const __half2*>(&two), *reinterpret_cast<const __half2*>(&as));
+    }
+};
+template <> struct KeyType<__nv_bfloat16> {
+    static constexpr int NEG_INF = 0xff80;
+    static __device__ __forceinline__ uint32_t same(uint32_t two, uint32_t as) {
+        return __heq2_mask(*reinterpret_cast<const __nv_bfloat162*>(&two), *reinterpret_cast<const __nv_bfloat162*>(&as));
+    }
+};
+__device__ __forceinline__ uint32_t bits_of_bin(uint32_t bin) { return bin < 0x8000u ? 0x7fffu - bin : bin; }
+__device__ __forceinline__ uint32_t bin_of_bits(uint32_t bits) { return bits == 0x8000u ? 0x7fffu : bits < 0x8000u ? 0x7fffu - bits : bits; }
+
+struct alignas(16) KeyShared {
+    uint4 counts[SK_BINS / 8];
+    uint64_t sums[SK_GROUPS];
+    uint64_t red[32];
+    double tab[16];
+    uint32_t tops[32], matches[32];
+    uint32_t extra;
+};
+
+template <class E>
+__global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs a) {
+    extern __shared__ __align__(16) unsigned char key_smem[];
+    KeyShared& s = *reinterpret_cast<KeyShared*>(key_smem);
+    using K = KeyType<E>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = blockIdx.x;
+    const E* logits = static_cast<const E*>(a.logits) + row * a.stride;
+    const Extent all = rows_extent(a.logits, a.rows, a.stride, a.V, 2);
+    for (int i = threadIdx.x; i < SK_BINS / 8; i += SK_NT) s.counts[i] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x < 16) s.tab[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
+    if (threadIdx.x == 0) s.extra = 0;
+    const double T = a.T ? (double)a.T[row] : a.T_all, p = a.p ? (double)a.p[row] : a.p_all, m = a.m ? (double)a.m[row] : a.m_all, u = fmin(fmax((double)a.u[row], 0.0), 1.0);
+    const int k = a.k ? a.k[row] : a.k_all;
+    // the row from its last 16-byte boundary on, as pieces of eight values; a warp's pieces follow one another
+    const int skip = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / 2), pieces = (skip + a.V + 7) / 8;
+    const int per_warp = (pieces + SK_NT - 1) / SK_NT * 32, own = warp * per_warp + lane, end = min(pieces, (warp + 1) * per_warp);
+    if (row + a.ahead < a.rows) {   // a row that a block will take when this one is done
+        const char* next = reinterpret_cast<const char*>(static_cast<const E*>(a.logits) + (row + a.ahead) * a.stride) + (size_t)threadIdx.x * 128;
+        if ((int64_t)threadIdx.x * 64 < a.V) asm volatile("prefetch.global.L2 [%0];" ::"l"(next));
+    }
+    auto piece = [&](int c) {   // (values outside of the row: -inf)
+        const int at = c * 8 - skip;
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (at >= 0 && at + 8 <= a.V) {
+            if (all.holds(logits + at, 8)) q = __ldg(reinterpret_cast<const uint4*>(logits + at));
+        } else {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = at + i >= 0 && at + i < a.V && all.holds(logits + at + i) ? to_f(logits[at + i]) : -INFINITY;
+            q = pack<E>(v);
+        }
+        return q;
+    };
+    __syncthreads();
+    uint32_t* words = reinterpret_cast<uint32_t*>(s.counts);
+    float top = -INFINITY;
+    auto count = [&](uint32_t bin) { atomicAdd(words + (bin >> 1), bin & 1 ? 0x10000u : 1u); };
+    for (int c0 = own; c0 < end; c0 += 32 * 4) {
+        uint4 q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c0 + 32 * j < end) q[j] = piece(c0 + 32 * j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = c0 + 32 * j;
+            if (c >= end) continue;
+            top = larger_or_nan(top, largest<E>(q[j]));
+            const int at = c * 8 - skip;
+            const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+            const bool whole = at >= 0 && at + 8 < a.V;   // (the last value is added below)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t sign = (w[i] >> 15) & 0x00010001u, bins = w[i] ^ (0x7fff7fffu - sign * 0x7fffu);
+                if (whole || (at + 2 * i >= 0 && at + 2 * i < a.V - 1)) count(bins & 0xffffu);
+                if (whole || (at + 2 * i + 1 >= 0 && at + 2 * i + 1 < a.V - 1)) count(bins >> 16);
+            }
+        }
+    }
+    const uint32_t own_top = own < end ? (top == top ? key_of(top) : 0xffffffffu) : 0;   // a NaN on top of all
+    uint32_t top_key = __reduce_max_sync(0xffffffffu, own_top);
+    if (lane == 0) s.tops[warp] = top_key;
+    __syncthreads();
+    top_key = __reduce_max_sync(0xffffffffu, s.tops[lane]);
+    if (top_key == 0xffffffffu || top_key <= key_of(-INFINITY)) {   // a NaN, or nothing to draw
+        if (threadIdx.x == 0) a.ids[row] = -1, a.logp[row] = NAN;
+        return;
+    }
+    top = value_of(top_key);
+    const bool greedy = !(T > 0.0 && k != 1 && a.V > 1);
+    const RowScale r = {top, 0.f, 1.4426950408889634074 / T, s.tab};
+    auto value_at = [&](uint32_t bin) { return to_f(from_bits<E>((unsigned short)bits_of_bin(bin))); };
+    auto bin_at = [&](float v) {
+        const E t = from_f<E>(v);
+        return bin_of_bits(*reinterpret_cast<const unsigned short*>(&t));
+    };
+    const uint32_t top_bin = bin_at(top);
+    uint32_t bin = top_bin;
+    uint64_t ordinal = 0;
+    double logp = 0.0;
+    if (!greedy) {
+        if (threadIdx.x == 0) {   // -0 is 0, and the last value
+            const uint32_t minus = words[0x4000] & 0xffffu;
+            words[0x4000] -= minus;
+            words[0x3fff] += minus << 16;
+            const uint32_t last = bin_of_bits(*reinterpret_cast<const unsigned short*>(logits + a.V - 1)), shift = 16 * (last & 1);
+            if ((words[last >> 1] >> shift & 0xffffu) == 0xffffu) s.extra = 1;
+            else words[last >> 1] += 1u << shift;
+        }
+        __syncthreads();
+        const uint32_t extra = s.extra;
+        auto counted = [&](uint32_t word, int half) {
+            const uint32_t n = half ? word >> 16 : word & 0xffffu;
+            return n == 0xffffu ? n + extra : n;
+        };
+        // Sums of groups [first, last) of what `of` makes of a unit and its first bin, run up; all threads then have them in s.sums. (Group g: units 8 g .. 8 g + 7.)
+        const int first = (int)(top_bin >> 6);
+        auto run_up = [&](int last, auto of) {
+            __syncthreads();   // (s.sums, s.red)
+            for (int i = 0; i < SK_ROUNDS; ++i) {
+                const int group = i * 128 + (lane >> 3) * 32 + warp, unit = group * 8 + (lane & 7);
+                uint64_t v = 0;
+                if (i * 128 < last && (i + 1) * 128 > first) {   // (the same for the whole block)
+                    if (group >= first && group < last) {
+                        const uint4 q = s.counts[unit];
+                        if ((q.x | q.y | q.z | q.w) != 0) v = of(q, unit * 8);
+                    }
+                    v += __shfl_xor_sync(0xffffffffu, v, 1);
+                    v += __shfl_xor_sync(0xffffffffu, v, 2);
+                    v += __shfl_xor_sync(0xffffffffu, v, 4);
+                }
+                if ((lane & 7) == 0) s.sums[group] = v;
+            }
+            __syncthreads();
+            uint64_t v = s.sums[threadIdx.x];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t w = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += w;
+            }
+            if (lane == 31) s.red[warp] = v;
+            __syncthreads();
+            uint64_t before = lane < warp ? s.red[lane] : 0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+            s.sums[threadIdx.x] = v + before;
+            __syncthreads();
+        };
+        // Where the running sum reaches X: by every warp for itself. `one`: of a counter and its bin. Bins from `floor_` on do not count.
+        struct At {
+            uint32_t bin, n;   // n: its counter
+            uint64_t before;
+        };
+        auto reach = [&](uint64_t X, uint32_t floor_, auto one) {
+            int lo = 0, hi = SK_GROUPS - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (s.sums[mid] >= X) hi = mid;
+                else lo = mid + 1;
+            }
+            const uint32_t word = words[lo * 32 + lane], b = lo * 64 + 2 * lane;   // this lane's two counters
+            const uint32_t n0 = counted(word, 0), n1 = counted(word, 1);
+            const uint64_t v0 = n0 && b < floor_ ? one(n0, b) : 0, v1 = n1 && b + 1 < floor_ ? one(n1, b + 1) : 0;
+            uint64_t up = v0 + v1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t w = __shfl_up_sync(0xffffffffu, up, o);
+                if (lane >= o) up += w;
+            }
+            up += lo ? s.sums[lo - 1] : 0;
+            const int at = __ffs(__ballot_sync(0xffffffffu, up >= X)) - 1;
+            const bool second = up - v1 < X;
+            At out;
+            out.bin = __shfl_sync(0xffffffffu, b + second, at & 31);
+            out.n = __shfl_sync(0xffffffffu, second ? n1 : n0, at & 31);
+            out.before = __shfl_sync(0xffffffffu, second ? up - v1 : up - v1 - v0, at & 31);
+            return out;
+        };
+        const bool by_rank = k > 0 && k < a.V;
+        uint32_t floor_ = K::NEG_INF;     // bins from here on are not kept, or have no weight
+        uint64_t ties = 0, tied = 0;
+        if (by_rank) {
+            auto ranks = [&](uint32_t n, uint32_t) { return (uint64_t)n; };
+            run_up(SK_GROUPS, [&](const uint4& q, int) {
+                uint64_t n = 0;
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) n += counted(w[i], 0) + counted(w[i], 1);
+                return n;
+            });
+            const At f = reach((uint64_t)k, SK_BINS, ranks);
+            if (f.bin < (uint32_t)K::NEG_INF) {
+                floor_ = f.bin;
+                ties = (uint64_t)k - f.before;
+                tied = whole_weight(weight(r, value_at(floor_)));
+            }
+        }
+        auto weights = [&](uint32_t n, uint32_t b) { return n * whole_weight(weight(r, value_at(b))); };
+        run_up(((int)floor_ + 63) / 64, [&](const uint4& q, int b) {
+            uint64_t v = 0;
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t n0 = counted(w[i], 0), n1 = counted(w[i], 1);
+                if (n0 && (uint32_t)b + 2 * i < floor_) v += weights(n0, b + 2 * i);
+                if (n1 && (uint32_t)b + 2 * i + 1 < floor_) v += weights(n1, b + 2 * i + 1);
+            }
+            return v;
+        });
+        const uint64_t above = s.sums[SK_GROUPS - 1];
+        uint64_t kept = above + ties * tied, before, w;
+        uint32_t last = ties ? floor_ : SK_BINS;   // bin of the last value that is kept, where a filter has set one
+        auto ends = [&](uint64_t X) {              // the bin in which the front part that reaches X ends; what lies in front of it; its weight
+            uint32_t b = floor_;
+            before = above, w = tied;
+            if (X <= above) {
+                const At f = reach(X, floor_, weights);
+                b = f.bin, before = f.before, w = whole_weight(weight(r, value_at(b)));
+            }
+            return b;
+        };
+        if (p < 1.0) {
+            const uint64_t X = min(kept, (uint64_t)fmax(1.0, ceil(p * (double)kept)));
+            last = ends(X);
+            kept = before + (X - before + w - 1) / w * w;
+        }
+        if (m > 0.0 && !(last < SK_BINS && weight(r, value_at(last)) >= m)) {
+            // the last bin whose weight is m or more lies near this one; weights fall from bin to bin
+            const int near = (int)bin_at(top < INFINITY ? fminf(top, (float)fmax(-3.4e38, (double)top + T * log(m))) : top), b = near - 15 + lane;
+            const bool large = b < (int)top_bin || (b < K::NEG_INF && weight(r, value_at((uint32_t)b)) >= m);
+            const int to = near - 16 + __popc(__ballot_sync(0xffffffffu, large));
+            // the sum up to that bin
+            uint64_t sum = 0;
+            if (to >= 0) {
+                const int g = to >> 6;
+                const uint32_t word = words[g * 32 + lane], c = g * 64 + 2 * lane;
+                const uint32_t n0 = counted(word, 0), n1 = counted(word, 1);
+                if (n0 && c < floor_ && (int)c <= to) sum += weights(n0, c);
+                if (n1 && c + 1 < floor_ && (int)c + 1 <= to) sum += weights(n1, c + 1);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                sum += g ? s.sums[g - 1] : 0;
+            }
+            kept = max(SP_ONE, min(kept, sum));
+        }
+        const uint64_t X = min(kept, (uint64_t)floor(u * (double)kept) + 1);
+        bin = ends(X);
+        ordinal = (X - before + w - 1) / w - 1;
+        logp = -log((double)kept * (1.0 / SP_ONE));
+        if (value_at(bin) != top) logp += ((double)value_at(bin) - (double)top) / T;
+    }
+    // the value of that bin with `ordinal` of them in front of it
+    const uint32_t as = bits_of_bin(bin) * 0x00010001u;
+    auto matching = [&](int c) {   // a bit for each of a piece's values
+        if (c >= end) return 0u;
+        const uint4 q = piece(c);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mask |= (K::same(w[i], as) & 0x00020001u) << (2 * i);   // (bits 0 and 17)
+        return (mask | mask >> 16) & 0xffu;
+    };
+    uint32_t n = 0;
+#pragma unroll 4
+    for (int c = own; c < end; c += 32) n += __popc(matching(c));
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) s.matches[warp] = n;
+    __syncthreads();
+    uint32_t ahead = __reduce_add_sync(0xffffffffu, lane < warp ? s.matches[lane] : 0u);
+    if (ordinal < ahead || ordinal >= (uint64_t)ahead + n) return;
+    for (int c0 = warp * per_warp; c0 < end; c0 += 32) {
+        uint32_t mask = matching(c0 + lane), up = __popc(mask);
+        const uint32_t mine = up;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, up, o);
+            if (lane >= o) up += v;
+        }
+        const uint32_t from = ahead + up - mine;
+        if (ordinal >= from && ordinal < from + mine) {
+            for (uint32_t i = from; i < ordinal; ++i) mask &= mask - 1;
+            a.ids[row] = (int64_t)(c0 + lane) * 8 - skip + __ffs(mask) - 1;
+            a.logp[row] = (float)logp;
+        }
+        ahead += __shfl_sync(0xffffffffu, up, 31);
+    }
+}
+template <class E>
+int sample_keys_launch(SampleArgs a, cudaStream_t st) {
+    static PerDeviceOnce once;
+    const DeviceProps* dev;
+    const auto kernel = sample_keys_kernel<E>;
+    const int err = once.run(&dev, [&](const DeviceProps&) -> int {
+        return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(KeyShared)), "cudaFuncSetAttribute(sampling)");
+    });
+    if (err != OK) return err;
+    AB_CHECK_ARG(a.rows <= INT32_MAX, "sampling: too many rows");
+    a.ahead = dev->n_sm;
+    kernel<<<(unsigned)a.rows, SK_NT, sizeof(KeyShared), st>>>(a);
+    AB_CUDA(cudaGetLastError());
+    return OK;
+}
+
 template <class E>
 int sample_launch(SampleArgs a, cudaStream_t st) {
     constexpr int PER = 16 / sizeof(E), NT = 1024;
@@ -850,7 +1171,8 @@ int sample_launch(SampleArgs a, cudaStream_t st) {
 }  // namespace
 
 int sample_filtered(int dtype, int64_t rows, int V, const void* logits, int64_t stride, const float* u, const ab_sampling& p, int64_t* ids, float* logp, cudaStream_t st) {
-    const SampleArgs a = {logits, u, p.temperature, p.top_p, p.min_p, p.top_k, p.temperature_all, p.top_p_all, p.min_p_all, p.top_k_all, V, rows, stride, ids, logp, 0};
+    const SampleArgs a = {logits, u, p.temperature, p.top_p, p.min_p, p.top_k, p.temperature_all, p.top_p_all, p.min_p_all, p.top_k_all, V, rows, stride, ids, logp, 0, 0};
+    if (V <= SK_BINS && dtype != AB_DT_F32) return dtype == AB_DT_F16 ? sample_keys_launch<__half>(a, st) : sample_keys_launch<__nv_bfloat16>(a, st);
     return dtype == AB_DT_F16 ? sample_launch<__half>(a, st) : dtype == AB_DT_BF16 ? sample_launch<__nv_bfloat16>(a, st) : sample_launch<float>(a, st);
 }
 

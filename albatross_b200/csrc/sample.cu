@@ -122,6 +122,137 @@ struct Found {
     uint64_t before;      // sum in front of the first of them
 };
 
+// A row's filters.
+struct RowFilters {
+    double T, p, m, u;
+    int k;
+    bool by_rank, by_sum, by_size, greedy;
+    __device__ __forceinline__ RowFilters(const SampleArgs& a, int64_t row) {
+        T = a.T ? (double)a.T[row] : a.T_all, p = a.p ? (double)a.p[row] : a.p_all, m = a.m ? (double)a.m[row] : a.m_all, k = a.k ? a.k[row] : a.k_all;
+        u = fmin(fmax((double)a.u[row], 0.0), 1.0);
+        by_rank = k > 0 && k < a.V, by_sum = p < 1.0, by_size = m > 0.0, greedy = !(T > 0.0 && k != 1 && a.V > 1);
+    }
+    // a value below which none has a weight of m (a little too low: the weights decide)
+    __device__ __forceinline__ float size_bound(float top) const {
+        const float least = m >= 1.0 ? top : fminf(top, (float)fmax(-3.4e38, (double)top + T * log(m) * (1 + 1e-6)));
+        return least - 1e-6f * fabsf(least);
+    }
+};
+
+enum SampleState : int { SP_LOOK, SP_DONE, SP_AGAIN };   // the row has its id; it has to be done in whole numbers
+
+// Few values of a row (key and id of each), sorted, and what they answer: by a block's first `size` threads.
+struct FewShared {
+    uint64_t red[32], told[2];
+    uint32_t votes[2][32], n[2];
+};
+template <int NT>
+struct Few {
+    FewShared& s;
+    uint64_t* lists;       // two of NT values, and two buffers
+    int lane, warp, size, turn;   // (two buffers in turn for what the threads tell each other: one barrier each)
+    static __device__ __forceinline__ uint64_t entry(float v, int id) { return (uint64_t)key_of(v) << 32 | (0xffffffffu - (uint32_t)id); }
+    __device__ __forceinline__ bool begin(uint32_t n) {   // whether this thread takes part in work on n values
+        size = n <= 32 ? 32 : 1 << (32 - __clz(n - 1)), turn = 0;
+        return (int)threadIdx.x < size;
+    }
+    __device__ __forceinline__ void meet() {
+        if (size == 32) __syncwarp();
+        else asm volatile("bar.sync 1, %0;" ::"r"(size) : "memory");
+    }
+    __device__ __forceinline__ uint32_t vote(bool yes) {   // how many
+        uint32_t n = __popc(__ballot_sync(0xffffffffu, yes));
+        if (size == 32) return n;
+        turn ^= 1;
+        if (lane == 0) s.votes[turn][warp] = n;
+        meet();
+        return __reduce_add_sync(0xffffffffu, 32 * lane < size ? s.votes[turn][lane] : 0u);
+    }
+    __device__ __forceinline__ uint64_t tell(bool mine, uint64_t v) {   // that of the thread for which it is `mine`
+        turn ^= 1;
+        if (mine) s.told[turn] = v;
+        meet();
+        return s.told[turn];
+    }
+    __device__ __forceinline__ uint64_t running(uint64_t v) {   // over the threads up to this one
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t w = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += w;
+        }
+        if (size == 32) return v;
+        if (lane == 31) s.red[warp] = v;
+        meet();
+        uint64_t ahead = lane < warp ? s.red[lane] : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+        return v + ahead;
+    }
+    // thread r's: the r-th of n <= size values, larger ones first (0 behind them)
+    __device__ uint64_t sorted(const uint64_t* list, uint32_t n) {
+        const uint32_t i = threadIdx.x;
+        uint64_t v = i < n ? list[i] : 0;
+        for (uint32_t run = 2; run <= (uint32_t)size; run *= 2)
+            for (uint32_t far = run / 2; far > 0; far /= 2) {
+                uint64_t other;
+                if (far >= 32) {
+                    turn ^= 1;
+                    uint64_t* x = lists + NT * (2 + turn);
+                    x[i] = v;
+                    meet();
+                    other = x[i ^ far];
+                } else {
+                    other = __shfl_xor_sync(0xffffffffu, v, far);
+                }
+                const bool larger = ((i & far) == 0) == ((i & run) == 0);
+                v = larger == (v > other) ? v : other;
+            }
+        return v;
+    }
+    // Of the n values of a list, behind a sum `front` of all in front of them: what is kept (`ends`: with total the row's sum; under top_k that of the first k is theirs), and
+    // the draw (`draws`). front, and total, may be `off` relative.
+    __device__ SampleState answer(const RowFilters& f, const RowScale& r, const uint64_t* list, uint32_t n, uint64_t front, uint64_t total, double off, bool from_top, bool ends,
+                                  bool draws, uint64_t& kept, int64_t* id, float* logp) {
+        const uint64_t e = sorted(list, n);
+        const float v = value_of((uint32_t)(e >> 32));
+        const bool on = threadIdx.x < n;
+        const double wd = on ? weight(r, v) : 0.0;
+        const uint64_t w = whole_weight(wd), cum = front + running(w), before = cum - w;
+        // whether X is met too closely, or not at all
+        auto unsure = [&](uint64_t X) {
+            const double slack = off * ((double)front + (double)X);
+            const bool close = on && fabs((double)cum - (double)X) <= slack, met = on && (double)cum >= (double)X + slack;
+            return vote(close) != 0 || vote(met) == 0 || (!from_top && (double)front + slack >= (double)X);
+        };
+        if (ends) {
+            uint32_t count = f.by_rank ? min((uint32_t)f.k, n) : n;
+            if (f.by_rank) total = tell(threadIdx.x + 1 == count, cum);
+            if (f.by_sum) {
+                const uint64_t X = (uint64_t)fmax(1.0, ceil(f.p * (double)total));
+                if (off > 0 && unsure(X)) return SP_AGAIN;
+                count = min(count, vote(on && before < X));
+            }
+            if (f.by_size) {
+                const uint32_t large = vote(on && wd >= f.m);
+                if (!from_top && large < count) return SP_AGAIN;   // (the end may lie in front of these)
+                count = max(1u, min(count, large));
+            }
+            kept = f.by_rank || f.by_sum || f.by_size ? tell(threadIdx.x + 1 == count, cum) : total;
+        }
+        if (draws) {
+            const uint64_t X = min(kept, (uint64_t)floor(f.u * (double)kept) + 1);
+            if (off > 0 && (!from_top || !(f.by_sum || f.by_size)) && unsure(X)) return SP_AGAIN;
+            if (on && before < X && X <= cum) {
+                *id = 0xffffffffu - (uint32_t)e;
+                double l = -log((double)kept * (1.0 / SP_ONE));
+                if (v != r.top) l += ((double)v - (double)r.top) / f.T;
+                *logp = (float)l;
+            }
+        }
+        return SP_DONE;
+    }
+};
+
 template <int NT>
 struct alignas(16) SampleShared {
     uint64_t cum[SP_BINS], sub[SP_SUB];
@@ -130,17 +261,15 @@ struct alignas(16) SampleShared {
     double tab[16];
     uint64_t red[NT / 32], mine;
     double part_sum[2];
-    uint32_t least, most, n[2], matches[NT / 32], matched;
+    uint64_t kept;
+    FewShared few;
+    uint32_t least, most, matches[NT / 32], matched;
     uint32_t top, tops[NT / 32];
     uint32_t digit, left, bound;          // of the search among the threads' maxima
-    uint32_t votes[2][NT / 32];
-    uint64_t told[2];
     int state;                            // what comes next: the bins of up to two brackets, or a SampleState
     int bins[4];
     Found found;
 };
-enum SampleState : int { SP_LOOK, SP_DONE, SP_AGAIN };   // the row has its id; it has to be done in whole numbers
-
 template <class E, int NT>
 struct Sampler {
     static constexpr int PER = 16 / sizeof(E), WARPS = NT / 32;
@@ -208,44 +337,11 @@ struct Sampler {
         atomicAdd(&s.part[1][bin], (uint32_t)(w >> 15) & 0x7fffu);
         atomicAdd(&s.part[2][bin], (uint32_t)(w >> 30));
     }
-    // ---- few values: key and id of each, in the first block, which works on them with its first `size` threads
-    __device__ __forceinline__ uint64_t* few() { return reinterpret_cast<uint64_t*>(s.part[1]); }   // 4 NT of them
+    // ---- few values, in the first block
+    __device__ __forceinline__ uint64_t* lists() { return reinterpret_cast<uint64_t*>(s.part[1]); }   // 4 NT of them
     __device__ __forceinline__ void keep(float v, int id, int list = 0) {
-        const uint32_t at = atomicAdd(of(&s.n[list], 0), 1u);
-        if (at < (uint32_t)NT) of(few() + NT * list, 0)[at] = (uint64_t)key_of(v) << 32 | (0xffffffffu - (uint32_t)id);
-    }
-    int size, turn;        // (two buffers in turn for what the threads tell each other: one barrier each)
-    __device__ __forceinline__ void meet() {
-        if (size == 32) __syncwarp();
-        else asm volatile("bar.sync 1, %0;" ::"r"(size) : "memory");
-    }
-    __device__ __forceinline__ uint32_t vote(bool yes) {   // how many
-        uint32_t n = __popc(__ballot_sync(0xffffffffu, yes));
-        if (size == 32) return n;
-        turn ^= 1;
-        if (lane == 0) s.votes[turn][warp] = n;
-        meet();
-        return __reduce_add_sync(0xffffffffu, 32 * lane < size ? s.votes[turn][lane] : 0u);
-    }
-    __device__ __forceinline__ uint64_t tell(bool mine, uint64_t v) {   // that of the thread for which it is `mine`
-        turn ^= 1;
-        if (mine) s.told[turn] = v;
-        meet();
-        return s.told[turn];
-    }
-    __device__ __forceinline__ uint64_t running(uint64_t v) {   // over the threads up to this one
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t w = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += w;
-        }
-        if (size == 32) return v;
-        if (lane == 31) s.red[warp] = v;
-        meet();
-        uint64_t ahead = lane < warp ? s.red[lane] : 0;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
-        return v + ahead;
+        const uint32_t at = atomicAdd(of(&s.few.n[list], 0), 1u);
+        if (at < (uint32_t)NT) of(lists() + NT * list, 0)[at] = Few<NT>::entry(v, id);
     }
     // A bound that at least k of this block's threads reach with their maxima (to its upper 16 bits), or 0. Each digit by a histogram of the threads.
     __device__ uint32_t reached(uint32_t k, uint32_t key) {
@@ -282,28 +378,6 @@ struct Sampler {
         }
         return bound;
     }
-    // thread r's: the r-th of n <= size values, larger ones first (0 behind them)
-    __device__ uint64_t sorted(const uint64_t* list, uint32_t n) {
-        const uint32_t i = threadIdx.x;
-        uint64_t v = i < n ? list[i] : 0;
-        for (uint32_t run = 2; run <= (uint32_t)size; run *= 2)
-            for (uint32_t far = run / 2; far > 0; far /= 2) {
-                uint64_t other;
-                if (far >= 32) {
-                    turn ^= 1;
-                    uint64_t* x = few() + NT * (2 + turn);
-                    x[i] = v;
-                    meet();
-                    other = x[i ^ far];
-                } else {
-                    other = __shfl_xor_sync(0xffffffffu, v, far);
-                }
-                const bool larger = ((i & far) == 0) == ((i & run) == 0);
-                v = larger == (v > other) ? v : other;
-            }
-        return v;
-    }
-
     // running sums of the histogram, over all blocks; every block has them
     template <int BINS>
     __device__ __forceinline__ void run_up(uint64_t* cum) {
@@ -351,12 +425,12 @@ struct Sampler {
         uint32_t lo = 0, hi = 0xffffffffu;
         for (int level = 0;; ++level) {
             auto inside = [&](float v, uint32_t key) { return key > floor_ && (level ? key >= lo && key <= hi : bin_of(r, v) == bin); };
-            if (threadIdx.x == 0) s.n[0] = 0, s.least = 0xffffffffu, s.most = 0;
+            if (threadIdx.x == 0) s.few.n[0] = 0, s.least = 0xffffffffu, s.most = 0;
             __syncthreads();
             each([&](float v) {
                 const uint32_t key = key_of(v);
                 if (!inside(v, key)) return;
-                const uint32_t at = atomicAdd(&s.n[0], 1u);
+                const uint32_t at = atomicAdd(&s.few.n[0], 1u);
                 if (at < SP_LIST) s.own[at] = key;
                 atomicMin(&s.least, key);
                 atomicMax(&s.most, key);
@@ -365,7 +439,7 @@ struct Sampler {
             uint32_t n = 0;
             lo = 0xffffffffu, hi = 0;
             for (int b = 0; b < blocks; ++b) {
-                const uint32_t have = *of(&s.n[0], b);
+                const uint32_t have = *of(&s.few.n[0], b);
                 if (n + have <= SP_LIST)
                     for (uint32_t i = threadIdx.x; i < have; i += NT) s.list[n + i] = *of(&s.own[0] + i, b);
                 n += have;
@@ -428,9 +502,11 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
     x.pieces = max(0, min(a.share, all_pieces - first));
     x.per_warp = (x.pieces + NT - 1) / NT * 32;
     if (threadIdx.x < 16) s.tab[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
-    if (threadIdx.x < 2) s.n[threadIdx.x] = 0;
-    const double T = a.T ? (double)a.T[row] : a.T_all, p = a.p ? (double)a.p[row] : a.p_all, m = a.m ? (double)a.m[row] : a.m_all, u = fmin(fmax((double)a.u[row], 0.0), 1.0);
-    const int k = a.k ? a.k[row] : a.k_all;
+    if (threadIdx.x < 2) s.few.n[threadIdx.x] = 0;
+    const RowFilters f = RowFilters(a, row);
+    const double T = f.T, p = f.p, m = f.m, u = f.u;
+    const int k = f.k;
+    const bool by_rank = f.by_rank, by_sum = f.by_sum, by_size = f.by_size, greedy = f.greedy;
     const int own = x.warp * x.per_warp + x.lane, end = min(x.pieces, (x.warp + 1) * x.per_warp);   // a thread's pieces: own, own + 32 ..
     float top = -INFINITY;
     {
@@ -469,54 +545,11 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
         return;
     }
     top = value_of(key);
-    const bool greedy = !(T > 0.0 && k != 1 && a.V > 1);
     x.r = {top, 0.f, 1.4426950408889634074 / T, s.tab};
-    const bool by_rank = k > 0 && k < a.V, by_sum = p < 1.0, by_size = m > 0.0;
     const int first_id = first * PER - skip;
 
-    // Of the n values of a list, behind a sum `front` of all in front of them: what is kept (`ends`: with total the row's sum, or 0: that of the first k is theirs), and the
-    // draw (`draws`). front, and total, may be `off` relative. In the first block, by its first x.size threads; the others wait.
+    Few<NT> few = {s.few, x.lists(), x.lane, x.warp, 32, 0};
     uint64_t kept = 0;
-    auto answer = [&](const uint64_t* list, uint32_t n, uint64_t front, uint64_t total, double off, bool from_top, bool ends, bool draws) {
-        const uint64_t e = x.sorted(list, n);
-        const float v = value_of((uint32_t)(e >> 32));
-        const bool on = threadIdx.x < n;
-        const double wd = on ? weight(x.r, v) : 0.0;
-        const uint64_t w = whole_weight(wd), cum = front + x.running(w), before = cum - w;
-        // whether X is met too closely, or not at all
-        auto unsure = [&](uint64_t X) {
-            const double slack = off * ((double)front + (double)X);
-            const bool close = on && fabs((double)cum - (double)X) <= slack, met = on && (double)cum >= (double)X + slack;
-            return x.vote(close) != 0 || x.vote(met) == 0 || (!from_top && (double)front + slack >= (double)X);
-        };
-        if (ends) {
-            uint32_t count = by_rank ? min((uint32_t)k, n) : n;
-            if (by_rank) total = x.tell(threadIdx.x + 1 == count, cum);
-            if (by_sum) {
-                const uint64_t X = (uint64_t)fmax(1.0, ceil(p * (double)total));
-                if (off > 0 && unsure(X)) return SP_AGAIN;
-                count = min(count, x.vote(on && before < X));
-            }
-            if (by_size) {
-                const uint32_t large = x.vote(on && wd >= m);
-                if (!from_top && large < count) return SP_AGAIN;   // (the end may lie in front of these)
-                count = max(1u, min(count, large));
-            }
-            kept = by_rank || by_sum || by_size ? x.tell(threadIdx.x + 1 == count, cum) : total;
-        }
-        if (draws) {
-            const uint64_t X = min(kept, (uint64_t)floor(u * (double)kept) + 1);
-            if (off > 0 && (!from_top || !(by_sum || by_size)) && unsure(X)) return SP_AGAIN;
-            if (on && before < X && X <= cum) {
-                a.ids[row] = 0xffffffffu - (uint32_t)e;
-                double logp = -log((double)kept * (1.0 / SP_ONE));
-                if (v != top) logp += ((double)v - (double)top) / T;
-                a.logp[row] = (float)logp;
-            }
-        }
-        return SP_DONE;
-    };
-    auto width = [](uint32_t n) { return n <= 32 ? 32 : 1 << (32 - __clz(n - 1)); };   // threads for n values
     bool done = false;
     if (!greedy && ((by_rank && k <= 600 / x.blocks) || (!by_rank && !by_sum && by_size && top < INFINITY))) {
         // ---- few values
@@ -529,9 +562,8 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
                 for (int b = 0; b < x.blocks; ++b) bound = max(bound, *x.of(&s.bound, b));
             }
             least = bound > key_of(-INFINITY) ? value_of(bound) : -INFINITY;
-        } else {   // (a little too low: the weights decide)
-            least = m >= 1.0 ? top : fminf(top, (float)fmax(-3.4e38, (double)top + T * log(m) * (1 + 1e-6)));
-            least -= 1e-6f * fabsf(least);
+        } else {
+            least = f.size_bound(top);
         }
         __syncthreads();
         for (int c = own; c < end; c += 32) {
@@ -544,10 +576,9 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
                 if (v[i] >= least && v[i] > -INFINITY) x.keep(v[i], first_id + c * PER + i);
         }
         x.join();
-        const uint32_t n = *x.of(&s.n[0], 0);
+        const uint32_t n = *x.of(&s.few.n[0], 0);
         if (n <= (uint32_t)NT) {   // (the same in all blocks)
-            x.size = width(n), x.turn = 0;
-            if (x.rank == 0 && (int)threadIdx.x < x.size) answer(x.few(), n, 0, 0, 0.0, true, true, true);
+            if (x.rank == 0 && few.begin(n)) few.answer(f, x.r, x.lists(), n, 0, 0, 0.0, true, true, true, kept, a.ids + row, a.logp + row);
             done = true;
         }
         if (x.blocks > 1) x.cluster.sync();   // (the first block's count has been read)
@@ -682,21 +713,18 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
             }
             block_sums(mine, ahead, sums);
             if (x.rank == 0) {
-                const uint32_t n0 = s.n[0], n1 = s.n[1];
+                const uint32_t n0 = s.few.n[0], n1 = s.few.n[1];
                 const uint64_t front = from_top ? 0 : (uint64_t)(sums[0] * SP_ONE);
                 state = n0 <= (uint32_t)NT && n1 <= (uint32_t)NT ? SP_DONE : SP_AGAIN;
                 if (two && state == SP_DONE) {
-                    x.size = width(n1), x.turn = 0;
-                    if ((int)threadIdx.x < x.size) state = answer(x.few() + NT, n1, (uint64_t)(sums[1] * SP_ONE), whole, EPS, false, true, false);
-                    if (threadIdx.x == 0) s.state = state, s.told[0] = kept;
+                    if (few.begin(n1)) state = few.answer(f, x.r, x.lists() + NT, n1, (uint64_t)(sums[1] * SP_ONE), whole, EPS, false, true, false, kept, nullptr, nullptr);
+                    if (threadIdx.x == 0) s.state = state, s.kept = kept;
                     __syncthreads();
-                    state = s.state, kept = s.told[0];
+                    state = s.state, kept = s.kept;
                     __syncthreads();
                 }
-                if (state == SP_DONE) {
-                    x.size = width(n0), x.turn = 0;
-                    if ((int)threadIdx.x < x.size) state = answer(x.few(), n0, front, whole, EPS, from_top, !two, true);
-                }
+                if (state == SP_DONE && few.begin(n0))
+                    state = few.answer(f, x.r, x.lists(), n0, front, whole, EPS, from_top, !two, true, kept, a.ids + row, a.logp + row);
                 if (threadIdx.x == 0) s.state = state;
             }
             x.join();
@@ -816,25 +844,27 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
 
 // ---- 16-bit logits: one counter for each of their 65536 values ------------------------------------------------------------------------------
 // A row's histogram over the values themselves, in shared memory, says everything but which id has a value: what is kept and drawn is found among the
-// counters, whose running sums are exact, and the row is read once more (from L2) for the id. No value of the row needs an exponential: the counters in use, some
-// 15 000 of a row of 65536 fp16 logits, do. What bounds it: the atomics (3.3 cycles for a warp's, two values meet a bank), then the counters' weights in 64 bits.
+// counters, whose running sums are exact, and the row is read once more (from L2) for the id. No value of the row needs an exponential: the counters do, and eight
+// of them that follow one another, a unit, whose values are equally far apart, need one of them and its products with exp(-distance / T). Where the filters leave
+// few values (top-k; min-p by itself), only those are counted that reach a bound: some k of the threads' own maxima do, and so do k values.
+// What bounds it: the atomics (3.3 cycles for a warp's: two of its values meet a bank), then the units' weights.
 //
-// Counters lie in the order of the values, larger ones first, eight in 16 bytes: a unit. Eight units are a group; a warp's eight lanes take one at a time, and groups
+// Counters lie in the order of the values, larger ones first, eight in 16 bytes. Eight units are a group; a warp's eight lanes take one at a time, and groups
 // go round the warps, since values lie densely in a few binades. Sums of groups are run up over the block; a question is answered by a search among them and by the 64
-// counters of one group, by every warp for itself.
+// counters of one group, by the first warp.
 //
 // A counter holds up to 65535: the row's last value is added when the others are counted, so that only a row of 65536 equal ones exceeds it (`extra`).
 constexpr int SK_NT = 1024, SK_BINS = 65536, SK_GROUPS = SK_BINS / 64, SK_ROUNDS = SK_BINS / 8 / SK_NT;
 
 template <class E> struct KeyType;   // how a type's 16 bits are ordered
 template <> struct KeyType<__half> {
-    static constexpr int NEG_INF = 0xfc00;   // its bin; NaNs lie behind it, and in front of the other infinity
+    static constexpr int NEG_INF = 0xfc00, MANTISSA = 10, EXPONENTS = 32, LEAST = -24;   // bin of -inf (NaNs lie behind it, and in front of the other infinity); 2^LEAST is the smallest value
     static __device__ __forceinline__ uint32_t same(uint32_t two, uint32_t as) {   // 16 bits of ones where equal (0 and -0 are)
         return __heq2_mask(*reinterpret_cast<const __half2*>(&two), *reinterpret_cast<const __half2*>(&as));
     }
 };
 template <> struct KeyType<__nv_bfloat16> {
-    static constexpr int NEG_INF = 0xff80;
+    static constexpr int NEG_INF = 0xff80, MANTISSA = 7, EXPONENTS = 256, LEAST = -133;
     static __device__ __forceinline__ uint32_t same(uint32_t two, uint32_t as) {
         return __heq2_mask(*reinterpret_cast<const __nv_bfloat162*>(&two), *reinterpret_cast<const __nv_bfloat162*>(&as));
     }
@@ -843,12 +873,15 @@ __device__ __forceinline__ uint32_t bits_of_bin(uint32_t bin) { return bin < 0x8
 __device__ __forceinline__ uint32_t bin_of_bits(uint32_t bits) { return bits == 0x8000u ? 0x7fffu : bits < 0x8000u ? 0x7fffu - bits : bits; }
 
 struct alignas(16) KeyShared {
-    uint4 counts[SK_BINS / 8];
+    uint4 counts[SK_BINS / 8];   // (or the lists of few values)
     uint64_t sums[SK_GROUPS];
+    double step[256][8];         // exp(-j * (distance of two neighbours) / T), by their exponent
     uint64_t red[32];
     double tab[16];
+    FewShared few;
     uint32_t tops[32], matches[32];
-    uint32_t extra;
+    uint32_t extra, bin;
+    uint64_t ties, tied, ordinal;
 };
 
 template <class E>
@@ -860,18 +893,9 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
     const int64_t row = blockIdx.x;
     const E* logits = static_cast<const E*>(a.logits) + row * a.stride;
     const Extent all = rows_extent(a.logits, a.rows, a.stride, a.V, 2);
-    for (int i = threadIdx.x; i < SK_BINS / 8; i += SK_NT) s.counts[i] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x < 16) s.tab[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
-    if (threadIdx.x == 0) s.extra = 0;
-    const double T = a.T ? (double)a.T[row] : a.T_all, p = a.p ? (double)a.p[row] : a.p_all, m = a.m ? (double)a.m[row] : a.m_all, u = fmin(fmax((double)a.u[row], 0.0), 1.0);
-    const int k = a.k ? a.k[row] : a.k_all;
     // the row from its last 16-byte boundary on, as pieces of eight values; a warp's pieces follow one another
     const int skip = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / 2), pieces = (skip + a.V + 7) / 8;
     const int per_warp = (pieces + SK_NT - 1) / SK_NT * 32, own = warp * per_warp + lane, end = min(pieces, (warp + 1) * per_warp);
-    if (row + a.ahead < a.rows) {   // a row that a block will take when this one is done
-        const char* next = reinterpret_cast<const char*>(static_cast<const E*>(a.logits) + (row + a.ahead) * a.stride) + (size_t)threadIdx.x * 128;
-        if ((int64_t)threadIdx.x * 64 < a.V) asm volatile("prefetch.global.L2 [%0];" ::"l"(next));
-    }
     auto piece = [&](int c) {   // (values outside of the row: -inf)
         const int at = c * 8 - skip;
         uint4 q = make_uint4(0, 0, 0, 0);
@@ -885,30 +909,58 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
         }
         return q;
     };
-    __syncthreads();
-    uint32_t* words = reinterpret_cast<uint32_t*>(s.counts);
-    float top = -INFINITY;
-    auto count = [&](uint32_t bin) { atomicAdd(words + (bin >> 1), bin & 1 ? 0x10000u : 1u); };
-    for (int c0 = own; c0 < end; c0 += 32 * 4) {
-        uint4 q[4];
+    // all of it under way at once (a row that begins off a boundary has one piece more for some threads)
+    constexpr int AHEAD = 8;
+    uint4 q[AHEAD];
+    auto request = [&](int c0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < AHEAD; ++j)
             if (c0 + 32 * j < end) q[j] = piece(c0 + 32 * j);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = c0 + 32 * j;
-            if (c >= end) continue;
-            top = larger_or_nan(top, largest<E>(q[j]));
-            const int at = c * 8 - skip;
-            const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
-            const bool whole = at >= 0 && at + 8 < a.V;   // (the last value is added below)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t sign = (w[i] >> 15) & 0x00010001u, bins = w[i] ^ (0x7fff7fffu - sign * 0x7fffu);
-                if (whole || (at + 2 * i >= 0 && at + 2 * i < a.V - 1)) count(bins & 0xffffu);
-                if (whole || (at + 2 * i + 1 >= 0 && at + 2 * i + 1 < a.V - 1)) count(bins >> 16);
-            }
+    };
+    request(own);
+    const RowFilters f = RowFilters(a, row);
+    if (row + a.ahead < a.rows) {   // a row that a block will take when this one is done
+        const char* next = reinterpret_cast<const char*>(static_cast<const E*>(a.logits) + (row + a.ahead) * a.stride) + (size_t)threadIdx.x * 128;
+        if ((int64_t)threadIdx.x * 64 < a.V) asm volatile("prefetch.global.L2 [%0];" ::"l"(next));
+    }
+    const bool bounded = f.by_rank ? f.k <= 600 : !f.by_sum && f.by_size, counting = !f.greedy && !bounded;
+    uint32_t* words = reinterpret_cast<uint32_t*>(s.counts);
+    auto count = [&](uint32_t bin) { atomicAdd(words + (bin >> 1), bin & 1 ? 0x10000u : 1u); };
+    auto clear = [&]() {
+        for (int i = threadIdx.x; i < SK_BINS / 8; i += SK_NT) s.counts[i] = make_uint4(0, 0, 0, 0);
+        if (threadIdx.x == 0) s.extra = 0;
+        const int e = threadIdx.x >> 2, j = (threadIdx.x & 3) * 2;
+        if (e < K::EXPONENTS) {
+            const double far = scalbn(1.0, max(e, 1) - 1 + K::LEAST) / f.T;
+            s.step[e][j] = j ? exp(-far * j) : 1.0, s.step[e][j + 1] = exp(-far * (j + 1));   // (far may be infinite)
         }
+    };
+    auto count_piece = [&](const uint4& q, int c) {
+        const int at = c * 8 - skip;
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        const bool whole = at >= 0 && at + 8 < a.V;   // (the last value is added below)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t sign = (w[i] >> 15) & 0x00010001u, bins = w[i] ^ (0x7fff7fffu - sign * 0x7fffu);
+            if (whole || (at + 2 * i >= 0 && at + 2 * i < a.V - 1)) count(bins & 0xffffu);
+            if (whole || (at + 2 * i + 1 >= 0 && at + 2 * i + 1 < a.V - 1)) count(bins >> 16);
+        }
+    };
+    if (threadIdx.x < 16) s.tab[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
+    if (threadIdx.x < 2) s.few.n[threadIdx.x] = 0;
+    if (counting) {
+        clear();
+        __syncthreads();
+    }
+    float top = -INFINITY;
+    for (int c0 = own; c0 < end; c0 += 32 * AHEAD) {
+        if (c0 != own) request(c0);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (c0 + 32 * j < end) {
+                top = larger_or_nan(top, largest<E>(q[j]));
+                if (counting) count_piece(q[j], c0 + 32 * j);
+            }
     }
     const uint32_t own_top = own < end ? (top == top ? key_of(top) : 0xffffffffu) : 0;   // a NaN on top of all
     uint32_t top_key = __reduce_max_sync(0xffffffffu, own_top);
@@ -919,19 +971,65 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
         if (threadIdx.x == 0) a.ids[row] = -1, a.logp[row] = NAN;
         return;
     }
-    top = value_of(top_key);
-    const bool greedy = !(T > 0.0 && k != 1 && a.V > 1);
-    const RowScale r = {top, 0.f, 1.4426950408889634074 / T, s.tab};
-    auto value_at = [&](uint32_t bin) { return to_f(from_bits<E>((unsigned short)bits_of_bin(bin))); };
     auto bin_at = [&](float v) {
         const E t = from_f<E>(v);
         return bin_of_bits(*reinterpret_cast<const unsigned short*>(&t));
     };
+    auto value_at = [&](uint32_t bin) { return to_f(from_bits<E>((unsigned short)bits_of_bin(bin))); };
+    const float own_largest = top;
+    top = value_of(top_key);
+    const RowScale r = {top, 0.f, 1.4426950408889634074 / f.T, s.tab};
+    if (bounded && !f.greedy) {
+        // ---- few values
+        float least = -INFINITY;
+        if (f.by_rank) {   // The largest of 16 bits that k threads' maxima reach, digit by digit; a little more than k will do.
+            const uint32_t mine = own < end ? 0xffffu - bin_at(own_largest) : 0;
+            uint32_t bound = 0;
+            for (int bit = 15; bit >= 0; --bit) {
+                const uint32_t t = bound | 1u << bit;
+                const int n = __syncthreads_count(mine >= t);
+                if (n < f.k) continue;
+                bound = t;
+                if (n <= f.k + f.k / 8 + 16) break;
+            }
+            if (bound > 0xffffu - K::NEG_INF) least = value_at(0xffffu - bound);
+        } else if (top < INFINITY) {
+            least = f.size_bound(top);
+        }
+        Few<SK_NT> few = {s.few, reinterpret_cast<uint64_t*>(s.counts), lane, warp, 32, 0};
+        for (int c0 = own; c0 < end; c0 += 32 * AHEAD) {
+            if (end - own > 32 * AHEAD) request(c0);   // (else it is still there)
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int c = c0 + 32 * j;
+                if (c >= end || !(largest<E>(q[j]) >= least)) continue;
+                float v[8];
+                unpack<E>(q[j], v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (v[i] >= least && v[i] > -INFINITY) {
+                        const uint32_t at = atomicAdd(&s.few.n[0], 1u);
+                        if (at < (uint32_t)SK_NT) few.lists[at] = few.entry(v[i], c * 8 - skip + i);
+                    }
+            }
+        }
+        __syncthreads();
+        const uint32_t n = s.few.n[0];
+        uint64_t kept = 0;
+        if (n <= (uint32_t)SK_NT) {
+            if (few.begin(n)) few.answer(f, r, few.lists, n, 0, 0, 0.0, true, true, true, kept, a.ids + row, a.logp + row);
+            return;
+        }
+        __syncthreads();
+        clear();   // (many equals, or a small min_p)
+        __syncthreads();
+        for (int c = own; c < end; c += 32) count_piece(piece(c), c);
+        __syncthreads();
+    }
     const uint32_t top_bin = bin_at(top);
     uint32_t bin = top_bin;
-    uint64_t ordinal = 0;
-    double logp = 0.0;
-    if (!greedy) {
+    uint64_t ordinal = 0, kept = SP_ONE;
+    if (!f.greedy) {
         if (threadIdx.x == 0) {   // -0 is 0, and the last value
             const uint32_t minus = words[0x4000] & 0xffffu;
             words[0x4000] -= minus;
@@ -946,26 +1044,32 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
             const uint32_t n = half ? word >> 16 : word & 0xffffu;
             return n == 0xffffu ? n + extra : n;
         };
-        // Sums of groups [first, last) of what `of` makes of a unit and its first bin, run up; all threads then have them in s.sums. (Group g: units 8 g .. 8 g + 7.)
+        // The weight of a bin's value, from that of its unit's first (of the largest value in its unit). One way for all who ask: sums are to agree to the last unit.
+        auto base_of = [&](uint32_t bin) { return max(bin & ~7u, top_bin); };
+        auto steps = [&](uint32_t bin) { return s.step[bits_of_bin(bin) >> K::MANTISSA & (K::EXPONENTS - 1)]; };
+        auto weight_at = [&](uint32_t bin) {
+            const uint32_t base = base_of(bin);
+            return weight(r, value_at(base)) * steps(bin)[bin - base & 7u];   // (1 times 1 for the largest value)
+        };
+        // Sums of the groups from `first` to `last` of what `of` makes of a unit and its first bin, run up; all threads then have them in s.sums, from 0 on. (Group g: units 8 g ..
+        // 8 g + 7.) Returns the sum of all.
         const int first = (int)(top_bin >> 6);
         auto run_up = [&](int last, auto of) {
-            __syncthreads();   // (s.sums, s.red)
-            for (int i = 0; i < SK_ROUNDS; ++i) {
-                const int group = i * 128 + (lane >> 3) * 32 + warp, unit = group * 8 + (lane & 7);
+            const int groups = last - first;
+            for (int i = 0; i * 128 < groups; ++i) {
+                const int group = i * 128 + (lane >> 3) * 32 + warp, unit = (first + group) * 8 + (lane & 7);
                 uint64_t v = 0;
-                if (i * 128 < last && (i + 1) * 128 > first) {   // (the same for the whole block)
-                    if (group >= first && group < last) {
-                        const uint4 q = s.counts[unit];
-                        if ((q.x | q.y | q.z | q.w) != 0) v = of(q, unit * 8);
-                    }
-                    v += __shfl_xor_sync(0xffffffffu, v, 1);
-                    v += __shfl_xor_sync(0xffffffffu, v, 2);
-                    v += __shfl_xor_sync(0xffffffffu, v, 4);
+                if (group < groups) {
+                    const uint4 q = s.counts[unit];
+                    if ((q.x | q.y | q.z | q.w) != 0) v = of(q, (uint32_t)unit * 8);
                 }
+                v += __shfl_xor_sync(0xffffffffu, v, 1);
+                v += __shfl_xor_sync(0xffffffffu, v, 2);
+                v += __shfl_xor_sync(0xffffffffu, v, 4);
                 if ((lane & 7) == 0) s.sums[group] = v;
             }
             __syncthreads();
-            uint64_t v = s.sums[threadIdx.x];
+            uint64_t v = (int)threadIdx.x < groups ? s.sums[threadIdx.x] : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint64_t w = __shfl_up_sync(0xffffffffu, v, o);
@@ -979,21 +1083,22 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
             s.sums[threadIdx.x] = v + before;
             __syncthreads();
         };
-        // Where the running sum reaches X: by every warp for itself. `one`: of a counter and its bin. Bins from `floor_` on do not count.
+        // Where the running sum reaches X (by one warp). `one`: of two neighbouring counters and the first one's bin. Bins from `floor_` on do not count.
         struct At {
-            uint32_t bin, n;   // n: its counter
-            uint64_t before;
+            uint32_t bin;
+            uint64_t before, one;   // one: what a value of the bin adds
+        };
+        struct Two {
+            uint64_t a, b;
         };
         auto reach = [&](uint64_t X, uint32_t floor_, auto one) {
-            int lo = 0, hi = SK_GROUPS - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (s.sums[mid] >= X) hi = mid;
-                else lo = mid + 1;
-            }
-            const uint32_t word = words[lo * 32 + lane], b = lo * 64 + 2 * lane;   // this lane's two counters
-            const uint32_t n0 = counted(word, 0), n1 = counted(word, 1);
-            const uint64_t v0 = n0 && b < floor_ ? one(n0, b) : 0, v1 = n1 && b + 1 < floor_ ? one(n1, b + 1) : 0;
+            // the group: 32 of the sums at a time
+            int lo = min(__popc(__ballot_sync(0xffffffffu, s.sums[lane * 32 + 31] < X)), 31) * 32;
+            lo = min(lo + __popc(__ballot_sync(0xffffffffu, s.sums[lo + lane] < X)), SK_GROUPS - 1 - first);
+            const uint32_t word = words[(first + lo) * 32 + lane], b = (first + lo) * 64 + 2 * lane;   // this lane's two counters
+            const uint32_t n0 = b < floor_ ? counted(word, 0) : 0, n1 = b + 1 < floor_ ? counted(word, 1) : 0;
+            const Two w = one(b);
+            const uint64_t v0 = n0 * w.a, v1 = n1 * w.b;
             uint64_t up = v0 + v1;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -1005,104 +1110,131 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
             const bool second = up - v1 < X;
             At out;
             out.bin = __shfl_sync(0xffffffffu, b + second, at & 31);
-            out.n = __shfl_sync(0xffffffffu, second ? n1 : n0, at & 31);
             out.before = __shfl_sync(0xffffffffu, second ? up - v1 : up - v1 - v0, at & 31);
+            out.one = __shfl_sync(0xffffffffu, second ? w.b : w.a, at & 31);
             return out;
         };
-        const bool by_rank = k > 0 && k < a.V;
+        // how many values of w make d, at least one: by a quotient that is off by one at most
+        auto how_many = [](uint64_t d, uint64_t w) {
+            uint64_t n = (uint64_t)__fdividef((float)d, (float)w);
+            while (n * w < d) ++n;
+            while (n > 1 && (n - 1) * w >= d) --n;
+            return n < 1 ? 1 : n;
+        };
         uint32_t floor_ = K::NEG_INF;     // bins from here on are not kept, or have no weight
         uint64_t ties = 0, tied = 0;
-        if (by_rank) {
-            auto ranks = [&](uint32_t n, uint32_t) { return (uint64_t)n; };
-            run_up(SK_GROUPS, [&](const uint4& q, int) {
-                uint64_t n = 0;
+        if (f.by_rank) {
+            run_up(SK_GROUPS, [&](const uint4& q, uint32_t) {
                 const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                uint32_t n = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) n += counted(w[i], 0) + counted(w[i], 1);
-                return n;
+                for (int i = 0; i < 4; ++i) n = __dp2a_lo(w[i], 0x0101u, n);
+                return (uint64_t)(extra ? (uint32_t)a.V : n);
             });
-            const At f = reach((uint64_t)k, SK_BINS, ranks);
-            if (f.bin < (uint32_t)K::NEG_INF) {
-                floor_ = f.bin;
-                ties = (uint64_t)k - f.before;
-                tied = whole_weight(weight(r, value_at(floor_)));
+            if (warp == 0) {
+                const At at = reach((uint64_t)f.k, SK_BINS, [](uint32_t) { return Two{1, 1}; });
+                const bool weighs = at.bin < (uint32_t)K::NEG_INF;
+                const uint64_t w = weighs ? whole_weight(weight_at(at.bin)) : 0;
+                if (lane == 0) s.bin = weighs ? at.bin : K::NEG_INF, s.ties = weighs ? (uint64_t)f.k - at.before : 0, s.tied = w;
             }
+            __syncthreads();
+            floor_ = s.bin, ties = s.ties, tied = s.tied;
         }
-        auto weights = [&](uint32_t n, uint32_t b) { return n * whole_weight(weight(r, value_at(b))); };
-        run_up(((int)floor_ + 63) / 64, [&](const uint4& q, int b) {
-            uint64_t v = 0;
+        auto weights = [&](uint32_t b) {   // (two neighbours are of one unit)
+            const uint32_t base = base_of(b);
+            const double w = weight(r, value_at(base));
+            const double* step = steps(b);
+            return Two{whole_weight(w * step[b - base & 7u]), whole_weight(w * step[b + 1 - base & 7u])};   // (in front of the largest value: of no counter)
+        };
+        run_up(((int)floor_ + 63) / 64, [&](const uint4& q, uint32_t b) {
             const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t n0 = counted(w[i], 0), n1 = counted(w[i], 1);
-                if (n0 && (uint32_t)b + 2 * i < floor_) v += weights(n0, b + 2 * i);
-                if (n1 && (uint32_t)b + 2 * i + 1 < floor_) v += weights(n1, b + 2 * i + 1);
+            const uint32_t base = base_of(b), off = base - b;
+            const double first_ = weight(r, value_at(base));
+            const double* step = steps(b);
+            uint64_t v = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t n = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu;
+                if (b + i < floor_) v += n * whole_weight(first_ * step[i - off & 7u]);
             }
+            if (extra && top_bin < floor_) v += SP_ONE;   // (the only bin in use is the largest value's)
             return v;
         });
-        const uint64_t above = s.sums[SK_GROUPS - 1];
-        uint64_t kept = above + ties * tied, before, w;
-        uint32_t last = ties ? floor_ : SK_BINS;   // bin of the last value that is kept, where a filter has set one
-        auto ends = [&](uint64_t X) {              // the bin in which the front part that reaches X ends; what lies in front of it; its weight
-            uint32_t b = floor_;
-            before = above, w = tied;
-            if (X <= above) {
-                const At f = reach(X, floor_, weights);
-                b = f.bin, before = f.before, w = whole_weight(weight(r, value_at(b)));
+        if (warp == 0) {   // the ends of what is kept, and the draw
+            const uint64_t above = s.sums[SK_GROUPS - 1];
+            kept = above + ties * tied;
+            uint64_t before, w;
+            uint32_t last = ties ? floor_ : SK_BINS;   // bin of the last value that is kept, where a filter has set one
+            auto ends = [&](uint64_t X) {              // the bin in which the front part that reaches X ends; what lies in front of it; its weight
+                uint32_t b = floor_;
+                before = above, w = tied;
+                if (X <= above) {
+                    const At at = reach(X, floor_, weights);
+                    b = at.bin, before = at.before, w = at.one;
+                }
+                return b;
+            };
+            if (f.by_sum) {
+                const uint64_t X = min(kept, (uint64_t)fmax(1.0, ceil(f.p * (double)kept)));
+                last = ends(X);
+                kept = before + how_many(X - before, w) * w;
             }
-            return b;
-        };
-        if (p < 1.0) {
-            const uint64_t X = min(kept, (uint64_t)fmax(1.0, ceil(p * (double)kept)));
-            last = ends(X);
-            kept = before + (X - before + w - 1) / w * w;
-        }
-        if (m > 0.0 && !(last < SK_BINS && weight(r, value_at(last)) >= m)) {
-            // the last bin whose weight is m or more lies near this one; weights fall from bin to bin
-            const int near = (int)bin_at(top < INFINITY ? fminf(top, (float)fmax(-3.4e38, (double)top + T * log(m))) : top), b = near - 15 + lane;
-            const bool large = b < (int)top_bin || (b < K::NEG_INF && weight(r, value_at((uint32_t)b)) >= m);
-            const int to = near - 16 + __popc(__ballot_sync(0xffffffffu, large));
-            // the sum up to that bin
-            uint64_t sum = 0;
-            if (to >= 0) {
-                const int g = to >> 6;
-                const uint32_t word = words[g * 32 + lane], c = g * 64 + 2 * lane;
-                const uint32_t n0 = counted(word, 0), n1 = counted(word, 1);
-                if (n0 && c < floor_ && (int)c <= to) sum += weights(n0, c);
-                if (n1 && c + 1 < floor_ && (int)c + 1 <= to) sum += weights(n1, c + 1);
+            if (f.by_size && !(last < SK_BINS && weight_at(last) >= f.m)) {
+                // the last bin whose weight is m or more lies near this one; weights fall from bin to bin
+                const int near = (int)bin_at(top < INFINITY ? fminf(top, (float)fmax(-3.4e38, (double)top + f.T * log(f.m))) : top), b = near - 15 + lane;
+                const bool large = b < (int)top_bin || (b < K::NEG_INF && weight_at((uint32_t)b) >= f.m);
+                const int to = near - 16 + __popc(__ballot_sync(0xffffffffu, large));
+                uint64_t sum = 0;   // up to that bin
+                if (to >= (int)top_bin) {
+                    const int g = to >> 6;
+                    const uint32_t word = words[g * 32 + lane], c = g * 64 + 2 * lane;
+                    const Two v = weights(c);
+                    if (c < floor_ && (int)c <= to) sum += counted(word, 0) * v.a;
+                    if (c + 1 < floor_ && (int)c + 1 <= to) sum += counted(word, 1) * v.b;
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                sum += g ? s.sums[g - 1] : 0;
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    sum += g > first ? s.sums[g - first - 1] : 0;
+                }
+                kept = max(SP_ONE, min(kept, sum));
             }
-            kept = max(SP_ONE, min(kept, sum));
+            const uint64_t X = min(kept, (uint64_t)floor(f.u * (double)kept) + 1);
+            const uint32_t b = ends(X);
+            const uint64_t n = how_many(X - before, w) - 1;
+            if (lane == 0) s.bin = b, s.ordinal = n;
         }
-        const uint64_t X = min(kept, (uint64_t)floor(u * (double)kept) + 1);
-        bin = ends(X);
-        ordinal = (X - before + w - 1) / w - 1;
-        logp = -log((double)kept * (1.0 / SP_ONE));
-        if (value_at(bin) != top) logp += ((double)value_at(bin) - (double)top) / T;
+        __syncthreads();
+        bin = s.bin, ordinal = s.ordinal;
     }
     // the value of that bin with `ordinal` of them in front of it
     const uint32_t as = bits_of_bin(bin) * 0x00010001u;
-    auto matching = [&](int c) {   // a bit for each of a piece's values
-        if (c >= end) return 0u;
-        const uint4 q = piece(c);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        uint32_t mask = 0;
+    uint32_t n = 0, masks[3] = {0, 0, 0};   // a bit for each of a piece's values, eight pieces and one
+    for (int i = 0, c0 = own; c0 < end; c0 += 32 * AHEAD, ++i) {
+        request(c0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mask |= (K::same(w[i], as) & 0x00020001u) << (2 * i);   // (bits 0 and 17)
-        return (mask | mask >> 16) & 0xffu;
-    };
-    uint32_t n = 0;
-#pragma unroll 4
-    for (int c = own; c < end; c += 32) n += __popc(matching(c));
+        for (int j = 0; j < AHEAD; ++j)
+            if (c0 + 32 * j < end) {
+                const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+                uint32_t mask = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mask |= (K::same(w[e], as) & 0x00020001u) << (2 * e);   // (bits 0 and 17)
+                mask = (mask | mask >> 16) & 0xffu;
+                n += __popc(mask);
+                if (i == 0) masks[j / 4] |= mask << (8 * (j & 3));
+                else masks[2] = mask;   // (j is 0)
+            }
+    }
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) s.matches[warp] = n;
     __syncthreads();
+    if (threadIdx.x == 0) {
+        double l = -log((double)kept * (1.0 / SP_ONE));
+        if (bin != top_bin) l += ((double)value_at(bin) - (double)top) / f.T;
+        a.logp[row] = (float)l;
+    }
     uint32_t ahead = __reduce_add_sync(0xffffffffu, lane < warp ? s.matches[lane] : 0u);
     if (ordinal < ahead || ordinal >= (uint64_t)ahead + n) return;
-    for (int c0 = warp * per_warp; c0 < end; c0 += 32) {
-        uint32_t mask = matching(c0 + lane), up = __popc(mask);
+    for (int i = 0; 32 * i < per_warp; ++i) {
+        uint32_t mask = (i < 4 ? masks[0] : i < 8 ? masks[1] : masks[2]) >> (8 * (i & 3)) & 0xffu, up = __popc(mask);
         const uint32_t mine = up;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -1111,9 +1243,8 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
         }
         const uint32_t from = ahead + up - mine;
         if (ordinal >= from && ordinal < from + mine) {
-            for (uint32_t i = from; i < ordinal; ++i) mask &= mask - 1;
-            a.ids[row] = (int64_t)(c0 + lane) * 8 - skip + __ffs(mask) - 1;
-            a.logp[row] = (float)logp;
+            for (uint32_t e = from; e < ordinal; ++e) mask &= mask - 1;
+            a.ids[row] = (int64_t)(own + 32 * i) * 8 - skip + __ffs(mask) - 1;
         }
         ahead += __shfl_sync(0xffffffffu, up, 31);
     }

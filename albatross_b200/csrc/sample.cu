@@ -875,13 +875,13 @@ __device__ __forceinline__ uint32_t bin_of_bits(uint32_t bits) { return bits == 
 struct alignas(16) KeyShared {
     uint4 counts[SK_BINS / 8];   // (or the lists of few values)
     uint64_t sums[SK_GROUPS];
-    double step[256][8];         // exp(-j * (distance of two neighbours) / T), by their exponent
+    double step[256][9];         // exp(-j * (distance of two neighbours) / T), by their exponent (nine: lanes of other exponents meet other banks)
     uint64_t red[32];
     double tab[16];
     FewShared few;
     uint32_t tops[32], matches[32];
     uint32_t extra, bin;
-    uint64_t ties, tied, ordinal;
+    uint64_t ties, tied, ordinal, kept;
 };
 
 template <class E>
@@ -1200,16 +1200,21 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
             const uint64_t X = min(kept, (uint64_t)floor(f.u * (double)kept) + 1);
             const uint32_t b = ends(X);
             const uint64_t n = how_many(X - before, w) - 1;
-            if (lane == 0) s.bin = b, s.ordinal = n;
+            if (lane == 0) s.bin = b, s.ordinal = n, s.kept = kept;
         }
         __syncthreads();
-        bin = s.bin, ordinal = s.ordinal;
+        bin = s.bin, ordinal = s.ordinal, kept = s.kept;
     }
     // the value of that bin with `ordinal` of them in front of it
     const uint32_t as = bits_of_bin(bin) * 0x00010001u;
     uint32_t n = 0, masks[3] = {0, 0, 0};   // a bit for each of a piece's values, eight pieces and one
-    for (int i = 0, c0 = own; c0 < end; c0 += 32 * AHEAD, ++i) {
+    for (int i = 0, c0 = own; i == 0 || c0 < end; c0 += 32 * AHEAD, ++i) {
         request(c0);
+        if (i == 0 && threadIdx.x == SK_NT - 32) {   // (while they are under way)
+            double l = -log((double)kept * (1.0 / SP_ONE));
+            if (bin != top_bin) l += ((double)value_at(bin) - (double)top) / f.T;
+            a.logp[row] = (float)l;
+        }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
             if (c0 + 32 * j < end) {
@@ -1226,11 +1231,6 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) s.matches[warp] = n;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        double l = -log((double)kept * (1.0 / SP_ONE));
-        if (bin != top_bin) l += ((double)value_at(bin) - (double)top) / f.T;
-        a.logp[row] = (float)l;
-    }
     uint32_t ahead = __reduce_add_sync(0xffffffffu, lane < warp ? s.matches[lane] : 0u);
     if (ordinal < ahead || ordinal >= (uint64_t)ahead + n) return;
     for (int i = 0; 32 * i < per_warp; ++i) {
@@ -1249,6 +1249,176 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
         ahead += __shfl_sync(0xffffffffu, up, 31);
     }
 }
+// ---- top-k of the same small k for every row --------------------------------------------------------------------------------------------
+// Rows are streamed, two blocks to an SM, so that one reads while the other sorts: a row's largest values per thread, a bound that k threads reach, then only the batches
+// of a thread that reach it once more (from L2), and what the few values answer. What bounds it is the reading; 512 x 65536 fp32: 106 us in clusters that keep rows in shared
+// memory. Where more values than threads reach the bound (equals, mostly), the k-th largest key is searched by counting, and of its equals the first ids are taken.
+constexpr int ST_NT = 512, ST_BATCH = 8, ST_MOST_K = 256;
+
+struct TopShared {
+    uint64_t lists[4 * ST_NT];
+    FewShared few;
+    double tab[16];
+    uint32_t tops[32], counts[2][32];
+};
+template <class E>
+__global__ void __launch_bounds__(ST_NT, 2) sample_top_kernel(const SampleArgs a) {
+    __shared__ TopShared s;
+    constexpr int PER = 16 / sizeof(E);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = blockIdx.x;
+    const E* logits = static_cast<const E*>(a.logits) + row * a.stride;
+    const Extent all = rows_extent(a.logits, a.rows, a.stride, a.V, sizeof(E));
+    const int skip = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(E)), pieces = (skip + a.V + PER - 1) / PER;
+    auto piece = [&](int c) {   // (values outside of the row: -inf)
+        const int at = c * PER - skip;
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (at >= 0 && at + PER <= a.V) {
+            if (all.holds(logits + at, PER)) q = __ldg(reinterpret_cast<const uint4*>(logits + at));
+        } else {
+            float v[PER];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[i] = at + i >= 0 && at + i < a.V && all.holds(logits + at + i) ? to_f(logits[at + i]) : -INFINITY;
+            q = pack<E>(v);
+        }
+        return q;
+    };
+    RowFilters f = RowFilters(a, row);
+    if (f.greedy) f.T = 1.0, f.k = 1, f.by_rank = true;   // (the first of the largest)
+    if (threadIdx.x < 16) s.tab[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
+    if (threadIdx.x == 0) s.few.n[0] = 0;
+    float largest_of[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // of this thread's batches (the last one's and all behind it)
+    for (int b = 0, c0 = threadIdx.x; c0 < pieces; ++b, c0 += ST_NT * ST_BATCH) {
+        uint4 q[ST_BATCH];
+#pragma unroll
+        for (int j = 0; j < ST_BATCH; ++j)
+            if (c0 + j * ST_NT < pieces) q[j] = piece(c0 + j * ST_NT);
+        float t = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < ST_BATCH; ++j)
+            if (c0 + j * ST_NT < pieces) t = larger_or_nan(t, largest<E>(q[j]));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j == min(b, 3)) largest_of[j] = larger_or_nan(largest_of[j], t);
+    }
+    float top = larger_or_nan(larger_or_nan(largest_of[0], largest_of[1]), larger_or_nan(largest_of[2], largest_of[3]));
+    const uint32_t own_top = (int)threadIdx.x < pieces ? (top == top ? key_of(top) : 0xffffffffu) : 0;   // a NaN on top of all
+    uint32_t top_key = __reduce_max_sync(0xffffffffu, own_top);
+    if (lane == 0) s.tops[warp] = top_key;
+    __syncthreads();
+    top_key = __reduce_max_sync(0xffffffffu, s.tops[lane % (ST_NT / 32)]);
+    if (top_key == 0xffffffffu || top_key <= key_of(-INFINITY)) {   // a NaN, or nothing to draw
+        if (threadIdx.x == 0) a.ids[row] = -1, a.logp[row] = NAN;
+        return;
+    }
+    top = value_of(top_key);
+    const RowScale r = {top, 0.f, 1.4426950408889634074 / f.T, s.tab};
+    const uint32_t none = key_of(-INFINITY) + 1;   // the least key that counts
+    uint32_t bound = 0;
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t t = bound | 1u << bit;
+        const int n = __syncthreads_count(own_top >= t);
+        if (n < f.k) continue;
+        bound = t;
+        if (n <= f.k + f.k / 8 + 16) break;
+    }
+    bound = max(bound, none);
+    auto gather = [&](uint32_t bound) {   // all of its key and more
+        const float least = value_of(bound);
+        for (int b = 0, c0 = threadIdx.x; c0 < pieces; ++b, c0 += ST_NT * ST_BATCH) {
+            const float t = b == 0 ? largest_of[0] : b == 1 ? largest_of[1] : b == 2 ? largest_of[2] : largest_of[3];
+            if (!(t >= least)) continue;
+            uint4 q[ST_BATCH];
+#pragma unroll
+            for (int j = 0; j < ST_BATCH; ++j)
+                if (c0 + j * ST_NT < pieces) q[j] = piece(c0 + j * ST_NT);
+#pragma unroll
+            for (int j = 0; j < ST_BATCH; ++j) {
+                const int c = c0 + j * ST_NT;
+                if (c >= pieces || !(largest<E>(q[j]) >= least)) continue;
+                float v[PER];
+                unpack<E>(q[j], v);
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (v[i] >= least) {
+                        const uint32_t at = atomicAdd(&s.few.n[0], 1u);
+                        if (at < (uint32_t)ST_NT) s.lists[at] = Few<ST_NT>::entry(v[i], c * PER - skip + i);
+                    }
+            }
+        }
+        __syncthreads();
+        return s.few.n[0];
+    };
+    uint32_t n = gather(bound);
+    if (n > (uint32_t)ST_NT) {
+        __syncthreads();   // (the count has been read)
+        int turn = 0;
+        auto sum = [&](uint32_t v) {   // over the block
+            turn ^= 1;
+            v = __reduce_add_sync(0xffffffffu, v);
+            if (lane == 0) s.counts[turn][warp] = v;
+            __syncthreads();
+            return __reduce_add_sync(0xffffffffu, lane < ST_NT / 32 ? s.counts[turn][lane] : 0u);
+        };
+        // k values or more reach `lo`, fewer reach `hi`
+        uint32_t lo = bound, hi = top_key + 1;
+        bool few_enough = false;
+        while (hi - lo > 1 && !few_enough) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            uint32_t count = 0;
+            for (int c = threadIdx.x; c < pieces; c += ST_NT) {
+                float v[PER];
+                unpack<E>(piece(c), v);
+#pragma unroll
+                for (int i = 0; i < PER; ++i) count += key_of(v[i]) >= mid;
+            }
+            count = sum(count);
+            if (count >= (uint32_t)f.k) lo = mid, few_enough = count <= (uint32_t)ST_NT;
+            else hi = mid;
+        }
+        if (threadIdx.x == 0) s.few.n[0] = 0;
+        __syncthreads();
+        n = gather(few_enough ? lo : lo + 1);
+        if (!few_enough) {   // and of those equal to the k-th, the first ids
+            for (int base = 0; base < pieces && n < (uint32_t)f.k; base += ST_NT) {
+                const int c = base + threadIdx.x;
+                uint32_t mask = 0;
+                if (c < pieces) {
+                    float v[PER];
+                    unpack<E>(piece(c), v);
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) mask |= (uint32_t)(key_of(v[i]) == lo) << i;
+                }
+                uint32_t up = __popc(mask);
+                const uint32_t mine = up;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, up, o);
+                    if (lane >= o) up += v;
+                }
+                turn ^= 1;
+                if (lane == 31) s.counts[turn][warp] = up;
+                __syncthreads();
+                const uint32_t of_warp = lane < ST_NT / 32 ? s.counts[turn][lane] : 0u;
+                uint32_t at = n + __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0u) + up - mine;
+                for (; mask && at < (uint32_t)f.k; mask &= mask - 1, ++at) s.lists[at] = Few<ST_NT>::entry(value_of(lo), c * PER - skip + __ffs(mask) - 1);
+                n = min((uint32_t)f.k, n + __reduce_add_sync(0xffffffffu, of_warp));
+            }
+            __syncthreads();
+        }
+    }
+    Few<ST_NT> few = {s.few, s.lists, lane, warp, 32, 0};
+    uint64_t kept = 0;
+    if (few.begin(n)) few.answer(f, r, s.lists, n, 0, 0, 0.0, true, true, true, kept, a.ids + row, a.logp + row);
+}
+template <class E>
+int sample_top_launch(const SampleArgs& a, cudaStream_t st) {
+    AB_CHECK_ARG(a.rows <= INT32_MAX, "sampling: too many rows");
+    sample_top_kernel<E><<<(unsigned)a.rows, ST_NT, 0, st>>>(a);
+    AB_CUDA(cudaGetLastError());
+    return OK;
+}
+
 template <class E>
 int sample_keys_launch(SampleArgs a, cudaStream_t st) {
     static PerDeviceOnce once;
@@ -1303,6 +1473,8 @@ int sample_launch(SampleArgs a, cudaStream_t st) {
 
 int sample_filtered(int dtype, int64_t rows, int V, const void* logits, int64_t stride, const float* u, const ab_sampling& p, int64_t* ids, float* logp, cudaStream_t st) {
     const SampleArgs a = {logits, u, p.temperature, p.top_p, p.min_p, p.top_k, p.temperature_all, p.top_p_all, p.min_p_all, p.top_k_all, V, rows, stride, ids, logp, 0, 0};
+    if (!p.top_k && p.top_k_all > 0 && p.top_k_all <= ST_MOST_K && p.top_k_all < V)
+        return dtype == AB_DT_F16 ? sample_top_launch<__half>(a, st) : dtype == AB_DT_BF16 ? sample_top_launch<__nv_bfloat16>(a, st) : sample_top_launch<float>(a, st);
     if (V <= SK_BINS && dtype != AB_DT_F32) return dtype == AB_DT_F16 ? sample_keys_launch<__half>(a, st) : sample_keys_launch<__nv_bfloat16>(a, st);
     return dtype == AB_DT_F16 ? sample_launch<__half>(a, st) : dtype == AB_DT_BF16 ? sample_launch<__nv_bfloat16>(a, st) : sample_launch<float>(a, st);
 }

@@ -112,6 +112,22 @@ def test_ties(f, dtype):
     check(signs, torch.rand(5, device="cuda", generator=g), **f)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_a_top_k_among_many_equals(dtype):
+    """More values than threads at the bound, of one key and of several; greedy rows beside them; fewer values than k."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    u = torch.rand(6, device="cuda", generator=g)
+    for V, k in ((700, 1), (5000, 3), (20011, 256), (65536, 100), (1 << 18, 200)):
+        x = torch.randint(0, 3, (6, V), device="cuda", generator=g).to(DT[dtype])
+        x[1] = 2.0
+        x[2] = (torch.arange(V, device="cuda") % 600).to(DT[dtype]) * 0.125
+        x[3, 5:] = -torch.inf
+        x[4] = torch.arange(V, device="cuda").flip(0).clamp(max=400).to(DT[dtype])
+        T = torch.tensor([1.0, 0.7, 2.0, 1.0, 0.0, 30.0], device="cuda")
+        check(x, u, T, k)
+        check(x, u, T, k, 0.8, 0.001)
+
+
 def test_32_bit_logits_that_come_from_16_bits():
     """Thousands of equals in 32-bit rows, and values that differ in their last bit only."""
     x, u = rows_of(4, 65536, "bf16", seed=8, spread=(0.3, 2.0))

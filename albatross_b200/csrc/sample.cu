@@ -849,12 +849,12 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
 // few values (top-k; min-p by itself), only those are counted that reach a bound: some k of the threads' own maxima do, and so do k values.
 // What bounds it: the atomics (3.3 cycles for a warp's: two of its values meet a bank), then the units' weights.
 //
-// Counters lie in the order of the values, larger ones first, eight in 16 bytes. Eight units are a group; a warp's eight lanes take one at a time, and groups
-// go round the warps, since values lie densely in a few binades. Sums of groups are run up over the block; a question is answered by a search among them and by the 64
-// counters of one group, by the first warp.
+// Counters lie in the order of the values, larger ones first, eight in 16 bytes. Eight units are a group, whose sums are run up over the block; a question is answered by
+// a search among them and by the 64 counters of one group, by the first warp.
 //
 // A counter holds up to 65535: the row's last value is added when the others are counted, so that only a row of 65536 equal ones exceeds it (`extra`).
-constexpr int SK_NT = 1024, SK_BINS = 65536, SK_GROUPS = SK_BINS / 64, SK_ROUNDS = SK_BINS / 8 / SK_NT;
+constexpr int SK_NT = 1024, SK_BINS = 65536, SK_GROUPS = SK_BINS / 64;
+static_assert(SK_GROUPS == SK_NT, "a thread per group");
 
 template <class E> struct KeyType;   // how a type's 16 bits are ordered
 template <> struct KeyType<__half> {
@@ -876,11 +876,12 @@ struct alignas(16) KeyShared {
     uint4 counts[SK_BINS / 8];   // (or the lists of few values)
     uint64_t sums[SK_GROUPS];
     double step[256][9];         // exp(-j * (distance of two neighbours) / T), by their exponent (nine: lanes of other exponents meet other banks)
+    unsigned short units[SK_BINS / 8];   // those with a counter in use
     uint64_t red[32];
-    double tab[16];
+    double tab[16], log_kept;
     FewShared few;
     uint32_t tops[32], matches[32];
-    uint32_t extra, bin;
+    uint32_t extra, bin, n_units;
     uint64_t ties, tied, ordinal, kept;
 };
 
@@ -929,10 +930,11 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
     auto clear = [&]() {
         for (int i = threadIdx.x; i < SK_BINS / 8; i += SK_NT) s.counts[i] = make_uint4(0, 0, 0, 0);
         if (threadIdx.x == 0) s.extra = 0;
-        const int e = threadIdx.x >> 2, j = (threadIdx.x & 3) * 2;
-        if (e < K::EXPONENTS) {
-            const double far = scalbn(1.0, max(e, 1) - 1 + K::LEAST) / f.T;
-            s.step[e][j] = j ? exp(-far * j) : 1.0, s.step[e][j + 1] = exp(-far * (j + 1));   // (far may be infinite)
+        if (threadIdx.x < K::EXPONENTS) {
+            const double one = exp(-scalbn(1.0, max((int)threadIdx.x, 1) - 1 + K::LEAST) / f.T);
+            double w = 1.0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j, w *= one) s.step[threadIdx.x][j] = w;
         }
     };
     auto count_piece = [&](const uint4& q, int c) {
@@ -1028,7 +1030,7 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
     }
     const uint32_t top_bin = bin_at(top);
     uint32_t bin = top_bin;
-    uint64_t ordinal = 0, kept = SP_ONE;
+    uint64_t ordinal = 0;
     if (!f.greedy) {
         if (threadIdx.x == 0) {   // -0 is 0, and the last value
             const uint32_t minus = words[0x4000] & 0xffffu;
@@ -1051,25 +1053,10 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
             const uint32_t base = base_of(bin);
             return weight(r, value_at(base)) * steps(bin)[bin - base & 7u];   // (1 times 1 for the largest value)
         };
-        // Sums of the groups from `first` to `last` of what `of` makes of a unit and its first bin, run up; all threads then have them in s.sums, from 0 on. (Group g: units 8 g ..
-        // 8 g + 7.) Returns the sum of all.
+        // s.sums: of the groups from that of the largest value on (group g: units 8 g .. 8 g + 7), filled by run_counts or run_weights, then run up over all of them.
         const int first = (int)(top_bin >> 6);
-        auto run_up = [&](int last, auto of) {
-            const int groups = last - first;
-            for (int i = 0; i * 128 < groups; ++i) {
-                const int group = i * 128 + (lane >> 3) * 32 + warp, unit = (first + group) * 8 + (lane & 7);
-                uint64_t v = 0;
-                if (group < groups) {
-                    const uint4 q = s.counts[unit];
-                    if ((q.x | q.y | q.z | q.w) != 0) v = of(q, (uint32_t)unit * 8);
-                }
-                v += __shfl_xor_sync(0xffffffffu, v, 1);
-                v += __shfl_xor_sync(0xffffffffu, v, 2);
-                v += __shfl_xor_sync(0xffffffffu, v, 4);
-                if ((lane & 7) == 0) s.sums[group] = v;
-            }
-            __syncthreads();
-            uint64_t v = (int)threadIdx.x < groups ? s.sums[threadIdx.x] : 0;
+        auto run_up = [&]() {
+            uint64_t v = s.sums[threadIdx.x];
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint64_t w = __shfl_up_sync(0xffffffffu, v, o);
@@ -1124,13 +1111,16 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
         uint32_t floor_ = K::NEG_INF;     // bins from here on are not kept, or have no weight
         uint64_t ties = 0, tied = 0;
         if (f.by_rank) {
-            run_up(SK_GROUPS, [&](const uint4& q, uint32_t) {
-                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-                uint32_t n = 0;
+            const int group = threadIdx.x;   // (one of a thread's own)
+            uint32_t n = 0;
+            if (first + group < SK_GROUPS)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) n = __dp2a_lo(w[i], 0x0101u, n);
-                return (uint64_t)(extra ? (uint32_t)a.V : n);
-            });
+                for (int j = 0; j < 8; ++j) {
+                    const uint4 q = s.counts[(first + group) * 8 + (j + lane & 7)];   // (lanes of a warp begin at different banks)
+                    n = __dp2a_lo(q.x, 0x0101u, n), n = __dp2a_lo(q.y, 0x0101u, n), n = __dp2a_lo(q.z, 0x0101u, n), n = __dp2a_lo(q.w, 0x0101u, n);
+                }
+            s.sums[group] = extra && n ? (uint32_t)a.V : n;
+            run_up();
             if (warp == 0) {
                 const At at = reach((uint64_t)f.k, SK_BINS, [](uint32_t) { return Two{1, 1}; });
                 const bool weighs = at.bin < (uint32_t)K::NEG_INF;
@@ -1146,24 +1136,50 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
             const double* step = steps(b);
             return Two{whole_weight(w * step[b - base & 7u]), whole_weight(w * step[b + 1 - base & 7u])};   // (in front of the largest value: of no counter)
         };
-        run_up(((int)floor_ + 63) / 64, [&](const uint4& q, uint32_t b) {
+        // The units in use, one behind the other (of 8192, some 2500 for fp16 and a few hundred for bf16), then their weights.
+        __syncthreads();   // (s.sums)
+        s.sums[threadIdx.x] = 0;
+        if (threadIdx.x == 0) s.n_units = 0;
+        __syncthreads();
+        const int to_unit = ((int)floor_ + 7) / 8;
+        for (int u0 = (int)(top_bin >> 3) & ~(SK_NT - 1); u0 < to_unit; u0 += SK_NT) {
+            const int unit = u0 + (int)threadIdx.x;
+            const uint4 q = s.counts[unit];
+            const bool used = unit < to_unit && (q.x | q.y | q.z | q.w) != 0;
+            const uint32_t mask = __ballot_sync(0xffffffffu, used);
+            uint32_t at = 0;
+            if (lane == 0 && mask) at = atomicAdd(&s.n_units, __popc(mask));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
+            if (used) s.units[at] = (unsigned short)unit;
+        }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < s.n_units; i += SK_NT) {
+            const uint32_t unit = s.units[i], b = unit * 8, base = base_of(b), off = base - b;
+            const uint4 q = s.counts[unit];
             const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-            const uint32_t base = base_of(b), off = base - b;
             const double first_ = weight(r, value_at(base));
             const double* step = steps(b);
             uint64_t v = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t n = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu;
-                if (b + i < floor_) v += n * whole_weight(first_ * step[i - off & 7u]);
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t n = j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu;
+                if (b + j < floor_) v += n * whole_weight(first_ * step[j - off & 7u]);
             }
             if (extra && top_bin < floor_) v += SP_ONE;   // (the only bin in use is the largest value's)
-            return v;
-        });
-        if (warp == 0) {   // the ends of what is kept, and the draw
+            if (v) atomicAdd(reinterpret_cast<unsigned long long*>(&s.sums[(b >> 6) - first]), (unsigned long long)v);
+        }
+        __syncthreads();
+        run_up();
+        // The ends of what is kept, and the draw: by the first warp. The second one takes the logarithm meanwhile.
+        auto hand_over = [] { asm volatile("bar.sync 2, 64;" ::: "memory"); };
+        if (warp == 1) {
+            hand_over();
+            const double l = log((double)s.kept * (1.0 / SP_ONE));
+            if (lane == 0) s.log_kept = l;
+        }
+        if (warp == 0) {
             const uint64_t above = s.sums[SK_GROUPS - 1];
-            kept = above + ties * tied;
-            uint64_t before, w;
+            uint64_t kept = above + ties * tied, before, w;
             uint32_t last = ties ? floor_ : SK_BINS;   // bin of the last value that is kept, where a filter has set one
             auto ends = [&](uint64_t X) {              // the bin in which the front part that reaches X ends; what lies in front of it; its weight
                 uint32_t b = floor_;
@@ -1197,24 +1213,23 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
                 }
                 kept = max(SP_ONE, min(kept, sum));
             }
+            if (lane == 0) s.kept = kept;
+            hand_over();
             const uint64_t X = min(kept, (uint64_t)floor(f.u * (double)kept) + 1);
             const uint32_t b = ends(X);
             const uint64_t n = how_many(X - before, w) - 1;
-            if (lane == 0) s.bin = b, s.ordinal = n, s.kept = kept;
+            if (lane == 0) s.bin = b, s.ordinal = n;
         }
         __syncthreads();
-        bin = s.bin, ordinal = s.ordinal, kept = s.kept;
+        bin = s.bin, ordinal = s.ordinal;
     }
     // the value of that bin with `ordinal` of them in front of it
     const uint32_t as = bits_of_bin(bin) * 0x00010001u;
     uint32_t n = 0, masks[3] = {0, 0, 0};   // a bit for each of a piece's values, eight pieces and one
     for (int i = 0, c0 = own; i == 0 || c0 < end; c0 += 32 * AHEAD, ++i) {
         request(c0);
-        if (i == 0 && threadIdx.x == SK_NT - 32) {   // (while they are under way)
-            double l = -log((double)kept * (1.0 / SP_ONE));
-            if (bin != top_bin) l += ((double)value_at(bin) - (double)top) / f.T;
-            a.logp[row] = (float)l;
-        }
+        if (i == 0 && threadIdx.x == 0)
+            a.logp[row] = f.greedy ? 0.f : (float)((bin != top_bin ? ((double)value_at(bin) - (double)top) * (r.c * 0.693147180559945309417) : 0.0) - s.log_kept);
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
             if (c0 + 32 * j < end) {

@@ -145,7 +145,9 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
         first_tile[warp] = tile0;
     }
     __syncwarp();
-    pdl_wait();
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+    pdl_wait();   // (codes and scales too may have been written just before)
 
     // The warp's pieces one behind the other, tile after tile; its first lane asks for them, a.stages ahead of the one worked on.
     int in_i = 0, in_c = in0, in_row = n0 + tile0 * a.height, in_stage = 0;

@@ -100,7 +100,8 @@ def _interface() -> float:
 def build_train_op(force: bool = False) -> str:
     """Builds csrc/train_op.cpp the same way: `torch.ops.albatross_b200.*`, the operators with gradients. It takes the kernel library's
     entries at run time (_shim.py says from which build of it)."""
-    return _build_shim(os.path.join(CSRC, "train_op.cpp"), TRAIN_OP_LIB, _interface(), force, ["-ldl"])
+    import sysconfig
+    return _build_shim(os.path.join(CSRC, "train_op.cpp"), TRAIN_OP_LIB, _interface(), force, ["-I" + sysconfig.get_paths()["include"], "-ltorch_python", "-ldl"])
 
 
 def build_serve_op(force: bool = False) -> str:

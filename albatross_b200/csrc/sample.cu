@@ -378,17 +378,28 @@ struct Sampler {
         }
         return bound;
     }
-    // running sums of the histogram, over all blocks; every block has them
+    // running sums of the histogram, over all blocks; every block has them. (Each adds up a share of the bins and hands it round: all of them by every block took 90 us in
+    // clusters of eight.)
     template <int BINS>
     __device__ __forceinline__ void run_up(uint64_t* cum) {
         constexpr int EACH = (BINS + NT - 1) / NT;
+        join();
+        const int share = BINS / blocks;
+        for (int bin = rank * share + threadIdx.x; bin < (rank + 1) * share; bin += NT) {
+            uint64_t sum = 0;
+#pragma unroll
+            for (int b = 0; b < SP_MAX_BLOCKS; ++b)
+                if (b < blocks) sum += (uint64_t)*of(&s.part[0][bin], b) + ((uint64_t)*of(&s.part[1][bin], b) << 15) + ((uint64_t)*of(&s.part[2][bin], b) << 30);
+#pragma unroll
+            for (int b = 0; b < SP_MAX_BLOCKS; ++b)
+                if (b < blocks) *of(&cum[bin], b) = sum;
+        }
         join();
         uint64_t v[EACH], sum = 0;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int bin = threadIdx.x * EACH + i;
-            for (int b = 0; b < blocks; ++b)
-                if (bin < BINS) sum += (uint64_t)*of(&s.part[0][bin], b) + ((uint64_t)*of(&s.part[1][bin], b) << 15) + ((uint64_t)*of(&s.part[2][bin], b) << 30);
+            if (bin < BINS) sum += cum[bin];
             v[i] = sum;
         }
         uint64_t up = sum;
@@ -399,12 +410,14 @@ struct Sampler {
         }
         if (lane == 31) s.red[warp] = up;
         __syncthreads();
-        uint64_t base = up - sum;
-        for (int i = 0; i < warp; ++i) base += s.red[i];
+        uint64_t base = lane < warp ? s.red[lane] : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
+        base += up - sum;
 #pragma unroll
         for (int i = 0; i < EACH; ++i)
             if (threadIdx.x * EACH + i < BINS) cum[threadIdx.x * EACH + i] = base + v[i];
-        join();
+        __syncthreads();
     }
     template <int BINS>
     static __device__ __forceinline__ int search(const uint64_t* cum, uint64_t X) {   // the first bin that reaches X
@@ -623,9 +636,18 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
         block_sums(mine, 0.0, sums);
         const double total = sums[0];
         const uint64_t whole = (uint64_t)(total * SP_ONE);
+        const int share = SP_BINS / x.blocks;
+        for (int bin = x.rank * share + threadIdx.x; bin < (x.rank + 1) * share; bin += NT) {   // the counts of all blocks, in the first one
+            uint32_t n = 0;
+#pragma unroll
+            for (int o = 0; o < SP_MAX_BLOCKS; ++o)
+                if (o < x.blocks) n += *x.of(&s.part[0][bin], o);
+            *x.of(&s.part[1][bin], 0) = n;
+        }
+        x.join();
         if (x.rank == 0) {
-            // Running counts, and sums of the weights as if a bin's values lay in its middle: they are off by half a bin's width each, 0.4 %, to either side. That they say
-            // where to look is all that is asked of them: `answer` sees whether the place was right.
+            // Running counts, and sums of the weights as if a bin's values lay in its middle: they are off by half a bin's width each, 0.4 %, to either side, and
+            // so, many together, by little. That they say where to look is all that is asked of them: `answer` sees whether the place was right.
             constexpr int EACH = SP_BINS / NT;
             float* run = reinterpret_cast<float*>(s.cum);
             uint32_t n[EACH], count = 0;
@@ -634,8 +656,7 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
                 const int bin = threadIdx.x * EACH + i;
-                n[i] = 0;
-                for (int o = 0; o < x.blocks; ++o) n[i] += *x.of(&s.part[0][bin], o);
+                n[i] = s.part[1][bin];
                 float w;
                 asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(-(float)bin * q));
                 weights += (float)n[i] * w;
@@ -664,7 +685,7 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
             __syncthreads();
             if (x.warp == 0) {   // lane 0 .. 3: the bins in which the lower and upper end of the draw's bracket lie, and of the end of what is kept
                 const double X = (x.lane < 2 ? u : 1.0) * (by_sum ? p : 1.0) * total;
-                const float at = (float)(x.lane & 1 ? X * 1.004 : X * 0.997);
+                const float at = (float)(x.lane & 1 ? X * 1.0015 : X * 0.9988);
                 int lo = 0, hi = SP_BINS - 1;
                 while (lo < hi) {
                     const int mid = (lo + hi) >> 1;
@@ -1265,20 +1286,21 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
     }
 }
 // ---- top-k of the same small k for every row --------------------------------------------------------------------------------------------
-// Rows are streamed, two blocks to an SM, so that one reads while the other sorts: a row's largest values per thread, a bound that k threads reach, then only the batches
+// Rows are streamed, two blocks of 512 threads to an SM (k up to 256; one of 1024 up to 600), so that one reads while the other sorts: a row's largest values per thread, a bound that k threads reach, then only the batches
 // of a thread that reach it once more (from L2), and what the few values answer. What bounds it is the reading; 512 x 65536 fp32: 106 us in clusters that keep rows in shared
 // memory. Where more values than threads reach the bound (equals, mostly), the k-th largest key is searched by counting, and of its equals the first ids are taken.
-constexpr int ST_NT = 512, ST_BATCH = 8, ST_MOST_K = 256;
+constexpr int ST_BATCH = 8, ST_MOST_K = 600;
 
-struct TopShared {
+template <int ST_NT>
+struct alignas(16) TopShared {
     uint64_t lists[4 * ST_NT];
     FewShared few;
     double tab[16];
     uint32_t tops[32], counts[2][32];
 };
-template <class E>
-__global__ void __launch_bounds__(ST_NT, 2) sample_top_kernel(const SampleArgs a) {
-    __shared__ TopShared s;
+template <class E, int ST_NT>
+__global__ void __launch_bounds__(ST_NT, 1024 / ST_NT) sample_top_kernel(const SampleArgs a) {
+    __shared__ TopShared<ST_NT> s;
     constexpr int PER = 16 / sizeof(E);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = blockIdx.x;
@@ -1429,7 +1451,9 @@ __global__ void __launch_bounds__(ST_NT, 2) sample_top_kernel(const SampleArgs a
 template <class E>
 int sample_top_launch(const SampleArgs& a, cudaStream_t st) {
     AB_CHECK_ARG(a.rows <= INT32_MAX, "sampling: too many rows");
-    sample_top_kernel<E><<<(unsigned)a.rows, ST_NT, 0, st>>>(a);
+    // some 1.4 k values reach the bound where k is half the threads
+    if (a.k_all <= 256) sample_top_kernel<E, 512><<<(unsigned)a.rows, 512, 0, st>>>(a);
+    else sample_top_kernel<E, 1024><<<(unsigned)a.rows, 1024, 0, st>>>(a);
     AB_CUDA(cudaGetLastError());
     return OK;
 }
@@ -1488,9 +1512,10 @@ int sample_launch(SampleArgs a, cudaStream_t st) {
 
 int sample_filtered(int dtype, int64_t rows, int V, const void* logits, int64_t stride, const float* u, const ab_sampling& p, int64_t* ids, float* logp, cudaStream_t st) {
     const SampleArgs a = {logits, u, p.temperature, p.top_p, p.min_p, p.top_k, p.temperature_all, p.top_p_all, p.min_p_all, p.top_k_all, V, rows, stride, ids, logp, 0, 0};
-    if (!p.top_k && p.top_k_all > 0 && p.top_k_all <= ST_MOST_K && p.top_k_all < V)
+    const bool keys = V <= SK_BINS && dtype != AB_DT_F32, streams = !p.top_k && p.top_k_all > 0 && p.top_k_all <= ST_MOST_K && p.top_k_all < V;
+    if (streams && !(keys && (rows <= current_sm_count() || p.top_k_all > 256)))
         return dtype == AB_DT_F16 ? sample_top_launch<__half>(a, st) : dtype == AB_DT_BF16 ? sample_top_launch<__nv_bfloat16>(a, st) : sample_top_launch<float>(a, st);
-    if (V <= SK_BINS && dtype != AB_DT_F32) return dtype == AB_DT_F16 ? sample_keys_launch<__half>(a, st) : sample_keys_launch<__nv_bfloat16>(a, st);
+    if (keys) return dtype == AB_DT_F16 ? sample_keys_launch<__half>(a, st) : sample_keys_launch<__nv_bfloat16>(a, st);
     return dtype == AB_DT_F16 ? sample_launch<__half>(a, st) : dtype == AB_DT_BF16 ? sample_launch<__nv_bfloat16>(a, st) : sample_launch<float>(a, st);
 }
 

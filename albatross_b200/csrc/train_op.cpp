@@ -7,6 +7,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/python_variable.h>
 
 #include "op.h"
 
@@ -419,8 +420,9 @@ Tensor clip_grad_norm(at::TensorList grads, double max_norm, double scale, at::T
     std::vector<ab_grad> list(grads.size());
     std::vector<Tensor> copies;                         // kept until the kernels are launched
     std::vector<std::pair<size_t, Tensor>> back;        // outputs that are copied to where they belong
-    auto fits = [&](const Tensor& t) {
-        return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.device() == device && is_known(t) && t.has_storage() && !t._fw_grad(/*level=*/0).defined();
+    auto fits = [&](const Tensor& t) {   // (what has no autograd metadata has no tangent)
+        return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.device() == device && is_known(t) && t.has_storage() &&
+               (!t.unsafeGetTensorImpl()->autograd_meta() || !t._fw_grad(/*level=*/0).defined());
     };
     at::AutoDispatchBelowADInplaceOrView below;
     for (size_t i = 0; i < grads.size(); ++i) {   // (a model has hundreds of them: what each needs is kept short)
@@ -467,6 +469,38 @@ TORCH_LIBRARY(albatross_b200, m) {
           "float scale, Tensor? out) -> (Tensor, Tensor, Tensor)", policy_loss_grad);
     m.def("clip_grad_norm(Tensor[] grads, float max_norm, float scale, Tensor[] out) -> Tensor", clip_grad_norm);
     m.def("preference_loss(Tensor logits, Tensor ids, Tensor ref_logp, Tensor? mask, float beta, float smoothing) -> (Tensor, Tensor)", preference_loss);
+}
+
+// clip_grad_norm for lists of hundreds of tensors: the dispatcher boxes and unboxes both lists, 0.2 us a tensor of the 0.3 that a call takes. Takes Python lists or
+// tuples of tensors (out: None, for the norm alone) with the interpreter's lock held; returns None, with the error set, where it throws.
+static bool tensors_of(PyObject* list, std::vector<Tensor>& out) {
+    PyObject* fast = PySequence_Fast(list, "clip_grad_norm: a list of tensors is expected");
+    if (!fast) return false;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast);
+    out.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* t = PySequence_Fast_GET_ITEM(fast, i);
+        if (!THPVariable_Check(t)) {
+            Py_DECREF(fast);
+            PyErr_SetString(PyExc_RuntimeError, "clip_grad_norm: a list of tensors is expected");
+            return false;
+        }
+        out.push_back(THPVariable_Unpack(t));
+    }
+    Py_DECREF(fast);
+    return true;
+}
+extern "C" PyObject* albatross_b200_clip_grad_norm(PyObject* grads, double max_norm, double scale, PyObject* out) {
+    try {
+        std::vector<Tensor> g, o;
+        if (!tensors_of(grads, g) || (out != Py_None && out != grads && !tensors_of(out, o))) return nullptr;
+        return THPVariable_Wrap(clip_grad_norm(g, max_norm, scale, out == grads ? g : o));
+    } catch (const c10::Error& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
 }
 
 // Takes the entries from the kernel library at `path` (already loaded). 0, or -1 with what is missing in `missing`.

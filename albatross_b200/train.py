@@ -21,6 +21,7 @@ calls the C entries of the kernel library; what does not fit raises RuntimeError
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -29,9 +30,9 @@ from . import _shim
 from . import build as _build
 
 
-_wkv7, _layer_norm, _token_logp, _policy_loss, _policy_loss_grad, _preference_loss, _clip_grad_norm = _shim.load(
+_wkv7, _layer_norm, _token_logp, _policy_loss, _policy_loss_grad, _preference_loss = _shim.load(
     _build.TRAIN_OP_LIB, "albatross_b200_train_bind",
-    ("wkv7", "layer_norm", "token_logp", "policy_loss", "policy_loss_grad", "preference_loss", "clip_grad_norm"))
+    ("wkv7", "layer_norm", "token_logp", "policy_loss", "policy_loss_grad", "preference_loss"))
 
 
 def RWKV7_TRAIN_OP(state: Optional[torch.Tensor], r, w, k, v, a, b, lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -102,10 +103,14 @@ def preference_loss(logits: torch.Tensor, ids: torch.Tensor, ref_logp: torch.Ten
     return _preference_loss(logits, ids, ref_logp, mask, beta, label_smoothing)
 
 
+_clip_list = C.PyDLL(_build.TRAIN_OP_LIB).albatross_b200_clip_grad_norm    # (the same without the dispatcher)
+_clip_list.argtypes, _clip_list.restype = [C.py_object, C.c_double, C.c_double, C.py_object], C.py_object
+
+
 def grad_norm(grads: Sequence[torch.Tensor], scale: float = 1.0) -> torch.Tensor:
     """`scale` times the 2-norm over all values of all tensors (fp16, bf16 and fp32, mixed as they come), as an fp32 number on their device. The
     squares are added up in 64 bits. A tensor that stands in the list twice counts twice."""
-    return _clip_grad_norm(grads, float("inf"), scale, [])
+    return _clip_list(grads, float("inf"), scale, None)
 
 
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, scale: float = 1.0, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
@@ -116,4 +121,4 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, scale: float 
 
     Outputs may not overlap each other, nor gradients other than their own. Up to 1000 tensors take two launches; tensors that are not dense, or lie in another
     order than their output, are copied."""
-    return _clip_grad_norm(grads, max_norm, scale, grads if out is None else out)
+    return _clip_list(grads, max_norm, scale, grads if out is None else out)

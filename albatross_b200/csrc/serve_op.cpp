@@ -1,5 +1,7 @@
 // What serves a token, as torch operators beside those of train_op.cpp (torch.ops.albatross_b200.*): arguments checked, memory from torch's allocator,
 // the C entries called on torch's current stream of the tensors' device. Neither has gradients.
+#include <ATen/MemoryOverlap.h>
+
 #include "op.h"
 
 namespace {
@@ -18,7 +20,8 @@ const Tensor per_row(const char* what, const OptTensor& t, const Tensor& logits,
     check_plain("sampler_batch", *t);
     TORCH_CHECK(t->device() == logits.device() && t->numel() == rows && (type == at::kInt ? at::isIntegralType(t->scalar_type(), false) : at::isFloatingType(t->scalar_type())),
                 "sampler_batch: ", what, " must be a number, or a tensor of one ", type == at::kInt ? "whole" : "floating", " number per row on the device of logits");
-    return t->to(type).contiguous();
+    // (a k that 32 bits do not hold filters nothing)
+    return (type == at::kInt && t->scalar_type() == at::kLong ? t->clamp(INT32_MIN, INT32_MAX) : *t).to(type).contiguous();
 }
 std::tuple<Tensor, Tensor> sample(const Tensor& logits_, const Tensor& uniform, const OptTensor& temperature, const OptTensor& top_k, const OptTensor& top_p, const OptTensor& min_p,
                                   double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all, const OptTensor& out_) {
@@ -39,6 +42,7 @@ std::tuple<Tensor, Tensor> sample(const Tensor& logits_, const Tensor& uniform, 
     if (ids.defined()) {
         TORCH_CHECK(ids.scalar_type() == at::kLong && ids.numel() == n && ids.is_contiguous() && (ids.device() == rows.device() || (ids.is_cpu() && ids.is_pinned())), who,
                     ": out must be a dense int64 tensor of one id per row, on the device of logits or in pinned host memory");
+        if (ids.is_cuda()) at::assert_no_overlap(ids, logits_), at::assert_no_overlap(ids, uniform);
         if (!ids.is_inference()) ids.unsafeGetTensorImpl()->bump_version();
     } else {
         ids = like(sizes, rows, at::kLong);

@@ -238,6 +238,7 @@ int ab_linear_int4(const ab_int4* m, int rows, const void* x, int64_t x_stride, 
     AB_CHECK_ARG(rows >= 0 && m->n_out > 0 && m->k > 0 && x_stride >= 0, "ab_linear_int4: bad shape (rows=%d n_out=%d k=%d)", rows, m->n_out, m->k);
     AB_CHECK_ARG((m->group == 32 || m->group == 64 || (m->group > 0 && m->group % 128 == 0)) && m->k % m->group == 0,
                  "ab_linear_int4: groups of %d inputs (32, 64 or a multiple of 128, which divides %d)", m->group, m->k);
+    AB_CHECK_ARG(rows <= 65535, "ab_linear_int4: %d rows are too many (65535 at most: each 16 of them read the matrix once more)", rows);
     if (rows == 0) return OK;
     AB_CHECK_ARG(m->w && m->scale && x && y, "ab_linear_int4: null pointer");
     AB_CHECK_ARG(on_boundary(m->w, 16), "ab_linear_int4: the codes must start on a 16-byte boundary");

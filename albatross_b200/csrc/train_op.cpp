@@ -9,6 +9,9 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <array>
+
 #include "op.h"
 
 namespace {
@@ -449,6 +452,20 @@ Tensor clip_grad_norm(at::TensorList grads, double max_norm, double scale, at::T
         }
         e.out_dtype = type_of(o);
         if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
+    }
+    if (!back.empty()) {   // an output that is copied to its place must not lie among the values of another one: which of the two would stay?
+        std::vector<std::array<uintptr_t, 3>> spans;
+        for (size_t i = 0; i < out.size(); ++i) {
+            if (out[i].numel() == 0) continue;
+            int64_t last = 0;
+            for (int64_t d = 0; d < out[i].dim(); ++d) last += (out[i].size(d) - 1) * out[i].stride(d);
+            const uintptr_t at = reinterpret_cast<uintptr_t>(out[i].data_ptr());
+            spans.push_back({at, at + (uintptr_t)(last + 1) * out[i].element_size(), i});
+        }
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i) {
+            TORCH_CHECK(spans[i][0] >= spans[i - 1][1], who, ": outputs ", std::to_string(spans[i - 1][2]), " and ", std::to_string(spans[i][2]), " lie between each other's values");
+        }
     }
     const c10::cuda::CUDAGuard guard(device);
     Tensor norm = like({}, grads[0], at::kFloat), scratch = like({(int64_t)lib.ab_clip_grad_norm_scratch_bytes((int64_t)list.size())}, grads[0], at::kByte);

@@ -150,7 +150,7 @@ typedef struct ab_int4 {
     const void* scale;                /* dtype [n_out, k/group] */
     const void* zero;                 /* uint8 [n_out, k/group] of 0 .. 15, or NULL: 8 everywhere */
 } ab_int4;
-/* x: rows of dtype, x_stride elements apart; y: dense [rows, n_out]. */
+/* x: rows of dtype, x_stride elements apart, up to 65535 of them; y: dense [rows, n_out], apart from x. */
 int ab_linear_int4(const ab_int4* m, int rows, const void* x, int64_t x_stride, void* y, void* stream);
 
 /* ---- token sampling on the device -----------------------------------------------------------

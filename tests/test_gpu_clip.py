@@ -98,7 +98,7 @@ def test_a_bucket_with_a_single_value_in_front():
     check(grads, 0.3)
 
 
-@pytest.mark.parametrize("count", [59, 60, 61, 999, 1000, 1001, 2500])
+@pytest.mark.parametrize("count", [60, 119, 120, 121, 999, 1000, 1001, 2500])
 def test_number_of_tensors(count):
     shapes = [(1 + (37 * i) % 300,) for i in range(count)]
     check(some(shapes, "bf16", seed=count), 1.0)
@@ -206,7 +206,9 @@ def test_what_does_not_fit_is_refused():
            dict(scale=float("inf")), dict(scale=float("nan")), dict(out=[g[0].clone()]), dict(out=[g[0].clone(), g[0].clone()]), dict(out=[g[0].cpu(), g[1].clone()]),
            dict(grads=[g[0], g[0]]), dict(grads=[flat[:100], flat[50:150]]), dict(grads=[flat[:100], flat[200:]], out=[flat[100:200], flat[150:250]]),
            dict(grads=[flat[:100], flat[100:200]], out=[flat[100:200], flat[200:]]), dict(grads=[flat[:100]], out=[flat[1:101]]), dict(grads=[flat[:1].expand(50)]),
-           dict(grads=[flat[:100]], out=[flat.view(torch.float32)[:100]]), dict(grads=[g[0]], out=[leaf]), dict(grads=[g[0].to_sparse()])]
+           dict(grads=[flat[:100]], out=[flat.view(torch.float32)[:100]]), dict(grads=[g[0]], out=[leaf]), dict(grads=[g[0].to_sparse()]),
+           # not dense, and among each other's values
+           dict(grads=[flat[:100:2], flat[1:100:2]]), dict(grads=[flat.view(30, 10)[:, :3], flat.view(30, 10)[:, 2:5]]), dict(grads=[flat.view(30, 10)[:20, :3], flat[50:60]])]
     for b in bad:
         args = {"grads": g, "max_norm": 1.0, **b}
         with pytest.raises(RuntimeError):

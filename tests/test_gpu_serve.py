@@ -85,6 +85,18 @@ def test_filters(f, dtype):
     check(*rows_of(3, 50277, dtype, seed=4, spread=(0.2, 3.0)), **f)
 
 
+LONG = [{}, {"p": 0.9}, {"p": 0.9999}, {"m": 0.001}, {"k": 5000}, {"k": 700, "p": 0.9}, {"T": 3.0, "p": 0.5}, {"T": 0.05}, {"p": 0.7, "m": 0.2}, {"p": 0.95, "m": 1e-4}, {"k": 400, "m": 0.3}]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("f", LONG, ids=lambda f: "_".join(f"{a}{b}" for a, b in f.items()) or "all")
+def test_filters_of_long_and_even_rows(f, dtype):
+    """Rows that several blocks share, and rows so even that no small part of them has most of the weight."""
+    check(*rows_of(5, 70001, dtype, seed=30, spread=(0.05, 3.0)), **f)
+    check(*rows_of(2, 200003, dtype, seed=31, spread=(0.5, 4.0)), **f)
+    check(*rows_of(40, 65536, dtype, seed=32, spread=(0.05, 1.5)), **f)
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
 def test_each_row_with_filters_of_its_own(dtype):
     n = 200   # more rows than SMs
@@ -178,6 +190,7 @@ def test_numbers_out_of_range_in_tensors_filter_nothing_or_everything():
     check(x, u, p=t(-1.0, 0.0, inf, nan, 1.0, 1e-38))
     check(x, u, m=t(-1.0, 0.0, inf, nan, 1.0, 1e-38))
     check(x, u, k=torch.tensor([-5, 0, 999, 2 ** 31 - 1, 998, 1], device="cuda", dtype=torch.int32))
+    check(x, u, k=torch.tensor([2 ** 32 + 5, -2 ** 32 + 5, 2 ** 31, 2 ** 62, 3, 2 ** 32 + 1], device="cuda"))
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
@@ -207,6 +220,26 @@ def test_large_vocabulary_and_many_rows():
     check(*rows_of(2, 1 << 18, "fp32", seed=14), p=0.9)
     check(*rows_of(1, (1 << 18) - 3, "bf16", seed=14))
     check(*rows_of(2000, 65, "fp16", seed=15), p=0.9)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^32 bytes, and 2^31 values, of logits; the last rows as by themselves."""
+    n, V = 34000, 65536
+    x = torch.zeros(n, V, device="cuda", dtype=torch.float16)
+    tail, u = rows_of(20, V, "fp16", seed=22)
+    x[-20:] = tail
+    v = torch.cat([torch.full((n - 20,), 0.5, device="cuda"), u])
+    for f in ({}, {"top_k": 40}, {"top_p": 0.8, "min_p": 0.01}):
+        ids, logp = ab.sampler_batch(x, v, **f)
+        want, want_p = ab.sampler_batch(tail, u, **f)
+        assert torch.equal(ids[-20:], want) and torch.equal(logp[-20:], want_p)
+        assert bool((ids[:-20] == ids[0]).all())
+    check(tail, u)
+    del x
+    x = torch.zeros(20000, V, device="cuda")
+    x[-20:] = tail.float()
+    ids, _ = ab.sampler_batch(x, torch.cat([torch.full((20000 - 20,), 0.5, device="cuda"), u]), top_k=40)
+    assert torch.equal(ids[-20:], ab.sampler_batch(tail, u, top_k=40)[0]) and bool((ids[:-20] == 20).all())   # 40 equals: the 21st
 
 
 def test_no_rows():
@@ -307,6 +340,17 @@ def test_products_with_4_bit_weights_of_model_sizes(M, N, K, group, dtype):
     int4_check(*int4_inputs(M, N, K, group, True, dtype, seed=1))
 
 
+def test_a_matrix_of_more_than_32_bits_of_bytes():
+    N, K = 131072 + 7, 65536
+    g = torch.Generator(device="cuda").manual_seed(9)
+    w = torch.randint(0, 256, (N, K // 2), device="cuda", generator=g, dtype=torch.uint8)
+    scale = (0.01 + 0.01 * torch.rand(N, K // 128, device="cuda", generator=g)).half()
+    x = torch.randn(2, K, device="cuda", generator=g).half()
+    y = ab.linear_int4(x, w, scale)
+    for rows in (slice(0, 50), slice(N // 2, N // 2 + 50), slice(N - 50, N)):
+        int4_check(x, w[rows].clone(), scale[rows], None, y[:, rows])
+
+
 def test_quantizer_and_its_product():
     g = torch.Generator(device="cuda").manual_seed(5)
     w = 0.02 * torch.randn(513, 1024, device="cuda", generator=g)
@@ -395,7 +439,8 @@ def test_what_does_not_fit_is_refused():
     for bad in (dict(u=u[:3]), dict(u=u.double()), dict(u=u.cpu()), dict(x=x.int()), dict(x=x.cpu()), dict(x=x[:, :0]), dict(x=torch.zeros(4, (1 << 18) + 1, device="cuda")),
                 dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_p=-0.1), dict(top_p=float("nan")), dict(min_p=-0.1), dict(temperature=u[:2]), dict(top_p=u.cpu()),
                 dict(top_k=u), dict(top_p=torch.ones(4, device="cuda", dtype=torch.int32)), dict(out=torch.zeros(4, device="cuda")), dict(out=torch.zeros(4, dtype=torch.int64)),
-                dict(out=torch.zeros(3, dtype=torch.int64, device="cuda")), dict(out=torch.zeros(8, dtype=torch.int64, device="cuda")[::2])):
+                dict(out=torch.zeros(3, dtype=torch.int64, device="cuda")), dict(out=torch.zeros(8, dtype=torch.int64, device="cuda")[::2]),
+                dict(x=x, out=x.view(torch.int64)[:, 0].as_strided((4,), (1,)))):
         args = {"x": x, "u": u, **bad}
         with pytest.raises(RuntimeError):
             ab.sampler_batch(args.pop("x"), args.pop("u"), **args)

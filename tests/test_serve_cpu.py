@@ -46,7 +46,7 @@ def int4(rows=1, x=256, stride=128, y=256, **more):
 
 
 def test_4_bit_products_refuse_bad_arguments():
-    for bad in (dict(dtype=2), dict(rows=-1), dict(n_out=0), dict(k=0), dict(k=-128), dict(group=16), dict(group=0), dict(group=-128), dict(group=96, k=192), dict(group=64, k=96), dict(k=100),
+    for bad in (dict(dtype=2), dict(rows=-1), dict(rows=65536), dict(n_out=0), dict(k=0), dict(k=-128), dict(group=16), dict(group=0), dict(group=-128), dict(group=96, k=192), dict(group=64, k=96), dict(k=100),
                 dict(w=None), dict(scale=None), dict(x=None), dict(y=None), dict(w=264), dict(scale=257), dict(x=257), dict(y=257), dict(stride=-1)):
         assert int4(**bad) == BAD, bad
         assert "ab_linear_int4" in message()

@@ -7,7 +7,7 @@
 // All three filters keep a front part of one and the same order, and so does the draw: each is a question "where in that order do the weights (or the
 // ranks) reach X?". What bounds it is less the reading of a row (it stays in shared memory, of one block or of a cluster's) than what is done for each of its values, so
 // the way goes by what the filters leave:
-//   few values    top-k up to 1024, or min-p: the k-th largest of the threads' own maxima is a bound that some k values and a few more reach. Those are
+//   few values    top-k up to 600 over the row's blocks, or min-p: the k-th largest of the threads' own maxima is a bound that some k values and a few more reach. Those are
 //                 gathered, sorted, and their weights added up: every question is answered among them, without an exponential for any other value.
 //   a bracket     else the sum over the row is needed: 32-bit exponentials and a histogram of counts over 4096 bins of max - l in one pass. A bin's counts
 //                 bound its weights within a percent, so they say in which few bins X is reached; their values are gathered and sorted, and what lies
@@ -35,7 +35,6 @@ constexpr int SP_LIST = 256;                   // values that are compared with 
 constexpr int SP_MAX_BLOCKS = 8;               // of a cluster: a row's at most
 constexpr int SP_ROW_BYTES = 129 * 1024;       // of a row in a block's shared memory, at most
 constexpr uint64_t SP_ONE = 1ull << 44;        // a weight of 1
-constexpr int SP_FEW = 1024;                   // values that are sorted: one per thread
 
 struct SampleArgs {
     const void* logits;
@@ -875,6 +874,8 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
 //
 // A counter holds up to 65535: the row's last value is added when the others are counted, so that only a row of 65536 equal ones exceeds it (`extra`).
 constexpr int SK_NT = 1024, SK_BINS = 65536, SK_GROUPS = SK_BINS / 64;
+// Few values' sorting costs what k does, counting the same for all: 1 x 65536 12.2 us of k 100, 15.1 of 300, 19.4 of 400, counted 16.7; 512 rows 48, 60, 75 against 65.
+constexpr int SK_MOST_K = 320;
 static_assert(SK_GROUPS == SK_NT, "a thread per group");
 
 template <class E> struct KeyType;   // how a type's 16 bits are ordered
@@ -931,21 +932,18 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
         }
         return q;
     };
-    // all of it under way at once (a row that begins off a boundary has one piece more for some threads)
-    constexpr int AHEAD = 8;
-    uint4 q[AHEAD];
-    auto request = [&](int c0) {
+    // Three pieces of a thread under way. (All eight at once make eight times the code of what is done with one, and the fetching of instructions, which run once a row
+    // here, was what the kernel waited for most: 1 x 65536 23.7 us against 21.0, 320 x 65536 48.4 against 42.7.)
+    uint4 q[3];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
-            if (c0 + 32 * j < end) q[j] = piece(c0 + 32 * j);
-    };
-    request(own);
+    for (int j = 0; j < 3; ++j)
+        if (own + 32 * j < end) q[j] = piece(own + 32 * j);
     const RowFilters f = RowFilters(a, row);
     if (row + a.ahead < a.rows) {   // a row that a block will take when this one is done
         const char* next = reinterpret_cast<const char*>(static_cast<const E*>(a.logits) + (row + a.ahead) * a.stride) + (size_t)threadIdx.x * 128;
         if ((int64_t)threadIdx.x * 64 < a.V) asm volatile("prefetch.global.L2 [%0];" ::"l"(next));
     }
-    const bool bounded = f.by_rank ? f.k <= 600 : !f.by_sum && f.by_size, counting = !f.greedy && !bounded;
+    const bool bounded = f.by_rank ? f.k <= SK_MOST_K : !f.by_sum && f.by_size, counting = !f.greedy && !bounded;
     uint32_t* words = reinterpret_cast<uint32_t*>(s.counts);
     auto count = [&](uint32_t bin) { atomicAdd(words + (bin >> 1), bin & 1 ? 0x10000u : 1u); };
     auto clear = [&]() {
@@ -961,12 +959,19 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
     auto count_piece = [&](const uint4& q, int c) {
         const int at = c * 8 - skip;
         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        const bool whole = at >= 0 && at + 8 < a.V;   // (the last value is added below)
+        if (at >= 0 && at + 8 < a.V) {   // (the row's last value is added below)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t sign = (w[i] >> 15) & 0x00010001u, bins = w[i] ^ (0x7fff7fffu - sign * 0x7fffu);
-            if (whole || (at + 2 * i >= 0 && at + 2 * i < a.V - 1)) count(bins & 0xffffu);
-            if (whole || (at + 2 * i + 1 >= 0 && at + 2 * i + 1 < a.V - 1)) count(bins >> 16);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t sign = (w[i] >> 15) & 0x00010001u, bins = w[i] ^ (0x7fff7fffu - sign * 0x7fffu);
+                count(bins & 0xffffu);
+                count(bins >> 16);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = max(0, -at); i < 8 && at + i < a.V - 1; ++i) {
+                const uint32_t two = i < 2 ? w[0] : i < 4 ? w[1] : i < 6 ? w[2] : w[3], bits = two >> (16 * (i & 1)) & 0xffffu;
+                count(bits < 0x8000u ? 0x7fffu - bits : bits);
+            }
         }
     };
     if (threadIdx.x < 16) s.tab[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
@@ -976,15 +981,15 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
         __syncthreads();
     }
     float top = -INFINITY;
-    for (int c0 = own; c0 < end; c0 += 32 * AHEAD) {
-        if (c0 != own) request(c0);
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
-            if (c0 + 32 * j < end) {
-                top = larger_or_nan(top, largest<E>(q[j]));
-                if (counting) count_piece(q[j], c0 + 32 * j);
-            }
+#pragma unroll 1
+    for (int c = own; c < end; c += 32) {
+        const uint4 v = q[0];
+        q[0] = q[1], q[1] = q[2];
+        if (c + 96 < end) q[2] = piece(c + 96);
+        top = larger_or_nan(top, largest<E>(v));
+        if (counting) count_piece(v, c);
     }
+    constexpr int AHEAD = 8;   // of the passes behind this one
     const uint32_t own_top = own < end ? (top == top ? key_of(top) : 0xffffffffu) : 0;   // a NaN on top of all
     uint32_t top_key = __reduce_max_sync(0xffffffffu, own_top);
     if (lane == 0) s.tops[warp] = top_key;
@@ -1020,8 +1025,11 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
             least = f.size_bound(top);
         }
         Few<SK_NT> few = {s.few, reinterpret_cast<uint64_t*>(s.counts), lane, warp, 32, 0};
-        for (int c0 = own; c0 < end; c0 += 32 * AHEAD) {
-            if (end - own > 32 * AHEAD) request(c0);   // (else it is still there)
+        for (int c0 = own; c0 < end && own_largest >= least; c0 += 32 * AHEAD) {   // (from L2, by the few threads that have some)
+            uint4 q[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+                if (c0 + 32 * j < end) q[j] = piece(c0 + 32 * j);
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const int c = c0 + 32 * j;
@@ -1046,6 +1054,7 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
         __syncthreads();
         clear();   // (many equals, or a small min_p)
         __syncthreads();
+#pragma unroll 1
         for (int c = own; c < end; c += 32) count_piece(piece(c), c);
         __syncthreads();
     }
@@ -1211,35 +1220,36 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
                 }
                 return b;
             };
-            if (f.by_sum) {
-                const uint64_t X = min(kept, (uint64_t)fmax(1.0, ceil(f.p * (double)kept)));
-                last = ends(X);
-                kept = before + how_many(X - before, w) * w;
-            }
-            if (f.by_size && !(last < SK_BINS && weight_at(last) >= f.m)) {
-                // the last bin whose weight is m or more lies near this one; weights fall from bin to bin
-                const int near = (int)bin_at(top < INFINITY ? fminf(top, (float)fmax(-3.4e38, (double)top + f.T * log(f.m))) : top), b = near - 15 + lane;
-                const bool large = b < (int)top_bin || (b < K::NEG_INF && weight_at((uint32_t)b) >= f.m);
-                const int to = near - 16 + __popc(__ballot_sync(0xffffffffu, large));
-                uint64_t sum = 0;   // up to that bin
-                if (to >= (int)top_bin) {
-                    const int g = to >> 6;
-                    const uint32_t word = words[g * 32 + lane], c = g * 64 + 2 * lane;
-                    const Two v = weights(c);
-                    if (c < floor_ && (int)c <= to) sum += counted(word, 0) * v.a;
-                    if (c + 1 < floor_ && (int)c + 1 <= to) sum += counted(word, 1) * v.b;
+#pragma unroll 1
+            for (int step = f.by_sum ? 0 : 1; step < 2; ++step) {   // where top-p ends; then the draw (one code for both)
+                if (step == 1) {
+                    if (f.by_size && !(last < SK_BINS && weight_at(last) >= f.m)) {
+                        // the last bin whose weight is m or more lies near this one; weights fall from bin to bin
+                        const int near = (int)bin_at(top < INFINITY ? fminf(top, (float)fmax(-3.4e38, (double)top + f.T * log(f.m))) : top), b = near - 15 + lane;
+                        const bool large = b < (int)top_bin || (b < K::NEG_INF && weight_at((uint32_t)b) >= f.m);
+                        const int to = near - 16 + __popc(__ballot_sync(0xffffffffu, large));
+                        uint64_t sum = 0;   // up to that bin
+                        if (to >= (int)top_bin) {
+                            const int g = to >> 6;
+                            const uint32_t word = words[g * 32 + lane], c = g * 64 + 2 * lane;
+                            const Two v = weights(c);
+                            if (c < floor_ && (int)c <= to) sum += counted(word, 0) * v.a;
+                            if (c + 1 < floor_ && (int)c + 1 <= to) sum += counted(word, 1) * v.b;
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    sum += g > first ? s.sums[g - first - 1] : 0;
+                            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                            sum += g > first ? s.sums[g - first - 1] : 0;
+                        }
+                        kept = max(SP_ONE, min(kept, sum));
+                    }
+                    if (lane == 0) s.kept = kept;
+                    hand_over();
                 }
-                kept = max(SP_ONE, min(kept, sum));
+                const uint64_t X = min(kept, step ? (uint64_t)floor(f.u * (double)kept) + 1 : (uint64_t)fmax(1.0, ceil(f.p * (double)kept)));
+                const uint32_t b = ends(X);
+                const uint64_t n = how_many(X - before, w);
+                if (step == 0) last = b, kept = before + n * w;
+                else if (lane == 0) s.bin = b, s.ordinal = n - 1;
             }
-            if (lane == 0) s.kept = kept;
-            hand_over();
-            const uint64_t X = min(kept, (uint64_t)floor(f.u * (double)kept) + 1);
-            const uint32_t b = ends(X);
-            const uint64_t n = how_many(X - before, w) - 1;
-            if (lane == 0) s.bin = b, s.ordinal = n;
         }
         __syncthreads();
         bin = s.bin, ordinal = s.ordinal;
@@ -1248,7 +1258,10 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
     const uint32_t as = bits_of_bin(bin) * 0x00010001u;
     uint32_t n = 0, masks[3] = {0, 0, 0};   // a bit for each of a piece's values, eight pieces and one
     for (int i = 0, c0 = own; i == 0 || c0 < end; c0 += 32 * AHEAD, ++i) {
-        request(c0);
+        uint4 q[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (c0 + 32 * j < end) q[j] = piece(c0 + 32 * j);
         if (i == 0 && threadIdx.x == 0)
             a.logp[row] = f.greedy ? 0.f : (float)((bin != top_bin ? ((double)value_at(bin) - (double)top) * (r.c * 0.693147180559945309417) : 0.0) - s.log_kept);
 #pragma unroll
@@ -1478,32 +1491,44 @@ template <class E>
 int sample_launch(SampleArgs a, cudaStream_t st) {
     constexpr int PER = 16 / sizeof(E), NT = 1024;
     static PerDeviceOnce once;
+    static int fit[AB_MAX_DEVICES][4];   // clusters of 1, 2, 4 and 8 blocks that a device holds at a time
     const DeviceProps* dev;
     const auto kernel = sample_filtered_kernel<E, NT>;
     const int head = (int)sizeof(SampleShared<NT>);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    auto configure = [&](int64_t rows, int blocks, size_t smem) {
+        cfg.gridDim = dim3((unsigned)(rows * blocks));
+        cfg.blockDim = dim3(NT);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = blocks;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    };
     const int err = once.run(&dev, [&](const DeviceProps& d) -> int {
         AB_CHECK_ARG(d.smem_optin >= (size_t)head + SP_ROW_BYTES, "sampling: %zu bytes of shared memory per block are too few", d.smem_optin);
-        return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, head + SP_ROW_BYTES), "cudaFuncSetAttribute(sampling)");
+        AB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, head + SP_ROW_BYTES));
+        for (int i = 0; 1 << i <= SP_MAX_BLOCKS; ++i) {
+            configure(1, 1 << i, (size_t)head + SP_ROW_BYTES);
+            AB_CUDA(cudaOccupancyMaxActiveClusters(&fit[&d - once.props][i], kernel, &cfg));
+        }
+        return OK;
     });
     if (err != OK) return err;
     const int pieces = (a.V + 2 * PER - 2) / PER;   // wherever the row starts
-    int blocks = 1;
-    while ((pieces + blocks - 1) / blocks * 16 > SP_ROW_BYTES) blocks *= 2;
-    AB_CHECK_ARG(blocks <= SP_MAX_BLOCKS, "sampling: a vocabulary of %d is too large", a.V);
-    while (blocks < SP_MAX_BLOCKS && a.rows * blocks * 2 <= dev->n_sm && pieces > 1024 * blocks) blocks *= 2;
+    int lg = 0;
+    while ((pieces + (1 << lg) - 1) / (1 << lg) * 16 > SP_ROW_BYTES) ++lg;
+    AB_CHECK_ARG(1 << lg <= SP_MAX_BLOCKS, "sampling: a vocabulary of %d is too large", a.V);
+    // More blocks to a row while all rows run at once, a piece or more to each thread. (fp32 65536, top-p: 1 row in eight blocks 48 us, in two 62. But 16 rows in eight blocks,
+    // of which 128 SMs hold fewer than 16 clusters at a time, take two turns: under top-k 50 24.8 us, in four 12.1.)
+    while (1 << lg < SP_MAX_BLOCKS && a.rows <= fit[dev - once.props][lg + 1] && pieces > 1024 << lg) ++lg;
+    const int blocks = 1 << lg;
     AB_CHECK_ARG(a.rows <= INT32_MAX / blocks, "sampling: too many rows");
     a.share = (pieces + blocks - 1) / blocks;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.rows * blocks));
-    cfg.blockDim = dim3(NT);
-    cfg.dynamicSmemBytes = (size_t)head + (size_t)a.share * 16;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = blocks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    configure(a.rows, blocks, (size_t)head + (size_t)a.share * 16);
     AB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
     return OK;
 }

@@ -12,6 +12,10 @@
 // Blocks divide the outputs evenly, to single ones (the tiles of a block are as high as its share asks for), and a block's warps its pieces, tile after tile: a warp
 // stores the tiles that it has to itself, leaves its sums of those that it shares in shared memory, and at the end they are added up in one order. Nobody waits before
 // that. Where the activations do not fit into shared memory, a cluster of `ks` blocks divides the inputs.
+//
+// Measured, one batch row: 65536 x 4096 fp16 in groups of 128 33 us, 4.2 TB/s of codes and scales (27 with the arithmetic left out: 5.1); 4096 x 4096 7.4 (6.3), of which some 6 are the
+// launch, the activations and the way to the first piece. The warps issue 147 instructions for 2048 codes, 2.2 a cycle and SM of 4; more warps or fewer (24, 8), codes taken as
+// subnormal numbers (132 instructions) and zero points taken out by sums of the inputs were no faster, the last two slower in groups of 32 and with eight rows (20.5 -> 26).
 #include <cuda.h>
 #include <cuda_bf16.h>
 

@@ -20,6 +20,9 @@
 // Precision: weights are taken as multiples of 2^-44 (the largest is 2^44 of them), so that sums are whole numbers and do not depend on the order of additions; they
 // come from a table and a polynomial in 64 bits (off by 1e-15). What comes out is the id that the definition in 64 bits gives, unless u or p meets a border
 // within some 1e-9 of the sum. The log-probability has the 32-bit sum where a bracket sufficed: off by EPS.
+//
+// Measured, fp32 x 65536: one row under top-p 0.9 20 us, 48 to 57 where it comes to whole numbers (a row in ten of normal logits), 9 under min-p 0.05; 512 rows under top-p 0.9 300, two blocks a
+// row, of which an SM holds one. 16-bit rows of up to 65536 values and a small top-k of the same k have kernels of their own, below.
 #include <cooperative_groups.h>
 
 #include "train.cuh"
@@ -866,8 +869,10 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
 // A row's histogram over the values themselves, in shared memory, says everything but which id has a value: what is kept and drawn is found among the
 // counters, whose running sums are exact, and the row is read once more (from L2) for the id. No value of the row needs an exponential: the counters do, and eight
 // of them that follow one another, a unit, whose values are equally far apart, need one of them and its products with exp(-distance / T). Where the filters leave
-// few values (top-k; min-p by itself), only those are counted that reach a bound: some k of the threads' own maxima do, and so do k values.
-// What bounds it: the atomics (3.3 cycles for a warp's: two of its values meet a bank), then the units' weights.
+// few values (a small top-k; min-p by itself), only those are gathered that reach a bound: some k of the threads' own maxima do, and so do k values.
+// What bounds it: for rows that wait for an SM the atomics (3.3 cycles for a warp's: two of its values meet a bank), the units' weights, and the row read twice; for the only row of an SM the steps
+// behind one another, each by code that has to be fetched. fp16, 65536 values: one row 21 us under top-p 0.7 (8 under min-p 0.05), 320 rows with filters of their own 43, in three turns of
+// 148; 37 x 50277 bf16 16. In clusters that take exponentials and search (as fp32 rows do, above) the 320 rows took 109.
 //
 // Counters lie in the order of the values, larger ones first, eight in 16 bytes. Eight units are a group, whose sums are run up over the block; a question is answered by
 // a search among them and by the 64 counters of one group, by the first warp.
@@ -1299,9 +1304,11 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
     }
 }
 // ---- top-k of the same small k for every row --------------------------------------------------------------------------------------------
-// Rows are streamed, two blocks of 512 threads to an SM (k up to 256; one of 1024 up to 600), so that one reads while the other sorts: a row's largest values per thread, a bound that k threads reach, then only the batches
-// of a thread that reach it once more (from L2), and what the few values answer. What bounds it is the reading; 512 x 65536 fp32: 106 us in clusters that keep rows in shared
-// memory. Where more values than threads reach the bound (equals, mostly), the k-th largest key is searched by counting, and of its equals the first ids are taken.
+// Rows are streamed, two blocks of 512 threads to an SM (k up to 256; one of 1024 up to 600), so that one reads while the other sorts: a row's largest values per thread,
+// a bound that k threads reach, then only the values of a thread that reach it once more (from L2), and what the few values answer. Where more values than threads reach the
+// bound (equals, mostly), the k-th largest key is searched by counting, and of its equals the first ids are taken.
+// What bounds it: reading, at 37 % of the memory's rate, and the barriers between the steps. 512 x 65536 fp32, top-k 50: 41 us (3.2 TB/s); in clusters that keep rows in shared memory 105. For
+// one fp32 row it takes 14 us where those take 12.7 (k 50), and 20 where they take 37 (k 400): one kernel for every number of rows.
 constexpr int ST_BATCH = 8, ST_MOST_K = 600;
 
 template <int ST_NT>
@@ -1537,6 +1544,8 @@ int sample_launch(SampleArgs a, cudaStream_t st) {
 
 int sample_filtered(int dtype, int64_t rows, int V, const void* logits, int64_t stride, const float* u, const ab_sampling& p, int64_t* ids, float* logp, cudaStream_t st) {
     const SampleArgs a = {logits, u, p.temperature, p.top_p, p.min_p, p.top_k, p.temperature_all, p.top_p_all, p.min_p_all, p.top_k_all, V, rows, stride, ids, logp, 0, 0};
+    // 16-bit rows of up to 65536: counters. Streamed instead where more rows than SMs have the same top-k of up to 256: 512 x 65536 fp16 with k of 50 38 us against 45, 256 50 against 59, but
+    // 400 72 against 67; and one row with k 50 14.5 against 11.5.
     const bool keys = V <= SK_BINS && dtype != AB_DT_F32, streams = !p.top_k && p.top_k_all > 0 && p.top_k_all <= ST_MOST_K && p.top_k_all < V;
     if (streams && !(keys && (rows <= current_sm_count() || p.top_k_all > 256)))
         return dtype == AB_DT_F16 ? sample_top_launch<__half>(a, st) : dtype == AB_DT_BF16 ? sample_top_launch<__nv_bfloat16>(a, st) : sample_top_launch<float>(a, st);

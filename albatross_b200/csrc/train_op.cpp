@@ -424,7 +424,7 @@ Tensor clip_grad_norm(at::TensorList grads, double max_norm, double scale, at::T
     std::vector<Tensor> copies;                         // kept until the kernels are launched
     std::vector<std::pair<size_t, Tensor>> back;        // outputs that are copied to where they belong
     auto fits = [&](const Tensor& t) {   // (what has no autograd metadata has no tangent)
-        return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.device() == device && is_known(t) && t.has_storage() &&
+        return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.device() == device && is_known(t) && t.has_storage() && !t.is_neg() &&
                (!t.unsafeGetTensorImpl()->autograd_meta() || !t._fw_grad(/*level=*/0).defined());
     };
     at::AutoDispatchBelowADInplaceOrView below;
@@ -484,7 +484,6 @@ TORCH_LIBRARY(albatross_b200, m) {
           "-> (Tensor, Tensor)", policy_loss);
     m.def("policy_loss_grad(Tensor logits, Tensor ids, Tensor? old_logp, Tensor advantages, Tensor? mask, Tensor? ref_logp, float clip_low, float clip_high, float kl, float denom, "
           "float scale, Tensor? out) -> (Tensor, Tensor, Tensor)", policy_loss_grad);
-    m.def("clip_grad_norm(Tensor[] grads, float max_norm, float scale, Tensor[] out) -> Tensor", clip_grad_norm);
     m.def("preference_loss(Tensor logits, Tensor ids, Tensor ref_logp, Tensor? mask, float beta, float smoothing) -> (Tensor, Tensor)", preference_loss);
 }
 

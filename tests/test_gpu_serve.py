@@ -98,6 +98,21 @@ def test_filters_of_long_and_even_rows(f, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_k_and_rows_on_either_side_of_the_lines_between_kernels(dtype):
+    """k around those that are sorted, streamed and counted, given once and for each row; batches that a row's blocks are counted by."""
+    x, u = rows_of(3, 9001, dtype, seed=40, spread=(0.2, 1.0))
+    many, v = rows_of(150, 1003, dtype, seed=41, spread=(0.2, 1.0))
+    for k in (75, 76, 150, 151, 255, 256, 257, 300, 301, 320, 321, 599, 600, 601):
+        check(x, u, 1.0, k, 0.98)
+        check(x, u, 1.0, torch.full((3,), k, device="cuda"), 1.0, 1e-3)
+        check(many, v, 0.7, k)
+    for n in (15, 16, 17, 18, 19, 33, 37, 38, 74, 75):
+        x, u = rows_of(n, 33001, dtype, seed=42)
+        check(x, u, 1.0, torch.full((n,), 40, device="cuda"), 0.95)
+        check(x, u, 1.0, 0, 0.9)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
 def test_each_row_with_filters_of_its_own(dtype):
     n = 200   # more rows than SMs
     x, u = rows_of(n, 2051, dtype, seed=5)

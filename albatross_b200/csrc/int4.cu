@@ -11,7 +11,7 @@
 //
 // Blocks divide the outputs evenly, to single ones (the tiles of a block are as high as its share asks for), and a block's warps its pieces, tile after tile: a warp
 // stores the tiles that it has to itself, leaves its sums of those that it shares in shared memory, and at the end they are added up in one order. Nobody waits before
-// that. Where the activations do not fit into shared memory, a cluster of `ks` blocks divides the inputs.
+// that. Where the activations do not fit into shared memory, or the outputs are few, a cluster of `ks` blocks divides the inputs.
 //
 // Measured, one batch row: 65536 x 4096 fp16 in groups of 128 33 us, 4.2 TB/s of codes and scales (27 with the arithmetic left out: 5.1); 4096 x 4096 7.4 (6.3), of which some 6 are the
 // launch, the activations and the way to the first piece. The warps issue 147 instructions for 2048 codes, 2.2 a cycle and SM of 4; more warps or fewer (24, 8), codes taken as
@@ -419,31 +419,68 @@ template <class E, int GROUPS, int NT, bool ZERO>
 int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
     constexpr int MR = NT * 8 / GROUPS, ROOM = I4_SMEM - 1024 - 2 * I4_WARPS * I4_PIECE;   // beside two stages
     static PerDeviceOnce once;
+    static int fits[AB_MAX_DEVICES][4];   // clusters of 1, 2, 4 and 8 blocks that a device holds at a time
     const DeviceProps* dev;
     const auto kernel = int4_rows_kernel<E, GROUPS, NT, ZERO>;
-    const int err = once.run(&dev, [&](const DeviceProps&) -> int {
-        return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, I4_SMEM), "cudaFuncSetAttribute(linear_int4)");
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    auto configure = [&](int clusters, int ks, int passes, int smem) {
+        cfg.gridDim = dim3(clusters * ks, passes);
+        cfg.blockDim = dim3(I4_THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = ks;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = ks > 1 ? 2 : 1;
+    };
+    const int err = once.run(&dev, [&](const DeviceProps& d) -> int {
+        AB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, I4_SMEM));
+        fits[&d - once.props][0] = d.n_sm;
+        for (int i = 1; i < 4; ++i) {
+            configure(1, 1 << i, 1, I4_SMEM);
+            AB_CUDA(cudaOccupancyMaxActiveClusters(&fits[&d - once.props][i], kernel, &cfg));
+            AB_CHECK_ARG(fits[&d - once.props][i] > 0, "linear_int4: the device holds no cluster of %d blocks", 1 << i);
+        }
+        return OK;
     });
     if (err != OK) return err;
     AB_CHECK_ARG((int64_t)a.N * (a.K / 32) < UINT32_MAX, "linear_int4: a matrix of %d x %d is too large", a.N, a.K);
     const int pieces = (a.K + 255) / 256;
     a.pass = MR < a.rows ? MR : a.rows;
-    int tiles = 0, shared = 0;   // of a block; shared memory behind the activations
-    for (a.ks = 1;;) {
+    // The blocks of a cluster divide the inputs where activations do not fit otherwise, and where outputs are few: then each loads a share of the activations, and has tiles of 32 outputs
+    // instead of single ones, as long as two of them hold its outputs. 1 row, groups of 128, undivided against four and eight blocks: 1024 x 4096 7.4 us, 7.2, 5.9; 512 x 16384 13.1, 8.7, 7.5;
+    // 2048 x 8224 (groups of 32) 11.1, 9.6, 10.3; 4096 x 8224 11.9, 13.0, 13.7.
+    int tiles = 0, shared = 0, lg = 0;   // of a block; shared memory behind the activations; of ks
+    const int* const fit_of = fits[dev - once.props];
+    for (const int l : {3, 2})
+        if (lg == 0 && pieces >= 1 << l && a.N <= 2 * I4_ROWS * fit_of[l]) lg = l;
+    for (a.ks = 1 << lg;;) {
         const int64_t x_bytes = (int64_t)((pieces + a.ks - 1) / a.ks) * 512 * a.pass;
         const int tile_bytes = I4_ROWS * a.pass * 4;
         if (x_bytes + (I4_SHARED + (a.ks > 1 ? 8 : 0)) * tile_bytes <= ROOM) {
-            const int fit = dev->n_sm / a.ks, most = (int)((ROOM - x_bytes) / tile_bytes - I4_SHARED) * I4_ROWS;   // outputs whose sums fit (ks > 1)
+            const int passes = (a.rows + a.pass - 1) / a.pass;
+            const int most = a.ks > 1 ? (int)((ROOM - x_bytes) / tile_bytes - I4_SHARED) * I4_ROWS : a.N;   // outputs whose sums fit
+            // All passes at once, one turn of clusters (their beginning is paid once; 1024 x 4096 in groups of 32, 16 rows 23.7 -> 12.2), unless the sums of so many outputs do not fit.
+            int fit = std::max(1, fit_of[lg] / passes);
+            if ((a.N + fit - 1) / fit > most) fit = fit_of[lg];
             a.x_bytes = (int)x_bytes;
             a.clusters = a.N < fit ? a.N : fit;
-            if (a.ks > 1 && (a.N + a.clusters - 1) / a.clusters > most) a.clusters = (a.N + most - 1) / most;
+            if ((a.N + a.clusters - 1) / a.clusters > most) a.clusters = (a.N + most - 1) / most;
+            if (a.clusters > fit && a.clusters <= 2 * fit && a.pass > 8) {   // two turns: rather two passes of half the rows (4096 x 4096, 16 rows: 26.4 -> 11.9)
+                a.pass = (a.pass + 1) / 2, lg = 0, a.ks = 1;
+                continue;
+            }
             const int share = (a.N + a.clusters - 1) / a.clusters;
             tiles = (share + I4_ROWS - 1) / I4_ROWS;
             a.height = (share + tiles - 1) / tiles;
             shared = (I4_SHARED + (a.ks > 1 ? tiles : 0)) * tile_bytes;
             break;
         }
-        if (a.ks < 8) a.ks *= 2;
+        if (a.ks < 8) a.ks *= 2, ++lg;
         else if (a.pass > 1) a.pass = (a.pass + 1) / 2;
         else AB_CHECK_ARG(false, "linear_int4: %d inputs are too many", a.K);
     }
@@ -462,19 +499,7 @@ int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
         set_error("linear_int4: cuTensorMapEncodeTiled failed with %d (%d x %d)", (int)cr, a.N, a.K);
         return ERR_CUDA;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.clusters * a.ks, (a.rows + a.pass - 1) / a.pass);
-    cfg.blockDim = dim3(I4_THREADS);
-    cfg.dynamicSmemBytes = 1024 + a.stages * I4_WARPS * I4_PIECE + a.x_bytes + shared;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = a.ks;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = a.ks > 1 ? 2 : 1;
+    configure(a.clusters, a.ks, (a.rows + a.pass - 1) / a.pass, 1024 + a.stages * I4_WARPS * I4_PIECE + a.x_bytes + shared);
     AB_CUDA(cudaLaunchKernelEx(&cfg, kernel, map, a));
     return OK;
 }

@@ -470,7 +470,7 @@ int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
             a.x_bytes = (int)x_bytes;
             a.clusters = a.N < fit ? a.N : fit;
             if ((a.N + a.clusters - 1) / a.clusters > most) a.clusters = (a.N + most - 1) / most;
-            if (a.clusters > fit && a.clusters <= 2 * fit && a.pass > 8) {   // two turns: rather two passes of half the rows (4096 x 4096, 16 rows: 26.4 -> 11.9)
+            if (a.clusters > fit && a.pass > 8) {   // more turns than one: rather two passes of half the rows (16 rows: 4096 x 4096 26.4 -> 11.9, 65536 x 4096 248 -> 80)
                 a.pass = (a.pass + 1) / 2, lg = 0, a.ks = 1;
                 continue;
             }

@@ -76,5 +76,5 @@ def linear_int4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, zero: Opt
 
     w: uint8 [N, K / 2], even k in the low nibble; scale [N, K / group] of the type of x; zero: uint8 [N, K / group], codes 0 .. 15, or None: 8. group is 32, 64 or
     a multiple of 128. Codes times activations are exact, sums and scales 32-bit; y is rounded once. For few rows, whose time is that of reading the codes: they are
-    read once for up to 16 rows (up to 8 in groups of 32), once more for each further 16. No gradients."""
+    taken in once for up to 8 rows, and for up to 16 where groups are not of 32 and the matrix is small; again for more (up to 65535). No gradients."""
     return _linear_int4(x, w, scale, zero)

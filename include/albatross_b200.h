@@ -142,8 +142,8 @@ int ab_gemm_static_debug_counter(int index, int write, uint32_t* value_host);
 
 /* ---- products with 4-bit weights in groups ---------------------------------------------------
  * No counterpart in the reference: the format that 4-bit checkpoints commonly come in, beside AB_FMT_FP4, which is made here from fp16 ones.
- * y[r, n] = sum_k x[r, k] * (q[n, k] - z[n, k / group]) * s[n, k / group], for few rows: the codes are read once for up to 16 of them (8 where group
- * is 32 and rows exceed 4), again for each further 16. Products of codes and activations are exact, their sums and scales 32-bit. */
+ * y[r, n] = sum_k x[r, k] * (q[n, k] - z[n, k / group]) * s[n, k / group], for few rows: the codes are taken in once for up to 8 of them, and for
+ * up to 16 where group is not 32 and the sums of all outputs fit beside the activations; again, from L2 if they fit there, for more. Products of codes and activations are exact, their sums and scales 32-bit. */
 typedef struct ab_int4 {
     int32_t dtype, n_out, k, group;   /* of scale, x and y: AB_DT_F16 or AB_DT_BF16; group: 32, 64 or a multiple of 128, divides k */
     const void* w;                    /* uint8 [n_out, k/2], even k in the low nibble, codes 0 .. 15; on a 16-byte boundary */

@@ -355,6 +355,17 @@ def test_products_with_4_bit_weights_of_model_sizes(M, N, K, group, dtype):
     int4_check(*int4_inputs(M, N, K, group, True, dtype, seed=1))
 
 
+@pytest.mark.parametrize("M", [1, 9, 16, 40])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_products_where_clusters_divide_the_inputs_and_passes_run_side_by_side(group, M):
+    """Outputs around those up to which four and eight blocks share the inputs, pieces fewer than blocks, rows that make one pass, two and several."""
+    for N in (1, 31, 33, 960, 1023, 1024, 1025, 2240, 2303, 2305):
+        int4_check(*int4_inputs(M, N, 4224, group, False, "fp16", seed=2))
+    for K in (896, 1024, 1152, 1920, 2048, 2176):
+        int4_check(*int4_inputs(M, 515, K, group, True, "bf16", seed=3))
+    int4_check(*int4_inputs(M, 16385, 4096, group, False, "fp16", seed=4))
+
+
 def test_a_matrix_of_more_than_32_bits_of_bytes():
     N, K = 131072 + 7, 65536
     g = torch.Generator(device="cuda").manual_seed(9)

@@ -267,7 +267,7 @@ struct alignas(16) SampleShared {
     FewShared few;
     uint32_t least, most, matches[NT / 32], matched;
     uint32_t top, tops[NT / 32];
-    uint32_t digit, left, bound;          // of the search among the threads' maxima
+    uint32_t digit[2], left[2], bound;    // of the search among the threads' maxima: of each pass its own
     int state;                            // what comes next: the bins of up to two brackets, or a SampleState
     int bins[4];
     Found found;
@@ -346,11 +346,13 @@ struct Sampler {
         if (at < (uint32_t)NT) of(lists() + NT * list, 0)[at] = Few<NT>::entry(v, id);
     }
     // A bound that at least k of this block's threads reach with their maxima (to its upper 16 bits), or 0. Each digit by a histogram of the threads.
+    // (A pass has a digit of its own: nobody waits between reading the first one's and the second pass.)
     __device__ uint32_t reached(uint32_t k, uint32_t key) {
         uint32_t bound = 0;
-        for (int shift = 24; shift >= 16; shift -= 8) {
+        if (threadIdx.x < 2) s.digit[threadIdx.x] = 256;
+        for (int pass = 0; pass < 2; ++pass) {
+            const int shift = 24 - 8 * pass;
             if (threadIdx.x < 256) s.part[0][threadIdx.x] = 0;
-            if (threadIdx.x == 0) s.digit = 256;
             __syncthreads();
             if (key != 0 && (shift == 24 || key >> 24 == bound >> 24)) atomicAdd(&s.part[0][key >> shift & 255], 1u);
             __syncthreads();
@@ -368,15 +370,15 @@ struct Sampler {
                 if (before < k && k <= up) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        if (before < k && k <= before + n[i]) s.digit = 255 - 8 * lane - i, s.left = k - before;
+                        if (before < k && k <= before + n[i]) s.digit[pass] = 255 - 8 * lane - i, s.left[pass] = k - before;
                         before += n[i];
                     }
                 }
             }
             __syncthreads();
-            if (s.digit == 256) return 0;
-            bound |= s.digit << shift;
-            k = s.left;
+            if (s.digit[pass] == 256) return 0;
+            bound |= s.digit[pass] << shift;
+            k = s.left[pass];
         }
         return bound;
     }

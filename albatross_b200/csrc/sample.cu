@@ -243,13 +243,16 @@ struct Few {
         }
         if (draws) {
             const uint64_t X = min(kept, (uint64_t)floor(f.u * (double)kept) + 1);
-            if (off > 0 && (!from_top || !(f.by_sum || f.by_size)) && unsure(X)) return SP_AGAIN;
-            if (on && before < X && X <= cum) {
+            // (kept is exact where its end was found here, among values from the top; one found in another list, or the row's sum, is off, and X with it)
+            if (off > 0 && !(ends && from_top && (f.by_sum || f.by_size)) && unsure(X)) return SP_AGAIN;
+            const bool mine = on && before < X && X <= cum;
+            if (mine) {
                 *id = 0xffffffffu - (uint32_t)e;
                 double l = -log((double)kept * (1.0 / SP_ONE));
                 if (v != r.top) l += ((double)v - (double)r.top) / f.T;
                 *logp = (float)l;
             }
+            if (off > 0 && vote(mine) == 0) return SP_AGAIN;   // (without `off` kept is this list's: X is met)
         }
         return SP_DONE;
     }

@@ -206,7 +206,7 @@ __device__ __forceinline__ void scale_units_to(int type, const ClipTensor& t, ui
 struct ClipHow {
     const double* sums;
     int32_t n_sums;
-    int32_t in_place;      // every out is its g: nothing is to be done where the factor is 1
+    int32_t in_place;      // every out is its g, and of its type: nothing is to be done where the factor is 1
     int32_t writes;        // 0: the norm alone is wanted
     double scale, max_norm;
     float* norm;           // null: another launch of the same call writes it
@@ -278,7 +278,7 @@ int clip_launch(const ab_grad* t, int64_t n, bool writes, double scale, double m
         const int err = clip_list(t, from, n, list);
         if (err != OK) return err;
         for (int i = 0; i < list.n; ++i)
-            if (list.t[i].g != list.t[i].out) how.in_place = 0;
+            if (list.t[i].g != list.t[i].out || (list.t[i].types & 3) != list.t[i].types >> 2) how.in_place = 0;
         const int grid = blocks();
         grad_squares_kernel<CAP><<<grid, CL_THREADS, 0, st>>>(list, sums + how.n_sums);
         AB_CUDA(cudaGetLastError());

@@ -1,6 +1,6 @@
 // The norm over many tensors of gradients, and clipping.
 //
-//   norm = scale sqrt(sum of g^2 over all tensors),   out = f g,   f = scale min(1, max_norm / norm)   (scale alone where the norm is not finite)
+//   norm = scale sqrt(sum of g^2 over all tensors),   out = f g,   f = scale min(1, max_norm / norm)   (scale alone where the norm is not finite in 32 bits)
 //
 // What bounds it: memory. The factor depends on every value, so that the gradients are read twice, and the floor (each read once) is out of reach
 // for what does not stay in L2.
@@ -222,7 +222,8 @@ __global__ void __launch_bounds__(CL_THREADS, CL_BLOCKS_PER_SM) grad_scale_kerne
     sum = clip_block_sum(sum, s);
     const double norm = how.scale * sqrt(sum);
     if (how.norm && blockIdx.x == 0 && threadIdx.x == 0) *how.norm = (float)norm;
-    const float f = (float)(norm > how.max_norm && norm < INFINITY ? how.scale * (how.max_norm / norm) : how.scale);
+    // (not finite: as it is handed out. A norm beyond 32 bits is an infinity to the caller, who is told that nothing is clipped then)
+    const float f = (float)(norm > how.max_norm && (float)norm < INFINITY ? how.scale * (how.max_norm / norm) : how.scale);
     if (!how.writes || (how.in_place && f == 1.f)) return;
     const uint64_t shares = ((uint64_t)list.units + CL_SHARE - 1) / CL_SHARE;
     for (uint64_t i = (uint64_t)blockIdx.x * CL_WARPS + (threadIdx.x >> 5); i < shares; i += (uint64_t)gridDim.x * CL_WARPS) {

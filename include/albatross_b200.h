@@ -268,8 +268,8 @@ int ab_preference_loss_fwd(const ab_logit_rows* t, int64_t pairs, int64_t steps,
                            float* logp32, float* stats, float* g, double* rows_scratch, void* stream);
 
 /* ---- the norm over all gradients, and clipping (no counterpart in the reference) -----------------------------------
- * norm = scale * sqrt(sum of g^2 over all tensors); out = g * f with f = scale * min(1, max_norm / norm), or f = scale where the norm is not
- * finite. Two launches for up to 1000 tensors, two more for each further 1000. */
+ * norm = scale * sqrt(sum of g^2 over all tensors); out = g * f with f = scale * min(1, max_norm / norm), or f = scale where the norm (in
+ * 32 bits) is not finite. Two launches for up to 1000 tensors, two more for each further 1000. */
 typedef struct ab_grad {
     const void* g;               /* n values of dtype, dense */
     void* out;                   /* n values of out_dtype: g itself, or apart from every tensor of the list; NULL in all of them: the norm alone */

@@ -1,4 +1,4 @@
-"""GPU: clipping of gradients where outputs have another type on the same memory."""
+"""GPU: clipping of gradients where outputs have another type on the same memory, and at the ends of the numbers' range."""
 import pytest
 import torch
 
@@ -27,3 +27,14 @@ def test_outputs_of_another_type_on_the_gradients_memory(dtype, to, limit):
             half = torch.finfo(t).eps / 2
             tiny = torch.finfo(t).smallest_normal * torch.finfo(t).eps
             assert bool(((g.view(t).double() - b * f).abs() <= (half + 2.0 ** -21) * b.abs() * f + tiny).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_norm_beyond_32_bits_clips_nothing(dtype):
+    """What is returned is not finite, so the gradients stay as they are, and go into other tensors times the scale alone."""
+    g = torch.full((64,), 3e38, device="cuda").to(dtype)
+    keep = g.clone()
+    assert bool(ab.clip_grad_norm([g], 1.0).isinf()) and torch.equal(g, keep)
+    out = torch.zeros(64, device="cuda")
+    assert bool(ab.clip_grad_norm([g], 1.0, scale=0.125, out=[out]).isfinite()) and not torch.equal(out, 0.125 * keep.float())
+    assert bool(ab.clip_grad_norm([g], 1.0, scale=0.5, out=[out]).isinf()) and torch.equal(out, 0.5 * keep.float())

@@ -151,8 +151,16 @@ __device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b)
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
 }
 
+// The factor, as 32 bits and a power of two: a norm of up to 2^128 leaves a limit's quotient below 2^-126, where 32 bits have few places. (A scale is below 2^128.)
+struct ClipFactor {
+    float f;
+    bool small;
+    __device__ __forceinline__ explicit ClipFactor(double v) : f((float)(v < 0x1p-126 ? v * 0x1p126 : v)), small(v < 0x1p-126) {}
+    __device__ __forceinline__ float of(float v) const { return small ? v * f * 0x1p-126f : v * f; }
+};
+
 template <class E, class O>
-__device__ __forceinline__ void scale_units(const ClipTensor& t, uint32_t lo, uint32_t hi, float f, int lane) {
+__device__ __forceinline__ void scale_units(const ClipTensor& t, uint32_t lo, uint32_t hi, ClipFactor f, int lane) {
     constexpr int N = 16 / sizeof(E), W = N * sizeof(O) / 16;   // stores of 16 bytes per unit (0: of 8)
     const Extent all(t.g, t.n * sizeof(E)), all_out(t.out, t.n * sizeof(O));
     const E* g = static_cast<const E*>(t.g);
@@ -172,7 +180,7 @@ __device__ __forceinline__ void scale_units(const ClipTensor& t, uint32_t lo, ui
         float v[N];
         unpack<E>(q[i], v);
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] *= f;
+        for (int k = 0; k < N; ++k) v[k] = f.of(v[k]);
         O* to = out + t.head + (uint64_t)u * N;
         if (!all_out.holds(to, N)) continue;
         if (t.out_apart == 2) {
@@ -193,11 +201,11 @@ __device__ __forceinline__ void scale_units(const ClipTensor& t, uint32_t lo, ui
     if (hi > whole) {
         const uint64_t behind = t.head + (uint64_t)whole * N;
         const uint64_t at = lane < t.head ? lane : behind + (lane - t.head);
-        if (at < t.n && all.holds(g + at) && all_out.holds(out + at)) out[at] = from_f<O>(to_f(g[at]) * f);
+        if (at < t.n && all.holds(g + at) && all_out.holds(out + at)) out[at] = from_f<O>(f.of(to_f(g[at])));
     }
 }
 template <class E>
-__device__ __forceinline__ void scale_units_to(int type, const ClipTensor& t, uint32_t lo, uint32_t hi, float f, int lane) {
+__device__ __forceinline__ void scale_units_to(int type, const ClipTensor& t, uint32_t lo, uint32_t hi, ClipFactor f, int lane) {
     if (type == AB_DT_F16) scale_units<E, __half>(t, lo, hi, f, lane);
     else if (type == AB_DT_BF16) scale_units<E, __nv_bfloat16>(t, lo, hi, f, lane);
     else scale_units<E, float>(t, lo, hi, f, lane);
@@ -223,8 +231,8 @@ __global__ void __launch_bounds__(CL_THREADS, CL_BLOCKS_PER_SM) grad_scale_kerne
     const double norm = how.scale * sqrt(sum);
     if (how.norm && blockIdx.x == 0 && threadIdx.x == 0) *how.norm = (float)norm;
     // (not finite: as it is handed out. A norm beyond 32 bits is an infinity to the caller, who is told that nothing is clipped then)
-    const float f = (float)(norm > how.max_norm && (float)norm < INFINITY ? how.scale * (how.max_norm / norm) : how.scale);
-    if (!how.writes || (how.in_place && f == 1.f)) return;
+    const ClipFactor f(norm > how.max_norm && (float)norm < INFINITY ? how.scale * (how.max_norm / norm) : how.scale);
+    if (!how.writes || (how.in_place && f.f == 1.f && !f.small)) return;
     const uint64_t shares = ((uint64_t)list.units + CL_SHARE - 1) / CL_SHARE;
     for (uint64_t i = (uint64_t)blockIdx.x * CL_WARPS + (threadIdx.x >> 5); i < shares; i += (uint64_t)gridDim.x * CL_WARPS) {
         const uint64_t at = (shares - 1 - i) * CL_SHARE;

@@ -210,7 +210,7 @@ size_t ab_clip_grad_norm_scratch_bytes(int64_t tensors) { return tensors < 0 ? 0
 int ab_clip_grad_norm(const ab_grad* t, int64_t tensors, double scale, double max_norm, float* norm, void* scratch, void* stream) {
     AB_CHECK_ARG(tensors >= 0 && (t || tensors == 0) && norm && scratch, "ab_clip_grad_norm: null pointer, or a negative number of tensors");
     AB_CHECK_ARG(on_boundary(scratch, 8) && on_boundary(norm, 4), "ab_clip_grad_norm: misaligned pointer");
-    AB_CHECK_ARG(scale > 0 && scale < INFINITY, "ab_clip_grad_norm: the scale must be positive and finite");
+    AB_CHECK_ARG(scale > 0 && (float)scale < INFINITY, "ab_clip_grad_norm: the scale must be positive and finite, in 32 bits");
     AB_CHECK_ARG(max_norm >= 0, "ab_clip_grad_norm: the largest norm is negative or not a number");
     bool with = false, without = false;
     for (int64_t i = 0; i < tensors; ++i) {

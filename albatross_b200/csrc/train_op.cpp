@@ -415,7 +415,7 @@ Tensor clip_grad_norm(at::TensorList grads, double max_norm, double scale, at::T
     constexpr const char* who = "clip_grad_norm";
     TORCH_CHECK(!grads.empty(), who, ": no gradients");
     TORCH_CHECK(out.empty() || out.size() == grads.size(), who, ": ", std::to_string(grads.size()), " gradients and ", std::to_string(out.size()), " outputs");
-    TORCH_CHECK(scale > 0 && scale <= std::numeric_limits<double>::max(), who, ": the scale must be positive and finite");
+    TORCH_CHECK(scale > 0 && scale <= std::numeric_limits<float>::max(), who, ": the scale must be positive and finite, in 32 bits");
     TORCH_CHECK(max_norm >= 0, who, ": the largest norm is negative or not a number");
     check_plain(who);
     const at::Device device = grads[0].device();

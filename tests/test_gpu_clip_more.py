@@ -38,3 +38,22 @@ def test_a_norm_beyond_32_bits_clips_nothing(dtype):
     out = torch.zeros(64, device="cuda")
     assert bool(ab.clip_grad_norm([g], 1.0, scale=0.125, out=[out]).isfinite()) and not torch.equal(out, 0.125 * keep.float())
     assert bool(ab.clip_grad_norm([g], 1.0, scale=0.5, out=[out]).isinf()) and torch.equal(out, 0.5 * keep.float())
+
+
+@pytest.mark.parametrize("dtype,to", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float16)])
+@pytest.mark.parametrize("value,limit,scale", [(1e38, 1.0, 1.0), (1e38, 1e-6, 1.0), (3e38, 1.0, 2.0 ** -10), (1e30, 1e-15, 1.0), (1e10, 1e-28, 1.0), (1.0, 1e-20, 1e-25)])
+def test_factors_below_32_bits_normal_numbers(dtype, to, value, limit, scale):
+    """limit / norm under 2^-126, where a 32-bit number has few places left: the outputs have all of theirs."""
+    g = (value * (0.1 + 0.9 * torch.rand(3, 67, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)))).to(dtype)
+    g[0, 0] = 0.0
+    g *= 8.0 ** -1
+    keep = g.double()
+    out = torch.full(g.shape, torch.nan, device="cuda", dtype=to)
+    norm = ab.clip_grad_norm([g], limit, scale=scale, out=[out])
+    want = scale * float(keep.square().sum()) ** 0.5
+    assert abs(float(norm) - want) <= 2.0 ** -21 * want + 2.0 ** -149
+    f = scale * min(1.0, limit / want)
+    # rounded to 32 bits and to the output's type; products below 2^-126 have steps of 2^-149, and the factor and its product are rounded there
+    tiny = torch.finfo(to).smallest_normal * torch.finfo(to).eps + 2.0 ** -148
+    assert bool(((out.double() - keep * f).abs() <= (torch.finfo(to).eps / 2 + 2.0 ** -21) * keep.abs() * f + tiny).all())
+    assert float(out[0, 0]) == 0.0

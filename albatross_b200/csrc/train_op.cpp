@@ -488,7 +488,14 @@ TORCH_LIBRARY(albatross_b200, m) {
 }
 
 // clip_grad_norm for lists of hundreds of tensors: the dispatcher boxes and unboxes both lists, 0.2 us a tensor of the 0.3 that a call takes. Takes Python lists or
-// tuples of tensors (out: None, for the norm alone) with the interpreter's lock held; returns None, with the error set, where it throws.
+// tuples of tensors (out: None, for the norm alone) with the interpreter's lock held; returns null, with the error set, where it throws. Neither dispatch modes nor the profiler
+// see the call.
+struct LetGo {   // of the interpreter's lock: a launch may have to wait for room in the queue, and what it waits for may need that lock (a host function)
+    PyThreadState* const state = PyEval_SaveThread();
+    LetGo() = default;
+    LetGo(const LetGo&) = delete;
+    ~LetGo() { PyEval_RestoreThread(state); }
+};
 static bool tensors_of(PyObject* list, std::vector<Tensor>& out) {
     PyObject* fast = PySequence_Fast(list, "clip_grad_norm: a list of tensors is expected");
     if (!fast) return false;
@@ -510,7 +517,12 @@ extern "C" PyObject* albatross_b200_clip_grad_norm(PyObject* grads, double max_n
     try {
         std::vector<Tensor> g, o;
         if (!tensors_of(grads, g) || (out != Py_None && out != grads && !tensors_of(out, o))) return nullptr;
-        return THPVariable_Wrap(clip_grad_norm(g, max_norm, scale, out == grads ? g : o));
+        Tensor norm;
+        {
+            const LetGo lock;
+            norm = clip_grad_norm(g, max_norm, scale, out == grads ? g : o);
+        }
+        return THPVariable_Wrap(norm);
     } catch (const c10::Error& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
     } catch (const std::exception& e) {

@@ -6,6 +6,7 @@
 // range-checking build).
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -523,10 +524,8 @@ extern "C" PyObject* albatross_b200_clip_grad_norm(PyObject* grads, double max_n
             norm = clip_grad_norm(g, max_norm, scale, out == grads ? g : o);
         }
         return THPVariable_Wrap(norm);
-    } catch (const c10::Error& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {
+        torch::translate_exception_to_python(std::current_exception());   // (as torch's own bindings do: memory that runs out is torch.OutOfMemoryError)
     }
     return nullptr;
 }

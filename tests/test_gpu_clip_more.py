@@ -1,4 +1,4 @@
-"""GPU: clipping of gradients where outputs have another type on the same memory, and at the ends of the numbers' range."""
+"""GPU: clipping of gradients where outputs have another type on the same memory, at the ends of the numbers' range, and without memory."""
 import pytest
 import torch
 
@@ -57,3 +57,16 @@ def test_factors_below_32_bits_normal_numbers(dtype, to, value, limit, scale):
     tiny = torch.finfo(to).smallest_normal * torch.finfo(to).eps + 2.0 ** -148
     assert bool(((out.double() - keep * f).abs() <= (torch.finfo(to).eps / 2 + 2.0 ** -21) * keep.abs() * f + tiny).all())
     assert float(out[0, 0]) == 0.0
+
+
+def test_memory_that_runs_out_is_told_as_torch_tells_it():
+    """A gradient without memory of its own for each value is copied: more than this process is allowed."""
+    g = torch.ones(1, device="cuda").expand(1 << 34)
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.05)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            ab.grad_norm([g])
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert float(ab.grad_norm([g[:9]])) == 3.0

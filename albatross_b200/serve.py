@@ -53,9 +53,11 @@ class Int4Matrix(NamedTuple):
         return ((q - (8.0 if self.zero is None else self.zero.float()[..., None])) * self.scale.float()[..., None]).view(N, -1)
 
 
+@torch.no_grad()
 def quantize_int4(w: torch.Tensor, group: int = 128, zeros: bool = False, dtype: torch.dtype = torch.float16) -> Int4Matrix:
     """w [N, K] (any float type), in groups of 32, 64 or a multiple of 128 inputs: s = max |w| / 7 and q = rint(w / s) + 8, or with `zeros`
-    s = (max - min) / 15 over the group's values and 0, z = rint(-min / s), q = rint(w / s) + z. `dtype`: of the scales, and so of the activations."""
+    s = (max - min) / 15 over the group's values and 0, z = rint(-min / s), q = rint(w / s) + z. `dtype`: of the scales, and so of the activations.
+    w may be a parameter: the result has no part in its gradients."""
     N, K = w.shape
     if K % group or not (group in (32, 64) or group % 128 == 0):
         raise ValueError(f"groups of {group} inputs (32, 64 or a multiple of 128, which divides {K})")

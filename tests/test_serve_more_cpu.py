@@ -4,6 +4,9 @@ import sys
 import threading
 import time
 
+import pytest
+import torch
+
 import albatross_b200 as ab
 from albatross_b200 import _lib
 
@@ -46,3 +49,14 @@ def test_the_gradient_norm_lets_other_threads_run():
         stop.set()
         thread.join()
     assert ran > 0
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_a_quantised_parameter_takes_no_part_in_gradients(zeros):
+    """A layer's weight as it stands in the module: the scales do not carry its graph, with which linear_int4 would refuse them."""
+    w = torch.nn.Linear(256, 16, bias=False).weight
+    m, plain = ab.quantize_int4(w, 64, zeros), ab.quantize_int4(w.detach(), 64, zeros)
+    assert all(a is b is None or torch.equal(a, b) for a, b in zip(m, plain))
+    assert not any(t is not None and t.requires_grad for t in m) and not m.dequantize().requires_grad
+    turned = ab.quantize_int4(w.detach().t().contiguous().t(), 64, zeros)          # in another order of memory
+    assert all(a is b is None or (torch.equal(a, b) and b.is_contiguous()) for a, b in zip(m, turned))

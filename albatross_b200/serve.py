@@ -33,6 +33,8 @@ def sampler_batch(logits: torch.Tensor, uniform: torch.Tensor, temperature: Numb
     top_p >= 1 and min_p <= 0 filter nothing. Each of the four is a number, or a tensor of one per row on the device of logits (in which a NaN filters nothing; as
     a temperature it is 0). -inf is never drawn; a row with a NaN, or of -inf alone, gives -1 and NaN.
 
+    There are no gradients: the log-probabilities carry none, whatever the logits require (they are an old_logp; token_logp of the ids has one).
+
     `out`: a dense int64 tensor of one id per row to write into, on the device or in pinned host memory (read it after synchronising the stream)."""
     T, k, p, m = temperature, top_k, top_p, min_p
     t = torch.is_tensor

@@ -175,3 +175,16 @@ def test_top_p_at_borders(dtype):
                 p = float(whole.cum[rank] / whole.cum[-1]) + off
                 if float((whole.cum - p * whole.cum[-1]).abs().min()) > GAP * float(whole.cum[-1]) and p < 1:
                     check(x, torch.cat([last, Row(x, p=p).borders(4)]), p=p)
+
+
+def test_draws_carry_no_gradient():
+    """Logits that require a gradient are drawn from; what comes out has none, as the function says, and the gradient by token_logp is not touched."""
+    x = normal(2000, 1.0, 20).expand(4, -1).clone().requires_grad_()
+    u = torch.linspace(0.1, 0.9, 4, device="cuda")
+    ids, logp = ab.sampler_batch(x, u, top_p=0.9)
+    assert not ids.requires_grad and not logp.requires_grad and "no gradients" in ab.sampler_batch.__doc__
+    with torch.no_grad():
+        again, again_p = ab.sampler_batch(x, u, top_p=0.9)
+    assert torch.equal(ids, again) and torch.equal(logp, again_p)
+    ab.token_logp(x, ids[:, 0]).sum().backward()
+    assert bool(x.grad.isfinite().all()) and float(x.grad.abs().max()) > 0

@@ -1,7 +1,5 @@
 // What serves a token, as torch operators beside those of train_op.cpp (torch.ops.albatross_b200.*): arguments checked, memory from torch's allocator,
 // the C entries called on torch's current stream of the tensors' device. Neither has gradients.
-#include <ATen/MemoryOverlap.h>
-
 #include "op.h"
 
 namespace {
@@ -23,6 +21,14 @@ const Tensor per_row(const char* what, const OptTensor& t, const Tensor& logits,
     // (a k that 32 bits do not hold filters nothing)
     return (type == at::kInt && t->scalar_type() == at::kLong ? t->clamp(INT32_MIN, INT32_MAX) : *t).to(type).contiguous();
 }
+// whether the bytes [from, to) meet one of n runs of `length` bytes that begin `step` apart
+bool meets(uintptr_t from, uintptr_t to, const void* base_, uint64_t n, uint64_t length, uint64_t step) {
+    const uintptr_t base = reinterpret_cast<uintptr_t>(base_);
+    if (from == to || n == 0 || length == 0) return false;
+    const uint64_t ended = from < base + length ? 0 : step == 0 ? n : (from - base - length) / step + 1;   // runs that end in front of it
+    return ended < n && base + ended * step < to;
+}
+bool meets(uintptr_t from, uintptr_t to, const Tensor& dense) { return dense.defined() && meets(from, to, dense.data_ptr(), 1, dense.nbytes(), 0); }
 std::tuple<Tensor, Tensor> sample(const Tensor& logits_, const Tensor& uniform, const OptTensor& temperature, const OptTensor& top_k, const OptTensor& top_p, const OptTensor& min_p,
                                   double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all, const OptTensor& out_) {
     constexpr const char* who = "sampler_batch";
@@ -42,7 +48,11 @@ std::tuple<Tensor, Tensor> sample(const Tensor& logits_, const Tensor& uniform, 
     if (ids.defined()) {
         TORCH_CHECK(ids.scalar_type() == at::kLong && ids.numel() == n && ids.is_contiguous() && (ids.device() == rows.device() || (ids.is_cpu() && ids.is_pinned())), who,
                     ": out must be a dense int64 tensor of one id per row, on the device of logits or in pinned host memory");
-        if (ids.is_cuda()) at::assert_no_overlap(ids, logits_), at::assert_no_overlap(ids, uniform);
+        // (rows are drawn side by side: an id must not fall into what another row still reads)
+        const uintptr_t from = reinterpret_cast<uintptr_t>(ids.data_ptr()), to = from + ids.nbytes();
+        TORCH_CHECK(!(ids.is_cuda() && (meets(from, to, rows.data_ptr(), n, V * rows.element_size(), rows.stride(0) * rows.element_size()) || meets(from, to, u) || meets(from, to, T) ||
+                                        meets(from, to, p) || meets(from, to, m) || meets(from, to, k))),
+                    who, ": out lies among the values of an input");
         if (!ids.is_inference()) ids.unsafeGetTensorImpl()->bump_version();
     } else {
         ids = like(sizes, rows, at::kLong);

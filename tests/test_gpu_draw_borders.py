@@ -188,3 +188,33 @@ def test_draws_carry_no_gradient():
     assert torch.equal(ids, again) and torch.equal(logp, again_p)
     ab.token_logp(x, ids[:, 0]).sum().backward()
     assert bool(x.grad.isfinite().all()) and float(x.grad.abs().max()) > 0
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+def test_ids_among_the_values_of_an_input_are_refused(dtype):
+    """Also where the logits' rows lie apart; between rows there is room for ids."""
+    size = DT[dtype].itemsize
+    big = torch.zeros(6, 1024, device="cuda", dtype=DT[dtype])
+    x, u = big[:, 8:1000], torch.full((6,), 0.5, device="cuda")
+    x.normal_()
+    want = ab.sampler_batch(x, u, top_p=0.9)[0]
+    memory = big.view(torch.int64).view(-1)
+    row = 1024 * size // 8
+    for at in (size, row - 1, 3 * row + 10, 5 * row + size - 5, 1000 * size // 8 - 6):
+        with pytest.raises(RuntimeError, match="among the values"):
+            ab.sampler_batch(x, u, top_p=0.9, out=memory[at:at + 6])
+    assert torch.equal(ab.sampler_batch(x, u, top_p=0.9)[0], want)
+    gap = memory[row + 1000 * size // 8:][:6]
+    assert torch.equal(ab.sampler_batch(x, u, top_p=0.9, out=gap)[0], want)
+    several = torch.zeros(12, device="cuda", dtype=torch.int64)
+    numbers = several.view(torch.float32)
+    for name, v in (("temperature", 1.0), ("top_p", 0.9), ("min_p", 0.1)):
+        numbers.fill_(v)
+        for at in (0, 2, 5):
+            with pytest.raises(RuntimeError, match="among the values"):
+                ab.sampler_batch(x, u, out=several[at // 2:at // 2 + 6], **{name: numbers[at:at + 6]})
+    with pytest.raises(RuntimeError, match="among the values"):
+        ab.sampler_batch(x, numbers.fill_(0.5)[:6], out=several[:6])
+    with pytest.raises(RuntimeError, match="among the values"):
+        ab.sampler_batch(x, u, out=several[:6], top_k=several.view(torch.int32)[:6])
+    assert torch.equal(ab.sampler_batch(x, u, top_p=0.9, out=several[:6])[0], want)

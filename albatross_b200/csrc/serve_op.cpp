@@ -16,7 +16,7 @@ struct Entries {
 const Tensor per_row(const char* what, const OptTensor& t, const Tensor& logits, int64_t rows, at::ScalarType type) {
     if (!t.has_value()) return Tensor();
     check_plain("sampler_batch", *t);
-    TORCH_CHECK(t->device() == logits.device() && t->numel() == rows && (type == at::kInt ? at::isIntegralType(t->scalar_type(), false) : at::isFloatingType(t->scalar_type())),
+    TORCH_CHECK(t->device() == logits.device() && t->numel() == rows && (type == at::kInt ? at::isIntegralType(t->scalar_type(), false) && t->scalar_type() != at::kUInt64 : at::isFloatingType(t->scalar_type())),
                 "sampler_batch: ", what, " must be a number, or a tensor of one ", type == at::kInt ? "whole" : "floating", " number per row on the device of logits");
     // (a k that 32 bits do not hold filters nothing)
     return (type == at::kInt && t->scalar_type() == at::kLong ? t->clamp(INT32_MIN, INT32_MAX) : *t).to(type).contiguous();

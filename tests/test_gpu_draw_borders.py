@@ -218,3 +218,13 @@ def test_ids_among_the_values_of_an_input_are_refused(dtype):
     with pytest.raises(RuntimeError, match="among the values"):
         ab.sampler_batch(x, u, out=several[:6], top_k=several.view(torch.int32)[:6])
     assert torch.equal(ab.sampler_batch(x, u, top_p=0.9, out=several[:6])[0], want)
+
+
+def test_a_top_k_of_any_whole_type():
+    """In 32 bits as it was given, or filtering nothing where those do not hold it; what would be cut to its lowest bits is refused."""
+    x, u = normal(1000, 1.0, 21).expand(3, -1), torch.full((3,), 0.999, device="cuda")
+    want = ab.sampler_batch(x, u, top_k=5)[0]
+    for dtype in (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64):
+        assert torch.equal(ab.sampler_batch(x, u, top_k=torch.full((3,), 5, device="cuda", dtype=dtype))[0], want)
+    with pytest.raises(RuntimeError, match="top_k"):
+        ab.sampler_batch(x, u, top_k=torch.full((3,), 2 ** 32 + 5, dtype=torch.uint64).cuda())

@@ -68,8 +68,9 @@ __device__ __forceinline__ int bin_of(const RowScale& r, float v) {   // never f
     const float d = v == r.top ? 0.f : r.top - v;
     return (int)(__float_as_uint(fminf(d * r.bins, SP_BINS - 1) + 8388608.f) & (2 * SP_BINS - 1));   // (2^23: the last places are whole numbers. A conversion has a quarter of the rate)
 }
-// w in 32 bits, by the hardware's 2^x (relative error 2^-22). The product's rounding and what 32 bits leave of c are made good, so that for 16-bit logits, whose differences
-// are exact where they matter, 2^-22 + 2^-23 remains; 32-bit ones add 2^-24 z ln 2 for the difference's rounding, below 2^-20 for z up to 22. d is finite.
+// w in 32 bits, by the hardware's 2^x (relative error 2^-22). The product's rounding and what 32 bits leave of c are made good, so that 2^-22 + 2^-23 remains, and 2^-24 z ln 2 for
+// the rounding of the difference d: below 2^-20 for z up to 22 (values beyond that weigh 2^-4 of the largest at most, all together). 16-bit logits are no better there: 513 and a
+// number of 2^-15 are 26 bits apart. d is finite.
 __device__ __forceinline__ float weight32(float d, float c, float c_low) {
     const float z = d * c, rest = fmaf(d, c_low, fmaf(d, c, -z));
     float w;
@@ -604,7 +605,7 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
         if (x.blocks > 1) x.cluster.sync();   // (the first block's count has been read)
     } else if (!greedy && !by_rank && top < INFINITY && T > 1e-6 && T < 1e6) {
         // ---- a bracket
-        constexpr double EPS = sizeof(E) == 2 ? 0x1p-21 : 0x1p-19;   // of sums of weight32, with room for the additions' own rounding
+        constexpr double EPS = 0x1p-19;                              // of sums of weight32: 2^-22 + 2^-23 + 2^-20, and up to 2^-21 for adding up a piece's eight
         constexpr float MAGIC = 8388608.f;                           // 2^23: the last places are whole numbers
         const float c = (float)x.r.c, c_low = (float)(x.r.c - (double)c), bins = (float)(SP_BINS / (32.0 * T)), far = (SP_BINS - 1) / bins;
         for (int i = threadIdx.x; i < SP_BINS; i += NT) s.part[0][i] = 0;

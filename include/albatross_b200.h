@@ -176,7 +176,7 @@ typedef struct ab_sampling {
     int32_t top_k_all, _pad;
 } ab_sampling;
 /* logits: rows of dtype (AB_DT_*), `stride` elements apart, vocab up to 2^18; uniform: fp32 [rows] in [0, 1) (others are taken into it); ids, logp: [rows], device or
- * pinned host memory. */
+ * pinned host memory, apart from all that is read. */
 int ab_sample_filtered(int dtype, int64_t rows, int vocab, const void* logits, int64_t stride, const float* uniform, const ab_sampling* p,
                        int64_t* ids, float* logp, void* stream);
 

@@ -228,3 +228,15 @@ def test_a_top_k_of_any_whole_type():
         assert torch.equal(ab.sampler_batch(x, u, top_k=torch.full((3,), 5, device="cuda", dtype=dtype))[0], want)
     with pytest.raises(RuntimeError, match="top_k"):
         ab.sampler_batch(x, u, top_k=torch.full((3,), 2 ** 32 + 5, dtype=torch.uint64).cuda())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("f", [{}, {"p": 0.95}, {"p": 0.9995}], ids=str)
+def test_16_bit_values_whose_differences_take_more_than_24(f, dtype):
+    """A largest value of 513 (512 in bf16) and many near 2^-15: each difference is rounded the same way, and weighs that much less or more under a large temperature."""
+    x = torch.full((1 << 18,), 2.0 ** -15 * 0.99, device="cuda")
+    x[:400] = -torch.linspace(1.0, 200.0, 400, device="cuda")
+    x[70000] = 513.0
+    x = x.to(DT[dtype])
+    f = {"T": 51.3, **f}
+    check(x, torch.cat([Row(x, **f).borders(60), torch.linspace(0, 0.09, 40, device="cuda")]), **f)

@@ -144,6 +144,9 @@ struct RowFilters {
 
 enum SampleState : int { SP_LOOK, SP_DONE, SP_AGAIN };   // the row has its id; it has to be done in whole numbers
 
+// Twice what adding up a piece's weights in 32 bits may lose: eight partial sums, 35 / 8 of 2^-24 of the last one.
+constexpr double ADDING = 8.75 * 0x1p-24;
+
 // Few values of a row (key and id of each), sorted, and what they answer: by a block's first `size` threads.
 struct FewShared {
     uint64_t red[32], told[2];
@@ -213,7 +216,7 @@ struct Few {
         return v;
     }
     // Of the n values of a list, behind a sum `front` of all in front of them: what is kept (`ends`: with total the row's sum; under top_k that of the first k is theirs), and
-    // the draw (`draws`). front, and total, may be `off` relative.
+    // the draw (`draws`). Sums of weights in 32 bits, as front is one and total has some, may be `off` relative.
     __device__ SampleState answer(const RowFilters& f, const RowScale& r, const uint64_t* list, uint32_t n, uint64_t front, uint64_t total, double off, bool from_top, bool ends,
                                   bool draws, uint64_t& kept, int64_t* id, float* logp) {
         const uint64_t e = sorted(list, n);
@@ -221,9 +224,11 @@ struct Few {
         const bool on = threadIdx.x < n;
         const double wd = on ? weight(r, v) : 0.0;
         const uint64_t w = whole_weight(wd), cum = front + running(w), before = cum - w;
-        // whether X is met too closely, or not at all
-        auto unsure = [&](uint64_t X) {
-            const double slack = off * ((double)front + (double)X);
+        // Whether X = q * all is met too closely, or not at all. With front off by a and what lies between it and all by b, relative, sums up to a value and X differ by
+        // (1 - q) a front - q b (all - front) more than they should; and by what the additions' own rounding makes of front in one pass and in another.
+        auto unsure = [&](uint64_t X, double q, uint64_t all) {
+            q = fmin(fmax(q, 0.0), 1.0);
+            const double slack = off * ((1.0 - q) * (double)front + q * fmax(0.0, (double)all - (double)front)) + ADDING * (double)front + 4.0;
             const bool close = on && fabs((double)cum - (double)X) <= slack, met = on && (double)cum >= (double)X + slack;
             return vote(close) != 0 || vote(met) == 0 || (!from_top && (double)front + slack >= (double)X);
         };
@@ -232,7 +237,7 @@ struct Few {
             if (f.by_rank) total = tell(threadIdx.x + 1 == count, cum);
             if (f.by_sum) {
                 const uint64_t X = (uint64_t)fmax(1.0, ceil(f.p * (double)total));
-                if (off > 0 && unsure(X)) return SP_AGAIN;
+                if (off > 0 && unsure(X, f.p, total)) return SP_AGAIN;
                 count = min(count, vote(on && before < X));
             }
             if (f.by_size) {
@@ -245,7 +250,7 @@ struct Few {
         if (draws) {
             const uint64_t X = min(kept, (uint64_t)floor(f.u * (double)kept) + 1);
             // (kept is exact where its end was found here, among values from the top; one found in another list, or the row's sum, is off, and X with it)
-            if (off > 0 && !(ends && from_top && (f.by_sum || f.by_size)) && unsure(X)) return SP_AGAIN;
+            if (off > 0 && !(ends && from_top && (f.by_sum || f.by_size)) && unsure(X, f.u, kept)) return SP_AGAIN;
             const bool mine = on && before < X && X <= cum;
             if (mine) {
                 *id = 0xffffffffu - (uint32_t)e;

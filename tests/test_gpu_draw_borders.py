@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 NONE = -77
 DT = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
-GAP = 2e-9     # of the sum: nearer to a border either neighbour may be drawn
+GAP = 1e-9     # of the sum: nearer to a border either neighbour may be drawn (weights are whole multiples of 2^-44)
 
 
 class Row:
@@ -240,3 +240,14 @@ def test_16_bit_values_whose_differences_take_more_than_24(f, dtype):
     x = x.to(DT[dtype])
     f = {"T": 51.3, **f}
     check(x, torch.cat([Row(x, **f).borders(60), torch.linspace(0, 0.09, 40, device="cuda")]), **f)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("f", [{}, {"p": 0.9}, {"p": 0.3}, {"p": 0.99, "T": 2.0}], ids=lambda f: "_".join(f"{a}{b}" for a, b in f.items()) or "all")
+def test_uniform_numbers_at_growing_distances_from_borders(f, dtype):
+    """From 2^-24 to 2^-13 off: where sums of 32-bit exponentials begin to be trusted."""
+    for x in (normal(70001, 0.1, 31, dtype), normal(70001, 1.0, 32, dtype), normal(200003, 2.5, 33, dtype)):
+        row = Row(x, **f)
+        u = row.borders(40)
+        off = torch.tensor([s * 2.0 ** j for j in range(12) for s in (-1, 1)], device="cuda") * 2.0 ** -24
+        check(x, (u[:, None] + off).clamp(0, 1 - 2.0 ** -24).view(-1), **f)

@@ -1,22 +1,26 @@
 // The norm over many tensors of gradients, and clipping.
 //
-//   norm = scale sqrt(sum of g^2 over all tensors),   out = f g,   f = scale min(1, max_norm / norm)   (scale alone where the norm is not finite in 32 bits)
+//   norm = scale sqrt(sum of g^2 over all tensors),   out = f g,   f = scale min(1, max_norm / norm)   (scale alone where the norm is not
+//                                                     finite in 32 bits)
 //
 // What bounds it: memory. The factor depends on every value, so that the gradients are read twice, and the floor (each read once) is out of reach
 // for what does not stay in L2.
 //
-// Two launches whatever the number of tensors: the list travels as a kernel parameter (up to 32 KB), which a captured graph keeps a copy of. All tensors
-// make one row of units, 16 bytes of a tensor each; what is in front of a tensor's first 16-byte boundary and behind its last one is one more unit. Warps take
-// 256 units at a time, across the ends of tensors, so that small vectors between large matrices cost no more than their bytes.
-// The first launch leaves one sum per block; each block of the second adds them all up in the same order (so the factor is the same everywhere, and the
-// result does not depend on the order in which blocks run), and goes through the units backwards: what was read last is still in L2.
+// Two launches whatever the number of tensors: the list travels as a kernel parameter (up to 32 KB), which a captured graph keeps a copy
+// of. All tensors make one row of units, 16 bytes of a tensor each; what is in front of a tensor's first 16-byte boundary and behind its
+// last one is one more unit. Warps take 256 units at a time, across the ends of tensors, so that small vectors between large matrices cost
+// no more than their bytes. The first launch leaves one sum per block; each block of the second adds them all up in the same order (so the
+// factor is the same everywhere, and the result does not depend on the order in which blocks run), and goes through the units backwards:
+// what was read last is still in L2.
 //
-// Precision: eight squares are added up in 32 bits, what comes of that in 64 (a unit's sum is 2e-7 off at most, the norm of many units 1e-8). Where 32
-// bits could overflow or lose small squares (bf16 and fp32), the unit is done again in 64. An output is rounded to 32 bits and then to its type; the
-// first of the two can move the second by 2^-24 of the value, which is below a 2^-13th of a 16-bit step.
+// Precision: eight squares are added up in 32 bits, what comes of that in 64 (a unit's sum is 2e-7 off at most, the norm of many units
+// 1e-8). Where 32 bits could overflow or lose small squares (bf16 and fp32), the unit is done again in 64. An output is rounded to 32 bits
+// and then to its type; the first of the two can move the second by 2^-24 of the value, which is below a 2^-13th of a 16-bit step.
 //
-// Measured: the squares of 0.38 GB of fp16 60 us (6.4 TB/s), the scaling into fp32 190 (0.38 read, 0.76 written: 6.1 TB/s; some of it comes from L2 where calls follow one another). In place,
-// 2.7 GB of bf16: 1.30 ms, 6.3 TB/s for the three passes. A list of little tensors costs the host 0.17 us each and the GPU 5 us in all.
+// Measured: the squares of 0.38 GB of fp16 60 us (6.4 TB/s), the scaling into fp32 190 (0.38 read, 0.76 written: 6.1 TB/s; some of it comes
+// from L2 where calls follow one another). In place, 2.7 GB of bf16: 1.30 ms, 6.3 TB/s for the three passes. A list of little tensors costs
+// the host 0.04 to 0.1 us each in place and 0.07 to 0.2 into others, beside some 11; the GPU 13 to 16 us in place for 20 to 440 tensors of
+// 100 values and 20 to 33 into others, one after the other by the warps that have them.
 #include <type_traits>
 
 #include "train.cuh"
@@ -29,8 +33,8 @@ constexpr int CL_THREADS = 512, CL_WARPS = CL_THREADS / 32;
 constexpr int CL_LOADS = 8;                     // units in flight per lane
 constexpr uint32_t CL_SHARE = 32 * CL_LOADS;    // units that a warp takes at a time
 constexpr int CL_BLOCKS_PER_SM = 2;
-// The list of a launch: few tensors in a small parameter (a launch copies all of it), many in the largest there is: 20 tensors 12 us of the host's time, and 20 in the large one;
-// 65 tensors 16 and 23, 110 tensors 19 and 25.
+// The list of a launch: few tensors in a small parameter (a launch copies all of it), many in the largest there is: 20 tensors 12 us of the
+// host's time, and 20 in the large one; 65 tensors 16 and 23, 110 tensors 19 and 25.
 constexpr int CL_FEW = 120, CL_MANY = 1000;
 
 struct ClipTensor {
@@ -151,7 +155,8 @@ __device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b)
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
 }
 
-// The factor, as 32 bits and a power of two: a norm of up to 2^128 leaves a limit's quotient below 2^-126, where 32 bits have few places. (A scale is below 2^128.)
+// The factor, as 32 bits and a power of two: a norm of up to 2^128 leaves a limit's quotient below 2^-126, where 32 bits have few places.
+// (A scale is below 2^128.)
 struct ClipFactor {
     float f;
     bool small;

@@ -1,21 +1,28 @@
 // Products of a few rows with 4-bit weights in groups:   y[m, n] = sum_k x[m, k] (q[n, k] - z[n, k / G]) s[n, k / G]
 //
-// What bounds it: reading the codes, half a byte each, and their scales. Every warp streams pieces of its own, 32 outputs (rows of the matrix) by 256 inputs, into
-// a ring in shared memory (TMA, 4 KB, 128 to 192 KB per SM in flight); nobody else is waited for until a tile of 32 outputs is done. It turns codes into exact
-// fp16 or bf16 by setting them into the last places of a constant and taking that and the zero point away, one operation each for two codes. A lane's 16
-// bytes of a row, 32 codes, are its own share of the inner indices of eight MMAs (m16n8k16); x lies in shared memory in the order in which codes fall
-// out of their words, 16 bytes for each word.
-// An MMA adds up over four lanes, which hold 128 inputs, and those may be of one, two or four groups. Scales are applied to its 32-bit sums, so the groups
-// must not meet in it: of its eight columns, a batch row takes as many as there are groups in 128 inputs, and in each of them only the lanes
-// of that group have inputs, the others zeros. For one batch row (where seven columns would be idle) this costs nothing.
+// What bounds it: reading the codes, half a byte each, and their scales. Every warp streams pieces of its own, 32 outputs (rows of the
+// matrix) by 256 inputs, into a ring in shared memory (TMA, 4 KB, 128 to 192 KB per SM in flight); nobody else is waited for until a tile
+// of 32 outputs is done. It turns codes into exact fp16 or bf16 by setting them into the last places of a constant and taking that and the
+// zero point away, one operation each for two codes. A lane's 16 bytes of a row, 32 codes, are its own share of the inner indices of eight
+// MMAs (m16n8k16); x lies in shared memory in the order in which codes fall out of their words, 16 bytes for each word.
+// An MMA adds up over four lanes, which hold 128 inputs, and those may be of one, two or four groups. Scales are applied to its 32-bit
+// sums, so the groups must not meet in it: of its eight columns, a batch row takes as many as there are groups in 128 inputs, and in each
+// of them only the lanes of that group have inputs, the others zeros. For one batch row (where seven columns would be idle) this costs
+// nothing.
 //
-// Blocks divide the outputs evenly, to single ones (the tiles of a block are as high as its share asks for), and a block's warps its pieces, tile after tile: a warp
-// stores the tiles that it has to itself, leaves its sums of those that it shares in shared memory, and at the end they are added up in one order. Nobody waits before
-// that. Where the activations do not fit into shared memory, or the outputs are few, a cluster of `ks` blocks divides the inputs.
+// Blocks divide the outputs evenly, to single ones (the tiles of a block are as high as its share asks for), and a block's warps its
+// pieces, tile after tile: a warp stores the tiles that it has to itself, leaves its sums of those that it shares in shared memory, and at
+// the end they are added up in one order. Nobody waits before that. Where the activations do not fit into shared memory, or the outputs are
+// few, a cluster of `ks` blocks divides the inputs.
 //
-// Measured, one batch row: 65536 x 4096 fp16 in groups of 128 33 us, 4.2 TB/s of codes and scales (27 with the arithmetic left out: 5.1); 4096 x 4096 7.4 (6.3), of which some 6 are the
-// launch, the activations and the way to the first piece. The warps issue 147 instructions for 2048 codes, 2.2 a cycle and SM of 4; more warps or fewer (24, 8), codes taken as
-// subnormal numbers (132 instructions) and zero points taken out by sums of the inputs were no faster, the last two slower in groups of 32 and with eight rows (20.5 -> 26).
+// Measured, one batch row: 65536 x 4096 fp16 in groups of 128 33 us, 4.2 TB/s of codes and scales (27 with the arithmetic left out: 5.1);
+// 4096 x 4096 7.4 (6.3), of which some 6 are the launch, the activations and the way to the first piece. Beyond the streaming, no unit is
+// near its rate: the warps issue 147 instructions for 2048 codes, 2.2 a cycle and SM of 4, the ALU pipe is 45 % busy and the matrix unit 24
+// %, with 16 warps an SM (a quarter of what it holds): what is left is waiting, for a piece's words, for each other's results and for the
+// scales, which come by loads of 4 bytes from eight rows. More warps or fewer (24, 8), codes taken as subnormal numbers (132 instructions)
+// and zero points taken out by sums of the inputs were no faster, the last two slower in groups of 32 and with eight rows (20.5 -> 26).
+// More rows than one pass takes cost a pass each, whatever their number: 16 rows of 65536 x 4096 81 us, 64 of 16384 x 4096 in groups of 64
+// 184, 320 of them 989, 2048 of 4096 x 4096 642.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -167,8 +174,8 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     if (lane == 0)
         for (int i = 0; i < a.stages; ++i) request();
 
-    // Scales and zero points of a piece, in registers, one piece ahead: of rows g, g + 8, g + 16 and g + 24 of the tile. Rows behind the tile's, whose sums nobody
-    // reads, take the last one's, and so do groups behind a row's, whose inputs are zeros.
+    // Scales and zero points of a piece, in registers, one piece ahead: of rows g, g + 8, g + 16 and g + 24 of the tile. Rows behind the
+    // tile's, whose sums nobody reads, take the last one's, and so do groups behind a row's, whose inputs are zeros.
     struct Scales {
         uint32_t s[4][PAIRS], z[ZERO ? 4 : 1];   // z: of the first chunk, and of the second one in the high half
     };
@@ -256,8 +263,8 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n) sum[m][n][0] = sum[m][n][1] = sum[m][n][2] = sum[m][n][3] = 0.f;
-    // Where this lane's inputs lie: of its column's batch row, if they are of its column's group; else its registers stay zero. (Columns behind the last batch
-    // row read that one's, and nobody reads them.)
+    // Where this lane's inputs lie: of its column's batch row, if they are of its column's group; else its registers stay zero. (Columns
+    // behind the last batch row read that one's, and nobody reads them.)
     const bool has = GROUPS == 1 || of_code == g % GROUPS;
     uint32_t x_at[NT];   // (defined behind the barrier: what reads through them cannot be moved in front of it)
 #pragma unroll
@@ -269,7 +276,8 @@ __global__ void __launch_bounds__(I4_THREADS, 1) int4_rows_kernel(const __grid_c
     const uint32_t has_it = has, x_word = rows * 64;
     auto low = [](uint32_t v) { return from_bits<E>((unsigned short)v); };
     auto high = [](uint32_t v) { return from_bits<E>((unsigned short)(v >> 16)); };
-    // The piece's two chunks. (Not unrolled: the code of both did not fit the instruction cache's first level.) Returns a combination of a word of each load from the stage.
+    // The piece's two chunks. (Not unrolled: the code of both did not fit the instruction cache's first level.) Returns a combination of a
+    // word of each load from the stage.
     auto piece = [&](const unsigned char* w, Scales& v, int c) -> uint32_t {
         uint32_t used = 0, x_c = (uint32_t)c * 8 * x_word;
         const unsigned char* w_at = w + g * 128 + ((t ^ g) << 4);   // (the second chunk's 16 bytes: bit 6 of the address)
@@ -451,9 +459,10 @@ int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
     AB_CHECK_ARG((int64_t)a.N * (a.K / 32) < UINT32_MAX, "linear_int4: a matrix of %d x %d is too large", a.N, a.K);
     const int pieces = (a.K + 255) / 256;
     a.pass = MR < a.rows ? MR : a.rows;
-    // The blocks of a cluster divide the inputs where activations do not fit otherwise, and where outputs are few: then each loads a share of the activations, and has tiles of 32 outputs
-    // instead of single ones, as long as two of them hold its outputs. 1 row, groups of 128, undivided against four and eight blocks: 1024 x 4096 7.4 us, 7.2, 5.9; 512 x 16384 13.1, 8.7, 7.5;
-    // 2048 x 8224 (groups of 32) 11.1, 9.6, 10.3; 4096 x 8224 11.9, 13.0, 13.7.
+    // The blocks of a cluster divide the inputs where activations do not fit otherwise, and where outputs are few: then each loads a share
+    // of the activations, and has tiles of 32 outputs instead of single ones, as long as two of them hold its outputs. 1 row, groups of
+    // 128, undivided against four and eight blocks: 1024 x 4096 7.4 us, 7.2, 5.9; 512 x 16384 13.1, 8.7, 7.5; 2048 x 8224 (groups of 32)
+    // 11.1, 9.6, 10.3; 4096 x 8224 11.9, 13.0, 13.7.
     int tiles = 0, shared = 0, lg = 0;   // of a block; shared memory behind the activations; of ks
     const int* const fit_of = fits[dev - once.props];
     for (const int l : {3, 2})
@@ -464,7 +473,8 @@ int i4_launch(const void* codes, I4Args a, cudaStream_t st) {
         if (x_bytes + (I4_SHARED + (a.ks > 1 ? 8 : 0)) * tile_bytes <= ROOM) {
             const int passes = (a.rows + a.pass - 1) / a.pass;
             const int most = a.ks > 1 ? (int)((ROOM - x_bytes) / tile_bytes - I4_SHARED) * I4_ROWS : a.N;   // outputs whose sums fit
-            // All passes at once, one turn of clusters (their beginning is paid once; 1024 x 4096 in groups of 32, 16 rows 23.7 -> 12.2), unless the sums of so many outputs do not fit.
+            // All passes at once, one turn of clusters (their beginning is paid once; 1024 x 4096 in groups of 32, 16 rows 23.7 -> 12.2),
+            // unless the sums of so many outputs do not fit.
             int fit = std::max(1, fit_of[lg] / passes);
             if ((a.N + fit - 1) / fit > most) fit = fit_of[lg];
             a.x_bytes = (int)x_bytes;

@@ -4,25 +4,31 @@
 //   each value but the first has   rank < k,   sum of the w in front of it < p * (sum of w over the first k),   w >= m.
 //   The id is the first one whose sum of w up to and with it exceeds u * (sum of w that is kept).
 //
-// All three filters keep a front part of one and the same order, and so does the draw: each is a question "where in that order do the weights (or the
-// ranks) reach X?". What bounds it is less the reading of a row (it stays in shared memory, of one block or of a cluster's) than what is done for each of its values, so
-// the way goes by what the filters leave:
-//   few values    top-k up to 600 over the row's blocks, or min-p: the k-th largest of the threads' own maxima is a bound that some k values and a few more reach. Those are
-//                 gathered, sorted, and their weights added up: every question is answered among them, without an exponential for any other value.
-//   a bracket     else the sum over the row is needed: 32-bit exponentials and a histogram of counts over 4096 bins of max - l in one pass. A bin's counts
-//                 bound its weights within a percent, so they say in which few bins X is reached; their values are gathered and sorted, and what lies
-//                 in front of them is added up in 32 bits (nothing, where the values down to there are few). Those sums are off by EPS at most: where a
-//                 border lies nearer than that, or the bracket holds more than 1024 values, it is done again in whole numbers.
-//   whole numbers a histogram over the same bins with exact sums, by atomics on shared memory; its running sums answer every question down to a bin. The
-//                 few values of that bin are gathered and compared with each other; where they are more than SP_LIST (ties of 16-bit logits), the
-//                 bin's keys' range is divided again.
+// All three filters keep a front part of one and the same order, and so does the draw: each is a question "where in that order do the
+// weights (or the ranks) reach X?". What bounds it is less the reading of a row (it stays in shared memory, of one block or of a cluster's)
+// than what is done for each of its values, so the way goes by what the filters leave:
+//   few values    top-k up to 600 over the row's blocks, or min-p: the k-th largest of the threads' own maxima is a bound that some k
+//                 values and a few more reach. Those are gathered, sorted, and their weights added up: every question is answered among
+//                 them, without an exponential for any other value.
+//   a bracket     else the sum over the row is needed: 32-bit exponentials and a histogram of counts over 4096 bins of max - l in one
+//                 pass. A bin's counts bound its weights within a percent, so they say in which few bins X is reached; their values are
+//                 gathered and sorted, and what lies in front of them is added up in 32 bits (nothing, where the values down to there are
+//                 few). Those sums are off by EPS at most: where that might move a border across the place, or the bracket holds more than
+//                 1024 values, it is done again in whole numbers.
+//   whole numbers a histogram over the same bins with exact sums, by atomics on shared memory; its running sums answer every question down
+//                 to a bin. The few values of that bin are gathered and compared with each other; where they are more than SP_LIST (ties
+//                 of 16-bit logits), the bin's keys' range is divided again.
 //
-// Precision: weights are taken as multiples of 2^-44 (the largest is 2^44 of them), so that sums are whole numbers and do not depend on the order of additions; they
-// come from a table and a polynomial in 64 bits (off by 1e-15). What comes out is the id that the definition in 64 bits gives, unless u or p meets a border
-// within some 1e-9 of the sum. The log-probability has the 32-bit sum where a bracket sufficed: off by EPS.
+// Precision: weights are taken as multiples of 2^-44 (the largest is 2^44 of them), so that sums are whole numbers and do not depend on the
+// order of additions; they come from a table and a polynomial in 64 bits (off by 1e-15). What comes out is the id that the definition in 64
+// bits gives, unless u or p meets a border within some 1e-9 of the sum. The log-probability has the 32-bit sum where a bracket sufficed:
+// off by EPS.
 //
-// Measured, fp32 x 65536: one row under top-p 0.9 20 us, 48 to 57 where it comes to whole numbers (a row in ten of normal logits), 9 under min-p 0.05; 512 rows under top-p 0.9 300, two blocks a
-// row, of which an SM holds one. 16-bit rows of up to 65536 values and a small top-k of the same k have kernels of their own, below.
+// Measured, fp32 x 65536: one row under top-p 0.9 19 to 27 us, 44 to 60 where it comes to whole numbers (a third of the rows of normal
+// logits with a deviation of 1, a sixth with 2, a thirtieth with 3; under top-p 0.99 most), 11 under min-p 0.05, 42 where that keeps more
+// than 1024 values; 512 rows under top-p 0.9 317, without filters 223, two blocks a row, of which an SM holds one. What bounds them: the
+// shared memory that a row takes (92 KB beside up to 129 of the row: one block an SM), and three or four passes over it, one with an atomic
+// for each value. 16-bit rows of up to 65536 values and a small top-k of the same k have kernels of their own, below.
 #include <cooperative_groups.h>
 
 #include "train.cuh"
@@ -68,9 +74,9 @@ __device__ __forceinline__ int bin_of(const RowScale& r, float v) {   // never f
     const float d = v == r.top ? 0.f : r.top - v;
     return (int)(__float_as_uint(fminf(d * r.bins, SP_BINS - 1) + 8388608.f) & (2 * SP_BINS - 1));   // (2^23: the last places are whole numbers. A conversion has a quarter of the rate)
 }
-// w in 32 bits, by the hardware's 2^x (relative error 2^-22). The product's rounding and what 32 bits leave of c are made good, so that 2^-22 + 2^-23 remains, and 2^-24 z ln 2 for
-// the rounding of the difference d: below 2^-20 for z up to 22 (values beyond that weigh 2^-4 of the largest at most, all together). 16-bit logits are no better there: 513 and a
-// number of 2^-15 are 26 bits apart. d is finite.
+// w in 32 bits, by the hardware's 2^x (relative error 2^-22). The product's rounding and what 32 bits leave of c are made good, so that
+// 2^-22 + 2^-23 remains, and 2^-24 z ln 2 for the rounding of the difference d: below 2^-20 for z up to 22 (values beyond that weigh 2^-4
+// of the largest at most, all together). 16-bit logits are no better there: 513 and a number of 2^-15 are 26 bits apart. d is finite.
 __device__ __forceinline__ float weight32(float d, float c, float c_low) {
     const float z = d * c, rest = fmaf(d, c_low, fmaf(d, c, -z));
     float w;
@@ -215,8 +221,9 @@ struct Few {
             }
         return v;
     }
-    // Of the n values of a list, behind a sum `front` of all in front of them: what is kept (`ends`: with total the row's sum; under top_k that of the first k is theirs), and
-    // the draw (`draws`). Sums of weights in 32 bits, as front is one and total has some, may be `off` relative.
+    // Of the n values of a list, behind a sum `front` of all in front of them: what is kept (`ends`: with total the row's sum; under top_k
+    // that of the first k is theirs), and the draw (`draws`). Sums of weights in 32 bits, as front is one and total has some, may be `off`
+    // relative.
     __device__ SampleState answer(const RowFilters& f, const RowScale& r, const uint64_t* list, uint32_t n, uint64_t front, uint64_t total, double off, bool from_top, bool ends,
                                   bool draws, uint64_t& kept, int64_t* id, float* logp) {
         const uint64_t e = sorted(list, n);
@@ -224,8 +231,9 @@ struct Few {
         const bool on = threadIdx.x < n;
         const double wd = on ? weight(r, v) : 0.0;
         const uint64_t w = whole_weight(wd), cum = front + running(w), before = cum - w;
-        // Whether X = q * all is met too closely, or not at all. With front off by a and what lies between it and all by b, relative, sums up to a value and X differ by
-        // (1 - q) a front - q b (all - front) more than they should; and by what the additions' own rounding makes of front in one pass and in another.
+        // Whether X = q * all is met too closely, or not at all. With front off by a and what lies between it and all by b, relative, sums
+        // up to a value and X differ by (1 - q) a front - q b (all - front) more than they should; and by what the additions' own rounding
+        // makes of front in one pass and in another.
         auto unsure = [&](uint64_t X, double q, uint64_t all) {
             q = fmin(fmax(q, 0.0), 1.0);
             const double slack = off * ((1.0 - q) * (double)front + q * fmax(0.0, (double)all - (double)front)) + ADDING * (double)front + 4.0;
@@ -249,7 +257,8 @@ struct Few {
         }
         if (draws) {
             const uint64_t X = min(kept, (uint64_t)floor(f.u * (double)kept) + 1);
-            // (kept is exact where its end was found here, among values from the top; one found in another list, or the row's sum, is off, and X with it)
+            // (kept is exact where its end was found here, among values from the top; one found in another list, or the row's sum, is off,
+            // and X with it)
             if (off > 0 && !(ends && from_top && (f.by_sum || f.by_size)) && unsure(X, f.u, kept)) return SP_AGAIN;
             const bool mine = on && before < X && X <= cum;
             if (mine) {
@@ -391,8 +400,8 @@ struct Sampler {
         }
         return bound;
     }
-    // running sums of the histogram, over all blocks; every block has them. (Each adds up a share of the bins and hands it round: all of them by every block took 90 us in
-    // clusters of eight.)
+    // running sums of the histogram, over all blocks; every block has them. (Each adds up a share of the bins and hands it round: all of
+    // them by every block took 90 us in clusters of eight.)
     template <int BINS>
     __device__ __forceinline__ void run_up(uint64_t* cum) {
         constexpr int EACH = (BINS + NT - 1) / NT;
@@ -659,8 +668,9 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
         }
         x.join();
         if (x.rank == 0) {
-            // Running counts, and sums of the weights as if a bin's values lay in its middle: they are off by half a bin's width each, 0.4 %, to either side, and
-            // so, many together, by little. That they say where to look is all that is asked of them: `answer` sees whether the place was right.
+            // Running counts, and sums of the weights as if a bin's values lay in its middle: they are off by half a bin's width each, 0.4
+            // %, to either side, and so, many together, by little. That they say where to look is all that is asked of them: `answer` sees
+            // whether the place was right.
             constexpr int EACH = SP_BINS / NT;
             float* run = reinterpret_cast<float*>(s.cum);
             uint32_t n[EACH], count = 0;
@@ -876,21 +886,26 @@ __global__ void __launch_bounds__(NT) sample_filtered_kernel(const SampleArgs a)
     }
 }
 
-// ---- 16-bit logits: one counter for each of their 65536 values ------------------------------------------------------------------------------
-// A row's histogram over the values themselves, in shared memory, says everything but which id has a value: what is kept and drawn is found among the
-// counters, whose running sums are exact, and the row is read once more (from L2) for the id. No value of the row needs an exponential: the counters do, and eight
-// of them that follow one another, a unit, whose values are equally far apart, need one of them and its products with exp(-distance / T). Where the filters leave
-// few values (a small top-k; min-p by itself), only those are gathered that reach a bound: some k of the threads' own maxima do, and so do k values.
-// What bounds it: for rows that wait for an SM the atomics (3.3 cycles for a warp's: two of its values meet a bank), the units' weights, and the row read twice; for the only row of an SM the steps
-// behind one another, each by code that has to be fetched. fp16, 65536 values: one row 21 us under top-p 0.7 (8 under min-p 0.05), 320 rows with filters of their own 43, in three turns of
-// 148; 37 x 50277 bf16 16. In clusters that take exponentials and search (as fp32 rows do, above) the 320 rows took 109.
+// ---- 16-bit logits: one counter for each of their 65536 values --------------------------------------------------------------------------
+// A row's histogram over the values themselves, in shared memory, says everything but which id has a value: what is kept and drawn is found
+// among the counters, whose running sums are exact, and the row is read once more (from L2) for the id. No value of the row needs an
+// exponential: the counters do, and eight of them that follow one another, a unit, whose values are equally far apart, need one of them and
+// its products with exp(-distance / T). Where the filters leave few values (a small top-k; min-p by itself), only those are gathered that
+// reach a bound: some k of the threads' own maxima do, and so do k values. What bounds it: for rows that wait for an SM the atomics (3.3
+// cycles for a warp's: two of its values meet a bank), the units' weights, and the row read twice; for the only row of an SM the steps
+// behind one another, each by code that has to be fetched. fp16, 65536 values, on several boxes: one row 21 to 23 us under top-p 0.7 (8 to
+// 17 under min-p 0.05), 320 rows with filters of their own 43 to 57, in three turns of 148; 37 x 50277 bf16 16 to 18.5. In clusters that
+// take exponentials and search (as fp32 rows do, above) the 320 rows took 109.
 //
-// Counters lie in the order of the values, larger ones first, eight in 16 bytes. Eight units are a group, whose sums are run up over the block; a question is answered by
-// a search among them and by the 64 counters of one group, by the first warp.
+// Counters lie in the order of the values, larger ones first, eight in 16 bytes. Eight units are a group, whose sums are run up over the
+// block; a question is answered by a search among them and by the 64 counters of one group, by the first warp.
 //
-// A counter holds up to 65535: the row's last value is added when the others are counted, so that only a row of 65536 equal ones exceeds it (`extra`).
+// A counter holds up to 65535: the row's last value is added when the others are counted, so that only a row of 65536 equal ones exceeds it
+// (`extra`).
 constexpr int SK_NT = 1024, SK_BINS = 65536, SK_GROUPS = SK_BINS / 64;
-// Few values' sorting costs what k does, counting the same for all: 1 x 65536 12.2 us of k 100, 15.1 of 300, 19.4 of 400, counted 16.7; 512 rows 48, 60, 75 against 65.
+// Few values' sorting costs what k does, counting the same for all. Top-k 320 and 400 sorted, and counted: 1 x 65536 17.0, 21.1 and 19.8
+// us; 1 x 32003 14.7, 18.8 and 15.0; 1 x 5003 14.7, 14.7 and 12.7 (256: 12.7); 512 x 65536 64.6, 81.3 and 72.3; 512 x 32003 51.8, 68.2 and
+// 58.0; 512 x 5003 43.4, 53.6 and 45.4.
 constexpr int SK_MOST_K = 320;
 static_assert(SK_GROUPS == SK_NT, "a thread per group");
 
@@ -948,8 +963,9 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
         }
         return q;
     };
-    // Three pieces of a thread under way. (All eight at once make eight times the code of what is done with one, and the fetching of instructions, which run once a row
-    // here, was what the kernel waited for most: 1 x 65536 23.7 us against 21.0, 320 x 65536 48.4 against 42.7.)
+    // Three pieces of a thread under way. (All eight at once make eight times the code of what is done with one, and the fetching of
+    // instructions, which run once a row here, was what the kernel waited for most: 1 x 65536 23.7 us against 21.0, 320 x 65536 48.4
+    // against 42.7.)
     uint4 q[3];
 #pragma unroll
     for (int j = 0; j < 3; ++j)
@@ -1092,14 +1108,16 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
             const uint32_t n = half ? word >> 16 : word & 0xffffu;
             return n == 0xffffu ? n + extra : n;
         };
-        // The weight of a bin's value, from that of its unit's first (of the largest value in its unit). One way for all who ask: sums are to agree to the last unit.
+        // The weight of a bin's value, from that of its unit's first (of the largest value in its unit). One way for all who ask: sums are
+        // to agree to the last unit.
         auto base_of = [&](uint32_t bin) { return max(bin & ~7u, top_bin); };
         auto steps = [&](uint32_t bin) { return s.step[bits_of_bin(bin) >> K::MANTISSA & (K::EXPONENTS - 1)]; };
         auto weight_at = [&](uint32_t bin) {
             const uint32_t base = base_of(bin);
             return weight(r, value_at(base)) * steps(bin)[bin - base & 7u];   // (1 times 1 for the largest value)
         };
-        // s.sums: of the groups from that of the largest value on (group g: units 8 g .. 8 g + 7), filled by run_counts or run_weights, then run up over all of them.
+        // s.sums: of the groups from that of the largest value on (group g: units 8 g .. 8 g + 7), filled by run_counts or run_weights,
+        // then run up over all of them.
         const int first = (int)(top_bin >> 6);
         auto run_up = [&]() {
             uint64_t v = s.sums[threadIdx.x];
@@ -1116,7 +1134,8 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
             s.sums[threadIdx.x] = v + before;
             __syncthreads();
         };
-        // Where the running sum reaches X (by one warp). `one`: of two neighbouring counters and the first one's bin. Bins from `floor_` on do not count.
+        // Where the running sum reaches X (by one warp). `one`: of two neighbouring counters and the first one's bin. Bins from `floor_` on
+        // do not count.
         struct At {
             uint32_t bin;
             uint64_t before, one;   // one: what a value of the bin adds
@@ -1315,11 +1334,14 @@ __global__ void __launch_bounds__(SK_NT, 1) sample_keys_kernel(const SampleArgs 
     }
 }
 // ---- top-k of the same small k for every row --------------------------------------------------------------------------------------------
-// Rows are streamed, two blocks of 512 threads to an SM (k up to 256; one of 1024 up to 600), so that one reads while the other sorts: a row's largest values per thread,
-// a bound that k threads reach, then only the values of a thread that reach it once more (from L2), and what the few values answer. Where more values than threads reach the
-// bound (equals, mostly), the k-th largest key is searched by counting, and of its equals the first ids are taken.
-// What bounds it: reading, at 37 % of the memory's rate, and the barriers between the steps. 512 x 65536 fp32, top-k 50: 41 us (3.2 TB/s); in clusters that keep rows in shared memory 105. For
-// one fp32 row it takes 14 us where those take 12.7 (k 50), and 20 where they take 37 (k 400): one kernel for every number of rows.
+// Rows are streamed, two blocks of 512 threads to an SM (k up to 256; one of 1024 up to 600), so that one reads while the other sorts: a
+// row's largest values per thread, a bound that k threads reach, then only the values of a thread that reach it once more (from L2), and
+// what the few values answer. Where more values than threads reach the bound (equals, mostly), the k-th largest key is searched by
+// counting, and of its equals the first ids are taken. What bounds it: latency. A block loads nothing while it searches its bound (up to 16
+// barriers) and sorts, and two of them to an SM read at 37 % of the memory's rate. 512 x 65536 fp32, top-k 50: 41 to 45 us on several boxes
+// (3 TB/s); in clusters that keep rows in shared memory 109. For one fp32 row it takes 15 us where those take 15.5 (k 50), and 23 where
+// they take 49 (k 400), of 32003 values 12.6 and 14.7, 18.8 and 44.9, of 5003 8.6 and 10.9, 16.7 and 33.6: one kernel for every number of
+// rows. (Those are ahead at k 600 from some 150 rows of 32003 on: 33 us against 25.)
 constexpr int ST_BATCH = 8, ST_MOST_K = 600;
 
 template <int ST_NT>
@@ -1540,8 +1562,9 @@ int sample_launch(SampleArgs a, cudaStream_t st) {
     int lg = 0;
     while ((pieces + (1 << lg) - 1) / (1 << lg) * 16 > SP_ROW_BYTES) ++lg;
     AB_CHECK_ARG(1 << lg <= SP_MAX_BLOCKS, "sampling: a vocabulary of %d is too large", a.V);
-    // More blocks to a row while all rows run at once, a piece or more to each thread. (fp32 65536, top-p: 1 row in eight blocks 48 us, in two 62. But 16 rows in eight blocks,
-    // of which 128 SMs hold fewer than 16 clusters at a time, take two turns: under top-k 50 24.8 us, in four 12.1.)
+    // More blocks to a row while all rows run at once, a piece or more to each thread. (fp32 65536, top-p: 1 row in eight blocks 48 us, in
+    // two 62. But 16 rows in eight blocks, of which 128 SMs hold fewer than 16 clusters at a time, take two turns: under top-k 50 24.8 us,
+    // in four 12.1.)
     while (1 << lg < SP_MAX_BLOCKS && a.rows <= fit[dev - once.props][lg + 1] && pieces > 1024 << lg) ++lg;
     const int blocks = 1 << lg;
     AB_CHECK_ARG(a.rows <= INT32_MAX / blocks, "sampling: too many rows");
@@ -1555,8 +1578,10 @@ int sample_launch(SampleArgs a, cudaStream_t st) {
 
 int sample_filtered(int dtype, int64_t rows, int V, const void* logits, int64_t stride, const float* u, const ab_sampling& p, int64_t* ids, float* logp, cudaStream_t st) {
     const SampleArgs a = {logits, u, p.temperature, p.top_p, p.min_p, p.top_k, p.temperature_all, p.top_p_all, p.min_p_all, p.top_k_all, V, rows, stride, ids, logp, 0, 0};
-    // 16-bit rows of up to 65536: counters. Streamed instead where more rows than SMs have the same top-k of up to 256: 512 x 65536 fp16 with k of 50 38 us against 45, 256 50 against 59, but
-    // 400 72 against 67; and one row with k 50 14.5 against 11.5.
+    // 16-bit rows of up to 65536: counters. Streamed instead where more rows than SMs have the same top-k of up to 256: 512 x 65536 fp16
+    // with k of 50 41.8 us against 49.0, 256 54.1 against 63.1, but 400 81.0 against 72.3; 512 x 32003 27.5 against 37.5, 39.8 against
+    // 50.3, 70.5 against 58.0; 512 x 5003 19.0 against 29.0, 31.6 against 39.3, 58.0 against 45.4. With 148 rows of k 50 19.1 against 16.0,
+    // 14.5 against 12.9, 10.6 and 10.6; with one 14.7 against 12.9, 10.6 and 10.6, 9.3 against 8.6.
     const bool keys = V <= SK_BINS && dtype != AB_DT_F32, streams = !p.top_k && p.top_k_all > 0 && p.top_k_all <= ST_MOST_K && p.top_k_all < V;
     if (streams && !(keys && (rows <= current_sm_count() || p.top_k_all > 256)))
         return dtype == AB_DT_F16 ? sample_top_launch<__half>(a, st) : dtype == AB_DT_BF16 ? sample_top_launch<__nv_bfloat16>(a, st) : sample_top_launch<float>(a, st);

@@ -1,5 +1,5 @@
-// What serves a token, as torch operators beside those of train_op.cpp (torch.ops.albatross_b200.*): arguments checked, memory from torch's allocator,
-// the C entries called on torch's current stream of the tensors' device. Neither has gradients.
+// What serves a token, as torch operators beside those of train_op.cpp (torch.ops.albatross_b200.*): arguments checked, memory from torch's
+// allocator, the C entries called on torch's current stream of the tensors' device. Neither has gradients.
 #include "op.h"
 
 namespace {

@@ -411,7 +411,8 @@ std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits_, const Tensor& 
 
 // ---- the norm over all gradients -------------------------------------------------------------------------------------------------------
 bool same_order(const Tensor& a, const Tensor& b) { return a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous()); }
-// out: empty (the norm alone), the gradients themselves, or one tensor for each. What is not dense, or lies in another order than its gradient, goes by way of a copy.
+// out: empty (the norm alone), the gradients themselves, or one tensor for each. What is not dense, or lies in another order than its
+// gradient, goes by way of a copy.
 Tensor clip_grad_norm(at::TensorList grads, double max_norm, double scale, at::TensorList out) {
     constexpr const char* who = "clip_grad_norm";
     TORCH_CHECK(!grads.empty(), who, ": no gradients");
@@ -488,9 +489,9 @@ TORCH_LIBRARY(albatross_b200, m) {
     m.def("preference_loss(Tensor logits, Tensor ids, Tensor ref_logp, Tensor? mask, float beta, float smoothing) -> (Tensor, Tensor)", preference_loss);
 }
 
-// clip_grad_norm for lists of hundreds of tensors: the dispatcher boxes and unboxes both lists, 0.2 us a tensor of the 0.3 that a call takes. Takes Python lists or
-// tuples of tensors (out: None, for the norm alone) with the interpreter's lock held; returns null, with the error set, where it throws. Neither dispatch modes nor the profiler
-// see the call.
+// clip_grad_norm for lists of hundreds of tensors: the dispatcher boxes and unboxes both lists, 0.2 us a tensor of the 0.3 that a call
+// takes. Takes Python lists or tuples of tensors (out: None, for the norm alone) with the interpreter's lock held; returns null, with the
+// error set, where it throws. Neither dispatch modes nor the profiler see the call.
 struct LetGo {   // of the interpreter's lock: a launch may have to wait for room in the queue, and what it waits for may need that lock (a host function)
     PyThreadState* const state = PyEval_SaveThread();
     LetGo() = default;

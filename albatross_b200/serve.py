@@ -27,15 +27,17 @@ def sampler_batch(logits: torch.Tensor, uniform: torch.Tensor, temperature: Numb
     """Draws one id per row of logits [..., V] (fp16, bf16 or fp32; V up to 2^18) by `uniform`, fp32 numbers in [0, 1), one per row: ids [..., 1] (int64)
     and their log-probabilities [..., 1] (fp32) under the distribution they were drawn from, which is what policy_loss wants for old_logp.
 
-    With w = exp((logit - largest) / temperature) and the values in order, larger ones first, equals by id, the front part is kept in which each value but
-    the first has a rank below top_k, a sum of w in front of it below top_p * (the sum over the first top_k), and w >= min_p. The id is the first one whose sum
-    of w up to and with it exceeds uniform * (the sum that is kept); it is decided as in 64 bits. temperature 0 or top_k 1: the first largest value. top_k <= 0,
-    top_p >= 1 and min_p <= 0 filter nothing. Each of the four is a number, or a tensor of one per row on the device of logits (in which a NaN filters nothing; as
-    a temperature it is 0). -inf is never drawn; a row with a NaN, or of -inf alone, gives -1 and NaN.
+    With w = exp((logit - largest) / temperature) and the values in order, larger ones first, equals by id, the front part is kept in which
+    each value but the first has a rank below top_k, a sum of w in front of it below top_p * (the sum over the first top_k), and w >= min_p.
+    The id is the first one whose sum of w up to and with it exceeds uniform * (the sum that is kept). It is the one that 64 bits give, unless
+    uniform or top_p meets a border within some 1e-9 of the sum. temperature 0 or top_k 1: the first largest value. top_k <= 0, top_p >= 1 and
+    min_p <= 0 filter nothing. Each of the four is a number, or a tensor of one per row on the device of logits, read as fp32 (top_k: int32),
+    in which a NaN filters nothing; as a temperature it is 0. -inf is never drawn; a row with a NaN, or of -inf alone, gives -1 and NaN.
 
     There are no gradients: the log-probabilities carry none, whatever the logits require (they are an old_logp; token_logp of the ids has one).
 
-    `out`: a dense int64 tensor of one id per row to write into, on the device or in pinned host memory (read it after synchronising the stream)."""
+    `out`: a dense int64 tensor of one id per row to write into, on the device, apart from the inputs, or in pinned host memory (read it
+    after synchronising the stream)."""
     T, k, p, m = temperature, top_k, top_p, min_p
     t = torch.is_tensor
     return _sample(logits, uniform, T if t(T) else None, k if t(k) else None, p if t(p) else None, m if t(m) else None, 1.0 if t(T) else T, 0 if t(k) else k,
@@ -78,7 +80,9 @@ def quantize_int4(w: torch.Tensor, group: int = 128, zeros: bool = False, dtype:
 def linear_int4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [..., K] (fp16 or bf16) by a matrix of 4-bit codes: y[..., n] = sum_k x[..., k] (q[n, k] - zero[n, k / group]) scale[n, k / group], in the type of x.
 
-    w: uint8 [N, K / 2], even k in the low nibble; scale [N, K / group] of the type of x; zero: uint8 [N, K / group], codes 0 .. 15, or None: 8. group is 32, 64 or
-    a multiple of 128. Codes times activations are exact, sums and scales 32-bit; y is rounded once. For few rows, whose time is that of reading the codes: they are
-    taken in once for up to 8 rows, and for up to 16 where groups are not of 32 and the matrix is small; again for more (up to 65535). No gradients."""
+    w: uint8 [N, K / 2], even k in the low nibble; scale [N, K / group] of the type of x; zero: uint8 [N, K / group], codes 0 .. 15, or None:
+    8. group is 32, 64 or a multiple of 128. Codes times activations are exact, sums and scales 32-bit; y is rounded once. For few rows, whose
+    time is that of reading the codes: they are taken in once for up to 8 rows, and for up to 16 where groups are not of 32 and the matrix is
+    small; again for more, up to 65535. (16384 x 4096 in groups of 64, and torch's product with the dequantised fp16 matrix: 8 rows 22 and 28
+    us, 16 rows 54 and 28, 64 rows 185 and 28, 320 rows 990 and 41.) No gradients."""
     return _linear_int4(x, w, scale, zero)

@@ -114,11 +114,12 @@ def grad_norm(grads: Sequence[torch.Tensor], scale: float = 1.0) -> torch.Tensor
 
 
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, scale: float = 1.0, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
-    """Writes grad * f with f = scale * min(1, max_norm / norm) over the gradients, or into `out` (a tensor for each, of its shape; fp16, bf16 or fp32), and
-    returns norm = scale * (the 2-norm over all values) from before the clipping. `scale` takes a loss scale out: 1 / 65536 where the loss was multiplied by
-    65536; gradients in fp16 then want `out` in fp32, in which small ones do not vanish. Where the norm is not finite nothing is clipped (f = scale), and what
-    is wrong stays visible: a training loop skips that step by norm.isfinite(). Nothing is read back to the host.
+    """Writes grad * f with f = scale * min(1, max_norm / norm) over the gradients, or into `out` (a tensor for each, of its shape; fp16, bf16
+    or fp32), and returns norm = scale * (the 2-norm over all values) from before the clipping. `scale` (positive, a number that fp32 holds)
+    takes a loss scale out: 1 / 65536 where the loss was multiplied by 65536; gradients in fp16 then want `out` in fp32, in which small ones
+    do not vanish. Where the norm that is returned is not finite nothing is clipped (f = scale), and what is wrong stays visible: a training
+    loop skips that step by norm.isfinite(). Nothing is read back to the host.
 
-    Outputs may not overlap each other, nor gradients other than their own. Up to 1000 tensors take two launches; tensors that are not dense, or lie in another
-    order than their output, are copied."""
+    Outputs may not overlap each other, nor gradients other than their own, and those that are not dense may not lie between each other's
+    values. Up to 1000 tensors take two launches; tensors that are not dense, or lie in another order than their output, are copied."""
     return _clip_list(grads, max_norm, scale, grads if out is None else out)
